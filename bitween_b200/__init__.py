@@ -9,7 +9,9 @@ written against the reference (`bitween.modules.QuantizedLinear`, `bitween.funct
 """
 import sys
 
+from .adapters import AdaptedLinear, adapter_matmul  # noqa: F401
 from .functional import dequantize_rtn, quantize_rtn  # noqa: F401
+from .kv_cache import QuantizedKVCache  # noqa: F401
 from .modules import QuantizedLinear, QuantizedLinearFunction  # noqa: F401
 from .quantizer.quantizer import Bitween  # noqa: F401
 

@@ -74,6 +74,20 @@ bool rows_path_ok(const void *x, int x_dtype, int64_t M, int64_t N, int64_t K, c
 int qmatmul_rows(const void *x, int x_dtype, int64_t M, int64_t N, int64_t K, const int32_t *q,
                  const __half *scale, const __half *zp, const __half *bias, void *out, int out_dtype,
                  int bits, int g, cudaStream_t st);
+int kv_append(const void *k, const void *v, int dtype, int64_t tokens, const int64_t *strides, const int64_t *slots, int heads, int dim, int bits,
+              int64_t pages, int page_size, int32_t *kc, int32_t *vc, void *params, cudaStream_t st);
+int kv_read(const int32_t *kc, const int32_t *vc, const void *params, int heads, int dim, int bits, int64_t pages, int page_size,
+            const int64_t *slots, int64_t tokens, void *k, void *v, int dtype, cudaStream_t st);
+size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages);
+int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *kc, const int32_t *vc,
+              const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *table, int64_t table_stride,
+              int max_pages, const int32_t *lengths, float alpha, void *out, void *workspace, cudaStream_t st);
+size_t adapter_hidden_bytes(int64_t M, int64_t K, int n, int r);
+size_t adapter_backward_bytes(int64_t M, int64_t N, int64_t K, int n, int r);
+int adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index,
+                    const float *scaling, const void *base, void *out, float *h, cudaStream_t st);
+int adapter_backward(const void *dy, int dtype, const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r,
+                     const int32_t *index, const float *scaling, const float *h, void *dx, void *d_down, void *d_up, void *workspace, cudaStream_t st);
 size_t peer_flag_bytes();
 size_t peer_state_bytes();
 int peer_device_status();
@@ -556,6 +570,114 @@ int bw_group_params_backward(const void *w_min, const void *w_max, int w_dtype, 
         return BW_ERR_ALIGN;
     return group_params_backward(w_min, w_max, w_dtype, scale, zero_point, span, count, bits, grad_scale, grad_zero_point,
                                  grad_min_scale, grad_max_scale, (cudaStream_t)stream);
+}
+
+// ---- quantised key-value cache ----
+// Checks of the cache's own arguments, shared by its three calls.
+static int kv_validate(const int32_t *k_codes, const int32_t *v_codes, const void *params, int64_t pages, int page_size, int heads, int dim, int bits) {
+    if (bits != 2 && bits != 4 && bits != 8) return BW_ERR_BITS;
+    if (pages < 0 || page_size < 1 || heads < 1 || dim < 1 || dim > 256 || dim % (32 / bits) != 0) return BW_ERR_SHAPE;
+    if (pages > ((int64_t)1 << 40) / page_size / heads) return BW_ERR_SHAPE;
+    if (pages > 0 && (!k_codes || !v_codes || !params)) return BW_ERR_NULL;
+    if (!aligned_to(k_codes, 16) || !aligned_to(v_codes, 16) || !aligned_to(params, 16)) return BW_ERR_ALIGN;
+    return BW_OK;
+}
+
+int bw_kv_append(const void *k, const void *v, int dtype, int64_t tokens, int64_t k_stride, int64_t k_head_stride, int64_t v_stride,
+                 int64_t v_head_stride, const int64_t *slots, int heads, int dim, int bits, int64_t pages, int page_size, int32_t *k_codes,
+                 int32_t *v_codes, void *params, void *stream) {
+    const int rc = kv_validate(k_codes, v_codes, params, pages, page_size, heads, dim, bits);
+    if (rc != BW_OK) return rc;
+    if (!is_float_dtype(dtype)) return BW_ERR_DTYPE;
+    if (tokens < 0 || tokens > ((int64_t)1 << 31) / heads / 8) return BW_ERR_SHAPE;
+    if (tokens == 0 || pages == 0) return BW_OK;
+    if (!k || !v || !slots) return BW_ERR_NULL;
+    if (!aligned_to(k, dtype_size(dtype)) || !aligned_to(v, dtype_size(dtype)) || !aligned_to(slots, 8)) return BW_ERR_ALIGN;
+    const int64_t strides[4] = {k_stride, k_head_stride, v_stride, v_head_stride};
+    return kv_append(k, v, dtype, tokens, strides, slots, heads, dim, bits, pages, page_size, k_codes, v_codes, params, (cudaStream_t)stream);
+}
+
+int bw_kv_read(const int32_t *k_codes, const int32_t *v_codes, const void *params, int heads, int dim, int bits, int64_t pages, int page_size,
+               const int64_t *slots, int64_t tokens, void *k, void *v, int dtype, void *stream) {
+    const int rc = kv_validate(k_codes, v_codes, params, pages, page_size, heads, dim, bits);
+    if (rc != BW_OK) return rc;
+    if (!is_float_dtype(dtype)) return BW_ERR_DTYPE;
+    if (tokens < 0 || tokens > ((int64_t)1 << 31) / heads / 8) return BW_ERR_SHAPE;
+    if (tokens == 0) return BW_OK;
+    if (!k || !v || !slots) return BW_ERR_NULL;
+    if (!aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(slots, 8)) return BW_ERR_ALIGN;
+    return kv_read(k_codes, v_codes, params, heads, dim, bits, pages, page_size, slots, tokens, k, v, dtype, (cudaStream_t)stream);
+}
+
+size_t bw_kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages) {
+    if (batch <= 0 || kv_heads < 1 || heads < kv_heads || dim < 1 || page_size < 1 || max_pages < 0) return 0;
+    return kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
+}
+
+int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *k_codes,
+                 const int32_t *v_codes, const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *page_table,
+                 int64_t table_stride, int64_t max_pages, const int32_t *lengths, float alpha, void *out, void *workspace, size_t workspace_bytes,
+                 void *stream) {
+    const int rc = kv_validate(k_codes, v_codes, params, pages, page_size, kv_heads, dim, bits);
+    if (rc != BW_OK) return rc;
+    if (dtype != BW_F16 && dtype != BW_BF16) return BW_ERR_DTYPE;
+    if (batch < 0 || heads < 1 || heads % kv_heads != 0 || batch > ((int64_t)1 << 30) / heads) return BW_ERR_SHAPE;
+    // (a length is an int32: a table that holds more is not read further)
+    if (max_pages < 0 || table_stride < 0 || max_pages > INT32_MAX / page_size) return BW_ERR_SHAPE;
+    if (batch == 0) return BW_OK;
+    if (!q || !out || !lengths || (max_pages > 0 && !page_table)) return BW_ERR_NULL;
+    if (!aligned_to(q, 2) || !aligned_to(out, 2) || !aligned_to(page_table, 4) || !aligned_to(lengths, 4)) return BW_ERR_ALIGN;
+    const size_t need = kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
+    if (need && (!workspace || workspace_bytes < need)) return BW_ERR_WORKSPACE;
+    if (!aligned_to(workspace, 16)) return BW_ERR_ALIGN;
+    std::lock_guard<std::mutex> lock(scratch_lock(workspace));
+    return kv_attend(q, dtype, batch, heads, q_stride, q_head_stride, k_codes, v_codes, params, bits, pages, page_size, kv_heads, dim, page_table,
+                     table_stride, (int)max_pages, lengths, alpha, out, workspace, (cudaStream_t)stream);
+}
+
+// ---- low-rank adapters ----
+static int adapter_validate(int dtype, int64_t M, int64_t N, int64_t K, int n, int r, const void *index, const void *scaling) {
+    if (dtype != BW_F16 && dtype != BW_BF16) return BW_ERR_DTYPE;
+    if (M < 0 || N < 1 || K < 1 || n < 1 || r < 1 || r > 256 || N > (int64_t)1 << 24 || K > (int64_t)1 << 24) return BW_ERR_SHAPE;
+    if (M > ((int64_t)1 << 31) / r || n > (1 << 30) / r) return BW_ERR_SHAPE;
+    if (M > 0 && !index) return BW_ERR_NULL;
+    return aligned_to(index, 4) && aligned_to(scaling, 4) ? BW_OK : BW_ERR_ALIGN;
+}
+
+size_t bw_adapter_hidden_bytes(int64_t M, int64_t K, int adapters, int rank) {
+    return M < 1 || K < 1 || adapters < 1 || rank < 1 ? 0 : adapter_hidden_bytes(M, K, adapters, rank);
+}
+size_t bw_adapter_backward_bytes(int64_t M, int64_t N, int64_t K, int adapters, int rank) {
+    return M < 1 || N < 1 || K < 1 || adapters < 1 || rank < 1 ? 0 : adapter_backward_bytes(M, N, K, adapters, rank);
+}
+
+int bw_adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int adapters, int rank,
+                       const int32_t *index, const float *scaling, const void *base, void *out, void *hidden, size_t hidden_bytes, void *stream) {
+    const int rc = adapter_validate(dtype, M, N, K, adapters, rank, index, scaling);
+    if (rc != BW_OK) return rc;
+    if (M == 0) return BW_OK;
+    if (!x || !down || !up || !out) return BW_ERR_NULL;
+    if (!aligned_to(x, 2) || !aligned_to(down, 2) || !aligned_to(up, 2) || !aligned_to(base, 2) || !aligned_to(out, 2) || !aligned_to(hidden, 16))
+        return BW_ERR_ALIGN;
+    if (!hidden || hidden_bytes < adapter_hidden_bytes(M, K, adapters, rank)) return BW_ERR_WORKSPACE;
+    std::lock_guard<std::mutex> lock(scratch_lock(hidden));
+    return adapter_forward(x, dtype, M, N, K, down, up, adapters, rank, index, scaling, base, out, (float *)hidden, (cudaStream_t)stream);
+}
+
+int bw_adapter_backward(const void *grad_out, int dtype, const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int adapters,
+                        int rank, const int32_t *index, const float *scaling, const void *hidden, size_t hidden_bytes, void *grad_x, void *grad_down,
+                        void *grad_up, void *workspace, size_t workspace_bytes, void *stream) {
+    const int rc = adapter_validate(dtype, M, N, K, adapters, rank, index, scaling);
+    if (rc != BW_OK) return rc;
+    if (M > 0 && (!grad_out || !x || !down || !up)) return BW_ERR_NULL;
+    if (!aligned_to(grad_out, 2) || !aligned_to(x, 2) || !aligned_to(down, 2) || !aligned_to(up, 2) || !aligned_to(grad_x, 2) || !aligned_to(grad_down, 2) ||
+        !aligned_to(grad_up, 2) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
+        return BW_ERR_ALIGN;
+    if (M > 0 && grad_up && (!hidden || hidden_bytes < adapter_hidden_bytes(M, K, adapters, rank))) return BW_ERR_WORKSPACE;
+    if (M > 0 && (!workspace || workspace_bytes < adapter_backward_bytes(M, N, K, adapters, rank))) return BW_ERR_WORKSPACE;
+    std::lock_guard<std::mutex> lock(scratch_lock(workspace));
+    return adapter_backward(grad_out, dtype, x, M, N, K, down, up, adapters, rank, index, scaling, (const float *)hidden, grad_x, grad_down, grad_up,
+                            workspace, (cudaStream_t)stream);
 }
 
 // ---- peer-memory all-reduce (row-parallel layers on one node) ----

@@ -339,6 +339,71 @@ BW_API int bw_group_params_backward(const void *w_min, const void *w_max, int w_
                              float *grad_max_scale, void *stream);
 
 /*
+ * Quantised key-value cache, paged.  A row is one token's `dim` values of one head (dim <= 256, a multiple of 32/bits); slot s is row
+ * s % page_size of page s / page_size.  The caller owns three tensors, each starting on a 16-byte boundary:
+ *   k_codes, v_codes  [pages][heads][page_size][dim*bits/32] int32, packed like weights
+ *   params            [pages][heads][page_size][4] fp16: scale and zero point of the key, then of the value
+ * A row stands for scale * (code - zero_point).
+ *
+ * bw_kv_append quantises the rows k[t], v[t] into slot slots[t]: with Q = 2^bits - 1, lo = min(row, 0), hi = max(row, 0),
+ *   scale = (hi - lo) / Q rounded up to fp16, at least 2^-24;  zero_point = round(-lo / scale);  code = clamp(round(x / scale + zero_point), 0, Q)
+ * every operation rounded once in fp32.  (What quantize_rtn does to a group that holds zero, with the scale that is stored.)  A row with a
+ * NaN or an infinity, or whose scale leaves fp16's range, reads back as NaN.  Slots outside the cache (padding: -1) are skipped; a slot may
+ * be named once in a call (a row that two tokens write is left with parts of either).
+ *   k, v     BW_F32 | BW_F16 | BW_BF16; value d of head h of token t at t*stride + h*head_stride + d (strides in elements)
+ * bw_kv_read returns the values of slots[t] in rows of dense [tokens][heads][dim] tensors (16-byte aligned); zeros for slots outside
+ * the cache.
+ */
+BW_API int bw_kv_append(const void *k, const void *v, int dtype, int64_t tokens, int64_t k_stride, int64_t k_head_stride,
+                 int64_t v_stride, int64_t v_head_stride, const int64_t *slots, int heads, int dim, int bits, int64_t pages,
+                 int page_size, int32_t *k_codes, int32_t *v_codes, void *params, void *stream);
+BW_API int bw_kv_read(const int32_t *k_codes, const int32_t *v_codes, const void *params, int heads, int dim, int bits,
+               int64_t pages, int page_size, const int64_t *slots, int64_t tokens, void *k, void *v, int dtype, void *stream);
+
+/*
+ * Attention of one new token per sequence over that cache:
+ *   out[b][h] = sum_t w_t V[t],  w = softmax of alpha * q[b][h] . K[t] over t < lengths[b],  K, V rows of head h / (heads / kv_heads)
+ * where token t of sequence b is row t % page_size of page page_table[b*table_stride + t / page_size].
+ *   q        BW_F16 | BW_BF16; value d of head h of sequence b at b*q_stride + h*q_head_stride + d
+ *   out      dense [batch][heads][dim] of q's dtype
+ *   lengths  [batch] int32; 0 or less: the output is zero.  A length beyond max_pages pages, and a page outside the cache within
+ *            the length, give NaN for that sequence; neither is read.
+ *   workspace  bw_kv_attend_workspace_bytes(...) bytes (16-byte aligned), under the rules of bw_qmatmul's
+ */
+BW_API size_t bw_kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages);
+BW_API int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride,
+                 const int32_t *k_codes, const int32_t *v_codes, const void *params, int bits, int64_t pages, int page_size,
+                 int kv_heads, int dim, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                 const int32_t *lengths, float alpha, void *out, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   h[t] = down[i] x[t],  out[t] = base[t] + scaling[i] * up[i]^T h[t],  i = index[t]
+ * Rows whose index is negative have no adapter: out[t] = base[t].  An index of `adapters` or more gives NaN.
+ *   x, down, up, base, out  one dtype, BW_F16 | BW_BF16, dense: x [M][K], down [adapters][rank][K], up [adapters][rank][N] (both
+ *                           rank-major), base [M][N] or NULL (zeros), out [M][N], which may be base but not overlap it otherwise
+ *   index    [M] int32       scaling [adapters] fp32 or NULL (ones)
+ *   hidden   scratch of bw_adapter_hidden_bytes(...) (16-byte aligned), under the rules of bw_qmatmul's workspace; it holds h, which the
+ *            backward call needs again for grad_up
+ * Sums are fp32; out is rounded once.  Ranks up to 256.
+ */
+BW_API size_t bw_adapter_hidden_bytes(int64_t M, int64_t K, int adapters, int rank);
+BW_API int bw_adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up,
+                       int adapters, int rank, const int32_t *index, const float *scaling, const void *base, void *out,
+                       void *hidden, size_t hidden_bytes, void *stream);
+/*
+ * Its gradients, each computed where the pointer is not NULL (that of base is grad_out itself):
+ *   dh[t] = scaling[i] * up[i] grad_out[t],  grad_x[t] = down[i]^T dh[t],  grad_down[i] = sum dh[t] x[t]^T,
+ *   grad_up[i] = scaling[i] * sum h[t] grad_out[t]^T,   sums over the tokens of adapter i, in an order that only the sizes set
+ * Rows without an adapter have grad_x zero, and what stands in their x and grad_out reaches no sum.
+ */
+BW_API size_t bw_adapter_backward_bytes(int64_t M, int64_t N, int64_t K, int adapters, int rank);
+BW_API int bw_adapter_backward(const void *grad_out, int dtype, const void *x, int64_t M, int64_t N, int64_t K, const void *down,
+                        const void *up, int adapters, int rank, const int32_t *index, const float *scaling,
+                        const void *hidden, size_t hidden_bytes, void *grad_x, void *grad_down, void *grad_up,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * All-reduce (sum) of the row-parallel layers' partial outputs over peer memory on one node,
  * without NCCL.  No counterpart in the reference (it is single-GPU); it replaces the
  * ncclAllReduce that follows o_proj / down_proj in the tensor-parallel layers of this library.
