@@ -3,6 +3,8 @@
 //     out[b][h] = sum_t w_t V[t],   w = softmax over t < lengths[b] of  alpha * q[b][h] . K[t],   K, V rows of head h / (heads / kv_heads)
 //
 // One pass over the cache with the running maximum and sum of the softmax; codes become values in registers.
+#include <atomic>
+
 #include "bw_common.cuh"
 
 namespace bw {
@@ -100,33 +102,39 @@ int attend_general(const AttendArgs &p, int64_t batch, int bits, cudaStream_t st
 
 // ---- head dimensions of 64, 128 and 256, pages of whole tiles of 16 tokens --------------------------------------------
 //
-// A warp takes tiles of 16 tokens; K and V codes are the A operand of mma.sync.m16n8k16 (16 tokens, then 16 values, by 8 heads of the
-// group), so that one read of the cache serves all heads that share it:
+// A warp takes steps of one or two tiles of 16 tokens; K and V codes are the A operand of mma.sync.m16n8k16 (16 tokens, then 16 values, by
+// 8 heads of the group), so that one read of the cache serves all heads that share it:
 //   scores   S[t][h] = scale_t * (sum_d code[t][d] q[h][d] - zero_t * sum_d q[h][d]).  A code, masked out of its word, IS an fp16 number:
 //            the subnormal code * 2^-24 (tensor cores take subnormals exactly), so expanding two codes costs one AND.  Codes that stand in
 //            higher bits of their byte (`planes`) are larger by a power of two and get accumulators of their own.  Scale and zero point
 //            are applied to the sums, in fp32: nothing is rounded.
 //   weights  p = 2^(x - m); p * (value's scale) goes to fp16 for the second product.  m covers p * scale, so that this stays in fp16's
-//            range whatever the scales are; it moves only when some p * scale leaves [0, 1024] (one vote a tile).  For fp16 results the
-//            rest p - fp16(p) is a second operand, in the unused columns of groups of up to 4 heads or by second MMAs: one rounding
-//            of 2^-11 less in the result.  For bf16 results that rounding is an eighth of the result's own.
-//   values   O[d][h] += (code - zero_t)[d][t] * p[t][h]: 1024 + code by one OR, minus (1024 + zero), exact.  Codes of two tokens are put
-//            beside each other by one byte permutation a word.
+//            range whatever the scales are; it moves only when some p * scale leaves [0, 1024] (one vote a step).  For fp16 results the
+//            rest p - fp16(p) goes through MMAs of its own: one rounding of 2^-11 less in the result.  For bf16 results that
+//            rounding is an eighth of the result's own.
+//   values   O[d][h] += (code - zero_t)[d][t] * p[t][h]: 1024 + code by one OR, minus (1024 + zero), exact.  ldmatrix.trans puts
+//            16 bits (2 to 8 codes) of two tokens beside each other, as the operand wants them.
+// Groups of up to 4 heads fill half of the eight columns: their steps are two tiles, whose scores share one set of registers (columns 0 to 3
+// the first tile's, 4 to 7 the second's), which halves the work on weights; the columns' sums meet at the end.
 //
-// Work: all tiles of all sequences and heads in one line, an equal share of it to each CTA, whatever the lengths are.  What
-// a share has of a sequence that others have too goes to scratch (running maximum, sum, unnormalised output), and
-// kv_attend_join_kernel joins it.  Tables of few tiles go without: one CTA a sequence and head.
-constexpr int WARPS = 4, TILE = 16;
+// Bound by the bytes of the cache up to here, and by instruction issue at 2 and 4 bits.  Each warp has a ring of steps in shared memory, filled by
+// 16-byte cp.async and read by it alone: no block-wide barrier in the loop, and the loads in flight cost no registers.
+//
+// Work: all steps of all sequences and heads in one line, an equal share of it to each CTA, whatever the lengths are; a part of a sequence
+// counts START steps more, which is what its start and end cost.  What a share has of a sequence that others have too goes to scratch (running
+// maximum, sum, unnormalised output), and kv_attend_join_kernel joins it.  Tables of few tiles go without: one CTA a sequence and head.
+constexpr int WARPS = 4, TILE = 16, START = 8;
 constexpr int MOST_CTAS = 592;              // shares of a call: four CTAs on each of 148 SMs
 constexpr int SINGLE_TILES = 16;            // tables of up to so many tiles (256 tokens): one CTA, four tiles a warp
 
 struct FastArgs {
     AttendArgs a;
     int64_t batch;
-    float *slots;                           // [2 * MOST_CTAS][cols][dim + 2]
+    float *slots;                           // [2 * MOST_CTAS][cols] x ([dim] output; then [2]: maximum, sum)
     int units;                              // of a sequence: cache heads x blocks of query heads
     int blocks, cols;                       // blocks of query heads of a cache head; heads of a block
     int ctas, most_tiles, tiles_per_page;
+    int pair;                               // tiles of a step
     bool single;
 };
 
@@ -148,17 +156,23 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 }
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
-
-template <int BYTES> __device__ __forceinline__ void load_bytes(const uint8_t *p, uint32_t *w) {
-    if constexpr (BYTES == 2) w[0] = __ldg(reinterpret_cast<const unsigned short *>(p));
-    else if constexpr (BYTES == 4) w[0] = __ldg(reinterpret_cast<const uint32_t *>(p));
-    else if constexpr (BYTES == 8) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = v.x; w[1] = v.y;
-    } else {
-        const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p));
-        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    }
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t to, const uint8_t *from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+template <int WORDS> __device__ __forceinline__ void load_words(uint32_t at, uint32_t *w) {
+    if constexpr (WORDS == 1) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at) : "memory");
+    else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+    else asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_transposed2(uint32_t at, uint32_t *x) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_transposed4(uint32_t at, uint32_t *x) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
 }
 
 // Tiles of a sequence within its table; its true length goes beside it.
@@ -166,94 +180,70 @@ __device__ __forceinline__ int tiles_of(int n, int most) {
     const int t = n > 0 ? (n - 1) / TILE + 1 : 0;
     return t < most ? t : most;
 }
-
-// Tiles of all sequences together (every warp by itself: a step of 32 sequences).
-__device__ __forceinline__ int64_t tiles_of_all(const FastArgs &p) {
-    const int lane = threadIdx.x % 32;
-    int64_t sum = 0;
-    for (int64_t b = lane; b < p.batch; b += 32) sum += tiles_of(__ldcg(p.a.lengths + b), p.most_tiles);
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    return sum;
+// What a unit (a block of heads of a sequence) counts in the line of work; 0 for an empty sequence.
+__device__ __forceinline__ int weight_of(const FastArgs &p, int64_t b) {
+    const int tiles = tiles_of(__ldcg(p.a.lengths + b), p.most_tiles);
+    return tiles ? (tiles + p.pair - 1) / p.pair + START : 0;
 }
-
-// The tiles of one CTA's share.  Shares of less than two tiles a warp are not worth another CTA.
+// The steps of one CTA's share of `total`.  Shares of less than two steps a warp are not worth another CTA.
 __device__ __forceinline__ int64_t share(const FastArgs &p, int64_t total) {
     const int64_t even = (total + p.ctas - 1) / p.ctas;
     return even < 2 * WARPS ? 2 * WARPS : even;
 }
 
+// How a tile lies in shared memory: 16 rows of keys, 16 of values, 16 constants; the 16-byte pieces of a row are exchanged by row so that eight
+// rows' pieces of one number (ldmatrix) lie in different banks.
 template <int BITS, int DIM> struct Shape {
     static constexpr int PLANES = 8 / BITS;                 // places of a code in a byte
-    static constexpr int KW = DIM * BITS / 128;             // words of a key row that a lane holds (of two rows)
-    static constexpr int VH = DIM * BITS / 128;             // 16-bit halves of a value row that a lane holds (of four rows)
-    static constexpr int VW = (VH + 1) / 2;
-    static constexpr int KMMAS = KW * PLANES, VMMAS = VH * PLANES;   // DIM / 16 each
-    static constexpr uint32_t MASK = ((1u << BITS) - 1) * 0x00010001u;
-    static constexpr bool AHEAD = KW <= 4;                  // the next tile is loaded before the present one is used: else registers run out
-    static constexpr int STRIDE = DIM + DIM / 16 + (36 - (DIM + DIM / 16) % 32) % 32;   // of a head's sums in shared memory: 4 mod 32, values padded by one in 16
-    // Byte of a lane's word i of a key row (quarter c), and of a value row (eighth r): 16-byte pieces side by side.
-    static __device__ __forceinline__ int key_byte(int i, int c) { return KW <= 4 ? (c * KW + i) * 4 : (i / 4) * 64 + c * 16 + (i % 4) * 4; }
-    static __device__ __forceinline__ int value_byte(int half, int r) { return VH <= 8 ? (r * VH + half) * 2 : (half / 8) * 128 + r * 16 + (half % 8) * 2; }
+    static constexpr int ROW = DIM * BITS / 8, PIECES = ROW / 16;
+    static constexpr int KW = ROW / 16;                     // words of a key row that a lane holds
+    static constexpr int MMAS = DIM / 16;                   // of a tile's keys, and of its values
+    static constexpr int BYTES = 32 * ROW + 128;
+    static constexpr int STRIDE = DIM + 1;                  // of a column's sums in shared memory
+    static __device__ __forceinline__ int swizzle(int row) { return ROW >= 128 ? row & 7 : ROW == 64 ? row >> 1 & 3 : ROW == 32 ? row >> 2 & 1 : 0; }
 };
 
-template <int BITS, int DIM>
-struct Tile {
-    using S = Shape<BITS, DIM>;
-    uint32_t k[2][S::KW], v[4][S::VW];
-    uint2 c[2];                             // constants of the lane's two key rows: (scale, zero) of key and value
+template <typename T, int BITS, int DIM, int NB, int PAIR>
+struct Config {
+    static constexpr int COLS = 8 * NB, STEP = PAIR * Shape<BITS, DIM>::BYTES;
+    static constexpr int STAGES = STEP <= 2304 ? 4 : STEP <= 4352 ? 3 : 2;      // of a warp's ring: 9 to 17 KB
+    static constexpr int RING = WARPS * STAGES * STEP, SUMS = WARPS * COLS * Shape<BITS, DIM>::STRIDE * 4;
+    static constexpr int SMEM = RING > SUMS ? RING : SUMS;
 };
 
-template <int BITS, int DIM>
-__device__ __forceinline__ void load_keys(Tile<BITS, DIM> &t, const AttendArgs &a, int64_t row0, int r, int c) {
-    using S = Shape<BITS, DIM>;
-    constexpr int BYTES = S::KW >= 4 ? 16 : S::KW * 4;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int64_t row = row0 + (r >> 1) + 4 * (r & 1) + 8 * j;
-        const uint8_t *p = reinterpret_cast<const uint8_t *>(a.k_codes) + row * (DIM * BITS / 8);
-#pragma unroll
-        for (int i = 0; i < S::KW; i += BYTES / 4) load_bytes<BYTES>(p + S::key_byte(i, c), t.k[j] + i);
-        t.c[j] = __ldg(reinterpret_cast<const uint2 *>(a.params) + row);
-    }
-}
-template <int BITS, int DIM>
-__device__ __forceinline__ void load_values(Tile<BITS, DIM> &t, const AttendArgs &a, int64_t row0, int r, int c) {
-    using S = Shape<BITS, DIM>;
-    constexpr int BYTES = S::VH >= 8 ? 16 : S::VH * 2;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint8_t *p = reinterpret_cast<const uint8_t *>(a.v_codes) + (row0 + c + 4 * j) * (DIM * BITS / 8);
-#pragma unroll
-        for (int h = 0; h < S::VH; h += BYTES / 2) load_bytes<BYTES>(p + S::value_byte(h, r), t.v[j] + h / 2);
-    }
-}
-
-// REST: how the rests of the weights' rounding enter.  0: not (bf16 results); 1: columns 4 to 7 repeat columns 0 to 3 and carry the rests
-// (groups of up to 4); 2: MMAs of their own.
-template <typename T, int BITS, int DIM, int NB, int REST>
+template <typename T, int BITS, int DIM, int NB, int PAIR>
 __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p) {
     using S = Shape<BITS, DIM>;
-    constexpr int COLS = 8 * NB;
+    using C = Config<T, BITS, DIM, NB, PAIR>;
+    static_assert(PAIR == 1 || NB == 1, "steps of two tiles are for groups of up to four heads");
+    constexpr bool REST = __is_same(T, __half);
+    constexpr int COLS = C::COLS, STAGES = C::STAGES, HEADS = PAIR == 2 ? 4 : COLS;
     const AttendArgs &a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-    __shared__ __align__(16) __half sq[COLS][DIM + 8];
-    __shared__ float s_factor[COLS], s_sum[COLS], s_m[WARPS][COLS], s_l[WARPS][COLS];
-    __shared__ __align__(16) float s_o[WARPS][COLS * S::STRIDE];
+    extern __shared__ __align__(128) uint8_t smem[];        // the warps' rings; at the end of a part, their sums
+    __shared__ __align__(16) __half sq[HEADS][DIM + 8];
+    __shared__ float s_factor[HEADS], s_sum[HEADS], s_m[WARPS][COLS], s_l[WARPS][COLS];
+    float *s_o = reinterpret_cast<float *>(smem);
+    const uint32_t ring = smem_addr(smem) + warp * (STAGES * C::STEP);
     pdl_launch_dependents();
 
-    // this CTA's share of the line of tiles, and the sequence in which it starts
-    int64_t at, end, b = 0, before = 0;      // `before`: tiles in front of sequence b
+    // this CTA's share of the line of work, and the sequence in which it starts
+    int64_t at, end, b = 0, before = 0;      // `before`: work in front of sequence b, of one unit
     if (p.single) {
         b = blockIdx.x / p.units;
         at = 0;
         end = INT64_MAX;
     } else {
-        const int64_t total = tiles_of_all(p) * p.units, per = share(p, total);
+        int64_t total = 0;
+        for (int64_t i = lane; i < p.batch; i += 32) total += weight_of(p, i);
+        for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+        total *= p.units;
+        const int64_t per = share(p, total);
         at = blockIdx.x * per;
         end = at + per < total ? at + per : total;
         if (at >= end) return;
         for (int64_t b0 = 0; b0 < p.batch; b0 += 32) {
-            const int mine = b0 + lane < p.batch ? tiles_of(__ldcg(a.lengths + b0 + lane), p.most_tiles) : 0;
+            const int mine = b0 + lane < p.batch ? weight_of(p, b0 + lane) : 0;
             int64_t sum = mine;
             for (int d = 1; d < 32; d *= 2) {
                 const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
@@ -272,29 +262,92 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
     }
 
     while (at < end && b < p.batch) {
-        // the next part of one sequence, cache head and block of query heads: tiles [from, to) of `tiles`
-        const int n = __ldcg(a.lengths + b), tiles = tiles_of(n, p.most_tiles);
+        // the next part of one sequence, cache head and block of query heads: steps [from, to) of `steps`
+        const int n = __ldcg(a.lengths + b), tiles = tiles_of(n, p.most_tiles), steps = (tiles + PAIR - 1) / PAIR, weight = steps + START;
         if (!p.single && tiles == 0) {
             ++b;
             continue;
         }
         const int64_t start = before * p.units;
-        const int unit = p.single ? (int)(blockIdx.x % p.units) : (int)((at - start) / tiles);
-        const int from = p.single ? 0 : (int)(at - start - (int64_t)unit * tiles);
-        const int to = p.single || end - at > tiles - from ? tiles : from + (int)(end - at);
+        const int unit = p.single ? (int)(blockIdx.x % p.units) : (int)((at - start) / weight);
         if (unit >= p.units) return;           // (lengths that change under the call)
+        int from = 0, to = steps;
+        if (!p.single) {
+            const int64_t in = at - start - (int64_t)unit * weight, out = in + (end - at);
+            from = in > START ? (int)in - START : 0;
+            to = out >= weight ? steps : out > START ? (int)out - START : 0;
+            at += (out < weight ? out : weight) - in;
+            if (to == steps && unit == p.units - 1) before += weight;
+            if (to <= from) continue;          // (only of what the part's start counts for; the sequence goes on in the next share)
+        }
+        const int64_t seq = b;
+        if (!p.single && to == steps && unit == p.units - 1) ++b;
         const int kh = unit / p.blocks, group = a.heads / a.kv_heads, h0 = (unit - kh * p.blocks) * p.cols;
         const int heads = group - h0 < p.cols ? group - h0 : p.cols;      // of this block
-        const int64_t out0 = (b * a.heads + (int64_t)kh * group + h0) * DIM;
+        const int64_t head0 = (int64_t)kh * group + h0;
+        __syncthreads();
+
+        // pages: `page_at` and `in` go forward with the warp's tiles; the ids are loaded a step before they are needed
+        bool bad = n > p.most_tiles * TILE;          // more than the table holds (pages are whole tiles)
+        int step = from + warp;                       // of the next look-up
+        int page_at = step * PAIR / p.tiles_per_page, in_page = step * PAIR - page_at * p.tiles_per_page;
+        const int step_pages = WARPS * PAIR / p.tiles_per_page, step_in = WARPS * PAIR - step_pages * p.tiles_per_page;
+        const int32_t *pages = a.table + seq * a.table_stride;
+        auto look_up = [&](int (&page)[PAIR], int (&place)[PAIR]) {
+            int at_page = page_at, at_in = in_page;
+#pragma unroll
+            for (int i = 0; i < PAIR; ++i) {
+                place[i] = at_in;
+                page[i] = step < to && step * PAIR + i < tiles ? __ldg(pages + at_page) : -2;
+                if (++at_in == p.tiles_per_page) {
+                    at_in = 0;
+                    ++at_page;
+                }
+            }
+            page_at += step_pages;
+            in_page += step_in;
+            if (in_page >= p.tiles_per_page) {
+                in_page -= p.tiles_per_page;
+                ++page_at;
+            }
+            step += WARPS;
+        };
+        const int page_rows = a.kv_heads * a.page_size, head_row = kh * a.page_size;
+        auto copy_step = [&](int stage, const int (&page)[PAIR], const int (&place)[PAIR]) {
+            const uint32_t to_smem = ring + stage * C::STEP;
+#pragma unroll
+            for (int i = 0; i < PAIR; ++i) {
+                if (page[i] >= 0 && page[i] < a.pages) {
+                    const int64_t row0 = (int64_t)page[i] * page_rows + (head_row + place[i] * TILE);
+                    const uint8_t *k = reinterpret_cast<const uint8_t *>(a.k_codes) + row0 * S::ROW + lane * 16;
+                    const uint8_t *v = reinterpret_cast<const uint8_t *>(a.v_codes) + row0 * S::ROW + lane * 16;
+                    const uint32_t t = to_smem + i * S::BYTES;
+#pragma unroll
+                    for (int j = 0; j < (S::ROW + 31) / 32; ++j) {
+                        const int piece = lane + 32 * j, row = piece / S::PIECES;
+                        const uint32_t o = t + row * S::ROW + ((piece % S::PIECES) ^ S::swizzle(row)) * 16;
+                        if (S::ROW >= 32 || lane < 16) {
+                            copy16(o, k + j * 512);
+                            copy16(o + 16 * S::ROW, v + j * 512);
+                        }
+                    }
+                    if (lane < 8) copy16(t + 32 * S::ROW + lane * 16, reinterpret_cast<const uint8_t *>(a.params) + row0 * 8 + lane * 16);
+                } else if (page[i] != -2) bad = true;
+            }
+            copies_commit();
+        };
+        int page[STAGES][PAIR], place[STAGES][PAIR];
+#pragma unroll
+        for (int i = 0; i < STAGES; ++i) look_up(page[i], place[i]);
+#pragma unroll
+        for (int i = 0; i < STAGES - 1; ++i) copy_step(i, page[i], place[i]);
 
         // the queries in fp16: as they are, or (bf16) divided by a power of two near their largest value, which the scores get back
-        __syncthreads();
-        for (int h = warp; h < COLS; h += WARPS) {
-            const int head = REST == 1 ? h % 4 : h;
+        for (int h = warp; h < HEADS; h += WARPS) {
             float v[DIM / 32], big = 0.0f, sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < DIM / 32; ++i) {
-                v[i] = head < heads ? to_f32(((const T *)a.q)[b * a.q_stride + (int64_t)(kh * group + h0 + head) * a.q_head_stride + lane + 32 * i]) : 0.0f;
+                v[i] = h < heads ? to_f32(((const T *)a.q)[seq * a.q_stride + (head0 + h) * a.q_head_stride + lane + 32 * i]) : 0.0f;
                 big = fmaxf(big, fabsf(v[i]));
             }
             float back = 1.0f;
@@ -319,114 +372,100 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
             }
         }
         __syncthreads();
-        uint32_t q[NB][S::KMMAS][2];
+        uint32_t q[NB][S::MMAS][2];
         float f[NB][2], fsum[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const __half *row = sq[nb * 8 + r];
+            const __half *row = sq[(nb * 8 + r) % HEADS] + c * (DIM / 4);
 #pragma unroll
-            for (int i = 0; i < S::KW; ++i) {
-                const int d0 = S::key_byte(i, c) * 8 / BITS;
+            for (int i = 0; i < S::KW; ++i)
 #pragma unroll
                 for (int pl = 0; pl < S::PLANES; ++pl) {
-                    const int d = d0 + pl;
-                    q[nb][i * S::PLANES + pl][0] = as_u32(__halves2half2(row[d], row[d + 16 / BITS]));
-                    q[nb][i * S::PLANES + pl][1] = as_u32(__halves2half2(row[d + S::PLANES], row[d + S::PLANES + 16 / BITS]));
+                    const __half *d = row + i * (32 / BITS) + pl;
+                    q[nb][i * S::PLANES + pl][0] = as_u32(__halves2half2(d[0], d[16 / BITS]));
+                    q[nb][i * S::PLANES + pl][1] = as_u32(__halves2half2(d[S::PLANES], d[S::PLANES + 16 / BITS]));
                 }
-            }
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                f[nb][j] = s_factor[nb * 8 + 2 * c + j];
-                fsum[nb][j] = f[nb][j] * s_sum[nb * 8 + 2 * c + j];
+                f[nb][j] = s_factor[(nb * 8 + 2 * c + j) % HEADS];
+                fsum[nb][j] = f[nb][j] * s_sum[(nb * 8 + 2 * c + j) % HEADS];
             }
         }
 
-        float o[NB][S::VMMAS][4] = {}, m[NB][2], l[NB][2] = {};
+        float o[NB][S::MMAS][4] = {}, m[NB][2], l[NB][2] = {};
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = -INFINITY;
-        bool bad = n > p.most_tiles * TILE;          // more than the table holds (pages are whole tiles)
-
-        // pages: the tile's place in its page goes forward with the tiles
-        int tile = from + warp, page_at = tile / p.tiles_per_page, in = tile - page_at * p.tiles_per_page;
-        const int step_pages = WARPS / p.tiles_per_page, step_in = WARPS - step_pages * p.tiles_per_page;
-        const int32_t *pages = a.table + b * a.table_stride;
-        int page = tile < to ? __ldg(pages + page_at) : 0, place = in;
-        auto forward = [&](int next) {               // `page` and `place` of tile `next`
-            page_at += step_pages;
-            in += step_in;
-            if (in >= p.tiles_per_page) {
-                in -= p.tiles_per_page;
-                ++page_at;
-            }
-            if (next < to) page = __ldg(pages + page_at);
-            place = in;
-        };
-        Tile<BITS, DIM> cur = {}, ahead = {};
-        auto row_of = [&]() { return ((int64_t)page * a.kv_heads + kh) * a.page_size + place * TILE; };
-        auto valid = [&]() { return page >= 0 && page < a.pages; };
-        if (S::AHEAD && tile < to) {
-            if (valid()) {
-                load_keys(cur, a, row_of(), r, c);
-                load_values(cur, a, row_of(), r, c);
-            } else bad = true;
-            forward(tile + WARPS);
-        }
-#pragma unroll 2
-        for (; tile < to; tile += WARPS) {
-            if constexpr (S::AHEAD) {
-                if (tile + WARPS < to) {
-                    if (valid()) {
-                        load_keys(ahead, a, row_of(), r, c);
-                        load_values(ahead, a, row_of(), r, c);
-                    } else bad = true;
-                    forward(tile + 2 * WARPS);
-                }
-            } else {
-                if (valid()) {
-                    load_keys(cur, a, row_of(), r, c);
-                    load_values(cur, a, row_of(), r, c);
-                } else bad = true;
-                forward(tile + WARPS);
-            }
+        const int half_tile = PAIR == 2 ? c / 2 : 0;         // the tile whose scores this lane's columns are
+        int stage = 0, next = STAGES - 1;
+#pragma unroll 1
+        for (int now = from + warp; now < to; now += WARPS) {
+            copies_wait<STAGES - 2>();
+            __syncwarp();                                     // all lanes' copies are there, and all have used the stage that is filled next
+            copy_step(next, page[STAGES - 1], place[STAGES - 1]);
+            look_up(page[STAGES - 1], place[STAGES - 1]);
+            const uint32_t buf = ring + stage * C::STEP;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            next = next + 1 == STAGES ? 0 : next + 1;
 
             // scores
-            float acc[NB][S::PLANES][4] = {};
+            float acc[NB][S::PLANES][4];
 #pragma unroll
-            for (int i = 0; i < S::KW; ++i) {
-                const uint32_t w0 = cur.k[0][i], w1 = cur.k[1][i], u0 = w0 >> 8, u1 = w1 >> 8;
+            for (int i = 0; i < PAIR; ++i) {
+                float sum[NB][S::PLANES][4] = {};
+                uint32_t w[2][S::KW];
 #pragma unroll
-                for (int pl = 0; pl < S::PLANES; ++pl) {
-                    constexpr uint32_t MASK = S::MASK;
-                    const uint32_t bits = MASK << (pl * BITS);
+                for (int j = 0; j < 2; ++j) {
+                    const int row = r + 8 * j;
+                    constexpr int WORDS = S::KW < 4 ? S::KW : 4;
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
-                        mma(acc[nb][pl], w0 & bits, w1 & bits, u0 & bits, u1 & bits, q[nb][i * S::PLANES + pl][0], q[nb][i * S::PLANES + pl][1]);
+                    for (int x = 0; x < S::KW; x += WORDS) {
+                        const int byte = (c * S::KW + x) * 4;
+                        load_words<WORDS>(buf + i * S::BYTES + row * S::ROW + (((byte / 16) ^ S::swizzle(row)) * 16 + byte % 16), w[j] + x);
+                    }
                 }
+#pragma unroll
+                for (int x = 0; x < S::KW; ++x) {
+                    const uint32_t u0 = w[0][x] >> 8, u1 = w[1][x] >> 8;
+#pragma unroll
+                    for (int pl = 0; pl < S::PLANES; ++pl) {
+                        const uint32_t bits = ((1u << BITS) - 1) * 0x00010001u << (pl * BITS);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            mma(sum[nb][pl], w[0][x] & bits, w[1][x] & bits, u0 & bits, u1 & bits, q[nb][x * S::PLANES + pl][0], q[nb][x * S::PLANES + pl][1]);
+                    }
+                }
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int pl = 0; pl < S::PLANES; ++pl)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[nb][pl][e] = i == 0 || half_tile == 1 ? sum[nb][pl][e] : acc[nb][pl][e];
             }
-            const int t0 = tile * TILE + (r >> 1) + 4 * (r & 1);
+            const int t0 = (now * PAIR + half_tile) * TILE + r;
             float ks[2], kz[2], vs[2];
             uint32_t vz[2];
             bool live[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const float2 kc = __half22float2(as_half2(cur.c[j].x));
-                live[j] = t0 + 8 * j < n;             // rows behind the sequence may hold anything
+                uint32_t constants[2];
+                load_words<2>(buf + half_tile * S::BYTES + 32 * S::ROW + (r + 8 * j) * 8, constants);
+                const float2 kc = __half22float2(as_half2(constants[0]));
+                live[j] = t0 + 8 * j < n && (PAIR == 1 || now * PAIR + half_tile < tiles);             // rows behind the sequence may hold anything
                 ks[j] = kc.x;
                 kz[j] = kc.y;
-                const __half2 vc = as_half2(cur.c[j].y);
+                const __half2 vc = as_half2(constants[1]);
                 vs[j] = live[j] ? __low2float(vc) : 0.0f;
                 vz[j] = live[j] ? as_u32(__high2half2(vc)) : 0u;
             }
             float u[NB][4];                           // [j * 2 + column]
-            uint32_t w[NB][2][2];                     // [j][weights, rests]
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float dot = acc[nb][0][e] * 0x1p24f;
+                    float dot = acc[nb][0][e];
 #pragma unroll
-                    for (int pl = 1; pl < S::PLANES; ++pl) dot = fmaf(acc[nb][pl][e], 0x1p24f / (1 << (pl * BITS)), dot);
-                    u[nb][e] = ks[e / 2] * fmaf(dot, f[nb][e % 2], -kz[e / 2] * fsum[nb][e % 2]);
+                    for (int pl = 1; pl < S::PLANES; ++pl) dot = fmaf(acc[nb][pl][e], 1.0f / (1 << (pl * BITS)), dot);
+                    u[nb][e] = ks[e / 2] * fmaf(dot, f[nb][e % 2] * 0x1p24f, -kz[e / 2] * fsum[nb][e % 2]);
                 }
             float pv[NB][4], pw[NB][4];
             bool over = false;
@@ -442,7 +481,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
             };
             weights();
             if (__any_sync(0xffffffffu, over)) {
-                // the maximum moves: the largest of this tile's p and p * scale becomes at most 1
+                // the maximum moves: the largest p * scale of this step becomes 1
                 const float lv[2] = {fmaxf(__log2f(vs[0]), -40.0f), fmaxf(__log2f(vs[1]), -40.0f)};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
@@ -457,13 +496,14 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
                         m[nb][j] = top;
                         l[nb][j] *= keep;
 #pragma unroll
-                        for (int i = 0; i < S::VMMAS; ++i) {
+                        for (int i = 0; i < S::MMAS; ++i) {
                             o[nb][i][j] *= keep;
                             o[nb][i][2 + j] *= keep;
                         }
                     }
                 weights();
             }
+            uint32_t w[NB][2][2];                     // [j][weights, rests]
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -471,48 +511,66 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
                     l[nb][0] += pw[nb][2 * j];
                     l[nb][1] += pw[nb][2 * j + 1];
                     const __half2 top = __floats2half2_rn(pv[nb][2 * j], pv[nb][2 * j + 1]);
-                    w[nb][j][0] = as_u32(top);
-                    if constexpr (REST != 0) {
+                    w[nb][j][0] = transpose8x8(as_u32(top));
+                    if constexpr (REST) {
                         const float2 t = __half22float2(top);
-                        const uint32_t rest = as_u32(__floats2half2_rn(pv[nb][2 * j] - t.x, pv[nb][2 * j + 1] - t.y));
-                        if constexpr (REST == 1) w[nb][j][0] = c >= 2 ? rest : w[nb][j][0];
-                        else w[nb][j][1] = transpose8x8(rest);
+                        w[nb][j][1] = transpose8x8(as_u32(__floats2half2_rn(pv[nb][2 * j] - t.x, pv[nb][2 * j + 1] - t.y)));
                     }
-                    w[nb][j][0] = transpose8x8(w[nb][j][0]);
                 }
+            // Zero points of two tokens beside each other.  (The transposed matrix has every column of a row alike where a step is one tile; of two tiles
+            // columns 0 to 3, now rows, have the first one's and 4 to 7 the second one's.)
+            uint32_t zt[2] = {transpose8x8(vz[0]), transpose8x8(vz[1])};
 
             // values
-            __half2 zero[S::PLANES][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const __half2 z = as_half2(transpose8x8(vz[j]));
+            for (int i = 0; i < PAIR; ++i) {
+                __half2 zero[S::PLANES][2];
+                uint32_t b0[NB][2], b1[NB][2];
 #pragma unroll
-                for (int pl = 0; pl < S::PLANES; ++pl) zero[pl][j] = __hfma2(z, __float2half2_rn((float)(1 << (pl * BITS))), __float2half2_rn(1024.0f));
-            }
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t z = zt[j];
+                    if constexpr (PAIR == 2) z = __shfl_sync(0xffffffffu, z, c + 16 * i);
 #pragma unroll
-            for (int h = 0; h < S::VH; ++h) {
-                const uint32_t sel = h % 2 ? 0x7632 : 0x5410;
-                const uint32_t x0 = __byte_perm(cur.v[0][h / 2], cur.v[1][h / 2], sel), x1 = __byte_perm(cur.v[2][h / 2], cur.v[3][h / 2], sel);
-                const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
+                    for (int pl = 0; pl < S::PLANES; ++pl) zero[pl][j] = __hfma2(as_half2(z), __float2half2_rn((float)(1 << (pl * BITS))), __float2half2_rn(1024.0f));
+                }
 #pragma unroll
-                for (int pl = 0; pl < S::PLANES; ++pl) {
-                    constexpr uint32_t MASK = S::MASK;
-                    const uint32_t bits = MASK << (pl * BITS);
-                    const uint32_t a0 = as_u32(__hsub2(as_half2((x0 & bits) | 0x64006400u), zero[pl][0]));
-                    const uint32_t a1 = as_u32(__hsub2(as_half2((y0 & bits) | 0x64006400u), zero[pl][0]));
-                    const uint32_t a2 = as_u32(__hsub2(as_half2((x1 & bits) | 0x64006400u), zero[pl][1]));
-                    const uint32_t a3 = as_u32(__hsub2(as_half2((y1 & bits) | 0x64006400u), zero[pl][1]));
+                for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        mma(o[nb][h * S::PLANES + pl], a0, a1, a2, a3, w[nb][0][0], w[nb][1][0]);
-                        if constexpr (REST == 2) mma(o[nb][h * S::PLANES + pl], a0, a1, a2, a3, w[nb][0][1], w[nb][1][1]);
+                    for (int k = 0; k < (REST ? 2 : 1); ++k) {
+                        const bool mine = PAIR == 1 || r / 4 == i;      // columns of this tile's weights
+                        b0[nb][k] = mine ? w[nb][0][k] : 0u;
+                        b1[nb][k] = mine ? w[nb][1][k] : 0u;
+                    }
+                const uint32_t values = buf + i * S::BYTES + 16 * S::ROW;
+#pragma unroll
+                for (int piece = 0; piece < S::PIECES; piece += 2) {
+                    uint32_t x[4];                    // [piece][tokens 0 to 7, 8 to 15]
+                    const int row = lane % 16;
+                    if constexpr (S::PIECES == 1) load_transposed2(values + row * S::ROW, x);
+                    else load_transposed4(values + row * S::ROW + ((piece + lane / 16) ^ S::swizzle(row)) * 16, x);
+#pragma unroll
+                    for (int h = 0; h < (S::PIECES == 1 ? 1 : 2); ++h) {
+                        const uint32_t x0 = x[2 * h], x1 = x[2 * h + 1], y0 = x0 >> 8, y1 = x1 >> 8;
+#pragma unroll
+                        for (int pl = 0; pl < S::PLANES; ++pl) {
+                            const uint32_t bits = ((1u << BITS) - 1) * 0x00010001u << (pl * BITS);
+                            const uint32_t a0 = as_u32(__hsub2(as_half2((x0 & bits) | 0x64006400u), zero[pl][0]));
+                            const uint32_t a1 = as_u32(__hsub2(as_half2((y0 & bits) | 0x64006400u), zero[pl][0]));
+                            const uint32_t a2 = as_u32(__hsub2(as_half2((x1 & bits) | 0x64006400u), zero[pl][1]));
+                            const uint32_t a3 = as_u32(__hsub2(as_half2((y1 & bits) | 0x64006400u), zero[pl][1]));
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                mma(o[nb][(piece + h) * S::PLANES + pl], a0, a1, a2, a3, b0[nb][0], b1[nb][0]);
+                                if constexpr (REST) mma(o[nb][(piece + h) * S::PLANES + pl], a0, a1, a2, a3, b0[nb][1], b1[nb][1]);
+                            }
+                        }
                     }
                 }
             }
-            if constexpr (S::AHEAD) cur = ahead;
         }
 
-        // the four warps' parts become one
+        // the warps' parts become one
+        copies_wait<0>();
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -529,109 +587,111 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const int col = nb * 8 + 2 * c + j;
-                float top = s_m[0][col];
+                float top = -INFINITY;
 #pragma unroll
-                for (int w2 = 1; w2 < WARPS; ++w2) top = fmaxf(top, s_m[w2][col]);
+                for (int i = 0; i < WARPS * PAIR; ++i) top = fmaxf(top, s_m[i / PAIR][PAIR == 2 ? col % 4 + i % 2 * 4 : col]);
                 const float by = m[nb][j] == -INFINITY ? 0.0f : ex2(m[nb][j] - top);
 #pragma unroll
-                for (int h = 0; h < S::VH; ++h)
+                for (int i = 0; i < S::MMAS; ++i)
 #pragma unroll
-                    for (int pl = 0; pl < S::PLANES; ++pl)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const int d = S::value_byte(h, r) * 8 / BITS + pl + k * S::PLANES;
-                            s_o[warp][col * S::STRIDE + d + d / 16] = o[nb][h * S::PLANES + pl][2 * k + j] * (by / (1 << (pl * BITS)));
-                        }
+                    for (int k = 0; k < 2; ++k) {
+                        const int pl = i % S::PLANES, d = (i / S::PLANES * 8 + r) * (16 / BITS) + pl + k * S::PLANES;
+                        s_o[(warp * COLS + col) * S::STRIDE + d] = o[nb][i][2 * k + j] * (by / (1 << (pl * BITS)));
+                    }
             }
         __syncthreads();
-        const bool whole = from == 0 && to == tiles;
+        const bool whole = from == 0 && to == steps;
         float *slot = p.slots + (int64_t)(2 * blockIdx.x + (from == 0)) * p.cols * (DIM + 2);
         for (int i = threadIdx.x; i < heads * DIM; i += 32 * WARPS) {
             const int col = i / DIM, d = i % DIM;
-            float sum = 0.0f, total = 0.0f, top = s_m[0][col];
+            float sum = 0.0f, total = 0.0f, top = -INFINITY;
 #pragma unroll
-            for (int w2 = 1; w2 < WARPS; ++w2) top = fmaxf(top, s_m[w2][col]);
+            for (int k = 0; k < WARPS * PAIR; ++k) top = fmaxf(top, s_m[k / PAIR][col + k % PAIR * 4]);
 #pragma unroll
-            for (int w2 = 0; w2 < WARPS; ++w2) {
-                sum += s_o[w2][col * S::STRIDE + d + d / 16];
-                if constexpr (REST == 1) sum += s_o[w2][(col + 4) * S::STRIDE + d + d / 16];
-                total += s_m[w2][col] == -INFINITY ? (s_l[w2][col] == s_l[w2][col] ? 0.0f : NAN) : s_l[w2][col] * ex2(s_m[w2][col] - top);
+            for (int k = 0; k < WARPS * PAIR; ++k) {
+                const int from_col = col + k % PAIR * 4;
+                const float km = s_m[k / PAIR][from_col], kl = s_l[k / PAIR][from_col];
+                sum += s_o[(k / PAIR * COLS + from_col) * S::STRIDE + d];
+                total += km == -INFINITY ? (kl == kl ? 0.0f : NAN) : kl * ex2(km - top);
             }
-            if (whole) ((T *)a.out)[out0 + i] = from_f32<T>(n <= 0 ? 0.0f : sum / total);
+            if (whole) ((T *)a.out)[(seq * a.heads + head0) * DIM + i] = from_f32<T>(n <= 0 ? 0.0f : sum / total);
             else {
-                slot[col * (DIM + 2) + d] = sum;
-                if (d == 0) {
-                    slot[col * (DIM + 2) + DIM] = top;
-                    slot[col * (DIM + 2) + DIM + 1] = total;
-                }
+                slot[i] = sum;
+                if (d == 0) *reinterpret_cast<float2 *>(slot + p.cols * DIM + 2 * col) = make_float2(top, total);
             }
         }
         if (p.single) return;
-        at += to - from;
-        if (to == tiles && unit == p.units - 1) {
-            before += tiles;
-            ++b;
-        }
     }
 }
 
 // One CTA a head of a sequence: zeros for an empty sequence, and the parts of one that several CTAs share.
-template <typename T>
-__global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p, int dim) {
+template <typename T, int DIM>
+__global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
     pdl_wait();
     const AttendArgs &a = p.a;
     const int64_t b = blockIdx.x / a.heads;
     const int h = (int)(blockIdx.x - b * a.heads), group = a.heads / a.kv_heads, kh = h / group, block = (h - kh * group) / p.cols,
               col = h - kh * group - block * p.cols, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    T *out = (T *)a.out + (int64_t)blockIdx.x * dim;
-    const int n = __ldcg(a.lengths + b), tiles = tiles_of(n, p.most_tiles);
-    if (tiles == 0) {
-        for (int d = threadIdx.x; d < dim; d += 128) out[d] = from_f32<T>(n > 0 ? NAN : 0.0f);
+    T *out = (T *)a.out + (int64_t)blockIdx.x * DIM;
+    const int n = __ldcg(a.lengths + b), weight = weight_of(p, b);
+    if (weight == 0) {
+        for (int d = threadIdx.x; d < DIM; d += 128) out[d] = from_f32<T>(n > 0 ? NAN : 0.0f);
         return;
     }
     int64_t total = 0, before = 0;
     for (int64_t i = lane; i < p.batch; i += 32) {
-        const int64_t t = tiles_of(__ldcg(a.lengths + i), p.most_tiles);
-        total += t;
-        before += i < b ? t : 0;
+        const int w = weight_of(p, i);
+        total += w;
+        before += i < b ? w : 0;
     }
     for (int d = 16; d; d >>= 1) {
         total += __shfl_xor_sync(0xffffffffu, total, d);
         before += __shfl_xor_sync(0xffffffffu, before, d);
     }
-    const int64_t per = share(p, total * p.units), from = before * p.units + (int64_t)(kh * p.blocks + block) * tiles;
-    const int64_t first = from / per, last = (from + tiles - 1) / per;
-    if (first == last) return;
-    const int64_t stride = (int64_t)2 * p.cols * (dim + 2);       // of CTAs; the first one's part is in its second slot
-    const float *parts = p.slots + (int64_t)col * (dim + 2);
-    const float *head = parts + first * stride + stride / 2;
-    __shared__ float s_o[4][256], s_l[4];
-    // each warp: every fourth part
+    const int64_t per = share(p, total * p.units), from = before * p.units + (int64_t)(kh * p.blocks + block) * weight + START;
+    const int first = (int)(from / per), last = (int)((from + weight - START - 1) / per), parts = last - first + 1;
+    if (parts == 1) return;
+    const int64_t size = (int64_t)p.cols * (DIM + 2);             // of a slot; the first CTA's part is in its second one, the others' in their first
+    auto slot = [&](int i) { return p.slots + (2 * (int64_t)(first + i) + (i == 0)) * size; };
+    __shared__ float s_f[MOST_CTAS], s_part[4], s_o[4][DIM];
+    // factors of the parts: 2^(m - largest m)
     float top = -INFINITY;
-    for (int64_t i = first + lane; i <= last; i += 32) top = fmaxf(top, __ldcg((i == first ? head : parts + i * stride) + dim));
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float o[8] = {}, l = 0.0f;
-#pragma unroll 4
-    for (int64_t i = first + warp; i <= last; i += 4) {
-        const float *s = i == first ? head : parts + i * stride;
-        const float m = __ldcg(s + dim), sum = __ldcg(s + dim + 1), f = m == -INFINITY ? 0.0f : ex2(m - top);
-        l += sum == sum ? f * sum : NAN;
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (lane + 32 * k < dim) o[k] += f * __ldcg(s + lane + 32 * k);
+    for (int i = threadIdx.x; i < parts; i += 128) {
+        s_f[i] = __ldcg(slot(i) + p.cols * DIM + 2 * col);
+        top = fmaxf(top, s_f[i]);
     }
-    if (lane == 0) s_l[warp] = l;
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-        if (lane + 32 * k < dim) s_o[warp][lane + 32 * k] = o[k];
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (lane == 0) s_part[warp] = top;
     __syncthreads();
-    for (int d = threadIdx.x; d < dim; d += 128)
-        out[d] = from_f32<T>((s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) / (s_l[0] + s_l[1] + s_l[2] + s_l[3]));
+    top = fmaxf(fmaxf(s_part[0], s_part[1]), fmaxf(s_part[2], s_part[3]));
+    float l = 0.0f;
+    for (int i = threadIdx.x; i < parts; i += 128) {
+        const float f = s_f[i] == -INFINITY ? 0.0f : ex2(s_f[i] - top), sum = __ldcg(slot(i) + p.cols * DIM + 2 * col + 1);
+        s_f[i] = f;
+        l += sum == sum ? f * sum : NAN;
+    }
+    for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    __syncthreads();
+    if (lane == 0) s_part[warp] = l;
+    // a warp takes every fourth part
+    constexpr int V = DIM / 32;
+    float o[V] = {};
+#pragma unroll 4
+    for (int i = warp; i < parts; i += 4) {
+        const float f = s_f[i], *from = slot(i) + (int64_t)col * DIM + lane;
+#pragma unroll
+        for (int k = 0; k < V; ++k) o[k] += f * __ldcg(from + 32 * k);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) s_o[warp][lane + 32 * k] = o[k];
+    __syncthreads();
+    for (int d = threadIdx.x; d < DIM; d += 128)
+        out[d] = from_f32<T>((s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) / (s_part[0] + s_part[1] + s_part[2] + s_part[3]));
 }
 
 // Whether the tiled kernel takes this cache, and how it divides a call.
 bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages) {
-    if ((dim != 64 && dim != 128 && dim != 256) || page_size % TILE != 0) return false;
+    if ((dim != 64 && dim != 128 && dim != 256) || page_size % TILE != 0 || (int64_t)kv_heads * page_size > INT32_MAX) return false;
     const int group = heads / kv_heads;
     p.batch = batch;
     p.cols = group > 8 && dim < 256 ? 16 : 8;
@@ -639,21 +699,28 @@ bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int
     p.units = kv_heads * p.blocks;
     p.tiles_per_page = page_size / TILE;
     p.most_tiles = (int)(max_pages * p.tiles_per_page);
+    p.pair = group <= 4 && dim < 256 ? 2 : 1;      // (of 256 values of 8 bits two tiles would be 16 KB a step)
     p.single = p.most_tiles <= SINGLE_TILES;
     return batch * p.units < (int64_t)1 << 31;
 }
 
-template <typename T, int BITS, int DIM, int NB, int REST>
+template <typename T, int BITS, int DIM, int NB, int PAIR>
 int launch_fast(FastArgs &p, cudaStream_t st) {
-    static int per_sm = 0;
-    if (!per_sm) {
-        int n = 0;
-        BW_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kv_attend_kernel<T, BITS, DIM, NB, REST>, 32 * WARPS, 0));
-        per_sm = n < 1 ? 1 : n > 4 ? 4 : n;
+    auto kern = kv_attend_kernel<T, BITS, DIM, NB, PAIR>;
+    constexpr int SMEM = Config<T, BITS, DIM, NB, PAIR>::SMEM;
+    static std::atomic<int> per_sm[64];                     // by device
+    int device = 0;
+    BW_CUDA_TRY(cudaGetDevice(&device));
+    int n = device < 64 ? per_sm[device].load() : 0;
+    if (!n) {
+        BW_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+        BW_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, 32 * WARPS, SMEM));
+        n = n < 1 ? 1 : n > 4 ? 4 : n;
+        if (device < 64) per_sm[device] = n;
     }
-    p.ctas = 148 * per_sm;
+    p.ctas = 148 * n;
     const int64_t grid = p.single ? p.batch * p.units : p.ctas;
-    kv_attend_kernel<T, BITS, DIM, NB, REST><<<(unsigned)grid, 32 * WARPS, 0, st>>>(p);
+    kern<<<(unsigned)grid, 32 * WARPS, SMEM, st>>>(p);
     int rc = check_launch("kv_attend_kernel");
     if (rc != BW_OK || p.single) return rc;
     cudaLaunchConfig_t cfg = {};
@@ -665,24 +732,23 @@ int launch_fast(FastArgs &p, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T>, p, DIM));
+    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T, DIM>, p));
     return BW_OK;
 }
 
 template <typename T, int BITS, int DIM>
-int launch_rest(FastArgs &p, cudaStream_t st) {
-    constexpr bool EXACT = __is_same(T, __half);
-    if constexpr (DIM < 256)
-        if (p.cols == 16) return launch_fast<T, BITS, DIM, 2, EXACT ? 2 : 0>(p, st);
-    if constexpr (EXACT)
-        if (p.a.heads / p.a.kv_heads <= 4) return launch_fast<T, BITS, DIM, 1, 1>(p, st);
-    return launch_fast<T, BITS, DIM, 1, EXACT ? 2 : 0>(p, st);
+int launch_group(FastArgs &p, cudaStream_t st) {
+    if constexpr (DIM < 256) {
+        if (p.cols == 16) return launch_fast<T, BITS, DIM, 2, 1>(p, st);
+        if (p.pair == 2) return launch_fast<T, BITS, DIM, 1, 2>(p, st);
+    }
+    return launch_fast<T, BITS, DIM, 1, 1>(p, st);
 }
 template <typename T, int BITS>
 int launch_dim(FastArgs &p, cudaStream_t st) {
-    if (p.a.dim == 64) return launch_rest<T, BITS, 64>(p, st);
-    if (p.a.dim == 128) return launch_rest<T, BITS, 128>(p, st);
-    return launch_rest<T, BITS, 256>(p, st);
+    if (p.a.dim == 64) return launch_group<T, BITS, 64>(p, st);
+    if (p.a.dim == 128) return launch_group<T, BITS, 128>(p, st);
+    return launch_group<T, BITS, 256>(p, st);
 }
 template <typename T>
 int launch_bits(FastArgs &p, int bits, cudaStream_t st) {
