@@ -9,6 +9,8 @@
 //
 // Layout: codes [pages][heads][page_size][D * bits / 32] words, packed like weights; constants [pages][heads][page_size][4]
 // fp16: (scale, zero) of the key, then of the value: what an attention step needs of one token lies in 8 bytes.
+#include <type_traits>
+
 #include "bw_common.cuh"
 
 namespace bw {
@@ -18,92 +20,191 @@ struct KvRows {
     int64_t tokens, slots;      // rows of tokens in the call; pages * page_size
     int64_t stride[2], head_stride[2];   // of k and v, in elements
     int heads, dim, words, page_size;
-    int lanes;                  // of a row: the power of two that holds its words, at most 32
+    int lanes;                  // of a row: the power of two that holds its pieces
 };
 
 // Where a slot's row of a head lies, in rows of the cache.
 __device__ __forceinline__ int64_t cache_row(const KvRows &p, int64_t slot, int head) {
-    const int64_t page = slot / p.page_size;
+    const int64_t page = slot >> 32 ? slot / p.page_size : (int64_t)((uint32_t)slot / (uint32_t)p.page_size);
     return (page * p.heads + head) * p.page_size + (slot - page * p.page_size);
 }
 
 // fp16 not below s (finite, positive), at least 2^-24; infinity beyond fp16's range.
 __device__ __forceinline__ __half scale_up(float s) { return __float2half_ru(fmaxf(s, 0x1p-24f)); }
 
-// One group of lanes a row; a lane holds whole words, so that it packs them by itself.
-template <typename T, int BITS>
-__global__ void __launch_bounds__(256) kv_append_kernel(const T *__restrict__ k, const T *__restrict__ v, const int64_t *__restrict__ slots,
-                                                        KvRows p, int32_t *k_codes, int32_t *v_codes, __half2 *params) {
-    constexpr int VPI = 32 / BITS, WORDS = BITS == 8 ? 2 : 1;      // words a lane: 256 values of 8 bits are 64 words
-    constexpr float Q = (1 << BITS) - 1;
-    const int64_t row = (int64_t)blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes;
-    const int lane = threadIdx.x % p.lanes;
-    const bool is_v = blockIdx.y;
-    const int64_t token = row / p.heads;
-    const int head = (int)(row - token * p.heads);
-    const int64_t slot = token < p.tokens ? slots[token] : -1;
-    const bool live = slot >= 0 && slot < p.slots;
-    const T *src = (is_v ? v : k) + (live ? token * p.stride[is_v] + head * p.head_stride[is_v] : 0);
+constexpr float MAGIC = 12582912.0f;                         // 1.5 * 2^23: the sum of 0 <= t <= 255 and this has rint(t) in its low bits
+constexpr uint32_t MAGIC_BITS = 0x4B400000u;
 
-    float x[WORDS][VPI], lo = 0.0f, hi = 0.0f;
-    bool fine = true;
-#pragma unroll
-    for (int w = 0; w < WORDS; ++w) {
-        const int at = (lane + w * p.lanes) * VPI;
-#pragma unroll
-        for (int i = 0; i < VPI; ++i) {
-            x[w][i] = live && at < p.dim ? to_f32(src[at + i]) : 0.0f;
-            lo = fminf(lo, x[w][i]);
-            hi = fmaxf(hi, x[w][i]);
-            fine &= isfinite(x[w][i]);
-        }
-    }
-    for (int d = p.lanes / 2; d; d >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-        fine &= (bool)__shfl_xor_sync(0xffffffffu, (int)fine, d);
-    }
-    const __half scale = scale_up(__fdiv_rn(__fsub_rn(hi, lo), Q));
-    fine &= !__hisinf(scale);
-    const float s = __half2float(scale), z = fminf(rintf(__fdiv_rn(-lo, s)), Q);
-    if (!live) return;
-    const int64_t at = cache_row(p, slot, head);
-    int32_t *dst = (is_v ? v_codes : k_codes) + at * p.words;
-#pragma unroll
-    for (int w = 0; w < WORDS; ++w) {
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < VPI; ++i) {
-            const float c = fminf(fmaxf(rintf(__fadd_rn(__fdiv_rn(x[w][i], s), z)), 0.0f), Q);
-            word |= (fine ? (uint32_t)c : 0u) << (i * BITS);
-        }
-        if (lane + w * p.lanes < p.words) dst[lane + w * p.lanes] = (int32_t)word;
-    }
-    if (lane == 0) params[2 * at + is_v] = fine ? __halves2half2(scale, __float2half_rn(z)) : __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0));
+// Values that a thread takes of a row: whole words of codes at any width.  (Of 8 the work on a row's ends, scale and place was most of it.)
+constexpr int E = 16;
+
+// min and max that keep NaN
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
 }
 
-template <typename T, int BITS>
+// E values of a row at `at` (fewer than E are left only at the end of a row that is no multiple of E: zeros), and their ends together with 0:
+// of 16-bit values in pairs.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_values(const T *row, int at, int dim, bool live, float (&x)[E], float &lo, float &hi) {
+    lo = hi = 0.0f;
+    if constexpr (VEC) {
+        uint4 raw[E * sizeof(T) / 16];
+#pragma unroll
+        for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) raw[i] = live ? __ldcs(reinterpret_cast<const uint4 *>(row + at) + i) : make_uint4(0, 0, 0, 0);
+        const T *v = reinterpret_cast<const T *>(raw);
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = to_f32(v[i]);
+        if constexpr (sizeof(T) == 2) {
+            using T2 = typename std::conditional<__is_same(T, __half), __half2, __nv_bfloat162>::type;
+            const T2 *p = reinterpret_cast<const T2 *>(raw);
+            T2 a = p[0], b = p[0];
+#pragma unroll
+            for (int i = 1; i < E / 2; ++i) {
+                a = __hmin2_nan(a, p[i]);
+                b = __hmax2_nan(b, p[i]);
+            }
+            lo = min_nan(0.0f, min_nan(to_f32(a.x), to_f32(a.y)));
+            hi = max_nan(0.0f, max_nan(to_f32(b.x), to_f32(b.y)));
+            return;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = live && at + i < dim ? to_f32(row[at + i]) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        lo = min_nan(lo, x[i]);
+        hi = max_nan(hi, x[i]);
+    }
+}
+
+// One group of lanes a row, each with whole words of codes; a thread has its piece of the key and of the value.  Bound by the bytes: 16384 tokens
+// of 8 heads of 128, fp16 to 8 bits, 29 us (the division in four FMAs and the packed adds of rtn_quantize.cu; one element a
+// load and a hardware division each: 174 us).
+template <typename T, int BITS, bool VEC>
+__global__ void __launch_bounds__(256) kv_append_kernel(const T *__restrict__ k, const T *__restrict__ v, const int64_t *__restrict__ slots,
+                                                        const KvRows p, int32_t *k_codes, int32_t *v_codes, __half2 *params) {
+    constexpr int WORDS = E * BITS / 32, VPI = 32 / BITS;
+    constexpr float Q = (1 << BITS) - 1, RQ = 1.0f / Q;
+    const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = row / (uint32_t)p.heads;
+    const int head = (int)(row - token * (uint32_t)p.heads), lane = threadIdx.x % p.lanes, at = lane * E;
+    const int64_t slot = token < p.tokens ? __ldg(slots + token) : -1;
+    const bool in = slot >= 0 && slot < p.slots, live = in && at < p.dim;
+    float x[2][E], lo[2], hi[2];
+    load_values<T, VEC>(k + (in ? token * p.stride[0] + head * p.head_stride[0] : 0), at, p.dim, live, x[0], lo[0], hi[0]);
+    load_values<T, VEC>(v + (in ? token * p.stride[1] + head * p.head_stride[1] : 0), at, p.dim, live, x[1], lo[1], hi[1]);
+    for (int d = p.lanes / 2; d; d >>= 1)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            lo[j] = min_nan(lo[j], __shfl_xor_sync(0xffffffffu, lo[j], d));
+            hi[j] = max_nan(hi[j], __shfl_xor_sync(0xffffffffu, hi[j], d));
+        }
+    if (!live) return;
+    const int64_t to = cache_row(p, slot, head);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        // (a NaN or an infinity in the row, and what leaves fp16's range, fails the comparison)
+        const float span = div_by_recip(__fsub_rn(hi[j], lo[j]), Q, RQ);
+        const bool ok = span <= 65504.0f;
+        const __half scale = scale_up(span);
+        const float s = __half2float(scale), r = __frcp_rn(s), z = rintf(div_by_recip(-lo[j], s, r));      // (at most Q: scale * Q >= hi - lo >= -lo)
+        uint32_t words[WORDS] = {};
+        if (ok) {
+            float c[E];
+#pragma unroll
+            for (int i = 0; i < E; i += 2) {
+                // x / s + z >= -1/2, which is 0 rounded: only the upper end has to be clamped
+                const float2 t = fadd2(div_by_recip2(make_float2(x[j][i], x[j][i + 1]), s, r), make_float2(z, z));
+                const float2 y = fadd2(make_float2(fminf(t.x, Q), fminf(t.y, Q)), make_float2(MAGIC, MAGIC));
+                c[i] = y.x;
+                c[i + 1] = y.y;
+            }
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w) {
+                // one shift and add a code; what the magic number adds on the way is a constant
+                uint32_t word = 0, extra = 0;
+#pragma unroll
+                for (int i = VPI - 1; i >= 0; --i) {
+                    word = (word << BITS) + __float_as_uint(c[w * VPI + i]);
+                    extra = (extra << BITS) + MAGIC_BITS;
+                }
+                words[w] = word - extra;
+            }
+        }
+        int32_t *dst = (j ? v_codes : k_codes) + to * p.words + lane * WORDS;
+        if constexpr (VEC && WORDS == 4) *reinterpret_cast<int4 *>(dst) = make_int4((int)words[0], (int)words[1], (int)words[2], (int)words[3]);
+        else if constexpr (VEC && WORDS == 2) *reinterpret_cast<int2 *>(dst) = make_int2((int)words[0], (int)words[1]);
+        else {
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w)
+                if (lane * WORDS + w < p.words) dst[w] = (int32_t)words[w];
+        }
+        if (lane == 0) params[2 * to + j] = ok ? __halves2half2(scale, __float2half_rn(z)) : __halves2half2(__ushort_as_half(0x7fff), __ushort_as_half(0));
+    }
+}
+
+// E values of a row: code + 2^23 by one OR, minus 2^23 + zero, both exact; times the scale, exact as well (19 bits); then the result's rounding.
+template <typename T, int BITS, bool VEC>
+__device__ __forceinline__ void read_piece(const int32_t *codes, uint32_t constants, int lane, int words, int dim, T *dst) {
+    constexpr int WORDS = E * BITS / 32, VPI = 32 / BITS;
+    const float2 c = __half22float2(*reinterpret_cast<const __half2 *>(&constants));
+    const float zero = 8388608.0f + c.y;
+    uint32_t w[WORDS] = {};
+    if constexpr (WORDS == 4 && VEC) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(codes) + lane);
+        w[0] = u.x;
+        w[1] = u.y;
+        w[2] = u.z;
+        w[3] = u.w;
+    } else if constexpr (WORDS == 2 && VEC) {
+        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(codes) + lane);
+        w[0] = u.x;
+        w[1] = u.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[i] = lane * WORDS + i < words ? (uint32_t)__ldg(codes + lane * WORDS + i) : 0u;
+    }
+    __align__(16) T out[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const uint32_t code = w[i / VPI] >> (i % VPI * BITS) & ((1u << BITS) - 1);
+        out[i] = from_f32<T>(c.x * (__uint_as_float(0x4B000000u | code) - zero));
+    }
+    if constexpr (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) __stcs(reinterpret_cast<uint4 *>(dst) + i, reinterpret_cast<const uint4 *>(out)[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (lane * E + i < dim) dst[i] = out[i];
+    }
+}
+
+template <typename T, int BITS, bool VEC>
 __global__ void __launch_bounds__(256) kv_read_kernel(const int32_t *__restrict__ k_codes, const int32_t *__restrict__ v_codes,
-                                                      const __half2 *__restrict__ params, const int64_t *__restrict__ slots, KvRows p, T *k, T *v) {
-    constexpr int VPI = 32 / BITS;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;       // a word of the output, both tensors' rows dense
-    const int64_t row = i / p.words;
-    const int word = (int)(i - row * p.words);
-    const bool is_v = blockIdx.y;
-    const int64_t token = row / p.heads;
-    if (token >= p.tokens) return;
-    const int64_t slot = slots[token];
-    T *dst = (is_v ? v : k) + row * p.dim + word * VPI;
+                                                      const uint2 *__restrict__ params, const int64_t *__restrict__ slots, const KvRows p, T *k, T *v) {
+    const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = row / (uint32_t)p.heads;
+    const int lane = threadIdx.x % p.lanes;
+    if (token >= p.tokens || lane * E >= p.dim) return;
+    const int64_t slot = __ldg(slots + token), to = (int64_t)row * p.dim + lane * E;
     if (slot < 0 || slot >= p.slots) {
 #pragma unroll
-        for (int j = 0; j < VPI; ++j) dst[j] = from_f32<T>(0.0f);
+        for (int i = 0; i < E; ++i)
+            if (lane * E + i < p.dim) k[to + i] = v[to + i] = from_f32<T>(0.0f);
         return;
     }
-    const int64_t at = cache_row(p, slot, (int)(row - token * p.heads));
-    const uint32_t w = (uint32_t)(is_v ? v_codes : k_codes)[at * p.words + word];
-    const float2 c = __half22float2(params[2 * at + is_v]);
-#pragma unroll
-    for (int j = 0; j < VPI; ++j) dst[j] = from_f32<T>(c.x * ((float)((w >> (j * BITS)) & ((1u << BITS) - 1)) - c.y));
+    const int64_t at = cache_row(p, slot, (int)(row - token * (uint32_t)p.heads));
+    const uint2 c = __ldg(params + at);
+    read_piece<T, BITS, VEC>(k_codes + at * p.words, c.x, lane, p.words, p.dim, k + to);
+    read_piece<T, BITS, VEC>(v_codes + at * p.words, c.y, lane, p.words, p.dim, v + to);
 }
 
 KvRows kv_rows(int64_t tokens, int heads, int dim, int bits, int64_t pages, int page_size) {
@@ -114,28 +215,44 @@ KvRows kv_rows(int64_t tokens, int heads, int dim, int bits, int64_t pages, int 
     p.dim = dim;
     p.words = dim * bits / 32;
     p.page_size = page_size;
+    const int pieces = (dim + E - 1) / E;
     p.lanes = 1;
-    while (p.lanes < p.words && p.lanes < 32) p.lanes *= 2;
+    while (p.lanes < pieces) p.lanes *= 2;
     return p;
 }
 
-template <typename T>
-int append_bits(const void *k, const void *v, const int64_t *slots, const KvRows &p, int bits, int32_t *kc, int32_t *vc, void *params, cudaStream_t st) {
-    const int64_t rows = p.tokens * p.heads, per = 256 / p.lanes;
-    const dim3 grid((unsigned)((rows + per - 1) / per), 2);
-    if (bits == 2) kv_append_kernel<T, 2><<<grid, 256, 0, st>>>((const T *)k, (const T *)v, slots, p, kc, vc, (__half2 *)params);
-    else if (bits == 4) kv_append_kernel<T, 4><<<grid, 256, 0, st>>>((const T *)k, (const T *)v, slots, p, kc, vc, (__half2 *)params);
-    else kv_append_kernel<T, 8><<<grid, 256, 0, st>>>((const T *)k, (const T *)v, slots, p, kc, vc, (__half2 *)params);
-    return check_launch("kv_append_kernel");
+unsigned kv_grid(const KvRows &p) {
+    const int64_t per = 256 / p.lanes;
+    return (unsigned)((p.tokens * p.heads + per - 1) / per);
 }
 
+template <typename T, int BITS>
+int append_typed(const void *kv, const void *vv, const int64_t *slots, const KvRows &p, int32_t *kc, int32_t *vc, void *params, cudaStream_t st) {
+    const T *k = (const T *)kv, *v = (const T *)vv;
+    constexpr int V = 16 / sizeof(T);
+    bool vec = p.dim % E == 0 && aligned_to(k, 16) && aligned_to(v, 16);
+    for (int i = 0; i < 2; ++i) vec = vec && p.stride[i] % V == 0 && p.head_stride[i] % V == 0;
+    if (vec) kv_append_kernel<T, BITS, true><<<kv_grid(p), 256, 0, st>>>(k, v, slots, p, kc, vc, (__half2 *)params);
+    else kv_append_kernel<T, BITS, false><<<kv_grid(p), 256, 0, st>>>(k, v, slots, p, kc, vc, (__half2 *)params);
+    return check_launch("kv_append_kernel");
+}
+template <typename T>
+int append_bits(const void *k, const void *v, const int64_t *slots, const KvRows &p, int bits, int32_t *kc, int32_t *vc, void *params, cudaStream_t st) {
+    return bits == 2 ? append_typed<T, 2>(k, v, slots, p, kc, vc, params, st) : bits == 4 ? append_typed<T, 4>(k, v, slots, p, kc, vc, params, st)
+                                                                                          : append_typed<T, 8>(k, v, slots, p, kc, vc, params, st);
+}
+
+template <typename T, int BITS>
+int read_typed(const int32_t *kc, const int32_t *vc, const void *params, const int64_t *slots, const KvRows &p, void *k, void *v, cudaStream_t st) {
+    // (k and v are dense and start on 16 bytes: so do all pieces of rows that are whole pieces)
+    if (p.dim % E == 0) kv_read_kernel<T, BITS, true><<<kv_grid(p), 256, 0, st>>>(kc, vc, (const uint2 *)params, slots, p, (T *)k, (T *)v);
+    else kv_read_kernel<T, BITS, false><<<kv_grid(p), 256, 0, st>>>(kc, vc, (const uint2 *)params, slots, p, (T *)k, (T *)v);
+    return check_launch("kv_read_kernel");
+}
 template <typename T>
 int read_bits(const int32_t *kc, const int32_t *vc, const void *params, const int64_t *slots, const KvRows &p, int bits, void *k, void *v, cudaStream_t st) {
-    const dim3 grid((unsigned)((p.tokens * p.heads * p.words + 255) / 256), 2);
-    if (bits == 2) kv_read_kernel<T, 2><<<grid, 256, 0, st>>>(kc, vc, (const __half2 *)params, slots, p, (T *)k, (T *)v);
-    else if (bits == 4) kv_read_kernel<T, 4><<<grid, 256, 0, st>>>(kc, vc, (const __half2 *)params, slots, p, (T *)k, (T *)v);
-    else kv_read_kernel<T, 8><<<grid, 256, 0, st>>>(kc, vc, (const __half2 *)params, slots, p, (T *)k, (T *)v);
-    return check_launch("kv_read_kernel");
+    return bits == 2 ? read_typed<T, 2>(kc, vc, params, slots, p, k, v, st) : bits == 4 ? read_typed<T, 4>(kc, vc, params, slots, p, k, v, st)
+                                                                                      : read_typed<T, 8>(kc, vc, params, slots, p, k, v, st);
 }
 
 }  // namespace

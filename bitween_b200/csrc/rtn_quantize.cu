@@ -139,59 +139,12 @@ __device__ __forceinline__ uint32_t code_of(float v, float s, float zf, float qm
 //
 // Per-element arithmetic on the common path (finite weights, scale within 2^-40..2^40):
 //   * w/scale: the correctly rounded fp32 quotient torch computes, obtained from one
-//     correctly rounded reciprocal per group and four FMAs per element (div_by_recip).
+//     correctly rounded reciprocal per group and four FMAs per element (div_by_recip, bw_common.cuh).
 //   * round-half-even + clamp + int conversion: clamp(rint(t),0,Q) == rint(clamp(t,0,Q)), and
 //     for 0 <= t <= 255 the sum t + 1.5*2^23 is rounded to an integer by the fp32 adder itself
 //     (half-to-even), leaving the code in the low mantissa bits.
 // Groups with a NaN/Inf weight or an out-of-range scale take the step-by-step path below,
 // which mirrors torch's NaN/Inf propagation (bitween/functional.py:25-29 on such inputs).
-// Correctly rounded fp32 quotient v/s from the correctly rounded reciprocal r = RN(1/s)
-// (one __frcp_rn per group) with fused multiply-adds only:
-//   q0 = RN(v*r)                      within 1.5 ulp of v/s
-//   q1 = RN(q0 + RN(v - s*q0) * r)    a faithful rounding (error <= 1/2 ulp + 2^-22 ulp)
-//   q2 = RN(q1 + (v - s*q1) * r)      the residual of a faithful quotient is exact, and
-//                                     Markstein's theorem (correction of a faithful quotient
-//                                     with the correctly rounded reciprocal) gives RN(v/s)
-// Valid for normal operands without over/underflow: the caller guarantees |v| <= 2^40 and
-// 2^-40 <= s <= 2^40.  For |v| < 2^-79 the residual may underflow, but then |v/s| < 2^-39 and
-// the code does not depend on the quotient's low bits (adding the integer zero-point absorbs
-// it).  tests/test_gpu_parity.py compares this against __fdiv_rn on 2^28 operand pairs.
-__device__ __forceinline__ float div_by_recip(float v, float s, float r) {
-    const float q0 = __fmul_rn(v, r);
-    const float q1 = __fmaf_rn(__fmaf_rn(-s, q0, v), r, q0);
-    return __fmaf_rn(__fmaf_rn(-s, q1, v), r, q1);
-}
-
-// The same division for two elements at a time with the packed fp32 instructions of sm_100
-// (fma.rn.f32x2 / mul.rn.f32x2 / add.rn.f32x2: each lane of the pair is an IEEE operation with
-// round-to-nearest-even, so the sequence above stays exact; one issue slot instead of two).
-__device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n .reg .b64 ra, rb, rc, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n mov.b64 rc, {%6, %7};\n"
-        " fma.rn.f32x2 rd, ra, rb, rc;\n mov.b64 {%0, %1}, rd;\n}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n"
-        " mul.rn.f32x2 rd, ra, rb;\n mov.b64 {%0, %1}, rd;\n}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 fadd2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n .reg .b64 ra, rb, rd;\n mov.b64 ra, {%2, %3};\n mov.b64 rb, {%4, %5};\n"
-        " add.rn.f32x2 rd, ra, rb;\n mov.b64 {%0, %1}, rd;\n}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ float2 div_by_recip2(float2 v, float s, float r) {
-    const float2 s2 = make_float2(-s, -s), r2 = make_float2(r, r);
-    const float2 q0 = fmul2(v, r2);
-    const float2 q1 = ffma2(ffma2(s2, q0, v), r2, q0);
-    return ffma2(ffma2(s2, q1, v), r2, q1);
-}
 
 // One 16-byte chunk per lane: group min/max over the lane segment, group parameters, codes,
 // packed words and the group's scale / zero-point.  `c` is the global chunk index of this lane.
