@@ -11,6 +11,12 @@ from .modules import QuantizedLinear, QuantizedLinearFunction
 _DTYPES = (torch.float16, torch.bfloat16)
 
 
+def _aligned(t):
+    """`t` contiguous and on a 16-byte boundary."""
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _forward(x, down, up, index, scaling, base, out, keep):
     """(out [M, N], hidden): `hidden` is what the backward pass needs again, or None."""
     M, K = x.shape
@@ -20,7 +26,7 @@ def _forward(x, down, up, index, scaling, base, out, keep):
         out = torch.empty((M, N), dtype=x.dtype, device=dev)
     L = _lib.lib()
     with _lib.on_device(dev):
-        need = L.bw_adapter_hidden_bytes(M, K, adapters, rank)
+        need = L.bw_adapter_hidden_bytes(M, rank)
         hidden = torch.empty(need, dtype=torch.uint8, device=dev) if keep else _lib.workspace(dev, need)
         rc = L.bw_adapter_forward(x.data_ptr(), _lib.dtype_code(x.dtype), M, N, K, down.data_ptr(), up.data_ptr(), adapters, rank, index.data_ptr(),
                                   None if scaling is None else scaling.data_ptr(), None if base is None else base.data_ptr(), out.data_ptr(),
@@ -48,10 +54,10 @@ class AdapterFunction(torch.autograd.Function):
             M, K = x.shape
             adapters, rank, N = up.shape
             dev = x.device
-            g = grad_out.contiguous()
+            g = _aligned(grad_out)
             L = _lib.lib()
             with _lib.on_device(dev):
-                ws = _lib.workspace(dev, L.bw_adapter_backward_bytes(M, N, K, adapters, rank))
+                ws = _lib.workspace(dev, L.bw_adapter_hidden_bytes(M, rank))
                 rc = L.bw_adapter_backward(g.data_ptr(), _lib.dtype_code(x.dtype), x.data_ptr(), M, N, K, down.data_ptr(), up.data_ptr(), adapters, rank,
                                            index.data_ptr(), None if scaling is None else scaling.data_ptr(),
                                            None if hidden is None else hidden.data_ptr(), 0 if hidden is None else hidden.numel(),
@@ -104,14 +110,16 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
     index = index.reshape(-1).contiguous()
     if scaling is not None:
         scaling = scaling.contiguous()
-    base2 = None if base is None else base.reshape(M, N).contiguous()
-    args = (x2.contiguous(), down.contiguous(), up.contiguous(), index, scaling, base2)
+    base2 = None if base is None else _aligned(base.reshape(M, N))
+    args = (_aligned(x2), _aligned(down), _aligned(up), index, scaling, base2)
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, base))
     if out is not None:
         if grad:
             raise ValueError("`out` is for calls that record no gradient")
         if out.shape != (*lead, N) or not out.is_contiguous():
             raise ValueError(f"`out` must be contiguous {(*lead, N)}")
+        if out.data_ptr() % 16 != 0:
+            return out.copy_(_forward(*args, None, False)[0].view(*lead, N))
         for i in (0, 1, 2, 5):      # kernels store outputs while others still read
             t = args[i]
             if t is not None and t.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < t.data_ptr() + t.nbytes and \

@@ -6,17 +6,18 @@
 // Both matrices of an adapter are stored rank-major, down [n][rank][K] and up [n][rank][N], so that forward and backward are the
 // same three passes: "shrink" (rows times a matrix of long rows -> rank values), "expand" (the reverse) and "outer" (sums of
 // products over an adapter's tokens).  All three are bound by the bytes of x, base, y and their gradients; the products run on
-// mma.sync.m16n8k16, whose fragments come straight from 16-byte loads:
-//   * the reduced index of a product may be permuted at will, if both operands are: where rows are long in it (shrink), a lane's 16 bytes
-//     of a row serve two MMAs, k pairs (0, 1), (2, 3) and (4, 5), (6, 7);
+// mma.sync.m16n8k16, whose fragments come from 16-byte loads:
+//   * the reduced index of a product may be permuted at will, if both operands are: where rows are long in it (shrink of a few tokens), a
+//     lane's 16 bytes of a row serve two MMAs, k pairs (0, 1), (2, 3) and (4, 5), (6, 7);
 //   * where it runs over rows (expand over ranks, outer over tokens), a lane takes 16 bytes of four rows, eight columns of its own, and
 //     pairs the rows by byte permutations: MMA j of eight has column j of every lane.  A lane's results are then 16 neighbours of a row.
-// Rank values stay in 32 bits between the passes and enter the second product as two 16-bit parts (value and rest), which keeps 16 (bf16) or 22
-// (fp16) of their bits.  fp16 parts are taken of h * 2^-e, e of the row's largest (expand) or of the largest so far (outer): gradients
-// without loss scaling would be lost below 2^-14, and large rank values beyond 65504.
+// Rank values are summed in 32 bits and kept as two 16-bit parts (value and rest), which hold 16 (bf16) or 22 (fp16) of their bits and are
+// what the second product takes.  fp16 parts are of h * 2^-e, e of the row's largest: gradients without loss scaling would be lost below
+// 2^-14, and large rank values beyond 65504.
 //
-// Tokens of one adapter need not be neighbours: a tile of tokens goes through the adapters that occur in it, one after the other or (a few
-// tokens, many adapters) a CTA each; outer gathers the tokens of its adapter first.  Rows of other adapters enter no product.
+// Tokens of one adapter need not be neighbours: a tile of 64 tokens goes through the adapters that occur in it, one after the other or (few
+// tokens, many adapters) a CTA each, with the rows of each gathered; outer gathers the tokens of its adapter from all.  Rows of other
+// adapters enter no product.
 #include <cooperative_groups.h>
 
 #include "bw_common.cuh"
@@ -25,16 +26,9 @@ namespace bw {
 namespace {
 
 // ---- any sizes and alignments -------------------------------------------------------------------------------------------
-// Rank values may be in parts (splits of their sums): the tensor-core forms write them so, and either form may read them.
-__device__ __forceinline__ float rank_value(const float *h, int64_t part, int64_t i, int parts) {
-    float s = h[i];
-    for (int k = 1; k < parts; ++k) s += h[k * part + i];
-    return s;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(128) adapter_shrink_general_kernel(const T *__restrict__ x, int64_t M, int64_t K, const T *__restrict__ w, int n, int r,
-                                                                     const int32_t *__restrict__ index, float *h, int parts) {
+                                                                     const int32_t *__restrict__ index, float *h) {
     const int64_t i = (int64_t)blockIdx.x * 4 + threadIdx.x / 32, t = i / r;
     const int j = (int)(i - t * r), lane = threadIdx.x % 32;
     if (t >= M) return;
@@ -43,20 +37,19 @@ __global__ void __launch_bounds__(128) adapter_shrink_general_kernel(const T *__
     if (a >= 0 && a < n)
         for (int64_t k = lane; k < K; k += 32) s += to_f32(x[t * K + k]) * to_f32(w[((int64_t)a * r + j) * K + k]);
     for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    if (lane == 0)
-        for (int k = 0; k < parts; ++k) h[k * M * r + i] = k ? 0.0f : s;
+    if (lane == 0) h[i] = s;
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) adapter_expand_general_kernel(const float *__restrict__ h, int64_t M, int64_t N, const T *__restrict__ w, int n, int r,
-                                                                     const int32_t *__restrict__ index, const float *__restrict__ scaling, const T *base, T *out, int parts) {
+                                                                     const int32_t *__restrict__ index, const float *__restrict__ scaling, const T *base, T *out) {
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= N) return;
     for (int64_t t = blockIdx.y; t < M; t += gridDim.y) {
         const int a = index[t];
         float s = a < n ? 0.0f : NAN;
         if (a >= 0 && a < n) {
-            for (int j = 0; j < r; ++j) s += rank_value(h, M * r, t * r + j, parts) * to_f32(w[((int64_t)a * r + j) * N + c]);
+            for (int j = 0; j < r; ++j) s += h[t * r + j] * to_f32(w[((int64_t)a * r + j) * N + c]);
             if (scaling) s *= scaling[a];
         }
         out[t * N + c] = from_f32<T>(base ? to_f32(base[t * N + c]) + s : s);
@@ -65,17 +58,19 @@ __global__ void __launch_bounds__(256) adapter_expand_general_kernel(const float
 
 template <typename T>
 __global__ void __launch_bounds__(256) adapter_outer_general_kernel(const float *__restrict__ h, const T *__restrict__ x, int64_t M, int64_t N, int r,
-                                                                    const int32_t *__restrict__ index, const float *__restrict__ scaling, T *dw, int parts) {
+                                                                    const int32_t *__restrict__ index, const float *__restrict__ scaling, T *dw) {
     const int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x;
     const int a = blockIdx.x / r, j = blockIdx.x % r;
     if (c >= N) return;
     float s = 0.0f;
     for (int64_t t = 0; t < M; ++t)
-        if (index[t] == a) s += rank_value(h, M * r, t * r + j, parts) * to_f32(x[t * N + c]);
+        if (index[t] == a) s += h[t * r + j] * to_f32(x[t * N + c]);
     dw[(int64_t)blockIdx.x * N + c] = from_f32<T>(scaling ? s * scaling[a] : s);
 }
 
-// ---- tensor-core forms: K and N multiples of 8, rows on 16-byte boundaries, rank a multiple of 8 up to 128 -----------------
+// ---- tensor-core forms: K and N multiples of 8, rank a multiple of 8 up to 128 -----------------------------------------------
+
+namespace cg = cooperative_groups;
 
 template <typename T> struct Pair;
 template <> struct Pair<__half> {
@@ -104,60 +99,143 @@ __device__ __forceinline__ uint32_t column_pair(const uint4 &even, const uint4 &
 __device__ __forceinline__ int exponent_of(float big) { return min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 100); }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
-// The adapters that occur in a tile of up to 64 tokens, in the order of their first token; every warp goes through them alike.  Tokens behind the
-// last are in no group.
-struct TileAdapters {
-    int lo, hi;               // of tokens lane and lane + 32
-    unsigned long long todo;
-    __device__ __forceinline__ TileAdapters(const int32_t *index, int64_t t0, int64_t M, int tokens) {
-        const int lane = threadIdx.x % 32;
-        const bool a = lane < tokens && t0 + lane < M, b = lane + 32 < tokens && t0 + lane + 32 < M;
-        lo = a ? __ldg(index + t0 + lane) : 0;
-        hi = b ? __ldg(index + t0 + lane + 32) : 0;
-        todo = __ballot_sync(0xffffffffu, a) | (unsigned long long)__ballot_sync(0xffffffffu, b) << 32;
-    }
-    // The next adapter and its tokens; false when there is none.
-    __device__ __forceinline__ bool next(int &adapter, unsigned long long &tokens) {
-        if (!todo) return false;
-        const int first = __ffsll((long long)todo) - 1;
-        adapter = first < 32 ? __shfl_sync(0xffffffffu, lo, first) : __shfl_sync(0xffffffffu, hi, first - 32);
-        tokens = todo & (__ballot_sync(0xffffffffu, lo == adapter) | (unsigned long long)__ballot_sync(0xffffffffu, hi == adapter) << 32);
-        todo &= ~tokens;
-        return true;
-    }
-};
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes to shared memory, asynchronously; zeros where there is nothing to copy.
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool ok) {
+    const int bytes = ok ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 load_shared16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void load_matrices(uint32_t at, uint32_t (&x)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t at, uint32_t (&x)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+}
+
+constexpr int TILE = 64;          // tokens
 
 struct AdapterArgs {
     int64_t M, cols;            // tokens; length of a row of w (K of down, N of up)
     const int32_t *index;
     const float *scaling;
     int adapters, rank;
-    int splits;                 // of the rank values' sums
     int slots;                  // CTAs among which the adapters of a tile of tokens are dealt
 };
 
-// Rank values of MW * 16 tokens, one split of the columns: MW warps of 16 tokens, KW parts of the split's columns, NBR * 8 ranks.
-template <typename T, int MW, int KW, int NBR>
-__global__ void __launch_bounds__(32 * MW * KW) adapter_shrink_kernel(const T *__restrict__ x, const T *__restrict__ w, const AdapterArgs p, int64_t per_split, float *h) {
-    constexpr int RANKS = 8 * NBR, UNROLL = NBR <= 2 ? 4 : 2;
-    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4, wm = warp % MW, wk = warp / MW;
-    const int slot = blockIdx.z % p.slots, rank0 = blockIdx.z / p.slots * RANKS;
-    const int64_t t0 = (int64_t)blockIdx.x * (16 * MW);
-    __shared__ float red[KW > 1 ? KW - 1 : 1][MW * 16][RANKS + 1];
-    const int64_t begin = blockIdx.y * per_split, end = begin + per_split < p.cols ? begin + per_split : p.cols;
-    const int64_t per_warp = (per_split / 32 + KW - 1) / KW * 32, k0 = begin + wk * per_warp, k1 = k0 + per_warp < end ? k0 + per_warp : end;
-    const int64_t ta = t0 + wm * 16 + r, tb = ta + 8;
+// Rank values: [M][rank] of 16 bits, the same of their rests, and (fp16) [M] powers of two by which both were divided.
+template <typename T> struct Hidden {
+    T *top, *rest;
+    float *back;
+    __host__ __device__ Hidden(void *p, int64_t M, int r) : top((T *)p), rest(top + M * r), back(reinterpret_cast<float *>(rest + M * r)) {}
+};
 
-    TileAdapters in_tile(p.index, t0, p.M, 16 * MW);
-    int a;
-    unsigned long long tokens;
-    for (int i = 0; in_tile.next(a, tokens); ++i) {
-        if (i % p.slots != slot || a < 0 || a >= p.adapters) continue;
-        const unsigned mine = (unsigned)(tokens >> (16 * wm)) & 0xffffu;
-        const bool has_a = mine >> r & 1, has_b = mine >> (r + 8) & 1;
-        float acc[NBR][4] = {};
-        if (mine) {
-            const T *xa = x + ta * p.cols + c * 8, *xb = x + tb * p.cols + c * 8, *wr = w + ((int64_t)a * p.rank + rank0 + r) * p.cols + c * 8;
+// The adapters that occur in a tile of tokens, in the order of their first token; every warp goes through them alike, with a list of their
+// tokens of its own.  Tokens behind the last are in no group.
+struct TileAdapters {
+    int lo, hi;               // of tokens lane and lane + 32
+    unsigned long long todo;
+    uint8_t *list;            // [TILE] places in the tile
+    int count, adapter;
+    __device__ __forceinline__ TileAdapters(const AdapterArgs &p, int64_t t0, uint8_t *list) : list(list) {
+        const int lane = threadIdx.x % 32;
+        const bool a = t0 + lane < p.M, b = t0 + lane + 32 < p.M;
+        lo = a ? __ldg(p.index + t0 + lane) : 0;
+        hi = b ? __ldg(p.index + t0 + lane + 32) : 0;
+        todo = __ballot_sync(0xffffffffu, a) | (unsigned long long)__ballot_sync(0xffffffffu, b) << 32;
+    }
+    // Takes the next adapter; false when there is none.
+    __device__ __forceinline__ bool next() {
+        if (!todo) return false;
+        const int first = __ffsll((long long)todo) - 1, lane = threadIdx.x % 32;
+        adapter = first < 32 ? __shfl_sync(0xffffffffu, lo, first) : __shfl_sync(0xffffffffu, hi, first - 32);
+        const unsigned long long tokens =
+            todo & (__ballot_sync(0xffffffffu, lo == adapter) | (unsigned long long)__ballot_sync(0xffffffffu, hi == adapter) << 32);
+        todo &= ~tokens;
+        const unsigned a = (unsigned)tokens, b = (unsigned)(tokens >> 32), below = (1u << lane) - 1;
+        if (a >> lane & 1) list[__popc(a & below)] = (uint8_t)lane;
+        if (b >> lane & 1) list[__popc(a) + __popc(b & below)] = (uint8_t)(lane + 32);
+        count = __popcll(tokens);
+        __syncwarp();
+        return true;
+    }
+};
+
+// The end of a shrink pass: the CTAs of a cluster have sums of their part of the columns in `sums` [rows][RANKS + 4]; each CTA adds up its share of
+// the rows, a warp a row, and writes them as two 16-bit parts.
+template <typename T, int RANKS>
+__device__ __forceinline__ void finish_rows(float *sums, int rows, int row0, int count, const uint8_t *list, int64_t t0, const AdapterArgs &p, const Hidden<T> &h) {
+    constexpr bool F16 = __is_same(T, __half);
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32, parts = gridDim.x, mine = blockIdx.x;
+    for (int row = mine + parts * warp; row < rows && row0 + row < count; row += parts * warps) {
+        constexpr int PAIRS = RANKS <= 64 ? 1 : 2;
+        float2 v[PAIRS];
+        float big = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            const int j = 2 * (lane + 32 * i);
+            v[i] = make_float2(0.0f, 0.0f);
+            if (j < RANKS)
+                for (int o = 0; o < parts; ++o) {
+                    const float2 u = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(sums, o) + row * (RANKS + 4) + j);
+                    v[i].x += u.x;
+                    v[i].y += u.y;
+                }
+            big = fmaxf(big, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+        }
+        float by = 1.0f;
+        const int64_t t = t0 + list[row0 + row];
+        if constexpr (F16) {
+            for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+            const int e = exponent_of(big);
+            by = power_of_two(-e);
+            if (lane == 0) h.back[t] = power_of_two(e);
+        }
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+            const int j = 2 * (lane + 32 * i);
+            if (j < p.rank) {
+                const uint32_t top = Pair<T>::pack(v[i].x * by, v[i].y * by);
+                const float2 f = Pair<T>::unpack(top);
+                *reinterpret_cast<uint32_t *>(h.top + t * p.rank + j) = top;
+                *reinterpret_cast<uint32_t *>(h.rest + t * p.rank + j) = Pair<T>::pack(v[i].x * by - f.x, v[i].y * by - f.y);
+            }
+        }
+    }
+    cluster.sync();                                          // the sums stay until the others have read them
+}
+
+// Rank values of a few tokens (up to 64): a CTA for each adapter and part of the columns, eight warps with a part of that each, fragments from global
+// memory.
+template <typename T, int NBR>
+__global__ void __launch_bounds__(256) adapter_shrink_few_kernel(const T *__restrict__ x, const T *__restrict__ w, const AdapterArgs p, int64_t per_split, void *hidden) {
+    constexpr int RANKS = 8 * NBR, UNROLL = NBR <= 4 ? 4 : 2;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+    __shared__ __align__(16) float sums[16][RANKS + 4];
+    extern __shared__ float red[];                            // [7][16][RANKS + 1]
+    __shared__ uint8_t lists[8][TILE];
+    const Hidden<T> h(hidden, p.M, p.rank);
+    const int64_t begin = blockIdx.x * per_split, end = begin + per_split < p.cols ? begin + per_split : p.cols;
+    const int64_t per_warp = (per_split / 32 + 7) / 8 * 32, k0 = begin + warp * per_warp, k1 = k0 + per_warp < end ? k0 + per_warp : end;
+
+    TileAdapters tile(p, 0, lists[warp]);
+    for (int i = 0; tile.next(); ++i) {
+        const int a = tile.adapter;
+        if (i % p.slots != (int)blockIdx.y || a < 0 || a >= p.adapters) continue;
+        for (int row0 = 0; row0 < tile.count; row0 += 16) {
+            const bool has_a = row0 + r < tile.count, has_b = row0 + r + 8 < tile.count;
+            const T *xa = x + (has_a ? tile.list[row0 + r] : 0) * p.cols + c * 8, *xb = x + (has_b ? tile.list[row0 + r + 8] : 0) * p.cols + c * 8;
+            const T *wr = w + ((int64_t)a * p.rank + r) * p.cols + c * 8;
+            float acc[NBR][4] = {};
 #pragma unroll UNROLL
             for (int64_t k = k0; k < k1; k += 32) {
                 const bool in = k + c * 8 < k1;
@@ -165,192 +243,324 @@ __global__ void __launch_bounds__(32 * MW * KW) adapter_shrink_kernel(const T *_
                 const uint32_t lo[4] = {va.x, vb.x, va.y, vb.y}, hi[4] = {va.z, vb.z, va.w, vb.w};
 #pragma unroll
                 for (int nb = 0; nb < NBR; ++nb) {
-                    const uint4 b = load16_if(wr + nb * 8 * p.cols + k, in && rank0 + nb * 8 < p.rank);
+                    const uint4 b = load16_if(wr + nb * 8 * p.cols + k, in && nb * 8 < p.rank);
                     Pair<T>::mma(acc[nb], lo, b.x, b.y);
                     Pair<T>::mma(acc[nb], hi, b.z, b.w);
                 }
             }
-        }
-        if constexpr (KW > 1) {
-            if (wk > 0) {
+            if (warp > 0) {
 #pragma unroll
                 for (int nb = 0; nb < NBR; ++nb)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) red[wk - 1][wm * 16 + r + 8 * (e / 2)][nb * 8 + 2 * c + e % 2] = acc[nb][e];
+                    for (int e = 0; e < 4; ++e) red[((warp - 1) * 16 + r + 8 * (e / 2)) * (RANKS + 1) + nb * 8 + 2 * c + e % 2] = acc[nb][e];
+            } else {
+#pragma unroll
+                for (int nb = 0; nb < NBR; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sums[r + 8 * (e / 2)][nb * 8 + 2 * c + e % 2] = acc[nb][e];
             }
             __syncthreads();
-            if (wk == 0) {
+            for (int j = threadIdx.x; j < 16 * RANKS; j += 256) {
+                float s = sums[j / RANKS][j % RANKS];
 #pragma unroll
-                for (int nb = 0; nb < NBR; ++nb)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-#pragma unroll
-                        for (int o = 0; o < KW - 1; ++o) acc[nb][e] += red[o][wm * 16 + r + 8 * (e / 2)][nb * 8 + 2 * c + e % 2];
+                for (int o = 0; o < 7; ++o) s += red[(o * 16 + j / RANKS) * (RANKS + 1) + j % RANKS];
+                sums[j / RANKS][j % RANKS] = s;
             }
+            finish_rows<T, RANKS>(&sums[0][0], 16, row0, tile.count, tile.list, 0, p, h);
         }
-        if (wk == 0) {
-#pragma unroll
-            for (int nb = 0; nb < NBR; ++nb)
-                if (rank0 + nb * 8 < p.rank) {
-                    float *to = h + ((int64_t)blockIdx.y * p.M + ta) * p.rank + rank0 + nb * 8 + 2 * c;
-                    if (has_a) *reinterpret_cast<float2 *>(to) = make_float2(acc[nb][0], acc[nb][1]);
-                    if (has_b) *reinterpret_cast<float2 *>(to + 8 * p.rank) = make_float2(acc[nb][2], acc[nb][3]);
-                }
-        }
-        if constexpr (KW > 1) __syncthreads();
     }
 }
 
-// Two neighbouring rank values of a token, summed over the splits.
-__device__ __forceinline__ float2 rank_pair(const float *h, const AdapterArgs &p, int64_t t, int j) {
-    float2 v = __ldg(reinterpret_cast<const float2 *>(h + t * p.rank + j));
-    for (int s = 1; s < p.splits; ++s) {
-        const float2 o = __ldg(reinterpret_cast<const float2 *>(h + (s * p.M + t) * p.rank + j));
-        v.x += o.x;
-        v.y += o.y;
-    }
-    return v;
-}
-
-// out[t] = base[t] + f * (h[t] times w) of SUB * 16 tokens, eight warps with 64 columns each at a time; KS steps of 16 ranks at once.
-template <typename T, int SUB, int KS>
-__global__ void __launch_bounds__(256) adapter_expand_kernel(const float *__restrict__ h, const T *__restrict__ w, const AdapterArgs p, const T *base, T *out) {
-    constexpr bool F16 = __is_same(T, __half);
+// Rank values of many tokens: 64 rows of one adapter, a part of the columns; rows of x and of w go through a ring in shared memory, 64 columns a
+// stage, in 16-byte pieces exchanged by row so that ldmatrix meets all banks.
+template <typename T, int NBR>
+__global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict__ x, const T *__restrict__ w, const AdapterArgs p, int64_t per_split, void *hidden) {
+    constexpr int RANKS = 8 * NBR, STAGE = (TILE + RANKS) * 128, STAGES = NBR <= 8 ? 4 : 3;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-    const int64_t t0 = (int64_t)blockIdx.x * (16 * SUB);
-    const int steps = (p.rank + 15) / 16;
-    extern __shared__ uint4 frag[];                              // [SUB][steps][2 (value, rest)][32]
-    __shared__ float s_factor[16 * SUB];
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint8_t lists[4][TILE];
+    const uint32_t ring = smem_addr(smem);
+    const Hidden<T> h(hidden, p.M, p.rank);
+    const int64_t t0 = (int64_t)blockIdx.y * TILE, begin = blockIdx.x * per_split, end = begin + per_split < p.cols ? begin + per_split : p.cols;
 
-    TileAdapters in_tile(p.index, t0, p.M, 16 * SUB);
-    // rank values as fragments; rows without an adapter hold zeros
-    for (int row = warp; row < 16 * SUB; row += 8) {
-        const int64_t t = t0 + row;
-        const int a = row < 32 ? __shfl_sync(0xffffffffu, in_tile.lo, row) : __shfl_sync(0xffffffffu, in_tile.hi, row - 32);
-        const bool has = t < p.M && a >= 0 && a < p.adapters;
-        float2 v[2];
-        float big = 0.0f;
+    TileAdapters tile(p, t0, lists[warp]);
+    for (int i = 0; tile.next(); ++i) {
+        const int a = tile.adapter;
+        if (i % p.slots != (int)blockIdx.z || a < 0 || a >= p.adapters) continue;
+        // a thread copies piece threadIdx % 8 of every 16th row
+        const int piece = threadIdx.x % 8;
+        const T *rows[4];
+        bool has[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int j = 2 * (lane + 32 * i);
-            v[i] = has && j < p.rank ? rank_pair(h, p, t, j) : make_float2(0.0f, 0.0f);
-            big = fmaxf(big, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+        for (int j = 0; j < 4; ++j) {
+            const int row = threadIdx.x / 8 + 16 * j;
+            has[j] = row < tile.count;
+            rows[j] = x + (t0 + (has[j] ? tile.list[row] : 0)) * p.cols + piece * 8;
         }
-        float by = 1.0f, back = 1.0f;
-        if constexpr (F16) {
-            for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-            const int e = exponent_of(big);
-            by = power_of_two(-e);
-            back = power_of_two(e);
-        }
-        if (lane == 0) s_factor[row] = has && p.scaling ? back * __ldg(p.scaling + a) : back;
+        const T *wrow = w + ((int64_t)a * p.rank + threadIdx.x / 8) * p.cols + piece * 8;
+        const int swizzled = threadIdx.x / 8 * 128 + ((piece ^ (threadIdx.x / 8 & 7)) * 16);
+        auto copy_stage = [&](int64_t k, int stage) {
+            if (k < end) {
+                const bool in = k + piece * 8 < end;
+                const uint32_t to = ring + stage * STAGE + swizzled;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int j = 2 * (lane + 32 * i);
-            if (j < 16 * steps) {
-                const uint32_t top = Pair<T>::pack(v[i].x * by, v[i].y * by);
-                const float2 f = Pair<T>::unpack(top);
-                const uint32_t rest = Pair<T>::pack(v[i].x * by - f.x, v[i].y * by - f.y);
-                uint32_t *to = reinterpret_cast<uint32_t *>(frag + (size_t)(row / 16 * steps + j / 16) * 64) + ((row % 8) * 4 + j % 8 / 2) * 4 + j % 16 / 8 * 2 + row % 16 / 8;
-                to[0] = top;
-                to[128] = rest;
+                for (int j = 0; j < 4; ++j) copy16(to + j * 2048, in && has[j] ? rows[j] + k : x, in && has[j]);
+#pragma unroll
+                for (int j = 0; j < (RANKS + 15) / 16; ++j) {
+                    const int rank = threadIdx.x / 8 + 16 * j;
+                    const bool ok = in && rank < p.rank;
+                    if (rank < RANKS) copy16(to + TILE * 128 + j * 2048, ok ? wrow + 16 * j * p.cols + k : w, ok);
+                }
+            }
+            copies_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) copy_stage(begin + s * 64, s);
+        float acc[NBR][4] = {};
+        const bool busy = warp * 16 < tile.count;
+        int stage = 0;
+        for (int64_t k = begin; k < end; k += 64) {
+            copies_wait<STAGES - 2>();
+            __syncthreads();                                 // the stage is there for all, and the one filled next has been used by all
+            copy_stage(k + (STAGES - 1) * 64, stage == 0 ? STAGES - 1 : stage - 1);
+            const uint32_t xs = ring + stage * STAGE, ws = xs + TILE * 128;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            if (busy) {
+#pragma unroll
+                for (int kk = 0; kk < 4; ++kk) {
+                    uint32_t xa[4];
+                    const int row = warp * 16 + lane % 16;
+                    load_matrices(xs + row * 128 + (((2 * kk + lane / 16) ^ (row & 7)) * 16), xa);
+#pragma unroll
+                    for (int nb = 0; nb < NBR; nb += 2) {
+                        uint32_t b[4];
+                        const int rank = (nb * 8 + lane % 8 + lane / 16 * 8) % RANKS;      // (rank 8: the second pair is the first again)
+                        load_matrices(ws + rank * 128 + (((2 * kk + lane / 8 % 2) ^ (rank & 7)) * 16), b);
+                        Pair<T>::mma(acc[nb], xa, b[0], b[1]);
+                        if (nb + 1 < NBR) Pair<T>::mma(acc[nb + 1 < NBR ? nb + 1 : nb], xa, b[2], b[3]);
+                    }
+                }
             }
         }
-    }
-    __syncthreads();
-
-    const int64_t first = ((int64_t)blockIdx.y * 8 + warp) * 64, step = (int64_t)gridDim.y * 512;
-    int a;
-    unsigned long long tokens;
-    for (int i = 0; in_tile.next(a, tokens); ++i) {
-        if (i % p.slots != (int)blockIdx.z) continue;
-        const bool has = a >= 0 && a < p.adapters;
-        if (a < 0 && base == out) continue;
-        for (int64_t cb = first; cb < p.cols; cb += step) {
-            const int64_t col = cb + r * 8;                       // of the lane's columns of w; its results: cb + 16 c and on
-            uint32_t b[KS][8][2];
-            auto load_w = [&](int k0) {
+        copies_wait<0>();
+        __syncthreads();
+        float *sums = reinterpret_cast<float *>(smem);       // [TILE][RANKS + 4]
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const int j = k0 + 16 * ks + 2 * c;
-                    const T *from = w + ((int64_t)a * p.rank + j) * p.cols + col;
-                    const bool in = has && col < p.cols;
-                    const uint4 w0 = load16_if(from, in && j < p.rank), w1 = load16_if(from + p.cols, in && j < p.rank),
-                                w2 = load16_if(from + 8 * p.cols, in && j + 8 < p.rank), w3 = load16_if(from + 9 * p.cols, in && j + 8 < p.rank);
+        for (int nb = 0; nb < NBR; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sums[(warp * 16 + r + 8 * (e / 2)) * (RANKS + 4) + nb * 8 + 2 * c + e % 2] = acc[nb][e];
+        finish_rows<T, RANKS>(sums, TILE, 0, tile.count, tile.list, t0, p, h);
+    }
+}
+
+// ---- expand --------------------------------------------------------------------------------------------------------------
+
+// Fragments of the rank values of 16 rows: [steps][value and rest].
+template <typename T, int KS>
+__device__ __forceinline__ void load_rank_values(const Hidden<T> &h, int rank, int64_t ta, int64_t tb, bool has_a, bool has_b, int c, uint32_t (&top)[KS][4], uint32_t (&rest)[KS][4]) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int j = 16 * ks + 2 * c + e / 2 * 8;
+            const bool has = (e % 2 ? has_b : has_a) && j < rank;
+            const int64_t at = (e % 2 ? tb : ta) * rank + j;
+            top[ks][e] = has ? __ldg(reinterpret_cast<const uint32_t *>(h.top + at)) : 0u;
+            rest[ks][e] = has ? __ldg(reinterpret_cast<const uint32_t *>(h.rest + at)) : 0u;
+        }
+}
+// What a row's product is multiplied by.
+template <typename T>
+__device__ __forceinline__ float row_factor(const Hidden<T> &h, const AdapterArgs &p, int a, int64_t t, bool has) {
+    if (a < 0 || !has) return 0.0f;
+    if (a >= p.adapters) return NAN;
+    return (__is_same(T, __half) ? __ldg(h.back + t) : 1.0f) * (p.scaling ? __ldg(p.scaling + a) : 1.0f);
+}
+// base + f * product, 16 neighbouring columns of two rows; `old` is base (zeros without one).
+template <typename T>
+__device__ __forceinline__ void store_rows(T *const (&to)[2], const bool (&live)[2], const bool (&in)[2], const uint4 (&old)[2][2], const float (&acc)[8][4], const float (&f)[2], bool plain) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (!live[j / 2] || !in[j % 2]) continue;
+        const uint32_t *o = reinterpret_cast<const uint32_t *>(&old[j / 2][j % 2]);
+        uint32_t y[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float2 v = Pair<T>::unpack(o[n]);
+            y[n] = plain ? o[n] : Pair<T>::pack(fmaf(acc[2 * n][j], f[j / 2], v.x), fmaf(acc[2 * n + 1][j], f[j / 2], v.y));
+        }
+        *reinterpret_cast<uint4 *>(to[j / 2] + j % 2 * 8) = make_uint4(y[0], y[1], y[2], y[3]);
+    }
+}
+
+// out[t] = base[t] + f * (h[t] times w) of a few tokens: a CTA an adapter and 512 columns, a warp 64 of them; w straight from global memory, KS steps
+// of 16 ranks at once.
+template <typename T, int KS>
+__global__ void __launch_bounds__(256) adapter_expand_few_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, const T *base, T *out) {
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+    __shared__ uint8_t lists[8][TILE];
+    const Hidden<T> h(hidden, p.M, p.rank);
+    const int64_t cb = ((int64_t)blockIdx.x * 8 + warp) * 64, col = cb + r * 8;
+    if (cb >= p.cols) return;
+    const bool in[2] = {cb + 16 * c < p.cols, cb + 16 * c + 8 < p.cols};
+    TileAdapters tile(p, 0, lists[warp]);
+    for (int i = 0; tile.next(); ++i) {
+        const int a = tile.adapter;
+        if (i % p.slots != (int)blockIdx.y || (a < 0 && base == out)) continue;
+        const bool has = a >= 0 && a < p.adapters;
+        uint4 raw[KS][4];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int j = 16 * ks + 2 * c + k % 2 + k / 2 * 8;
+                raw[ks][k] = load16_if(w + ((int64_t)(has ? a : 0) * p.rank + j) * p.cols + col, has && col < p.cols && j < p.rank);
+            }
+        for (int row0 = 0; row0 < tile.count; row0 += 16) {
+            const bool live[2] = {row0 + r < tile.count, row0 + r + 8 < tile.count};
+            const int64_t t[2] = {live[0] ? tile.list[row0 + r] : 0, live[1] ? tile.list[row0 + r + 8] : 0};
+            uint4 old[2][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                old[j / 2][j % 2] = base && live[j / 2] && in[j % 2] ? *reinterpret_cast<const uint4 *>(base + t[j / 2] * p.cols + cb + 16 * c + j % 2 * 8)
+                                                                      : make_uint4(0, 0, 0, 0);
+            const float f[2] = {row_factor(h, p, a, t[0], live[0]), row_factor(h, p, a, t[1], live[1])};
+            float acc[8][4] = {};
+            if (has) {
+                uint32_t top[KS][4], rest[KS][4];
+                load_rank_values<T, KS>(h, p.rank, t[0], t[1], live[0], live[1], c, top, rest);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                     for (int n = 0; n < 8; ++n) {
-                        b[ks][n][0] = column_pair(w0, w1, n);
-                        b[ks][n][1] = column_pair(w2, w3, n);
+                        const uint32_t b0 = column_pair(raw[ks][0], raw[ks][1], n), b1 = column_pair(raw[ks][2], raw[ks][3], n);
+                        Pair<T>::mma(acc[n], top[ks], b0, b1);
+                        Pair<T>::mma(acc[n], rest[ks], b0, b1);
                     }
-                }
-            };
-            if (has) load_w(0);
-#pragma unroll 1
-            for (int sub = 0; sub < SUB; ++sub) {
-                const unsigned mine = (unsigned)(tokens >> (16 * sub)) & 0xffffu;
-                if (!mine) continue;
-                const int64_t at = (t0 + sub * 16 + r) * p.cols + cb + 16 * c;
-                const bool live[2] = {(bool)(mine >> r & 1), (bool)(mine >> (r + 8) & 1)};
-                uint4 old[2][2];
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    old[j / 2][j % 2] = base && live[j / 2] && cb + 16 * c + j % 2 * 8 < p.cols
-                                            ? *reinterpret_cast<const uint4 *>(base + at + j / 2 * 8 * p.cols + j % 2 * 8) : make_uint4(0, 0, 0, 0);
-                float acc[8][4] = {};
-                if (has)
-                    for (int k = 0; k < steps; k += KS) {
-                        if (k > 0 || (steps > KS && sub > 0)) load_w(16 * k);
-#pragma unroll
-                        for (int ks = 0; ks < KS; ++ks) {
-                            if (k + ks >= steps) break;
-                            const uint4 *f = frag + (size_t)(sub * steps + k + ks) * 64 + lane;
-                            const uint4 top = f[0], rest = f[32];
-                            const uint32_t at4[4] = {top.x, top.y, top.z, top.w}, ar[4] = {rest.x, rest.y, rest.z, rest.w};
-#pragma unroll
-                            for (int n = 0; n < 8; ++n) {
-                                Pair<T>::mma(acc[n], at4, b[ks][n][0], b[ks][n][1]);
-                                Pair<T>::mma(acc[n], ar, b[ks][n][0], b[ks][n][1]);
-                            }
-                        }
-                    }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {                      // row r or r + 8, columns 0 to 7 or 8 to 15 of the lane's
-                    if (!live[j / 2] || cb + 16 * c + j % 2 * 8 >= p.cols) continue;
-                    const float f = a >= p.adapters ? NAN : s_factor[sub * 16 + r + j / 2 * 8];
-                    const uint32_t *o = reinterpret_cast<const uint32_t *>(&old[j / 2][j % 2]);
-                    uint32_t y[4];
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        const float2 v = Pair<T>::unpack(o[n]);
-                        y[n] = a < 0 ? o[n] : Pair<T>::pack(fmaf(acc[2 * n][j], f, v.x), fmaf(acc[2 * n + 1][j], f, v.y));
-                    }
-                    *reinterpret_cast<uint4 *>(out + at + j / 2 * 8 * p.cols + j % 2 * 8) = make_uint4(y[0], y[1], y[2], y[3]);
-                }
             }
+            T *const to[2] = {out + t[0] * p.cols + cb + 16 * c, out + t[1] * p.cols + cb + 16 * c};
+            store_rows<T>(to, live, in, old, acc, f, a < 0);
         }
     }
 }
 
-constexpr int OUTER_LIST = 2048, OUTER_TOKENS = 64;
+// The same of many tokens: 64 rows of one adapter, 16 a warp with their rank values in registers; blocks of 64 columns of w go through a ring in shared
+// memory, and the rows of base are loaded a block ahead.
+template <typename T, int KS>
+__global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, int64_t per_group, const T *base, T *out) {
+    constexpr int STAGE = KS * 16 * 128, STAGES = KS <= 4 ? 4 : 3;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint8_t lists[4][TILE];
+    const uint32_t ring = smem_addr(smem);
+    const Hidden<T> h(hidden, p.M, p.rank);
+    const int64_t t0 = (int64_t)blockIdx.x * TILE, begin = blockIdx.y * per_group, end = begin + per_group < p.cols ? begin + per_group : p.cols;
+
+    TileAdapters tile(p, t0, lists[warp]);
+    for (int i = 0; tile.next(); ++i) {
+        const int a = tile.adapter;
+        if (i % p.slots != (int)blockIdx.z || (a < 0 && base == out)) continue;
+        const bool has = a >= 0 && a < p.adapters;
+        const T *wrow = w + ((int64_t)(has ? a : 0) * p.rank + threadIdx.x / 8) * p.cols + threadIdx.x % 8 * 8;
+        auto copy_stage = [&](int64_t cb, int stage) {
+            if (cb < end && has) {
+                const bool in = cb + threadIdx.x % 8 * 8 < p.cols;
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    const int row = threadIdx.x / 8 + 16 * j;
+                    const bool ok = in && row < p.rank;
+                    copy16(ring + stage * STAGE + row * 128 + ((threadIdx.x % 8) ^ (row >> 1 & 3) << 1) * 16, ok ? wrow + 16 * j * p.cols + cb : w, ok);
+                }
+            }
+            copies_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) copy_stage(begin + 64 * s, s);
+
+        const int row = warp * 16 + r;
+        const bool live[2] = {row < tile.count, row + 8 < tile.count};
+        const int64_t t[2] = {t0 + (live[0] ? tile.list[row] : 0), t0 + (live[1] ? tile.list[row + 8] : 0)};
+        uint32_t top[KS][4], rest[KS][4];
+        load_rank_values<T, KS>(h, p.rank, t[0], t[1], live[0] && has, live[1] && has, c, top, rest);
+        const float f[2] = {row_factor(h, p, a, t[0], live[0]), row_factor(h, p, a, t[1], live[1])};
+        auto load_base = [&](int64_t cb, uint4 (&v)[2][2]) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                v[j / 2][j % 2] = base && live[j / 2] && cb < end && cb + 16 * c + j % 2 * 8 < p.cols
+                                      ? *reinterpret_cast<const uint4 *>(base + t[j / 2] * p.cols + cb + 16 * c + j % 2 * 8) : make_uint4(0, 0, 0, 0);
+        };
+        uint4 old[2][2], ahead[2][2];
+        load_base(begin, old);
+        int stage = 0;
+        const bool busy = warp * 16 < tile.count;
+        for (int64_t cb = begin; cb < end; cb += 64) {
+            copies_wait<STAGES - 2>();
+            __syncthreads();
+            copy_stage(cb + (STAGES - 1) * 64, stage == 0 ? STAGES - 1 : stage - 1);
+            const uint32_t ws = ring + stage * STAGE;
+            stage = stage + 1 == STAGES ? 0 : stage + 1;
+            if (!busy) continue;
+            load_base(cb + 64, ahead);
+            float acc[8][4] = {};
+            if (has) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    uint4 raw[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int j = 16 * ks + 2 * c + k % 2 + k / 2 * 8;
+                        raw[k] = load_shared16(ws + j * 128 + (r ^ (j >> 1 & 3) << 1) * 16);
+                    }
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const uint32_t b0 = column_pair(raw[0], raw[1], n), b1 = column_pair(raw[2], raw[3], n);
+                        Pair<T>::mma(acc[n], top[ks], b0, b1);
+                        Pair<T>::mma(acc[n], rest[ks], b0, b1);
+                    }
+                }
+            }
+            T *const to[2] = {out + t[0] * p.cols + cb + 16 * c, out + t[1] * p.cols + cb + 16 * c};
+            const bool in[2] = {cb + 16 * c < p.cols, cb + 16 * c + 8 < p.cols};
+            store_rows<T>(to, live, in, old, acc, f, a < 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) old[j / 2][j % 2] = ahead[j / 2][j % 2];
+        }
+        copies_wait<0>();
+        __syncthreads();
+    }
+}
+
+// ---- outer ---------------------------------------------------------------------------------------------------------------
+
+constexpr int OUTER_LIST = 2048, OUTER_STEP = 32;
+
+template <int RB> struct OuterShape {
+    static constexpr int RANKS = 16 * RB, ROW = RANKS * 2;                    // bytes of a token's rank values
+    static constexpr int STAGE = OUTER_STEP * (512 + 2 * ROW), STAGES = RB <= 2 ? 4 : 3;
+    static constexpr int SUMS = RANKS * 256 * 4, SMEM = STAGE * STAGES > SUMS ? STAGE * STAGES : SUMS;
+    static __device__ __forceinline__ int swizzle(int token) { return ROW >= 128 ? token & 7 : ROW == 64 ? token >> 1 & 3 : token >> 2 & 1; }
+};
 
 // dw[a][rank0 .. + 16 RB][256 columns] = f_a * sum over the adapter's tokens of h[t] x[t]^T.  The CTAs of a cluster (blockIdx.z) take equal shares of
-// the tokens and add their sums through each other's shared memory.
+// the tokens and add their sums through each other's shared memory.  Rows of x and of the rank values go through a ring, 32 tokens a stage.
 template <typename T, int RB>
-__global__ void __launch_bounds__(128) adapter_outer_kernel(const float *__restrict__ h, const T *__restrict__ x, const AdapterArgs p, T *dw) {
-    namespace cg = cooperative_groups;
+__global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
+    using S = OuterShape<RB>;
     constexpr bool F16 = __is_same(T, __half);
-    constexpr int RANKS = 16 * RB;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-    const int rank_blocks = (p.rank + RANKS - 1) / RANKS, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * RANKS;
-    const int64_t cb = (int64_t)blockIdx.x * 256 + warp * 64, col = cb + r * 8;
-    extern __shared__ uint4 outer_smem[];
-    uint4 *frag = outer_smem;                                    // [4 token steps][RB][2 (value, rest)][32]
-    float *sums = reinterpret_cast<float *>(outer_smem);         // [RANKS][256], at the end
-    __shared__ int list[OUTER_LIST], s_count[4], s_big[4];
+    const int rank_blocks = (p.rank + S::RANKS - 1) / S::RANKS, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * S::RANKS;
+    const int64_t col0 = (int64_t)blockIdx.x * 256;
+    extern __shared__ __align__(128) uint8_t smem[];
+    float *sums = reinterpret_cast<float *>(smem);               // [RANKS][256], at the end
+    const uint32_t ring = smem_addr(smem);
+    const Hidden<T> h(hidden, p.M, p.rank);
+    __shared__ int list[OUTER_LIST], s_count[4];
+    __shared__ float s_back[OUTER_LIST], s_big[4];
 
     // the adapter's tokens before this warp's quarter of all, and in all
     const int64_t quarter = (p.M + 127) / 128 * 32, q0 = warp * quarter, q1 = q0 + quarter < p.M ? q0 + quarter : p.M;
     int count = 0;
+#pragma unroll 4
     for (int64_t t = q0; t < q1; t += 32) count += __popc(__ballot_sync(0xffffffffu, t + lane < q1 && __ldg(p.index + t + lane) == a));
     if (lane == 0) s_count[warp] = count;
     __syncthreads();
@@ -362,7 +572,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(const float *__restr
     const int share = (all + gridDim.z - 1) / gridDim.z, lo = blockIdx.z * share, hi = lo + share < all ? lo + share : all;
 
     float acc[RB][8][4] = {};
-    int e = -100;                                                // fp16: the sums are of h * 2^-e
+    float big = 0.0f;                                            // fp16: the sums are of h / big, the largest power of two of a row so far
     for (int from = lo; from < hi; from += OUTER_LIST) {
         const int n = hi - from < OUTER_LIST ? hi - from : OUTER_LIST;
         __syncthreads();
@@ -375,89 +585,110 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(const float *__restr
             at += __popc(m);
         }
         __syncthreads();
-        for (int chunk = 0; chunk < n; chunk += OUTER_TOKENS) {
-            // rank values of 64 tokens as fragments (rows are ranks here): a thread takes pairs of tokens of one rank pair
-            constexpr int ITEMS = OUTER_TOKENS / 2 * RANKS / 2 / 128;
-            float2 v[ITEMS][2];
-            float big = 0.0f;
+        auto copy_stage = [&](int first, int stage) {
+            if (first < n) {
+                const uint32_t to = ring + stage * S::STAGE;
+                // 32 rows of 32 pieces of x: a warp a row
 #pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const int item = threadIdx.x + 128 * i, j = rank0 + item % (RANKS / 2) * 2, tp = chunk + item / (RANKS / 2) * 2;
+                for (int j = 0; j < OUTER_STEP / 4; ++j) {
+                    const int row = warp + 4 * j;
+                    const bool ok = first + row < n && col0 + lane * 8 < p.cols;
+                    const int64_t t = list[first + row < n ? first + row : 0];
+                    copy16(to + row * 512 + (lane ^ (row >> 1 & 3) << 1) * 16, ok ? x + t * p.cols + col0 + lane * 8 : x, ok);
+                }
+                constexpr int PIECES = S::ROW / 16;              // of a token's rank values
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    v[i][k] = tp + k < n && j < p.rank ? rank_pair(h, p, list[tp + k], j) : make_float2(0.0f, 0.0f);
-                    big = fmaxf(big, fmaxf(fabsf(v[i][k].x), fabsf(v[i][k].y)));
+                for (int j = 0; j < (OUTER_STEP * PIECES * 2 + 127) / 128; ++j) {
+                    const int i = threadIdx.x + 128 * j, part = i / (OUTER_STEP * PIECES), row = i / PIECES % OUTER_STEP, piece = i % PIECES;
+                    const bool ok = first + row < n && rank0 + piece * 8 < p.rank;
+                    const int64_t t = list[first + row < n ? first + row : 0];
+                    copy16(to + OUTER_STEP * (512 + part * S::ROW) + row * S::ROW + (piece ^ S::swizzle(row)) * 16,
+                           ok ? (part ? h.rest : h.top) + t * p.rank + rank0 + piece * 8 : h.top, ok);
                 }
             }
-            float by = 1.0f;
-            if constexpr (F16) {
-                for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-                if (lane == 0) s_big[warp] = exponent_of(big);
+            copies_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < S::STAGES - 1; ++s) copy_stage(s * OUTER_STEP, s);
+        if constexpr (F16) {
+            // powers of two of the rows, relative to the largest
+            float most = 0.0f;
+            for (int j = threadIdx.x; j < n; j += 128) {
+                s_back[j] = __ldg(h.back + list[j]);
+                most = fmaxf(most, s_back[j]);
             }
-            __syncthreads();                                     // (and the fragments before have been used)
-            if constexpr (F16) {
-                const int now = max(max(s_big[0], s_big[1]), max(s_big[2], s_big[3]));
-                if (now > e) {
-                    const float down = power_of_two(max(e - now, -126));
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) acc[rb][j][k] *= down;
-                    e = now;
-                }
-                by = power_of_two(-e);
-            }
-#pragma unroll
-            for (int i = 0; i < ITEMS; ++i) {
-                const int item = threadIdx.x + 128 * i, j = item % (RANKS / 2) * 2, tp = item / (RANKS / 2) * 2;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {                     // rank j + k, tokens tp and tp + 1
-                    const float v0 = (k ? v[i][0].y : v[i][0].x) * by, v1 = (k ? v[i][1].y : v[i][1].x) * by;
-                    const uint32_t top = Pair<T>::pack(v0, v1);
-                    const float2 f = Pair<T>::unpack(top);
-                    uint32_t *to = reinterpret_cast<uint32_t *>(frag + (size_t)(tp / 16 * RB + j / 16) * 64) + (((j + k) % 8) * 4 + tp % 8 / 2) * 4 + tp % 16 / 8 * 2 + j % 16 / 8;
-                    to[0] = top;
-                    to[128] = Pair<T>::pack(v0 - f.x, v1 - f.y);
-                }
-            }
+            for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            if (lane == 0) s_big[warp] = most;
             __syncthreads();
-            if (cb < p.cols) {
-#pragma unroll 2
-                for (int step = 0; step < OUTER_TOKENS / 16; ++step) {
-                    if (chunk + step * 16 >= n) break;
-                    uint4 rows[4];
+            most = fmaxf(big, fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3])));
+            if (big > 0.0f && most > big) {
+                const float down = big / most;
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int i = chunk + step * 16 + 2 * c + k % 2 + k / 2 * 8;
-                        const bool in = i < n && col < p.cols;
-                        rows[k] = load16_if(x + (in ? (int64_t)list[i] * p.cols + col : 0), in);
-                    }
-                    uint32_t b[8][2];
+                for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        b[j][0] = column_pair(rows[0], rows[1], j);
-                        b[j][1] = column_pair(rows[2], rows[3], j);
-                    }
+                    for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        const uint4 *f = frag + (size_t)(step * RB + rb) * 64 + lane;
-                        const uint4 top = f[0], rest = f[32];
-                        const uint32_t at4[4] = {top.x, top.y, top.z, top.w}, ar[4] = {rest.x, rest.y, rest.z, rest.w};
+                        for (int k = 0; k < 4; ++k) acc[rb][j][k] *= down;
+            }
+            big = most;
+            for (int j = threadIdx.x; j < n; j += 128) s_back[j] /= big;
+            // (the barrier of the first stage lies between this and its use)
+        }
+        int stage = 0;
+        for (int first = 0; first < n; first += OUTER_STEP) {
+            copies_wait<S::STAGES - 2>();
+            __syncthreads();
+            copy_stage(first + (S::STAGES - 1) * OUTER_STEP, stage == 0 ? S::STAGES - 1 : stage - 1);
+            const uint32_t xs = ring + stage * S::STAGE, hs = xs + OUTER_STEP * 512;
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+            if (col0 + warp * 64 >= p.cols) continue;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            Pair<T>::mma(acc[rb][j], at4, b[j][0], b[j][1]);
-                            Pair<T>::mma(acc[rb][j], ar, b[j][0], b[j][1]);
-                        }
+            for (int step = 0; step < OUTER_STEP / 16; ++step) {
+                if (first + step * 16 >= n) break;
+                uint4 raw[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int row = step * 16 + 2 * c + k % 2 + k / 2 * 8;
+                    raw[k] = load_shared16(xs + row * 512 + warp * 128 + (r ^ (row >> 1 & 3) << 1) * 16);
+                }
+                uint32_t b[8][2];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    b[j][0] = column_pair(raw[0], raw[1], j);
+                    b[j][1] = column_pair(raw[2], raw[3], j);
+                }
+                __half2 scale[2];
+                if constexpr (F16) {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int i = first + step * 16 + 2 * c + 8 * k;
+                        scale[k] = __floats2half2_rn(i < n ? s_back[i] : 0.0f, i + 1 < n ? s_back[i + 1] : 0.0f);
                     }
                 }
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        const int token = step * 16 + lane % 8 + lane / 16 * 8, piece = rb * 2 + lane / 8 % 2;
+                        uint32_t ha[4];
+                        load_matrices_transposed(hs + part * OUTER_STEP * S::ROW + token * S::ROW + (piece ^ S::swizzle(token)) * 16, ha);
+                        if constexpr (F16) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&ha[k]), scale[k / 2]);
+                                ha[k] = *reinterpret_cast<const uint32_t *>(&y);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) Pair<T>::mma(acc[rb][j], ha, b[j][0], b[j][1]);
+                    }
             }
         }
+        copies_wait<0>();
     }
 
     // sums of this CTA, in 16 neighbouring columns a lane; then those of the cluster
-    const float f = (F16 ? power_of_two(e) : 1.0f) * (p.scaling ? __ldg(p.scaling + a) : 1.0f);
+    const float f = (F16 ? big : 1.0f) * (p.scaling ? __ldg(p.scaling + a) : 1.0f);
     __syncthreads();
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -468,9 +699,9 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(const float *__restr
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     const int parts = gridDim.z, mine = blockIdx.z;
-    for (int i = mine * 128 + threadIdx.x; i < RANKS * 32; i += parts * 128) {        // eight columns of a rank
+    for (int i = mine * 128 + threadIdx.x; i < S::RANKS * 32; i += parts * 128) {        // eight columns of a rank
         const int rank = rank0 + i / 32;
-        const int64_t at = (int64_t)blockIdx.x * 256 + i % 32 * 8;
+        const int64_t at = col0 + i % 32 * 8;
         if (rank >= p.rank || at >= p.cols) continue;
         float4 s0 = make_float4(0, 0, 0, 0), s1 = s0;
         for (int o = 0; o < parts; ++o) {
@@ -487,153 +718,156 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(const float *__restr
 
 // ---- host side -------------------------------------------------------------------------------------------------------
 
-bool fast_rank(int r) { return r % 8 == 0 && r <= 128; }
+constexpr int64_t FEW = TILE;       // tokens up to which each adapter has CTAs of its own
 
-// Splits of a shrink pass's columns.  They go by sizes alone, so that whoever reads the rank values knows how many parts they have.
-int shrink_splits(int64_t M, int64_t cols, int r) {
-    if (!fast_rank(r) || cols % 8 != 0) return 1;
-    const int64_t tiles = M <= 64 ? (M + 15) / 16 : (M + 31) / 32;
-    int64_t s = 256 / (tiles > 0 ? tiles : 1), most = (cols + 511) / 512;
-    if (s > most) s = most;
-    if (s > 8) s = 8;
-    return s < 1 ? 1 : (int)s;
-}
-
-template <typename T, int NBR>
-int shrink_fast(const T *x, const T *w, AdapterArgs p, float *h, cudaStream_t st) {
-    const int64_t per_split = ((p.cols + p.splits - 1) / p.splits + 31) / 32 * 32;
-    const int rank_blocks = (p.rank + 8 * NBR - 1) / (8 * NBR);
-    if (p.M <= 64) {
-        p.slots = p.adapters + 1 < 16 ? p.adapters + 1 : 16;
-        adapter_shrink_kernel<T, 1, 8, NBR><<<dim3((unsigned)((p.M + 15) / 16), p.splits, p.slots * rank_blocks), 256, 0, st>>>(x, w, p, per_split, h);
-    } else {
-        p.slots = 1;
-        adapter_shrink_kernel<T, 2, 4, NBR><<<dim3((unsigned)((p.M + 31) / 32), p.splits, rank_blocks), 256, 0, st>>>(x, w, p, per_split, h);
-    }
-    return check_launch("adapter_shrink_kernel");
-}
-
-template <typename T>
-int shrink(const void *xv, const void *wv, const AdapterArgs &p, float *h, cudaStream_t st) {
-    const T *x = (const T *)xv, *w = (const T *)wv;
-    if (fast_rank(p.rank) && p.cols % 8 == 0 && aligned_to(x, 16) && aligned_to(w, 16)) {
-        if (p.rank <= 8) return shrink_fast<T, 1>(x, w, p, h, st);
-        if (p.rank <= 16) return shrink_fast<T, 2>(x, w, p, h, st);
-        if (p.rank <= 32) return shrink_fast<T, 4>(x, w, p, h, st);
-        return shrink_fast<T, 8>(x, w, p, h, st);
-    }
-    adapter_shrink_general_kernel<T><<<(unsigned)((p.M * p.rank + 3) / 4), 128, 0, st>>>(x, p.M, p.cols, w, p.adapters, p.rank, p.index, h, p.splits);
-    return check_launch("adapter_shrink_general_kernel");
-}
-
-template <typename T, int SUB, int KS>
-int expand_fast(const float *h, const T *w, const AdapterArgs &p, const T *base, T *out, cudaStream_t st) {
-    const int64_t tiles = (p.M + 16 * SUB - 1) / (16 * SUB), most = (p.cols + 511) / 512;
-    int64_t groups = SUB == 1 ? most : (592 + tiles - 1) / tiles;
-    if (groups > most) groups = most;
-    const size_t smem = (size_t)SUB * ((p.rank + 15) / 16) * 1024;
-    adapter_expand_kernel<T, SUB, KS><<<dim3((unsigned)tiles, (unsigned)groups, p.slots), 256, smem, st>>>(h, w, p, base, out);
-    return check_launch("adapter_expand_kernel");
-}
-
-template <typename T>
-int expand(const float *h, const void *wv, AdapterArgs p, const void *base, void *out, cudaStream_t st) {
-    const T *w = (const T *)wv, *b = (const T *)base;
-    T *o = (T *)out;
-    if (fast_rank(p.rank) && p.cols % 8 == 0 && aligned_to(w, 16) && aligned_to(b, 16) && aligned_to(o, 16)) {
-        if (p.M <= 64) {
-            p.slots = p.adapters + 1 < 16 ? p.adapters + 1 : 16;
-            if (p.rank <= 16) return expand_fast<T, 1, 1>(h, w, p, b, o, st);
-            if (p.rank <= 32) return expand_fast<T, 1, 2>(h, w, p, b, o, st);
-            return expand_fast<T, 1, 4>(h, w, p, b, o, st);
-        }
-        p.slots = 1;
-        if (p.rank <= 16) return expand_fast<T, 4, 1>(h, w, p, b, o, st);
-        if (p.rank <= 32) return expand_fast<T, 4, 2>(h, w, p, b, o, st);
-        return expand_fast<T, 4, 4>(h, w, p, b, o, st);
-    }
-    adapter_expand_general_kernel<T><<<dim3((unsigned)((p.cols + 255) / 256), (unsigned)(p.M < 16384 ? p.M : 16384)), 256, 0, st>>>(
-        h, p.M, p.cols, w, p.adapters, p.rank, p.index, p.scaling, b, o, p.splits);
-    return check_launch("adapter_expand_general_kernel");
-}
-
-template <typename T, int RB>
-int outer_fast(const float *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
-    const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 16 * RB - 1) / (16 * RB));
-    int parts = 1;
-    while (parts < 8 && blocks * rows * parts < 296 && p.M > (int64_t)parts * OUTER_TOKENS) parts *= 2;
-    const size_t sums = (size_t)RB * 16 * 256 * sizeof(float);      // (the fragments, RB * 4 KB, are less)
-    auto kern = adapter_outer_kernel<T, RB>;
-    if (sums > 48 * 1024) BW_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sums));
+template <typename Kern, typename... Args>
+int launch(const char *name, Kern kern, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args) {
+    if (smem > 32 * 1024)      // (48 KB with what the kernel declares)
+        BW_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks, (unsigned)rows, parts);
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = sums;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 1;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = parts;
+    attr[0].val.clusterDim.x = cluster.x;
+    attr[0].val.clusterDim.y = cluster.y;
+    attr[0].val.clusterDim.z = cluster.z;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, h, x, p, dw));
-    return check_launch("adapter_outer_kernel");
+    cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 1 : 0;
+    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+    return check_launch(name);
 }
 
+// Into how many parts the columns of a shrink pass are cut: a power of two up to 8 (the CTAs of a cluster), 256 columns or more each.
+int parts_of(int64_t ctas, int64_t cols) {
+    int s = 1;
+    while (s < 8 && ctas * s < 296 && cols > 256 * s) s *= 2;
+    return s;
+}
+// CTAs among which a tile's adapters are dealt: with few tokens each may be another; prompts are runs of one.
+int slots_of(const AdapterArgs &p) {
+    const int most = p.M <= FEW ? 64 : p.M <= 512 ? 16 : 2;
+    return p.adapters + 1 < most ? p.adapters + 1 : most;
+}
+
+template <typename T, int NBR>
+int shrink_fast(const T *x, const T *w, AdapterArgs p, void *h, cudaStream_t st) {
+    constexpr int RANKS = 8 * NBR;
+    p.slots = slots_of(p);
+    const bool few = p.M <= FEW;
+    const unsigned tiles = (unsigned)((p.M + TILE - 1) / TILE);
+    const int parts = few ? parts_of(p.M < p.slots ? p.M : p.slots, p.cols) : parts_of(tiles, p.cols);
+    const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
+    if (few)
+        return launch("adapter_shrink_few_kernel", adapter_shrink_few_kernel<T, NBR>, dim3(parts, p.slots), 256, 7 * 16 * (RANKS + 1) * 4, dim3(parts), st, x, w, p, per_split, h);
+    constexpr int RING = (TILE + RANKS) * 128 * (NBR <= 8 ? 4 : 3), SUMS = TILE * (RANKS + 4) * 4;
+    return launch("adapter_shrink_kernel", adapter_shrink_kernel<T, NBR>, dim3(parts, tiles, p.slots), 128, RING > SUMS ? RING : SUMS, dim3(parts), st, x, w, p, per_split, h);
+}
 template <typename T>
-int outer(const float *h, const void *xv, const AdapterArgs &p, void *dwv, cudaStream_t st) {
-    const T *x = (const T *)xv;
-    T *dw = (T *)dwv;
-    const int rb = p.rank <= 16 ? 1 : p.rank <= 32 ? 2 : 4;
-    if (fast_rank(p.rank) && p.cols % 8 == 0 && aligned_to(x, 16) && aligned_to(dw, 16) && p.M < INT32_MAX &&
-        (int64_t)p.adapters * ((p.rank + 16 * rb - 1) / (16 * rb)) <= 65535) {
-        if (rb == 1) return outer_fast<T, 1>(h, x, p, dw, st);
-        if (rb == 2) return outer_fast<T, 2>(h, x, p, dw, st);
-        return outer_fast<T, 4>(h, x, p, dw, st);
-    }
+int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStream_t st) {
+    if (p.rank <= 8) return shrink_fast<T, 1>((const T *)x, (const T *)w, p, h, st);
+    if (p.rank <= 16) return shrink_fast<T, 2>((const T *)x, (const T *)w, p, h, st);
+    if (p.rank <= 32) return shrink_fast<T, 4>((const T *)x, (const T *)w, p, h, st);
+    if (p.rank <= 64) return shrink_fast<T, 8>((const T *)x, (const T *)w, p, h, st);
+    return shrink_fast<T, 16>((const T *)x, (const T *)w, p, h, st);
+}
+
+template <typename T, int KS>
+int expand_fast(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaStream_t st) {
+    p.slots = slots_of(p);
+    if (p.M <= FEW)
+        return launch("adapter_expand_few_kernel", adapter_expand_few_kernel<T, KS>, dim3((unsigned)((p.cols + 511) / 512), p.slots), 256, 0, dim3(1), st, h, w, p, base, out);
+    const int64_t tiles = (p.M + TILE - 1) / TILE, blocks = (p.cols + 63) / 64;
+    int64_t groups = 592 / tiles;                                 // CTAs of a wave
+    groups = groups < 1 ? 1 : groups > (blocks + 3) / 4 ? (blocks + 3) / 4 : groups;
+    const int64_t per_group = (blocks + groups - 1) / groups * 64;
+    return launch("adapter_expand_kernel", adapter_expand_kernel<T, KS>, dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), 128,
+                  KS * 16 * 128 * (KS <= 4 ? 4 : 3), dim3(1), st, h, w, p, per_group, base, out);
+}
+template <typename T>
+int expand(void *h, const void *w, const AdapterArgs &p, const void *base, void *out, cudaStream_t st) {
+    if (p.rank <= 16) return expand_fast<T, 1>(h, (const T *)w, p, (const T *)base, (T *)out, st);
+    if (p.rank <= 32) return expand_fast<T, 2>(h, (const T *)w, p, (const T *)base, (T *)out, st);
+    if (p.rank <= 64) return expand_fast<T, 4>(h, (const T *)w, p, (const T *)base, (T *)out, st);
+    return expand_fast<T, 8>(h, (const T *)w, p, (const T *)base, (T *)out, st);
+}
+
+template <typename T, int RB>
+int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
+    const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 16 * RB - 1) / (16 * RB));
+    int parts = 1;
+    while (parts < 8 && blocks * rows * parts < 296 && p.M > (int64_t)parts * 2 * OUTER_STEP) parts *= 2;
+    return launch("adapter_outer_kernel", adapter_outer_kernel<T, RB>, dim3((unsigned)blocks, (unsigned)rows, parts), 128, OuterShape<RB>::SMEM, dim3(1, 1, parts), st, h, x, p, dw);
+}
+template <typename T>
+int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
+    if (p.rank <= 16) return outer_fast<T, 1>(h, (const T *)x, p, (T *)dw, st);
+    if (p.rank <= 32) return outer_fast<T, 2>(h, (const T *)x, p, (T *)dw, st);
+    return outer_fast<T, 4>(h, (const T *)x, p, (T *)dw, st);
+}
+
+// The same three by the general kernels, whose rank values are fp32.
+template <typename T>
+int shrink_general(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStream_t st) {
+    adapter_shrink_general_kernel<T><<<(unsigned)((p.M * p.rank + 3) / 4), 128, 0, st>>>((const T *)x, p.M, p.cols, (const T *)w, p.adapters, p.rank, p.index, (float *)h);
+    return check_launch("adapter_shrink_general_kernel");
+}
+template <typename T>
+int expand_general(void *h, const void *w, const AdapterArgs &p, const void *base, void *out, cudaStream_t st) {
+    adapter_expand_general_kernel<T><<<dim3((unsigned)((p.cols + 255) / 256), (unsigned)(p.M < 16384 ? p.M : 16384)), 256, 0, st>>>(
+        (const float *)h, p.M, p.cols, (const T *)w, p.adapters, p.rank, p.index, p.scaling, (const T *)base, (T *)out);
+    return check_launch("adapter_expand_general_kernel");
+}
+template <typename T>
+int outer_general(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
     adapter_outer_general_kernel<T><<<dim3((unsigned)(p.adapters * p.rank), (unsigned)((p.cols + 255) / 256)), 256, 0, st>>>(
-        h, x, p.M, p.cols, p.rank, p.index, p.scaling, dw, p.splits);
+        (const float *)h, (const T *)x, p.M, p.cols, p.rank, p.index, p.scaling, (T *)dw);
     return check_launch("adapter_outer_general_kernel");
 }
 
-AdapterArgs args_of(int64_t M, int64_t cols, const int32_t *index, const float *scaling, int n, int r, int splits) {
-    return {M, cols, index, scaling, n, r, splits, 1};
+// One form for all passes of an adapter, forward and backward, by sizes alone: what holds the rank values depends on it.
+bool fast_sizes(int64_t M, int64_t N, int64_t K, int n, int r) {
+    return r % 8 == 0 && r <= 128 && K % 8 == 0 && N % 8 == 0 && M < (int64_t)65535 * TILE && (int64_t)n * 2 <= 65535;
 }
 
 template <typename T>
 int forward(const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index, const float *scaling,
-            const void *base, void *out, float *h, cudaStream_t st) {
-    const int splits = shrink_splits(M, K, r);
-    const int rc = shrink<T>(x, down, args_of(M, K, index, nullptr, n, r, splits), h, st);
-    return rc != BW_OK ? rc : expand<T>(h, up, args_of(M, N, index, scaling, n, r, splits), base, out, st);
+            const void *base, void *out, void *h, cudaStream_t st) {
+    const bool fast = fast_sizes(M, N, K, n, r);
+    const AdapterArgs in = {M, K, index, nullptr, n, r, 1}, to = {M, N, index, scaling, n, r, 1};
+    const int rc = fast ? shrink<T>(x, down, in, h, st) : shrink_general<T>(x, down, in, h, st);
+    if (rc != BW_OK) return rc;
+    return fast ? expand<T>(h, up, to, base, out, st) : expand_general<T>(h, up, to, base, out, st);
 }
 template <typename T>
 int backward(const void *dy, const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index,
-             const float *scaling, const float *h, void *dx, void *d_down, void *d_up, float *dh, cudaStream_t st) {
-    const int splits = shrink_splits(M, N, r);
+             const float *scaling, void *h, void *dx, void *d_down, void *d_up, void *dh, cudaStream_t st) {
+    const bool fast = fast_sizes(M, N, K, n, r);
+    const AdapterArgs in = {M, N, index, nullptr, n, r, 1}, over_k = {M, K, index, scaling, n, r, 1}, over_n = {M, N, index, scaling, n, r, 1};
     int rc = BW_OK;
-    if (M > 0 && (dx || d_down)) rc = shrink<T>(dy, up, args_of(M, N, index, nullptr, n, r, splits), dh, st);
-    if (rc == BW_OK && M > 0 && dx) rc = expand<T>(dh, down, args_of(M, K, index, scaling, n, r, splits), nullptr, dx, st);
-    if (rc == BW_OK && d_down) rc = outer<T>(dh, x, args_of(M, K, index, scaling, n, r, splits), d_down, st);
-    if (rc == BW_OK && d_up) rc = outer<T>(h, dy, args_of(M, N, index, scaling, n, r, shrink_splits(M, K, r)), d_up, st);
+    if (M > 0 && (dx || d_down)) rc = fast ? shrink<T>(dy, up, in, dh, st) : shrink_general<T>(dy, up, in, dh, st);
+    if (rc == BW_OK && M > 0 && dx) rc = fast ? expand<T>(dh, down, over_k, nullptr, dx, st) : expand_general<T>(dh, down, over_k, nullptr, dx, st);
+    if (rc == BW_OK && d_down) rc = fast ? outer<T>(dh, x, over_k, d_down, st) : outer_general<T>(dh, x, over_k, d_down, st);
+    if (rc == BW_OK && d_up) rc = fast ? outer<T>(h, dy, over_n, d_up, st) : outer_general<T>(h, dy, over_n, d_up, st);
     return rc;
 }
 
 }  // namespace
 
-size_t adapter_hidden_bytes(int64_t M, int64_t K, int, int r) { return (size_t)M * r * shrink_splits(M, K, r) * sizeof(float); }
-size_t adapter_backward_bytes(int64_t M, int64_t N, int64_t, int, int r) { return (size_t)M * r * shrink_splits(M, N, r) * sizeof(float); }
+// (two 16-bit parts and a power of two a row; the general kernels' fp32 values are less)
+size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * 4 + (size_t)M * 4; }
 
 int adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index,
-                    const float *scaling, const void *base, void *out, float *h, cudaStream_t st) {
+                    const float *scaling, const void *base, void *out, void *h, cudaStream_t st) {
     if (dtype == BW_F16) return forward<__half>(x, M, N, K, down, up, n, r, index, scaling, base, out, h, st);
     return forward<__nv_bfloat16>(x, M, N, K, down, up, n, r, index, scaling, base, out, h, st);
 }
 int adapter_backward(const void *dy, int dtype, const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r,
-                     const int32_t *index, const float *scaling, const float *h, void *dx, void *d_down, void *d_up, void *workspace, cudaStream_t st) {
-    if (dtype == BW_F16) return backward<__half>(dy, x, M, N, K, down, up, n, r, index, scaling, h, dx, d_down, d_up, (float *)workspace, st);
-    return backward<__nv_bfloat16>(dy, x, M, N, K, down, up, n, r, index, scaling, h, dx, d_down, d_up, (float *)workspace, st);
+                     const int32_t *index, const float *scaling, void *h, void *dx, void *d_down, void *d_up, void *workspace, cudaStream_t st) {
+    if (dtype == BW_F16) return backward<__half>(dy, x, M, N, K, down, up, n, r, index, scaling, h, dx, d_down, d_up, workspace, st);
+    return backward<__nv_bfloat16>(dy, x, M, N, K, down, up, n, r, index, scaling, h, dx, d_down, d_up, workspace, st);
 }
 
 }  // namespace bw

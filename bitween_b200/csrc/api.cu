@@ -82,12 +82,11 @@ size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim
 int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *kc, const int32_t *vc,
               const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *table, int64_t table_stride,
               int max_pages, const int32_t *lengths, float alpha, void *out, void *workspace, cudaStream_t st);
-size_t adapter_hidden_bytes(int64_t M, int64_t K, int n, int r);
-size_t adapter_backward_bytes(int64_t M, int64_t N, int64_t K, int n, int r);
+size_t adapter_hidden_bytes(int64_t M, int r);
 int adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index,
-                    const float *scaling, const void *base, void *out, float *h, cudaStream_t st);
+                    const float *scaling, const void *base, void *out, void *h, cudaStream_t st);
 int adapter_backward(const void *dy, int dtype, const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r,
-                     const int32_t *index, const float *scaling, const float *h, void *dx, void *d_down, void *d_up, void *workspace, cudaStream_t st);
+                     const int32_t *index, const float *scaling, void *h, void *dx, void *d_down, void *d_up, void *workspace, cudaStream_t st);
 size_t peer_flag_bytes();
 size_t peer_state_bytes();
 int peer_device_status();
@@ -644,12 +643,7 @@ static int adapter_validate(int dtype, int64_t M, int64_t N, int64_t K, int n, i
     return aligned_to(index, 4) && aligned_to(scaling, 4) ? BW_OK : BW_ERR_ALIGN;
 }
 
-size_t bw_adapter_hidden_bytes(int64_t M, int64_t K, int adapters, int rank) {
-    return M < 1 || K < 1 || adapters < 1 || rank < 1 ? 0 : adapter_hidden_bytes(M, K, adapters, rank);
-}
-size_t bw_adapter_backward_bytes(int64_t M, int64_t N, int64_t K, int adapters, int rank) {
-    return M < 1 || N < 1 || K < 1 || adapters < 1 || rank < 1 ? 0 : adapter_backward_bytes(M, N, K, adapters, rank);
-}
+size_t bw_adapter_hidden_bytes(int64_t M, int rank) { return M < 1 || rank < 1 ? 0 : adapter_hidden_bytes(M, rank); }
 
 int bw_adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int adapters, int rank,
                        const int32_t *index, const float *scaling, const void *base, void *out, void *hidden, size_t hidden_bytes, void *stream) {
@@ -657,11 +651,11 @@ int bw_adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K
     if (rc != BW_OK) return rc;
     if (M == 0) return BW_OK;
     if (!x || !down || !up || !out) return BW_ERR_NULL;
-    if (!aligned_to(x, 2) || !aligned_to(down, 2) || !aligned_to(up, 2) || !aligned_to(base, 2) || !aligned_to(out, 2) || !aligned_to(hidden, 16))
+    if (!aligned_to(x, 16) || !aligned_to(down, 16) || !aligned_to(up, 16) || !aligned_to(base, 16) || !aligned_to(out, 16) || !aligned_to(hidden, 16))
         return BW_ERR_ALIGN;
-    if (!hidden || hidden_bytes < adapter_hidden_bytes(M, K, adapters, rank)) return BW_ERR_WORKSPACE;
+    if (!hidden || hidden_bytes < adapter_hidden_bytes(M, rank)) return BW_ERR_WORKSPACE;
     std::lock_guard<std::mutex> lock(scratch_lock(hidden));
-    return adapter_forward(x, dtype, M, N, K, down, up, adapters, rank, index, scaling, base, out, (float *)hidden, (cudaStream_t)stream);
+    return adapter_forward(x, dtype, M, N, K, down, up, adapters, rank, index, scaling, base, out, hidden, (cudaStream_t)stream);
 }
 
 int bw_adapter_backward(const void *grad_out, int dtype, const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int adapters,
@@ -670,13 +664,14 @@ int bw_adapter_backward(const void *grad_out, int dtype, const void *x, int64_t 
     const int rc = adapter_validate(dtype, M, N, K, adapters, rank, index, scaling);
     if (rc != BW_OK) return rc;
     if (M > 0 && (!grad_out || !x || !down || !up)) return BW_ERR_NULL;
-    if (!aligned_to(grad_out, 2) || !aligned_to(x, 2) || !aligned_to(down, 2) || !aligned_to(up, 2) || !aligned_to(grad_x, 2) || !aligned_to(grad_down, 2) ||
-        !aligned_to(grad_up, 2) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
+    if (!aligned_to(grad_out, 16) || !aligned_to(x, 16) || !aligned_to(down, 16) || !aligned_to(up, 16) || !aligned_to(grad_x, 16) ||
+        !aligned_to(grad_down, 16) || !aligned_to(grad_up, 16) || !aligned_to(hidden, 16) || !aligned_to(workspace, 16))
         return BW_ERR_ALIGN;
-    if (M > 0 && grad_up && (!hidden || hidden_bytes < adapter_hidden_bytes(M, K, adapters, rank))) return BW_ERR_WORKSPACE;
-    if (M > 0 && (!workspace || workspace_bytes < adapter_backward_bytes(M, N, K, adapters, rank))) return BW_ERR_WORKSPACE;
+    const size_t need = M > 0 ? adapter_hidden_bytes(M, rank) : 0;
+    if (need && grad_up && (!hidden || hidden_bytes < need)) return BW_ERR_WORKSPACE;
+    if (need && (!workspace || workspace_bytes < need)) return BW_ERR_WORKSPACE;
     std::lock_guard<std::mutex> lock(scratch_lock(workspace));
-    return adapter_backward(grad_out, dtype, x, M, N, K, down, up, adapters, rank, index, scaling, (const float *)hidden, grad_x, grad_down, grad_up,
+    return adapter_backward(grad_out, dtype, x, M, N, K, down, up, adapters, rank, index, scaling, const_cast<void *>(hidden), grad_x, grad_down, grad_up,
                             workspace, (cudaStream_t)stream);
 }
 

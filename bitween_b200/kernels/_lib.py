@@ -98,12 +98,10 @@ def _declare(L):
     L.bw_kv_attend_workspace_bytes.restype = sz
     L.bw_kv_attend.argtypes = [vp, i32, i64, i32, i64, i64, vp, vp, vp, i32, i64, i32, i32, i32, vp, i64, i64, vp, f32, vp, vp, sz, vp]
     L.bw_kv_attend.restype = i32
-    L.bw_adapter_hidden_bytes.argtypes = [i64, i64, i32, i32]
+    L.bw_adapter_hidden_bytes.argtypes = [i64, i32]
     L.bw_adapter_hidden_bytes.restype = sz
     L.bw_adapter_forward.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp, sz, vp]
     L.bw_adapter_forward.restype = i32
-    L.bw_adapter_backward_bytes.argtypes = [i64, i64, i64, i32, i32]
-    L.bw_adapter_backward_bytes.restype = sz
     L.bw_adapter_backward.argtypes = [vp, i32, vp, i64, i64, i64, vp, vp, i32, i32, vp, vp, vp, sz, vp, vp, vp, vp, sz, vp]
     L.bw_adapter_backward.restype = i32
     L.bw_dequantize.argtypes = [vp, vp, i32, vp, i32, i64, i64, i32, i32, vp, i32, vp]

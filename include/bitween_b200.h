@@ -382,12 +382,14 @@ BW_API int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int6
  * Rows whose index is negative have no adapter: out[t] = base[t].  An index of `adapters` or more gives NaN.
  *   x, down, up, base, out  one dtype, BW_F16 | BW_BF16, dense: x [M][K], down [adapters][rank][K], up [adapters][rank][N] (both
  *                           rank-major), base [M][N] or NULL (zeros), out [M][N], which may be base but not overlap it otherwise
+ *                           All start on 16-byte boundaries.
  *   index    [M] int32       scaling [adapters] fp32 or NULL (ones)
  *   hidden   scratch of bw_adapter_hidden_bytes(...) (16-byte aligned), under the rules of bw_qmatmul's workspace; it holds h, which the
  *            backward call needs again for grad_up
- * Sums are fp32; out is rounded once.  Ranks up to 256.
+ * Sums are fp32; out is rounded once.  Ranks up to 256 (tensor cores: ranks of 8 to 128 and K, N in steps of 8; other sizes run on
+ * slower general kernels).
  */
-BW_API size_t bw_adapter_hidden_bytes(int64_t M, int64_t K, int adapters, int rank);
+BW_API size_t bw_adapter_hidden_bytes(int64_t M, int rank);
 BW_API int bw_adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up,
                        int adapters, int rank, const int32_t *index, const float *scaling, const void *base, void *out,
                        void *hidden, size_t hidden_bytes, void *stream);
@@ -395,9 +397,9 @@ BW_API int bw_adapter_forward(const void *x, int dtype, int64_t M, int64_t N, in
  * Its gradients, each computed where the pointer is not NULL (that of base is grad_out itself):
  *   dh[t] = scaling[i] * up[i] grad_out[t],  grad_x[t] = down[i]^T dh[t],  grad_down[i] = sum dh[t] x[t]^T,
  *   grad_up[i] = scaling[i] * sum h[t] grad_out[t]^T,   sums over the tokens of adapter i, in an order that only the sizes set
+ * workspace: bw_adapter_hidden_bytes(...) as well, 16-byte aligned.
  * Rows without an adapter have grad_x zero, and what stands in their x and grad_out reaches no sum.
  */
-BW_API size_t bw_adapter_backward_bytes(int64_t M, int64_t N, int64_t K, int adapters, int rank);
 BW_API int bw_adapter_backward(const void *grad_out, int dtype, const void *x, int64_t M, int64_t N, int64_t K, const void *down,
                         const void *up, int adapters, int rank, const int32_t *index, const float *scaling,
                         const void *hidden, size_t hidden_bytes, void *grad_x, void *grad_down, void *grad_up,

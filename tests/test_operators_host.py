@@ -50,7 +50,7 @@ def test_adapter_entry_points_check_their_arguments():
     assert forward(M=-1) == 3 and forward(n=0) == 3 and forward(r=0) == 3 and forward(r=257) == 3 and forward(K=0) == 3 and forward(N=1 << 25) == 3
     assert forward(x=None) == 6 and forward(index=None) == 6 and forward(out=None) == 6
     assert forward(x=P + 1) == 5 and forward(index=P + 2) == 5 and forward(hidden=P + 4) == 5
-    assert forward(hidden=None) == 7 and forward(size=L.bw_adapter_hidden_bytes(4, 64, 2, 8) - 1) == 7
+    assert forward(hidden=None) == 7 and forward(size=L.bw_adapter_hidden_bytes(4, 8) - 1) == 7
     assert forward(M=0) == 0
 
     def backward(M=4, x=P, hidden=P, size=1 << 40, ws=P, wsize=1 << 40, dtype=2):
@@ -58,7 +58,7 @@ def test_adapter_entry_points_check_their_arguments():
 
     assert backward(dtype=0) == 4 and backward(M=-1) == 3 and backward(x=None) == 6 and backward(x=P + 1) == 5 and backward(ws=P + 4) == 5
     assert backward(hidden=None) == 7 and backward(size=8) == 7 and backward(ws=None) == 7 and backward(wsize=8) == 7
-    assert L.bw_adapter_hidden_bytes(0, 64, 2, 8) == 0 and L.bw_adapter_backward_bytes(0, 64, 64, 2, 8) == 0
+    assert L.bw_adapter_hidden_bytes(0, 8) == 0 and L.bw_adapter_hidden_bytes(4, 8) == 4 * 8 * 4 + 16
 
 
 def test_cache_refusals():
