@@ -75,6 +75,9 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
     one); an index beyond the bank gives NaN.  `scaling`: fp32 [adapters] or None (ones); it has no gradient.  x, down, up and base share one
     dtype, fp16 or bf16; sums are fp32 and the result is rounded once.  Ranks up to 256.  Differentiable in x, down, up and base.
     `out`, a contiguous tensor of the result's shape, takes the result where no gradient is recorded; it may be `base` itself."""
+    y = (_lib._operators or _lib.host_operators()).adapter_matmul(x, down, up, index, scaling, base, out)
+    if y is not None:
+        return y
     _lib.require_cuda(x, "x")
     if x.dtype not in _DTYPES:
         raise TypeError(f"adapter_matmul: unsupported dtype {x.dtype} (float16/bfloat16)")

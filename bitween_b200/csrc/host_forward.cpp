@@ -1,6 +1,8 @@
-// The host side of QuantizedLinear's forward where no gradient is recorded, in one native call: checks, output
-// allocation and bw_qmatmul on the current stream.  A decode step is launches of a few microseconds each, and in Python
-// the autograd function (7.5 us), the checks, torch.empty and the foreign call took 21 us a layer.
+// The host side of the calls that a decode step makes, each in one native call: checks, output allocation and the library's entry
+// point on the current stream.  Such a step is launches of a few microseconds each.
+//
+// First QuantizedLinear's forward where no gradient is recorded: in Python the autograd function (7.5 us), the checks, torch.empty
+// and the foreign call took 21 us a layer.
 //
 // forward(x, qweight, scale, zero_point, bias, bits, group_size) returns the fp16 output, or None for every call that
 // is not plain: the caller then goes through QuantizedLinearFunction, which converts, records, or raises.  Plain means
@@ -18,6 +20,8 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -125,7 +129,299 @@ PyObject *set_entry(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
 }
 
+// ---- the quantised key-value cache and the adapters ------------------------------------------------------------------
+// None, again, for every call that is not plain (the Python path converts, copies or raises).  Scratch comes from the caching allocator, so
+// that calls of other streams, threads and graphs have their own.
+
+using KvAppend = decltype(&bw_kv_append);
+using KvRead = decltype(&bw_kv_read);
+using KvAttend = decltype(&bw_kv_attend);
+using KvAttendBytes = decltype(&bw_kv_attend_workspace_bytes);
+using AdapterBytes = decltype(&bw_adapter_hidden_bytes);
+using AdapterForward = decltype(&bw_adapter_forward);
+using AdapterBackward = decltype(&bw_adapter_backward);
+struct Operators {
+    KvAppend kv_append;
+    KvRead kv_read;
+    KvAttend kv_attend;
+    KvAttendBytes kv_attend_bytes;
+    AdapterBytes adapter_bytes;
+    AdapterForward adapter_forward;
+    AdapterBackward adapter_backward;
+} g_ops = {};
+
+int float_code(at::ScalarType t) { return t == at::kHalf ? BW_F16 : t == at::kBFloat16 ? BW_BF16 : t == at::kFloat ? BW_F32 : -1; }
+
+// Like plain(), of any strides, and recorded gradients or not.
+bool usable(const at::Tensor *t, const c10::Device &device) {
+    return t && t->defined() && t->layout() == c10::kStrided && t->is_cuda() && t->device() == device && !t->is_neg() && !t->_is_zerotensor() &&
+           !t->key_set().has(c10::DispatchKey::Python) && !t->_fw_grad(/*level=*/0).defined();
+}
+bool dense(const at::Tensor *t, const c10::Device &device) { return usable(t, device) && t->is_contiguous(); }
+bool on_16_bytes(const at::Tensor &t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0; }
+at::Tensor bytes_of(size_t n, const c10::Device &device) {
+    return n ? at::empty({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(device)) : at::Tensor();
+}
+
+// The cache's tensors, arguments 0 to 3 of each of its calls (k_codes, v_codes, params, bits), on the current device.
+struct Cache {
+    const at::Tensor *k = nullptr, *v = nullptr, *params = nullptr;
+    int bits = 0, heads = 0, page_size = 0, dim = 0;
+    int64_t pages = 0;
+    c10::Device device = c10::Device(c10::kCPU);
+    bool of(PyObject *const *args) {
+        k = tensor_of(args[0]);
+        v = tensor_of(args[1]);
+        params = tensor_of(args[2]);
+        if (!k || !v || !params || !PyLong_CheckExact(args[3]) || modes_active()) return false;
+        const long b = PyLong_AsLong(args[3]);
+        if (b != 2 && b != 4 && b != 8) {
+            PyErr_Clear();
+            return false;
+        }
+        bits = (int)b;
+        device = k->device();
+        if (!device.is_cuda() || device.index() != c10::cuda::current_device() || !dense(k, device) || !dense(v, device) || !dense(params, device)) return false;
+        if (k->scalar_type() != at::kInt || v->scalar_type() != at::kInt || params->scalar_type() != at::kHalf) return false;
+        if (k->dim() != 4 || v->sizes() != k->sizes() || params->dim() != 4 || params->size(3) != 4) return false;
+        for (int i = 0; i < 3; ++i)
+            if (params->size(i) != k->size(i) || k->size(i) > INT32_MAX) return false;
+        pages = k->size(0);
+        heads = (int)k->size(1);
+        page_size = (int)k->size(2);
+        if (k->size(3) > 64) return false;
+        dim = (int)k->size(3) * (32 / bits);
+        return true;
+    }
+    int32_t *k_codes() const { return static_cast<int32_t *>(k->mutable_data_ptr()); }
+    int32_t *v_codes() const { return static_cast<int32_t *>(v->mutable_data_ptr()); }
+};
+bool slots_ok(const at::Tensor *slots, const Cache &c) { return dense(slots, c.device) && slots->scalar_type() == at::kLong && slots->dim() == 1; }
+
+// kv_append(k_codes, v_codes, params, bits, k, v, slots): True
+PyObject *kv_append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Cache c;
+    if (nargs != 7 || !g_ops.kv_append || !c.of(args)) Py_RETURN_NONE;
+    const at::Tensor *k = tensor_of(args[4]), *v = tensor_of(args[5]), *slots = tensor_of(args[6]);
+    if (!usable(k, c.device) || !usable(v, c.device) || !slots_ok(slots, c)) Py_RETURN_NONE;
+    const int code = float_code(k->scalar_type());
+    if (code < 0 || v->scalar_type() != k->scalar_type() || k->dim() != 3 || v->sizes() != k->sizes()) Py_RETURN_NONE;
+    if (k->size(0) != slots->size(0) || k->size(1) != c.heads || k->size(2) != c.dim || k->stride(2) != 1 || v->stride(2) != 1) Py_RETURN_NONE;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        rc = g_ops.kv_append(k->const_data_ptr(), v->const_data_ptr(), code, k->size(0), k->stride(0), k->stride(1), v->stride(0), v->stride(1),
+                             static_cast<const int64_t *>(slots->const_data_ptr()), c.heads, c.dim, c.bits, c.pages, c.page_size, c.k_codes(), c.v_codes(),
+                             c.params->mutable_data_ptr(), c10::cuda::getCurrentCUDAStream(c.device.index()).stream());
+    }
+    if (rc != BW_OK) Py_RETURN_NONE;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_read(k_codes, v_codes, params, bits, slots, dtype code): (k, v)
+PyObject *kv_read(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Cache c;
+    if (nargs != 6 || !g_ops.kv_read || !c.of(args)) Py_RETURN_NONE;
+    const at::Tensor *slots = tensor_of(args[4]);
+    const long code = PyLong_CheckExact(args[5]) ? PyLong_AsLong(args[5]) : -1;
+    if (!slots_ok(slots, c) || code < BW_F32 || code > BW_BF16) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    at::Tensor k, v;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const auto options = at::TensorOptions().dtype(code == BW_F32 ? at::kFloat : code == BW_F16 ? at::kHalf : at::kBFloat16).device(c.device);
+        k = at::empty({slots->size(0), c.heads, c.dim}, options);
+        v = at::empty({slots->size(0), c.heads, c.dim}, options);
+        rc = g_ops.kv_read(c.k_codes(), c.v_codes(), c.params->const_data_ptr(), c.heads, c.dim, c.bits, c.pages, c.page_size,
+                           static_cast<const int64_t *>(slots->const_data_ptr()), slots->size(0), k.mutable_data_ptr(), v.mutable_data_ptr(), (int)code,
+                           c10::cuda::getCurrentCUDAStream(c.device.index()).stream());
+    }
+    if (rc != BW_OK) Py_RETURN_NONE;
+    PyObject *pk = THPVariable_Wrap(std::move(k)), *pv = THPVariable_Wrap(std::move(v));
+    return Py_BuildValue("(NN)", pk, pv);
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_attend(k_codes, v_codes, params, bits, q, page_table, lengths, softmax_scale): the attended values
+PyObject *kv_attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Cache c;
+    if (nargs != 8 || !g_ops.kv_attend || !PyFloat_CheckExact(args[7]) || !c.of(args)) Py_RETURN_NONE;
+    const at::Tensor *q = tensor_of(args[4]), *table = tensor_of(args[5]), *lengths = tensor_of(args[6]);
+    if (!usable(q, c.device) || !usable(table, c.device) || !dense(lengths, c.device)) Py_RETURN_NONE;
+    const int code = float_code(q->scalar_type());
+    if ((code != BW_F16 && code != BW_BF16) || table->scalar_type() != at::kInt || lengths->scalar_type() != at::kInt) Py_RETURN_NONE;
+    if (q->dim() != 3 || q->size(2) != c.dim || q->stride(2) != 1 || q->size(1) < 1 || c.heads < 1 || q->size(1) % c.heads || q->size(1) > INT32_MAX) Py_RETURN_NONE;
+    const int64_t batch = q->size(0);
+    if (table->dim() != 2 || table->size(0) != batch || table->stride(1) != 1 || lengths->dim() != 1 || lengths->size(0) != batch) Py_RETURN_NONE;
+    const float scale = (float)PyFloat_AS_DOUBLE(args[7]);
+    at::Tensor out;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const int heads = (int)q->size(1);
+        out = at::empty({batch, heads, c.dim}, q->options());
+        const at::Tensor ws = bytes_of(g_ops.kv_attend_bytes(batch, heads, c.heads, c.dim, c.page_size, table->size(1)), c.device);
+        rc = g_ops.kv_attend(q->const_data_ptr(), code, batch, heads, q->stride(0), q->stride(1), c.k_codes(), c.v_codes(), c.params->const_data_ptr(), c.bits,
+                             c.pages, c.page_size, c.heads, c.dim, static_cast<const int32_t *>(table->const_data_ptr()), table->stride(0), table->size(1),
+                             static_cast<const int32_t *>(lengths->const_data_ptr()), scale, out.mutable_data_ptr(), ws.defined() ? ws.mutable_data_ptr() : nullptr,
+                             ws.defined() ? (size_t)ws.numel() : 0, c10::cuda::getCurrentCUDAStream(c.device.index()).stream());
+    }
+    if (rc != BW_OK) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// One call of bw_adapter_forward; `hidden` is what the backward pass needs again.  x [..., K] and the rest are checked.
+int adapter_call(const at::Tensor &x, const at::Tensor &down, const at::Tensor &up, const at::Tensor &index, const at::Tensor &scaling, const at::Tensor &base,
+                 at::Tensor &out, at::Tensor &hidden) {
+    const int64_t K = down.size(2), N = up.size(2), M = x.numel() / K;
+    const c10::Device device = x.device();
+    if (!out.defined()) {
+        c10::SmallVector<int64_t, 5> sizes(x.sizes().begin(), x.sizes().end());
+        sizes.back() = N;
+        out = at::empty(sizes, at::TensorOptions().dtype(x.scalar_type()).device(device));
+    }
+    hidden = bytes_of(g_ops.adapter_bytes(M, (int)down.size(1)), device);
+    return g_ops.adapter_forward(x.const_data_ptr(), float_code(x.scalar_type()), M, N, K, down.const_data_ptr(), up.const_data_ptr(), (int)down.size(0),
+                                 (int)down.size(1), static_cast<const int32_t *>(index.const_data_ptr()),
+                                 scaling.defined() ? static_cast<const float *>(scaling.const_data_ptr()) : nullptr,
+                                 base.defined() ? base.const_data_ptr() : nullptr, out.mutable_data_ptr(), hidden.mutable_data_ptr(), (size_t)hidden.numel(),
+                                 c10::cuda::getCurrentCUDAStream(device.index()).stream());
+}
+
+// AdapterFunction of the Python package (adapters.py), with the same gradients and the same error where they are differentiated again.
+struct AdapterNode : torch::autograd::Function<AdapterNode> {
+    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &down, const at::Tensor &up, const at::Tensor &index,
+                              const std::optional<at::Tensor> &scaling_or, const std::optional<at::Tensor> &base_or) {
+        at::Tensor out, hidden;
+        const at::Tensor scaling = scaling_or.value_or(at::Tensor()), base = base_or.value_or(at::Tensor());
+        const int rc = adapter_call(x, down, up, index, scaling, base, out, hidden);
+        TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_adapter_forward returned status ", rc);
+        ctx->save_for_backward({x, down, up, index, scaling, up.requires_grad() ? hidden : at::Tensor()});
+        ctx->saved_data["base"] = base.defined();
+        return out;
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x = saved[0], &down = saved[1], &up = saved[2], &index = saved[3], &scaling = saved[4], &hidden = saved[5];
+        at::Tensor g = grads[0], gx, gdown, gup;
+        const bool again = c10::GradMode::is_enabled();
+        {
+            at::AutoGradMode off(false);
+            const int64_t K = down.size(2), N = up.size(2), M = x.numel() / K;
+            const c10::Device device = x.device();
+            at::Tensor dense = g.contiguous();
+            if (!on_16_bytes(dense)) dense = dense.clone();
+            if (ctx->needs_input_grad(0)) gx = at::empty_like(x);
+            if (ctx->needs_input_grad(1)) gdown = at::empty_like(down);
+            if (ctx->needs_input_grad(2)) gup = at::empty_like(up);
+            if (gx.defined() || gdown.defined() || gup.defined()) {
+                const at::Tensor ws = bytes_of(g_ops.adapter_bytes(M, (int)down.size(1)), device);
+                const int rc = g_ops.adapter_backward(
+                    dense.const_data_ptr(), float_code(x.scalar_type()), x.const_data_ptr(), M, N, K, down.const_data_ptr(), up.const_data_ptr(),
+                    (int)down.size(0), (int)down.size(1), static_cast<const int32_t *>(index.const_data_ptr()),
+                    scaling.defined() ? static_cast<const float *>(scaling.const_data_ptr()) : nullptr, hidden.defined() ? hidden.const_data_ptr() : nullptr,
+                    hidden.defined() ? (size_t)hidden.numel() : 0, gx.defined() ? gx.mutable_data_ptr() : nullptr,
+                    gdown.defined() ? gdown.mutable_data_ptr() : nullptr, gup.defined() ? gup.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(),
+                    (size_t)ws.numel(), c10::cuda::getCurrentCUDAStream(device.index()).stream());
+                TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_adapter_backward returned status ", rc);
+            }
+        }
+        torch::autograd::variable_list result = {gx, gdown, gup};
+        if (again) {
+            // as once_differentiable has it: an error for whoever differentiates these
+            for (auto &t : result)
+                if (t.defined()) t = (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", 1))(
+                                     {t.detach().requires_grad_()})[0];
+        }
+        result.insert(result.end(), {at::Tensor(), at::Tensor(), ctx->saved_data["base"].toBool() ? g : at::Tensor()});
+        return result;
+    }
+};
+
+// adapter_matmul(x, down, up, index, scaling, base, out): the result (`out` only where no gradient is recorded)
+PyObject *adapter_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 7 || !g_ops.adapter_forward || modes_active()) Py_RETURN_NONE;
+    const at::Tensor *t[7] = {};
+    for (int i = 0; i < 7; ++i) {
+        if (i >= 4 && args[i] == Py_None) continue;
+        if (!(t[i] = tensor_of(args[i]))) Py_RETURN_NONE;
+    }
+    const at::Tensor *x = t[0], *down = t[1], *up = t[2], *index = t[3], *scaling = t[4], *base = t[5], *given = t[6];
+    const c10::Device device = x->device();
+    if (!device.is_cuda() || device.index() != c10::cuda::current_device()) Py_RETURN_NONE;
+    for (int i = 0; i < 7; ++i)
+        if (t[i] && (!dense(t[i], device) || !(i == 3 || i == 4 || (on_16_bytes(*t[i]) && t[i]->scalar_type() == x->scalar_type())))) Py_RETURN_NONE;
+    const int code = float_code(x->scalar_type());
+    if ((code != BW_F16 && code != BW_BF16) || index->scalar_type() != at::kInt) Py_RETURN_NONE;
+    if (x->dim() < 1 || down->dim() != 3 || up->dim() != 3 || down->size(0) != up->size(0) || down->size(1) != up->size(1)) Py_RETURN_NONE;
+    const int64_t K = down->size(2), N = up->size(2);
+    if (down->size(0) < 1 || down->size(0) > INT32_MAX || down->size(1) < 1 || down->size(1) > 256 || K < 1 || N < 1 || x->size(-1) != K || x->numel() < 1) Py_RETURN_NONE;
+    const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+    if (index->numel() != x->numel() / K || (index->dim() != 1 && index->sizes() != lead)) Py_RETURN_NONE;
+    if (scaling && (scaling->scalar_type() != at::kFloat || scaling->dim() != 1 || scaling->size(0) != down->size(0) || scaling->requires_grad())) Py_RETURN_NONE;
+    for (const at::Tensor *y : {base, given})
+        if (y && (y->dim() != x->dim() || y->sizes().slice(0, x->dim() - 1) != lead || y->size(-1) != N)) Py_RETURN_NONE;
+    const bool recording = c10::GradMode::is_enabled() && (x->requires_grad() || down->requires_grad() || up->requires_grad() || (base && base->requires_grad()));
+    const at::Tensor none;
+    at::Tensor out;
+    if (recording) {
+        if (given) Py_RETURN_NONE;
+        pybind11::gil_scoped_release no_gil;
+        out = AdapterNode::apply(*x, *down, *up, *index, scaling ? std::make_optional(*scaling) : std::nullopt, base ? std::make_optional(*base) : std::nullopt);
+    } else {
+        if (given) {
+            const uintptr_t o = reinterpret_cast<uintptr_t>(given->const_data_ptr());
+            for (const at::Tensor *y : {x, down, up, base}) {
+                const uintptr_t a = y ? reinterpret_cast<uintptr_t>(y->const_data_ptr()) : 0;
+                if (y && a < o + given->nbytes() && o < a + y->nbytes() && !(y == base && a == o)) Py_RETURN_NONE;
+            }
+            if (given->requires_grad()) Py_RETURN_NONE;
+            out = *given;
+        }
+        int rc;
+        {
+            pybind11::gil_scoped_release no_gil;
+            at::Tensor hidden;
+            rc = adapter_call(*x, *down, *up, *index, scaling ? *scaling : none, base ? *base : none, out, hidden);
+        }
+        if (rc != BW_OK) Py_RETURN_NONE;
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// set_operators(addresses of the entry points, in the order of Operators)
+PyObject *set_operators(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    void *p[7];
+    if (nargs != 7) {
+        PyErr_SetString(PyExc_TypeError, "set_operators(seven addresses)");
+        return nullptr;
+    }
+    for (int i = 0; i < 7; ++i) {
+        p[i] = PyLong_AsVoidPtr(args[i]);
+        if (!p[i] && PyErr_Occurred()) return nullptr;
+    }
+    g_ops = {reinterpret_cast<KvAppend>(p[0]),     reinterpret_cast<KvRead>(p[1]),         reinterpret_cast<KvAttend>(p[2]),       reinterpret_cast<KvAttendBytes>(p[3]),
+             reinterpret_cast<AdapterBytes>(p[4]), reinterpret_cast<AdapterForward>(p[5]), reinterpret_cast<AdapterBackward>(p[6])};
+    Py_RETURN_NONE;
+}
+
+#define BW_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
+    BW_METHOD(kv_append),
+    BW_METHOD(kv_read),
+    BW_METHOD(kv_attend),
+    BW_METHOD(adapter_matmul),
+    BW_METHOD(set_operators),
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
     {"set_entry", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(set_entry)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -164,7 +164,13 @@ def _takes_no_call(*args):
     return None
 
 
+class _NoOperators:
+    """Stands for the native host side of the operators where there is none: it takes no call."""
+    kv_append = kv_read = kv_attend = adapter_matmul = staticmethod(_takes_no_call)
+
+
 _host = None
+_operators = None
 # (compiled against torch's C++ interfaces: one for each Python and torch)
 HOST_LIB_PATH = os.path.join(_PKG, "_C", f"_host_forward.{sys.implementation.cache_tag}.torch-{torch.__version__}.so")
 
@@ -173,7 +179,7 @@ def host_forward():
     """The native host side of a layer's forward (csrc/host_forward.cpp), loaded with the library and built with it.
     Where it can be neither loaded nor built (no g++, no torch headers), that is reported once, and what is returned
     takes no call: each goes through the autograd function, to the same kernels."""
-    global _host
+    global _host, _operators
     if _host is None:
         L = lib()
         with _lock:
@@ -186,11 +192,24 @@ def host_forward():
                     module = importlib.util.module_from_spec(spec)
                     spec.loader.exec_module(module)
                     module.set_entry(ctypes.cast(L.bw_qmatmul, ctypes.c_void_p).value, _workspaces)
+                    module.set_operators(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                        L.bw_kv_append, L.bw_kv_read, L.bw_kv_attend, L.bw_kv_attend_workspace_bytes, L.bw_adapter_hidden_bytes,
+                        L.bw_adapter_forward, L.bw_adapter_backward)))
+                    _operators = module
                     _host = module.forward
                 except Exception as e:  # noqa: BLE001
                     warnings.warn(f"bitween_b200: forwards run without the native host side ({e})", stacklevel=2)
+                    _operators = _NoOperators
                     _host = _takes_no_call
     return _host
+
+
+def host_operators():
+    """The native host side of the key-value cache's and the adapters' calls, from the same module: each takes plain calls and
+    answers None to the others."""
+    if _operators is None:
+        host_forward()
+    return _operators
 
 
 def check(status):

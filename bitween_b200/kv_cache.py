@@ -49,11 +49,23 @@ class QuantizedKVCache:
         return cache
 
     def _set_up(self, k_codes, v_codes, params, bits):
-        self.k_codes, self.v_codes, self.params, self.bits = k_codes, v_codes, params, bits
+        self._cache = (k_codes, v_codes, params, bits)
         self.num_pages, self.num_kv_heads, self.page_size = k_codes.shape[:3]
         self.head_dim = k_codes.shape[3] * (32 // bits)
         self.device = k_codes.device
-        self._tensors = (k_codes.data_ptr(), v_codes.data_ptr(), params.data_ptr())
+        self._shapes = (k_codes.shape, v_codes.shape, params.shape)
+        self._softmax_scale = 1.0 / math.sqrt(self.head_dim)
+
+    k_codes = property(lambda self: self._cache[0])
+    v_codes = property(lambda self: self._cache[1])
+    params = property(lambda self: self._cache[2])
+    bits = property(lambda self: self._cache[3])
+
+    def _tensors(self):
+        tensors = self._cache[:3]
+        if tuple(t.shape for t in tensors) != self._shapes or not all(t.is_contiguous() and t.device == self.device for t in tensors):
+            raise RuntimeError("the cache's tensors have been changed in shape or place")
+        return tuple(t.data_ptr() for t in tensors)
 
     def _check_slots(self, slots):
         if slots.dtype != torch.int64 or slots.dim() != 1:
@@ -63,11 +75,12 @@ class QuantizedKVCache:
             raise RuntimeError(f"`slots` is on {slots.device} but the cache is on {self.device}")
         return slots if slots.is_contiguous() else slots.contiguous()
 
-    @torch.no_grad()
     def append(self, k, v, slots):
         """Quantises k[t], v[t] ([tokens, num_kv_heads, head_dim], fp16, bf16 or fp32; any strides of tokens and heads) into slot
         slots[t].  Slots outside the cache are skipped (padding: -1); each slot may be named once in a call.  A row with a NaN or an
         infinity, or whose scale leaves fp16's range, reads back as NaN."""
+        if (_lib._operators or _lib.host_operators()).kv_append(*self._cache, k, v, slots):
+            return
         _lib.require_cuda(self.k_codes, "cache")
         slots = self._check_slots(slots)
         shape = (slots.shape[0], self.num_kv_heads, self.head_dim)
@@ -86,28 +99,29 @@ class QuantizedKVCache:
         L = _lib.lib()
         with _lib.on_device(self.device):
             rc = L.bw_kv_append(k.data_ptr(), v.data_ptr(), _lib.dtype_code(k.dtype), shape[0], k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                                slots.data_ptr(), self.num_kv_heads, self.head_dim, self.bits, self.num_pages, self.page_size, *self._tensors,
+                                slots.data_ptr(), self.num_kv_heads, self.head_dim, self.bits, self.num_pages, self.page_size, *self._tensors(),
                                 _lib.raw_stream(self.device))
         _lib.check(rc)
 
-    @torch.no_grad()
     def read(self, slots, dtype=torch.float16):
         """(k, v) of `slots` as [tokens, num_kv_heads, head_dim] tensors of `dtype` (fp16, bf16 or fp32): the values that the cache
         stands for, rounded once.  Slots outside the cache give zeros."""
         if dtype not in _FLOAT_DTYPES:
             raise TypeError(f"unsupported dtype {dtype}")
+        both = (_lib._operators or _lib.host_operators()).kv_read(*self._cache, slots, _lib.dtype_code(dtype))
+        if both is not None:
+            return both
         _lib.require_cuda(self.k_codes, "cache")
         slots = self._check_slots(slots)
         shape = (slots.shape[0], self.num_kv_heads, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=self.device), torch.empty(shape, dtype=dtype, device=self.device)
         L = _lib.lib()
         with _lib.on_device(self.device):
-            rc = L.bw_kv_read(*self._tensors, self.num_kv_heads, self.head_dim, self.bits, self.num_pages, self.page_size, slots.data_ptr(), shape[0],
+            rc = L.bw_kv_read(*self._tensors(), self.num_kv_heads, self.head_dim, self.bits, self.num_pages, self.page_size, slots.data_ptr(), shape[0],
                               k.data_ptr(), v.data_ptr(), _lib.dtype_code(dtype), _lib.raw_stream(self.device))
         _lib.check(rc)
         return k, v
 
-    @torch.no_grad()
     def attend(self, q, page_table, lengths, softmax_scale=None):
         """Attention of one new token per sequence: q [batch, heads, head_dim] (fp16 or bf16; heads a multiple of num_kv_heads, head h
         reads cache head h // (heads / num_kv_heads)) over the first lengths[b] tokens of the sequence whose pages page_table[b]
@@ -116,6 +130,11 @@ class QuantizedKVCache:
         `softmax_scale` defaults to head_dim ** -0.5.  The new token's own row is attended to if it has been appended and counted.  Sequences
         of length 0 (or less) give zeros.  A length that is more than the table holds, and a page outside the cache within the
         length, give NaN for that sequence; nothing is read there."""
+        if softmax_scale is None:
+            softmax_scale = self._softmax_scale
+        out = (_lib._operators or _lib.host_operators()).kv_attend(*self._cache, q, page_table, lengths, softmax_scale)
+        if out is not None:
+            return out
         _lib.require_cuda(q, "q")
         if q.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"attend: unsupported dtype {q.dtype} (float16/bfloat16)")
@@ -135,14 +154,12 @@ class QuantizedKVCache:
             page_table = page_table.contiguous()
         if not lengths.is_contiguous():
             lengths = lengths.contiguous()
-        if softmax_scale is None:
-            softmax_scale = 1.0 / math.sqrt(self.head_dim)
         out = torch.empty((batch, heads, self.head_dim), dtype=q.dtype, device=self.device)
         L = _lib.lib()
         with _lib.on_device(self.device):
             ws = _lib.workspace(self.device, L.bw_kv_attend_workspace_bytes(batch, heads, self.num_kv_heads, self.head_dim, self.page_size,
                                                                             page_table.shape[1]))
-            rc = L.bw_kv_attend(q.data_ptr(), _lib.dtype_code(q.dtype), batch, heads, q.stride(0), q.stride(1), *self._tensors, self.bits, self.num_pages,
+            rc = L.bw_kv_attend(q.data_ptr(), _lib.dtype_code(q.dtype), batch, heads, q.stride(0), q.stride(1), *self._tensors(), self.bits, self.num_pages,
                                 self.page_size, self.num_kv_heads, self.head_dim, page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
                                 lengths.data_ptr(), softmax_scale, out.data_ptr(), None if ws is None else ws.data_ptr(),
                                 0 if ws is None else ws.numel(), _lib.raw_stream(self.device))
