@@ -20,6 +20,8 @@
 // adapters enter no product.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "bw_common.cuh"
 
 namespace bw {
@@ -137,36 +139,52 @@ template <typename T> struct Hidden {
     __host__ __device__ Hidden(void *p, int64_t M, int r) : top((T *)p), rest(top + M * r), back(reinterpret_cast<float *>(rest + M * r)) {}
 };
 
-// The adapters that occur in a tile of tokens, in the order of their first token; every warp goes through them alike, with a list of their
-// tokens of its own.  Tokens behind the last are in no group.
+// The adapters that occur in a tile of tokens, in the order of their first token, each with a list of its tokens (every warp has its own).  Tokens
+// behind the last are in no group.
 struct TileAdapters {
     int lo, hi;               // of tokens lane and lane + 32
-    unsigned long long todo;
+    unsigned has_lo, has_hi;  // tokens there are
+    bool first_lo, first_hi;  // the lane's tokens are the first of their adapters
+    int rank_lo, rank_hi;     // how many adapters come before them
     uint8_t *list;            // [TILE] places in the tile
-    int count, adapter;
+    int groups, count, adapter;
     __device__ __forceinline__ TileAdapters(const AdapterArgs &p, int64_t t0, uint8_t *list) : list(list) {
         const int lane = threadIdx.x % 32;
+        const unsigned below = (1u << lane) - 1;
         const bool a = t0 + lane < p.M, b = t0 + lane + 32 < p.M;
         lo = a ? __ldg(p.index + t0 + lane) : 0;
         hi = b ? __ldg(p.index + t0 + lane + 32) : 0;
-        todo = __ballot_sync(0xffffffffu, a) | (unsigned long long)__ballot_sync(0xffffffffu, b) << 32;
+        has_lo = __ballot_sync(0xffffffffu, a);
+        has_hi = __ballot_sync(0xffffffffu, b);
+        const unsigned like_lo = __match_any_sync(0xffffffffu, lo), like_hi = __match_any_sync(0xffffffffu, hi);      // (by all lanes)
+        first_lo = a && !(like_lo & has_lo & below);
+        first_hi = b && !(like_hi & has_hi & below);
+        if (has_hi) {         // (then all of the first 32 are there)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (__shfl_sync(0xffffffffu, lo, i) == hi) first_hi = false;
+        }
+        const unsigned f = __ballot_sync(0xffffffffu, first_lo), g = __ballot_sync(0xffffffffu, first_hi);
+        rank_lo = __popc(f & below);
+        rank_hi = __popc(f) + __popc(g & below);
+        groups = __popc(f) + __popc(g);
     }
-    // Takes the next adapter; false when there is none.
-    __device__ __forceinline__ bool next() {
-        if (!todo) return false;
-        const int first = __ffsll((long long)todo) - 1, lane = threadIdx.x % 32;
-        adapter = first < 32 ? __shfl_sync(0xffffffffu, lo, first) : __shfl_sync(0xffffffffu, hi, first - 32);
-        const unsigned long long tokens =
-            todo & (__ballot_sync(0xffffffffu, lo == adapter) | (unsigned long long)__ballot_sync(0xffffffffu, hi == adapter) << 32);
-        todo &= ~tokens;
-        const unsigned a = (unsigned)tokens, b = (unsigned)(tokens >> 32), below = (1u << lane) - 1;
+    // Takes adapter i of `groups`.
+    __device__ __forceinline__ void take(int i) {
+        const int lane = threadIdx.x % 32;
+        const unsigned below = (1u << lane) - 1, f = __ballot_sync(0xffffffffu, first_lo && rank_lo == i), g = __ballot_sync(0xffffffffu, first_hi && rank_hi == i);
+        adapter = f ? __shfl_sync(0xffffffffu, lo, __ffs(f) - 1) : __shfl_sync(0xffffffffu, hi, (__ffs(g) - 1) & 31);
+        const unsigned a = __ballot_sync(0xffffffffu, lo == adapter) & has_lo, b = __ballot_sync(0xffffffffu, hi == adapter) & has_hi;
+        __syncwarp();         // (the list before has been read)
         if (a >> lane & 1) list[__popc(a & below)] = (uint8_t)lane;
         if (b >> lane & 1) list[__popc(a) + __popc(b & below)] = (uint8_t)(lane + 32);
-        count = __popcll(tokens);
+        count = __popc(a) + __popc(b);
         __syncwarp();
-        return true;
     }
 };
+
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // The end of a shrink pass: the CTAs of a cluster have sums of their part of the columns in `sums` [rows][RANKS + 4]; each CTA adds up its share of
 // the rows, a warp a row, and writes them as two 16-bit parts.
@@ -224,13 +242,15 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(const T *__rest
     extern __shared__ float red[];                            // [7][16][RANKS + 1]
     __shared__ uint8_t lists[8][TILE];
     const Hidden<T> h(hidden, p.M, p.rank);
+    pdl_launch_dependents();
     const int64_t begin = blockIdx.x * per_split, end = begin + per_split < p.cols ? begin + per_split : p.cols;
     const int64_t per_warp = (per_split / 32 + 7) / 8 * 32, k0 = begin + warp * per_warp, k1 = k0 + per_warp < end ? k0 + per_warp : end;
 
     TileAdapters tile(p, 0, lists[warp]);
-    for (int i = 0; tile.next(); ++i) {
+    for (int i = blockIdx.y; i < tile.groups; i += p.slots) {
+        tile.take(i);
         const int a = tile.adapter;
-        if (i % p.slots != (int)blockIdx.y || a < 0 || a >= p.adapters) continue;
+        if (a < 0 || a >= p.adapters) continue;
         for (int row0 = 0; row0 < tile.count; row0 += 16) {
             const bool has_a = row0 + r < tile.count, has_b = row0 + r + 8 < tile.count;
             const T *xa = x + (has_a ? tile.list[row0 + r] : 0) * p.cols + c * 8, *xb = x + (has_b ? tile.list[row0 + r + 8] : 0) * p.cols + c * 8;
@@ -281,12 +301,14 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
     __shared__ uint8_t lists[4][TILE];
     const uint32_t ring = smem_addr(smem);
     const Hidden<T> h(hidden, p.M, p.rank);
+    pdl_launch_dependents();
     const int64_t t0 = (int64_t)blockIdx.y * TILE, begin = blockIdx.x * per_split, end = begin + per_split < p.cols ? begin + per_split : p.cols;
 
     TileAdapters tile(p, t0, lists[warp]);
-    for (int i = 0; tile.next(); ++i) {
+    for (int i = blockIdx.z; i < tile.groups; i += p.slots) {
+        tile.take(i);
         const int a = tile.adapter;
-        if (i % p.slots != (int)blockIdx.z || a < 0 || a >= p.adapters) continue;
+        if (a < 0 || a >= p.adapters) continue;
         // a thread copies piece threadIdx % 8 of every 16th row
         const int piece = threadIdx.x % 8;
         const T *rows[4];
@@ -355,7 +377,7 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
 
 // ---- expand --------------------------------------------------------------------------------------------------------------
 
-// Fragments of the rank values of 16 rows: [steps][value and rest].
+// Fragments of the rank values of 16 rows: [steps][value and rest].  (From L2: a kernel that was launched early has been there while they were made.)
 template <typename T, int KS>
 __device__ __forceinline__ void load_rank_values(const Hidden<T> &h, int rank, int64_t ta, int64_t tb, bool has_a, bool has_b, int c, uint32_t (&top)[KS][4], uint32_t (&rest)[KS][4]) {
 #pragma unroll
@@ -365,8 +387,8 @@ __device__ __forceinline__ void load_rank_values(const Hidden<T> &h, int rank, i
             const int j = 16 * ks + 2 * c + e / 2 * 8;
             const bool has = (e % 2 ? has_b : has_a) && j < rank;
             const int64_t at = (e % 2 ? tb : ta) * rank + j;
-            top[ks][e] = has ? __ldg(reinterpret_cast<const uint32_t *>(h.top + at)) : 0u;
-            rest[ks][e] = has ? __ldg(reinterpret_cast<const uint32_t *>(h.rest + at)) : 0u;
+            top[ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.top + at)) : 0u;
+            rest[ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.rest + at)) : 0u;
         }
 }
 // What a row's product is multiplied by.
@@ -374,7 +396,7 @@ template <typename T>
 __device__ __forceinline__ float row_factor(const Hidden<T> &h, const AdapterArgs &p, int a, int64_t t, bool has) {
     if (a < 0 || !has) return 0.0f;
     if (a >= p.adapters) return NAN;
-    return (__is_same(T, __half) ? __ldg(h.back + t) : 1.0f) * (p.scaling ? __ldg(p.scaling + a) : 1.0f);
+    return (__is_same(T, __half) ? __ldcg(h.back + t) : 1.0f) * (p.scaling ? __ldg(p.scaling + a) : 1.0f);
 }
 // base + f * product, 16 neighbouring columns of two rows; `old` is base (zeros without one).
 template <typename T>
@@ -396,17 +418,18 @@ __device__ __forceinline__ void store_rows(T *const (&to)[2], const bool (&live)
 // out[t] = base[t] + f * (h[t] times w) of a few tokens: a CTA an adapter and 512 columns, a warp 64 of them; w straight from global memory, KS steps
 // of 16 ranks at once.
 template <typename T, int KS>
-__global__ void __launch_bounds__(256) adapter_expand_few_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, const T *base, T *out) {
+__global__ void __launch_bounds__(128) adapter_expand_few_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, const T *base, T *out) {
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
-    __shared__ uint8_t lists[8][TILE];
+    __shared__ uint8_t lists[4][TILE];
     const Hidden<T> h(hidden, p.M, p.rank);
-    const int64_t cb = ((int64_t)blockIdx.x * 8 + warp) * 64, col = cb + r * 8;
-    if (cb >= p.cols) return;
+    const int64_t cb = ((int64_t)blockIdx.x * 4 + warp) * 64, col = cb + r * 8;
     const bool in[2] = {cb + 16 * c < p.cols, cb + 16 * c + 8 < p.cols};
     TileAdapters tile(p, 0, lists[warp]);
-    for (int i = 0; tile.next(); ++i) {
+    bool waited = false;
+    for (int i = blockIdx.y; i < tile.groups; i += p.slots) {
+        tile.take(i);
         const int a = tile.adapter;
-        if (i % p.slots != (int)blockIdx.y || (a < 0 && base == out)) continue;
+        if (a < 0 && base == out) continue;
         const bool has = a >= 0 && a < p.adapters;
         uint4 raw[KS][4];
 #pragma unroll
@@ -416,6 +439,8 @@ __global__ void __launch_bounds__(256) adapter_expand_few_kernel(void *hidden, c
                 const int j = 16 * ks + 2 * c + k % 2 + k / 2 * 8;
                 raw[ks][k] = load16_if(w + ((int64_t)(has ? a : 0) * p.rank + j) * p.cols + col, has && col < p.cols && j < p.rank);
             }
+        if (!waited) pdl_wait();                  // (what comes before is the launch that makes the rank values; all that came before that is done)
+        waited = true;
         for (int row0 = 0; row0 < tile.count; row0 += 16) {
             const bool live[2] = {row0 + r < tile.count, row0 + r + 8 < tile.count};
             const int64_t t[2] = {live[0] ? tile.list[row0 + r] : 0, live[1] ? tile.list[row0 + r + 8] : 0};
@@ -442,35 +467,52 @@ __global__ void __launch_bounds__(256) adapter_expand_few_kernel(void *hidden, c
             store_rows<T>(to, live, in, old, acc, f, a < 0);
         }
     }
+    if (!waited) pdl_wait();                      // a grid that was launched early is not done before the one in front of it
 }
 
-// The same of many tokens: 64 rows of one adapter, 16 a warp with their rank values in registers; blocks of 64 columns of w go through a ring in shared
-// memory, and the rows of base are loaded a block ahead.
+// The same of many tokens: 64 rows of one adapter, 16 a warp with their rank values in registers; blocks of 64 columns of w and of base go through
+// a ring in shared memory.
 template <typename T, int KS>
 __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, int64_t per_group, const T *base, T *out) {
-    constexpr int STAGE = KS * 16 * 128, STAGES = KS <= 4 ? 4 : 3;
+    constexpr int W_BYTES = KS * 16 * 128, STAGE = W_BYTES + TILE * 128, STAGES = KS <= 4 ? 4 : 3;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint8_t lists[4][TILE];
     const uint32_t ring = smem_addr(smem);
     const Hidden<T> h(hidden, p.M, p.rank);
+    pdl_launch_dependents();
     const int64_t t0 = (int64_t)blockIdx.x * TILE, begin = blockIdx.y * per_group, end = begin + per_group < p.cols ? begin + per_group : p.cols;
 
     TileAdapters tile(p, t0, lists[warp]);
-    for (int i = 0; tile.next(); ++i) {
+    pdl_wait();                                   // (what comes before is the launch that makes the rank values, or one behind it)
+    for (int i = blockIdx.z; i < tile.groups; i += p.slots) {
+        tile.take(i);
         const int a = tile.adapter;
-        if (i % p.slots != (int)blockIdx.z || (a < 0 && base == out)) continue;
+        if (a < 0 && base == out) continue;
         const bool has = a >= 0 && a < p.adapters;
-        const T *wrow = w + ((int64_t)(has ? a : 0) * p.rank + threadIdx.x / 8) * p.cols + threadIdx.x % 8 * 8;
-        auto copy_stage = [&](int64_t cb, int stage) {
-            if (cb < end && has) {
-                const bool in = cb + threadIdx.x % 8 * 8 < p.cols;
+        // a thread copies piece threadIdx % 8 of every 16th row of w and of base
+        const int piece = threadIdx.x % 8, row0 = threadIdx.x / 8;
+        const T *wrow = w + ((int64_t)(has ? a : 0) * p.rank + row0) * p.cols + piece * 8;
+        const T *rows[4];
+        bool here[4];
 #pragma unroll
-                for (int j = 0; j < KS; ++j) {
-                    const int row = threadIdx.x / 8 + 16 * j;
-                    const bool ok = in && row < p.rank;
-                    copy16(ring + stage * STAGE + row * 128 + ((threadIdx.x % 8) ^ (row >> 1 & 3) << 1) * 16, ok ? wrow + 16 * j * p.cols + cb : w, ok);
+        for (int j = 0; j < 4; ++j) {
+            here[j] = base && row0 + 16 * j < tile.count;
+            rows[j] = here[j] ? base + (t0 + tile.list[row0 + 16 * j]) * p.cols + piece * 8 : w;
+        }
+        auto copy_stage = [&](int64_t cb, int stage) {
+            if (cb < end) {
+                const bool in = cb + piece * 8 < p.cols;
+                const uint32_t to = ring + stage * STAGE + row0 * 128;
+                if (has) {
+#pragma unroll
+                    for (int j = 0; j < KS; ++j) {
+                        const bool ok = in && row0 + 16 * j < p.rank;
+                        copy16(to + j * 2048 + (piece ^ (row0 >> 1 & 3) << 1) * 16, ok ? wrow + 16 * j * p.cols + cb : w, ok);
+                    }
                 }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) copy16(to + W_BYTES + j * 2048 + (piece ^ (row0 & 7)) * 16, in && here[j] ? rows[j] + cb : w, in && here[j]);
             }
             copies_commit();
         };
@@ -483,24 +525,15 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
         uint32_t top[KS][4], rest[KS][4];
         load_rank_values<T, KS>(h, p.rank, t[0], t[1], live[0] && has, live[1] && has, c, top, rest);
         const float f[2] = {row_factor(h, p, a, t[0], live[0]), row_factor(h, p, a, t[1], live[1])};
-        auto load_base = [&](int64_t cb, uint4 (&v)[2][2]) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                v[j / 2][j % 2] = base && live[j / 2] && cb < end && cb + 16 * c + j % 2 * 8 < p.cols
-                                      ? *reinterpret_cast<const uint4 *>(base + t[j / 2] * p.cols + cb + 16 * c + j % 2 * 8) : make_uint4(0, 0, 0, 0);
-        };
-        uint4 old[2][2], ahead[2][2];
-        load_base(begin, old);
         int stage = 0;
         const bool busy = warp * 16 < tile.count;
         for (int64_t cb = begin; cb < end; cb += 64) {
             copies_wait<STAGES - 2>();
             __syncthreads();
             copy_stage(cb + (STAGES - 1) * 64, stage == 0 ? STAGES - 1 : stage - 1);
-            const uint32_t ws = ring + stage * STAGE;
+            const uint32_t ws = ring + stage * STAGE, bs = ws + W_BYTES + row * 128;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             if (!busy) continue;
-            load_base(cb + 64, ahead);
             float acc[8][4] = {};
             if (has) {
 #pragma unroll
@@ -519,11 +552,12 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
                     }
                 }
             }
+            uint4 old[2][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) old[j / 2][j % 2] = load_shared16(bs + j / 2 * 1024 + ((2 * c + j % 2) ^ (row & 7)) * 16);
             T *const to[2] = {out + t[0] * p.cols + cb + 16 * c, out + t[1] * p.cols + cb + 16 * c};
             const bool in[2] = {cb + 16 * c < p.cols, cb + 16 * c + 8 < p.cols};
             store_rows<T>(to, live, in, old, acc, f, a < 0);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) old[j / 2][j % 2] = ahead[j / 2][j % 2];
         }
         copies_wait<0>();
         __syncthreads();
@@ -557,6 +591,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
     __shared__ int list[OUTER_LIST], s_count[4];
     __shared__ float s_back[OUTER_LIST], s_big[4];
 
+    pdl_launch_dependents();
     // the adapter's tokens before this warp's quarter of all, and in all
     const int64_t quarter = (p.M + 127) / 128 * 32, q0 = warp * quarter, q1 = q0 + quarter < p.M ? q0 + quarter : p.M;
     int count = 0;
@@ -569,6 +604,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
         before += i < warp ? s_count[i] : 0;
         all += s_count[i];
     }
+    pdl_wait();                                                  // (the rank values are made by one of the launches before)
     const int share = (all + gridDim.z - 1) / gridDim.z, lo = blockIdx.z * share, hi = lo + share < all ? lo + share : all;
 
     float acc[RB][8][4] = {};
@@ -614,7 +650,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
             // powers of two of the rows, relative to the largest
             float most = 0.0f;
             for (int j = threadIdx.x; j < n; j += 128) {
-                s_back[j] = __ldg(h.back + list[j]);
+                s_back[j] = __ldcg(h.back + list[j]);
                 most = fmaxf(most, s_back[j]);
             }
             for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
@@ -720,50 +756,86 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
 
 constexpr int64_t FEW = TILE;       // tokens up to which each adapter has CTAs of its own
 
-template <typename Kern, typename... Args>
-int launch(const char *name, Kern kern, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args) {
+// What a kernel needs to know of a device once: its shared memory asked for, and how many of its CTAs an SM holds.
+template <auto KERN>
+int ctas_per_sm(int threads, int smem, int &n) {
+    static std::atomic<int> known[64];
+    int device = 0;
+    BW_CUDA_TRY(cudaGetDevice(&device));
+    n = device < 64 ? known[device].load(std::memory_order_relaxed) : 0;
+    if (n) return BW_OK;
     if (smem > 32 * 1024)      // (48 KB with what the kernel declares)
-        BW_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        BW_CUDA_TRY(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    BW_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERN, threads, smem));
+    if (n < 1) n = 1;
+    if (device < 64) known[device].store(n, std::memory_order_relaxed);
+    return BW_OK;
+}
+constexpr int SMS = 148;
+
+// `early`: the kernel may start while the one before it still runs (it waits for that itself).
+template <auto KERN, typename... Args>
+int launch(const char *name, dim3 grid, int threads, int smem, dim3 cluster, bool early, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster.x;
-    attr[0].val.clusterDim.y = cluster.y;
-    attr[0].val.clusterDim.z = cluster.z;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = cluster.x * cluster.y * cluster.z > 1 ? 1 : 0;
-    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+    if (cluster.x * cluster.y * cluster.z > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster.x;
+        attr[cfg.numAttrs].val.clusterDim.y = cluster.y;
+        attr[cfg.numAttrs++].val.clusterDim.z = cluster.z;
+    }
+    if (early) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, KERN, args...));
     return check_launch(name);
 }
 
-// Into how many parts the columns of a shrink pass are cut: a power of two up to 8 (the CTAs of a cluster), 256 columns or more each.
-int parts_of(int64_t ctas, int64_t cols) {
-    int s = 1;
-    while (s < 8 && ctas * s < 296 && cols > 256 * s) s *= 2;
-    return s;
+// Into how many parts, up to `most`, `ctas` pieces of work are cut where `at_once` fit on the chip: as few rounds of as short parts as can be.  A part
+// costs `fixed` of an uncut piece's time on top.
+int parts_of(int64_t ctas, int64_t at_once, int64_t most, double fixed) {
+    int best = 1;
+    double least = 0.0;
+    for (int s = 1; s <= most; ++s) {
+        const double time = (double)((ctas * s + at_once - 1) / at_once) * (1.0 / s + fixed);
+        if (s == 1 || time < least) {
+            least = time;
+            best = s;
+        }
+    }
+    return best;
 }
 // CTAs among which a tile's adapters are dealt: with few tokens each may be another; prompts are runs of one.
 int slots_of(const AdapterArgs &p) {
-    const int most = p.M <= FEW ? 64 : p.M <= 512 ? 16 : 2;
-    return p.adapters + 1 < most ? p.adapters + 1 : most;
+    const int most = p.M <= FEW ? 64 : p.M <= 512 ? 16 : 2, tokens = p.M < TILE ? (int)p.M : TILE;
+    const int n = p.adapters + 1 < tokens ? p.adapters + 1 : tokens;
+    return n < most ? n : most;
 }
 
 template <typename T, int NBR>
 int shrink_fast(const T *x, const T *w, AdapterArgs p, void *h, cudaStream_t st) {
-    constexpr int RANKS = 8 * NBR;
+    constexpr int RANKS = 8 * NBR, FEW_SMEM = 7 * 16 * (RANKS + 1) * 4, RING = (TILE + RANKS) * 128 * (NBR <= 8 ? 4 : 3), SUMS = TILE * (RANKS + 4) * 4,
+                  SMEM = RING > SUMS ? RING : SUMS;
     p.slots = slots_of(p);
-    const bool few = p.M <= FEW;
+    const int64_t most = (p.cols + 255) / 256;                    // (a part has 256 columns at least; a cluster 8 CTAs at most)
     const unsigned tiles = (unsigned)((p.M + TILE - 1) / TILE);
-    const int parts = few ? parts_of(p.M < p.slots ? p.M : p.slots, p.cols) : parts_of(tiles, p.cols);
+    int per_sm = 0, rc;
+    if (p.M <= FEW) {
+        if ((rc = ctas_per_sm<adapter_shrink_few_kernel<T, NBR>>(256, FEW_SMEM, per_sm)) != BW_OK) return rc;
+        const int parts = most < 8 ? (int)most : 8;
+        const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
+        return launch<adapter_shrink_few_kernel<T, NBR>>("adapter_shrink_few_kernel", dim3(parts, p.slots), 256, FEW_SMEM, dim3(parts), false, st, x, w, p, per_split, h);
+    }
+    if ((rc = ctas_per_sm<adapter_shrink_kernel<T, NBR>>(128, SMEM, per_sm)) != BW_OK) return rc;
+    const int parts = parts_of(tiles, SMS * per_sm, most < 8 ? most : 8, 0.02);
     const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
-    if (few)
-        return launch("adapter_shrink_few_kernel", adapter_shrink_few_kernel<T, NBR>, dim3(parts, p.slots), 256, 7 * 16 * (RANKS + 1) * 4, dim3(parts), st, x, w, p, per_split, h);
-    constexpr int RING = (TILE + RANKS) * 128 * (NBR <= 8 ? 4 : 3), SUMS = TILE * (RANKS + 4) * 4;
-    return launch("adapter_shrink_kernel", adapter_shrink_kernel<T, NBR>, dim3(parts, tiles, p.slots), 128, RING > SUMS ? RING : SUMS, dim3(parts), st, x, w, p, per_split, h);
+    return launch<adapter_shrink_kernel<T, NBR>>("adapter_shrink_kernel", dim3(parts, tiles, p.slots), 128, SMEM, dim3(parts), false, st, x, w, p, per_split, h);
 }
 template <typename T>
 int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStream_t st) {
@@ -776,15 +848,18 @@ int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStre
 
 template <typename T, int KS>
 int expand_fast(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaStream_t st) {
+    constexpr int SMEM = (KS * 16 + TILE) * 128 * (KS <= 4 ? 4 : 3);
     p.slots = slots_of(p);
     if (p.M <= FEW)
-        return launch("adapter_expand_few_kernel", adapter_expand_few_kernel<T, KS>, dim3((unsigned)((p.cols + 511) / 512), p.slots), 256, 0, dim3(1), st, h, w, p, base, out);
-    const int64_t tiles = (p.M + TILE - 1) / TILE, blocks = (p.cols + 63) / 64;
-    int64_t groups = 592 / tiles;                                 // CTAs of a wave
-    groups = groups < 1 ? 1 : groups > (blocks + 3) / 4 ? (blocks + 3) / 4 : groups;
+        return launch<adapter_expand_few_kernel<T, KS>>("adapter_expand_few_kernel", dim3((unsigned)((p.cols + 255) / 256), p.slots), 128, 0, dim3(1), true, st, h, w, p, base, out);
+    int per_sm = 0;
+    const int rc = ctas_per_sm<adapter_expand_kernel<T, KS>>(128, SMEM, per_sm);
+    if (rc != BW_OK) return rc;
+    const int64_t tiles = (p.M + TILE - 1) / TILE, blocks = (p.cols + 63) / 64, most = (blocks + 1) / 2;
+    const int groups = parts_of(tiles, SMS * per_sm, most < 64 ? most : 64, 3.0 / blocks);
     const int64_t per_group = (blocks + groups - 1) / groups * 64;
-    return launch("adapter_expand_kernel", adapter_expand_kernel<T, KS>, dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), 128,
-                  KS * 16 * 128 * (KS <= 4 ? 4 : 3), dim3(1), st, h, w, p, per_group, base, out);
+    return launch<adapter_expand_kernel<T, KS>>("adapter_expand_kernel", dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), 128, SMEM, dim3(1), true, st,
+                                                h, w, p, per_group, base, out);
 }
 template <typename T>
 int expand(void *h, const void *w, const AdapterArgs &p, const void *base, void *out, cudaStream_t st) {
@@ -795,17 +870,19 @@ int expand(void *h, const void *w, const AdapterArgs &p, const void *base, void 
 }
 
 template <typename T, int RB>
-int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
-    const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 16 * RB - 1) / (16 * RB));
-    int parts = 1;
-    while (parts < 8 && blocks * rows * parts < 296 && p.M > (int64_t)parts * 2 * OUTER_STEP) parts *= 2;
-    return launch("adapter_outer_kernel", adapter_outer_kernel<T, RB>, dim3((unsigned)blocks, (unsigned)rows, parts), 128, OuterShape<RB>::SMEM, dim3(1, 1, parts), st, h, x, p, dw);
+int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, bool early, cudaStream_t st) {
+    const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 16 * RB - 1) / (16 * RB)), most = (p.M + 2 * OUTER_STEP - 1) / (2 * OUTER_STEP);
+    int per_sm = 0;
+    const int rc = ctas_per_sm<adapter_outer_kernel<T, RB>>(128, OuterShape<RB>::SMEM, per_sm);
+    if (rc != BW_OK) return rc;
+    const int parts = parts_of(blocks * rows, SMS * per_sm, most < 8 ? most : 8, 0.02);
+    return launch<adapter_outer_kernel<T, RB>>("adapter_outer_kernel", dim3((unsigned)blocks, (unsigned)rows, parts), 128, OuterShape<RB>::SMEM, dim3(1, 1, parts), early, st, h, x, p, dw);
 }
 template <typename T>
-int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
-    if (p.rank <= 16) return outer_fast<T, 1>(h, (const T *)x, p, (T *)dw, st);
-    if (p.rank <= 32) return outer_fast<T, 2>(h, (const T *)x, p, (T *)dw, st);
-    return outer_fast<T, 4>(h, (const T *)x, p, (T *)dw, st);
+int outer(void *h, const void *x, const AdapterArgs &p, void *dw, bool early, cudaStream_t st) {
+    if (p.rank <= 16) return outer_fast<T, 1>(h, (const T *)x, p, (T *)dw, early, st);
+    if (p.rank <= 32) return outer_fast<T, 2>(h, (const T *)x, p, (T *)dw, early, st);
+    return outer_fast<T, 4>(h, (const T *)x, p, (T *)dw, early, st);
 }
 
 // The same three by the general kernels, whose rank values are fp32.
@@ -847,10 +924,12 @@ int backward(const void *dy, const void *x, int64_t M, int64_t N, int64_t K, con
     const bool fast = fast_sizes(M, N, K, n, r);
     const AdapterArgs in = {M, N, index, nullptr, n, r, 1}, over_k = {M, K, index, scaling, n, r, 1}, over_n = {M, N, index, scaling, n, r, 1};
     int rc = BW_OK;
+    bool early = false;            // (behind a launch of this call: what those read and write was there before the first)
     if (M > 0 && (dx || d_down)) rc = fast ? shrink<T>(dy, up, in, dh, st) : shrink_general<T>(dy, up, in, dh, st);
+    early = fast && M > 0 && (dx || d_down);
     if (rc == BW_OK && M > 0 && dx) rc = fast ? expand<T>(dh, down, over_k, nullptr, dx, st) : expand_general<T>(dh, down, over_k, nullptr, dx, st);
-    if (rc == BW_OK && d_down) rc = fast ? outer<T>(dh, x, over_k, d_down, st) : outer_general<T>(dh, x, over_k, d_down, st);
-    if (rc == BW_OK && d_up) rc = fast ? outer<T>(h, dy, over_n, d_up, st) : outer_general<T>(h, dy, over_n, d_up, st);
+    if (rc == BW_OK && d_down) rc = fast ? outer<T>(dh, x, over_k, d_down, early, st) : outer_general<T>(dh, x, over_k, d_down, st);
+    if (rc == BW_OK && d_up) rc = fast ? outer<T>(h, dy, over_n, d_up, early, st) : outer_general<T>(h, dy, over_n, d_up, st);
     return rc;
 }
 
