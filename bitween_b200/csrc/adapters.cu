@@ -511,8 +511,10 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
                         copy16(to + j * 2048 + (piece ^ (row0 >> 1 & 3) << 1) * 16, ok ? wrow + 16 * j * p.cols + cb : w, ok);
                     }
                 }
+                if (base) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) copy16(to + W_BYTES + j * 2048 + (piece ^ (row0 & 7)) * 16, in && here[j] ? rows[j] + cb : w, in && here[j]);
+                    for (int j = 0; j < 4; ++j) copy16(to + W_BYTES + j * 2048 + (piece ^ (row0 & 7)) * 16, in && here[j] ? rows[j] + cb : w, in && here[j]);
+                }
             }
             copies_commit();
         };
@@ -554,7 +556,7 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
             }
             uint4 old[2][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) old[j / 2][j % 2] = load_shared16(bs + j / 2 * 1024 + ((2 * c + j % 2) ^ (row & 7)) * 16);
+            for (int j = 0; j < 4; ++j) old[j / 2][j % 2] = base ? load_shared16(bs + j / 2 * 1024 + ((2 * c + j % 2) ^ (row & 7)) * 16) : make_uint4(0, 0, 0, 0);
             T *const to[2] = {out + t[0] * p.cols + cb + 16 * c, out + t[1] * p.cols + cb + 16 * c};
             const bool in[2] = {cb + 16 * c < p.cols, cb + 16 * c + 8 < p.cols};
             store_rows<T>(to, live, in, old, acc, f, a < 0);
@@ -568,39 +570,42 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
 
 constexpr int OUTER_LIST = 2048, OUTER_STEP = 32;
 
-template <int RB> struct OuterShape {
-    static constexpr int RANKS = 16 * RB, ROW = RANKS * 2;                    // bytes of a token's rank values
-    static constexpr int STAGE = OUTER_STEP * (512 + 2 * ROW), STAGES = RB <= 2 ? 4 : 3;
+// RB blocks of 16 ranks a warp, RG groups of four warps with ranks of their own.
+template <int RB, int RG> struct OuterShape {
+    static constexpr int WARPS = 4 * RG, THREADS = 32 * WARPS;
+    static constexpr int RANKS = 16 * RB * RG, ROW = RANKS * 2;               // bytes of a token's rank values
+    static constexpr int STAGE = OUTER_STEP * (512 + 2 * ROW), STAGES = RG == 1 ? 4 : 3;
     static constexpr int SUMS = RANKS * 256 * 4, SMEM = STAGE * STAGES > SUMS ? STAGE * STAGES : SUMS;
     static __device__ __forceinline__ int swizzle(int token) { return ROW >= 128 ? token & 7 : ROW == 64 ? token >> 1 & 3 : token >> 2 & 1; }
 };
 
-// dw[a][rank0 .. + 16 RB][256 columns] = f_a * sum over the adapter's tokens of h[t] x[t]^T.  The CTAs of a cluster (blockIdx.z) take equal shares of
+// dw[a][rank0 .. + RANKS][256 columns] = f_a * sum over the adapter's tokens of h[t] x[t]^T.  The CTAs of a cluster (blockIdx.z) take equal shares of
 // the tokens and add their sums through each other's shared memory.  Rows of x and of the rank values go through a ring, 32 tokens a stage.
-template <typename T, int RB>
-__global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
-    using S = OuterShape<RB>;
+// (64 ranks in one warp's registers leave eight warps an SM: 143 us for OUTER_CASE; in two warps, sixteen: OUTER_US.)
+template <typename T, int RB, int RG>
+__global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
+    using S = OuterShape<RB, RG>;
     constexpr bool F16 = __is_same(T, __half);
-    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4, wc = warp % 4, wr = warp / 4;
     const int rank_blocks = (p.rank + S::RANKS - 1) / S::RANKS, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * S::RANKS;
     const int64_t col0 = (int64_t)blockIdx.x * 256;
     extern __shared__ __align__(128) uint8_t smem[];
     float *sums = reinterpret_cast<float *>(smem);               // [RANKS][256], at the end
     const uint32_t ring = smem_addr(smem);
     const Hidden<T> h(hidden, p.M, p.rank);
-    __shared__ int list[OUTER_LIST], s_count[4];
-    __shared__ float s_back[OUTER_LIST], s_big[4];
+    __shared__ int list[OUTER_LIST], s_count[S::WARPS];
+    __shared__ float s_back[OUTER_LIST], s_big[S::WARPS];
 
     pdl_launch_dependents();
-    // the adapter's tokens before this warp's quarter of all, and in all
-    const int64_t quarter = (p.M + 127) / 128 * 32, q0 = warp * quarter, q1 = q0 + quarter < p.M ? q0 + quarter : p.M;
+    // the adapter's tokens before this warp's part of all, and in all
+    const int64_t part = (p.M + S::THREADS - 1) / S::THREADS * 32, q0 = warp * part, q1 = q0 + part < p.M ? q0 + part : p.M;
     int count = 0;
 #pragma unroll 4
     for (int64_t t = q0; t < q1; t += 32) count += __popc(__ballot_sync(0xffffffffu, t + lane < q1 && __ldg(p.index + t + lane) == a));
     if (lane == 0) s_count[warp] = count;
     __syncthreads();
     int before = 0, all = 0;
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < S::WARPS; ++i) {
         before += i < warp ? s_count[i] : 0;
         all += s_count[i];
     }
@@ -626,16 +631,16 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
                 const uint32_t to = ring + stage * S::STAGE;
                 // 32 rows of 32 pieces of x: a warp a row
 #pragma unroll
-                for (int j = 0; j < OUTER_STEP / 4; ++j) {
-                    const int row = warp + 4 * j;
+                for (int j = 0; j < OUTER_STEP / S::WARPS; ++j) {
+                    const int row = warp + S::WARPS * j;
                     const bool ok = first + row < n && col0 + lane * 8 < p.cols;
                     const int64_t t = list[first + row < n ? first + row : 0];
                     copy16(to + row * 512 + (lane ^ (row >> 1 & 3) << 1) * 16, ok ? x + t * p.cols + col0 + lane * 8 : x, ok);
                 }
                 constexpr int PIECES = S::ROW / 16;              // of a token's rank values
 #pragma unroll
-                for (int j = 0; j < (OUTER_STEP * PIECES * 2 + 127) / 128; ++j) {
-                    const int i = threadIdx.x + 128 * j, part = i / (OUTER_STEP * PIECES), row = i / PIECES % OUTER_STEP, piece = i % PIECES;
+                for (int j = 0; j < OUTER_STEP * PIECES * 2 / S::THREADS; ++j) {
+                    const int i = threadIdx.x + S::THREADS * j, part = i / (OUTER_STEP * PIECES), row = i / PIECES % OUTER_STEP, piece = i % PIECES;
                     const bool ok = first + row < n && rank0 + piece * 8 < p.rank;
                     const int64_t t = list[first + row < n ? first + row : 0];
                     copy16(to + OUTER_STEP * (512 + part * S::ROW) + row * S::ROW + (piece ^ S::swizzle(row)) * 16,
@@ -649,14 +654,15 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
         if constexpr (F16) {
             // powers of two of the rows, relative to the largest
             float most = 0.0f;
-            for (int j = threadIdx.x; j < n; j += 128) {
+            for (int j = threadIdx.x; j < n; j += S::THREADS) {
                 s_back[j] = __ldcg(h.back + list[j]);
                 most = fmaxf(most, s_back[j]);
             }
             for (int d = 16; d; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
             if (lane == 0) s_big[warp] = most;
             __syncthreads();
-            most = fmaxf(big, fmaxf(fmaxf(s_big[0], s_big[1]), fmaxf(s_big[2], s_big[3])));
+            most = big;
+            for (int j = 0; j < S::WARPS; ++j) most = fmaxf(most, s_big[j]);
             if (big > 0.0f && most > big) {
                 const float down = big / most;
 #pragma unroll
@@ -667,7 +673,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
                         for (int k = 0; k < 4; ++k) acc[rb][j][k] *= down;
             }
             big = most;
-            for (int j = threadIdx.x; j < n; j += 128) s_back[j] /= big;
+            for (int j = threadIdx.x; j < n; j += S::THREADS) s_back[j] /= big;
             // (the barrier of the first stage lies between this and its use)
         }
         int stage = 0;
@@ -677,7 +683,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
             copy_stage(first + (S::STAGES - 1) * OUTER_STEP, stage == 0 ? S::STAGES - 1 : stage - 1);
             const uint32_t xs = ring + stage * S::STAGE, hs = xs + OUTER_STEP * 512;
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-            if (col0 + warp * 64 >= p.cols) continue;
+            if (col0 + wc * 64 >= p.cols) continue;
 #pragma unroll
             for (int step = 0; step < OUTER_STEP / 16; ++step) {
                 if (first + step * 16 >= n) break;
@@ -685,7 +691,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const int row = step * 16 + 2 * c + k % 2 + k / 2 * 8;
-                    raw[k] = load_shared16(xs + row * 512 + warp * 128 + (r ^ (row >> 1 & 3) << 1) * 16);
+                    raw[k] = load_shared16(xs + row * 512 + wc * 128 + (r ^ (row >> 1 & 3) << 1) * 16);
                 }
                 uint32_t b[8][2];
 #pragma unroll
@@ -705,7 +711,7 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {
-                        const int token = step * 16 + lane % 8 + lane / 16 * 8, piece = rb * 2 + lane / 8 % 2;
+                        const int token = step * 16 + lane % 8 + lane / 16 * 8, piece = (wr * RB + rb) * 2 + lane / 8 % 2;
                         uint32_t ha[4];
                         load_matrices_transposed(hs + part * OUTER_STEP * S::ROW + token * S::ROW + (piece ^ S::swizzle(token)) * 16, ha);
                         if constexpr (F16) {
@@ -731,11 +737,11 @@ __global__ void __launch_bounds__(128) adapter_outer_kernel(void *hidden, const 
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sums[(rb * 16 + r + k / 2 * 8) * 256 + warp * 64 + c * 16 + k % 2 * 8 + j] = acc[rb][j][k] * f;
+            for (int k = 0; k < 4; ++k) sums[((wr * RB + rb) * 16 + r + k / 2 * 8) * 256 + wc * 64 + c * 16 + k % 2 * 8 + j] = acc[rb][j][k] * f;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     const int parts = gridDim.z, mine = blockIdx.z;
-    for (int i = mine * 128 + threadIdx.x; i < S::RANKS * 32; i += parts * 128) {        // eight columns of a rank
+    for (int i = mine * S::THREADS + threadIdx.x; i < S::RANKS * 32; i += parts * S::THREADS) {        // eight columns of a rank
         const int rank = rank0 + i / 32;
         const int64_t at = col0 + i % 32 * 8;
         if (rank >= p.rank || at >= p.cols) continue;
@@ -869,20 +875,21 @@ int expand(void *h, const void *w, const AdapterArgs &p, const void *base, void 
     return expand_fast<T, 8>(h, (const T *)w, p, (const T *)base, (T *)out, st);
 }
 
-template <typename T, int RB>
+template <typename T, int RB, int RG>
 int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, bool early, cudaStream_t st) {
-    const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 16 * RB - 1) / (16 * RB)), most = (p.M + 2 * OUTER_STEP - 1) / (2 * OUTER_STEP);
+    using S = OuterShape<RB, RG>;
+    const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + S::RANKS - 1) / S::RANKS), most = (p.M + 2 * OUTER_STEP - 1) / (2 * OUTER_STEP);
     int per_sm = 0;
-    const int rc = ctas_per_sm<adapter_outer_kernel<T, RB>>(128, OuterShape<RB>::SMEM, per_sm);
+    const int rc = ctas_per_sm<adapter_outer_kernel<T, RB, RG>>(S::THREADS, S::SMEM, per_sm);
     if (rc != BW_OK) return rc;
     const int parts = parts_of(blocks * rows, SMS * per_sm, most < 8 ? most : 8, 0.02);
-    return launch<adapter_outer_kernel<T, RB>>("adapter_outer_kernel", dim3((unsigned)blocks, (unsigned)rows, parts), 128, OuterShape<RB>::SMEM, dim3(1, 1, parts), early, st, h, x, p, dw);
+    return launch<adapter_outer_kernel<T, RB, RG>>("adapter_outer_kernel", dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, dim3(1, 1, parts), early, st, h, x, p, dw);
 }
 template <typename T>
 int outer(void *h, const void *x, const AdapterArgs &p, void *dw, bool early, cudaStream_t st) {
-    if (p.rank <= 16) return outer_fast<T, 1>(h, (const T *)x, p, (T *)dw, early, st);
-    if (p.rank <= 32) return outer_fast<T, 2>(h, (const T *)x, p, (T *)dw, early, st);
-    return outer_fast<T, 4>(h, (const T *)x, p, (T *)dw, early, st);
+    if (p.rank <= 16) return outer_fast<T, 1, 1>(h, (const T *)x, p, (T *)dw, early, st);
+    if (p.rank <= 32) return outer_fast<T, 2, 1>(h, (const T *)x, p, (T *)dw, early, st);
+    return outer_fast<T, 2, 2>(h, (const T *)x, p, (T *)dw, early, st);
 }
 
 // The same three by the general kernels, whose rank values are fp32.

@@ -235,7 +235,8 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
         end = INT64_MAX;
     } else {
         int64_t total = 0;
-        for (int64_t i = lane; i < p.batch; i += 32) total += weight_of(p, i);
+        int mine = 0;
+        for (int64_t i = lane; i < p.batch; i += 32) total += mine = weight_of(p, i);
         for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
         total *= p.units;
         const int64_t per = share(p, total);
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
         end = at + per < total ? at + per : total;
         if (at >= end) return;
         for (int64_t b0 = 0; b0 < p.batch; b0 += 32) {
-            const int mine = b0 + lane < p.batch ? weight_of(p, b0 + lane) : 0;
+            if (p.batch > 32) mine = b0 + lane < p.batch ? weight_of(p, b0 + lane) : 0;
             int64_t sum = mine;
             for (int d = 1; d < 32; d *= 2) {
                 const int64_t o = __shfl_up_sync(0xffffffffu, sum, d);
@@ -627,17 +628,13 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
 // One CTA a head of a sequence: zeros for an empty sequence, and the parts of one that several CTAs share.
 template <typename T, int DIM>
 __global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
-    pdl_wait();
     const AttendArgs &a = p.a;
     const int64_t b = blockIdx.x / a.heads;
     const int h = (int)(blockIdx.x - b * a.heads), group = a.heads / a.kv_heads, kh = h / group, block = (h - kh * group) / p.cols,
               col = h - kh * group - block * p.cols, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     T *out = (T *)a.out + (int64_t)blockIdx.x * DIM;
+    // (the lengths are not the work of the launch before this one, which is not waited for to read them)
     const int n = __ldcg(a.lengths + b), weight = weight_of(p, b);
-    if (weight == 0) {
-        for (int d = threadIdx.x; d < DIM; d += 128) out[d] = from_f32<T>(n > 0 ? NAN : 0.0f);
-        return;
-    }
     int64_t total = 0, before = 0;
     for (int64_t i = lane; i < p.batch; i += 32) {
         const int w = weight_of(p, i);
@@ -650,6 +647,11 @@ __global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
     }
     const int64_t per = share(p, total * p.units), from = before * p.units + (int64_t)(kh * p.blocks + block) * weight + START;
     const int first = (int)(from / per), last = (int)((from + weight - START - 1) / per), parts = last - first + 1;
+    pdl_wait();
+    if (weight == 0) {
+        for (int d = threadIdx.x; d < DIM; d += 128) out[d] = from_f32<T>(n > 0 ? NAN : 0.0f);
+        return;
+    }
     if (parts == 1) return;
     const int64_t size = (int64_t)p.cols * (DIM + 2);             // of a slot; the first CTA's part is in its second one, the others' in their first
     auto slot = [&](int i) { return p.slots + (2 * (int64_t)(first + i) + (i == 0)) * size; };
