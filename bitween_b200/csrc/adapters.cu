@@ -102,9 +102,8 @@ __device__ __forceinline__ int exponent_of(float big) { return min(max((int)(__f
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes to shared memory, asynchronously; zeros where there is nothing to copy.
-__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool ok) {
-    const int bytes = ok ? 16 : 0;
+// 16 bytes to shared memory, asynchronously, or 16 zeros (`bytes` 0: nothing is read).
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -291,11 +290,13 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(const T *__rest
     }
 }
 
+constexpr int SHRINK_STAGES = 3;
+
 // Rank values of many tokens: 64 rows of one adapter, a part of the columns; rows of x and of w go through a ring in shared memory, 64 columns a
 // stage, in 16-byte pieces exchanged by row so that ldmatrix meets all banks.
 template <typename T, int NBR>
 __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict__ x, const T *__restrict__ w, const AdapterArgs p, int64_t per_split, void *hidden) {
-    constexpr int RANKS = 8 * NBR, STAGE = (TILE + RANKS) * 128, STAGES = NBR <= 8 ? 4 : 3;
+    constexpr int RANKS = 8 * NBR, STAGE = (TILE + RANKS) * 128, STAGES = SHRINK_STAGES;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint8_t lists[4][TILE];
@@ -311,28 +312,31 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
         if (a < 0 || a >= p.adapters) continue;
         // a thread copies piece threadIdx % 8 of every 16th row
         const int piece = threadIdx.x % 8;
-        const T *rows[4];
-        bool has[4];
+        constexpr int WROWS = (RANKS + 15) / 16;
+        const T *rows[4], *wrows[WROWS];
+        int bytes[4], wbytes[WROWS];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int row = threadIdx.x / 8 + 16 * j;
-            has[j] = row < tile.count;
-            rows[j] = x + (t0 + (has[j] ? tile.list[row] : 0)) * p.cols + piece * 8;
+            bytes[j] = row < tile.count ? 16 : 0;
+            rows[j] = x + (t0 + (row < tile.count ? tile.list[row] : 0)) * p.cols + piece * 8;
         }
-        const T *wrow = w + ((int64_t)a * p.rank + threadIdx.x / 8) * p.cols + piece * 8;
+#pragma unroll
+        for (int j = 0; j < WROWS; ++j) {
+            const int rank = threadIdx.x / 8 + 16 * j;
+            wbytes[j] = rank < p.rank ? 16 : 0;
+            wrows[j] = w + ((int64_t)a * p.rank + (rank < p.rank ? rank : 0)) * p.cols + piece * 8;
+        }
         const int swizzled = threadIdx.x / 8 * 128 + ((piece ^ (threadIdx.x / 8 & 7)) * 16);
         auto copy_stage = [&](int64_t k, int stage) {
             if (k < end) {
                 const bool in = k + piece * 8 < end;
                 const uint32_t to = ring + stage * STAGE + swizzled;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) copy16(to + j * 2048, in && has[j] ? rows[j] + k : x, in && has[j]);
+                for (int j = 0; j < 4; ++j) copy16(to + j * 2048, rows[j] + k, in ? bytes[j] : 0);
 #pragma unroll
-                for (int j = 0; j < (RANKS + 15) / 16; ++j) {
-                    const int rank = threadIdx.x / 8 + 16 * j;
-                    const bool ok = in && rank < p.rank;
-                    if (rank < RANKS) copy16(to + TILE * 128 + j * 2048, ok ? wrow + 16 * j * p.cols + k : w, ok);
-                }
+                for (int j = 0; j < WROWS; ++j)
+                    if (RANKS >= 16 || threadIdx.x / 8 < RANKS) copy16(to + TILE * 128 + j * 2048, wrows[j] + k, in ? wbytes[j] : 0);
             }
             copies_commit();
         };
@@ -473,7 +477,7 @@ __global__ void __launch_bounds__(128) adapter_expand_few_kernel(void *hidden, c
 // The same of many tokens: 64 rows of one adapter, 16 a warp with their rank values in registers; blocks of 64 columns of w and of base go through
 // a ring in shared memory.
 template <typename T, int KS>
-__global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, int64_t per_group, const T *base, T *out) {
+__global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, int64_t per_group, const T *base, T *out) {
     constexpr int W_BYTES = KS * 16 * 128, STAGE = W_BYTES + TILE * 128, STAGES = KS <= 4 ? 4 : 3;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -492,13 +496,13 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
         const bool has = a >= 0 && a < p.adapters;
         // a thread copies piece threadIdx % 8 of every 16th row of w and of base
         const int piece = threadIdx.x % 8, row0 = threadIdx.x / 8;
-        const T *wrow = w + ((int64_t)(has ? a : 0) * p.rank + row0) * p.cols + piece * 8;
-        const T *rows[4];
-        bool here[4];
+        const T *wrow = w + ((int64_t)(has ? a : 0) * p.rank + row0) * p.cols + piece * 8, *rows[4];
+        const uint32_t wstep = (uint32_t)p.cols * 16;
+        int bytes[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            here[j] = base && row0 + 16 * j < tile.count;
-            rows[j] = here[j] ? base + (t0 + tile.list[row0 + 16 * j]) * p.cols + piece * 8 : w;
+            bytes[j] = row0 + 16 * j < tile.count ? 16 : 0;
+            rows[j] = base + (t0 + (row0 + 16 * j < tile.count ? tile.list[row0 + 16 * j] : 0)) * p.cols + piece * 8;
         }
         auto copy_stage = [&](int64_t cb, int stage) {
             if (cb < end) {
@@ -508,12 +512,12 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
 #pragma unroll
                     for (int j = 0; j < KS; ++j) {
                         const bool ok = in && row0 + 16 * j < p.rank;
-                        copy16(to + j * 2048 + (piece ^ (row0 >> 1 & 3) << 1) * 16, ok ? wrow + 16 * j * p.cols + cb : w, ok);
+                        copy16(to + j * 2048 + (piece ^ (row0 >> 1 & 3) << 1) * 16, wrow + (ok ? (int64_t)(wstep * j) + cb : 0), ok ? 16 : 0);
                     }
                 }
                 if (base) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) copy16(to + W_BYTES + j * 2048 + (piece ^ (row0 & 7)) * 16, in && here[j] ? rows[j] + cb : w, in && here[j]);
+                    for (int j = 0; j < 4; ++j) copy16(to + W_BYTES + j * 2048 + (piece ^ (row0 & 7)) * 16, rows[j] + cb, in ? bytes[j] : 0);
                 }
             }
             copies_commit();
@@ -570,12 +574,13 @@ __global__ void __launch_bounds__(128) adapter_expand_kernel(void *hidden, const
 
 constexpr int OUTER_LIST = 2048, OUTER_STEP = 32;
 
+constexpr int SUM_ROW = 260;             // (a row of sums, padded: eight rows meet in four banks otherwise)
 // RB blocks of 16 ranks a warp, RG groups of four warps with ranks of their own.
 template <int RB, int RG> struct OuterShape {
     static constexpr int WARPS = 4 * RG, THREADS = 32 * WARPS;
     static constexpr int RANKS = 16 * RB * RG, ROW = RANKS * 2;               // bytes of a token's rank values
     static constexpr int STAGE = OUTER_STEP * (512 + 2 * ROW), STAGES = RG == 1 ? 4 : 3;
-    static constexpr int SUMS = RANKS * 256 * 4, SMEM = STAGE * STAGES > SUMS ? STAGE * STAGES : SUMS;
+    static constexpr int SUMS = RANKS * SUM_ROW * 4, SMEM = STAGE * STAGES > SUMS ? STAGE * STAGES : SUMS;
     static __device__ __forceinline__ int swizzle(int token) { return ROW >= 128 ? token & 7 : ROW == 64 ? token >> 1 & 3 : token >> 2 & 1; }
 };
 
@@ -590,17 +595,17 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     const int rank_blocks = (p.rank + S::RANKS - 1) / S::RANKS, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * S::RANKS;
     const int64_t col0 = (int64_t)blockIdx.x * 256;
     extern __shared__ __align__(128) uint8_t smem[];
-    float *sums = reinterpret_cast<float *>(smem);               // [RANKS][256], at the end
+    float *sums = reinterpret_cast<float *>(smem);               // [RANKS][SUM_ROW], at the end
     const uint32_t ring = smem_addr(smem);
     const Hidden<T> h(hidden, p.M, p.rank);
-    __shared__ int list[OUTER_LIST], s_count[S::WARPS];
+    __shared__ int list[OUTER_LIST + OUTER_STEP], s_count[S::WARPS];
     __shared__ float s_back[OUTER_LIST], s_big[S::WARPS];
 
     pdl_launch_dependents();
     // the adapter's tokens before this warp's part of all, and in all
     const int64_t part = (p.M + S::THREADS - 1) / S::THREADS * 32, q0 = warp * part, q1 = q0 + part < p.M ? q0 + part : p.M;
     int count = 0;
-#pragma unroll 4
+#pragma unroll 16
     for (int64_t t = q0; t < q1; t += 32) count += __popc(__ballot_sync(0xffffffffu, t + lane < q1 && __ldg(p.index + t + lane) == a));
     if (lane == 0) s_count[warp] = count;
     __syncthreads();
@@ -612,6 +617,10 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     pdl_wait();                                                  // (the rank values are made by one of the launches before)
     const int share = (all + gridDim.z - 1) / gridDim.z, lo = blockIdx.z * share, hi = lo + share < all ? lo + share : all;
 
+    // this thread's piece of a row of x (columns behind the last: zeros), and bytes of a row
+    const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0;
+    const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0));
+    const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2;
     float acc[RB][8][4] = {};
     float big = 0.0f;                                            // fp16: the sums are of h / big, the largest power of two of a row so far
     for (int from = lo; from < hi; from += OUTER_LIST) {
@@ -626,6 +635,8 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
             at += __popc(m);
         }
         __syncthreads();
+        if (threadIdx.x < OUTER_STEP) list[n + threadIdx.x] = list[0];      // (the last stage's places behind the last token)
+        __syncthreads();
         auto copy_stage = [&](int first, int stage) {
             if (first < n) {
                 const uint32_t to = ring + stage * S::STAGE;
@@ -633,18 +644,15 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 #pragma unroll
                 for (int j = 0; j < OUTER_STEP / S::WARPS; ++j) {
                     const int row = warp + S::WARPS * j;
-                    const bool ok = first + row < n && col0 + lane * 8 < p.cols;
-                    const int64_t t = list[first + row < n ? first + row : 0];
-                    copy16(to + row * 512 + (lane ^ (row >> 1 & 3) << 1) * 16, ok ? x + t * p.cols + col0 + lane * 8 : x, ok);
+                    copy16(to + row * 512 + (lane ^ (row >> 1 & 3) << 1) * 16, xs0 + (uint64_t)(uint32_t)list[first + row] * x_row, first + row < n ? x_bytes : 0);
                 }
                 constexpr int PIECES = S::ROW / 16;              // of a token's rank values
 #pragma unroll
                 for (int j = 0; j < OUTER_STEP * PIECES * 2 / S::THREADS; ++j) {
                     const int i = threadIdx.x + S::THREADS * j, part = i / (OUTER_STEP * PIECES), row = i / PIECES % OUTER_STEP, piece = i % PIECES;
                     const bool ok = first + row < n && rank0 + piece * 8 < p.rank;
-                    const int64_t t = list[first + row < n ? first + row : 0];
                     copy16(to + OUTER_STEP * (512 + part * S::ROW) + row * S::ROW + (piece ^ S::swizzle(row)) * 16,
-                           ok ? (part ? h.rest : h.top) + t * p.rank + rank0 + piece * 8 : h.top, ok);
+                           (const uint8_t *)((part ? h.rest : h.top) + (ok ? rank0 + piece * 8 : 0)) + (uint64_t)(uint32_t)list[first + row] * h_row, ok ? 16 : 0);
                 }
             }
             copies_commit();
@@ -737,7 +745,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sums[((wr * RB + rb) * 16 + r + k / 2 * 8) * 256 + wc * 64 + c * 16 + k % 2 * 8 + j] = acc[rb][j][k] * f;
+            for (int k = 0; k < 4; ++k) sums[((wr * RB + rb) * 16 + r + k / 2 * 8) * SUM_ROW + wc * 64 + c * 16 + k % 2 * 8 + j] = acc[rb][j][k] * f;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     const int parts = gridDim.z, mine = blockIdx.z;
@@ -747,7 +755,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         if (rank >= p.rank || at >= p.cols) continue;
         float4 s0 = make_float4(0, 0, 0, 0), s1 = s0;
         for (int o = 0; o < parts; ++o) {
-            const float4 *from = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, o) + i * 8);
+            const float4 *from = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, o) + i / 32 * SUM_ROW + i % 32 * 8);
             const float4 u = from[0], v = from[1];
             s0.x += u.x; s0.y += u.y; s0.z += u.z; s0.w += u.w;
             s1.x += v.x; s1.y += v.y; s1.z += v.z; s1.w += v.w;
@@ -803,13 +811,53 @@ int launch(const char *name, dim3 grid, int threads, int smem, dim3 cluster, boo
     return check_launch(name);
 }
 
-// Into how many parts, up to `most`, `ctas` pieces of work are cut where `at_once` fit on the chip: as few rounds of as short parts as can be.  A part
-// costs `fixed` of an uncut piece's time on top.
-int parts_of(int64_t ctas, int64_t at_once, int64_t most, double fixed) {
+// Clusters of `size` CTAs that the chip holds at once (the groups of SMs that a cluster has to fit into are of uneven sizes).
+template <auto KERN>
+int clusters_at_once(int size, int threads, int smem, int &n) {
+    static std::atomic<int> known[64][8];
+    int device = 0;
+    BW_CUDA_TRY(cudaGetDevice(&device));
+    n = device < 64 ? known[device][size - 1].load(std::memory_order_relaxed) : 0;
+    if (n) return BW_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    BW_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, KERN, &cfg));
+    if (n < 1) n = 1;
+    if (device < 64) known[device][size - 1].store(n, std::memory_order_relaxed);
+    return BW_OK;
+}
+// Into how many parts, up to `most` (8 CTAs a cluster), each of `pieces` of work is cut: as few rounds of clusters as short as can be; a part costs
+// `fixed` of an uncut piece on top.
+template <auto KERN>
+int cluster_parts(int64_t pieces, int64_t most, double fixed, int threads, int smem, int &best) {
+    double least = 0.0;
+    best = 1;
+    for (int s = 1; s <= most && s <= 8; ++s) {
+        int at_once = 0;
+        const int rc = clusters_at_once<KERN>(s, threads, smem, at_once);
+        if (rc != BW_OK) return rc;
+        const double time = (double)((pieces + at_once - 1) / at_once) * (1.0 / s + fixed);
+        if (s == 1 || time < least) {
+            least = time;
+            best = s;
+        }
+    }
+    return BW_OK;
+}
+// The same for pieces that need not run together.
+int parts_of(int64_t pieces, int64_t at_once, int64_t most, double fixed) {
     int best = 1;
     double least = 0.0;
     for (int s = 1; s <= most; ++s) {
-        const double time = (double)((ctas * s + at_once - 1) / at_once) * (1.0 / s + fixed);
+        const double time = (double)((pieces * s + at_once - 1) / at_once) * (1.0 / s + fixed);
         if (s == 1 || time < least) {
             least = time;
             best = s;
@@ -826,7 +874,7 @@ int slots_of(const AdapterArgs &p) {
 
 template <typename T, int NBR>
 int shrink_fast(const T *x, const T *w, AdapterArgs p, void *h, cudaStream_t st) {
-    constexpr int RANKS = 8 * NBR, FEW_SMEM = 7 * 16 * (RANKS + 1) * 4, RING = (TILE + RANKS) * 128 * (NBR <= 8 ? 4 : 3), SUMS = TILE * (RANKS + 4) * 4,
+    constexpr int RANKS = 8 * NBR, FEW_SMEM = 7 * 16 * (RANKS + 1) * 4, RING = (TILE + RANKS) * 128 * SHRINK_STAGES, SUMS = TILE * (RANKS + 4) * 4,
                   SMEM = RING > SUMS ? RING : SUMS;
     p.slots = slots_of(p);
     const int64_t most = (p.cols + 255) / 256;                    // (a part has 256 columns at least; a cluster 8 CTAs at most)
@@ -839,7 +887,8 @@ int shrink_fast(const T *x, const T *w, AdapterArgs p, void *h, cudaStream_t st)
         return launch<adapter_shrink_few_kernel<T, NBR>>("adapter_shrink_few_kernel", dim3(parts, p.slots), 256, FEW_SMEM, dim3(parts), false, st, x, w, p, per_split, h);
     }
     if ((rc = ctas_per_sm<adapter_shrink_kernel<T, NBR>>(128, SMEM, per_sm)) != BW_OK) return rc;
-    const int parts = parts_of(tiles, SMS * per_sm, most < 8 ? most : 8, 0.02);
+    int parts = 1;
+    if ((rc = cluster_parts<adapter_shrink_kernel<T, NBR>>(tiles, most, 0.02, 128, SMEM, parts)) != BW_OK) return rc;
     const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
     return launch<adapter_shrink_kernel<T, NBR>>("adapter_shrink_kernel", dim3(parts, tiles, p.slots), 128, SMEM, dim3(parts), false, st, x, w, p, per_split, h);
 }
@@ -879,10 +928,9 @@ template <typename T, int RB, int RG>
 int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, bool early, cudaStream_t st) {
     using S = OuterShape<RB, RG>;
     const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + S::RANKS - 1) / S::RANKS), most = (p.M + 2 * OUTER_STEP - 1) / (2 * OUTER_STEP);
-    int per_sm = 0;
-    const int rc = ctas_per_sm<adapter_outer_kernel<T, RB, RG>>(S::THREADS, S::SMEM, per_sm);
+    int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_kernel<T, RB, RG>>(S::THREADS, S::SMEM, per_sm);
+    if (rc == BW_OK) rc = cluster_parts<adapter_outer_kernel<T, RB, RG>>(blocks * rows, most, 0.02, S::THREADS, S::SMEM, parts);
     if (rc != BW_OK) return rc;
-    const int parts = parts_of(blocks * rows, SMS * per_sm, most < 8 ? most : 8, 0.02);
     return launch<adapter_outer_kernel<T, RB, RG>>("adapter_outer_kernel", dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, dim3(1, 1, parts), early, st, h, x, p, dw);
 }
 template <typename T>
