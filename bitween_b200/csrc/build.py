@@ -63,7 +63,7 @@ def build_host(force=False, verbose=False):
     includes = [os.path.join(ROOT, "include"), os.path.join(cuda, "include"), sysconfig.get_paths()["include"]] + cpp_extension.include_paths()
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + \
-        [f"-I{d}" for d in includes] + [src, "-o", part, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+        [f"-I{d}" for d in includes] + [src, "-o", part, f"-L{libs}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
                                                "-L" + os.path.join(cuda, "lib64"), "-lcudart"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if verbose or r.returncode != 0:
