@@ -22,7 +22,7 @@
 
 #include <atomic>
 
-#include "bw_common.cuh"
+#include "early_launch.cuh"
 
 namespace bw {
 namespace {
@@ -91,7 +91,8 @@ template <> struct Pair<__nv_bfloat16> {
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
-__device__ __forceinline__ uint4 load16_if(const void *p, bool ok) { return ok ? __ldg(reinterpret_cast<const uint4 *>(p)) : make_uint4(0, 0, 0, 0); }
+// (From L2, as all that a kernel before may have written: the SM's L1 may hold lines from before this kernel's start, at which they were still being written.)
+__device__ __forceinline__ uint4 load16_if(const void *p, bool ok) { return ok ? __ldcg(reinterpret_cast<const uint4 *>(p)) : make_uint4(0, 0, 0, 0); }
 // Column j (of a lane's eight) of two rows beside each other.
 __device__ __forceinline__ uint32_t column_pair(const uint4 &even, const uint4 &odd, int j) {
     const uint32_t *a = reinterpret_cast<const uint32_t *>(&even), *b = reinterpret_cast<const uint32_t *>(&odd);
@@ -129,6 +130,7 @@ struct AdapterArgs {
     const float *scaling;
     int adapters, rank;
     int slots;                  // CTAs among which the adapters of a tile of tokens are dealt
+    bool behind;                // another launch of this call comes before: all that came before that is done when this one starts
 };
 
 // Rank values: [M][rank] of 16 bits, the same of their rests, and (fp16) [M] powers of two by which both were divided.
@@ -151,8 +153,8 @@ struct TileAdapters {
         const int lane = threadIdx.x % 32;
         const unsigned below = (1u << lane) - 1;
         const bool a = t0 + lane < p.M, b = t0 + lane + 32 < p.M;
-        lo = a ? __ldg(p.index + t0 + lane) : 0;
-        hi = b ? __ldg(p.index + t0 + lane + 32) : 0;
+        lo = a ? __ldcg(p.index + t0 + lane) : 0;
+        hi = b ? __ldcg(p.index + t0 + lane + 32) : 0;
         has_lo = __ballot_sync(0xffffffffu, a);
         has_hi = __ballot_sync(0xffffffffu, b);
         const unsigned like_lo = __match_any_sync(0xffffffffu, lo), like_hi = __match_any_sync(0xffffffffu, hi);      // (by all lanes)
@@ -181,9 +183,6 @@ struct TileAdapters {
         __syncwarp();
     }
 };
-
-__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // The end of a shrink pass: the CTAs of a cluster have sums of their part of the columns in `sums` [rows][RANKS + 4]; each CTA adds up its share of
 // the rows, a warp a row, and writes them as two 16-bit parts.
@@ -241,6 +240,7 @@ __global__ void __launch_bounds__(256) adapter_shrink_few_kernel(const T *__rest
     extern __shared__ float red[];                            // [7][16][RANKS + 1]
     __shared__ uint8_t lists[8][TILE];
     const Hidden<T> h(hidden, p.M, p.rank);
+    pdl_wait();
     pdl_launch_dependents();
     const int64_t begin = blockIdx.x * per_split, end = begin + per_split < p.cols ? begin + per_split : p.cols;
     const int64_t per_warp = (per_split / 32 + 7) / 8 * 32, k0 = begin + warp * per_warp, k1 = k0 + per_warp < end ? k0 + per_warp : end;
@@ -302,6 +302,7 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
     __shared__ uint8_t lists[4][TILE];
     const uint32_t ring = smem_addr(smem);
     const Hidden<T> h(hidden, p.M, p.rank);
+    pdl_wait();
     pdl_launch_dependents();
     const int64_t t0 = (int64_t)blockIdx.y * TILE, begin = blockIdx.x * per_split, end = begin + per_split < p.cols ? begin + per_split : p.cols;
 
@@ -381,7 +382,7 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
 
 // ---- expand --------------------------------------------------------------------------------------------------------------
 
-// Fragments of the rank values of 16 rows: [steps][value and rest].  (From L2: a kernel that was launched early has been there while they were made.)
+// Fragments of the rank values of 16 rows: [steps][value and rest].  
 template <typename T, int KS>
 __device__ __forceinline__ void load_rank_values(const Hidden<T> &h, int rank, int64_t ta, int64_t tb, bool has_a, bool has_b, int c, uint32_t (&top)[KS][4], uint32_t (&rest)[KS][4]) {
 #pragma unroll
@@ -400,7 +401,7 @@ template <typename T>
 __device__ __forceinline__ float row_factor(const Hidden<T> &h, const AdapterArgs &p, int a, int64_t t, bool has) {
     if (a < 0 || !has) return 0.0f;
     if (a >= p.adapters) return NAN;
-    return (__is_same(T, __half) ? __ldcg(h.back + t) : 1.0f) * (p.scaling ? __ldg(p.scaling + a) : 1.0f);
+    return (__is_same(T, __half) ? __ldcg(h.back + t) : 1.0f) * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
 }
 // base + f * product, 16 neighbouring columns of two rows; `old` is base (zeros without one).
 template <typename T>
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(128) adapter_expand_few_kernel(void *hidden, c
             uint4 old[2][2];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                old[j / 2][j % 2] = base && live[j / 2] && in[j % 2] ? *reinterpret_cast<const uint4 *>(base + t[j / 2] * p.cols + cb + 16 * c + j % 2 * 8)
+                old[j / 2][j % 2] = base && live[j / 2] && in[j % 2] ? __ldcg(reinterpret_cast<const uint4 *>(base + t[j / 2] * p.cols + cb + 16 * c + j % 2 * 8))
                                                                       : make_uint4(0, 0, 0, 0);
             const float f[2] = {row_factor(h, p, a, t[0], live[0]), row_factor(h, p, a, t[1], live[1])};
             float acc[8][4] = {};
@@ -601,12 +602,13 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     __shared__ int list[OUTER_LIST + OUTER_STEP], s_count[S::WARPS];
     __shared__ float s_back[OUTER_LIST], s_big[S::WARPS];
 
+    if (!p.behind) pdl_wait();
     pdl_launch_dependents();
     // the adapter's tokens before this warp's part of all, and in all
     const int64_t part = (p.M + S::THREADS - 1) / S::THREADS * 32, q0 = warp * part, q1 = q0 + part < p.M ? q0 + part : p.M;
     int count = 0;
 #pragma unroll 16
-    for (int64_t t = q0; t < q1; t += 32) count += __popc(__ballot_sync(0xffffffffu, t + lane < q1 && __ldg(p.index + t + lane) == a));
+    for (int64_t t = q0; t < q1; t += 32) count += __popc(__ballot_sync(0xffffffffu, t + lane < q1 && __ldcg(p.index + t + lane) == a));
     if (lane == 0) s_count[warp] = count;
     __syncthreads();
     int before = 0, all = 0;
@@ -614,7 +616,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         before += i < warp ? s_count[i] : 0;
         all += s_count[i];
     }
-    pdl_wait();                                                  // (the rank values are made by one of the launches before)
+    if (p.behind) pdl_wait();                                    // (the rank values are made by one of the launches before)
     const int share = (all + gridDim.z - 1) / gridDim.z, lo = blockIdx.z * share, hi = lo + share < all ? lo + share : all;
 
     // this thread's piece of a row of x (columns behind the last: zeros), and bytes of a row
@@ -628,7 +630,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         __syncthreads();
         int at = before;
         for (int64_t t = q0; t < q1 && at < from + n; t += 32) {
-            const bool mine = t + lane < q1 && __ldg(p.index + t + lane) == a;
+            const bool mine = t + lane < q1 && __ldcg(p.index + t + lane) == a;
             const unsigned m = __ballot_sync(0xffffffffu, mine);
             const int place = at + __popc(m & ((1u << lane) - 1)) - from;
             if (mine && place >= 0 && place < n) list[place] = (int)(t + lane);
@@ -738,7 +740,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     }
 
     // sums of this CTA, in 16 neighbouring columns a lane; then those of the cluster
-    const float f = (F16 ? big : 1.0f) * (p.scaling ? __ldg(p.scaling + a) : 1.0f);
+    const float f = (F16 ? big : 1.0f) * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
     __syncthreads();
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
@@ -787,9 +789,9 @@ int ctas_per_sm(int threads, int smem, int &n) {
 }
 constexpr int SMS = 148;
 
-// `early`: the kernel may start while the one before it still runs (it waits for that itself).
+// launch_early with a cluster.
 template <auto KERN, typename... Args>
-int launch(const char *name, dim3 grid, int threads, int smem, dim3 cluster, bool early, cudaStream_t st, Args... args) {
+int launch(const char *name, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
@@ -803,10 +805,8 @@ int launch(const char *name, dim3 grid, int threads, int smem, dim3 cluster, boo
         attr[cfg.numAttrs].val.clusterDim.y = cluster.y;
         attr[cfg.numAttrs++].val.clusterDim.z = cluster.z;
     }
-    if (early) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    }
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, KERN, args...));
     return check_launch(name);
 }
@@ -884,13 +884,13 @@ int shrink_fast(const T *x, const T *w, AdapterArgs p, void *h, cudaStream_t st)
         if ((rc = ctas_per_sm<adapter_shrink_few_kernel<T, NBR>>(256, FEW_SMEM, per_sm)) != BW_OK) return rc;
         const int parts = most < 8 ? (int)most : 8;
         const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
-        return launch<adapter_shrink_few_kernel<T, NBR>>("adapter_shrink_few_kernel", dim3(parts, p.slots), 256, FEW_SMEM, dim3(parts), false, st, x, w, p, per_split, h);
+        return launch<adapter_shrink_few_kernel<T, NBR>>("adapter_shrink_few_kernel", dim3(parts, p.slots), 256, FEW_SMEM, dim3(parts), st, x, w, p, per_split, h);
     }
     if ((rc = ctas_per_sm<adapter_shrink_kernel<T, NBR>>(128, SMEM, per_sm)) != BW_OK) return rc;
     int parts = 1;
     if ((rc = cluster_parts<adapter_shrink_kernel<T, NBR>>(tiles, most, 0.02, 128, SMEM, parts)) != BW_OK) return rc;
     const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
-    return launch<adapter_shrink_kernel<T, NBR>>("adapter_shrink_kernel", dim3(parts, tiles, p.slots), 128, SMEM, dim3(parts), false, st, x, w, p, per_split, h);
+    return launch<adapter_shrink_kernel<T, NBR>>("adapter_shrink_kernel", dim3(parts, tiles, p.slots), 128, SMEM, dim3(parts), st, x, w, p, per_split, h);
 }
 template <typename T>
 int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStream_t st) {
@@ -906,14 +906,14 @@ int expand_fast(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaS
     constexpr int SMEM = (KS * 16 + TILE) * 128 * (KS <= 4 ? 4 : 3);
     p.slots = slots_of(p);
     if (p.M <= FEW)
-        return launch<adapter_expand_few_kernel<T, KS>>("adapter_expand_few_kernel", dim3((unsigned)((p.cols + 255) / 256), p.slots), 128, 0, dim3(1), true, st, h, w, p, base, out);
+        return launch<adapter_expand_few_kernel<T, KS>>("adapter_expand_few_kernel", dim3((unsigned)((p.cols + 255) / 256), p.slots), 128, 0, dim3(1), st, h, w, p, base, out);
     int per_sm = 0;
     const int rc = ctas_per_sm<adapter_expand_kernel<T, KS>>(128, SMEM, per_sm);
     if (rc != BW_OK) return rc;
     const int64_t tiles = (p.M + TILE - 1) / TILE, blocks = (p.cols + 63) / 64, most = (blocks + 1) / 2;
     const int groups = parts_of(tiles, SMS * per_sm, most < 64 ? most : 64, 3.0 / blocks);
     const int64_t per_group = (blocks + groups - 1) / groups * 64;
-    return launch<adapter_expand_kernel<T, KS>>("adapter_expand_kernel", dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), 128, SMEM, dim3(1), true, st,
+    return launch<adapter_expand_kernel<T, KS>>("adapter_expand_kernel", dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), 128, SMEM, dim3(1), st,
                                                 h, w, p, per_group, base, out);
 }
 template <typename T>
@@ -925,19 +925,19 @@ int expand(void *h, const void *w, const AdapterArgs &p, const void *base, void 
 }
 
 template <typename T, int RB, int RG>
-int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, bool early, cudaStream_t st) {
+int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
     using S = OuterShape<RB, RG>;
     const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + S::RANKS - 1) / S::RANKS), most = (p.M + 2 * OUTER_STEP - 1) / (2 * OUTER_STEP);
     int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_kernel<T, RB, RG>>(S::THREADS, S::SMEM, per_sm);
     if (rc == BW_OK) rc = cluster_parts<adapter_outer_kernel<T, RB, RG>>(blocks * rows, most, 0.02, S::THREADS, S::SMEM, parts);
     if (rc != BW_OK) return rc;
-    return launch<adapter_outer_kernel<T, RB, RG>>("adapter_outer_kernel", dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, dim3(1, 1, parts), early, st, h, x, p, dw);
+    return launch<adapter_outer_kernel<T, RB, RG>>("adapter_outer_kernel", dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, dim3(1, 1, parts), st, h, x, p, dw);
 }
 template <typename T>
-int outer(void *h, const void *x, const AdapterArgs &p, void *dw, bool early, cudaStream_t st) {
-    if (p.rank <= 16) return outer_fast<T, 1, 1>(h, (const T *)x, p, (T *)dw, early, st);
-    if (p.rank <= 32) return outer_fast<T, 2, 1>(h, (const T *)x, p, (T *)dw, early, st);
-    return outer_fast<T, 2, 2>(h, (const T *)x, p, (T *)dw, early, st);
+int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
+    if (p.rank <= 16) return outer_fast<T, 1, 1>(h, (const T *)x, p, (T *)dw, st);
+    if (p.rank <= 32) return outer_fast<T, 2, 1>(h, (const T *)x, p, (T *)dw, st);
+    return outer_fast<T, 2, 2>(h, (const T *)x, p, (T *)dw, st);
 }
 
 // The same three by the general kernels, whose rank values are fp32.
@@ -968,7 +968,7 @@ template <typename T>
 int forward(const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index, const float *scaling,
             const void *base, void *out, void *h, cudaStream_t st) {
     const bool fast = fast_sizes(M, N, K, n, r);
-    const AdapterArgs in = {M, K, index, nullptr, n, r, 1}, to = {M, N, index, scaling, n, r, 1};
+    const AdapterArgs in = {M, K, index, nullptr, n, r, 1, false}, to = {M, N, index, scaling, n, r, 1, true};
     const int rc = fast ? shrink<T>(x, down, in, h, st) : shrink_general<T>(x, down, in, h, st);
     if (rc != BW_OK) return rc;
     return fast ? expand<T>(h, up, to, base, out, st) : expand_general<T>(h, up, to, base, out, st);
@@ -977,14 +977,13 @@ template <typename T>
 int backward(const void *dy, const void *x, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index,
              const float *scaling, void *h, void *dx, void *d_down, void *d_up, void *dh, cudaStream_t st) {
     const bool fast = fast_sizes(M, N, K, n, r);
-    const AdapterArgs in = {M, N, index, nullptr, n, r, 1}, over_k = {M, K, index, scaling, n, r, 1}, over_n = {M, N, index, scaling, n, r, 1};
+    const bool behind = M > 0 && (dx || d_down);
+    const AdapterArgs in = {M, N, index, nullptr, n, r, 1, false}, over_k = {M, K, index, scaling, n, r, 1, behind}, over_n = {M, N, index, scaling, n, r, 1, behind};
     int rc = BW_OK;
-    bool early = false;            // (behind a launch of this call: what those read and write was there before the first)
-    if (M > 0 && (dx || d_down)) rc = fast ? shrink<T>(dy, up, in, dh, st) : shrink_general<T>(dy, up, in, dh, st);
-    early = fast && M > 0 && (dx || d_down);
+    if (behind) rc = fast ? shrink<T>(dy, up, in, dh, st) : shrink_general<T>(dy, up, in, dh, st);
     if (rc == BW_OK && M > 0 && dx) rc = fast ? expand<T>(dh, down, over_k, nullptr, dx, st) : expand_general<T>(dh, down, over_k, nullptr, dx, st);
-    if (rc == BW_OK && d_down) rc = fast ? outer<T>(dh, x, over_k, d_down, early, st) : outer_general<T>(dh, x, over_k, d_down, st);
-    if (rc == BW_OK && d_up) rc = fast ? outer<T>(h, dy, over_n, d_up, early, st) : outer_general<T>(h, dy, over_n, d_up, st);
+    if (rc == BW_OK && d_down) rc = fast ? outer<T>(dh, x, over_k, d_down, st) : outer_general<T>(dh, x, over_k, d_down, st);
+    if (rc == BW_OK && d_up) rc = fast ? outer<T>(h, dy, over_n, d_up, st) : outer_general<T>(h, dy, over_n, d_up, st);
     return rc;
 }
 

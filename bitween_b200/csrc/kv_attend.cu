@@ -5,7 +5,7 @@
 // One pass over the cache with the running maximum and sum of the softmax; codes become values in registers.
 #include <atomic>
 
-#include "bw_common.cuh"
+#include "early_launch.cuh"
 
 namespace bw {
 namespace {
@@ -123,7 +123,7 @@ int attend_general(const AttendArgs &p, int64_t batch, int bits, cudaStream_t st
 // Work: all steps of all sequences and heads in one line, an equal share of it to each CTA, whatever the lengths are; a part of a sequence
 // counts START steps more, which is what its start and end cost.  What a share has of a sequence that others have too goes to scratch (running
 // maximum, sum, unnormalised output), and kv_attend_join_kernel joins it.  Tables of few tiles go without: one CTA a sequence and head.
-constexpr int WARPS = 4, TILE = 16, START = 8;
+constexpr int WARPS = 4, TILE = 16, START = 16;
 constexpr int MOST_CTAS = 592;              // shares of a call: four CTAs on each of 148 SMs
 constexpr int SINGLE_TILES = 16;            // tables of up to so many tiles (256 tokens): one CTA, four tiles a warp
 
@@ -138,8 +138,6 @@ struct FastArgs {
     bool single;
 };
 
-__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -225,6 +223,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
     __shared__ float s_factor[HEADS], s_sum[HEADS], s_m[WARPS][COLS], s_l[WARPS][COLS];
     float *s_o = reinterpret_cast<float *>(smem);
     const uint32_t ring = smem_addr(smem) + warp * (STAGES * C::STEP);
+    pdl_wait();
     pdl_launch_dependents();
 
     // this CTA's share of the line of work, and the sequence in which it starts
@@ -299,7 +298,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
 #pragma unroll
             for (int i = 0; i < PAIR; ++i) {
                 place[i] = at_in;
-                page[i] = step < to && step * PAIR + i < tiles ? __ldg(pages + at_page) : -2;
+                page[i] = step < to && step * PAIR + i < tiles ? __ldcg(pages + at_page) : -2;
                 if (++at_in == p.tiles_per_page) {
                     at_in = 0;
                     ++at_page;
@@ -348,7 +347,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
             float v[DIM / 32], big = 0.0f, sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < DIM / 32; ++i) {
-                v[i] = h < heads ? to_f32(((const T *)a.q)[seq * a.q_stride + (head0 + h) * a.q_head_stride + lane + 32 * i]) : 0.0f;
+                v[i] = h < heads ? to_f32(__ldcg((const T *)a.q + seq * a.q_stride + (head0 + h) * a.q_head_stride + lane + 32 * i)) : 0.0f;
                 big = fmaxf(big, fabsf(v[i]));
             }
             float back = 1.0f;
@@ -633,7 +632,7 @@ __global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
     const int h = (int)(blockIdx.x - b * a.heads), group = a.heads / a.kv_heads, kh = h / group, block = (h - kh * group) / p.cols,
               col = h - kh * group - block * p.cols, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     T *out = (T *)a.out + (int64_t)blockIdx.x * DIM;
-    // (the lengths are not the work of the launch before this one, which is not waited for to read them)
+    // (the lengths were there when the launch before this one began its work, which then is all that is waited for)
     const int n = __ldcg(a.lengths + b), weight = weight_of(p, b);
     int64_t total = 0, before = 0;
     for (int64_t i = lane; i < p.batch; i += 32) {
@@ -722,20 +721,9 @@ int launch_fast(FastArgs &p, cudaStream_t st) {
     }
     p.ctas = 148 * n;
     const int64_t grid = p.single ? p.batch * p.units : p.ctas;
-    kern<<<(unsigned)grid, 32 * WARPS, SMEM, st>>>(p);
-    int rc = check_launch("kv_attend_kernel");
+    const int rc = launch_early("kv_attend_kernel", kern, dim3((unsigned)grid), 32 * WARPS, SMEM, st, p);
     if (rc != BW_OK || p.single) return rc;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(p.batch * p.a.heads));
-    cfg.blockDim = dim3(128);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv_attend_join_kernel<T, DIM>, p));
-    return BW_OK;
+    return launch_early("kv_attend_join_kernel", kv_attend_join_kernel<T, DIM>, dim3((unsigned)(p.batch * p.a.heads)), 128, 0, st, p);
 }
 
 template <typename T, int BITS, int DIM>

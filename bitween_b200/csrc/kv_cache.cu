@@ -11,7 +11,7 @@
 // fp16: (scale, zero) of the key, then of the value: what an attention step needs of one token lies in 8 bytes.
 #include <type_traits>
 
-#include "bw_common.cuh"
+#include "early_launch.cuh"
 
 namespace bw {
 namespace {
@@ -38,6 +38,11 @@ constexpr uint32_t MAGIC_BITS = 0x4B400000u;
 // Values that a thread takes of a row: whole words of codes at any width.  (Of 8 the work on a row's ends, scale and place was most of it.)
 constexpr int E = 16;
 
+// (From L2, as all that a kernel before may have written: the SM's L1 may hold lines from before this kernel's start, at which they were still being written.)
+__device__ __forceinline__ float ld_l2(const float *p) { return __ldcg(p); }
+__device__ __forceinline__ __half ld_l2(const __half *p) { return __ldcg(p); }
+__device__ __forceinline__ __nv_bfloat16 ld_l2(const __nv_bfloat16 *p) { return __ldcg(p); }
+
 // min and max that keep NaN
 __device__ __forceinline__ float min_nan(float a, float b) {
     float y;
@@ -58,7 +63,7 @@ __device__ __forceinline__ void load_values(const T *row, int at, int dim, bool 
     if constexpr (VEC) {
         uint4 raw[E * sizeof(T) / 16];
 #pragma unroll
-        for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) raw[i] = live ? __ldcs(reinterpret_cast<const uint4 *>(row + at) + i) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < (int)(E * sizeof(T) / 16); ++i) raw[i] = live ? __ldcg(reinterpret_cast<const uint4 *>(row + at) + i) : make_uint4(0, 0, 0, 0);
         const T *v = reinterpret_cast<const T *>(raw);
 #pragma unroll
         for (int i = 0; i < E; ++i) x[i] = to_f32(v[i]);
@@ -77,7 +82,7 @@ __device__ __forceinline__ void load_values(const T *row, int at, int dim, bool 
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) x[i] = live && at + i < dim ? to_f32(row[at + i]) : 0.0f;
+        for (int i = 0; i < E; ++i) x[i] = live && at + i < dim ? to_f32(ld_l2(row + at + i)) : 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -94,9 +99,11 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T *__restrict__ k,
                                                         const KvRows p, int32_t *k_codes, int32_t *v_codes, __half2 *params) {
     constexpr int WORDS = E * BITS / 32, VPI = 32 / BITS;
     constexpr float Q = (1 << BITS) - 1, RQ = 1.0f / Q;
+    pdl_wait();
+    pdl_launch_dependents();
     const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = row / (uint32_t)p.heads;
     const int head = (int)(row - token * (uint32_t)p.heads), lane = threadIdx.x % p.lanes, at = lane * E;
-    const int64_t slot = token < p.tokens ? __ldg(slots + token) : -1;
+    const int64_t slot = token < p.tokens ? __ldcg(slots + token) : -1;
     const bool in = slot >= 0 && slot < p.slots, live = in && at < p.dim;
     float x[2][E], lo[2], hi[2];
     load_values<T, VEC>(k + (in ? token * p.stride[0] + head * p.head_stride[0] : 0), at, p.dim, live, x[0], lo[0], hi[0]);
@@ -159,18 +166,18 @@ __device__ __forceinline__ void read_piece(const int32_t *codes, uint32_t consta
     const float zero = 8388608.0f + c.y;
     uint32_t w[WORDS] = {};
     if constexpr (WORDS == 4 && VEC) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(codes) + lane);
+        const uint4 u = __ldcg(reinterpret_cast<const uint4 *>(codes) + lane);
         w[0] = u.x;
         w[1] = u.y;
         w[2] = u.z;
         w[3] = u.w;
     } else if constexpr (WORDS == 2 && VEC) {
-        const uint2 u = __ldg(reinterpret_cast<const uint2 *>(codes) + lane);
+        const uint2 u = __ldcg(reinterpret_cast<const uint2 *>(codes) + lane);
         w[0] = u.x;
         w[1] = u.y;
     } else {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = lane * WORDS + i < words ? (uint32_t)__ldg(codes + lane * WORDS + i) : 0u;
+        for (int i = 0; i < WORDS; ++i) w[i] = lane * WORDS + i < words ? (uint32_t)__ldcg(codes + lane * WORDS + i) : 0u;
     }
     __align__(16) T out[E];
 #pragma unroll
@@ -191,10 +198,12 @@ __device__ __forceinline__ void read_piece(const int32_t *codes, uint32_t consta
 template <typename T, int BITS, bool VEC>
 __global__ void __launch_bounds__(256) kv_read_kernel(const int32_t *__restrict__ k_codes, const int32_t *__restrict__ v_codes,
                                                       const uint2 *__restrict__ params, const int64_t *__restrict__ slots, const KvRows p, T *k, T *v) {
+    pdl_wait();
+    pdl_launch_dependents();
     const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = row / (uint32_t)p.heads;
     const int lane = threadIdx.x % p.lanes;
     if (token >= p.tokens || lane * E >= p.dim) return;
-    const int64_t slot = __ldg(slots + token), to = (int64_t)row * p.dim + lane * E;
+    const int64_t slot = __ldcg(slots + token), to = (int64_t)row * p.dim + lane * E;
     if (slot < 0 || slot >= p.slots) {
 #pragma unroll
         for (int i = 0; i < E; ++i)
@@ -202,7 +211,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const int32_t *__restrict_
         return;
     }
     const int64_t at = cache_row(p, slot, (int)(row - token * (uint32_t)p.heads));
-    const uint2 c = __ldg(params + at);
+    const uint2 c = __ldcg(params + at);
     read_piece<T, BITS, VEC>(k_codes + at * p.words, c.x, lane, p.words, p.dim, k + to);
     read_piece<T, BITS, VEC>(v_codes + at * p.words, c.y, lane, p.words, p.dim, v + to);
 }
@@ -232,9 +241,8 @@ int append_typed(const void *kv, const void *vv, const int64_t *slots, const KvR
     constexpr int V = 16 / sizeof(T);
     bool vec = p.dim % E == 0 && aligned_to(k, 16) && aligned_to(v, 16);
     for (int i = 0; i < 2; ++i) vec = vec && p.stride[i] % V == 0 && p.head_stride[i] % V == 0;
-    if (vec) kv_append_kernel<T, BITS, true><<<kv_grid(p), 256, 0, st>>>(k, v, slots, p, kc, vc, (__half2 *)params);
-    else kv_append_kernel<T, BITS, false><<<kv_grid(p), 256, 0, st>>>(k, v, slots, p, kc, vc, (__half2 *)params);
-    return check_launch("kv_append_kernel");
+    return launch_early("kv_append_kernel", vec ? kv_append_kernel<T, BITS, true> : kv_append_kernel<T, BITS, false>, dim3(kv_grid(p)), 256, 0, st, k, v, slots, p,
+                        kc, vc, (__half2 *)params);
 }
 template <typename T>
 int append_bits(const void *k, const void *v, const int64_t *slots, const KvRows &p, int bits, int32_t *kc, int32_t *vc, void *params, cudaStream_t st) {
@@ -245,9 +253,8 @@ int append_bits(const void *k, const void *v, const int64_t *slots, const KvRows
 template <typename T, int BITS>
 int read_typed(const int32_t *kc, const int32_t *vc, const void *params, const int64_t *slots, const KvRows &p, void *k, void *v, cudaStream_t st) {
     // (k and v are dense and start on 16 bytes: so do all pieces of rows that are whole pieces)
-    if (p.dim % E == 0) kv_read_kernel<T, BITS, true><<<kv_grid(p), 256, 0, st>>>(kc, vc, (const uint2 *)params, slots, p, (T *)k, (T *)v);
-    else kv_read_kernel<T, BITS, false><<<kv_grid(p), 256, 0, st>>>(kc, vc, (const uint2 *)params, slots, p, (T *)k, (T *)v);
-    return check_launch("kv_read_kernel");
+    return launch_early("kv_read_kernel", p.dim % E == 0 ? kv_read_kernel<T, BITS, true> : kv_read_kernel<T, BITS, false>, dim3(kv_grid(p)), 256, 0, st, kc, vc,
+                        (const uint2 *)params, slots, p, (T *)k, (T *)v);
 }
 template <typename T>
 int read_bits(const int32_t *kc, const int32_t *vc, const void *params, const int64_t *slots, const KvRows &p, int bits, void *k, void *v, cudaStream_t st) {
