@@ -789,28 +789,6 @@ int ctas_per_sm(int threads, int smem, int &n) {
 }
 constexpr int SMS = 148;
 
-// launch_early with a cluster.
-template <auto KERN, typename... Args>
-int launch(const char *name, dim3 grid, int threads, int smem, dim3 cluster, cudaStream_t st, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    cfg.attrs = attr;
-    if (cluster.x * cluster.y * cluster.z > 1) {
-        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        attr[cfg.numAttrs].val.clusterDim.x = cluster.x;
-        attr[cfg.numAttrs].val.clusterDim.y = cluster.y;
-        attr[cfg.numAttrs++].val.clusterDim.z = cluster.z;
-    }
-    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-    BW_CUDA_TRY(cudaLaunchKernelEx(&cfg, KERN, args...));
-    return check_launch(name);
-}
-
 // Clusters of `size` CTAs that the chip holds at once (the groups of SMs that a cluster has to fit into are of uneven sizes).
 template <auto KERN>
 int clusters_at_once(int size, int threads, int smem, int &n) {
@@ -884,13 +862,13 @@ int shrink_fast(const T *x, const T *w, AdapterArgs p, void *h, cudaStream_t st)
         if ((rc = ctas_per_sm<adapter_shrink_few_kernel<T, NBR>>(256, FEW_SMEM, per_sm)) != BW_OK) return rc;
         const int parts = most < 8 ? (int)most : 8;
         const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
-        return launch<adapter_shrink_few_kernel<T, NBR>>("adapter_shrink_few_kernel", dim3(parts, p.slots), 256, FEW_SMEM, dim3(parts), st, x, w, p, per_split, h);
+        return launch_early("adapter_shrink_few_kernel", adapter_shrink_few_kernel<T, NBR>, dim3(parts, p.slots), 256, FEW_SMEM, st, dim3(parts), x, w, p, per_split, h);
     }
     if ((rc = ctas_per_sm<adapter_shrink_kernel<T, NBR>>(128, SMEM, per_sm)) != BW_OK) return rc;
     int parts = 1;
     if ((rc = cluster_parts<adapter_shrink_kernel<T, NBR>>(tiles, most, 0.02, 128, SMEM, parts)) != BW_OK) return rc;
     const int64_t per_split = ((p.cols + parts - 1) / parts + 63) / 64 * 64;
-    return launch<adapter_shrink_kernel<T, NBR>>("adapter_shrink_kernel", dim3(parts, tiles, p.slots), 128, SMEM, dim3(parts), st, x, w, p, per_split, h);
+    return launch_early("adapter_shrink_kernel", adapter_shrink_kernel<T, NBR>, dim3(parts, tiles, p.slots), 128, SMEM, st, dim3(parts), x, w, p, per_split, h);
 }
 template <typename T>
 int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStream_t st) {
@@ -906,14 +884,14 @@ int expand_fast(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaS
     constexpr int SMEM = (KS * 16 + TILE) * 128 * (KS <= 4 ? 4 : 3);
     p.slots = slots_of(p);
     if (p.M <= FEW)
-        return launch<adapter_expand_few_kernel<T, KS>>("adapter_expand_few_kernel", dim3((unsigned)((p.cols + 255) / 256), p.slots), 128, 0, dim3(1), st, h, w, p, base, out);
+        return launch_early("adapter_expand_few_kernel", adapter_expand_few_kernel<T, KS>, dim3((unsigned)((p.cols + 255) / 256), p.slots), 128, 0, st, dim3(1), h, w, p, base, out);
     int per_sm = 0;
     const int rc = ctas_per_sm<adapter_expand_kernel<T, KS>>(128, SMEM, per_sm);
     if (rc != BW_OK) return rc;
     const int64_t tiles = (p.M + TILE - 1) / TILE, blocks = (p.cols + 63) / 64, most = (blocks + 1) / 2;
     const int groups = parts_of(tiles, SMS * per_sm, most < 64 ? most : 64, 3.0 / blocks);
     const int64_t per_group = (blocks + groups - 1) / groups * 64;
-    return launch<adapter_expand_kernel<T, KS>>("adapter_expand_kernel", dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), 128, SMEM, dim3(1), st,
+    return launch_early("adapter_expand_kernel", adapter_expand_kernel<T, KS>, dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), 128, SMEM, st, dim3(1),
                                                 h, w, p, per_group, base, out);
 }
 template <typename T>
@@ -931,7 +909,7 @@ int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st
     int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_kernel<T, RB, RG>>(S::THREADS, S::SMEM, per_sm);
     if (rc == BW_OK) rc = cluster_parts<adapter_outer_kernel<T, RB, RG>>(blocks * rows, most, 0.02, S::THREADS, S::SMEM, parts);
     if (rc != BW_OK) return rc;
-    return launch<adapter_outer_kernel<T, RB, RG>>("adapter_outer_kernel", dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, dim3(1, 1, parts), st, h, x, p, dw);
+    return launch_early("adapter_outer_kernel", adapter_outer_kernel<T, RB, RG>, dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, st, dim3(1, 1, parts), h, x, p, dw);
 }
 template <typename T>
 int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {

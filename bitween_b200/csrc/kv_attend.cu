@@ -3,6 +3,8 @@
 //     out[b][h] = sum_t w_t V[t],   w = softmax over t < lengths[b] of  alpha * q[b][h] . K[t],   K, V rows of head h / (heads / kv_heads)
 //
 // One pass over the cache with the running maximum and sum of the softmax; codes become values in registers.
+#include <cooperative_groups.h>
+
 #include <atomic>
 
 #include "early_launch.cuh"
@@ -122,10 +124,11 @@ int attend_general(const AttendArgs &p, int64_t batch, int bits, cudaStream_t st
 //
 // Work: all steps of all sequences and heads in one line, an equal share of it to each CTA, whatever the lengths are; a part of a sequence
 // counts START steps more, which is what its start and end cost.  What a share has of a sequence that others have too goes to scratch (running
-// maximum, sum, unnormalised output), and kv_attend_join_kernel joins it.  Tables of few tiles go without: one CTA a sequence and head.
+// maximum, sum, unnormalised output), and kv_attend_join_kernel joins it.  Where tables are short enough for a cluster of CTAs to take a
+// sequence and head, it does, and joins its parts through shared memory: no scratch, no second launch.
 constexpr int WARPS = 4, TILE = 16, START = 16;
 constexpr int MOST_CTAS = 592;              // shares of a call: four CTAs on each of 148 SMs
-constexpr int SINGLE_TILES = 16;            // tables of up to so many tiles (256 tokens): one CTA, four tiles a warp
+constexpr int CLUSTER_ROUNDS = 5;           // tables of up to so many steps a warp: clusters
 
 struct FastArgs {
     AttendArgs a;
@@ -135,7 +138,7 @@ struct FastArgs {
     int blocks, cols;                       // blocks of query heads of a cache head; heads of a block
     int ctas, most_tiles, tiles_per_page;
     int pair;                               // tiles of a step
-    bool single;
+    int cluster;                            // CTAs of a cluster, one unit each; 0: shares of the line of work, and a join
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -172,6 +175,12 @@ __device__ __forceinline__ void load_transposed4(uint32_t at, uint32_t *x) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
 }
+
+namespace cg = cooperative_groups;
+
+// A part's share of the sum of weights, given its maximum, its sum and the largest maximum.  (Without a finite score it has none, but for the mark of a bad
+// page or length.)
+__device__ __forceinline__ float part_of(float m, float l, float top) { return m == -INFINITY ? (l == l ? 0.0f : NAN) : l * ex2(m - top); }
 
 // Tiles of a sequence within its table; its true length goes beside it.
 __device__ __forceinline__ int tiles_of(int n, int most) {
@@ -221,6 +230,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
     extern __shared__ __align__(128) uint8_t smem[];        // the warps' rings; at the end of a part, their sums
     __shared__ __align__(16) __half sq[HEADS][DIM + 8];
     __shared__ float s_factor[HEADS], s_sum[HEADS], s_m[WARPS][COLS], s_l[WARPS][COLS];
+    __shared__ float2 s_total[HEADS];                       // maximum and sum of this CTA's part
     float *s_o = reinterpret_cast<float *>(smem);
     const uint32_t ring = smem_addr(smem) + warp * (STAGES * C::STEP);
     pdl_wait();
@@ -228,8 +238,10 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
 
     // this CTA's share of the line of work, and the sequence in which it starts
     int64_t at, end, b = 0, before = 0;      // `before`: work in front of sequence b, of one unit
-    if (p.single) {
-        b = blockIdx.x / p.units;
+    const int rank = p.cluster ? (int)(blockIdx.x % p.cluster) : 0;
+    const int64_t item = p.cluster ? blockIdx.x / p.cluster : 0;
+    if (p.cluster) {
+        b = item / p.units;
         at = 0;
         end = INT64_MAX;
     } else {
@@ -264,15 +276,18 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
     while (at < end && b < p.batch) {
         // the next part of one sequence, cache head and block of query heads: steps [from, to) of `steps`
         const int n = __ldcg(a.lengths + b), tiles = tiles_of(n, p.most_tiles), steps = (tiles + PAIR - 1) / PAIR, weight = steps + START;
-        if (!p.single && tiles == 0) {
+        if (!p.cluster && tiles == 0) {
             ++b;
             continue;
         }
         const int64_t start = before * p.units;
-        const int unit = p.single ? (int)(blockIdx.x % p.units) : (int)((at - start) / weight);
+        const int unit = p.cluster ? (int)(item % p.units) : (int)((at - start) / weight);
         if (unit >= p.units) return;           // (lengths that change under the call)
-        int from = 0, to = steps;
-        if (!p.single) {
+        int from, to;
+        if (p.cluster) {
+            from = (int)((int64_t)steps * rank / p.cluster);
+            to = (int)((int64_t)steps * (rank + 1) / p.cluster);
+        } else {
             const int64_t in = at - start - (int64_t)unit * weight, out = in + (end - at);
             from = in > START ? (int)in - START : 0;
             to = out >= weight ? steps : out > START ? (int)out - START : 0;
@@ -281,7 +296,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
             if (to <= from) continue;          // (only of what the part's start counts for; the sequence goes on in the next share)
         }
         const int64_t seq = b;
-        if (!p.single && to == steps && unit == p.units - 1) ++b;
+        if (!p.cluster && to == steps && unit == p.units - 1) ++b;
         const int kh = unit / p.blocks, group = a.heads / a.kv_heads, h0 = (unit - kh * p.blocks) * p.cols;
         const int heads = group - h0 < p.cols ? group - h0 : p.cols;      // of this block
         const int64_t head0 = (int64_t)kh * group + h0;
@@ -599,28 +614,53 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
                         s_o[(warp * COLS + col) * S::STRIDE + d] = o[nb][i][2 * k + j] * (by / (1 << (pl * BITS)));
                     }
             }
+        if (threadIdx.x < heads) {
+            const int col = threadIdx.x;
+            float total = 0.0f, top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < WARPS * PAIR; ++k) top = fmaxf(top, s_m[k / PAIR][col + k % PAIR * 4]);
+#pragma unroll
+            for (int k = 0; k < WARPS * PAIR; ++k) total += part_of(s_m[k / PAIR][col + k % PAIR * 4], s_l[k / PAIR][col + k % PAIR * 4], top);
+            s_total[col] = make_float2(top, total);
+        }
         __syncthreads();
+        auto sum_of = [&](int col, int d) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < WARPS * PAIR; ++k) sum += s_o[(k / PAIR * COLS + col + k % PAIR * 4) * S::STRIDE + d];
+            return sum;
+        };
+        if (p.cluster > 1) {
+            // the CTAs' parts become one: each CTA adds up its own first, then takes its share of the values from all
+            cg::cluster_group cluster = cg::this_cluster();
+            for (int i = threadIdx.x; i < heads * DIM; i += 32 * WARPS) s_o[i / DIM * S::STRIDE + i % DIM] = sum_of(i / DIM, i % DIM);
+            cluster.sync();
+            for (int i = rank * 32 * WARPS + threadIdx.x; i < heads * DIM; i += p.cluster * 32 * WARPS) {
+                const int col = i / DIM, d = i % DIM;
+                float top = -INFINITY, sum = 0.0f, total = 0.0f;
+                for (int k = 0; k < p.cluster; ++k) top = fmaxf(top, cluster.map_shared_rank(s_total, k)[col].x);
+                for (int k = 0; k < p.cluster; ++k) {
+                    const float2 t = cluster.map_shared_rank(s_total, k)[col];
+                    total += part_of(t.x, t.y, top);
+                    sum += t.x == -INFINITY ? 0.0f : cluster.map_shared_rank(s_o, k)[col * S::STRIDE + d] * ex2(t.x - top);
+                }
+                ((T *)a.out)[(seq * a.heads + head0) * DIM + i] = from_f32<T>(n <= 0 ? 0.0f : sum / total);
+            }
+            cluster.sync();
+            return;
+        }
         const bool whole = from == 0 && to == steps;
         float *slot = p.slots + (int64_t)(2 * blockIdx.x + (from == 0)) * p.cols * (DIM + 2);
         for (int i = threadIdx.x; i < heads * DIM; i += 32 * WARPS) {
             const int col = i / DIM, d = i % DIM;
-            float sum = 0.0f, total = 0.0f, top = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < WARPS * PAIR; ++k) top = fmaxf(top, s_m[k / PAIR][col + k % PAIR * 4]);
-#pragma unroll
-            for (int k = 0; k < WARPS * PAIR; ++k) {
-                const int from_col = col + k % PAIR * 4;
-                const float km = s_m[k / PAIR][from_col], kl = s_l[k / PAIR][from_col];
-                sum += s_o[(k / PAIR * COLS + from_col) * S::STRIDE + d];
-                total += km == -INFINITY ? (kl == kl ? 0.0f : NAN) : kl * ex2(km - top);
-            }
-            if (whole) ((T *)a.out)[(seq * a.heads + head0) * DIM + i] = from_f32<T>(n <= 0 ? 0.0f : sum / total);
+            const float sum = sum_of(col, d);
+            if (whole) ((T *)a.out)[(seq * a.heads + head0) * DIM + i] = from_f32<T>(n <= 0 ? 0.0f : sum / s_total[col].y);
             else {
                 slot[i] = sum;
-                if (d == 0) *reinterpret_cast<float2 *>(slot + p.cols * DIM + 2 * col) = make_float2(top, total);
+                if (d == 0) *reinterpret_cast<float2 *>(slot + p.cols * DIM + 2 * col) = s_total[col];
             }
         }
-        if (p.single) return;
+        if (p.cluster) return;
     }
 }
 
@@ -701,8 +741,14 @@ bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int
     p.tiles_per_page = page_size / TILE;
     p.most_tiles = (int)(max_pages * p.tiles_per_page);
     p.pair = group <= 4 && dim < 256 ? 2 : 1;      // (of 256 values of 8 bits two tiles would be 16 KB a step)
-    p.single = p.most_tiles <= SINGLE_TILES;
-    return batch * p.units < (int64_t)1 << 31;
+    // Clusters, where one wave of them (of 444 CTAs: three an SM) goes through the longest table in CLUSTER_ROUNDS steps a warp.  8 cache heads of 128, 4 bits:
+    // 4 sequences of 1000 tokens 8.0 us, in shares with a join 10.3; 16 of 600 10.9 / 13.9; 16 of up to 2048 (5.3 steps) 16.8 / 15.8: the longest is waited for.
+    const int64_t items = batch * p.units, steps = (p.most_tiles + p.pair - 1) / p.pair, wide = 444 / (items < 444 ? items : 444);
+    int64_t size = (steps + 2 * WARPS - 1) / (2 * WARPS);            // (a part of less than two steps a warp is not worth a CTA)
+    if (size > wide) size = wide;
+    size = size > 8 ? 8 : size < 1 ? 1 : size;
+    p.cluster = steps <= size * WARPS * (size > 1 ? CLUSTER_ROUNDS : 2) ? (int)size : 0;
+    return batch * p.units < (int64_t)1 << 28;
 }
 
 template <typename T, int BITS, int DIM, int NB, int PAIR>
@@ -720,10 +766,10 @@ int launch_fast(FastArgs &p, cudaStream_t st) {
         if (device < 64) per_sm[device] = n;
     }
     p.ctas = 148 * n;
-    const int64_t grid = p.single ? p.batch * p.units : p.ctas;
-    const int rc = launch_early("kv_attend_kernel", kern, dim3((unsigned)grid), 32 * WARPS, SMEM, st, p);
-    if (rc != BW_OK || p.single) return rc;
-    return launch_early("kv_attend_join_kernel", kv_attend_join_kernel<T, DIM>, dim3((unsigned)(p.batch * p.a.heads)), 128, 0, st, p);
+    if (p.cluster) return launch_early("kv_attend_kernel", kern, dim3((unsigned)(p.batch * p.units * p.cluster)), 32 * WARPS, SMEM, st, dim3(p.cluster), p);
+    const int rc = launch_early("kv_attend_kernel", kern, dim3((unsigned)p.ctas), 32 * WARPS, SMEM, st, dim3(1), p);
+    if (rc != BW_OK) return rc;
+    return launch_early("kv_attend_join_kernel", kv_attend_join_kernel<T, DIM>, dim3((unsigned)(p.batch * p.a.heads)), 128, 0, st, dim3(1), p);
 }
 
 template <typename T, int BITS, int DIM>
@@ -749,7 +795,7 @@ int launch_bits(FastArgs &p, int bits, cudaStream_t st) {
 
 size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages) {
     FastArgs p;
-    if (!fast_args(p, batch, heads, kv_heads, dim, page_size, max_pages) || p.single) return 0;
+    if (!fast_args(p, batch, heads, kv_heads, dim, page_size, max_pages) || p.cluster) return 0;
     return (size_t)2 * MOST_CTAS * p.cols * (dim + 2) * sizeof(float);
 }
 

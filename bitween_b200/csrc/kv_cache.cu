@@ -241,7 +241,7 @@ int append_typed(const void *kv, const void *vv, const int64_t *slots, const KvR
     constexpr int V = 16 / sizeof(T);
     bool vec = p.dim % E == 0 && aligned_to(k, 16) && aligned_to(v, 16);
     for (int i = 0; i < 2; ++i) vec = vec && p.stride[i] % V == 0 && p.head_stride[i] % V == 0;
-    return launch_early("kv_append_kernel", vec ? kv_append_kernel<T, BITS, true> : kv_append_kernel<T, BITS, false>, dim3(kv_grid(p)), 256, 0, st, k, v, slots, p,
+    return launch_early("kv_append_kernel", vec ? kv_append_kernel<T, BITS, true> : kv_append_kernel<T, BITS, false>, dim3(kv_grid(p)), 256, 0, st, dim3(1), k, v, slots, p,
                         kc, vc, (__half2 *)params);
 }
 template <typename T>
@@ -253,7 +253,7 @@ int append_bits(const void *k, const void *v, const int64_t *slots, const KvRows
 template <typename T, int BITS>
 int read_typed(const int32_t *kc, const int32_t *vc, const void *params, const int64_t *slots, const KvRows &p, void *k, void *v, cudaStream_t st) {
     // (k and v are dense and start on 16 bytes: so do all pieces of rows that are whole pieces)
-    return launch_early("kv_read_kernel", p.dim % E == 0 ? kv_read_kernel<T, BITS, true> : kv_read_kernel<T, BITS, false>, dim3(kv_grid(p)), 256, 0, st, kc, vc,
+    return launch_early("kv_read_kernel", p.dim % E == 0 ? kv_read_kernel<T, BITS, true> : kv_read_kernel<T, BITS, false>, dim3(kv_grid(p)), 256, 0, st, dim3(1), kc, vc,
                         (const uint2 *)params, slots, p, (T *)k, (T *)v);
 }
 template <typename T>
