@@ -216,10 +216,11 @@ struct Config {
     static constexpr int STAGES = STEP <= 2304 ? 4 : STEP <= 4352 ? 3 : 2;      // of a warp's ring: 9 to 17 KB
     static constexpr int RING = WARPS * STAGES * STEP, SUMS = WARPS * COLS * Shape<BITS, DIM>::STRIDE * 4;
     static constexpr int SMEM = RING > SUMS ? RING : SUMS;
+    static constexpr int CTAS = DIM == 256 ? 2 : NB == 2 ? (DIM == 64 ? 3 : 2) : BITS == 8 && DIM == 128 ? 3 : 4;      // an SM, which registers are made to fit
 };
 
 template <typename T, int BITS, int DIM, int NB, int PAIR>
-__global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p) {
+__global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::CTAS)) kv_attend_kernel(const FastArgs p) {
     using S = Shape<BITS, DIM>;
     using C = Config<T, BITS, DIM, NB, PAIR>;
     static_assert(PAIR == 1 || NB == 1, "steps of two tiles are for groups of up to four heads");
@@ -302,40 +303,31 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
         const int64_t head0 = (int64_t)kh * group + h0;
         __syncthreads();
 
-        // pages: `page_at` and `in` go forward with the warp's tiles; the ids are loaded a step before they are needed
+        // Where the warp's tiles lie: a lane looks up one tile of the next 32, a batch ahead of its use, and hands its first row of the cache around.
         bool bad = n > p.most_tiles * TILE;          // more than the table holds (pages are whole tiles)
-        int step = from + warp;                       // of the next look-up
-        int page_at = step * PAIR / p.tiles_per_page, in_page = step * PAIR - page_at * p.tiles_per_page;
-        const int step_pages = WARPS * PAIR / p.tiles_per_page, step_in = WARPS * PAIR - step_pages * p.tiles_per_page;
         const int32_t *pages = a.table + seq * a.table_stride;
-        auto look_up = [&](int (&page)[PAIR], int (&place)[PAIR]) {
-            int at_page = page_at, at_in = in_page;
-#pragma unroll
-            for (int i = 0; i < PAIR; ++i) {
-                place[i] = at_in;
-                page[i] = step < to && step * PAIR + i < tiles ? __ldcg(pages + at_page) : -2;
-                if (++at_in == p.tiles_per_page) {
-                    at_in = 0;
-                    ++at_page;
-                }
+        constexpr int BATCH = 32 / PAIR;              // steps
+        constexpr uint32_t NONE = 0xffffffffu, BAD = 0xfffffffeu;
+        auto look_up = [&](int step0) {
+            const int tile = (step0 + lane / PAIR * WARPS) * PAIR + lane % PAIR;
+            uint32_t row = NONE;
+            if (tile < to * PAIR && tile < tiles) {
+                const int at_page = tile / p.tiles_per_page;
+                const uint32_t page = (uint32_t)__ldcg(pages + at_page);
+                row = page < (uint32_t)a.pages ? page * (uint32_t)(a.kv_heads * a.page_size) + (uint32_t)(kh * a.page_size + (tile - at_page * p.tiles_per_page) * TILE) : BAD;
             }
-            page_at += step_pages;
-            in_page += step_in;
-            if (in_page >= p.tiles_per_page) {
-                in_page -= p.tiles_per_page;
-                ++page_at;
-            }
-            step += WARPS;
+            return row;
         };
-        const int page_rows = a.kv_heads * a.page_size, head_row = kh * a.page_size;
-        auto copy_step = [&](int stage, const int (&page)[PAIR], const int (&place)[PAIR]) {
-            const uint32_t to_smem = ring + stage * C::STEP;
+        uint32_t rows = look_up(from + warp), rows_ahead = look_up(from + warp + BATCH * WARPS);
+        int looked = from + warp, in_batch = 0;       // first step of `rows`; steps of it that have been copied
+        const uint8_t *k_at = reinterpret_cast<const uint8_t *>(a.k_codes) + lane * 16, *v_at = reinterpret_cast<const uint8_t *>(a.v_codes) + lane * 16,
+                      *c_at = reinterpret_cast<const uint8_t *>(a.params) + lane * 16;
+        auto copy_step = [&](uint32_t to_smem) {      // the next step into the ring
 #pragma unroll
             for (int i = 0; i < PAIR; ++i) {
-                if (page[i] >= 0 && page[i] < a.pages) {
-                    const int64_t row0 = (int64_t)page[i] * page_rows + (head_row + place[i] * TILE);
-                    const uint8_t *k = reinterpret_cast<const uint8_t *>(a.k_codes) + row0 * S::ROW + lane * 16;
-                    const uint8_t *v = reinterpret_cast<const uint8_t *>(a.v_codes) + row0 * S::ROW + lane * 16;
+                const uint32_t row0 = __shfl_sync(0xffffffffu, rows, in_batch * PAIR + i);
+                if (row0 < BAD) {
+                    const uint8_t *k = k_at + (uint64_t)row0 * S::ROW, *v = v_at + (uint64_t)row0 * S::ROW;
                     const uint32_t t = to_smem + i * S::BYTES;
 #pragma unroll
                     for (int j = 0; j < (S::ROW + 31) / 32; ++j) {
@@ -346,16 +338,19 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
                             copy16(o + 16 * S::ROW, v + j * 512);
                         }
                     }
-                    if (lane < 8) copy16(t + 32 * S::ROW + lane * 16, reinterpret_cast<const uint8_t *>(a.params) + row0 * 8 + lane * 16);
-                } else if (page[i] != -2) bad = true;
+                    if (lane < 8) copy16(t + 32 * S::ROW + lane * 16, c_at + (uint64_t)row0 * 8);
+                } else if (row0 == BAD) bad = true;
             }
             copies_commit();
+            if (++in_batch == BATCH) {
+                in_batch = 0;
+                looked += BATCH * WARPS;
+                rows = rows_ahead;
+                rows_ahead = look_up(looked + BATCH * WARPS);
+            }
         };
-        int page[STAGES][PAIR], place[STAGES][PAIR];
 #pragma unroll
-        for (int i = 0; i < STAGES; ++i) look_up(page[i], place[i]);
-#pragma unroll
-        for (int i = 0; i < STAGES - 1; ++i) copy_step(i, page[i], place[i]);
+        for (int i = 0; i < STAGES - 1; ++i) copy_step(ring + i * C::STEP);
 
         // the queries in fp16: as they are, or (bf16) divided by a power of two near their largest value, which the scores get back
         for (int h = warp; h < HEADS; h += WARPS) {
@@ -416,8 +411,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv_attend_kernel(const FastArgs p)
         for (int now = from + warp; now < to; now += WARPS) {
             copies_wait<STAGES - 2>();
             __syncwarp();                                     // all lanes' copies are there, and all have used the stage that is filled next
-            copy_step(next, page[STAGES - 1], place[STAGES - 1]);
-            look_up(page[STAGES - 1], place[STAGES - 1]);
+            copy_step(ring + next * C::STEP);
             const uint32_t buf = ring + stage * C::STEP;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             next = next + 1 == STAGES ? 0 : next + 1;
@@ -731,8 +725,9 @@ __global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
 }
 
 // Whether the tiled kernel takes this cache, and how it divides a call.
-bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages) {
-    if ((dim != 64 && dim != 128 && dim != 256) || page_size % TILE != 0 || (int64_t)kv_heads * page_size > INT32_MAX) return false;
+bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int64_t pages, int page_size, int64_t max_pages) {
+    // (rows of the cache are numbered in 32 bits)
+    if ((dim != 64 && dim != 128 && dim != 256) || page_size % TILE != 0 || pages * kv_heads * page_size >= 0xfffffffell) return false;
     const int group = heads / kv_heads;
     p.batch = batch;
     p.cols = group > 8 && dim < 256 ? 16 : 8;
@@ -795,7 +790,7 @@ int launch_bits(FastArgs &p, int bits, cudaStream_t st) {
 
 size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages) {
     FastArgs p;
-    if (!fast_args(p, batch, heads, kv_heads, dim, page_size, max_pages) || p.cluster) return 0;
+    if (!fast_args(p, batch, heads, kv_heads, dim, 0, page_size, max_pages) || p.cluster) return 0;      // (a cache of more rows asks for scratch that it does not use)
     return (size_t)2 * MOST_CTAS * p.cols * (dim + 2) * sizeof(float);
 }
 
@@ -805,7 +800,7 @@ int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stri
     FastArgs f = {};
     AttendArgs p = {q, kc, vc, (const __half2 *)params, table, lengths, out, q_stride, q_head_stride, table_stride, pages,
                     heads, kv_heads, dim, dim * bits / 32, page_size, max_pages, alpha};
-    if (fast_args(f, batch, heads, kv_heads, dim, page_size, max_pages)) {
+    if (fast_args(f, batch, heads, kv_heads, dim, pages, page_size, max_pages)) {
         f.a = p;
         f.slots = (float *)workspace;
         return dtype == BW_F16 ? launch_bits<__half>(f, bits, st) : launch_bits<__nv_bfloat16>(f, bits, st);
