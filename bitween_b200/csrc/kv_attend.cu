@@ -158,8 +158,15 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 __device__ __forceinline__ uint32_t as_u32(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t to, const uint8_t *from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+// (a predicate, not a branch: the loop has ten of these)
+__device__ __forceinline__ void copy16_if(bool ok, uint32_t to, const uint8_t *from) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %0, 0;\n @p cp.async.cg.shared.global [%1], [%2], 16;\n}" ::"r"((int)ok), "r"(to), "l"(from) : "memory");
+}
+// (x & bits) | magic in one operation: the compiler, which knows both constants, makes two of it.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t bits, uint32_t magic) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(bits), "r"(magic));
+    return y;
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -326,20 +333,20 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
             for (int i = 0; i < PAIR; ++i) {
                 const uint32_t row0 = __shfl_sync(0xffffffffu, rows, in_batch * PAIR + i);
-                if (row0 < BAD) {
+                const bool ok = row0 < BAD;
+                bad |= row0 == BAD;
+                {
                     const uint8_t *k = k_at + (uint64_t)row0 * S::ROW, *v = v_at + (uint64_t)row0 * S::ROW;
                     const uint32_t t = to_smem + i * S::BYTES;
 #pragma unroll
                     for (int j = 0; j < (S::ROW + 31) / 32; ++j) {
                         const int piece = lane + 32 * j, row = piece / S::PIECES;
                         const uint32_t o = t + row * S::ROW + ((piece % S::PIECES) ^ S::swizzle(row)) * 16;
-                        if (S::ROW >= 32 || lane < 16) {
-                            copy16(o, k + j * 512);
-                            copy16(o + 16 * S::ROW, v + j * 512);
-                        }
+                        copy16_if(ok && (S::ROW >= 32 || lane < 16), o, k + j * 512);
+                        copy16_if(ok && (S::ROW >= 32 || lane < 16), o + 16 * S::ROW, v + j * 512);
                     }
-                    if (lane < 8) copy16(t + 32 * S::ROW + lane * 16, c_at + (uint64_t)row0 * 8);
-                } else if (row0 == BAD) bad = true;
+                    copy16_if(ok && lane < 8, t + 32 * S::ROW + lane * 16, c_at + (uint64_t)row0 * 8);
+                }
             }
             copies_commit();
             if (++in_batch == BATCH) {
@@ -402,6 +409,8 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
             }
         }
 
+        uint32_t magic;                                       // 1024 in both halves
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
         float o[NB][S::MMAS][4] = {}, m[NB][2], l[NB][2] = {};
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = -INFINITY;
@@ -563,10 +572,10 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
                         for (int pl = 0; pl < S::PLANES; ++pl) {
                             const uint32_t bits = ((1u << BITS) - 1) * 0x00010001u << (pl * BITS);
-                            const uint32_t a0 = as_u32(__hsub2(as_half2((x0 & bits) | 0x64006400u), zero[pl][0]));
-                            const uint32_t a1 = as_u32(__hsub2(as_half2((y0 & bits) | 0x64006400u), zero[pl][0]));
-                            const uint32_t a2 = as_u32(__hsub2(as_half2((x1 & bits) | 0x64006400u), zero[pl][1]));
-                            const uint32_t a3 = as_u32(__hsub2(as_half2((y1 & bits) | 0x64006400u), zero[pl][1]));
+                            const uint32_t a0 = as_u32(__hsub2(as_half2(and_or(x0, bits, magic)), zero[pl][0]));
+                            const uint32_t a1 = as_u32(__hsub2(as_half2(and_or(y0, bits, magic)), zero[pl][0]));
+                            const uint32_t a2 = as_u32(__hsub2(as_half2(and_or(x1, bits, magic)), zero[pl][1]));
+                            const uint32_t a3 = as_u32(__hsub2(as_half2(and_or(y1, bits, magic)), zero[pl][1]));
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
                                 mma(o[nb][(piece + h) * S::PLANES + pl], a0, a1, a2, a3, b0[nb][0], b1[nb][0]);
