@@ -498,12 +498,16 @@ def run_case(args, torch, device):
     """`--case kind:shape:tokens[:bits[:group]]` -- one kernel on one Llama-3-8B shape, a handful of
     plain (ungraphed) launches over 4 distinct layer copies, so that a profiler can capture a single
     launch without the rest of the benchmark.  kind: decode | prefill (both the qmatmul call),
-    rtn, gradinput, fakequant.  Prints one small JSON line with the CUDA-event time per launch."""
+    rtn, gradinput, fakequant; adapter | adaptertrain (`...:shape:tokens:rank`, one adapter beside that shape);
+    attend | append | read (`...:sequences x tokens:bits`, 32 query and 8 cache heads of 128).
+    Prints one small JSON line with the CUDA-event time per launch."""
     from bitween_b200 import functional as fn
     from bitween_b200.kernels import _lib
     from bitween_b200.kernels.cuda_loader import quantized_matmul_cuda as qmm, quantized_matmul_grad_input as qgrad
     parts = args.case.split(":")
     kind, shape = parts[0], parts[1]
+    if kind in ("attend", "append", "read"):
+        return run_cache_case(args, torch, device, kind, *(int(v) for v in shape.split("x")), int(parts[2]) if len(parts) > 2 else 4)
     M = int(parts[2]) if len(parts) > 2 else 1
     bits = int(parts[3]) if len(parts) > 3 else 4
     g = int(parts[4]) if len(parts) > 4 else 128
@@ -531,6 +535,18 @@ def run_case(args, torch, device):
         def body(wl):
             wl.min_scale.grad = wl.max_scale.grad = None
             wl._quantize_weight_with_learnable_params()[0].backward(r)
+    elif kind in ("adapter", "adaptertrain"):
+        from bitween_b200 import adapter_matmul
+        rank = int(parts[3]) if len(parts) > 3 else 16
+        index = torch.zeros(M, dtype=torch.int32, device=device)
+        grad = torch.randn(M, N, device=device, generator=gen).to(torch.bfloat16)
+        layers = [[torch.randn(s, device=device, generator=gen).to(torch.bfloat16).requires_grad_(kind == "adaptertrain")
+                   for s in ((M, K), (1, rank, K), (1, rank, N))] for _ in range(copies)]
+
+        def body(bank):
+            y = adapter_matmul(*bank, index, base=grad)
+            if kind == "adaptertrain":
+                torch.autograd.grad(y, bank, grad)
     else:
         raise SystemExit(f"unknown case kind {kind!r}")
     for L in layers:                       # warm-up pass (also the launches a profiler skips)
@@ -538,6 +554,38 @@ def run_case(args, torch, device):
     ms = time_region(torch, lambda: [body(L) for L in layers]) / copies
     print(json.dumps({"case": args.case, "kernel": _lib.last_kernel() if kind in ("decode", "prefill") else kind,
                       "us_per_launch": round(ms * 1e3, 2), "copies": copies,
+                      "note": "plain launches, back to back, no L2 flush: a profiling aid, not a benchmark value"}), flush=True)
+
+
+def run_cache_case(args, torch, device, kind, sequences, tokens, bits):
+    """The key-value cache's part of run_case: every sequence has `tokens` rows on scattered pages of 16."""
+    from bitween_b200 import QuantizedKVCache
+    from bitween_b200.kernels import _lib
+    gen = torch.Generator(device=device).manual_seed(6)
+    wide = -(-tokens // 16)
+    cache = QuantizedKVCache(sequences * wide, 16, 8, 128, bits=bits, device=device)
+    table = torch.randperm(sequences * wide, generator=gen, device=device).view(sequences, wide)
+    pos = torch.arange(tokens, device=device)
+    slots = (table[:, pos // 16] * 16 + pos % 16).flatten()
+    for part in slots.split(1 << 16):
+        rows = torch.randn(part.numel(), 16, 128, device=device, generator=gen).to(torch.bfloat16)
+        cache.append(rows[:, :8], rows[:, 8:], part)
+    q = torch.randn(sequences, 32, 128, device=device, generator=gen).to(torch.bfloat16)
+    lengths = torch.full((sequences,), tokens, dtype=torch.int32, device=device)
+    table = table.to(torch.int32)
+    last = slots[-(1 << 16):]
+    rows = torch.randn(last.numel(), 16, 128, device=device, generator=gen).to(torch.bfloat16)
+    body = {"attend": lambda: cache.attend(q, table, lengths), "append": lambda: cache.append(rows[:, :8], rows[:, 8:], last),
+            "read": lambda: cache.read(last, dtype=torch.bfloat16)}[kind]
+    copies = 4
+
+    def some():
+        for _ in range(copies):
+            body()
+
+    some()
+    ms = time_region(torch, some) / copies
+    print(json.dumps({"case": args.case, "kernel": _lib.last_kernel(), "us_per_launch": round(ms * 1e3, 2), "copies": copies,
                       "note": "plain launches, back to back, no L2 flush: a profiling aid, not a benchmark value"}), flush=True)
 
 
@@ -782,7 +830,7 @@ def main():
     ap.add_argument("--graph", type=int, default=1, help="replay each step as one CUDA graph")
     ap.add_argument("--tp-layers", type=int, default=3, help="70B-shaped decoder layers of the tensor-parallel workload")
     ap.add_argument("--rtn-layers", type=int, default=80, help="70B-shaped layers whose weights the sharded RTN run quantizes")
-    ap.add_argument("--case", default="", help="kind:shape:tokens[:bits[:group]] -- run one kernel on one shape (for profilers)")
+    ap.add_argument("--case", default="", help="kind:shape:tokens[:bits[:group]] -- run one kernel on one shape (for profilers; run_case lists the kinds)")
     ap.add_argument("--no-extra", action="store_true")
     ap.add_argument("--no-cpu", action="store_true")
     args = ap.parse_args()

@@ -142,3 +142,51 @@ def test_modes_and_subclasses_go_the_python_way():
         y = adapter_matmul(x, down, up, index, scaling=scaling, base=base)
     side.synchronize()
     assert torch.equal(y, want) and math.isfinite(float(y.float().sum()))
+
+
+@pytest.mark.gpu
+def test_first_calls_may_be_captured():
+    """Nothing that a first call sets up keeps it from being captured: a process whose first call of each kind is in a graph."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    program = """
+import torch
+from bitween_b200 import QuantizedKVCache, adapter_matmul
+dev = "cuda"
+g = torch.Generator(device=dev).manual_seed(0)
+cache = QuantizedKVCache(700, 16, 2, 128, bits=4, device=dev)
+k, v = (torch.randn(10000, 2, 128, generator=g, device=dev).half() for _ in range(2))
+slots = torch.arange(10000, device=dev)
+table = torch.arange(700, device=dev, dtype=torch.int32)[None].contiguous()
+n = torch.tensor([9990], dtype=torch.int32, device=dev)
+short = torch.tensor([300], dtype=torch.int32, device=dev)
+q = torch.randn(1, 8, 128, generator=g, device=dev).half()
+banks = []
+for M in (20, 300):
+    x = torch.randn(M, 512, generator=g, device=dev).half()
+    down, up = torch.randn(2, 32, 512, generator=g, device=dev).half() / 20, torch.randn(2, 32, 256, generator=g, device=dev).half() / 20
+    banks.append((x, down, up, torch.randint(-1, 2, (M,), generator=g, device=dev).int(), torch.randn(M, 256, generator=g, device=dev).half()))
+
+def step():
+    cache.append(k, v, slots)
+    out = [cache.attend(q, table, n), cache.attend(q, table[:, :20], short), *cache.read(slots)]
+    for x, down, up, index, grad in banks:
+        leaves = [t.detach().requires_grad_() for t in (x, down, up)]
+        y = adapter_matmul(*leaves, index)
+        out += [y.detach(), *torch.autograd.grad(y, leaves, grad)]
+    return out
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = step()
+graph.replay()
+torch.cuda.synchronize()
+want = step()
+assert all(torch.equal(a, b) for a, b in zip(got, want)), [torch.equal(a, b) for a, b in zip(got, want)]
+assert got[0].isfinite().all()
+"""
+    r = subprocess.run([sys.executable, "-c", program], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
