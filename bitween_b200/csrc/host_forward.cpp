@@ -21,8 +21,10 @@
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -299,55 +301,66 @@ int adapter_call(const at::Tensor &x, const at::Tensor &down, const at::Tensor &
                                  c10::cuda::getCurrentCUDAStream(device.index()).stream());
 }
 
-// AdapterFunction of the Python package (adapters.py), with the same gradients and the same error where they are differentiated again.
-struct AdapterNode : torch::autograd::Function<AdapterNode> {
-    static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &down, const at::Tensor &up, const at::Tensor &index,
-                              const std::optional<at::Tensor> &scaling_or, const std::optional<at::Tensor> &base_or) {
-        at::Tensor out, hidden;
-        const at::Tensor scaling = scaling_or.value_or(at::Tensor()), base = base_or.value_or(at::Tensor());
-        const int rc = adapter_call(x, down, up, index, scaling, base, out, hidden);
-        TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_adapter_forward returned status ", rc);
-        ctx->save_for_backward({x, down, up, index, scaling, up.requires_grad() ? hidden : at::Tensor()});
-        ctx->saved_data["base"] = base.defined();
-        return out;
+// AdapterFunction of the Python package (adapters.py) as a node of the graph, with the same gradients and the same error where they are differentiated
+// again.  Edges: x, down, up, base.
+struct AdapterNode : torch::autograd::Node {
+    torch::autograd::SavedVariable x, down, up, index, scaling, hidden;
+
+    std::string name() const override { return "AdapterNode"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (auto *v : {&x, &down, &up, &index, &scaling, &hidden}) v->reset_data();
     }
-    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        const auto saved = ctx->get_saved_variables();
-        const at::Tensor &x = saved[0], &down = saved[1], &up = saved[2], &index = saved[3], &scaling = saved[4], &hidden = saved[5];
-        at::Tensor g = grads[0], gx, gdown, gup;
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        torch::autograd::variable_list result(4);
+        const at::Tensor g = grads[0];
+        if (!g.defined()) return result;
         const bool again = c10::GradMode::is_enabled();
-        {
+        if (task_should_compute_output(0) || task_should_compute_output(1) || task_should_compute_output(2)) {
+            const at::Tensor xt = x.unpack(), dt = down.unpack(), ut = up.unpack(), it = index.unpack(), st = scaling.unpack(), ht = hidden.unpack();
             at::AutoGradMode off(false);
-            const int64_t K = down.size(2), N = up.size(2), M = x.numel() / K;
-            const c10::Device device = x.device();
+            const int64_t K = dt.size(2), N = ut.size(2), M = xt.numel() / K;
             at::Tensor dense = g.contiguous();
             if (!on_16_bytes(dense)) dense = dense.clone();
-            if (ctx->needs_input_grad(0)) gx = at::empty_like(x);
-            if (ctx->needs_input_grad(1)) gdown = at::empty_like(down);
-            if (ctx->needs_input_grad(2)) gup = at::empty_like(up);
-            if (gx.defined() || gdown.defined() || gup.defined()) {
-                const at::Tensor ws = bytes_of(g_ops.adapter_bytes(M, (int)down.size(1)), device);
-                const int rc = g_ops.adapter_backward(
-                    dense.const_data_ptr(), float_code(x.scalar_type()), x.const_data_ptr(), M, N, K, down.const_data_ptr(), up.const_data_ptr(),
-                    (int)down.size(0), (int)down.size(1), static_cast<const int32_t *>(index.const_data_ptr()),
-                    scaling.defined() ? static_cast<const float *>(scaling.const_data_ptr()) : nullptr, hidden.defined() ? hidden.const_data_ptr() : nullptr,
-                    hidden.defined() ? (size_t)hidden.numel() : 0, gx.defined() ? gx.mutable_data_ptr() : nullptr,
-                    gdown.defined() ? gdown.mutable_data_ptr() : nullptr, gup.defined() ? gup.mutable_data_ptr() : nullptr, ws.mutable_data_ptr(),
-                    (size_t)ws.numel(), c10::cuda::getCurrentCUDAStream(device.index()).stream());
-                TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_adapter_backward returned status ", rc);
-            }
+            const at::Tensor *like[3] = {&xt, &dt, &ut};
+            for (int i = 0; i < 3; ++i)
+                if (task_should_compute_output(i)) result[i] = fresh(like[i]->sizes(), like[i]->scalar_type(), like[i]->device());
+            const at::Tensor ws = bytes_of(g_ops.adapter_bytes(M, (int)dt.size(1)), xt.device());
+            const auto into = [&](int i) { return result[i].defined() ? result[i].mutable_data_ptr() : nullptr; };
+            const int rc = g_ops.adapter_backward(dense.const_data_ptr(), float_code(xt.scalar_type()), xt.const_data_ptr(), M, N, K, dt.const_data_ptr(),
+                                                  ut.const_data_ptr(), (int)dt.size(0), (int)dt.size(1), static_cast<const int32_t *>(it.const_data_ptr()),
+                                                  st.defined() ? static_cast<const float *>(st.const_data_ptr()) : nullptr,
+                                                  ht.defined() ? ht.const_data_ptr() : nullptr, ht.defined() ? (size_t)ht.numel() : 0, into(0), into(1), into(2),
+                                                  ws.mutable_data_ptr(), (size_t)ws.numel(), c10::cuda::getCurrentCUDAStream(xt.device().index()).stream());
+            TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_adapter_backward returned status ", rc);
         }
-        torch::autograd::variable_list result = {gx, gdown, gup};
         if (again) {
             // as once_differentiable has it: an error for whoever differentiates these
             for (auto &t : result)
                 if (t.defined()) t = (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", 1))(
                                      {t.detach().requires_grad_()})[0];
         }
-        result.insert(result.end(), {at::Tensor(), at::Tensor(), ctx->saved_data["base"].toBool() ? g : at::Tensor()});
+        if (task_should_compute_output(3)) result[3] = g;
         return result;
     }
 };
+
+// The recorded call: null where it cannot be made (nothing has been launched then).
+at::Tensor adapter_recorded(const at::Tensor &x, const at::Tensor &down, const at::Tensor &up, const at::Tensor &index, const at::Tensor &scaling, const at::Tensor &base) {
+    at::Tensor out, hidden;
+    if (adapter_call(x, down, up, index, scaling, base, out, hidden) != BW_OK) return at::Tensor();
+    const std::shared_ptr<AdapterNode> node(new AdapterNode(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x, down, up, base));
+    node->x = torch::autograd::SavedVariable(x, false);
+    node->down = torch::autograd::SavedVariable(down, false);
+    node->up = torch::autograd::SavedVariable(up, false);
+    node->index = torch::autograd::SavedVariable(index, false);
+    node->scaling = torch::autograd::SavedVariable(scaling, false);
+    node->hidden = torch::autograd::SavedVariable(up.requires_grad() ? hidden : at::Tensor(), false);
+    torch::autograd::set_history(out, node);
+    return out;
+}
 
 // adapter_matmul(x, down, up, index, scaling, base, out): the result (`out` only where no gradient is recorded)
 PyObject *adapter_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
@@ -378,8 +391,11 @@ PyObject *adapter_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     at::Tensor out;
     if (recording) {
         if (given) Py_RETURN_NONE;
-        pybind11::gil_scoped_release no_gil;
-        out = AdapterNode::apply(*x, *down, *up, *index, scaling ? std::make_optional(*scaling) : std::nullopt, base ? std::make_optional(*base) : std::nullopt);
+        {
+            pybind11::gil_scoped_release no_gil;
+            out = adapter_recorded(*x, *down, *up, *index, scaling ? *scaling : none, base ? *base : none);
+        }
+        if (!out.defined()) Py_RETURN_NONE;
     } else {
         if (given) {
             const uintptr_t o = reinterpret_cast<uintptr_t>(given->const_data_ptr());
