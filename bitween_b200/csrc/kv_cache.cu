@@ -16,16 +16,32 @@
 namespace bw {
 namespace {
 
+// Division of 32-bit numbers by one that is known on the host: the high half of a product, and shifts (Granlund and Montgomery).
+struct Divisor {
+    uint32_t d, m;
+    int sh1, sh2;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        const uint32_t t = __umulhi(m, n);
+        return (t + ((n - t) >> sh1)) >> sh2;
+    }
+};
+Divisor divisor(uint32_t d) {
+    int l = 0;
+    while (l < 32 && ((uint64_t)1 << l) < d) ++l;
+    return {d, (uint32_t)((((uint64_t)1 << l) - d) * ((uint64_t)1 << 32) / d + 1), l < 1 ? l : 1, l < 1 ? 0 : l - 1};
+}
+
 struct KvRows {
     int64_t tokens, slots;      // rows of tokens in the call; pages * page_size
     int64_t stride[2], head_stride[2];   // of k and v, in elements
+    Divisor by_heads, by_page;
     int heads, dim, words, page_size;
     int lanes;                  // of a row: the power of two that holds its pieces
 };
 
 // Where a slot's row of a head lies, in rows of the cache.
 __device__ __forceinline__ int64_t cache_row(const KvRows &p, int64_t slot, int head) {
-    const int64_t page = slot >> 32 ? slot / p.page_size : (int64_t)((uint32_t)slot / (uint32_t)p.page_size);
+    const int64_t page = slot >> 32 ? slot / p.page_size : (int64_t)p.by_page((uint32_t)slot);
     return (page * p.heads + head) * p.page_size + (slot - page * p.page_size);
 }
 
@@ -101,13 +117,19 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T *__restrict__ k,
     constexpr float Q = (1 << BITS) - 1, RQ = 1.0f / Q;
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = row / (uint32_t)p.heads;
+    const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = p.by_heads(row);
     const int head = (int)(row - token * (uint32_t)p.heads), lane = threadIdx.x % p.lanes, at = lane * E;
     const int64_t slot = token < p.tokens ? __ldcg(slots + token) : -1;
     const bool in = slot >= 0 && slot < p.slots, live = in && at < p.dim;
     float x[2][E], lo[2], hi[2];
-    load_values<T, VEC>(k + (in ? token * p.stride[0] + head * p.head_stride[0] : 0), at, p.dim, live, x[0], lo[0], hi[0]);
-    load_values<T, VEC>(v + (in ? token * p.stride[1] + head * p.head_stride[1] : 0), at, p.dim, live, x[1], lo[1], hi[1]);
+    // (strides that are read 16 bytes at a time are known to fit 32 bits: a product of 64 bits is three operations)
+    const auto offset = [&](int j) {
+        if (!in) return (int64_t)0;
+        if constexpr (VEC) return (int64_t)((uint64_t)token * (uint32_t)p.stride[j] + (uint64_t)(uint32_t)head * (uint32_t)p.head_stride[j]);
+        return token * p.stride[j] + head * p.head_stride[j];
+    };
+    load_values<T, VEC>(k + offset(0), at, p.dim, live, x[0], lo[0], hi[0]);
+    load_values<T, VEC>(v + offset(1), at, p.dim, live, x[1], lo[1], hi[1]);
     for (int d = p.lanes / 2; d; d >>= 1)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -200,7 +222,7 @@ __global__ void __launch_bounds__(256) kv_read_kernel(const int32_t *__restrict_
                                                       const uint2 *__restrict__ params, const int64_t *__restrict__ slots, const KvRows p, T *k, T *v) {
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = row / (uint32_t)p.heads;
+    const uint32_t row = blockIdx.x * (256 / p.lanes) + threadIdx.x / p.lanes, token = p.by_heads(row);
     const int lane = threadIdx.x % p.lanes;
     if (token >= p.tokens || lane * E >= p.dim) return;
     const int64_t slot = __ldcg(slots + token), to = (int64_t)row * p.dim + lane * E;
@@ -224,6 +246,8 @@ KvRows kv_rows(int64_t tokens, int heads, int dim, int bits, int64_t pages, int 
     p.dim = dim;
     p.words = dim * bits / 32;
     p.page_size = page_size;
+    p.by_heads = divisor((uint32_t)heads);
+    p.by_page = divisor((uint32_t)page_size);
     const int pieces = (dim + E - 1) / E;
     p.lanes = 1;
     while (p.lanes < pieces) p.lanes *= 2;
@@ -240,7 +264,8 @@ int append_typed(const void *kv, const void *vv, const int64_t *slots, const KvR
     const T *k = (const T *)kv, *v = (const T *)vv;
     constexpr int V = 16 / sizeof(T);
     bool vec = p.dim % E == 0 && aligned_to(k, 16) && aligned_to(v, 16);
-    for (int i = 0; i < 2; ++i) vec = vec && p.stride[i] % V == 0 && p.head_stride[i] % V == 0;
+    for (int i = 0; i < 2; ++i)
+        for (int64_t stride : {p.stride[i], p.head_stride[i]}) vec = vec && stride % V == 0 && stride >= 0 && stride <= UINT32_MAX;
     return launch_early("kv_append_kernel", vec ? kv_append_kernel<T, BITS, true> : kv_append_kernel<T, BITS, false>, dim3(kv_grid(p)), 256, 0, st, dim3(1), k, v, slots, p,
                         kc, vc, (__half2 *)params);
 }
