@@ -345,24 +345,25 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
         for (int s = 0; s < STAGES - 1; ++s) copy_stage(begin + s * 64, s);
         float acc[NBR][4] = {};
         const bool busy = warp * 16 < tile.count;
+        // a lane's places in the stage (rows of x, of w; a step of 16 columns changes bits 5 and 6)
+        const uint32_t x_place = (warp * 16 + lane % 16) * 128 + ((lane / 16) ^ (lane & 7)) * 16,
+                       w_place = TILE * 128 + (NBR == 1 ? lane % 8 : lane % 8 + lane / 16 * 8) * 128 + ((lane / 8 % 2) ^ (lane & 7)) * 16;
         int stage = 0;
         for (int64_t k = begin; k < end; k += 64) {
             copies_wait<STAGES - 2>();
             __syncthreads();                                 // the stage is there for all, and the one filled next has been used by all
             copy_stage(k + (STAGES - 1) * 64, stage == 0 ? STAGES - 1 : stage - 1);
-            const uint32_t xs = ring + stage * STAGE, ws = xs + TILE * 128;
+            const uint32_t at = ring + stage * STAGE;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             if (busy) {
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk) {
                     uint32_t xa[4];
-                    const int row = warp * 16 + lane % 16;
-                    load_matrices(xs + row * 128 + (((2 * kk + lane / 16) ^ (row & 7)) * 16), xa);
+                    load_matrices(at + (x_place ^ kk * 32), xa);
 #pragma unroll
                     for (int nb = 0; nb < NBR; nb += 2) {
-                        uint32_t b[4];
-                        const int rank = (nb * 8 + lane % 8 + lane / 16 * 8) % RANKS;      // (rank 8: the second pair is the first again)
-                        load_matrices(ws + rank * 128 + (((2 * kk + lane / 8 % 2) ^ (rank & 7)) * 16), b);
+                        uint32_t b[4];                                   // (rank 8: the second pair is the first again)
+                        load_matrices(at + (w_place ^ kk * 32) + nb * 1024, b);
                         Pair<T>::mma(acc[nb], xa, b[0], b[1]);
                         if (nb + 1 < NBR) Pair<T>::mma(acc[nb + 1 < NBR ? nb + 1 : nb], xa, b[2], b[3]);
                     }
@@ -534,11 +535,14 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
         const float f[2] = {row_factor(h, p, a, t[0], live[0]), row_factor(h, p, a, t[1], live[1])};
         int stage = 0;
         const bool busy = warp * 16 < tile.count;
+        // a lane's places in the stage: row 2 c of a step of 16 ranks, piece r; piece 2 c of its row of base; and its results
+        const uint32_t w_place = c * 256 + (r ^ c << 1) * 16, base_place = W_BYTES + row * 128 + ((2 * c) ^ r) * 16;
+        T *const to[2] = {out + t[0] * p.cols + 16 * c, out + t[1] * p.cols + 16 * c};
         for (int64_t cb = begin; cb < end; cb += 64) {
             copies_wait<STAGES - 2>();
             __syncthreads();
             copy_stage(cb + (STAGES - 1) * 64, stage == 0 ? STAGES - 1 : stage - 1);
-            const uint32_t ws = ring + stage * STAGE, bs = ws + W_BYTES + row * 128;
+            const uint32_t at = ring + stage * STAGE;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             if (!busy) continue;
             float acc[8][4] = {};
@@ -547,10 +551,7 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
                 for (int ks = 0; ks < KS; ++ks) {
                     uint4 raw[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int j = 16 * ks + 2 * c + k % 2 + k / 2 * 8;
-                        raw[k] = load_shared16(ws + j * 128 + (r ^ (j >> 1 & 3) << 1) * 16);
-                    }
+                    for (int k = 0; k < 4; ++k) raw[k] = load_shared16(at + w_place + ks * 2048 + k % 2 * 128 + k / 2 * 1024);
 #pragma unroll
                     for (int n = 0; n < 8; ++n) {
                         const uint32_t b0 = column_pair(raw[0], raw[1], n), b1 = column_pair(raw[2], raw[3], n);
@@ -561,10 +562,10 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
             }
             uint4 old[2][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) old[j / 2][j % 2] = base ? load_shared16(bs + j / 2 * 1024 + ((2 * c + j % 2) ^ (row & 7)) * 16) : make_uint4(0, 0, 0, 0);
-            T *const to[2] = {out + t[0] * p.cols + cb + 16 * c, out + t[1] * p.cols + cb + 16 * c};
+            for (int j = 0; j < 4; ++j) old[j / 2][j % 2] = base ? load_shared16(at + (base_place ^ j % 2 * 16) + j / 2 * 1024) : make_uint4(0, 0, 0, 0);
             const bool in[2] = {cb + 16 * c < p.cols, cb + 16 * c + 8 < p.cols};
-            store_rows<T>(to, live, in, old, acc, f, a < 0);
+            T *const here[2] = {to[0] + cb, to[1] + cb};
+            store_rows<T>(here, live, in, old, acc, f, a < 0);
         }
         copies_wait<0>();
         __syncthreads();
@@ -622,7 +623,26 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     // this thread's piece of a row of x (columns behind the last: zeros), and bytes of a row
     const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0;
     const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0));
-    const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2;
+    const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2, x_to = warp * 512 + (lane ^ (warp >> 1 & 3) << 1) * 16;
+    // and its pieces of the rank values and of their rests
+    constexpr int PIECES = S::ROW / 16, HJ = OUTER_STEP * PIECES * 2 / S::THREADS;
+    const uint8_t *h_from[HJ];
+    uint32_t h_to[HJ];
+    int h_token[HJ], h_bytes[HJ];
+#pragma unroll
+    for (int j = 0; j < HJ; ++j) {
+        const int i = threadIdx.x + S::THREADS * j, part = i / (OUTER_STEP * PIECES), token = i / PIECES % OUTER_STEP, piece = i % PIECES;
+        h_token[j] = token;
+        h_bytes[j] = rank0 + piece * 8 < p.rank ? 16 : 0;
+        h_from[j] = (const uint8_t *)((part ? h.rest : h.top) + (h_bytes[j] ? rank0 + piece * 8 : 0));
+        h_to[j] = OUTER_STEP * (512 + part * S::ROW) + token * S::ROW + (piece ^ S::swizzle(token)) * 16;
+    }
+    // a lane's places in the stage: token 2 c, piece r of its warp's columns; and rows of rank values for ldmatrix
+    const uint32_t x_place = c * 1024 + wc * 128 + (r ^ c << 1) * 16;
+    uint32_t h_place[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+        h_place[rb] = OUTER_STEP * 512 + (lane % 8 + lane / 16 * 8) * S::ROW + (((wr * RB + rb) * 2 + lane / 8 % 2) ^ S::swizzle(lane % 8)) * 16;
     float acc[RB][8][4] = {};
     float big = 0.0f;                                            // fp16: the sums are of h / big, the largest power of two of a row so far
     for (int from = lo; from < hi; from += OUTER_LIST) {
@@ -642,20 +662,13 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         auto copy_stage = [&](int first, int stage) {
             if (first < n) {
                 const uint32_t to = ring + stage * S::STAGE;
-                // 32 rows of 32 pieces of x: a warp a row
+                // 32 rows of 32 pieces of x: a warp a row.  (Behind the last token a row is the first one's; its rank values are zeros.)
 #pragma unroll
-                for (int j = 0; j < OUTER_STEP / S::WARPS; ++j) {
-                    const int row = warp + S::WARPS * j;
-                    copy16(to + row * 512 + (lane ^ (row >> 1 & 3) << 1) * 16, xs0 + (uint64_t)(uint32_t)list[first + row] * x_row, first + row < n ? x_bytes : 0);
-                }
-                constexpr int PIECES = S::ROW / 16;              // of a token's rank values
+                for (int j = 0; j < OUTER_STEP / S::WARPS; ++j)
+                    copy16(to + (x_to ^ (S::WARPS * j / 2 & 3) * 32) + S::WARPS * j * 512, xs0 + (uint64_t)(uint32_t)list[first + warp + S::WARPS * j] * x_row, x_bytes);
 #pragma unroll
-                for (int j = 0; j < OUTER_STEP * PIECES * 2 / S::THREADS; ++j) {
-                    const int i = threadIdx.x + S::THREADS * j, part = i / (OUTER_STEP * PIECES), row = i / PIECES % OUTER_STEP, piece = i % PIECES;
-                    const bool ok = first + row < n && rank0 + piece * 8 < p.rank;
-                    copy16(to + OUTER_STEP * (512 + part * S::ROW) + row * S::ROW + (piece ^ S::swizzle(row)) * 16,
-                           (const uint8_t *)((part ? h.rest : h.top) + (ok ? rank0 + piece * 8 : 0)) + (uint64_t)(uint32_t)list[first + row] * h_row, ok ? 16 : 0);
-                }
+                for (int j = 0; j < HJ; ++j)
+                    copy16(to + h_to[j], h_from[j] + (uint64_t)(uint32_t)list[first + h_token[j]] * h_row, first + h_token[j] < n ? h_bytes[j] : 0);
             }
             copies_commit();
         };
@@ -691,7 +704,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
             copies_wait<S::STAGES - 2>();
             __syncthreads();
             copy_stage(first + (S::STAGES - 1) * OUTER_STEP, stage == 0 ? S::STAGES - 1 : stage - 1);
-            const uint32_t xs = ring + stage * S::STAGE, hs = xs + OUTER_STEP * 512;
+            const uint32_t place = ring + stage * S::STAGE;
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
             if (col0 + wc * 64 >= p.cols) continue;
 #pragma unroll
@@ -699,10 +712,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                 if (first + step * 16 >= n) break;
                 uint4 raw[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = step * 16 + 2 * c + k % 2 + k / 2 * 8;
-                    raw[k] = load_shared16(xs + row * 512 + wc * 128 + (r ^ (row >> 1 & 3) << 1) * 16);
-                }
+                for (int k = 0; k < 4; ++k) raw[k] = load_shared16(place + x_place + step * 8192 + k % 2 * 512 + k / 2 * 4096);
                 uint32_t b[8][2];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -721,9 +731,8 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {
-                        const int token = step * 16 + lane % 8 + lane / 16 * 8, piece = (wr * RB + rb) * 2 + lane / 8 % 2;
                         uint32_t ha[4];
-                        load_matrices_transposed(hs + part * OUTER_STEP * S::ROW + token * S::ROW + (piece ^ S::swizzle(token)) * 16, ha);
+                        load_matrices_transposed(place + h_place[rb] + (part * OUTER_STEP + step * 16) * S::ROW, ha);
                         if constexpr (F16) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
