@@ -703,13 +703,14 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         for (int first = 0; first < n; first += OUTER_STEP) {
             copies_wait<S::STAGES - 2>();
             __syncthreads();
-            copy_stage(first + (S::STAGES - 1) * OUTER_STEP, stage == 0 ? S::STAGES - 1 : stage - 1);
+            // (copies take about 1000 cycles of a stage to issue: of the two warps that share a quarter of the SM one makes its own before, one after its MMAs)
+            const int refill = stage == 0 ? S::STAGES - 1 : stage - 1;
+            if (wr == 0) copy_stage(first + (S::STAGES - 1) * OUTER_STEP, refill);
             const uint32_t place = ring + stage * S::STAGE;
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-            if (col0 + wc * 64 >= p.cols) continue;
 #pragma unroll
             for (int step = 0; step < OUTER_STEP / 16; ++step) {
-                if (first + step * 16 >= n) break;
+                if (first + step * 16 >= n || col0 + wc * 64 >= p.cols) break;
                 uint4 raw[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) raw[k] = load_shared16(place + x_place + step * 8192 + k % 2 * 512 + k / 2 * 4096);
@@ -744,6 +745,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                         for (int j = 0; j < 8; ++j) Pair<T>::mma(acc[rb][j], ha, b[j][0], b[j][1]);
                     }
             }
+            if (wr != 0) copy_stage(first + (S::STAGES - 1) * OUTER_STEP, refill);
         }
         copies_wait<0>();
     }
