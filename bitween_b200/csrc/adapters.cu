@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
 
 // ---- outer ---------------------------------------------------------------------------------------------------------------
 
-constexpr int OUTER_LIST = 2048, OUTER_STEP = 32;
+constexpr int OUTER_LIST = 2048, OUTER_STEP = 32, OUTER_WINDOW = 1024;      // tokens of a list, of a stage; words of 32 tokens looked at together
 
 constexpr int SUM_ROW = 260;             // (a row of sums, padded: eight rows meet in four banks otherwise)
 // RB blocks of 16 ranks a warp, RG groups of four warps with ranks of their own.
@@ -588,7 +588,8 @@ template <int RB, int RG> struct OuterShape {
 
 // dw[a][rank0 .. + RANKS][256 columns] = f_a * sum over the adapter's tokens of h[t] x[t]^T.  The CTAs of a cluster (blockIdx.z) take equal shares of
 // the tokens and add their sums through each other's shared memory.  Rows of x and of the rank values go through a ring, 32 tokens a stage.
-// (64 ranks in one warp's registers leave eight warps an SM: 143 us for OUTER_CASE; in two warps, sixteen: OUTER_US.)
+// (64 ranks in the registers of one warp would leave eight warps an SM.  8192 tokens, 14336 columns, rank 64: 136 us, 40 % of
+// what mma.sync can do; the copies' issue, the barrier of a stage and the MMAs take turns.)
 template <typename T, int RB, int RG>
 __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
     using S = OuterShape<RB, RG>;
@@ -601,22 +602,54 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     const uint32_t ring = smem_addr(smem);
     const Hidden<T> h(hidden, p.M, p.rank);
     __shared__ int list[OUTER_LIST + OUTER_STEP], s_count[S::WARPS];
+    __shared__ uint32_t s_bits[OUTER_WINDOW];                    // which tokens of the window are the adapter's
     __shared__ float s_back[OUTER_LIST], s_big[S::WARPS];
 
     if (!p.behind) pdl_wait();
     pdl_launch_dependents();
-    // the adapter's tokens before this warp's part of all, and in all
-    const int64_t part = (p.M + S::THREADS - 1) / S::THREADS * 32, q0 = warp * part, q1 = q0 + part < p.M ? q0 + part : p.M;
-    int count = 0;
-#pragma unroll 16
-    for (int64_t t = q0; t < q1; t += 32) count += __popc(__ballot_sync(0xffffffffu, t + lane < q1 && __ldcg(p.index + t + lane) == a));
-    if (lane == 0) s_count[warp] = count;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < S::WARPS; ++i) {
-        before += i < warp ? s_count[i] : 0;
-        all += s_count[i];
+    // Marks the adapter's tokens in the window of 32768 tokens from word w0 on.  Returns how many there are; `before`: those in front of this thread's words.
+    constexpr int OWN = OUTER_WINDOW / S::THREADS;               // words of a thread
+    const int words = (int)((p.M + 31) / 32);
+    auto mark = [&](int w0, int &before) {
+        __syncthreads();
+        for (int w = warp; w < OUTER_WINDOW && w0 + w < words; w += 8 * S::WARPS) {
+            int id[8];                                           // (all asked for before the first is looked at)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int64_t t = (int64_t)(w0 + w + k * S::WARPS) * 32 + lane;
+                id[k] = t < p.M ? __ldcg(p.index + t) : -1;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t bits = __ballot_sync(0xffffffffu, id[k] == a);
+                if (lane == 0 && w + k * S::WARPS < OUTER_WINDOW) s_bits[w + k * S::WARPS] = bits;
+            }
+        }
+        __syncthreads();
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) mine += w0 + (int)threadIdx.x * OWN + k < words ? __popc(s_bits[threadIdx.x * OWN + k]) : 0;
+        int sum = mine;
+        for (int d = 1; d < 32; d *= 2) {
+            const int o = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += o;
+        }
+        if (lane == 31) s_count[warp] = sum;
+        __syncthreads();
+        before = sum - mine;
+        int all = 0;
+        for (int k = 0; k < S::WARPS; ++k) {
+            before += k < warp ? s_count[k] : 0;
+            all += s_count[k];
+        }
+        return all;
+    };
+    int before = 0, in_window = mark(0, before), all = in_window;
+    for (int w0 = OUTER_WINDOW; w0 < words; w0 += OUTER_WINDOW) {
+        int unused;
+        all += mark(w0, unused);
     }
+    if (words > OUTER_WINDOW) in_window = mark(0, before);
     if (p.behind) pdl_wait();                                    // (the rank values are made by one of the launches before)
     const int share = (all + gridDim.z - 1) / gridDim.z, lo = blockIdx.z * share, hi = lo + share < all ? lo + share : all;
 
@@ -645,16 +678,23 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         h_place[rb] = OUTER_STEP * 512 + (lane % 8 + lane / 16 * 8) * S::ROW + (((wr * RB + rb) * 2 + lane / 8 % 2) ^ S::swizzle(lane % 8)) * 16;
     float acc[RB][8][4] = {};
     float big = 0.0f;                                            // fp16: the sums are of h / big, the largest power of two of a row so far
-    for (int from = lo; from < hi; from += OUTER_LIST) {
-        const int n = hi - from < OUTER_LIST ? hi - from : OUTER_LIST;
+    int window = 0, passed = 0;                                  // the marked window's first word, and the adapter's tokens in front of it
+    for (int from = lo, n; from < hi; from += n) {
+        while (passed + in_window <= from && window + OUTER_WINDOW < words) {
+            passed += in_window;
+            window += OUTER_WINDOW;
+            in_window = mark(window, before);
+        }
+        if (passed + in_window <= from) break;                   // (an index that changes under the call)
+        n = passed + in_window < hi ? passed + in_window - from : hi - from;      // (of one window)
+        n = n < OUTER_LIST ? n : OUTER_LIST;
         __syncthreads();
-        int at = before;
-        for (int64_t t = q0; t < q1 && at < from + n; t += 32) {
-            const bool mine = t + lane < q1 && __ldcg(p.index + t + lane) == a;
-            const unsigned m = __ballot_sync(0xffffffffu, mine);
-            const int place = at + __popc(m & ((1u << lane) - 1)) - from;
-            if (mine && place >= 0 && place < n) list[place] = (int)(t + lane);
-            at += __popc(m);
+        int place = passed + before - from;
+#pragma unroll 1
+        for (int k = 0; k < OWN && place < n; ++k) {
+            const int w = threadIdx.x * OWN + k;
+            for (uint32_t bits = window + w < words ? s_bits[w] : 0u; bits; bits &= bits - 1, ++place)
+                if (place >= 0 && place < n) list[place] = (window + w) * 32 + __ffs(bits) - 1;
         }
         __syncthreads();
         if (threadIdx.x < OUTER_STEP) list[n + threadIdx.x] = list[0];      // (the last stage's places behind the last token)
@@ -766,13 +806,22 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         const int rank = rank0 + i / 32;
         const int64_t at = col0 + i % 32 * 8;
         if (rank >= p.rank || at >= p.cols) continue;
-        float4 s0 = make_float4(0, 0, 0, 0), s1 = s0;
-        for (int o = 0; o < parts; ++o) {
-            const float4 *from = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, o) + i / 32 * SUM_ROW + i % 32 * 8);
-            const float4 u = from[0], v = from[1];
-            s0.x += u.x; s0.y += u.y; s0.z += u.z; s0.w += u.w;
-            s1.x += v.x; s1.y += v.y; s1.z += v.z; s1.w += v.w;
+        float4 u[8][2];                                          // (all asked for before the first is added)
+#pragma unroll
+        for (int o = 0; o < 8; ++o) {
+            const float4 *from = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, o < parts ? o : 0) + i / 32 * SUM_ROW + i % 32 * 8);
+            if (o < parts) {
+                u[o][0] = from[0];
+                u[o][1] = from[1];
+            }
         }
+        float4 s0 = u[0][0], s1 = u[0][1];
+#pragma unroll
+        for (int o = 1; o < 8; ++o)
+            if (o < parts) {
+                s0.x += u[o][0].x; s0.y += u[o][0].y; s0.z += u[o][0].z; s0.w += u[o][0].w;
+                s1.x += u[o][1].x; s1.y += u[o][1].y; s1.z += u[o][1].z; s1.w += u[o][1].w;
+            }
         *reinterpret_cast<uint4 *>(dw + ((int64_t)a * p.rank + rank) * p.cols + at) =
             make_uint4(Pair<T>::pack(s0.x, s0.y), Pair<T>::pack(s0.z, s0.w), Pair<T>::pack(s1.x, s1.y), Pair<T>::pack(s1.z, s1.w));
     }
@@ -918,7 +967,7 @@ int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st
     using S = OuterShape<RB, RG>;
     const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + S::RANKS - 1) / S::RANKS), most = (p.M + 2 * OUTER_STEP - 1) / (2 * OUTER_STEP);
     int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_kernel<T, RB, RG>>(S::THREADS, S::SMEM, per_sm);
-    if (rc == BW_OK) rc = cluster_parts<adapter_outer_kernel<T, RB, RG>>(blocks * rows, most, 0.02, S::THREADS, S::SMEM, parts);
+    if (rc == BW_OK) rc = cluster_parts<adapter_outer_kernel<T, RB, RG>>(blocks * rows, most, 0.12, S::THREADS, S::SMEM, parts);
     if (rc != BW_OK) return rc;
     return launch_early("adapter_outer_kernel", adapter_outer_kernel<T, RB, RG>, dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, st, dim3(1, 1, parts), h, x, p, dw);
 }

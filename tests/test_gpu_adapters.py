@@ -209,6 +209,21 @@ def test_shapes_strides_and_empty_batches():
     assert dx.shape == (0, 256) and bool((ddown == 0).all()) and bool((dup == 0).all())
 
 
+@pytest.mark.parametrize("M,n", [(70000, 2), (33000, 5), (40000, 1)])
+def test_gradients_of_more_tokens_than_one_window(M, n):
+    """Tokens are gathered from windows of 32768; an adapter may have none in the first, or all."""
+    x, down, up, index, scaling, _ = _bank(M, 64, 72, n, 8, torch.float16, seed=12)
+    if n == 2:
+        index[:40000] = 0                   # the other one begins in the second window
+    leaves = [t.requires_grad_() for t in (x, down, up)]
+    grad = torch.randn(M, 72, generator=_gen(13), device=DEV).half()
+    y = adapter_matmul(*leaves, index, scaling=scaling)
+    want = _formula(x.detach(), down.detach(), up.detach(), index, scaling, None, grad)
+    _check(y.detach(), *want["y"])
+    for name, g in zip(("dx", "ddown", "dup"), torch.autograd.grad(y, leaves, grad)):
+        _check(g, *want[name])
+
+
 def test_graphs_of_forward_and_backward():
     """Captured training steps replayed beside each other and beside eager calls."""
     sets = []
