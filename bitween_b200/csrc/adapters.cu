@@ -603,14 +603,15 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     const Hidden<T> h(hidden, p.M, p.rank);
     __shared__ int list[OUTER_LIST + OUTER_STEP], s_count[S::WARPS];
     __shared__ uint32_t s_bits[OUTER_WINDOW];                    // which tokens of the window are the adapter's
+    __shared__ int s_before[OUTER_WINDOW];                       // and how many of them come before each word's
     __shared__ float s_back[OUTER_LIST], s_big[S::WARPS];
 
     if (!p.behind) pdl_wait();
     pdl_launch_dependents();
-    // Marks the adapter's tokens in the window of 32768 tokens from word w0 on.  Returns how many there are; `before`: those in front of this thread's words.
+    // Marks the adapter's tokens in the window of 32768 tokens from word w0 on; returns how many there are.
     constexpr int OWN = OUTER_WINDOW / S::THREADS;               // words of a thread
     const int words = (int)((p.M + 31) / 32);
-    auto mark = [&](int w0, int &before) {
+    auto mark = [&](int w0) {
         __syncthreads();
         for (int w = warp; w < OUTER_WINDOW && w0 + w < words; w += 8 * S::WARPS) {
             int id[8];                                           // (all asked for before the first is looked at)
@@ -636,20 +637,22 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         }
         if (lane == 31) s_count[warp] = sum;
         __syncthreads();
-        before = sum - mine;
-        int all = 0;
+        int before = sum - mine, all = 0;
         for (int k = 0; k < S::WARPS; ++k) {
             before += k < warp ? s_count[k] : 0;
             all += s_count[k];
         }
+#pragma unroll
+        for (int k = 0; k < OWN; ++k) {
+            const int w = threadIdx.x * OWN + k;
+            s_before[w] = before;
+            before += w0 + w < words ? __popc(s_bits[w]) : 0;
+        }
         return all;
     };
-    int before = 0, in_window = mark(0, before), all = in_window;
-    for (int w0 = OUTER_WINDOW; w0 < words; w0 += OUTER_WINDOW) {
-        int unused;
-        all += mark(w0, unused);
-    }
-    if (words > OUTER_WINDOW) in_window = mark(0, before);
+    int in_window = mark(0), all = in_window;
+    for (int w0 = OUTER_WINDOW; w0 < words; w0 += OUTER_WINDOW) all += mark(w0);
+    if (words > OUTER_WINDOW) in_window = mark(0);
     if (p.behind) pdl_wait();                                    // (the rank values are made by one of the launches before)
     const int share = (all + gridDim.z - 1) / gridDim.z, lo = blockIdx.z * share, hi = lo + share < all ? lo + share : all;
 
@@ -683,18 +686,17 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         while (passed + in_window <= from && window + OUTER_WINDOW < words) {
             passed += in_window;
             window += OUTER_WINDOW;
-            in_window = mark(window, before);
+            in_window = mark(window);
         }
         if (passed + in_window <= from) break;                   // (an index that changes under the call)
         n = passed + in_window < hi ? passed + in_window - from : hi - from;      // (of one window)
         n = n < OUTER_LIST ? n : OUTER_LIST;
         __syncthreads();
-        int place = passed + before - from;
-#pragma unroll 1
-        for (int k = 0; k < OWN && place < n; ++k) {
-            const int w = threadIdx.x * OWN + k;
-            for (uint32_t bits = window + w < words ? s_bits[w] : 0u; bits; bits &= bits - 1, ++place)
-                if (place >= 0 && place < n) list[place] = (window + w) * 32 + __ffs(bits) - 1;
+#pragma unroll 4
+        for (int w = warp; w < OUTER_WINDOW && window + w < words; w += S::WARPS) {      // a lane a token
+            const uint32_t bits = s_bits[w];
+            const int place = passed + s_before[w] + __popc(bits & ((1u << lane) - 1)) - from;
+            if ((bits >> lane & 1) && place >= 0 && place < n) list[place] = (window + w) * 32 + lane;
         }
         __syncthreads();
         if (threadIdx.x < OUTER_STEP) list[n + threadIdx.x] = list[0];      // (the last stage's places behind the last token)
