@@ -123,12 +123,14 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
             raise ValueError(f"`out` must be contiguous {(*lead, N)}")
         if out.data_ptr() % 16 != 0:
             return out.copy_(_forward(*args, None, False)[0].view(*lead, N))
-        for i in (0, 1, 2, 5):      # kernels store outputs while others still read
+        for i in range(6):          # kernels store outputs while others still read
             t = args[i]
             if t is not None and t.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < t.data_ptr() + t.nbytes and \
                     not (i == 5 and t.data_ptr() == out.data_ptr()):
                 args = (*args[:i], t.clone(), *args[i + 1:])
         _forward(*args, out.view(M, N), False)
+        if not out.is_inference():
+            torch.autograd.graph.increment_version(out)      # (written in place, as autograd has to know)
         return out
     y = AdapterFunction.apply(*args) if grad else _forward(*args, None, False)[0]
     return y.view(*lead, N)
@@ -138,7 +140,7 @@ class AdaptedLinear(nn.Module):
     """A QuantizedLinear and a bank of low-rank adapters beside it: forward(x, index) is layer(x) plus each row's adapter.
 
     The packed layer stays as it is (frozen, shared); `down` [adapters, rank, in_features] and `up` [adapters, rank, out_features] are
-    parameters of `dtype` (fp16 or bf16), in which x is taken and the result is returned.  `scaling` is a buffer, fp32 [adapters].  New adapters
+    parameters of `dtype` (fp16 or bf16), in which x is taken and the result is returned.  `scaling` is a buffer, [adapters].  New adapters
     have `up` zero, so that they change nothing."""
 
     def __init__(self, layer, num_adapters, rank, scaling=1.0, dtype=torch.float16):
@@ -160,7 +162,7 @@ class AdaptedLinear(nn.Module):
         x = x.to(dtype)
         base = QuantizedLinearFunction.apply(x, layer.qweight, layer.scale, layer.zero_point, layer.bias, layer.bits, layer.group_size, dtype)
         in_place = not (torch.is_grad_enabled() and (base.requires_grad or self.down.requires_grad or self.up.requires_grad))
-        return adapter_matmul(x, self.down, self.up, index, scaling=self.scaling, base=base, out=base if in_place else None)
+        return adapter_matmul(x, self.down, self.up, index, scaling=self.scaling.float(), base=base, out=base if in_place else None)
 
     def extra_repr(self):
         return f"num_adapters={self.down.shape[0]}, rank={self.down.shape[1]}"

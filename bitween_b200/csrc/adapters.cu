@@ -588,7 +588,7 @@ template <int RB, int RG> struct OuterShape {
 
 // dw[a][rank0 .. + RANKS][256 columns] = f_a * sum over the adapter's tokens of h[t] x[t]^T.  The CTAs of a cluster (blockIdx.z) take equal shares of
 // the tokens and add their sums through each other's shared memory.  Rows of x and of the rank values go through a ring, 32 tokens a stage.
-// (64 ranks in the registers of one warp would leave eight warps an SM.  8192 tokens, 14336 columns, rank 64: 136 us, 40 % of
+// (64 ranks in the registers of one warp would leave eight warps an SM.  8192 tokens, 14336 columns, rank 64: 129 us, 43 % of
 // what mma.sync can do; the copies' issue, the barrier of a stage and the MMAs take turns.)
 template <typename T, int RB, int RG>
 __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {

@@ -637,7 +637,7 @@ int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_s
 // ---- low-rank adapters ----
 static int adapter_validate(int dtype, int64_t M, int64_t N, int64_t K, int n, int r, const void *index, const void *scaling) {
     if (dtype != BW_F16 && dtype != BW_BF16) return BW_ERR_DTYPE;
-    if (M < 0 || N < 1 || K < 1 || n < 1 || r < 1 || r > 256 || N > (int64_t)1 << 24 || K > (int64_t)1 << 24) return BW_ERR_SHAPE;
+    if (M < 0 || N < 1 || K < 1 || n < 1 || r < 1 || r > 256 || N > (int64_t)65535 * 256 || K > (int64_t)65535 * 256) return BW_ERR_SHAPE;
     if (M > ((int64_t)1 << 31) / r || n > (1 << 30) / r) return BW_ERR_SHAPE;
     if (M > 0 && !index) return BW_ERR_NULL;
     return aligned_to(index, 4) && aligned_to(scaling, 4) ? BW_OK : BW_ERR_ALIGN;

@@ -259,7 +259,7 @@ PyObject *kv_attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Cache c;
     if (nargs != 8 || !g_ops.kv_attend || !PyFloat_CheckExact(args[7]) || !c.of(args)) Py_RETURN_NONE;
     const at::Tensor *q = tensor_of(args[4]), *table = tensor_of(args[5]), *lengths = tensor_of(args[6]);
-    if (!usable(q, c.device) || !usable(table, c.device) || !dense(lengths, c.device)) Py_RETURN_NONE;
+    if (!usable(q, c.device) || !usable(table, c.device) || !dense(lengths, c.device) || (c10::GradMode::is_enabled() && q->requires_grad())) Py_RETURN_NONE;
     const int code = float_code(q->scalar_type());
     if ((code != BW_F16 && code != BW_BF16) || table->scalar_type() != at::kInt || lengths->scalar_type() != at::kInt) Py_RETURN_NONE;
     if (q->dim() != 3 || q->size(2) != c.dim || q->stride(2) != 1 || q->size(1) < 1 || c.heads < 1 || q->size(1) % c.heads || q->size(1) > INT32_MAX) Py_RETURN_NONE;
@@ -311,11 +311,24 @@ struct AdapterNode : torch::autograd::Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         for (auto *v : {&x, &down, &up, &index, &scaling, &hidden}) v->reset_data();
     }
+    // The engine hands each gradient to the stream on which its consumer was recorded.  The default stream cannot take one from a capture, and torch
+    // does not survive the attempt.
+    void check_capture() const {
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+        for (uint32_t i = 0; i < num_outputs(); ++i) {
+            if (!task_should_compute_output(i)) continue;
+            const auto stream = next_edge(i).function->stream();
+            TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
+                        "adapter_matmul: this backward pass cannot be captured while a graph of the same tensors, recorded on the default stream, is alive; free it, or "
+                        "record it on another stream");
+        }
+    }
     torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
         torch::autograd::variable_list result(4);
         const at::Tensor g = grads[0];
         if (!g.defined()) return result;
+        check_capture();
         const bool again = c10::GradMode::is_enabled();
         if (task_should_compute_output(0) || task_should_compute_output(1) || task_should_compute_output(2)) {
             const at::Tensor xt = x.unpack(), dt = down.unpack(), ut = up.unpack(), it = index.unpack(), st = scaling.unpack(), ht = hidden.unpack();
@@ -399,7 +412,7 @@ PyObject *adapter_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     } else {
         if (given) {
             const uintptr_t o = reinterpret_cast<uintptr_t>(given->const_data_ptr());
-            for (const at::Tensor *y : {x, down, up, base}) {
+            for (const at::Tensor *y : {x, down, up, index, scaling, base}) {
                 const uintptr_t a = y ? reinterpret_cast<uintptr_t>(y->const_data_ptr()) : 0;
                 if (y && a < o + given->nbytes() && o < a + y->nbytes() && !(y == base && a == o)) Py_RETURN_NONE;
             }
@@ -413,6 +426,7 @@ PyObject *adapter_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
             rc = adapter_call(*x, *down, *up, *index, scaling ? *scaling : none, base ? *base : none, out, hidden);
         }
         if (rc != BW_OK) Py_RETURN_NONE;
+        if (given && !given->is_inference()) given->unsafeGetTensorImpl()->bump_version();      // (written in place, as autograd has to know)
     }
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS

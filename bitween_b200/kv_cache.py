@@ -78,7 +78,7 @@ class QuantizedKVCache:
     def append(self, k, v, slots):
         """Quantises k[t], v[t] ([tokens, num_kv_heads, head_dim], fp16, bf16 or fp32; any strides of tokens and heads) into slot
         slots[t].  Slots outside the cache are skipped (padding: -1); each slot may be named once in a call.  A row with a NaN or an
-        infinity, or whose scale leaves fp16's range, reads back as NaN."""
+        infinity, or whose scale leaves fp16's range, reads back as NaN.  Codes have no gradient: nothing is recorded."""
         if (_lib._operators or _lib.host_operators()).kv_append(*self._cache, k, v, slots):
             return
         _lib.require_cuda(self.k_codes, "cache")
@@ -129,7 +129,8 @@ class QuantizedKVCache:
 
         `softmax_scale` defaults to head_dim ** -0.5.  The new token's own row is attended to if it has been appended and counted.  Sequences
         of length 0 (or less) give zeros.  A length that is more than the table holds, and a page outside the cache within the
-        length, give NaN for that sequence; nothing is read there."""
+        length, give NaN for that sequence; nothing is read there.  There is no gradient: a q that requires one is refused where
+        gradients are recorded."""
         if softmax_scale is None:
             softmax_scale = self._softmax_scale
         out = (_lib._operators or _lib.host_operators()).kv_attend(*self._cache, q, page_table, lengths, softmax_scale)
@@ -138,6 +139,8 @@ class QuantizedKVCache:
         _lib.require_cuda(q, "q")
         if q.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"attend: unsupported dtype {q.dtype} (float16/bfloat16)")
+        if q.requires_grad and torch.is_grad_enabled():
+            raise ValueError("attend has no gradient; detach q or call it under torch.no_grad()")
         if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] < 1 or q.shape[1] % self.num_kv_heads != 0:
             raise ValueError(f"q must be [batch, heads, {self.head_dim}] with a multiple of {self.num_kv_heads} heads")
         if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
@@ -161,7 +164,7 @@ class QuantizedKVCache:
                                                                             page_table.shape[1]))
             rc = L.bw_kv_attend(q.data_ptr(), _lib.dtype_code(q.dtype), batch, heads, q.stride(0), q.stride(1), *self._tensors(), self.bits, self.num_pages,
                                 self.page_size, self.num_kv_heads, self.head_dim, page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                                lengths.data_ptr(), softmax_scale, out.data_ptr(), None if ws is None else ws.data_ptr(),
+                                lengths.data_ptr(), float(softmax_scale), out.data_ptr(), None if ws is None else ws.data_ptr(),
                                 0 if ws is None else ws.numel(), _lib.raw_stream(self.device))
         _lib.check(rc)
         return out

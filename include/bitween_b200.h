@@ -386,7 +386,7 @@ BW_API int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int6
  *   index    [M] int32       scaling [adapters] fp32 or NULL (ones)
  *   hidden   scratch of bw_adapter_hidden_bytes(...) (16-byte aligned), under the rules of bw_qmatmul's workspace; it holds h, which the
  *            backward call needs again for grad_up
- * Sums are fp32; out is rounded once.  Ranks up to 256 (tensor cores: ranks of 8 to 128 and K, N in steps of 8; other sizes run on
+ * Sums are fp32; out is rounded once.  Ranks up to 256, K and N up to 65535 * 256 (tensor cores: ranks of 8 to 128 and K, N in steps of 8; other sizes run on
  * slower general kernels).
  */
 BW_API size_t bw_adapter_hidden_bytes(int64_t M, int rank);
