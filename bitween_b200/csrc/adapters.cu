@@ -23,6 +23,7 @@
 #include <atomic>
 
 #include "early_launch.cuh"
+#include "umma.cuh"
 
 namespace bw {
 namespace {
@@ -108,6 +109,8 @@ __device__ __forceinline__ void copy16(uint32_t to, const void *from, int bytes)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Arrives once this thread's copies so far have been made (counted among the barrier's arrivals).
+__device__ __forceinline__ void copies_arrive(uint64_t *bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint4 load_shared16(uint32_t at) {
     uint4 v;
@@ -576,7 +579,91 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
 
 constexpr int OUTER_LIST = 2048, OUTER_STEP = 32, OUTER_WINDOW = 1024;      // tokens of a list, of a stage; words of 32 tokens looked at together
 
+// Which tokens of the window of 32 * WINDOW tokens from word w0 on are adapter a's (s_bits), and how many of them come before each word's (s_before);
+// returns how many there are.  Made by WARPS warps, which meet at `barrier`.
+template <int WARPS, int WINDOW, typename Barrier>
+__device__ __forceinline__ int mark_tokens(const AdapterArgs &p, int a, int w0, uint32_t *s_bits, int *s_before, int *s_count, Barrier barrier) {
+    constexpr int OWN = WINDOW / (32 * WARPS);                   // words of a thread
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, words = (int)((p.M + 31) / 32);
+    barrier();
+    for (int w = warp; w < WINDOW && w0 + w < words; w += 8 * WARPS) {
+        int id[8];                                               // (all asked for before the first is looked at)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int64_t t = (int64_t)(w0 + w + k * WARPS) * 32 + lane;
+            id[k] = t < p.M ? __ldcg(p.index + t) : -1;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const uint32_t bits = __ballot_sync(0xffffffffu, id[k] == a);
+            if (lane == 0 && w + k * WARPS < WINDOW) s_bits[w + k * WARPS] = bits;
+        }
+    }
+    barrier();
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) mine += w0 + (int)threadIdx.x * OWN + k < words ? __popc(s_bits[threadIdx.x * OWN + k]) : 0;
+    int sum = mine;
+    for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += o;
+    }
+    if (lane == 31) s_count[warp] = sum;
+    barrier();
+    int before = sum - mine, all = 0;
+    for (int k = 0; k < WARPS; ++k) {
+        before += k < warp ? s_count[k] : 0;
+        all += s_count[k];
+    }
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) {
+        const int w = threadIdx.x * OWN + k;
+        s_before[w] = before;
+        before += w0 + w < words ? __popc(s_bits[w]) : 0;
+    }
+    return all;
+}
+// Tokens `skip` to skip + n of the marked ones.  A lane a token.
+template <int WARPS, int WINDOW>
+__device__ __forceinline__ void list_tokens(const AdapterArgs &p, int w0, int skip, int n, const uint32_t *s_bits, const int *s_before, int *list) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, words = (int)((p.M + 31) / 32);
+#pragma unroll 4
+    for (int w = warp; w < WINDOW && w0 + w < words; w += WARPS) {
+        const uint32_t bits = s_bits[w];
+        const int place = s_before[w] + __popc(bits & ((1u << lane) - 1)) - skip;
+        if ((bits >> lane & 1) && place >= 0 && place < n) list[place] = (w0 + w) * 32 + lane;
+    }
+}
+// The end of outer: the CTAs of a cluster (along z) have sums [ranks][SUM_ROW] of 256 columns; each adds up its share of them and writes it.
 constexpr int SUM_ROW = 260;             // (a row of sums, padded: eight rows meet in four banks otherwise)
+template <typename T, int THREADS, int RANKS>
+__device__ __forceinline__ void join_sums(float *sums, const AdapterArgs &p, int a, int rank0, int64_t col0, T *dw) {
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int parts = gridDim.z, mine = blockIdx.z;
+    for (int i = mine * THREADS + threadIdx.x; i < RANKS * 32; i += parts * THREADS) {        // eight columns of a rank
+        const int rank = rank0 + i / 32;
+        const int64_t at = col0 + i % 32 * 8;
+        if (rank >= p.rank || at >= p.cols) continue;
+        float4 u[8][2];                                          // (all asked for before the first is added)
+#pragma unroll
+        for (int o = 0; o < 8; ++o) {
+            const float4 *from = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, o < parts ? o : 0) + i / 32 * SUM_ROW + i % 32 * 8);
+            if (o < parts) {
+                u[o][0] = from[0];
+                u[o][1] = from[1];
+            }
+        }
+        float4 s0 = u[0][0], s1 = u[0][1];
+#pragma unroll
+        for (int o = 1; o < 8; ++o)
+            if (o < parts) {
+                s0.x += u[o][0].x; s0.y += u[o][0].y; s0.z += u[o][0].z; s0.w += u[o][0].w;
+                s1.x += u[o][1].x; s1.y += u[o][1].y; s1.z += u[o][1].z; s1.w += u[o][1].w;
+            }
+        *reinterpret_cast<uint4 *>(dw + ((int64_t)a * p.rank + rank) * p.cols + at) =
+            make_uint4(Pair<T>::pack(s0.x, s0.y), Pair<T>::pack(s0.z, s0.w), Pair<T>::pack(s1.x, s1.y), Pair<T>::pack(s1.z, s1.w));
+    }
+}
 // RB blocks of 16 ranks a warp, RG groups of four warps with ranks of their own.
 template <int RB, int RG> struct OuterShape {
     static constexpr int WARPS = 4 * RG, THREADS = 32 * WARPS;
@@ -588,7 +675,7 @@ template <int RB, int RG> struct OuterShape {
 
 // dw[a][rank0 .. + RANKS][256 columns] = f_a * sum over the adapter's tokens of h[t] x[t]^T.  The CTAs of a cluster (blockIdx.z) take equal shares of
 // the tokens and add their sums through each other's shared memory.  Rows of x and of the rank values go through a ring, 32 tokens a stage.
-// (64 ranks in the registers of one warp would leave eight warps an SM.  8192 tokens, 14336 columns, rank 64: 129 us, 43 % of
+// (For few tokens and ranks up to 16; 64 ranks in the registers of one warp would leave eight warps an SM.  8192 tokens, 14336 columns, rank 64: 129 us, 43 % of
 // what mma.sync can do; the copies' issue, the barrier of a stage and the MMAs take turns.)
 template <typename T, int RB, int RG>
 __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
@@ -608,48 +695,8 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 
     if (!p.behind) pdl_wait();
     pdl_launch_dependents();
-    // Marks the adapter's tokens in the window of 32768 tokens from word w0 on; returns how many there are.
-    constexpr int OWN = OUTER_WINDOW / S::THREADS;               // words of a thread
     const int words = (int)((p.M + 31) / 32);
-    auto mark = [&](int w0) {
-        __syncthreads();
-        for (int w = warp; w < OUTER_WINDOW && w0 + w < words; w += 8 * S::WARPS) {
-            int id[8];                                           // (all asked for before the first is looked at)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const int64_t t = (int64_t)(w0 + w + k * S::WARPS) * 32 + lane;
-                id[k] = t < p.M ? __ldcg(p.index + t) : -1;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t bits = __ballot_sync(0xffffffffu, id[k] == a);
-                if (lane == 0 && w + k * S::WARPS < OUTER_WINDOW) s_bits[w + k * S::WARPS] = bits;
-            }
-        }
-        __syncthreads();
-        int mine = 0;
-#pragma unroll
-        for (int k = 0; k < OWN; ++k) mine += w0 + (int)threadIdx.x * OWN + k < words ? __popc(s_bits[threadIdx.x * OWN + k]) : 0;
-        int sum = mine;
-        for (int d = 1; d < 32; d *= 2) {
-            const int o = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += o;
-        }
-        if (lane == 31) s_count[warp] = sum;
-        __syncthreads();
-        int before = sum - mine, all = 0;
-        for (int k = 0; k < S::WARPS; ++k) {
-            before += k < warp ? s_count[k] : 0;
-            all += s_count[k];
-        }
-#pragma unroll
-        for (int k = 0; k < OWN; ++k) {
-            const int w = threadIdx.x * OWN + k;
-            s_before[w] = before;
-            before += w0 + w < words ? __popc(s_bits[w]) : 0;
-        }
-        return all;
-    };
+    auto mark = [&](int w0) { return mark_tokens<S::WARPS, OUTER_WINDOW>(p, a, w0, s_bits, s_before, s_count, [] { __syncthreads(); }); };
     int in_window = mark(0), all = in_window;
     for (int w0 = OUTER_WINDOW; w0 < words; w0 += OUTER_WINDOW) all += mark(w0);
     if (words > OUTER_WINDOW) in_window = mark(0);
@@ -692,12 +739,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         n = passed + in_window < hi ? passed + in_window - from : hi - from;      // (of one window)
         n = n < OUTER_LIST ? n : OUTER_LIST;
         __syncthreads();
-#pragma unroll 4
-        for (int w = warp; w < OUTER_WINDOW && window + w < words; w += S::WARPS) {      // a lane a token
-            const uint32_t bits = s_bits[w];
-            const int place = passed + s_before[w] + __popc(bits & ((1u << lane) - 1)) - from;
-            if ((bits >> lane & 1) && place >= 0 && place < n) list[place] = (window + w) * 32 + lane;
-        }
+        list_tokens<S::WARPS, OUTER_WINDOW>(p, window, from - passed, n, s_bits, s_before, list);
         __syncthreads();
         if (threadIdx.x < OUTER_STEP) list[n + threadIdx.x] = list[0];      // (the last stage's places behind the last token)
         __syncthreads();
@@ -803,31 +845,221 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
             for (int k = 0; k < 4; ++k) sums[((wr * RB + rb) * 16 + r + k / 2 * 8) * SUM_ROW + wc * 64 + c * 16 + k % 2 * 8 + j] = acc[rb][j][k] * f;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    const int parts = gridDim.z, mine = blockIdx.z;
-    for (int i = mine * S::THREADS + threadIdx.x; i < S::RANKS * 32; i += parts * S::THREADS) {        // eight columns of a rank
-        const int rank = rank0 + i / 32;
-        const int64_t at = col0 + i % 32 * 8;
-        if (rank >= p.rank || at >= p.cols) continue;
-        float4 u[8][2];                                          // (all asked for before the first is added)
+    join_sums<T, S::THREADS, S::RANKS>(sums, p, a, rank0, col0, dw);
+    cluster.sync();                                              // a CTA's sums stay until the others have read them
+}
+
+// The same on tcgen05, for adapters of many tokens: 64 ranks x 256 columns a CTA, reduced over tokens, 32 a stage.  Rows of x and of the rank values keep
+// the order in which memory holds them, which is the MN-major form of both operands (blocks of 64 elements by 32 tokens, 128-byte swizzle).  Values and
+// rests of 64 ranks are the two halves of the M dimension, so that one MMA multiplies both; their sums meet at the end.  Eight warps fill the ring with
+// 16-byte cp.async of rows that a list names, one warp issues the MMAs; for fp16 two warps between them bring the rows' powers of two into the rank
+// values.  (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between the copies and themselves, waits for all that
+// its own thread has in flight: 86 us instead of 76.)  Bound by the rows of x and the rank values, which every 256 columns read again: 8192 tokens of 2 adapters, 14336
+// columns, rank 64, bf16: 352 MB in 76 us, on the 112 SMs that there are CTAs for.  (mma.sync: 129 us.  Sixteen copying warps: the same, and 2 us more to begin.)
+constexpr int OU_STAGES = 8, OU_A = 2 * OUTER_STEP * 128, OU_B = 4 * OUTER_STEP * 128, OU_STAGE = OU_A + OU_B, OU_THREADS = 352,
+              OU_SMEM = OU_STAGES * OU_STAGE + 1024, OU_LIST = 1024, OU_WINDOW = 512;
+static_assert(64 * SUM_ROW * 4 <= OU_STAGES * OU_STAGE, "the sums take the ring's place");
+__device__ int g_adapter_status = 0;
+
+template <typename T>
+__global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
+    constexpr bool F16 = __is_same(T, __half);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const int rank_blocks = (p.rank + 63) / 64, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * 64;
+    const int64_t col0 = (int64_t)blockIdx.x * 256;
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [OU_STAGES][values, rests | 4 blocks of columns][tokens][128 B]
+    float *sums = reinterpret_cast<float *>(smem);                                      // [64][SUM_ROW], at the end
+    __shared__ int list[OU_LIST + OUTER_STEP], s_before[OU_WINDOW], s_count[8], s_end[OU_STAGES], s_abort;
+    __shared__ uint32_t s_bits[OU_WINDOW], s_tmem;
+    __shared__ float s_back[F16 ? OU_LIST : 1], s_big[8], s_scale[F16 ? OU_STAGES : 1][OUTER_STEP];
+    __shared__ __align__(8) uint64_t full[OU_STAGES], scaled[OU_STAGES], empty[OU_STAGES], done;
+    volatile int *abort_flag = &s_abort;
+    const Hidden<T> h(hidden, p.M, p.rank);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < OU_STAGES; ++i) {
+            umma::mbar_init(&full[i], 256 + 8);                  // (copies of each thread, and each warp)
+            umma::mbar_init(&scaled[i], 2);
+            umma::mbar_init(&empty[i], 1);
+            s_end[i] = 0;
+        }
+        umma::mbar_init(&done, 1);
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        umma::fence_proxy_async_smem();
+    }
+    if (warp == 8) umma::tmem_alloc(&s_tmem, 256);
+    umma::tc_fence_before();
+    __syncthreads();
+    umma::tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    if (!p.behind) pdl_wait();
+    pdl_launch_dependents();       // (not before the tensor memory is there: the launch behind may take as much of it, and waits for this one)
+
+    int stages = 0;                // made in all
+    float f = 0.0f;                // what the sums are multiplied by
+    if (warp == 8) {
+        // ---- products ----
+        if (p.behind) pdl_wait();
+        const uint32_t idesc = umma::umma_idesc_f16(256, !F16, true) | 1u << 16;      // (B MN-major as well)
+        const uint32_t ring = smem_addr(smem);
+        for (;; ++stages) {
+            const int slot = stages % OU_STAGES;
+            if (!__all_sync(0xffffffffu, umma::mbar_wait(F16 ? &scaled[slot] : &full[slot], stages / OU_STAGES & 1, abort_flag, 1, &g_adapter_status))) break;
+            if (*(volatile int *)&s_end[slot]) {
+                umma::umma_commit(&done);
+                break;
+            }
+            umma::fence_proxy_async_smem();
+            umma::tc_fence_after();
+            const uint32_t at = ring + slot * OU_STAGE;
 #pragma unroll
-        for (int o = 0; o < 8; ++o) {
-            const float4 *from = reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums, o < parts ? o : 0) + i / 32 * SUM_ROW + i % 32 * 8);
-            if (o < parts) {
-                u[o][0] = from[0];
-                u[o][1] = from[1];
+            for (int k = 0; k < OUTER_STEP / 16; ++k)
+                umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(at + k * 2048, OUTER_STEP * 128), umma::umma_smem_desc_mn(at + OU_A + k * 2048, OUTER_STEP * 128), idesc,
+                                  (stages | k) != 0 ? 1u : 0u);
+            umma::umma_commit(&empty[slot]);
+        }
+    } else if (warp > 8) {
+        // ---- fp16: rank values times their row's power of two ----
+        if (p.behind) pdl_wait();
+        if constexpr (F16)
+            for (;; ++stages) {
+                const int slot = stages % OU_STAGES;
+                if (!__all_sync(0xffffffffu, umma::mbar_wait(&full[slot], stages / OU_STAGES & 1, abort_flag, 5, &g_adapter_status))) break;
+                const bool end = *(volatile int *)&s_end[slot];
+                if (!end) {
+#pragma unroll
+                    for (int i = 0; i < OU_A / 16 / 64; ++i) {
+                        const int at = (warp - 9) * 32 + lane + i * 64;      // of 16 bytes, eight a row
+                        const __half2 scale = __float2half2_rn(s_scale[slot][at / 8 % OUTER_STEP]);
+                        uint4 *own = reinterpret_cast<uint4 *>(smem + slot * OU_STAGE) + at, v = *own;
+                        __half2 *y = reinterpret_cast<__half2 *>(&v);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) y[k] = __hmul2(y[k], scale);
+                        *own = v;
+                    }
+                    umma::fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) umma::mbar_arrive(&scaled[slot]);
+                if (end) break;
+            }
+    } else {
+        // ---- copies ----
+        const auto meet = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+        const int words = (int)((p.M + 31) / 32);
+        auto mark = [&](int w0) { return mark_tokens<8, OU_WINDOW>(p, a, w0, s_bits, s_before, s_count, meet); };
+        int in_window = mark(0), all = in_window;
+        for (int w0 = OU_WINDOW; w0 < words; w0 += OU_WINDOW) all += mark(w0);
+        if (words > OU_WINDOW) in_window = mark(0);
+        if (p.behind) pdl_wait();                                // (the rank values are made by one of the launches before)
+        const int share = (all + gridDim.z - 1) / gridDim.z, lo = blockIdx.z * share, hi = lo + share < all ? lo + share : all;
+        float big = 1.0f;                                        // fp16: the sums are of h / big, the largest power of two of a row
+        if constexpr (F16) {
+            big = 0.0f;
+#pragma unroll 4
+            for (int w = warp; w < words; w += 8) {
+                const int64_t t = (int64_t)w * 32 + lane;
+                const int id = t < p.M ? __ldcg(p.index + t) : -1;
+                const float back = t < p.M ? __ldcg(h.back + t) : 0.0f;      // (of a row without an adapter: anything)
+                if (id == a) big = fmaxf(big, back);
+            }
+            for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+            if (lane == 0) s_big[warp] = big;
+            meet();
+            for (int i = 0; i < 8; ++i) big = fmaxf(big, s_big[i]);
+        }
+        f = big * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
+
+        // this thread's pieces: of rows warp, warp + 8, .. of x piece `lane`; of row threadIdx / 8 of the values and of the rests piece threadIdx % 8
+        const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0, token = threadIdx.x / 8, piece = threadIdx.x % 8, h_bytes = rank0 + piece * 8 < p.rank ? 16 : 0;
+        const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0)), *top0 = (const uint8_t *)(h.top + (h_bytes ? rank0 + piece * 8 : 0)),
+                      *rest0 = (const uint8_t *)(h.rest + (h_bytes ? rank0 + piece * 8 : 0));
+        const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2, ring = smem_addr(smem);
+        const uint32_t x_to = OU_A + lane / 8 * (OUTER_STEP * 128) + warp * 128 + (lane % 8 ^ warp) * 16, h_to = token * 128 + (piece ^ (token & 7)) * 16;
+        bool alive = true;                                       // (after a failed wait the loops go on without copies: the warps meet in them)
+        int window = 0, passed = 0;
+        for (int from = lo, n; from < hi; from += n) {
+            while (passed + in_window <= from && window + OU_WINDOW < words) {
+                passed += in_window;
+                window += OU_WINDOW;
+                in_window = mark(window);
+            }
+            if (passed + in_window <= from) break;               // (an index that changes under the call)
+            n = passed + in_window < hi ? passed + in_window - from : hi - from;      // (of one window)
+            n = n < OU_LIST ? n : OU_LIST;
+            meet();
+            list_tokens<8, OU_WINDOW>(p, window, from - passed, n, s_bits, s_before, list);
+            meet();
+            if constexpr (F16) {
+                for (int j = threadIdx.x; j < n; j += 256) s_back[j] = __ldcg(h.back + list[j]) / big;
+                meet();
+            }
+            const int count = (n + OUTER_STEP - 1) / OUTER_STEP;
+            for (int i = 0; i < count; ++i, ++stages) {
+                const int slot = stages % OU_STAGES, first = i * OUTER_STEP;
+                alive = alive && umma::mbar_wait(&empty[slot], (stages / OU_STAGES & 1) ^ 1, abort_flag, 2, &g_adapter_status);
+                if (alive) {
+                    const uint32_t to = ring + slot * OU_STAGE;
+#pragma unroll
+                    for (int j = 0; j < OUTER_STEP / 8; ++j) {
+                        const int at = first + warp + 8 * j;
+                        copy16(to + x_to + j * 1024, xs0 + (at < n ? (uint64_t)(uint32_t)list[at] * x_row : 0), at < n ? x_bytes : 0);
+                    }
+                    const int at = first + token;
+                    const uint64_t row = at < n ? (uint64_t)(uint32_t)list[at] * h_row : 0;
+                    copy16(to + h_to, top0 + row, at < n ? h_bytes : 0);
+                    copy16(to + h_to + OUTER_STEP * 128, rest0 + row, at < n ? h_bytes : 0);
+                    if constexpr (F16)
+                        if (piece == 0) s_scale[slot][token] = at < n ? s_back[at] : 0.0f;
+                    copies_arrive(&full[slot]);
+                }
+                __syncwarp();
+                if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
             }
         }
-        float4 s0 = u[0][0], s1 = u[0][1];
+        // one more stage, without tokens: the end
+        const int slot = stages % OU_STAGES;
+        alive = alive && umma::mbar_wait(&empty[slot], (stages / OU_STAGES & 1) ^ 1, abort_flag, 3, &g_adapter_status);
+        if (threadIdx.x == 0) *(volatile int *)&s_end[slot] = 1;
+        if (alive) copies_arrive(&full[slot]);
+        __syncwarp();
+        if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // ---- sums of this CTA: tensor memory's lanes 0 to 63 are the values' ranks, 64 to 127 the rests' ----
+        if (warp < 4) alive = __all_sync(0xffffffffu, umma::mbar_wait(&done, 0, abort_flag, 4, &g_adapter_status));
+        umma::tc_fence_after();
 #pragma unroll
-        for (int o = 1; o < 8; ++o)
-            if (o < parts) {
-                s0.x += u[o][0].x; s0.y += u[o][0].y; s0.z += u[o][0].z; s0.w += u[o][0].w;
-                s1.x += u[o][1].x; s1.y += u[o][1].y; s1.z += u[o][1].z; s1.w += u[o][1].w;
+        for (int part = 1; part >= 0; --part) {
+            if (warp < 4 && warp / 2 == part) {
+                float *row = sums + (warp % 2 * 32 + lane) * SUM_ROW;
+                for (int cb = 0; cb < 256; cb += 32) {
+                    uint32_t r[32] = {};
+                    if (alive && stages) umma::tmem_ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + cb, r);
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        float4 v = make_float4(__uint_as_float(r[k]), __uint_as_float(r[k + 1]), __uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]));
+                        float4 *to = reinterpret_cast<float4 *>(row + cb + k);
+                        if (part == 0) {
+                            const float4 rest = *to;
+                            v = make_float4((v.x + rest.x) * f, (v.y + rest.y) * f, (v.z + rest.z) * f, (v.w + rest.w) * f);
+                        }
+                        *to = v;
+                    }
+                }
             }
-        *reinterpret_cast<uint4 *>(dw + ((int64_t)a * p.rank + rank) * p.cols + at) =
-            make_uint4(Pair<T>::pack(s0.x, s0.y), Pair<T>::pack(s0.z, s0.w), Pair<T>::pack(s1.x, s1.y), Pair<T>::pack(s1.z, s1.w));
+            meet();
+        }
+        umma::tc_fence_before();
     }
+    __syncwarp();
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (*abort_flag == 0) join_sums<T, OU_THREADS, 64>(sums, p, a, rank0, col0, dw);
     cluster.sync();                                              // a CTA's sums stay until the others have read them
+    umma::tc_fence_after();
+    if (warp == 8) umma::tmem_dealloc(tmem, 256);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------
@@ -974,7 +1206,22 @@ int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st
     return launch_early("adapter_outer_kernel", adapter_outer_kernel<T, RB, RG>, dim3((unsigned)blocks, (unsigned)rows, parts), S::THREADS, S::SMEM, st, dim3(1, 1, parts), h, x, p, dw);
 }
 template <typename T>
+int outer_umma(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
+    const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 63) / 64), most = (p.M + 4 * OUTER_STEP - 1) / (4 * OUTER_STEP);
+    int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_umma_kernel<T>>(OU_THREADS, OU_SMEM, per_sm);
+    // (a part's start and end take as long as about 384 of its tokens)
+    if (rc == BW_OK) rc = cluster_parts<adapter_outer_umma_kernel<T>>(blocks * rows, most, 384.0 * p.adapters / p.M, OU_THREADS, OU_SMEM, parts);
+    if (rc != BW_OK) return rc;
+    return launch_early("adapter_outer_umma_kernel", adapter_outer_umma_kernel<T>, dim3((unsigned)blocks, (unsigned)rows, parts), OU_THREADS, OU_SMEM, st, dim3(1, 1, parts), h, x, p, dw);
+}
+template <typename T>
 int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
+    // tcgen05 has 64 ranks' work for any rank and one CTA an SM, mma.sync two or three of less.  bf16, us, mma.sync / tcgen05: rank 64, 14336 columns, 8192 tokens
+    // of one adapter 107 / 68, of 16 151 / 116; 512 tokens of 4096 columns of one 18 / 12, of 16 (256 CTAs) 10 / 15; rank 32, 1024 columns, 2048 tokens 13.3 / 12.9,
+    // 512 tokens 7.7 / 9.6; rank 16, 14336 columns, 8192 tokens 60 / 67.
+    const int64_t rows = (int64_t)p.adapters * ((p.rank + 63) / 64);
+    const bool at_once = (p.cols + 255) / 256 * rows <= SMS;
+    if (p.rank > 32 ? p.M >= 512 * rows || (at_once && p.M >= 512) : p.rank > 16 && at_once && p.M >= 2048) return outer_umma<T>(h, (const T *)x, p, (T *)dw, st);
     if (p.rank <= 16) return outer_fast<T, 1, 1>(h, (const T *)x, p, (T *)dw, st);
     if (p.rank <= 32) return outer_fast<T, 2, 1>(h, (const T *)x, p, (T *)dw, st);
     return outer_fast<T, 2, 2>(h, (const T *)x, p, (T *)dw, st);
@@ -1031,6 +1278,13 @@ int backward(const void *dy, const void *x, int64_t M, int64_t N, int64_t K, con
 
 // (two 16-bit parts and a power of two a row; the general kernels' fp32 values are less)
 size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * 4 + (size_t)M * 4; }
+
+int adapter_device_status() {
+    int v = 0, zero = 0;
+    if (cudaMemcpyFromSymbol(&v, g_adapter_status, sizeof(int)) != cudaSuccess) return -1;
+    if (v) (void)cudaMemcpyToSymbol(g_adapter_status, &zero, sizeof(int));
+    return v;
+}
 
 int adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index,
                     const float *scaling, const void *base, void *out, void *h, cudaStream_t st) {

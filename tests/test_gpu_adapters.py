@@ -334,3 +334,20 @@ def test_an_attention_block_decodes_with_adapters_and_a_quantised_cache():
         assert bool(((a[b].double() - want).abs() <= half * want.abs() + half * size + 1e-6).all())
     assert torch.equal(out[1], wo.layer(a.view(batch, -1))[1]) and not torch.equal(out[0], wo.layer(a.view(batch, -1))[0])
     assert bool(out.isfinite().all())
+
+
+@pytest.mark.parametrize("M, N, n, r, dtype", [
+    (512, 264, 1, 64, torch.bfloat16), (513, 520, 1, 40, torch.float16), (1023, 2048, 2, 128, torch.bfloat16), (1500, 72, 2, 104, torch.float16),
+    (2049, 136, 3, 24, torch.float16), (2048, 1000, 1, 32, torch.bfloat16), (17000, 128, 2, 64, torch.float16), (16385, 264, 1, 64, torch.bfloat16),
+    (4096, 4096, 8, 64, torch.bfloat16), (4100, 14336, 4, 72, torch.float16)])
+def test_gradients_of_many_tokens(M, N, n, r, dtype):
+    """Sizes at which sums over tokens are formed on tcgen05: ragged stages, columns, rank blocks, lists and windows; tokens in no order."""
+    x, down, up, index, scaling, base = _bank(M, 64, N, n, r, dtype, seed=60)
+    grad = torch.randn(M, N, generator=_gen(61), device=DEV).to(dtype)
+    leaves = [t.requires_grad_() for t in (x, down, up)]
+    y = adapter_matmul(*leaves, index, scaling=scaling, base=base)
+    dx, ddown, dup = torch.autograd.grad(y, leaves, grad)
+    want = _formula(x.detach(), down.detach(), up.detach(), index, scaling, base, grad)
+    for got, name in ((dx, "dx"), (ddown, "ddown"), (dup, "dup")):
+        _check(got, *want[name])
+    assert _lib.lib().bw_device_status() == 0
