@@ -575,6 +575,240 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
     }
 }
 
+// The same on tcgen05, for many tokens: 128 rows of one adapter (M) x blocks of 128 columns (N), reduced over the ranks of values and rests.  Rank values lie
+// K-major as memory has them, rows of w MN-major.  Eight warps bring w and base into a ring, one issues the MMAs (accumulators in turn), eight
+// add the products to base in the ring, a row and half of its columns a lane, and write whole rows from there.
+// Bound by the bytes of base and out: 8192 tokens of 2 adapters, 14336 columns, rank 64, bf16: 88 us (mma.sync 133), 5.4 TB/s, on the 128 SMs that there are CTAs for.
+constexpr int EU_TILE = 128, EU_COLS = 128, EU_JOIN = 8, EU_COPY = 8, EU_THREADS = 32 * (EU_JOIN + EU_COPY + 1);
+__device__ int g_adapter_status = 0;
+
+template <int KS> struct ExpandShape {
+    static constexpr int BLOCKS = KS <= 4 ? 1 : 2;                             // of 64 ranks, of each part
+    static constexpr int A = 2 * BLOCKS * EU_TILE * 128, W_BLOCK = KS * 16 * 128, STAGE = 2 * W_BLOCK + EU_TILE * EU_COLS * 2, STAGES = KS <= 4 ? 4 : 2;
+    static constexpr int SMEM = A + STAGES * STAGE + 1024;
+};
+
+template <typename T, int KS>
+__global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, int64_t per_group, const T *base, T *out) {
+    using S = ExpandShape<KS>;
+    constexpr bool F16 = __is_same(T, __half);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // rank values, rests; the ring: [w | base]
+    __shared__ __align__(16) int s_id[EU_TILE];
+    __shared__ int s_leader[EU_TILE], s_count[4], s_abort;
+    __shared__ uint32_t s_tmem;
+    __shared__ uint8_t list[EU_TILE];
+    __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], acc_full[2], acc_empty[2];
+    volatile int *abort_flag = &s_abort;
+    const Hidden<T> h(hidden, p.M, p.rank);
+    const int64_t t0 = (int64_t)blockIdx.x * EU_TILE, begin = blockIdx.y * per_group, end = begin + per_group < p.cols ? begin + per_group : p.cols;
+    const uint32_t rank_values = smem_addr(smem), ring = rank_values + S::A;
+
+    if (tid == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            umma::mbar_init(&full[i], 33 * EU_COPY);             // (copies of each thread, and each warp)
+            umma::mbar_init(&empty[i], EU_JOIN);
+        }
+        for (int i = 0; i < 2; ++i) {
+            umma::mbar_init(&acc_full[i], 1);
+            umma::mbar_init(&acc_empty[i], EU_JOIN);
+        }
+        s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        umma::fence_proxy_async_smem();
+    }
+    if (warp == EU_JOIN + EU_COPY) umma::tmem_alloc(&s_tmem, 2 * EU_COLS);
+    // the adapters of the tile, in the order of their first token
+    const bool has = tid < EU_TILE && t0 + tid < p.M;
+    const int id = has ? __ldcg(p.index + t0 + tid) : 0;
+    bool first = false;
+    if (warp < 4) {
+        const unsigned there = __ballot_sync(0xffffffffu, has), like = __match_any_sync(0xffffffffu, id);
+        first = has && !(like & there & ((1u << lane) - 1));
+        s_id[tid] = id;
+    }
+    umma::tc_fence_before();
+    __syncthreads();
+    umma::tc_fence_after();
+    pdl_launch_dependents();       // (not before the tensor memory is there: the launch behind may take as much of it, and waits for this one)
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
+    unsigned leaders = 0;
+    if (warp < 4) {
+        for (int j = 0; j < warp * 32; j += 4) {
+            const int4 o = *reinterpret_cast<const int4 *>(s_id + j);
+            if (o.x == id || o.y == id || o.z == id || o.w == id) first = false;
+        }
+        leaders = __ballot_sync(0xffffffffu, first);
+        if (lane == 0) s_count[warp] = __popc(leaders);
+    }
+    __syncthreads();
+    int groups = 0;
+    for (int i = 0; i < 4; ++i) {
+        if (i == warp && first) s_leader[groups + __popc(leaders & ((1u << lane) - 1))] = id;
+        groups += s_count[i];
+    }
+    pdl_wait();                                   // (what comes before is the launch that makes the rank values, or one behind it)
+
+    bool alive = true;                            // (after a failed wait the loops go on without work: the warps meet in them)
+    int it = 0;                                   // blocks of columns so far
+    for (int pass = blockIdx.z; pass < groups; pass += p.slots) {
+        __syncthreads();
+        const int a = s_leader[pass];
+        if (a < 0 && base == out) continue;
+        unsigned mine = 0;
+        if (warp < 4) {
+            mine = __ballot_sync(0xffffffffu, has && id == a);
+            if (lane == 0) s_count[warp] = __popc(mine);
+        }
+        __syncthreads();
+        int count = 0;
+        for (int i = 0; i < 4; ++i) {
+            if (i == warp && (mine >> lane & 1)) list[count + __popc(mine & ((1u << lane) - 1))] = (uint8_t)tid;
+            count += s_count[i];
+        }
+        __syncthreads();
+        if (a < 0 || a >= p.adapters) {
+            // rows without an adapter are base, or zeros; of one beyond the bank NaN
+            const int pieces = (int)((end - begin) / 8);
+            const uint32_t nan = Pair<T>::pack(NAN, NAN);
+            for (int r = warp; r < count; r += EU_THREADS / 32)
+                for (int i = lane; i < pieces; i += 32) {
+                    const int64_t at = (t0 + list[r]) * p.cols + begin + i * 8;
+                    uint4 v = make_uint4(nan, nan, nan, nan);
+                    if (a < 0) v = base ? __ldcg(reinterpret_cast<const uint4 *>(base + at)) : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(out + at) = v;
+                }
+            continue;
+        }
+        if (warp < EU_JOIN) {
+            // ---- products and base; rows of the result ----
+            const int quarter = warp % 4, half = warp / 4 * (EU_COLS / 2), row = quarter * 32 + lane;
+            const bool live = row < count;
+            const int64_t t = t0 + (live ? list[row] : 0);
+            const float f = live ? (F16 ? __ldcg(h.back + t) : 1.0f) * (p.scaling ? __ldcg(p.scaling + a) : 1.0f) : 0.0f;
+            // what the lane stores: piece `lane` % 8 of the half's rows lane / 8, 4 + lane / 8, ..
+            const int stored = quarter * 32 + lane / 8, piece0 = half / 8 + lane % 8;
+            T *to[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[j] = stored + 4 * j < count ? out + (t0 + list[stored + 4 * j]) * p.cols + piece0 * 8 : nullptr;
+            for (int64_t cb = begin; cb < end; cb += EU_COLS, ++it) {
+                const int slot = it % S::STAGES, acc = it & 1;
+                uint8_t *tile = smem + S::A + slot * S::STAGE + 2 * S::W_BLOCK;
+                alive = __all_sync(0xffffffffu, alive && umma::mbar_wait(&acc_full[acc], it >> 1 & 1, abort_flag, 11, &g_adapter_status) &&
+                                                    umma::mbar_wait(&full[slot], it / S::STAGES & 1, abort_flag, 12, &g_adapter_status));
+                const bool work = alive && quarter * 32 < count;
+                if (work) {
+                    umma::tc_fence_after();
+                    uint8_t *own = tile + row * (EU_COLS * 2);
+#pragma unroll
+                    for (int c = 0; c < EU_COLS / 2; c += 32) {
+                        uint4 old[4] = {};
+                        if (base) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) old[k] = *reinterpret_cast<const uint4 *>(own + (((half + c) / 8 + k) ^ (row & 7)) * 16);
+                        }
+                        uint32_t r[32];
+                        umma::tmem_ld_32x32b_x32(tmem + ((uint32_t)(quarter * 32) << 16) + acc * EU_COLS + half + c, r);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            uint32_t *y = reinterpret_cast<uint32_t *>(&old[k]);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 v = Pair<T>::unpack(y[e]);
+                                y[e] = Pair<T>::pack(fmaf(__uint_as_float(r[8 * k + 2 * e]), f, v.x), fmaf(__uint_as_float(r[8 * k + 2 * e + 1]), f, v.y));
+                            }
+                            *reinterpret_cast<uint4 *>(own + (((half + c) / 8 + k) ^ (row & 7)) * 16) = old[k];
+                        }
+                    }
+                    umma::tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0 && alive) umma::mbar_arrive(&acc_empty[acc]);
+                if (work) {
+                    const bool in = cb + piece0 * 8 < end;
+                    uint4 v[8];                              // (all asked for before the first is stored)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int r = stored + 4 * j;
+                        v[j] = *reinterpret_cast<const uint4 *>(tile + r * (EU_COLS * 2) + (piece0 ^ (r & 7)) * 16);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (to[j] && in) *reinterpret_cast<uint4 *>(to[j] + cb) = v[j];
+                }
+                __syncwarp();
+                if (lane == 0 && alive) umma::mbar_arrive(&empty[slot]);
+            }
+        } else if (warp < EU_JOIN + EU_COPY) {
+            // ---- copies ----
+            const int me = tid - 32 * EU_JOIN;
+            // rank values: row me / 2 of either part, ranks in pieces of 8 (ranks behind the last: zeros)
+#pragma unroll
+            for (int i = 0; i < 2 * EU_TILE * KS * 2 / (32 * EU_COPY); ++i) {
+                const int at = me + 32 * EU_COPY * i, piece = at % (2 * KS), row = at / (2 * KS) % EU_TILE, part = at / (2 * KS * EU_TILE);
+                const bool ok = row < count && piece * 8 < p.rank;
+                const T *from = part ? h.rest : h.top;
+                copy16(rank_values + ((part * S::BLOCKS + piece / 8) * EU_TILE + row) * 128 + (piece % 8 ^ (row & 7)) * 16,
+                       ok ? from + (t0 + list[row]) * p.rank + piece * 8 : from, ok ? 16 : 0);
+            }
+            const int piece = me % 16;
+            const T *rows[EU_TILE / 16];                     // this thread's piece of the rows of base
+#pragma unroll
+            for (int i = 0; i < EU_TILE / 16; ++i) rows[i] = base && me / 16 + 16 * i < count ? base + (t0 + list[me / 16 + 16 * i]) * p.cols + piece * 8 : nullptr;
+            for (int64_t cb = begin; cb < end; cb += EU_COLS, ++it) {
+                const int slot = it % S::STAGES;
+                alive = alive && umma::mbar_wait(&empty[slot], (it / S::STAGES & 1) ^ 1, abort_flag, 13, &g_adapter_status);
+                if (alive) {
+                    const uint32_t to = ring + slot * S::STAGE;
+                    const bool in = cb + piece * 8 < end;
+                    // rows of w: blocks of 64 columns
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        const int rank = me / 16 + 16 * i;
+                        const bool ok = in && rank < p.rank;
+                        copy16(to + piece / 8 * S::W_BLOCK + rank * 128 + (piece % 8 ^ (rank & 7)) * 16, ok ? w + ((int64_t)a * p.rank + rank) * p.cols + cb + piece * 8 : w,
+                               ok ? 16 : 0);
+                    }
+                    if (base) {
+#pragma unroll
+                        for (int i = 0; i < EU_TILE / 16; ++i) {
+                            const int row = me / 16 + 16 * i;
+                            if (rows[i]) copy16(to + 2 * S::W_BLOCK + row * (EU_COLS * 2) + (piece ^ (row & 7)) * 16, in ? rows[i] + cb : base, in ? 16 : 0);
+                        }
+                    }
+                    copies_arrive(&full[slot]);
+                }
+                __syncwarp();
+                if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        } else {
+            // ---- products ----
+            const uint32_t idesc = umma::umma_idesc_f16(EU_COLS, !F16, false) | 1u << 16;      // (B MN-major)
+            for (int64_t cb = begin; cb < end; cb += EU_COLS, ++it) {
+                const int slot = it % S::STAGES, acc = it & 1;
+                alive = __all_sync(0xffffffffu, alive && umma::mbar_wait(&acc_empty[acc], (it >> 1 & 1) ^ 1, abort_flag, 14, &g_adapter_status) &&
+                                                    umma::mbar_wait(&full[slot], it / S::STAGES & 1, abort_flag, 15, &g_adapter_status));
+                if (!alive) continue;
+                umma::fence_proxy_async_smem();
+                umma::tc_fence_after();
+                const uint32_t at = ring + slot * S::STAGE;
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int k = 0; k < KS; ++k)
+                        umma::umma_f16_ss(tmem + acc * EU_COLS, umma::umma_smem_desc(rank_values + (part * S::BLOCKS + k / 4) * EU_TILE * 128 + k % 4 * 32),
+                                          umma::umma_smem_desc_mn(at + k * 2048, S::W_BLOCK), idesc, (part | k) != 0 ? 1u : 0u);
+                umma::umma_commit(&acc_full[acc]);
+            }
+        }
+    }
+    __syncthreads();
+    umma::tc_fence_after();
+    if (warp == EU_JOIN + EU_COPY) umma::tmem_dealloc(tmem, 2 * EU_COLS);
+}
+
 // ---- outer ---------------------------------------------------------------------------------------------------------------
 
 constexpr int OUTER_LIST = 2048, OUTER_STEP = 32, OUTER_WINDOW = 1024;      // tokens of a list, of a stage; words of 32 tokens looked at together
@@ -859,8 +1093,6 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 constexpr int OU_STAGES = 8, OU_A = 2 * OUTER_STEP * 128, OU_B = 4 * OUTER_STEP * 128, OU_STAGE = OU_A + OU_B, OU_THREADS = 352,
               OU_SMEM = OU_STAGES * OU_STAGE + 1024, OU_LIST = 1024, OU_WINDOW = 512;
 static_assert(64 * SUM_ROW * 4 <= OU_STAGES * OU_STAGE, "the sums take the ring's place");
-__device__ int g_adapter_status = 0;
-
 template <typename T>
 __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
     constexpr bool F16 = __is_same(T, __half);
@@ -1174,7 +1406,27 @@ int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStre
 }
 
 template <typename T, int KS>
+int expand_umma(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaStream_t st) {
+    using S = ExpandShape<KS>;
+    p.slots = p.adapters + 1 < 2 ? p.adapters + 1 : 2;
+    int per_sm = 0;
+    const int rc = ctas_per_sm<adapter_expand_umma_kernel<T, KS>>(EU_THREADS, S::SMEM, per_sm);
+    if (rc != BW_OK) return rc;
+    const int64_t tiles = (p.M + EU_TILE - 1) / EU_TILE, blocks = (p.cols + EU_COLS - 1) / EU_COLS, most = (blocks + 1) / 2;
+    // (where an adapter's run of tokens ends, a tile has another one's as well)
+    const int64_t passes = tiles + (p.adapters - 1 < tiles ? p.adapters - 1 : tiles);
+    const int groups = parts_of(passes, SMS, most < 64 ? most : 64, 5.0 / blocks);      // (a start takes as long as five blocks)
+    const int64_t per_group = (blocks + groups - 1) / groups * EU_COLS;
+    return launch_early("adapter_expand_umma_kernel", adapter_expand_umma_kernel<T, KS>, dim3((unsigned)tiles, (unsigned)((p.cols + per_group - 1) / per_group), p.slots), EU_THREADS, S::SMEM,
+                        st, dim3(1), h, w, p, per_group, base, out);
+}
+template <typename T, int KS>
 int expand_fast(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaStream_t st) {
+    // tcgen05 has one CTA an SM, whose start takes some microseconds.  Rank 64, bf16, shrink of 64 columns and expand, us, mma.sync / tcgen05: 8192 tokens of one
+    // adapter to 14336 columns 127 / 91, of 8 144 / 105; 8192 tokens to 4096 columns 49 / 36, 49 / 48; 2048 of one 19 / 17, of two 22 / 23; 1024 of one 14.7 / 13.6, to 1024 columns
+    // 9.3 / 11.9; rank 32, 8192 tokens of one to 14336 columns 99 / 91, of 8 in any order 370 / 488.
+    if constexpr (KS > 2)
+        if (p.M >= 1024 && p.M >= (int64_t)256 * p.adapters && p.M * p.cols >= (int64_t)(p.adapters == 1 ? 8 : 24) << 20) return expand_umma<T, KS>(h, w, p, base, out, st);
     constexpr int SMEM = (KS * 16 + TILE) * 128 * (KS <= 4 ? 4 : 3);
     p.slots = slots_of(p);
     if (p.M <= FEW)

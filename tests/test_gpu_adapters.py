@@ -348,6 +348,29 @@ def test_gradients_of_many_tokens(M, N, n, r, dtype):
     y = adapter_matmul(*leaves, index, scaling=scaling, base=base)
     dx, ddown, dup = torch.autograd.grad(y, leaves, grad)
     want = _formula(x.detach(), down.detach(), up.detach(), index, scaling, base, grad)
-    for got, name in ((dx, "dx"), (ddown, "ddown"), (dup, "dup")):
+    for got, name in ((y.detach(), "y"), (dx, "dx"), (ddown, "ddown"), (dup, "dup")):
         _check(got, *want[name])
+    assert _lib.lib().bw_device_status() == 0
+
+
+@pytest.mark.parametrize("M, K, N, n, r, order, dtype", [
+    (1027, 64, 8200, 1, 64, "any", torch.float16), (2050, 128, 12296, 3, 128, "any", torch.bfloat16), (6300, 64, 4000, 5, 40, "runs", torch.float16),
+    (24600, 64, 1032, 2, 48, "any", torch.bfloat16), (3200, 256, 8064, 12, 104, "runs", torch.float16), (2050, 64, 1288, 9, 16, "any", torch.bfloat16),
+    (5000, 64, 8, 3, 8, "runs", torch.bfloat16), (4096, 512, 2048, 200, 64, "any", torch.float16)])
+def test_results_of_many_tokens(M, K, N, n, r, order, dtype):
+    """With a base, without one and over it; an index beyond the bank gives NaN in its rows alone."""
+    x, down, up, index, scaling, base = _bank(M, K, N, n, r, dtype, seed=70, order=order)
+    want = _formula(x, down, up, index, scaling, base)["y"]
+    y = adapter_matmul(x, down, up, index, scaling=scaling, base=base)
+    _check(y, *want)
+    over = base.clone()
+    assert adapter_matmul(x, down, up, index, scaling=scaling, base=over, out=over) is over and torch.equal(over, y)
+    _check(adapter_matmul(x, down, up, index, scaling=scaling), *_formula(x, down, up, index, scaling, None)["y"])
+    beyond = index.clone()
+    beyond[::7] = n + 3
+    z = adapter_matmul(x, down, up, beyond, scaling=scaling, base=base)
+    assert bool(z[::7].isnan().all())
+    keep = torch.ones(M, dtype=torch.bool, device=DEV)
+    keep[::7] = False
+    assert torch.equal(z[keep], y[keep])
     assert _lib.lib().bw_device_status() == 0
