@@ -697,12 +697,24 @@ __global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
     if (parts == 1) return;
     const int64_t size = (int64_t)p.cols * (DIM + 2);             // of a slot; the first CTA's part is in its second one, the others' in their first
     auto slot = [&](int i) { return p.slots + (2 * (int64_t)(first + i) + (i == 0)) * size; };
-    __shared__ float s_f[MOST_CTAS], s_part[4], s_o[4][DIM];
+    __shared__ float s_f[MOST_CTAS], s_l[MOST_CTAS], s_part[4], s_o[4][DIM];
+    // A warp takes every fourth part; the first of them are asked for before their factors are known.
+    constexpr int V = DIM / 32, AHEAD = 32 / V;
+    float ahead[AHEAD][V];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (warp + 4 * i < parts) {
+            const float *from = slot(warp + 4 * i) + (int64_t)col * DIM + lane;
+#pragma unroll
+            for (int k = 0; k < V; ++k) ahead[i][k] = __ldcg(from + 32 * k);
+        }
     // factors of the parts: 2^(m - largest m)
     float top = -INFINITY;
     for (int i = threadIdx.x; i < parts; i += 128) {
-        s_f[i] = __ldcg(slot(i) + p.cols * DIM + 2 * col);
-        top = fmaxf(top, s_f[i]);
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(i) + p.cols * DIM + 2 * col));
+        s_f[i] = ml.x;
+        s_l[i] = ml.y;
+        top = fmaxf(top, ml.x);
     }
     for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     if (lane == 0) s_part[warp] = top;
@@ -710,18 +722,22 @@ __global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
     top = fmaxf(fmaxf(s_part[0], s_part[1]), fmaxf(s_part[2], s_part[3]));
     float l = 0.0f;
     for (int i = threadIdx.x; i < parts; i += 128) {
-        const float f = s_f[i] == -INFINITY ? 0.0f : ex2(s_f[i] - top), sum = __ldcg(slot(i) + p.cols * DIM + 2 * col + 1);
+        const float f = s_f[i] == -INFINITY ? 0.0f : ex2(s_f[i] - top), sum = s_l[i];
         s_f[i] = f;
         l += sum == sum ? f * sum : NAN;
     }
     for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
     __syncthreads();
     if (lane == 0) s_part[warp] = l;
-    // a warp takes every fourth part
-    constexpr int V = DIM / 32;
     float o[V] = {};
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (warp + 4 * i < parts) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) o[k] += s_f[warp + 4 * i] * ahead[i][k];
+        }
 #pragma unroll 4
-    for (int i = warp; i < parts; i += 4) {
+    for (int i = warp + 4 * AHEAD; i < parts; i += 4) {
         const float f = s_f[i], *from = slot(i) + (int64_t)col * DIM + lane;
 #pragma unroll
         for (int k = 0; k < V; ++k) o[k] += f * __ldcg(from + 32 * k);
