@@ -111,13 +111,14 @@ int attend_general(const AttendArgs &p, int64_t batch, int bits, cudaStream_t st
 //            higher bits of their byte (`planes`) are larger by a power of two and get accumulators of their own.  Scale and zero point
 //            are applied to the sums, in fp32: nothing is rounded.
 //   weights  p = 2^(x - m); p * (value's scale) goes to fp16 for the second product.  m covers p * scale, so that this stays in fp16's
-//            range whatever the scales are; it moves only when some p * scale leaves [0, 1024] (one vote a step).  For fp16 results the
-//            rest p - fp16(p) goes through MMAs of its own: one rounding of 2^-11 less in the result.  For bf16 results that
-//            rounding is an eighth of the result's own.
+//            range whatever the scales are; it moves only when some p * scale leaves [0, 1024] (one vote a step).  The
+//            rest p - fp16(p) is multiplied as well: 22 bits of a weight count, for bf16 results too (without, they were off by up to 2^-12 of sum w |v|,
+//            an eighth of their own rounding).
 //   values   O[d][h] += (code - zero_t)[d][t] * p[t][h]: 1024 + code by one OR, minus (1024 + zero), exact.  ldmatrix.trans puts
 //            16 bits (2 to 8 codes) of two tokens beside each other, as the operand wants them.
 // Groups of up to 4 heads fill half of the eight columns: their steps are two tiles, whose scores share one set of registers (columns 0 to 3
-// the first tile's, 4 to 7 the second's), which halves the work on weights; the columns' sums meet at the end.
+// the first tile's, 4 to 7 the second's), which halves the work on weights; the columns' sums meet at the end, and where one tile's values are
+// multiplied the other's columns take the rests of its weights: they cost no MMA (both columns of a head go by one maximum).
 //
 // Bound by the bytes of the cache up to here, and by instruction issue at 2 and 4 bits.  Each warp has a ring of steps in shared memory, filled by
 // 16-byte cp.async and read by it alone: no block-wide barrier in the loop, and the loads in flight cost no registers.
@@ -231,7 +232,6 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
     using S = Shape<BITS, DIM>;
     using C = Config<T, BITS, DIM, NB, PAIR>;
     static_assert(PAIR == 1 || NB == 1, "steps of two tiles are for groups of up to four heads");
-    constexpr bool REST = __is_same(T, __half);
     constexpr int COLS = C::COLS, STAGES = C::STAGES, HEADS = PAIR == 2 ? 4 : COLS;
     const AttendArgs &a = p.a;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4;
@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
                         for (int row = 0; row < 2; ++row)
                             if (live[row]) top = fmaxf(top, u[nb][2 * row + j] + lv[row]);
-                        for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        for (int d = PAIR == 2 ? 2 : 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));      // (of a head's two columns as well)
                         const float keep = m[nb][j] == -INFINITY ? 0.0f : ex2(m[nb][j] - top);
                         m[nb][j] = top;
                         l[nb][j] *= keep;
@@ -529,11 +529,10 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
                     l[nb][0] += pw[nb][2 * j];
                     l[nb][1] += pw[nb][2 * j + 1];
                     const __half2 top = __floats2half2_rn(pv[nb][2 * j], pv[nb][2 * j + 1]);
+                    const float2 t = __half22float2(top);
                     w[nb][j][0] = transpose8x8(as_u32(top));
-                    if constexpr (REST) {
-                        const float2 t = __half22float2(top);
-                        w[nb][j][1] = transpose8x8(as_u32(__floats2half2_rn(pv[nb][2 * j] - t.x, pv[nb][2 * j + 1] - t.y)));
-                    }
+                    w[nb][j][1] = transpose8x8(as_u32(__floats2half2_rn(pv[nb][2 * j] - t.x, pv[nb][2 * j + 1] - t.y)));
+                    if constexpr (PAIR == 2) w[nb][j][1] = __shfl_xor_sync(0xffffffffu, w[nb][j][1], 16);      // to the head's other column
                 }
             // Zero points of two tokens beside each other.  (The transposed matrix has every column of a row alike where a step is one tile; of two tiles
             // columns 0 to 3, now rows, have the first one's and 4 to 7 the second one's.)
@@ -543,7 +542,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
             for (int i = 0; i < PAIR; ++i) {
                 __half2 zero[S::PLANES][2];
-                uint32_t b0[NB][2], b1[NB][2];
+                uint32_t b0[NB][3 - PAIR], b1[NB][3 - PAIR];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     uint32_t z = zt[j];
@@ -554,10 +553,10 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                    for (int k = 0; k < (REST ? 2 : 1); ++k) {
-                        const bool mine = PAIR == 1 || r / 4 == i;      // columns of this tile's weights
-                        b0[nb][k] = mine ? w[nb][0][k] : 0u;
-                        b1[nb][k] = mine ? w[nb][1][k] : 0u;
+                    for (int k = 0; k < 3 - PAIR; ++k) {
+                        const int part = PAIR == 1 ? k : r / 4 != i;      // (of two tiles the columns of the other one's weights take this one's rests)
+                        b0[nb][k] = part ? w[nb][0][1] : w[nb][0][0];
+                        b1[nb][k] = part ? w[nb][1][1] : w[nb][1][0];
                     }
                 const uint32_t values = buf + i * S::BYTES + 16 * S::ROW;
 #pragma unroll
@@ -579,7 +578,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
                                 mma(o[nb][(piece + h) * S::PLANES + pl], a0, a1, a2, a3, b0[nb][0], b1[nb][0]);
-                                if constexpr (REST) mma(o[nb][(piece + h) * S::PLANES + pl], a0, a1, a2, a3, b0[nb][1], b1[nb][1]);
+                                if constexpr (PAIR == 1) mma(o[nb][(piece + h) * S::PLANES + pl], a0, a1, a2, a3, b0[nb][2 - PAIR], b1[nb][2 - PAIR]);
                             }
                         }
                     }

@@ -1,0 +1,58 @@
+"""Attention over the quantised cache holds its weights and queries as exactly as fp32 sums do, whatever the result's type."""
+import pytest
+import torch
+
+from bitween_b200 import QuantizedKVCache
+from bitween_b200.kernels import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _between(got, want, slack):
+    """Rounding keeps order: a value within `slack` of `want`, rounded once, lies between the two ends' roundings."""
+    return (got >= (want - slack).to(got.dtype)) & (got <= (want + slack).to(got.dtype))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,bits,lengths", [
+    (4, 4, 128, 4, [24] * 48),                     # up to four heads a cache head: steps of two tiles
+    (16, 4, 64, 8, [40, 9, 24, 1] * 16),
+    (16, 4, 128, 2, [33] * 24),
+    (12, 2, 128, 8, [24] * 32),                    # five to eight: steps of one
+    (32, 2, 64, 4, [24] * 32),                     # more: two blocks of eight columns
+    (4, 2, 256, 4, [24] * 24),
+    (8, 2, 128, 4, [700, 30] * 20),                # shares of the line of work, and a join
+    (6, 6, 80, 4, [24] * 32),                      # the general kernel
+])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_weights_keep_more_bits_than_the_result(heads, kv_heads, dim, bits, lengths, dtype):
+    """With scores of at most 1/2 (in powers of two) their fp32 errors are below 2^-19.5 of a weight: at most 20 truncated accumulations of products and three roundings
+    of the zero point's part, 2^-23 of 1/2 each.  ex2 is good to 2^-22, a weight is held to 2^-22 (value and rest, 11 bits each) and the sums over a warp's few steps
+    and the join to some 2^-23.  Numerator and denominator together: less than 2^-17.5 of sum w |v|.  (A weight of 11 bits is off by up to 2^-12.)"""
+    page, batch = 16, len(lengths)
+    wide = -(-max(lengths) // page)
+    cache = QuantizedKVCache(batch * wide, page, kv_heads, dim, bits=bits, device=DEV)
+    table = torch.randperm(batch * wide, generator=_gen(1), device=DEV).view(batch, wide)
+    pos = torch.arange(wide * page, device=DEV)
+    slots = table[:, pos // page] * page + pos % page
+    cache.append(*(torch.randn(slots.numel(), kv_heads, dim, generator=_gen(s), device=DEV) * (0.5 + torch.rand(slots.numel(), kv_heads, 1, generator=_gen(s + 9), device=DEV))
+                   for s in (2, 3)), slots.flatten())
+    q = torch.randn(batch, heads, dim, generator=_gen(4), device=DEV).to(dtype)
+    k, v = (x.double().view(batch, wide * page, kv_heads, dim) for x in cache.read(slots.flatten(), dtype=torch.float32))
+    span = cache.params[..., 0].float().amax() * (2 ** bits - 1)
+    alpha = 0.5 / (1.4427 * float(span * q.float().abs().sum(-1).amax()))
+    got = cache.attend(q, table.to(torch.int32), torch.tensor(lengths, dtype=torch.int32, device=DEV), softmax_scale=alpha)
+    group = heads // kv_heads
+    score = torch.einsum("bhgd,bthd->bhgt", q.double().view(batch, kv_heads, group, dim), k) * alpha
+    live = pos[None] < torch.tensor(lengths, device=DEV)[:, None]
+    w = torch.softmax(score.masked_fill(~live[:, None, None], -torch.inf), -1)
+    want = torch.einsum("bhgt,bthd->bhgd", w, v).view(q.shape)
+    size = torch.einsum("bhgt,bthd->bhgd", w, v.abs()).view(q.shape)
+    ok = _between(got, want, 2.0 ** -17.5 * size)
+    bad = int((~ok).sum())
+    assert bad == 0, f"{bad} of {ok.numel()}"
+    assert _lib.lib().bw_device_status() == 0
