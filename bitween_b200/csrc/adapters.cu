@@ -11,8 +11,8 @@
 //     lane's 16 bytes of a row serve two MMAs, k pairs (0, 1), (2, 3) and (4, 5), (6, 7);
 //   * where it runs over rows (expand over ranks, outer over tokens), a lane takes 16 bytes of four rows, eight columns of its own, and
 //     pairs the rows by byte permutations: MMA j of eight has column j of every lane.  A lane's results are then 16 neighbours of a row.
-// Rank values are summed in 32 bits and kept as two 16-bit parts (value and rest), which hold 16 (bf16) or 22 (fp16) of their bits and are
-// what the second product takes.  fp16 parts are of h * 2^-e, e of the row's largest: gradients without loss scaling would be lost below
+// Rank values are summed in 32 bits and kept in 16-bit parts (value and rests: three of bf16, two of fp16), which hold 24 (bf16) or 22 (fp16) of their bits and are
+// what the second product takes.  (Two of bf16 hold 16: results of bf16 were off by up to 2^-17 more than their own rounding.)  fp16 parts are of h * 2^-e, e of the row's largest: gradients without loss scaling would be lost below
 // 2^-14, and large rank values beyond 65504.
 //
 // Tokens of one adapter need not be neighbours: a tile of 64 tokens goes through the adapters that occur in it, one after the other or (few
@@ -136,11 +136,14 @@ struct AdapterArgs {
     bool behind;                // another launch of this call comes before: all that came before that is done when this one starts
 };
 
-// Rank values: [M][rank] of 16 bits, the same of their rests, and (fp16) [M] powers of two by which both were divided.
+// Rank values: [parts][M][rank] of 16 bits (the values, their rests, for bf16 the rests of those), and (fp16) [M] powers of two by which all were divided.
+template <typename T> constexpr int PARTS = __is_same(T, __half) ? 2 : 3;
 template <typename T> struct Hidden {
-    T *top, *rest;
+    T *top;
+    int64_t size;             // of a part
     float *back;
-    __host__ __device__ Hidden(void *p, int64_t M, int r) : top((T *)p), rest(top + M * r), back(reinterpret_cast<float *>(rest + M * r)) {}
+    __host__ __device__ Hidden(void *p, int64_t M, int r) : top((T *)p), size(M * r), back(reinterpret_cast<float *>(top + PARTS<T> * size)) {}
+    __device__ __forceinline__ T *part(int i) const { return top + i * size; }
 };
 
 // The adapters that occur in a tile of tokens, in the order of their first token, each with a list of its tokens (every warp has its own).  Tokens
@@ -188,7 +191,7 @@ struct TileAdapters {
 };
 
 // The end of a shrink pass: the CTAs of a cluster have sums of their part of the columns in `sums` [rows][RANKS + 4]; each CTA adds up its share of
-// the rows, a warp a row, and writes them as two 16-bit parts.
+// the rows, a warp a row, and writes them in 16-bit parts.
 template <typename T, int RANKS>
 __device__ __forceinline__ void finish_rows(float *sums, int rows, int row0, int count, const uint8_t *list, int64_t t0, const AdapterArgs &p, const Hidden<T> &h) {
     constexpr bool F16 = __is_same(T, __half);
@@ -223,10 +226,14 @@ __device__ __forceinline__ void finish_rows(float *sums, int rows, int row0, int
         for (int i = 0; i < PAIRS; ++i) {
             const int j = 2 * (lane + 32 * i);
             if (j < p.rank) {
-                const uint32_t top = Pair<T>::pack(v[i].x * by, v[i].y * by);
-                const float2 f = Pair<T>::unpack(top);
-                *reinterpret_cast<uint32_t *>(h.top + t * p.rank + j) = top;
-                *reinterpret_cast<uint32_t *>(h.rest + t * p.rank + j) = Pair<T>::pack(v[i].x * by - f.x, v[i].y * by - f.y);
+                float2 left = make_float2(v[i].x * by, v[i].y * by);
+#pragma unroll
+                for (int part = 0; part < PARTS<T>; ++part) {
+                    const uint32_t here = Pair<T>::pack(left.x, left.y);
+                    const float2 f = Pair<T>::unpack(here);
+                    *reinterpret_cast<uint32_t *>(h.part(part) + t * p.rank + j) = here;
+                    left = make_float2(left.x - f.x, left.y - f.y);
+                }
             }
         }
     }
@@ -386,18 +393,19 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
 
 // ---- expand --------------------------------------------------------------------------------------------------------------
 
-// Fragments of the rank values of 16 rows: [steps][value and rest].  
+// Fragments of the rank values of 16 rows, from step `first` of 16 ranks on: [parts][steps].
 template <typename T, int KS>
-__device__ __forceinline__ void load_rank_values(const Hidden<T> &h, int rank, int64_t ta, int64_t tb, bool has_a, bool has_b, int c, uint32_t (&top)[KS][4], uint32_t (&rest)[KS][4]) {
+__device__ __forceinline__ void load_rank_values(const Hidden<T> &h, int rank, int first, int64_t ta, int64_t tb, bool has_a, bool has_b, int c,
+                                                 uint32_t (&values)[PARTS<T>][KS][4]) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int j = 16 * ks + 2 * c + e / 2 * 8;
+            const int j = 16 * (first + ks) + 2 * c + e / 2 * 8;
             const bool has = (e % 2 ? has_b : has_a) && j < rank;
             const int64_t at = (e % 2 ? tb : ta) * rank + j;
-            top[ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.top + at)) : 0u;
-            rest[ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.rest + at)) : 0u;
+#pragma unroll
+            for (int part = 0; part < PARTS<T>; ++part) values[part][ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.part(part) + at)) : 0u;
         }
 }
 // What a row's product is multiplied by.
@@ -461,16 +469,20 @@ __global__ void __launch_bounds__(128) adapter_expand_few_kernel(void *hidden, c
             const float f[2] = {row_factor(h, p, a, t[0], live[0]), row_factor(h, p, a, t[1], live[1])};
             float acc[8][4] = {};
             if (has) {
-                uint32_t top[KS][4], rest[KS][4];
-                load_rank_values<T, KS>(h, p.rank, t[0], t[1], live[0], live[1], c, top, rest);
+                constexpr int SOME = KS < 4 ? KS : 4;             // (steps at once, which registers hold)
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
+                for (int k0 = 0; k0 < KS; k0 += SOME) {
+                    uint32_t values[PARTS<T>][SOME][4];
+                    load_rank_values<T, SOME>(h, p.rank, k0, t[0], t[1], live[0], live[1], c, values);
 #pragma unroll
-                    for (int n = 0; n < 8; ++n) {
-                        const uint32_t b0 = column_pair(raw[ks][0], raw[ks][1], n), b1 = column_pair(raw[ks][2], raw[ks][3], n);
-                        Pair<T>::mma(acc[n], top[ks], b0, b1);
-                        Pair<T>::mma(acc[n], rest[ks], b0, b1);
-                    }
+                    for (int ks = 0; ks < SOME; ++ks)
+#pragma unroll
+                        for (int n = 0; n < 8; ++n) {
+                            const uint32_t b0 = column_pair(raw[k0 + ks][0], raw[k0 + ks][1], n), b1 = column_pair(raw[k0 + ks][2], raw[k0 + ks][3], n);
+#pragma unroll
+                            for (int part = 0; part < PARTS<T>; ++part) Pair<T>::mma(acc[n], values[part][ks], b0, b1);
+                        }
+                }
             }
             T *const to[2] = {out + t[0] * p.cols + cb + 16 * c, out + t[1] * p.cols + cb + 16 * c};
             store_rows<T>(to, live, in, old, acc, f, a < 0);
@@ -533,8 +545,8 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
         const int row = warp * 16 + r;
         const bool live[2] = {row < tile.count, row + 8 < tile.count};
         const int64_t t[2] = {t0 + (live[0] ? tile.list[row] : 0), t0 + (live[1] ? tile.list[row + 8] : 0)};
-        uint32_t top[KS][4], rest[KS][4];
-        load_rank_values<T, KS>(h, p.rank, t[0], t[1], live[0] && has, live[1] && has, c, top, rest);
+        uint32_t values[PARTS<T>][KS][4];
+        load_rank_values<T, KS>(h, p.rank, 0, t[0], t[1], live[0] && has, live[1] && has, c, values);
         const float f[2] = {row_factor(h, p, a, t[0], live[0]), row_factor(h, p, a, t[1], live[1])};
         int stage = 0;
         const bool busy = warp * 16 < tile.count;
@@ -558,8 +570,8 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
 #pragma unroll
                     for (int n = 0; n < 8; ++n) {
                         const uint32_t b0 = column_pair(raw[0], raw[1], n), b1 = column_pair(raw[2], raw[3], n);
-                        Pair<T>::mma(acc[n], top[ks], b0, b1);
-                        Pair<T>::mma(acc[n], rest[ks], b0, b1);
+#pragma unroll
+                        for (int part = 0; part < PARTS<T>; ++part) Pair<T>::mma(acc[n], values[part][ks], b0, b1);
                     }
                 }
             }
@@ -576,25 +588,25 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
 }
 
 // The same on tcgen05, for many tokens: 128 rows of one adapter (M) x blocks of 128 columns (N), reduced over the ranks of values and rests.  Rank values lie
-// K-major as memory has them, rows of w MN-major.  Eight warps bring w and base into a ring, one issues the MMAs (accumulators in turn), eight
+// K-major as memory has them (their parts one after the other), rows of w MN-major.  Eight warps bring w and base into a ring, one issues the MMAs (accumulators in turn), eight
 // add the products to base in the ring, a row and half of its columns a lane, and write whole rows from there.
 // Bound by the bytes of base and out: 8192 tokens of 2 adapters, 14336 columns, rank 64, bf16: 88 us (mma.sync 133), 5.4 TB/s, on the 128 SMs that there are CTAs for.
 constexpr int EU_TILE = 128, EU_COLS = 128, EU_JOIN = 8, EU_COPY = 8, EU_THREADS = 32 * (EU_JOIN + EU_COPY + 1);
 __device__ int g_adapter_status = 0;
 
-template <int KS> struct ExpandShape {
+template <int KS, int PARTS> struct ExpandShape {
     static constexpr int BLOCKS = KS <= 4 ? 1 : 2;                             // of 64 ranks, of each part
-    static constexpr int A = 2 * BLOCKS * EU_TILE * 128, W_BLOCK = KS * 16 * 128, STAGE = 2 * W_BLOCK + EU_TILE * EU_COLS * 2, STAGES = KS <= 4 ? 4 : 2;
+    static constexpr int A = PARTS * BLOCKS * EU_TILE * 128, W_BLOCK = KS * 16 * 128, STAGE = 2 * W_BLOCK + EU_TILE * EU_COLS * 2, STAGES = KS > 4 ? 2 : PARTS == 2 ? 4 : 3;
     static constexpr int SMEM = A + STAGES * STAGE + 1024;
 };
 
 template <typename T, int KS>
 __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, int64_t per_group, const T *base, T *out) {
-    using S = ExpandShape<KS>;
+    using S = ExpandShape<KS, PARTS<T>>;
     constexpr bool F16 = __is_same(T, __half);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
     extern __shared__ uint8_t raw_smem[];
-    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // rank values, rests; the ring: [w | base]
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // parts of the rank values; the ring: [w | base]
     __shared__ __align__(16) int s_id[EU_TILE];
     __shared__ int s_leader[EU_TILE], s_count[4], s_abort;
     __shared__ uint32_t s_tmem;
@@ -743,12 +755,12 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
         } else if (warp < EU_JOIN + EU_COPY) {
             // ---- copies ----
             const int me = tid - 32 * EU_JOIN;
-            // rank values: row me / 2 of either part, ranks in pieces of 8 (ranks behind the last: zeros)
+            // rank values: rows of each part, ranks in pieces of 8 (ranks behind the last: zeros)
 #pragma unroll
-            for (int i = 0; i < 2 * EU_TILE * KS * 2 / (32 * EU_COPY); ++i) {
+            for (int i = 0; i < PARTS<T> * EU_TILE * KS * 2 / (32 * EU_COPY); ++i) {
                 const int at = me + 32 * EU_COPY * i, piece = at % (2 * KS), row = at / (2 * KS) % EU_TILE, part = at / (2 * KS * EU_TILE);
                 const bool ok = row < count && piece * 8 < p.rank;
-                const T *from = part ? h.rest : h.top;
+                const T *from = h.part(part);
                 copy16(rank_values + ((part * S::BLOCKS + piece / 8) * EU_TILE + row) * 128 + (piece % 8 ^ (row & 7)) * 16,
                        ok ? from + (t0 + list[row]) * p.rank + piece * 8 : from, ok ? 16 : 0);
             }
@@ -795,7 +807,7 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
                 umma::tc_fence_after();
                 const uint32_t at = ring + slot * S::STAGE;
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+                for (int part = 0; part < PARTS<T>; ++part)
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
                         umma::umma_f16_ss(tmem + acc * EU_COLS, umma::umma_smem_desc(rank_values + (part * S::BLOCKS + k / 4) * EU_TILE * 128 + k % 4 * 32),
@@ -899,10 +911,10 @@ __device__ __forceinline__ void join_sums(float *sums, const AdapterArgs &p, int
     }
 }
 // RB blocks of 16 ranks a warp, RG groups of four warps with ranks of their own.
-template <int RB, int RG> struct OuterShape {
+template <int RB, int RG, int PARTS> struct OuterShape {
     static constexpr int WARPS = 4 * RG, THREADS = 32 * WARPS;
-    static constexpr int RANKS = 16 * RB * RG, ROW = RANKS * 2;               // bytes of a token's rank values
-    static constexpr int STAGE = OUTER_STEP * (512 + 2 * ROW), STAGES = RG == 1 ? 4 : 3;
+    static constexpr int RANKS = 16 * RB * RG, ROW = RANKS * 2;               // bytes of a part of a token's rank values
+    static constexpr int STAGE = OUTER_STEP * (512 + PARTS * ROW), STAGES = RG == 1 ? 4 : 3;
     static constexpr int SUMS = RANKS * SUM_ROW * 4, SMEM = STAGE * STAGES > SUMS ? STAGE * STAGES : SUMS;
     static __device__ __forceinline__ int swizzle(int token) { return ROW >= 128 ? token & 7 : ROW == 64 ? token >> 1 & 3 : token >> 2 & 1; }
 };
@@ -913,7 +925,7 @@ template <int RB, int RG> struct OuterShape {
 // what mma.sync can do; the copies' issue, the barrier of a stage and the MMAs take turns.)
 template <typename T, int RB, int RG>
 __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
-    using S = OuterShape<RB, RG>;
+    using S = OuterShape<RB, RG, PARTS<T>>;
     constexpr bool F16 = __is_same(T, __half);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32, r = lane / 4, c = lane % 4, wc = warp % 4, wr = warp / 4;
     const int rank_blocks = (p.rank + S::RANKS - 1) / S::RANKS, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * S::RANKS;
@@ -941,8 +953,8 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0;
     const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0));
     const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2, x_to = warp * 512 + (lane ^ (warp >> 1 & 3) << 1) * 16;
-    // and its pieces of the rank values and of their rests
-    constexpr int PIECES = S::ROW / 16, HJ = OUTER_STEP * PIECES * 2 / S::THREADS;
+    // and its pieces of the rank values' parts
+    constexpr int PIECES = S::ROW / 16, ALL = OUTER_STEP * PIECES * PARTS<T>, HJ = (ALL + S::THREADS - 1) / S::THREADS;
     const uint8_t *h_from[HJ];
     uint32_t h_to[HJ];
     int h_token[HJ], h_bytes[HJ];
@@ -951,7 +963,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
         const int i = threadIdx.x + S::THREADS * j, part = i / (OUTER_STEP * PIECES), token = i / PIECES % OUTER_STEP, piece = i % PIECES;
         h_token[j] = token;
         h_bytes[j] = rank0 + piece * 8 < p.rank ? 16 : 0;
-        h_from[j] = (const uint8_t *)((part ? h.rest : h.top) + (h_bytes[j] ? rank0 + piece * 8 : 0));
+        h_from[j] = (const uint8_t *)(h.part(part) + (h_bytes[j] ? rank0 + piece * 8 : 0));
         h_to[j] = OUTER_STEP * (512 + part * S::ROW) + token * S::ROW + (piece ^ S::swizzle(token)) * 16;
     }
     // a lane's places in the stage: token 2 c, piece r of its warp's columns; and rows of rank values for ldmatrix
@@ -986,7 +998,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                     copy16(to + (x_to ^ (S::WARPS * j / 2 & 3) * 32) + S::WARPS * j * 512, xs0 + (uint64_t)(uint32_t)list[first + warp + S::WARPS * j] * x_row, x_bytes);
 #pragma unroll
                 for (int j = 0; j < HJ; ++j)
-                    copy16(to + h_to[j], h_from[j] + (uint64_t)(uint32_t)list[first + h_token[j]] * h_row, first + h_token[j] < n ? h_bytes[j] : 0);
+                    if (ALL % S::THREADS == 0 || threadIdx.x + S::THREADS * j < ALL) copy16(to + h_to[j], h_from[j] + (uint64_t)(uint32_t)list[first + h_token[j]] * h_row, first + h_token[j] < n ? h_bytes[j] : 0);
             }
             copies_commit();
         };
@@ -1049,7 +1061,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-                    for (int part = 0; part < 2; ++part) {
+                    for (int part = 0; part < PARTS<T>; ++part) {
                         uint32_t ha[4];
                         load_matrices_transposed(place + h_place[rb] + (part * OUTER_STEP + step * 16) * S::ROW, ha);
                         if constexpr (F16) {
@@ -1085,32 +1097,37 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 
 // The same on tcgen05, for adapters of many tokens: 64 ranks x 256 columns a CTA, reduced over tokens, 32 a stage.  Rows of x and of the rank values keep
 // the order in which memory holds them, which is the MN-major form of both operands (blocks of 64 elements by 32 tokens, 128-byte swizzle).  Values and
-// rests of 64 ranks are the two halves of the M dimension, so that one MMA multiplies both; their sums meet at the end.  Eight warps fill the ring with
+// rests of 64 ranks are the two halves of the M dimension, so that one MMA multiplies both; their sums meet at the end.  The third part of bf16 takes MMAs of
+// its own, with a block of zeros as the other half (MMAs do not bound this).  Eight warps fill the ring with
 // 16-byte cp.async of rows that a list names, one warp issues the MMAs; for fp16 two warps between them bring the rows' powers of two into the rank
 // values.  (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between the copies and themselves, waits for all that
 // its own thread has in flight: 86 us instead of 76.)  Bound by the rows of x and the rank values, which every 256 columns read again: 8192 tokens of 2 adapters, 14336
 // columns, rank 64, bf16: 352 MB in 76 us, on the 112 SMs that there are CTAs for.  (mma.sync: 129 us.  Sixteen copying warps: the same, and 2 us more to begin.)
-constexpr int OU_STAGES = 8, OU_A = 2 * OUTER_STEP * 128, OU_B = 4 * OUTER_STEP * 128, OU_STAGE = OU_A + OU_B, OU_THREADS = 352,
-              OU_SMEM = OU_STAGES * OU_STAGE + 1024, OU_LIST = 1024, OU_WINDOW = 512;
-static_assert(64 * SUM_ROW * 4 <= OU_STAGES * OU_STAGE, "the sums take the ring's place");
+constexpr int OU_THREADS = 352, OU_LIST = 1024, OU_WINDOW = 512;
+template <typename T> struct OuterUmma {
+    static constexpr int BLOCK = OUTER_STEP * 128, A = PARTS<T> * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 7;
+    static constexpr int ZEROS = STAGES * STAGE, SMEM = ZEROS + (PARTS<T> == 3 ? BLOCK : 0) + 1024;
+    static_assert(64 * SUM_ROW * 4 <= ZEROS, "the sums take the ring's place");
+};
 template <typename T>
 __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
+    using S = OuterUmma<T>;
     constexpr bool F16 = __is_same(T, __half);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const int rank_blocks = (p.rank + 63) / 64, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * 64;
     const int64_t col0 = (int64_t)blockIdx.x * 256;
     extern __shared__ uint8_t raw_smem[];
-    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [OU_STAGES][values, rests | 4 blocks of columns][tokens][128 B]
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [STAGES][parts of the rank values | 4 blocks of columns][tokens][128 B]; zeros
     float *sums = reinterpret_cast<float *>(smem);                                      // [64][SUM_ROW], at the end
-    __shared__ int list[OU_LIST + OUTER_STEP], s_before[OU_WINDOW], s_count[8], s_end[OU_STAGES], s_abort;
+    __shared__ int list[OU_LIST + OUTER_STEP], s_before[OU_WINDOW], s_count[8], s_end[S::STAGES], s_abort;
     __shared__ uint32_t s_bits[OU_WINDOW], s_tmem;
-    __shared__ float s_back[F16 ? OU_LIST : 1], s_big[8], s_scale[F16 ? OU_STAGES : 1][OUTER_STEP];
-    __shared__ __align__(8) uint64_t full[OU_STAGES], scaled[OU_STAGES], empty[OU_STAGES], done;
+    __shared__ float s_back[F16 ? OU_LIST : 1], s_big[8], s_scale[F16 ? S::STAGES : 1][OUTER_STEP];
+    __shared__ __align__(8) uint64_t full[S::STAGES], scaled[S::STAGES], empty[S::STAGES], done;
     volatile int *abort_flag = &s_abort;
     const Hidden<T> h(hidden, p.M, p.rank);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < OU_STAGES; ++i) {
+        for (int i = 0; i < S::STAGES; ++i) {
             umma::mbar_init(&full[i], 256 + 8);                  // (copies of each thread, and each warp)
             umma::mbar_init(&scaled[i], 2);
             umma::mbar_init(&empty[i], 1);
@@ -1119,6 +1136,10 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
         umma::mbar_init(&done, 1);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        umma::fence_proxy_async_smem();
+    }
+    if constexpr (PARTS<T> == 3) {
+        for (int i = threadIdx.x; i < S::BLOCK / 16; i += OU_THREADS) reinterpret_cast<uint4 *>(smem + S::ZEROS)[i] = make_uint4(0, 0, 0, 0);
         umma::fence_proxy_async_smem();
     }
     if (warp == 8) umma::tmem_alloc(&s_tmem, 256);
@@ -1137,19 +1158,23 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
         const uint32_t idesc = umma::umma_idesc_f16(256, !F16, true) | 1u << 16;      // (B MN-major as well)
         const uint32_t ring = smem_addr(smem);
         for (;; ++stages) {
-            const int slot = stages % OU_STAGES;
-            if (!__all_sync(0xffffffffu, umma::mbar_wait(F16 ? &scaled[slot] : &full[slot], stages / OU_STAGES & 1, abort_flag, 1, &g_adapter_status))) break;
+            const int slot = stages % S::STAGES;
+            if (!__all_sync(0xffffffffu, umma::mbar_wait(F16 ? &scaled[slot] : &full[slot], stages / S::STAGES & 1, abort_flag, 1, &g_adapter_status))) break;
             if (*(volatile int *)&s_end[slot]) {
                 umma::umma_commit(&done);
                 break;
             }
             umma::fence_proxy_async_smem();
             umma::tc_fence_after();
-            const uint32_t at = ring + slot * OU_STAGE;
+            const uint32_t at = ring + slot * S::STAGE;
 #pragma unroll
-            for (int k = 0; k < OUTER_STEP / 16; ++k)
-                umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(at + k * 2048, OUTER_STEP * 128), umma::umma_smem_desc_mn(at + OU_A + k * 2048, OUTER_STEP * 128), idesc,
-                                  (stages | k) != 0 ? 1u : 0u);
+            for (int k = 0; k < OUTER_STEP / 16; ++k) {
+                const uint64_t columns = umma::umma_smem_desc_mn(at + S::A + k * 2048, S::BLOCK);
+                umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(at + k * 2048, S::BLOCK), columns, idesc, (stages | k) != 0 ? 1u : 0u);
+                // (the third part above a block of zeros)
+                if constexpr (PARTS<T> == 3)
+                    umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(at + 2 * S::BLOCK + k * 2048, ring + S::ZEROS - (at + 2 * S::BLOCK)), columns, idesc, 1u);
+            }
             umma::umma_commit(&empty[slot]);
         }
     } else if (warp > 8) {
@@ -1157,15 +1182,15 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
         if (p.behind) pdl_wait();
         if constexpr (F16)
             for (;; ++stages) {
-                const int slot = stages % OU_STAGES;
-                if (!__all_sync(0xffffffffu, umma::mbar_wait(&full[slot], stages / OU_STAGES & 1, abort_flag, 5, &g_adapter_status))) break;
+                const int slot = stages % S::STAGES;
+                if (!__all_sync(0xffffffffu, umma::mbar_wait(&full[slot], stages / S::STAGES & 1, abort_flag, 5, &g_adapter_status))) break;
                 const bool end = *(volatile int *)&s_end[slot];
                 if (!end) {
 #pragma unroll
-                    for (int i = 0; i < OU_A / 16 / 64; ++i) {
+                    for (int i = 0; i < S::A / 16 / 64; ++i) {
                         const int at = (warp - 9) * 32 + lane + i * 64;      // of 16 bytes, eight a row
                         const __half2 scale = __float2half2_rn(s_scale[slot][at / 8 % OUTER_STEP]);
-                        uint4 *own = reinterpret_cast<uint4 *>(smem + slot * OU_STAGE) + at, v = *own;
+                        uint4 *own = reinterpret_cast<uint4 *>(smem + slot * S::STAGE) + at, v = *own;
                         __half2 *y = reinterpret_cast<__half2 *>(&v);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) y[k] = __hmul2(y[k], scale);
@@ -1204,12 +1229,12 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
         }
         f = big * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
 
-        // this thread's pieces: of rows warp, warp + 8, .. of x piece `lane`; of row threadIdx / 8 of the values and of the rests piece threadIdx % 8
+        // this thread's pieces: of rows warp, warp + 8, .. of x piece `lane`; of row threadIdx / 8 of the rank values' parts piece threadIdx % 8
         const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0, token = threadIdx.x / 8, piece = threadIdx.x % 8, h_bytes = rank0 + piece * 8 < p.rank ? 16 : 0;
-        const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0)), *top0 = (const uint8_t *)(h.top + (h_bytes ? rank0 + piece * 8 : 0)),
-                      *rest0 = (const uint8_t *)(h.rest + (h_bytes ? rank0 + piece * 8 : 0));
+        const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0));
+        const T *h0 = h.top + (h_bytes ? rank0 + piece * 8 : 0);
         const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2, ring = smem_addr(smem);
-        const uint32_t x_to = OU_A + lane / 8 * (OUTER_STEP * 128) + warp * 128 + (lane % 8 ^ warp) * 16, h_to = token * 128 + (piece ^ (token & 7)) * 16;
+        const uint32_t x_to = S::A + lane / 8 * (S::BLOCK) + warp * 128 + (lane % 8 ^ warp) * 16, h_to = token * 128 + (piece ^ (token & 7)) * 16;
         bool alive = true;                                       // (after a failed wait the loops go on without copies: the warps meet in them)
         int window = 0, passed = 0;
         for (int from = lo, n; from < hi; from += n) {
@@ -1230,10 +1255,10 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
             }
             const int count = (n + OUTER_STEP - 1) / OUTER_STEP;
             for (int i = 0; i < count; ++i, ++stages) {
-                const int slot = stages % OU_STAGES, first = i * OUTER_STEP;
-                alive = alive && umma::mbar_wait(&empty[slot], (stages / OU_STAGES & 1) ^ 1, abort_flag, 2, &g_adapter_status);
+                const int slot = stages % S::STAGES, first = i * OUTER_STEP;
+                alive = alive && umma::mbar_wait(&empty[slot], (stages / S::STAGES & 1) ^ 1, abort_flag, 2, &g_adapter_status);
                 if (alive) {
-                    const uint32_t to = ring + slot * OU_STAGE;
+                    const uint32_t to = ring + slot * S::STAGE;
 #pragma unroll
                     for (int j = 0; j < OUTER_STEP / 8; ++j) {
                         const int at = first + warp + 8 * j;
@@ -1241,8 +1266,9 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
                     }
                     const int at = first + token;
                     const uint64_t row = at < n ? (uint64_t)(uint32_t)list[at] * h_row : 0;
-                    copy16(to + h_to, top0 + row, at < n ? h_bytes : 0);
-                    copy16(to + h_to + OUTER_STEP * 128, rest0 + row, at < n ? h_bytes : 0);
+#pragma unroll
+                    for (int part = 0; part < PARTS<T>; ++part)
+                        copy16(to + h_to + part * S::BLOCK, (const uint8_t *)(h0 + part * h.size) + row, at < n ? h_bytes : 0);
                     if constexpr (F16)
                         if (piece == 0) s_scale[slot][token] = at < n ? s_back[at] : 0.0f;
                     copies_arrive(&full[slot]);
@@ -1252,8 +1278,8 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
             }
         }
         // one more stage, without tokens: the end
-        const int slot = stages % OU_STAGES;
-        alive = alive && umma::mbar_wait(&empty[slot], (stages / OU_STAGES & 1) ^ 1, abort_flag, 3, &g_adapter_status);
+        const int slot = stages % S::STAGES;
+        alive = alive && umma::mbar_wait(&empty[slot], (stages / S::STAGES & 1) ^ 1, abort_flag, 3, &g_adapter_status);
         if (threadIdx.x == 0) *(volatile int *)&s_end[slot] = 1;
         if (alive) copies_arrive(&full[slot]);
         __syncwarp();
@@ -1407,7 +1433,7 @@ int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStre
 
 template <typename T, int KS>
 int expand_umma(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaStream_t st) {
-    using S = ExpandShape<KS>;
+    using S = ExpandShape<KS, PARTS<T>>;
     p.slots = p.adapters + 1 < 2 ? p.adapters + 1 : 2;
     int per_sm = 0;
     const int rc = ctas_per_sm<adapter_expand_umma_kernel<T, KS>>(EU_THREADS, S::SMEM, per_sm);
@@ -1450,7 +1476,7 @@ int expand(void *h, const void *w, const AdapterArgs &p, const void *base, void 
 
 template <typename T, int RB, int RG>
 int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
-    using S = OuterShape<RB, RG>;
+    using S = OuterShape<RB, RG, PARTS<T>>;
     const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + S::RANKS - 1) / S::RANKS), most = (p.M + 2 * OUTER_STEP - 1) / (2 * OUTER_STEP);
     int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_kernel<T, RB, RG>>(S::THREADS, S::SMEM, per_sm);
     if (rc == BW_OK) rc = cluster_parts<adapter_outer_kernel<T, RB, RG>>(blocks * rows, most, 0.12, S::THREADS, S::SMEM, parts);
@@ -1460,11 +1486,11 @@ int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st
 template <typename T>
 int outer_umma(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
     const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 63) / 64), most = (p.M + 4 * OUTER_STEP - 1) / (4 * OUTER_STEP);
-    int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_umma_kernel<T>>(OU_THREADS, OU_SMEM, per_sm);
+    int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_umma_kernel<T>>(OU_THREADS, OuterUmma<T>::SMEM, per_sm);
     // (a part's start and end take as long as about 384 of its tokens)
-    if (rc == BW_OK) rc = cluster_parts<adapter_outer_umma_kernel<T>>(blocks * rows, most, 384.0 * p.adapters / p.M, OU_THREADS, OU_SMEM, parts);
+    if (rc == BW_OK) rc = cluster_parts<adapter_outer_umma_kernel<T>>(blocks * rows, most, 384.0 * p.adapters / p.M, OU_THREADS, OuterUmma<T>::SMEM, parts);
     if (rc != BW_OK) return rc;
-    return launch_early("adapter_outer_umma_kernel", adapter_outer_umma_kernel<T>, dim3((unsigned)blocks, (unsigned)rows, parts), OU_THREADS, OU_SMEM, st, dim3(1, 1, parts), h, x, p, dw);
+    return launch_early("adapter_outer_umma_kernel", adapter_outer_umma_kernel<T>, dim3((unsigned)blocks, (unsigned)rows, parts), OU_THREADS, OuterUmma<T>::SMEM, st, dim3(1, 1, parts), h, x, p, dw);
 }
 template <typename T>
 int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
@@ -1528,8 +1554,8 @@ int backward(const void *dy, const void *x, int64_t M, int64_t N, int64_t K, con
 
 }  // namespace
 
-// (two 16-bit parts and a power of two a row; the general kernels' fp32 values are less)
-size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * 4 + (size_t)M * 4; }
+// (three 16-bit parts, or two and a power of two a row; the general kernels' fp32 values are less)
+size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * 6 + (size_t)M * 4; }
 
 int adapter_device_status() {
     int v = 0, zero = 0;

@@ -1,0 +1,78 @@
+"""Rank values of the adapters are held as exactly as fp32 sums are, whatever their range and the result's type."""
+import pytest
+import torch
+
+from bitween_b200 import adapter_matmul
+from bitween_b200.kernels import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _rand(shape, seed):
+    return 0.5 + torch.rand(shape, generator=_gen(seed), device=DEV)
+
+
+def _outside(got, want, slack):
+    """How many values are not a value within `slack` of `want` rounded once (rounding keeps order)."""
+    return int((~((got >= (want - slack).to(got.dtype)) & (got <= (want + slack).to(got.dtype)))).sum())
+
+
+# A result that is ONE product of a rank value, of positive numbers: fp32 sums of 64 products (4 blocks truncated at 2^-23 of the sum, in parts that are added up: 2^-20.5),
+# the factor and the product's parts (2^-22 in all).  (A rank value of 16 bits is off by up to 2^-17.)
+ONE_PRODUCT = 2.0 ** -19.5
+
+
+@pytest.mark.parametrize("M,n,r,N", [(40, 3, 8, 4096), (300, 3, 16, 1024), (300, 2, 32, 1024), (700, 1, 64, 256), (2100, 1, 64, 8200), (2100, 1, 128, 8200), (700, 9, 128, 256), (61, 24, 4, 512)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_results_hold_more_than_sixteen_bits_of_a_rank_value(M, n, r, N, dtype):
+    """y and dx, in which one rank of each adapter is not zero."""
+    K = 64
+    index = torch.randint(0, n, (M,), generator=_gen(1), device=DEV).sort().values.to(torch.int32)
+    x, down, up, grad = (_rand(s, i + 2).to(dtype) for i, s in enumerate(((M, K), (n, r, K), (n, r, N), (M, N))))
+    keep = torch.arange(r, device=DEV) == r - 3
+    up = torch.where(keep[:, None], up, 0)
+    y = adapter_matmul(x, down, up, index)
+    h = torch.einsum("tk,trk->tr", x.double(), down.double()[index.long()])
+    want = h[:, r - 3, None] * up.double()[index.long(), r - 3]
+    bad = _outside(y, want, ONE_PRODUCT * want)
+    assert bad == 0, f"{bad} of {want.numel()}"
+    # backward, with the sides of the bank exchanged: dh is a sum of 64 products
+    x2 = grad.clone().requires_grad_()
+    y2 = adapter_matmul(x2, up, down, index)
+    (dx,) = torch.autograd.grad(y2, (x2,), x)
+    bad = _outside(dx, want, ONE_PRODUCT * want)
+    assert bad == 0, f"{bad} of {want.numel()}"
+    assert _lib.lib().bw_device_status() == 0
+
+
+@pytest.mark.parametrize("M,n,r,N", [(40, 2, 8, 1024), (100, 1, 16, 2048), (100, 3, 32, 2048), (100, 1, 64, 1024), (700, 1, 64, 2048), (2100, 1, 32, 2048), (700, 1, 128, 1032), (40, 1, 5, 256)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gradients_of_banks_hold_more_than_sixteen_bits_of_a_rank_value(M, n, r, N, dtype):
+    """d up and d down of one token whose gradient is not zero."""
+    K = 64
+    index = torch.zeros(M, dtype=torch.int32, device=DEV)
+    x, down, up, dy = (_rand(s, i + 12).to(dtype) for i, s in enumerate(((M, K), (n, r, K), (n, r, N), (N,))))
+    t = M // 2 + 1
+    grad = torch.zeros(M, N, dtype=dtype, device=DEV)
+    grad[t] = dy
+    leaf = up.clone().requires_grad_()
+    (dup,) = torch.autograd.grad(adapter_matmul(x, down, leaf, index), (leaf,), grad)
+    want = (x[t].double() @ down[0].double().T)[:, None] * dy.double()
+    bad = _outside(dup[0], want, ONE_PRODUCT * want)
+    assert bad == 0, f"{bad} of {want.numel()}"
+    assert bool((dup[1:] == 0).all())
+    # d down: dh of 64 products, x of N columns
+    wide = torch.zeros(M, N, dtype=dtype, device=DEV)
+    wide[t] = dy
+    leaf = up.clone().requires_grad_()
+    g2 = torch.zeros(M, K, dtype=dtype, device=DEV)
+    g2[t] = x[t]
+    (ddown,) = torch.autograd.grad(adapter_matmul(wide, leaf, down, index), (leaf,), g2)
+    bad = _outside(ddown[0], want, ONE_PRODUCT * want)
+    assert bad == 0, f"{bad} of {want.numel()}"
+    assert _lib.lib().bw_device_status() == 0
