@@ -359,7 +359,8 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
         for (int i = 0; i < STAGES - 1; ++i) copy_step(ring + i * C::STEP);
 
-        // the queries in fp16: as they are, or (bf16) divided by a power of two near their largest value, which the scores get back
+        // the queries in fp16: as they are, or (bf16) times the power of two that takes their largest value to 2^14 and more, which the scores get back: elements down
+        // to 2^-30 of it keep all their bits, and below that what is lost is less than 2^-39 of it
         for (int h = warp; h < HEADS; h += WARPS) {
             float v[DIM / 32], big = 0.0f, sum = 0.0f;
 #pragma unroll
@@ -370,9 +371,9 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
             float back = 1.0f;
             if constexpr (__is_same(T, __nv_bfloat16)) {
                 for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-                const int e = min(max((int)(__float_as_uint(big) >> 23), 2), 252);       // (a zero or infinite row: any power; infinities stay what they are)
-                back = __uint_as_float(e << 23);
-                const float by = __uint_as_float((254 - e) << 23);
+                const int e = min(max((int)(__float_as_uint(big) >> 23), 16), 254);      // (a zero or infinite row: any power; infinities stay what they are)
+                back = __uint_as_float((e - 14) << 23);
+                const float by = __uint_as_float((268 - e) << 23);
 #pragma unroll
                 for (int i = 0; i < DIM / 32; ++i) v[i] *= by;
             }

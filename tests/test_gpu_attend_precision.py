@@ -56,3 +56,28 @@ def test_weights_keep_more_bits_than_the_result(heads, kv_heads, dim, bits, leng
     bad = int((~ok).sum())
     assert bad == 0, f"{bad} of {ok.numel()}"
     assert _lib.lib().bw_device_status() == 0
+
+
+@pytest.mark.parametrize("dim,heads", [(64, 2), (128, 8), (256, 2), (128, 16), (80, 2)])
+def test_bf16_queries_of_a_wide_range(dim, heads):
+    """One element 2^22 times the others, where every key is zero: the others keep all their bits.  (Rows that are not negative have a zero point of 0: nothing
+    cancels, and scores have the fp32 errors of the small elements' products alone.)"""
+    batch, n = 8, 40
+    cache = QuantizedKVCache(batch * 3, 16, 1, dim, bits=8, device=DEV)
+    slots = torch.arange(batch * 48, device=DEV)
+    k = torch.rand(batch * 48, 1, dim, generator=_gen(11), device=DEV)
+    k[..., 0] = 0
+    cache.append(k, torch.randn(k.shape, generator=_gen(12), device=DEV), slots)
+    q = torch.randn(batch, heads, dim, generator=_gen(13), device=DEV) * 2.0 ** -12
+    q[..., 0] = 2.0 ** 10
+    q = q.bfloat16()
+    table = torch.arange(batch * 3, dtype=torch.int32, device=DEV).view(batch, 3)
+    alpha = 2.0 ** 12 * dim ** -0.5
+    got = cache.attend(q, table, torch.full((batch,), n, dtype=torch.int32, device=DEV), softmax_scale=alpha)
+    kd, vd = (x.double().view(batch, 48, dim)[:, :n] for x in cache.read(slots, dtype=torch.float32))
+    w = torch.softmax(torch.einsum("bhd,btd->bht", q.double(), kd) * alpha, -1)
+    want, size = torch.einsum("bht,btd->bhd", w, vd), torch.einsum("bht,btd->bhd", w, vd.abs())
+    # scores of sums of up to 256 products of about 1/2, 2^-23 of their absolute sum (up to 14) a block of 16: 2^-15; twice, for numerator and denominator
+    ok = _between(got, want, 2.0 ** -14 * size)
+    bad = int((~ok).sum())
+    assert bad == 0, f"{bad} of {ok.numel()}"
