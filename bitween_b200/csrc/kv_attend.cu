@@ -111,7 +111,9 @@ int attend_general(const AttendArgs &p, int64_t batch, int bits, cudaStream_t st
 //            higher bits of their byte (`planes`) are larger by a power of two and get accumulators of their own.  Scale and zero point
 //            are applied to the sums, in fp32: nothing is rounded.
 //   weights  p = 2^(x - m); p * (value's scale) goes to fp16 for the second product.  m covers p * scale, so that this stays in fp16's
-//            range whatever the scales are; it moves only when some p * scale leaves [0, 1024] (one vote a step).  The
+//            range whatever the scales are; it moves only when some p * scale is about to leave that range (one vote a step), and then the largest of the step becomes 2^12: a
+//            weight counts to within 2^-37 of the largest.  (With 1 at the top weights below 2^-25 of it left the numerator and stayed in the sum of weights: many of them
+//            beside a token that dominates were lost.)  The
 //            rest p - fp16(p) is multiplied as well: 22 bits of a weight count, for bf16 results too (without, they were off by up to 2^-12 of sum w |v|,
 //            an eighth of their own rounding).
 //   values   O[d][h] += (code - zero_t)[d][t] * p[t][h]: 1024 + code by one OR, minus (1024 + zero), exact.  ldmatrix.trans puts
@@ -495,13 +497,13 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
                     for (int e = 0; e < 4; ++e) {
                         pw[nb][e] = live[e / 2] ? ex2(u[nb][e] - m[nb][e % 2]) : 0.0f;
                         pv[nb][e] = pw[nb][e] * vs[e / 2];
-                        over |= pw[nb][e] > 0x1p40f || pv[nb][e] > 1024.0f;
+                        over |= pw[nb][e] > 0x1p40f || pv[nb][e] > 65000.0f;
                     }
             };
             weights();
             if (__any_sync(0xffffffffu, over)) {
-                // the maximum moves: the largest p * scale of this step becomes 1
-                const float lv[2] = {fmaxf(__log2f(vs[0]), -40.0f), fmaxf(__log2f(vs[1]), -40.0f)};
+                // the maximum moves: the largest p * scale of this step becomes 2^12 (scales are 2^-24 at least; of rows that are zero p stays below 2^40)
+                const float lv[2] = {fmaxf(__log2f(vs[0]), -27.0f) - 12.0f, fmaxf(__log2f(vs[1]), -27.0f) - 12.0f};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll

@@ -81,3 +81,33 @@ def test_bf16_queries_of_a_wide_range(dim, heads):
     ok = _between(got, want, 2.0 ** -14 * size)
     bad = int((~ok).sum())
     assert bad == 0, f"{bad} of {ok.numel()}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("below", [25.5, 28.5])
+def test_many_tokens_far_below_one_that_dominates(dtype, below):
+    """4095 tokens at 2^-25.5 of a dominant one: they are all of the result where the dominant token's value is zero.  64 sequences of the same pages, so that a
+    warp has some hundred of the tokens beside the dominant one."""
+    n, dim, batch, kv_heads = 4096, 64, 64, 8
+    cache = QuantizedKVCache(n // 16, 16, kv_heads, dim, bits=8, device=DEV)
+    k, v = torch.zeros(n, kv_heads, dim, device=DEV), torch.ones(n, kv_heads, dim, device=DEV)
+    v[..., 0] = 0
+    for h in range(kv_heads):
+        k[500 * h + 77, h, 0] = 1
+        v[500 * h + 77, h] = 0
+        v[500 * h + 77, h, 0] = 1
+    cache.append(k, v, torch.arange(n, device=DEV))
+    kd, vd = (x.double().transpose(0, 1) for x in cache.read(torch.arange(n, device=DEV), dtype=torch.float32))
+    q = torch.zeros(batch, 4 * kv_heads, dim, device=DEV)
+    q[..., 0] = 1
+    alpha = below * 0.6931471805599453 / float(kd.amax())
+    table = torch.arange(n // 16, dtype=torch.int32, device=DEV)[None].expand(batch, -1)
+    got = cache.attend(q.to(dtype), table, torch.full((batch,), n, dtype=torch.int32, device=DEV), softmax_scale=alpha)
+    w = torch.softmax(kd[..., 0] * alpha, -1)[:, None]
+    want, size = ((w @ x).expand(-1, 4, -1).reshape(1, 4 * kv_heads, dim).expand(batch, -1, -1) for x in (vd, vd.abs()))
+    # The largest weight times its scale is 2^12 at least where it is reached, fp16's smallest step 2^-24: a weight counts to within 2^-37 of the largest, 4096 of them to 2^-25;
+    # 2^-17 for the score (30, 2^-24 of it a rounding) and the sums.
+    slack = 2.0 ** -17 * size + 2.0 ** -25
+    ok = _between(got, want, slack + (2.0 ** -25 if dtype == torch.float16 else 0))
+    bad = int((~ok).sum())
+    assert bad == 0, (bad, got[0, 0, :3].tolist(), want[0, 0, :3].tolist())
