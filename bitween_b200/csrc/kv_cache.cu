@@ -180,12 +180,13 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const T *__restrict__ k,
     }
 }
 
-// E values of a row: code + 2^23 by one OR, minus 2^23 + zero, both exact; times the scale, exact as well (19 bits); then the result's rounding.
+// E values of a row: code + 2^23 by one OR, minus 2^23, exact; then scale * code - scale * zero, whose second product is exact (22 bits), in one rounding to fp32
+// (none where the zero point is an integer as append writes it: 19 bits); then the result's rounding.
 template <typename T, int BITS, bool VEC>
 __device__ __forceinline__ void read_piece(const int32_t *codes, uint32_t constants, int lane, int words, int dim, T *dst) {
     constexpr int WORDS = E * BITS / 32, VPI = 32 / BITS;
     const float2 c = __half22float2(*reinterpret_cast<const __half2 *>(&constants));
-    const float zero = 8388608.0f + c.y;
+    const float zero = -c.x * c.y;
     uint32_t w[WORDS] = {};
     if constexpr (WORDS == 4 && VEC) {
         const uint4 u = __ldcg(reinterpret_cast<const uint4 *>(codes) + lane);
@@ -205,7 +206,7 @@ __device__ __forceinline__ void read_piece(const int32_t *codes, uint32_t consta
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const uint32_t code = w[i / VPI] >> (i % VPI * BITS) & ((1u << BITS) - 1);
-        out[i] = from_f32<T>(c.x * (__uint_as_float(0x4B000000u | code) - zero));
+        out[i] = from_f32<T>(__fmaf_rn(c.x, __uint_as_float(0x4B000000u | code) - 8388608.0f, zero));
     }
     if constexpr (VEC) {
 #pragma unroll
