@@ -116,7 +116,8 @@ int attend_general(const AttendArgs &p, int64_t batch, int bits, cudaStream_t st
 //            beside a token that dominates were lost.)  The
 //            rest p - fp16(p) is multiplied as well: 22 bits of a weight count, for bf16 results too (without, they were off by up to 2^-12 of sum w |v|,
 //            an eighth of their own rounding).
-//   values   O[d][h] += (code - zero_t)[d][t] * p[t][h]: 1024 + code by one OR, minus (1024 + zero), exact.  ldmatrix.trans puts
+//   values   O[d][h] += (code - zero_t)[d][t] * p[t][h]: 1024 + code by one OR, minus (1024 + the zero point's nearest code), exact.  What the zero point is off that code
+//            (nothing where append wrote it) is the same for all d: sum_t p * (nearest code - zero_t), in fp32 beside the sum of weights, is added at the end.  ldmatrix.trans puts
 //            16 bits (2 to 8 codes) of two tokens beside each other, as the operand wants them.
 // Groups of up to 4 heads fill half of the eight columns: their steps are two tiles, whose scores share one set of registers (columns 0 to 3
 // the first tile's, 4 to 7 the second's), which halves the work on weights; the columns' sums meet at the end, and where one tile's values are
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 
         uint32_t magic;                                       // 1024 in both halves
         asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
-        float o[NB][S::MMAS][4] = {}, m[NB][2], l[NB][2] = {};
+        float o[NB][S::MMAS][4] = {}, m[NB][2], l[NB][2] = {}, off[NB][2] = {};
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) m[nb][0] = m[nb][1] = -INFINITY;
         const int half_tile = PAIR == 2 ? c / 2 : 0;         // the tile whose scores this lane's columns are
@@ -463,7 +464,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
                         for (int e = 0; e < 4; ++e) acc[nb][pl][e] = i == 0 || half_tile == 1 ? sum[nb][pl][e] : acc[nb][pl][e];
             }
             const int t0 = (now * PAIR + half_tile) * TILE + r;
-            float ks[2], kz[2], vs[2];
+            float ks[2], kz[2], vs[2], vr[2];
             uint32_t vz[2];
             bool live[2];
 #pragma unroll
@@ -475,8 +476,10 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
                 ks[j] = kc.x;
                 kz[j] = kc.y;
                 const __half2 vc = as_half2(constants[1]);
+                const __half2 z = __high2half2(vc), code = __hmin2(__hmax2(h2rint(z), __float2half2_rn(0.0f)), __float2half2_rn((float)((1 << BITS) - 1)));
                 vs[j] = live[j] ? __low2float(vc) : 0.0f;
-                vz[j] = live[j] ? as_u32(__high2half2(vc)) : 0u;
+                vr[j] = live[j] ? __low2float(code) - __low2float(z) : 0.0f;
+                vz[j] = live[j] ? as_u32(code) : 0u;
             }
             float u[NB][4];                           // [j * 2 + column]
 #pragma unroll
@@ -516,6 +519,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
                         const float keep = m[nb][j] == -INFINITY ? 0.0f : ex2(m[nb][j] - top);
                         m[nb][j] = top;
                         l[nb][j] *= keep;
+                        off[nb][j] *= keep;
 #pragma unroll
                         for (int i = 0; i < S::MMAS; ++i) {
                             o[nb][i][j] *= keep;
@@ -531,6 +535,8 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
                 for (int j = 0; j < 2; ++j) {
                     l[nb][0] += pw[nb][2 * j];
                     l[nb][1] += pw[nb][2 * j + 1];
+                    off[nb][0] = fmaf(pv[nb][2 * j], vr[j], off[nb][0]);
+                    off[nb][1] = fmaf(pv[nb][2 * j + 1], vr[j], off[nb][1]);
                     const __half2 top = __floats2half2_rn(pv[nb][2 * j], pv[nb][2 * j + 1]);
                     const float2 t = __half22float2(top);
                     w[nb][j][0] = transpose8x8(as_u32(top));
@@ -595,7 +601,10 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                for (int d = 4; d < 32; d *= 2) l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], d);
+                for (int d = 4; d < 32; d *= 2) {
+                    l[nb][j] += __shfl_xor_sync(0xffffffffu, l[nb][j], d);
+                    off[nb][j] += __shfl_xor_sync(0xffffffffu, off[nb][j], d);
+                }
                 if (r == 0) {
                     s_m[warp][nb * 8 + 2 * c + j] = m[nb][j];
                     s_l[warp][nb * 8 + 2 * c + j] = bad ? NAN : l[nb][j];
@@ -616,7 +625,7 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const int pl = i % S::PLANES, d = (i / S::PLANES * 8 + r) * (16 / BITS) + pl + k * S::PLANES;
-                        s_o[(warp * COLS + col) * S::STRIDE + d] = o[nb][i][2 * k + j] * (by / (1 << (pl * BITS)));
+                        s_o[(warp * COLS + col) * S::STRIDE + d] = fmaf(o[nb][i][2 * k + j], by / (1 << (pl * BITS)), off[nb][j] * by);
                     }
             }
         if (threadIdx.x < heads) {
