@@ -500,13 +500,13 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
                     for (int e = 0; e < 4; ++e) {
                         pw[nb][e] = live[e / 2] ? ex2(u[nb][e] - m[nb][e % 2]) : 0.0f;
                         pv[nb][e] = pw[nb][e] * vs[e / 2];
-                        over |= pw[nb][e] > 0x1p40f || pv[nb][e] > 65000.0f;
+                        over |= pw[nb][e] > 0x1p40f || fabsf(pv[nb][e]) > 65000.0f;      // (scales may be negative)
                     }
             };
             weights();
             if (__any_sync(0xffffffffu, over)) {
                 // the maximum moves: the largest p * scale of this step becomes 2^12 (scales are 2^-24 at least; of rows that are zero p stays below 2^40)
-                const float lv[2] = {fmaxf(__log2f(vs[0]), -27.0f) - 12.0f, fmaxf(__log2f(vs[1]), -27.0f) - 12.0f};
+                const float lv[2] = {fmaxf(__log2f(fabsf(vs[0])), -27.0f) - 12.0f, fmaxf(__log2f(fabsf(vs[1])), -27.0f) - 12.0f};
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll

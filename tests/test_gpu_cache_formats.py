@@ -46,7 +46,7 @@ def test_read_gives_what_a_row_stands_for(zeros, bits, dim):
             assert torch.equal(got, want[slots].float().to(dtype))
 
 
-@pytest.mark.parametrize("zeros", [z for z in ZEROS if z != "signs"])
+@pytest.mark.parametrize("zeros", ZEROS)
 @pytest.mark.parametrize("bits", [2, 4, 8])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,lengths", [
     (8, 2, 128, 16, [300, 1, 40, 0, 17]), (6, 1, 64, 32, [300, 55]), (16, 1, 128, 16, [100, 31]), (4, 2, 256, 16, [200, 3]),
