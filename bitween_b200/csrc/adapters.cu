@@ -12,7 +12,7 @@
 //   * where it runs over rows (expand over ranks, outer over tokens), a lane takes 16 bytes of four rows, eight columns of its own, and
 //     pairs the rows by byte permutations: MMA j of eight has column j of every lane.  A lane's results are then 16 neighbours of a row.
 // Rank values are summed in 32 bits and kept in 16-bit parts (value and rests: three of bf16, two of fp16), which hold 24 (bf16) or 22 (fp16) of their bits and are
-// what the second product takes.  (Two of bf16 hold 16: results of bf16 were off by up to 2^-17 more than their own rounding.)  fp16 parts are of h * 2^-e, e of the row's largest: gradients without loss scaling would be lost below
+// what the second product takes.  (Two of bf16 hold 16: results of bf16 were off by up to 2^-17 more than their own rounding.)  fp16 parts are of h * 2^(14 - e), e of the row's largest: gradients without loss scaling would be lost below
 // 2^-14, and large rank values beyond 65504.
 //
 // Tokens of one adapter need not be neighbours: a tile of 64 tokens goes through the adapters that occur in it, one after the other or (few
@@ -219,8 +219,9 @@ __device__ __forceinline__ void finish_rows(float *sums, int rows, int row0, int
         if constexpr (F16) {
             for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
             const int e = exponent_of(big);
-            by = power_of_two(-e);
-            if (lane == 0) h.back[t] = power_of_two(e);
+            // (the largest to 2^14 and more: a rank has 22 bits down to 2^-16 of it, and what is lost below is less than 2^-39 of it)
+            by = power_of_two(14 - e);
+            if (lane == 0) h.back[t] = power_of_two(e - 14);
         }
 #pragma unroll
         for (int i = 0; i < PAIRS; ++i) {

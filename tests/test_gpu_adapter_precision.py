@@ -76,3 +76,33 @@ def test_gradients_of_banks_hold_more_than_sixteen_bits_of_a_rank_value(M, n, r,
     bad = _outside(ddown[0], want, ONE_PRODUCT * want)
     assert bad == 0, f"{bad} of {want.numel()}"
     assert _lib.lib().bw_device_status() == 0
+
+
+def _check(got, want, size):
+    """The bound of test_gpu_adapters.py: within 2^-12 of the absolute products, rounded once."""
+    slack = 2.0 ** -12 * size + (2.0 ** -24 if got.dtype == torch.float16 else 1e-30)
+    bad = _outside(got, want, slack)
+    assert bad == 0, f"{bad} of {want.numel()}"
+
+
+@pytest.mark.parametrize("M,r,N", [(40, 16, 512), (300, 32, 512), (1100, 64, 1024), (1100, 64, 8200), (300, 64, 256)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_ranks_of_very_different_sizes(M, r, N, dtype):
+    """Ranks down to 2^-20 of the largest: each one's gradient, and a y in which small rows of `down` meet large rows of `up`."""
+    K = 128
+    index = torch.zeros(M, dtype=torch.int32, device=DEV)
+    size = 2.0 ** (-20.0 * torch.arange(r, device=DEV) / (r - 1))
+    x = (torch.randn(M, K, generator=_gen(21), device=DEV) * 256).to(dtype)
+    down = (torch.randn(1, r, K, generator=_gen(22), device=DEV) * size[:, None] * 4).to(dtype)
+    up = (torch.randn(1, r, N, generator=_gen(23), device=DEV) / size[:, None] * 2.0 ** -9).to(dtype)
+    grad = (torch.randn(M, N, generator=_gen(24), device=DEV) * 2.0 ** -4).to(dtype)
+    leaves = [t.requires_grad_() for t in (x, down, up)]
+    y = adapter_matmul(*leaves, index)
+    dx, ddown, dup = torch.autograd.grad(y, leaves, grad)
+    xd, dd, ud, gd = (t.detach().double() for t in (x, down[0], up[0], grad))
+    h, ha = xd @ dd.T, xd.abs() @ dd.T.abs()
+    dh, dha = gd @ ud.T, gd.abs() @ ud.T.abs()
+    _check(y.detach(), h @ ud, ha @ ud.abs())
+    _check(dup[0], h.T @ gd, ha.T @ gd.abs())
+    _check(dx, dh @ dd, dha @ dd.abs())
+    _check(ddown[0], dh.T @ xd, dha.T @ xd.abs())
