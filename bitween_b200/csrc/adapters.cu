@@ -974,7 +974,8 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     for (int rb = 0; rb < RB; ++rb)
         h_place[rb] = OUTER_STEP * 512 + (lane % 8 + lane / 16 * 8) * S::ROW + (((wr * RB + rb) * 2 + lane / 8 % 2) ^ S::swizzle(lane % 8)) * 16;
     float acc[RB][8][4] = {};
-    float big = 0.0f;                                            // fp16: the sums are of h / big, the largest power of two of a row so far
+    float big = 0.0f;                                            // fp16: the sums are of h / big, the largest power of two of a row so far: what is lost of a row is less
+                                                                 // than 2^-38 of the largest one's values
     int window = 0, passed = 0;                                  // the marked window's first word, and the adapter's tokens in front of it
     for (int from = lo, n; from < hi; from += n) {
         while (passed + in_window <= from && window + OUTER_WINDOW < words) {
@@ -1051,12 +1052,14 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                     b[j][0] = column_pair(raw[0], raw[1], j);
                     b[j][1] = column_pair(raw[2], raw[3], j);
                 }
-                __half2 scale[2];
+                __half2 scale[2], more[2];                      // (as two factors: powers below 2^-24 as well)
                 if constexpr (F16) {
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const int i = first + step * 16 + 2 * c + 8 * k;
-                        scale[k] = __floats2half2_rn(i < n ? s_back[i] : 0.0f, i + 1 < n ? s_back[i + 1] : 0.0f);
+                        const float f0 = i < n ? s_back[i] : 0.0f, f1 = i + 1 < n ? s_back[i + 1] : 0.0f;
+                        scale[k] = __floats2half2_rn(fmaxf(f0, 0x1p-24f), fmaxf(f1, 0x1p-24f));
+                        more[k] = __floats2half2_rn(fminf(f0 * 0x1p24f, 1.0f), fminf(f1 * 0x1p24f, 1.0f));
                     }
                 }
 #pragma unroll
@@ -1068,7 +1071,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                         if constexpr (F16) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                const __half2 y = __hmul2(*reinterpret_cast<const __half2 *>(&ha[k]), scale[k / 2]);
+                                const __half2 y = __hmul2(__hmul2(*reinterpret_cast<const __half2 *>(&ha[k]), scale[k / 2]), more[k / 2]);
                                 ha[k] = *reinterpret_cast<const uint32_t *>(&y);
                             }
                         }
@@ -1190,11 +1193,12 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
 #pragma unroll
                     for (int i = 0; i < S::A / 16 / 64; ++i) {
                         const int at = (warp - 9) * 32 + lane + i * 64;      // of 16 bytes, eight a row
-                        const __half2 scale = __float2half2_rn(s_scale[slot][at / 8 % OUTER_STEP]);
+                        const float f = s_scale[slot][at / 8 % OUTER_STEP];
+                        const __half2 scale = __float2half2_rn(fmaxf(f, 0x1p-24f)), more = __float2half2_rn(fminf(f * 0x1p24f, 1.0f));      // (powers below 2^-24 as well)
                         uint4 *own = reinterpret_cast<uint4 *>(smem + slot * S::STAGE) + at, v = *own;
                         __half2 *y = reinterpret_cast<__half2 *>(&v);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) y[k] = __hmul2(y[k], scale);
+                        for (int k = 0; k < 4; ++k) y[k] = __hmul2(__hmul2(y[k], scale), more);
                         *own = v;
                     }
                     umma::fence_proxy_async_smem();

@@ -78,9 +78,9 @@ def test_gradients_of_banks_hold_more_than_sixteen_bits_of_a_rank_value(M, n, r,
     assert _lib.lib().bw_device_status() == 0
 
 
-def _check(got, want, size):
+def _check(got, want, size, more=0.0):
     """The bound of test_gpu_adapters.py: within 2^-12 of the absolute products, rounded once."""
-    slack = 2.0 ** -12 * size + (2.0 ** -24 if got.dtype == torch.float16 else 1e-30)
+    slack = 2.0 ** -12 * size + (2.0 ** -24 if got.dtype == torch.float16 else 1e-30) + more
     bad = _outside(got, want, slack)
     assert bad == 0, f"{bad} of {want.numel()}"
 
@@ -106,3 +106,36 @@ def test_ranks_of_very_different_sizes(M, r, N, dtype):
     _check(dup[0], h.T @ gd, ha.T @ gd.abs())
     _check(dx, dh @ dd, dha @ dd.abs())
     _check(ddown[0], dh.T @ xd, dha.T @ xd.abs())
+
+
+@pytest.mark.parametrize("M,r,N", [(64, 16, 512), (300, 32, 512), (300, 64, 256), (1100, 64, 1024), (2100, 32, 1024)])
+@pytest.mark.parametrize("below", [10, 16, 22, 30])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tokens_whose_gradients_are_far_below_the_largest(M, r, N, below, dtype):
+    """Columns of x in which only tokens with small gradients are not zero: their sums keep their precision.
+
+    fp16 rank values enter these sums as multiples of one power of two, by which the largest row's largest lies in [2^14, 2^15): value and rest are each rounded by at most
+    2^-25 there, which is 2^-24 of 2^14 for both, 2^-38 of the largest.  That much of it, times the absolute sum of the other operand's column, is allowed as well (at 2^-30 it is
+    seen: 2^-8 of a small row; sums in fp32 that hold the large rows would be off by 2^-24 of them)."""
+    K = 64
+    index = torch.zeros(M, dtype=torch.int32, device=DEV)
+    small = torch.arange(M, device=DEV) % 2 == 1
+    x = torch.randn(M, N, generator=_gen(31), device=DEV)
+    x[~small, ::2] = 0
+    x = (x * 256).to(dtype)
+    # (two factors: a gradient of 2^-30 is nothing in fp16)
+    grad = torch.randn(M, K, generator=_gen(32), device=DEV) * torch.where(small, 2.0 ** -(below // 2), 2.0 ** ((below + 1) // 2))[:, None] * 2.0 ** -4
+    grad = grad.to(dtype)
+    down = (torch.randn(1, r, N, generator=_gen(33), device=DEV) * N ** -0.5).to(dtype).requires_grad_()
+    up = (torch.randn(1, r, K, generator=_gen(34), device=DEV) * 2.0 ** -4).to(dtype).requires_grad_()
+    ddown, dup = torch.autograd.grad(adapter_matmul(x, down, up, index), (down, up), grad)
+    gd, ud, xd, dd = (t.detach().double() for t in (grad, up[0], x, down[0]))
+    dh, dha = gd @ ud.T, gd.abs() @ ud.T.abs()
+    floor = 2.0 ** -38 if dtype == torch.float16 else 0.0
+    _check(ddown[0], dh.T @ xd, dha.T @ xd.abs(), floor * dh.abs().max() * xd.abs().sum(0))
+    # and rank values of tokens far below the largest, beside gradients that only they have
+    x2 = (torch.randn(M, K, generator=_gen(35), device=DEV) * torch.where(small, 2.0 ** -(below // 2), 2.0 ** ((below + 1) // 2))[:, None] * 2.0 ** -4).to(dtype)
+    g2 = x.detach()
+    (dup,) = torch.autograd.grad(adapter_matmul(x2, up.detach(), down, index), (down,), g2)
+    h, ha = x2.double() @ ud.T, x2.double().abs() @ ud.T.abs()
+    _check(dup[0], h.T @ g2.double(), ha.T @ g2.double().abs(), floor * h.abs().max() * g2.double().abs().sum(0))
