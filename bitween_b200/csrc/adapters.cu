@@ -65,9 +65,16 @@ __global__ void __launch_bounds__(256) adapter_outer_general_kernel(const float 
     const int64_t c = (int64_t)blockIdx.y * 256 + threadIdx.x;
     const int a = blockIdx.x / r, j = blockIdx.x % r;
     if (c >= N) return;
-    float s = 0.0f;
-    for (int64_t t = 0; t < M; ++t)
-        if (index[t] == a) s += h[t * r + j] * to_f32(x[t * N + c]);
+    // sums of 64 tokens, added up with the part that the addition rounds off carried along (Kahan): one running fp32 sum of M products could be off by M * 2^-24 of them
+    float s = 0.0f, carry = 0.0f;
+    for (int64_t t0 = 0; t0 < M; t0 += 64) {
+        float block = 0.0f;
+        for (int64_t t = t0; t < M && t < t0 + 64; ++t)
+            if (index[t] == a) block += h[t * r + j] * to_f32(x[t * N + c]);
+        const float y = __fsub_rn(block, carry), next = __fadd_rn(s, y);
+        carry = isfinite(next) ? __fsub_rn(__fsub_rn(next, s), y) : 0.0f;
+        s = next;
+    }
     dw[(int64_t)blockIdx.x * N + c] = from_f32<T>(scaling ? s * scaling[a] : s);
 }
 

@@ -139,3 +139,44 @@ def test_tokens_whose_gradients_are_far_below_the_largest(M, r, N, below, dtype)
     (dup,) = torch.autograd.grad(adapter_matmul(x2, up.detach(), down, index), (down,), g2)
     h, ha = x2.double() @ ud.T, x2.double().abs() @ ud.T.abs()
     _check(dup[0], h.T @ g2.double(), ha.T @ g2.double().abs(), floor * h.abs().max() * g2.double().abs().sum(0))
+
+
+@pytest.mark.parametrize("r", [1, 4, 12])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_long_sums_of_the_general_kernels(r, dtype):
+    """A product of 1 and 2^17 - 1 of 2^-25: one running fp32 sum would stay at 1, off by 2^-8."""
+    M, K, N = 1 << 17, 8, 8
+    index = torch.zeros(M, dtype=torch.int32, device=DEV)
+    x, grad = torch.zeros(M, K, device=DEV), torch.full((M, N), 2.0 ** -13, device=DEV)
+    x[:, 0] = 2.0 ** -12
+    x[0, 0], grad[0] = 1, 1
+    down, up = torch.zeros(1, r, K, device=DEV), torch.zeros(1, r, N, device=DEV)
+    down[..., 0] = 1
+    up = up.to(dtype).requires_grad_()
+    (dup,) = torch.autograd.grad(adapter_matmul(x.to(dtype), down.to(dtype), up, index), (up,), grad.to(dtype))
+    want = torch.full(dup.shape, 1 + (M - 1) * 2.0 ** -25, dtype=torch.float64, device=DEV)
+    # blocks of fp32 sums, joined: 2^-20 at most
+    assert _outside(dup, want, 2.0 ** -20 * want) == 0, (dup.flatten()[0], want.flatten()[0])
+
+
+def test_infinities_stay_what_they_are_in_the_general_kernels():
+    M = 200
+    x, grad = torch.ones(M, 8, device=DEV).bfloat16(), torch.ones(M, 8, device=DEV).bfloat16()
+    grad[10, 3], grad[150, 5] = torch.inf, -torch.inf
+    up = torch.zeros(1, 3, 8, device=DEV).bfloat16().requires_grad_()
+    (dup,) = torch.autograd.grad(adapter_matmul(x, torch.ones(1, 3, 8, device=DEV).bfloat16(), up, torch.zeros(M, dtype=torch.int32, device=DEV)), (up,), grad)
+    want = 8.0 * grad.float().sum(0)
+    assert torch.equal(dup[0].float(), want.bfloat16().float().expand(3, -1)) and float(want[3]) == torch.inf
+
+
+def test_gradients_of_many_tokens_and_a_rank_that_is_no_multiple_of_eight():
+    M, K, N, r = 5000, 64, 72, 4
+    x, grad = (torch.randn(M, c, generator=_gen(41 + c), device=DEV).bfloat16() for c in (K, N))
+    down, up = ((torch.randn(2, r, c, generator=_gen(43 + c), device=DEV) / 8).bfloat16().requires_grad_() for c in (K, N))
+    index = torch.randint(-1, 2, (M,), generator=_gen(45), device=DEV).to(torch.int32)
+    got = torch.autograd.grad(adapter_matmul(x, down, up, index), (down, up), grad)
+    for a in range(2):
+        t = index == a
+        xd, gd, dd, ud = x[t].double(), grad[t].double(), down[a].detach().double(), up[a].detach().double()
+        _check(got[0][a], (gd @ ud.T).T @ xd, (gd.abs() @ ud.T.abs()).T @ xd.abs())
+        _check(got[1][a], (xd @ dd.T).T @ gd, (xd.abs() @ dd.T.abs()).T @ gd.abs())
