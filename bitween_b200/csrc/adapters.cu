@@ -11,9 +11,9 @@
 //     lane's 16 bytes of a row serve two MMAs, k pairs (0, 1), (2, 3) and (4, 5), (6, 7);
 //   * where it runs over rows (expand over ranks, outer over tokens), a lane takes 16 bytes of four rows, eight columns of its own, and
 //     pairs the rows by byte permutations: MMA j of eight has column j of every lane.  A lane's results are then 16 neighbours of a row.
-// Rank values are summed in 32 bits and kept in 16-bit parts (value and rests: three of bf16, two of fp16), which hold 24 (bf16) or 22 (fp16) of their bits and are
-// what the second product takes.  (Two of bf16 hold 16: results of bf16 were off by up to 2^-17 more than their own rounding.)  fp16 parts are of h * 2^(14 - e), e of the row's largest: gradients without loss scaling would be lost below
-// 2^-14, and large rank values beyond 65504.
+// Rank values are summed in 32 bits.  The second product takes them in 16-bit parts: value and rests, three of bf16, which hold all 24 bits, two of fp16, which hold 22.
+// (Two of bf16 hold 16: results of bf16 were off by up to 2^-17 more than their own rounding.)  Between the launches bf16 rank values are fp32, split where they are used;
+// fp16 parts are kept as such, of h * 2^(14 - e), e of the row's largest: gradients without loss scaling would be lost below 2^-14, and large rank values beyond 65504.
 //
 // Tokens of one adapter need not be neighbours: a tile of 64 tokens goes through the adapters that occur in it, one after the other or (few
 // tokens, many adapters) a CTA each, with the rows of each gathered; outer gathers the tokens of its adapter from all.  Rows of other
@@ -143,15 +143,39 @@ struct AdapterArgs {
     bool behind;                // another launch of this call comes before: all that came before that is done when this one starts
 };
 
-// Rank values: [parts][M][rank] of 16 bits (the values, their rests, for bf16 the rests of those), and (fp16) [M] powers of two by which all were divided.
+// Rank values.  bf16: fp32 [M][rank].  fp16: [2][M][rank], values and their rests, and [M] powers of two by which both were divided.
 template <typename T> constexpr int PARTS = __is_same(T, __half) ? 2 : 3;
 template <typename T> struct Hidden {
-    T *top;
-    int64_t size;             // of a part
-    float *back;
-    __host__ __device__ Hidden(void *p, int64_t M, int r) : top((T *)p), size(M * r), back(reinterpret_cast<float *>(top + PARTS<T> * size)) {}
-    __device__ __forceinline__ T *part(int i) const { return top + i * size; }
+    float *sum;
+    __host__ __device__ Hidden(void *p, int64_t, int) : sum((float *)p) {}
 };
+template <> struct Hidden<__half> {
+    __half *top, *rest;
+    float *back;
+    __host__ __device__ Hidden(void *p, int64_t M, int r) : top((__half *)p), rest(top + M * r), back(reinterpret_cast<float *>(rest + M * r)) {}
+};
+// Two values as pairs of 16 bits: themselves and rests.
+template <typename T, int N>
+__device__ __forceinline__ void split(float2 v, uint32_t (&parts)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        parts[i] = Pair<T>::pack(v.x, v.y);
+        const float2 f = Pair<T>::unpack(parts[i]);
+        v = make_float2(v.x - f.x, v.y - f.y);
+    }
+}
+// Eight neighbouring fp32 values as 16 bytes of each part.
+template <typename T, int N>
+__device__ __forceinline__ void split8(const float4 &a, const float4 &b, uint4 (&parts)[N]) {
+    const float2 v[4] = {make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t u[N];
+        split<T>(v[i], u);
+#pragma unroll
+        for (int k = 0; k < N; ++k) reinterpret_cast<uint32_t *>(&parts[k])[i] = u[k];
+    }
+}
 
 // The adapters that occur in a tile of tokens, in the order of their first token, each with a list of its tokens (every warp has its own).  Tokens
 // behind the last are in no group.
@@ -198,7 +222,7 @@ struct TileAdapters {
 };
 
 // The end of a shrink pass: the CTAs of a cluster have sums of their part of the columns in `sums` [rows][RANKS + 4]; each CTA adds up its share of
-// the rows, a warp a row, and writes them in 16-bit parts.
+// the rows, a warp a row, and writes them.
 template <typename T, int RANKS>
 __device__ __forceinline__ void finish_rows(float *sums, int rows, int row0, int count, const uint8_t *list, int64_t t0, const AdapterArgs &p, const Hidden<T> &h) {
     constexpr bool F16 = __is_same(T, __half);
@@ -221,27 +245,28 @@ __device__ __forceinline__ void finish_rows(float *sums, int rows, int row0, int
                 }
             big = fmaxf(big, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
         }
-        float by = 1.0f;
         const int64_t t = t0 + list[row0 + row];
         if constexpr (F16) {
             for (int d = 16; d; d >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
             const int e = exponent_of(big);
             // (the largest to 2^14 and more: a rank has 22 bits down to 2^-16 of it, and what is lost below is less than 2^-39 of it)
-            by = power_of_two(14 - e);
+            const float by = power_of_two(14 - e);
             if (lane == 0) h.back[t] = power_of_two(e - 14);
-        }
 #pragma unroll
-        for (int i = 0; i < PAIRS; ++i) {
-            const int j = 2 * (lane + 32 * i);
-            if (j < p.rank) {
-                float2 left = make_float2(v[i].x * by, v[i].y * by);
-#pragma unroll
-                for (int part = 0; part < PARTS<T>; ++part) {
-                    const uint32_t here = Pair<T>::pack(left.x, left.y);
-                    const float2 f = Pair<T>::unpack(here);
-                    *reinterpret_cast<uint32_t *>(h.part(part) + t * p.rank + j) = here;
-                    left = make_float2(left.x - f.x, left.y - f.y);
+            for (int i = 0; i < PAIRS; ++i) {
+                const int j = 2 * (lane + 32 * i);
+                if (j < p.rank) {
+                    uint32_t parts[2];
+                    split<T>(make_float2(v[i].x * by, v[i].y * by), parts);
+                    *reinterpret_cast<uint32_t *>(h.top + t * p.rank + j) = parts[0];
+                    *reinterpret_cast<uint32_t *>(h.rest + t * p.rank + j) = parts[1];
                 }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PAIRS; ++i) {
+                const int j = 2 * (lane + 32 * i);
+                if (j < p.rank) *reinterpret_cast<float2 *>(h.sum + t * p.rank + j) = v[i];
             }
         }
     }
@@ -412,16 +437,26 @@ __device__ __forceinline__ void load_rank_values(const Hidden<T> &h, int rank, i
             const int j = 16 * (first + ks) + 2 * c + e / 2 * 8;
             const bool has = (e % 2 ? has_b : has_a) && j < rank;
             const int64_t at = (e % 2 ? tb : ta) * rank + j;
+            if constexpr (__is_same(T, __half)) {
+                values[0][ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.top + at)) : 0u;
+                values[1][ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.rest + at)) : 0u;
+            } else {
+                uint32_t parts[3];
+                split<T>(has ? __ldcg(reinterpret_cast<const float2 *>(h.sum + at)) : make_float2(0.0f, 0.0f), parts);
 #pragma unroll
-            for (int part = 0; part < PARTS<T>; ++part) values[part][ks][e] = has ? __ldcg(reinterpret_cast<const uint32_t *>(h.part(part) + at)) : 0u;
+                for (int i = 0; i < 3; ++i) values[i][ks][e] = parts[i];
+            }
         }
 }
+// The power of two by which a row's rank values were divided.
+__device__ __forceinline__ float power_of_row(const Hidden<__half> &h, int64_t t) { return __ldcg(h.back + t); }
+__device__ __forceinline__ float power_of_row(const Hidden<__nv_bfloat16> &, int64_t) { return 1.0f; }
 // What a row's product is multiplied by.
 template <typename T>
 __device__ __forceinline__ float row_factor(const Hidden<T> &h, const AdapterArgs &p, int a, int64_t t, bool has) {
     if (a < 0 || !has) return 0.0f;
     if (a >= p.adapters) return NAN;
-    return (__is_same(T, __half) ? __ldcg(h.back + t) : 1.0f) * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
+    return power_of_row(h, t) * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
 }
 // base + f * product, 16 neighbouring columns of two rows; `old` is base (zeros without one).
 template <typename T>
@@ -596,34 +631,64 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
 }
 
 // The same on tcgen05, for many tokens: 128 rows of one adapter (M) x blocks of 128 columns (N), reduced over the ranks of values and rests.  Rank values lie
-// K-major as memory has them (their parts one after the other), rows of w MN-major.  Eight warps bring w and base into a ring, one issues the MMAs (accumulators in turn), eight
+// in tensor memory, a row a lane, their parts one after the other, rows of w MN-major in shared memory.  Eight warps bring w and base into a ring, one issues the MMAs (accumulators in turn), eight
 // add the products to base in the ring, a row and half of its columns a lane, and write whole rows from there.
 // Bound by the bytes of base and out: 8192 tokens of 2 adapters, 14336 columns, rank 64, bf16: 88 us (mma.sync 133), 5.4 TB/s, on the 128 SMs that there are CTAs for.
 constexpr int EU_TILE = 128, EU_COLS = 128, EU_JOIN = 8, EU_COPY = 8, EU_THREADS = 32 * (EU_JOIN + EU_COPY + 1);
 __device__ int g_adapter_status = 0;
 
-template <int KS, int PARTS> struct ExpandShape {
-    static constexpr int BLOCKS = KS <= 4 ? 1 : 2;                             // of 64 ranks, of each part
-    static constexpr int A = PARTS * BLOCKS * EU_TILE * 128, W_BLOCK = KS * 16 * 128, STAGE = 2 * W_BLOCK + EU_TILE * EU_COLS * 2, STAGES = KS > 4 ? 2 : PARTS == 2 ? 4 : 3;
-    static constexpr int SMEM = A + STAGES * STAGE + 1024;
+template <int KS> struct ExpandShape {
+    static constexpr int W_BLOCK = KS * 16 * 128, STAGE = 2 * W_BLOCK + EU_TILE * EU_COLS * 2, STAGES = KS <= 4 ? 4 : 3, SMEM = STAGES * STAGE + 1024;
 };
+
+// Rank values `ks` * 16 to + 16 of a row (ranks behind the last, and no row: zeros) as pairs of 16 bits of each part.
+__device__ __forceinline__ void rank_step(const Hidden<__half> &h, int rank, int64_t t, bool live, int ks, uint32_t (&parts)[2][8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool ok = live && ks * 16 + i * 8 < rank;
+        const int64_t at = ok ? t * rank + ks * 16 + i * 8 : 0;
+        const uint4 u[2] = {load16_if(h.top + at, ok), load16_if(h.rest + at, ok)};
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+            parts[part][4 * i] = u[part].x;
+            parts[part][4 * i + 1] = u[part].y;
+            parts[part][4 * i + 2] = u[part].z;
+            parts[part][4 * i + 3] = u[part].w;
+        }
+    }
+}
+__device__ __forceinline__ void rank_step(const Hidden<__nv_bfloat16> &h, int rank, int64_t t, bool live, int ks, uint32_t (&parts)[3][8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool ok = live && ks * 16 + i * 4 < rank;
+        const uint4 u = load16_if(h.sum + (ok ? t * rank + ks * 16 + i * 4 : 0), ok);
+        const float2 v[2] = {make_float2(__uint_as_float(u.x), __uint_as_float(u.y)), make_float2(__uint_as_float(u.z), __uint_as_float(u.w))};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            uint32_t s[3];
+            split<__nv_bfloat16>(v[k], s);
+#pragma unroll
+            for (int part = 0; part < 3; ++part) parts[part][2 * i + k] = s[part];
+        }
+    }
+}
 
 template <typename T, int KS>
 __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void *hidden, const T *__restrict__ w, const AdapterArgs p, int64_t per_group, const T *base, T *out) {
-    using S = ExpandShape<KS, PARTS<T>>;
+    using S = ExpandShape<KS>;
     constexpr bool F16 = __is_same(T, __half);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
     extern __shared__ uint8_t raw_smem[];
-    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // parts of the rank values; the ring: [w | base]
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // the ring: [w | base]
     __shared__ __align__(16) int s_id[EU_TILE];
     __shared__ int s_leader[EU_TILE], s_count[4], s_abort;
     __shared__ uint32_t s_tmem;
     __shared__ uint8_t list[EU_TILE];
-    __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], acc_full[2], acc_empty[2];
+    __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], acc_full[2], acc_empty[2], values_full;
     volatile int *abort_flag = &s_abort;
     const Hidden<T> h(hidden, p.M, p.rank);
     const int64_t t0 = (int64_t)blockIdx.x * EU_TILE, begin = blockIdx.y * per_group, end = begin + per_group < p.cols ? begin + per_group : p.cols;
-    const uint32_t rank_values = smem_addr(smem), ring = rank_values + S::A;
+    const uint32_t ring = smem_addr(smem);
 
     if (tid == 0) {
         for (int i = 0; i < S::STAGES; ++i) {
@@ -634,11 +699,12 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
             umma::mbar_init(&acc_full[i], 1);
             umma::mbar_init(&acc_empty[i], EU_JOIN);
         }
+        umma::mbar_init(&values_full, EU_JOIN);
         s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         umma::fence_proxy_async_smem();
     }
-    if (warp == EU_JOIN + EU_COPY) umma::tmem_alloc(&s_tmem, 2 * EU_COLS);
+    if (warp == EU_JOIN + EU_COPY) umma::tmem_alloc(&s_tmem, 512);
     // the adapters of the tile, in the order of their first token
     const bool has = tid < EU_TILE && t0 + tid < p.M;
     const int id = has ? __ldcg(p.index + t0 + tid) : 0;
@@ -671,7 +737,7 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
     pdl_wait();                                   // (what comes before is the launch that makes the rank values, or one behind it)
 
     bool alive = true;                            // (after a failed wait the loops go on without work: the warps meet in them)
-    int it = 0;                                   // blocks of columns so far
+    int it = 0, turn = 0;                         // blocks of columns so far; adapters
     for (int pass = blockIdx.z; pass < groups; pass += p.slots) {
         __syncthreads();
         const int a = s_leader[pass];
@@ -706,7 +772,20 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
             const int quarter = warp % 4, half = warp / 4 * (EU_COLS / 2), row = quarter * 32 + lane;
             const bool live = row < count;
             const int64_t t = t0 + (live ? list[row] : 0);
-            const float f = live ? (F16 ? __ldcg(h.back + t) : 1.0f) * (p.scaling ? __ldcg(p.scaling + a) : 1.0f) : 0.0f;
+            const float f = live ? power_of_row(h, t) * (p.scaling ? __ldcg(p.scaling + a) : 1.0f) : 0.0f;
+            // the row's rank values into tensor memory, behind the two accumulators: [part][step] of 16 ranks in 8 columns (the adapter's before were last read for a block
+            // whose sums this warp has waited for)
+#pragma unroll 2
+            for (int ks = warp / 4; ks < KS; ks += 2) {
+                uint32_t parts[PARTS<T>][8];
+                rank_step(h, p.rank, t, live, ks, parts);
+#pragma unroll
+                for (int part = 0; part < PARTS<T>; ++part) umma::tmem_st_32x32b_x8(tmem + ((uint32_t)(quarter * 32) << 16) + 2 * EU_COLS + (part * KS + ks) * 8, parts[part]);
+            }
+            umma::tmem_st_wait();
+            umma::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(&values_full);
             // what the lane stores: piece `lane` % 8 of the half's rows lane / 8, 4 + lane / 8, ..
             const int stored = quarter * 32 + lane / 8, piece0 = half / 8 + lane % 8;
             T *to[8];
@@ -714,7 +793,7 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
             for (int j = 0; j < 8; ++j) to[j] = stored + 4 * j < count ? out + (t0 + list[stored + 4 * j]) * p.cols + piece0 * 8 : nullptr;
             for (int64_t cb = begin; cb < end; cb += EU_COLS, ++it) {
                 const int slot = it % S::STAGES, acc = it & 1;
-                uint8_t *tile = smem + S::A + slot * S::STAGE + 2 * S::W_BLOCK;
+                uint8_t *tile = smem + slot * S::STAGE + 2 * S::W_BLOCK;
                 alive = __all_sync(0xffffffffu, alive && umma::mbar_wait(&acc_full[acc], it >> 1 & 1, abort_flag, 11, &g_adapter_status) &&
                                                     umma::mbar_wait(&full[slot], it / S::STAGES & 1, abort_flag, 12, &g_adapter_status));
                 const bool work = alive && quarter * 32 < count;
@@ -763,15 +842,6 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
         } else if (warp < EU_JOIN + EU_COPY) {
             // ---- copies ----
             const int me = tid - 32 * EU_JOIN;
-            // rank values: rows of each part, ranks in pieces of 8 (ranks behind the last: zeros)
-#pragma unroll
-            for (int i = 0; i < PARTS<T> * EU_TILE * KS * 2 / (32 * EU_COPY); ++i) {
-                const int at = me + 32 * EU_COPY * i, piece = at % (2 * KS), row = at / (2 * KS) % EU_TILE, part = at / (2 * KS * EU_TILE);
-                const bool ok = row < count && piece * 8 < p.rank;
-                const T *from = h.part(part);
-                copy16(rank_values + ((part * S::BLOCKS + piece / 8) * EU_TILE + row) * 128 + (piece % 8 ^ (row & 7)) * 16,
-                       ok ? from + (t0 + list[row]) * p.rank + piece * 8 : from, ok ? 16 : 0);
-            }
             const int piece = me % 16;
             const T *rows[EU_TILE / 16];                     // this thread's piece of the rows of base
 #pragma unroll
@@ -806,6 +876,8 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
         } else {
             // ---- products ----
             const uint32_t idesc = umma::umma_idesc_f16(EU_COLS, !F16, false) | 1u << 16;      // (B MN-major)
+            alive = __all_sync(0xffffffffu, alive && umma::mbar_wait(&values_full, turn & 1, abort_flag, 16, &g_adapter_status));
+            umma::tc_fence_after();
             for (int64_t cb = begin; cb < end; cb += EU_COLS, ++it) {
                 const int slot = it % S::STAGES, acc = it & 1;
                 alive = __all_sync(0xffffffffu, alive && umma::mbar_wait(&acc_empty[acc], (it >> 1 & 1) ^ 1, abort_flag, 14, &g_adapter_status) &&
@@ -818,15 +890,16 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
                 for (int part = 0; part < PARTS<T>; ++part)
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
-                        umma::umma_f16_ss(tmem + acc * EU_COLS, umma::umma_smem_desc(rank_values + (part * S::BLOCKS + k / 4) * EU_TILE * 128 + k % 4 * 32),
-                                          umma::umma_smem_desc_mn(at + k * 2048, S::W_BLOCK), idesc, (part | k) != 0 ? 1u : 0u);
+                        umma::umma_f16_ts(tmem + acc * EU_COLS, tmem + 2 * EU_COLS + (part * KS + k) * 8, umma::umma_smem_desc_mn(at + k * 2048, S::W_BLOCK), idesc,
+                                          (part | k) != 0 ? 1u : 0u);
                 umma::umma_commit(&acc_full[acc]);
             }
         }
+        ++turn;
     }
     __syncthreads();
     umma::tc_fence_after();
-    if (warp == EU_JOIN + EU_COPY) umma::tmem_dealloc(tmem, 2 * EU_COLS);
+    if (warp == EU_JOIN + EU_COPY) umma::tmem_dealloc(tmem, 512);
 }
 
 // ---- outer ---------------------------------------------------------------------------------------------------------------
@@ -922,8 +995,9 @@ __device__ __forceinline__ void join_sums(float *sums, const AdapterArgs &p, int
 template <int RB, int RG, int PARTS> struct OuterShape {
     static constexpr int WARPS = 4 * RG, THREADS = 32 * WARPS;
     static constexpr int RANKS = 16 * RB * RG, ROW = RANKS * 2;               // bytes of a part of a token's rank values
-    static constexpr int STAGE = OUTER_STEP * (512 + PARTS * ROW), STAGES = RG == 1 ? 4 : 3;
-    static constexpr int SUMS = RANKS * SUM_ROW * 4, SMEM = STAGE * STAGES > SUMS ? STAGE * STAGES : SUMS;
+    static constexpr int STAGE = OUTER_STEP * (512 + 2 * ROW), STAGES = RG == 1 ? 4 : 3;
+    static constexpr int SPLIT = STAGE * STAGES, RING = SPLIT + (PARTS == 3 ? OUTER_STEP * 3 * ROW : 0);       // (bf16: the parts of the stage at work, behind the ring)
+    static constexpr int SUMS = RANKS * SUM_ROW * 4, SMEM = RING > SUMS ? RING : SUMS;
     static __device__ __forceinline__ int swizzle(int token) { return ROW >= 128 ? token & 7 : ROW == 64 ? token >> 1 & 3 : token >> 2 & 1; }
 };
 
@@ -960,26 +1034,35 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
     // this thread's piece of a row of x (columns behind the last: zeros), and bytes of a row
     const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0;
     const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0));
-    const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2, x_to = warp * 512 + (lane ^ (warp >> 1 & 3) << 1) * 16;
-    // and its pieces of the rank values' parts
-    constexpr int PIECES = S::ROW / 16, ALL = OUTER_STEP * PIECES * PARTS<T>, HJ = (ALL + S::THREADS - 1) / S::THREADS;
+    const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * (F16 ? 2 : 4), x_to = warp * 512 + (lane ^ (warp >> 1 & 3) << 1) * 16;
+    // and its pieces of the rank values: 2 * ROW bytes a token, of both parts or of fp32
+    constexpr int PIECES = S::ROW / 16, HJ = OUTER_STEP * PIECES * 2 / S::THREADS;
     const uint8_t *h_from[HJ];
     uint32_t h_to[HJ];
     int h_token[HJ], h_bytes[HJ];
 #pragma unroll
     for (int j = 0; j < HJ; ++j) {
-        const int i = threadIdx.x + S::THREADS * j, part = i / (OUTER_STEP * PIECES), token = i / PIECES % OUTER_STEP, piece = i % PIECES;
-        h_token[j] = token;
-        h_bytes[j] = rank0 + piece * 8 < p.rank ? 16 : 0;
-        h_from[j] = (const uint8_t *)(h.part(part) + (h_bytes[j] ? rank0 + piece * 8 : 0));
-        h_to[j] = OUTER_STEP * (512 + part * S::ROW) + token * S::ROW + (piece ^ S::swizzle(token)) * 16;
+        const int i = threadIdx.x + S::THREADS * j;
+        if constexpr (F16) {
+            const int part = i / (OUTER_STEP * PIECES), token = i / PIECES % OUTER_STEP, piece = i % PIECES;
+            h_token[j] = token;
+            h_bytes[j] = rank0 + piece * 8 < p.rank ? 16 : 0;
+            h_from[j] = (const uint8_t *)((part ? h.rest : h.top) + (h_bytes[j] ? rank0 + piece * 8 : 0));
+            h_to[j] = OUTER_STEP * (512 + part * S::ROW) + token * S::ROW + (piece ^ S::swizzle(token)) * 16;
+        } else {
+            const int token = i / (2 * PIECES), piece = i % (2 * PIECES);
+            h_token[j] = token;
+            h_bytes[j] = rank0 + piece * 4 < p.rank ? 16 : 0;
+            h_from[j] = (const uint8_t *)(h.sum + (h_bytes[j] ? rank0 + piece * 4 : 0));
+            h_to[j] = OUTER_STEP * 512 + token * 2 * S::ROW + piece * 16;
+        }
     }
     // a lane's places in the stage: token 2 c, piece r of its warp's columns; and rows of rank values for ldmatrix
     const uint32_t x_place = c * 1024 + wc * 128 + (r ^ c << 1) * 16;
     uint32_t h_place[RB];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb)
-        h_place[rb] = OUTER_STEP * 512 + (lane % 8 + lane / 16 * 8) * S::ROW + (((wr * RB + rb) * 2 + lane / 8 % 2) ^ S::swizzle(lane % 8)) * 16;
+        h_place[rb] = (lane % 8 + lane / 16 * 8) * S::ROW + (((wr * RB + rb) * 2 + lane / 8 % 2) ^ S::swizzle(lane % 8)) * 16;
     float acc[RB][8][4] = {};
     float big = 0.0f;                                            // fp16: the sums are of h / big, the largest power of two of a row so far: what is lost of a row is less
                                                                  // than 2^-38 of the largest one's values
@@ -1007,7 +1090,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                     copy16(to + (x_to ^ (S::WARPS * j / 2 & 3) * 32) + S::WARPS * j * 512, xs0 + (uint64_t)(uint32_t)list[first + warp + S::WARPS * j] * x_row, x_bytes);
 #pragma unroll
                 for (int j = 0; j < HJ; ++j)
-                    if (ALL % S::THREADS == 0 || threadIdx.x + S::THREADS * j < ALL) copy16(to + h_to[j], h_from[j] + (uint64_t)(uint32_t)list[first + h_token[j]] * h_row, first + h_token[j] < n ? h_bytes[j] : 0);
+                    copy16(to + h_to[j], h_from[j] + (uint64_t)(uint32_t)list[first + h_token[j]] * h_row, first + h_token[j] < n ? h_bytes[j] : 0);
             }
             copies_commit();
         };
@@ -1045,7 +1128,20 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
             // (copies take about 1000 cycles of a stage to issue: of the two warps that share a quarter of the SM one makes its own before, one after its MMAs)
             const int refill = stage == 0 ? S::STAGES - 1 : stage - 1;
             if (wr == 0) copy_stage(first + (S::STAGES - 1) * OUTER_STEP, refill);
-            const uint32_t place = ring + stage * S::STAGE;
+            const uint32_t place = ring + stage * S::STAGE, h_at = F16 ? place + OUTER_STEP * 512 : ring + S::SPLIT;
+            if constexpr (!F16) {
+                // the stage's rank values in parts (which all warps are done with since the barrier above)
+                for (int i = threadIdx.x; i < OUTER_STEP * PIECES; i += S::THREADS) {
+                    const int token = i / PIECES, piece = i % PIECES;
+                    const float4 *from = reinterpret_cast<const float4 *>(smem + stage * S::STAGE + OUTER_STEP * 512 + token * 2 * S::ROW + piece * 32);
+                    uint4 parts[3];
+                    split8<T>(from[0], from[1], parts);
+#pragma unroll
+                    for (int part = 0; part < 3; ++part)
+                        *reinterpret_cast<uint4 *>(smem + S::SPLIT + (part * OUTER_STEP + token) * S::ROW + (piece ^ S::swizzle(token)) * 16) = parts[part];
+                }
+                __syncthreads();
+            }
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
 #pragma unroll
             for (int step = 0; step < OUTER_STEP / 16; ++step) {
@@ -1074,7 +1170,7 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 #pragma unroll
                     for (int part = 0; part < PARTS<T>; ++part) {
                         uint32_t ha[4];
-                        load_matrices_transposed(place + h_place[rb] + (part * OUTER_STEP + step * 16) * S::ROW, ha);
+                        load_matrices_transposed(h_at + h_place[rb] + (part * OUTER_STEP + step * 16) * S::ROW, ha);
                         if constexpr (F16) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
@@ -1108,27 +1204,29 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 
 // The same on tcgen05, for adapters of many tokens: 64 ranks x 256 columns a CTA, reduced over tokens, 32 a stage.  Rows of x and of the rank values keep
 // the order in which memory holds them, which is the MN-major form of both operands (blocks of 64 elements by 32 tokens, 128-byte swizzle).  Values and
-// rests of 64 ranks are the two halves of the M dimension, so that one MMA multiplies both; their sums meet at the end.  The third part of bf16 takes MMAs of
-// its own, with a block of zeros as the other half (MMAs do not bound this).  Eight warps fill the ring with
-// 16-byte cp.async of rows that a list names, one warp issues the MMAs; for fp16 two warps between them bring the rows' powers of two into the rank
-// values.  (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between the copies and themselves, waits for all that
-// its own thread has in flight: 86 us instead of 76.)  Bound by the rows of x and the rank values, which every 256 columns read again: 8192 tokens of 2 adapters, 14336
-// columns, rank 64, bf16: 352 MB in 76 us, on the 112 SMs that there are CTAs for.  (mma.sync: 129 us.  Sixteen copying warps: the same, and 2 us more to begin.)
-constexpr int OU_THREADS = 352, OU_LIST = 1024, OU_WINDOW = 512;
+// rests of 64 ranks are the two halves of the M dimension, so that one MMA multiplies both; their sums meet at the end.  Eight warps fill the ring with
+// 16-byte cp.async of rows that a list names, one warp issues the MMAs.  Between them stand pairs of warps, a stage each in turn: for fp16 one pair, which brings the rows' powers
+// of two into the rank values, for bf16 three, which split the fp32 rank values into parts behind the ring.  The third part takes MMAs of its own, with zeros as the other half.
+// (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between the copies and themselves, waits for all that its own thread has in flight: 86 us
+// instead of 76.)  Bound by the rows of x and the rank values, which every 256 columns read again, and by shared memory: 8192 tokens of 1 adapter, 14336 columns, rank 64, on the
+// 112 SMs that there are CTAs for: bf16 93 us (in two parts that came as such 73; one pair of warps 113, two 105, four 93; parts in tensor memory, a rank a lane, 101).
+constexpr int OU_LIST = 1024, OU_WINDOW = 512;
 template <typename T> struct OuterUmma {
-    static constexpr int BLOCK = OUTER_STEP * 128, A = PARTS<T> * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 7;
-    static constexpr int ZEROS = STAGES * STAGE, SMEM = ZEROS + (PARTS<T> == 3 ? BLOCK : 0) + 1024;
-    static_assert(64 * SUM_ROW * 4 <= ZEROS, "the sums take the ring's place");
+    static constexpr int BLOCK = OUTER_STEP * 128, A = 2 * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 6;
+    static constexpr int PAIRS = PARTS<T> == 2 ? 1 : 3, THREADS = 288 + 64 * PAIRS;                             // pairs of warps that work on rank values, a stage each in turn
+    static constexpr int SPLIT = STAGES * STAGE, ZEROS = SPLIT + (PARTS<T> == 3 ? PAIRS * 3 * BLOCK : 0);      // bf16: their parts, and zeros, behind the ring
+    static constexpr int SMEM = ZEROS + (PARTS<T> == 3 ? BLOCK : 0) + 1024;
+    static_assert(64 * SUM_ROW * 4 <= SPLIT, "the sums take the ring's place");
 };
 template <typename T>
-__global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
+__global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
     using S = OuterUmma<T>;
     constexpr bool F16 = __is_same(T, __half);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const int rank_blocks = (p.rank + 63) / 64, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * 64;
     const int64_t col0 = (int64_t)blockIdx.x * 256;
     extern __shared__ uint8_t raw_smem[];
-    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [STAGES][parts of the rank values | 4 blocks of columns][tokens][128 B]; zeros
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [STAGES][rank values | 4 blocks of columns][tokens][128 B]; bf16: [PAIRS][parts][tokens][128 B]; zeros
     float *sums = reinterpret_cast<float *>(smem);                                      // [64][SUM_ROW], at the end
     __shared__ int list[OU_LIST + OUTER_STEP], s_before[OU_WINDOW], s_count[8], s_end[S::STAGES], s_abort;
     __shared__ uint32_t s_bits[OU_WINDOW], s_tmem;
@@ -1150,7 +1248,7 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
         umma::fence_proxy_async_smem();
     }
     if constexpr (PARTS<T> == 3) {
-        for (int i = threadIdx.x; i < S::BLOCK / 16; i += OU_THREADS) reinterpret_cast<uint4 *>(smem + S::ZEROS)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < S::BLOCK / 16; i += S::THREADS) reinterpret_cast<uint4 *>(smem + S::ZEROS)[i] = make_uint4(0, 0, 0, 0);
         umma::fence_proxy_async_smem();
     }
     if (warp == 8) umma::tmem_alloc(&s_tmem, 256);
@@ -1170,50 +1268,68 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
         const uint32_t ring = smem_addr(smem);
         for (;; ++stages) {
             const int slot = stages % S::STAGES;
-            if (!__all_sync(0xffffffffu, umma::mbar_wait(F16 ? &scaled[slot] : &full[slot], stages / S::STAGES & 1, abort_flag, 1, &g_adapter_status))) break;
+            if (!__all_sync(0xffffffffu, umma::mbar_wait(&scaled[slot], stages / S::STAGES & 1, abort_flag, 1, &g_adapter_status))) break;
             if (*(volatile int *)&s_end[slot]) {
                 umma::umma_commit(&done);
                 break;
             }
             umma::fence_proxy_async_smem();
             umma::tc_fence_after();
-            const uint32_t at = ring + slot * S::STAGE;
+            const uint32_t at = ring + slot * S::STAGE, values = F16 ? at : ring + S::SPLIT + stages % S::PAIRS * 3 * S::BLOCK;
 #pragma unroll
             for (int k = 0; k < OUTER_STEP / 16; ++k) {
                 const uint64_t columns = umma::umma_smem_desc_mn(at + S::A + k * 2048, S::BLOCK);
-                umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(at + k * 2048, S::BLOCK), columns, idesc, (stages | k) != 0 ? 1u : 0u);
+                umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(values + k * 2048, S::BLOCK), columns, idesc, (stages | k) != 0 ? 1u : 0u);
                 // (the third part above a block of zeros)
-                if constexpr (PARTS<T> == 3)
-                    umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(at + 2 * S::BLOCK + k * 2048, ring + S::ZEROS - (at + 2 * S::BLOCK)), columns, idesc, 1u);
+                if constexpr (!F16)
+                    umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(values + 2 * S::BLOCK + k * 2048, ring + S::ZEROS - (values + 2 * S::BLOCK)), columns, idesc, 1u);
             }
             umma::umma_commit(&empty[slot]);
         }
     } else if (warp > 8) {
-        // ---- fp16: rank values times their row's power of two ----
+        // ---- fp16: rank values times their row's power of two; bf16: fp32 rank values in parts ----
         if (p.behind) pdl_wait();
-        if constexpr (F16)
-            for (;; ++stages) {
-                const int slot = stages % S::STAGES;
-                if (!__all_sync(0xffffffffu, umma::mbar_wait(&full[slot], stages / S::STAGES & 1, abort_flag, 5, &g_adapter_status))) break;
-                const bool end = *(volatile int *)&s_end[slot];
-                if (!end) {
+        const int pair = (warp - 9) / 2, me = (warp - 9) % 2 * 32 + lane;
+        for (stages = pair;; stages += S::PAIRS) {
+            const int slot = stages % S::STAGES;
+            bool ok = umma::mbar_wait(&full[slot], stages / S::STAGES & 1, abort_flag, 5, &g_adapter_status);
+            // (the MMAs that took this pair's parts before are done)
+            if constexpr (!F16)
+                if (const int last = stages - S::PAIRS; last >= 0) ok = ok && umma::mbar_wait(&empty[last % S::STAGES], last / S::STAGES & 1, abort_flag, 6, &g_adapter_status);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const bool end = *(volatile int *)&s_end[slot];
+            if (!end) {
+                uint8_t *stage = smem + slot * S::STAGE;
+                if constexpr (F16) {
 #pragma unroll
                     for (int i = 0; i < S::A / 16 / 64; ++i) {
-                        const int at = (warp - 9) * 32 + lane + i * 64;      // of 16 bytes, eight a row
+                        const int at = me + i * 64;      // of 16 bytes, eight a row
                         const float f = s_scale[slot][at / 8 % OUTER_STEP];
                         const __half2 scale = __float2half2_rn(fmaxf(f, 0x1p-24f)), more = __float2half2_rn(fminf(f * 0x1p24f, 1.0f));      // (powers below 2^-24 as well)
-                        uint4 *own = reinterpret_cast<uint4 *>(smem + slot * S::STAGE) + at, v = *own;
+                        uint4 *own = reinterpret_cast<uint4 *>(stage) + at, v = *own;
                         __half2 *y = reinterpret_cast<__half2 *>(&v);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) y[k] = __hmul2(__hmul2(y[k], scale), more);
                         *own = v;
                     }
-                    umma::fence_proxy_async_smem();
+                } else {
+                    uint8_t *to = smem + S::SPLIT + pair * 3 * S::BLOCK;
+#pragma unroll
+                    for (int i = 0; i < OUTER_STEP * 8 / 64; ++i) {
+                        const int at = me + i * 64, token = at / 8, piece = at % 8;      // of eight ranks
+                        const float4 *from = reinterpret_cast<const float4 *>(stage + token * 256);
+                        uint4 parts[3];
+                        split8<T>(from[(2 * piece) ^ (token & 7)], from[(2 * piece + 1) ^ (token & 7)], parts);
+#pragma unroll
+                        for (int part = 0; part < 3; ++part) *reinterpret_cast<uint4 *>(to + part * S::BLOCK + token * 128 + (piece ^ (token & 7)) * 16) = parts[part];
+                    }
                 }
-                __syncwarp();
-                if (lane == 0) umma::mbar_arrive(&scaled[slot]);
-                if (end) break;
+                umma::fence_proxy_async_smem();
             }
+            __syncwarp();
+            if (lane == 0) umma::mbar_arrive(&scaled[slot]);
+            if (end) break;
+        }
     } else {
         // ---- copies ----
         const auto meet = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
@@ -1241,12 +1357,25 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
         }
         f = big * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
 
-        // this thread's pieces: of rows warp, warp + 8, .. of x piece `lane`; of row threadIdx / 8 of the rank values' parts piece threadIdx % 8
-        const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0, token = threadIdx.x / 8, piece = threadIdx.x % 8, h_bytes = rank0 + piece * 8 < p.rank ? 16 : 0;
-        const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0));
-        const T *h0 = h.top + (h_bytes ? rank0 + piece * 8 : 0);
-        const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2, ring = smem_addr(smem);
-        const uint32_t x_to = S::A + lane / 8 * (S::BLOCK) + warp * 128 + (lane % 8 ^ warp) * 16, h_to = token * 128 + (piece ^ (token & 7)) * 16;
+        // this thread's pieces: of rows warp, warp + 8, .. of x piece `lane`; of row threadIdx / 8 of the rank values pieces threadIdx % 8 of values and rests, or (fp32)
+        // that one and the one eight further on
+        const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0, token = threadIdx.x / 8, piece = threadIdx.x % 8;
+        const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0)), *h0[2];
+        const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * (F16 ? 2 : 4), ring = smem_addr(smem);
+        const uint32_t x_to = S::A + lane / 8 * S::BLOCK + warp * 128 + (lane % 8 ^ warp) * 16;
+        uint32_t h_to[2];
+        int h_bytes[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if constexpr (F16) {
+                h_bytes[i] = rank0 + piece * 8 < p.rank ? 16 : 0;
+                h0[i] = (const uint8_t *)((i ? h.rest : h.top) + (h_bytes[i] ? rank0 + piece * 8 : 0));
+                h_to[i] = i * S::BLOCK + token * 128 + (piece ^ (token & 7)) * 16;
+            } else {
+                h_bytes[i] = rank0 + (piece + 8 * i) * 4 < p.rank ? 16 : 0;
+                h0[i] = (const uint8_t *)(h.sum + (h_bytes[i] ? rank0 + (piece + 8 * i) * 4 : 0));
+                h_to[i] = token * 256 + ((piece + 8 * i) ^ (token & 7)) * 16;
+            }
         bool alive = true;                                       // (after a failed wait the loops go on without copies: the warps meet in them)
         int window = 0, passed = 0;
         for (int from = lo, n; from < hi; from += n) {
@@ -1279,8 +1408,7 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
                     const int at = first + token;
                     const uint64_t row = at < n ? (uint64_t)(uint32_t)list[at] * h_row : 0;
 #pragma unroll
-                    for (int part = 0; part < PARTS<T>; ++part)
-                        copy16(to + h_to + part * S::BLOCK, (const uint8_t *)(h0 + part * h.size) + row, at < n ? h_bytes : 0);
+                    for (int k = 0; k < 2; ++k) copy16(to + h_to[k], h0[k] + row, at < n ? h_bytes[k] : 0);
                     if constexpr (F16)
                         if (piece == 0) s_scale[slot][token] = at < n ? s_back[at] : 0.0f;
                     copies_arrive(&full[slot]);
@@ -1289,13 +1417,15 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
                 if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
             }
         }
-        // one more stage, without tokens: the end
-        const int slot = stages % S::STAGES;
-        alive = alive && umma::mbar_wait(&empty[slot], (stages / S::STAGES & 1) ^ 1, abort_flag, 3, &g_adapter_status);
-        if (threadIdx.x == 0) *(volatile int *)&s_end[slot] = 1;
-        if (alive) copies_arrive(&full[slot]);
-        __syncwarp();
-        if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
+        // more stages, without tokens: the end, one for each pair
+        for (int i = 0; i < S::PAIRS; ++i) {
+            const int slot = (stages + i) % S::STAGES;
+            alive = alive && umma::mbar_wait(&empty[slot], ((stages + i) / S::STAGES & 1) ^ 1, abort_flag, 3, &g_adapter_status);
+            if (threadIdx.x == 0) *(volatile int *)&s_end[slot] = 1;
+            if (alive) copies_arrive(&full[slot]);
+            __syncwarp();
+            if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
+        }
         asm volatile("cp.async.wait_all;" ::: "memory");
         // ---- sums of this CTA: tensor memory's lanes 0 to 63 are the values' ranks, 64 to 127 the rests' ----
         if (warp < 4) alive = __all_sync(0xffffffffu, umma::mbar_wait(&done, 0, abort_flag, 4, &g_adapter_status));
@@ -1326,7 +1456,7 @@ __global__ void __launch_bounds__(OU_THREADS, 1) adapter_outer_umma_kernel(void 
     __syncwarp();
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
-    if (*abort_flag == 0) join_sums<T, OU_THREADS, 64>(sums, p, a, rank0, col0, dw);
+    if (*abort_flag == 0) join_sums<T, S::THREADS, 64>(sums, p, a, rank0, col0, dw);
     cluster.sync();                                              // a CTA's sums stay until the others have read them
     umma::tc_fence_after();
     if (warp == 8) umma::tmem_dealloc(tmem, 256);
@@ -1445,7 +1575,7 @@ int shrink(const void *x, const void *w, const AdapterArgs &p, void *h, cudaStre
 
 template <typename T, int KS>
 int expand_umma(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaStream_t st) {
-    using S = ExpandShape<KS, PARTS<T>>;
+    using S = ExpandShape<KS>;
     p.slots = p.adapters + 1 < 2 ? p.adapters + 1 : 2;
     int per_sm = 0;
     const int rc = ctas_per_sm<adapter_expand_umma_kernel<T, KS>>(EU_THREADS, S::SMEM, per_sm);
@@ -1498,11 +1628,11 @@ int outer_fast(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st
 template <typename T>
 int outer_umma(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st) {
     const int64_t blocks = (p.cols + 255) / 256, rows = (int64_t)p.adapters * ((p.rank + 63) / 64), most = (p.M + 4 * OUTER_STEP - 1) / (4 * OUTER_STEP);
-    int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_umma_kernel<T>>(OU_THREADS, OuterUmma<T>::SMEM, per_sm);
+    int per_sm = 0, parts = 1, rc = ctas_per_sm<adapter_outer_umma_kernel<T>>(OuterUmma<T>::THREADS, OuterUmma<T>::SMEM, per_sm);
     // (a part's start and end take as long as about 384 of its tokens)
-    if (rc == BW_OK) rc = cluster_parts<adapter_outer_umma_kernel<T>>(blocks * rows, most, 384.0 * p.adapters / p.M, OU_THREADS, OuterUmma<T>::SMEM, parts);
+    if (rc == BW_OK) rc = cluster_parts<adapter_outer_umma_kernel<T>>(blocks * rows, most, 384.0 * p.adapters / p.M, OuterUmma<T>::THREADS, OuterUmma<T>::SMEM, parts);
     if (rc != BW_OK) return rc;
-    return launch_early("adapter_outer_umma_kernel", adapter_outer_umma_kernel<T>, dim3((unsigned)blocks, (unsigned)rows, parts), OU_THREADS, OuterUmma<T>::SMEM, st, dim3(1, 1, parts), h, x, p, dw);
+    return launch_early("adapter_outer_umma_kernel", adapter_outer_umma_kernel<T>, dim3((unsigned)blocks, (unsigned)rows, parts), OuterUmma<T>::THREADS, OuterUmma<T>::SMEM, st, dim3(1, 1, parts), h, x, p, dw);
 }
 template <typename T>
 int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
@@ -1566,8 +1696,8 @@ int backward(const void *dy, const void *x, int64_t M, int64_t N, int64_t K, con
 
 }  // namespace
 
-// (three 16-bit parts, or two and a power of two a row; the general kernels' fp32 values are less)
-size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * 6 + (size_t)M * 4; }
+// (two 16-bit parts and a power of two a row; fp32 values, of bf16 and of the general kernels, are less)
+size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * 4 + (size_t)M * 4; }
 
 int adapter_device_status() {
     int v = 0, zero = 0;
