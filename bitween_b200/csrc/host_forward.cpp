@@ -412,9 +412,9 @@ PyObject *adapter_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     } else {
         if (given) {
             const uintptr_t o = reinterpret_cast<uintptr_t>(given->const_data_ptr());
-            for (const at::Tensor *y : {x, down, up, index, scaling, base}) {
-                const uintptr_t a = y ? reinterpret_cast<uintptr_t>(y->const_data_ptr()) : 0;
-                if (y && a < o + given->nbytes() && o < a + y->nbytes() && !(y == base && a == o)) Py_RETURN_NONE;
+            for (int i = 0; i < 6; ++i) {                            // (by position: one tensor may be several arguments, and only as base may it be written over)
+                const uintptr_t a = t[i] ? reinterpret_cast<uintptr_t>(t[i]->const_data_ptr()) : 0;
+                if (t[i] && a < o + given->nbytes() && o < a + t[i]->nbytes() && !(i == 5 && a == o)) Py_RETURN_NONE;
             }
             if (given->requires_grad()) Py_RETURN_NONE;
             out = *given;

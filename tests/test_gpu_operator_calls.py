@@ -1,0 +1,34 @@
+"""Calls of the cache and the adapters that the documentation allows and that are easily got wrong."""
+import pytest
+import torch
+
+from bitween_b200 import adapter_matmul
+from bitween_b200.kernels import _lib
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _bank(M, K, N, n, r, dtype=torch.float16, seed=1):
+    g = _gen(seed)
+    x, down, up = torch.randn(M, K, generator=g, device=DEV), torch.randn(n, r, K, generator=g, device=DEV) * K ** -0.5, 0.2 * torch.randn(n, r, N, generator=g, device=DEV)
+    return (*(t.to(dtype) for t in (x, down, up)), torch.randint(-1, n, (M,), generator=g, device=DEV).to(torch.int32), torch.randn(M, N, generator=g, device=DEV).to(dtype))
+
+
+@pytest.mark.parametrize("n,r", [(4, 8), (8, 16), (40, 64)])
+def test_one_tensor_as_several_arguments_and_as_the_result(n, r):
+    """A tensor that is base and result may be another argument as well: what is read of that is what stood there before."""
+    K = N = 128
+    x, down, up, index, _ = _bank(n * r, K, N, n, r)
+    ops, lead = _lib.host_operators(), (n, r)
+    for which in ("up", "down", "x"):
+        args = {"x": x.view(*lead, K), "down": down.clone(), "up": up.clone()}
+        both = args[which]
+        want = adapter_matmul(args["x"], args["down"], args["up"], index.view(lead), base=both.clone())
+        assert ops.adapter_matmul(args["x"], args["down"], args["up"], index.view(lead), None, both, both) is None
+        got = adapter_matmul(args["x"], args["down"], args["up"], index.view(lead), base=both, out=both)
+        assert got is both and torch.equal(got, want)
