@@ -74,7 +74,8 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
     `index`, int32 of x's leading shape (or flat): the adapter of each row; rows below 0 have none and get `base` (zeros without
     one); an index beyond the bank gives NaN.  `scaling`: fp32 [adapters] or None (ones); it has no gradient.  x, down, up and base share one
     dtype, fp16 or bf16; sums are fp32 and the result is rounded once.  Ranks up to 256.  Differentiable in x, down, up and base.
-    `out`, a contiguous tensor of the result's shape, takes the result where no gradient is recorded; it may be `base` itself."""
+    `out`, a contiguous tensor of the result's shape, takes the result where no gradient is recorded (one that requires a gradient is refused, too); it may be `base`
+    itself."""
     y = (_lib._operators or _lib.host_operators()).adapter_matmul(x, down, up, index, scaling, base, out)
     if y is not None:
         return y
@@ -117,7 +118,7 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
     args = (_aligned(x2), _aligned(down), _aligned(up), index, scaling, base2)
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, base))
     if out is not None:
-        if grad:
+        if grad or (torch.is_grad_enabled() and out.requires_grad):
             raise ValueError("`out` is for calls that record no gradient")
         if out.shape != (*lead, N) or not out.is_contiguous():
             raise ValueError(f"`out` must be contiguous {(*lead, N)}")

@@ -32,3 +32,19 @@ def test_one_tensor_as_several_arguments_and_as_the_result(n, r):
         assert ops.adapter_matmul(args["x"], args["down"], args["up"], index.view(lead), None, both, both) is None
         got = adapter_matmul(args["x"], args["down"], args["up"], index.view(lead), base=both, out=both)
         assert got is both and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_result_that_requires_a_gradient_is_refused(native, monkeypatch):
+    """Written in place it would keep the history of what stood there before."""
+    if not native:
+        monkeypatch.setattr(_lib, "_operators", _lib._NoOperators)
+    x, down, up, index, base = _bank(9, 64, 128, 2, 8)
+    for out in (base.clone().requires_grad_(), base.clone().requires_grad_() * 2):
+        before = out.detach().clone()
+        with pytest.raises(ValueError, match="no gradient"):
+            adapter_matmul(x, down, up, index, base=base, out=out)
+        assert torch.equal(out.detach(), before)
+        with torch.no_grad():
+            adapter_matmul(x, down, up, index, base=base, out=out)
+        assert torch.equal(out.detach(), adapter_matmul(x, down, up, index, base=base))
