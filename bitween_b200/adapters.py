@@ -42,12 +42,17 @@ class AdapterFunction(torch.autograd.Function):
     def forward(ctx, x, down, up, index, scaling, base):
         out, hidden = _forward(x, down, up, index, scaling, base, None, ctx.needs_input_grad[2])
         ctx.save_for_backward(x, down, up, index, scaling, hidden)
+        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in (x, down, up, index, scaling, hidden)]
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        x, down, up, index, scaling, hidden = ctx.saved_tensors
+        saved = ctx.saved_tensors
+        # (hooks may have made other tensors of them in the meantime: moved, packed)
+        if any((t is None) != (like is None) or (t is not None and (t.shape, t.dtype, t.device) != like) for t, like in zip(saved, ctx.like)):
+            raise RuntimeError("adapter_matmul: a tensor saved for the backward pass has come back from its hooks in another shape, type or place")
+        x, down, up, index, scaling, hidden = (t if t is None else _aligned(t.resolve_neg()) for t in saved)
         want_x, want_down, want_up = ctx.needs_input_grad[:3]
         grads = [torch.empty_like(t) if want else None for t, want in ((x, want_x), (down, want_down), (up, want_up))]
         if want_x or want_down or want_up:

@@ -305,6 +305,20 @@ int adapter_call(const at::Tensor &x, const at::Tensor &down, const at::Tensor &
 // again.  Edges: x, down, up, base.
 struct AdapterNode : torch::autograd::Node {
     torch::autograd::SavedVariable x, down, up, index, scaling, hidden;
+    c10::SmallVector<int64_t, 5> x_sizes, index_sizes;
+    bool scaled = false, kept = false;        // there are scaling, hidden
+    int64_t adapters = 0, rank = 0, K = 0, N = 0, M = 0;
+    at::ScalarType type = at::kHalf;
+    c10::Device device = c10::Device(c10::kCPU);
+
+    // A saved tensor, as the kernels take it.  Hooks may have made another tensor of it in the meantime (moved, packed).
+    at::Tensor back(const torch::autograd::SavedVariable &saved, at::IntArrayRef sizes, at::ScalarType as) const {
+        at::Tensor t = saved.unpack();
+        TORCH_CHECK(t.defined() && t.layout() == c10::kStrided && t.device() == device && t.scalar_type() == as && t.sizes() == sizes,
+                    "adapter_matmul: a tensor saved for the backward pass has come back from its hooks in another shape, type or place");
+        t = t.resolve_neg().contiguous();
+        return on_16_bytes(t) ? t : t.clone();
+    }
 
     std::string name() const override { return "AdapterNode"; }
     void release_variables() override {
@@ -331,9 +345,9 @@ struct AdapterNode : torch::autograd::Node {
         check_capture();
         const bool again = c10::GradMode::is_enabled();
         if (task_should_compute_output(0) || task_should_compute_output(1) || task_should_compute_output(2)) {
-            const at::Tensor xt = x.unpack(), dt = down.unpack(), ut = up.unpack(), it = index.unpack(), st = scaling.unpack(), ht = hidden.unpack();
             at::AutoGradMode off(false);
-            const int64_t K = dt.size(2), N = ut.size(2), M = xt.numel() / K;
+            const at::Tensor xt = back(x, x_sizes, type), dt = back(down, {adapters, rank, K}, type), ut = back(up, {adapters, rank, N}, type), it = back(index, index_sizes, at::kInt),
+                             st = scaled ? back(scaling, {adapters}, at::kFloat) : at::Tensor(), ht = kept ? back(hidden, {(int64_t)g_ops.adapter_bytes(M, (int)rank)}, at::kByte) : at::Tensor();
             at::Tensor dense = g.contiguous();
             if (!on_16_bytes(dense)) dense = dense.clone();
             const at::Tensor *like[3] = {&xt, &dt, &ut};
@@ -365,12 +379,23 @@ at::Tensor adapter_recorded(const at::Tensor &x, const at::Tensor &down, const a
     if (adapter_call(x, down, up, index, scaling, base, out, hidden) != BW_OK) return at::Tensor();
     const std::shared_ptr<AdapterNode> node(new AdapterNode(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x, down, up, base));
+    node->x_sizes.assign(x.sizes().begin(), x.sizes().end());
+    node->index_sizes.assign(index.sizes().begin(), index.sizes().end());
+    node->scaled = scaling.defined();
+    node->kept = up.requires_grad();
+    node->adapters = down.size(0);
+    node->rank = down.size(1);
+    node->K = down.size(2);
+    node->N = up.size(2);
+    node->M = x.numel() / node->K;
+    node->type = x.scalar_type();
+    node->device = x.device();
     node->x = torch::autograd::SavedVariable(x, false);
     node->down = torch::autograd::SavedVariable(down, false);
     node->up = torch::autograd::SavedVariable(up, false);
     node->index = torch::autograd::SavedVariable(index, false);
     node->scaling = torch::autograd::SavedVariable(scaling, false);
-    node->hidden = torch::autograd::SavedVariable(up.requires_grad() ? hidden : at::Tensor(), false);
+    node->hidden = torch::autograd::SavedVariable(node->kept ? hidden : at::Tensor(), false);
     torch::autograd::set_history(out, node);
     return out;
 }

@@ -48,3 +48,42 @@ def test_a_result_that_requires_a_gradient_is_refused(native, monkeypatch):
         with torch.no_grad():
             adapter_matmul(x, down, up, index, base=base, out=out)
         assert torch.equal(out.detach(), adapter_matmul(x, down, up, index, base=base))
+
+
+def _spread(t):
+    """The same values, not contiguous."""
+    wide = t.new_empty((*t.shape, 2))
+    wide[..., 0] = t
+    return wide[..., 0]
+
+
+def _shifted(t):
+    """The same values, off a 16-byte boundary."""
+    return torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_saved_tensors_that_hooks_have_moved_or_packed(native, monkeypatch):
+    """What the hooks give back is what the backward pass works on: in any layout, but of the saved shape, type and device."""
+    if not native:
+        monkeypatch.setattr(_lib, "_operators", _lib._NoOperators)
+    x, down, up, index, base = _bank(40, 64, 128, 2, 8)
+    scaling = torch.tensor([0.5, 2.0], device=DEV)
+
+    def gradients(hooks=None):
+        leaves = [t.clone().requires_grad_() for t in (x, down, up)]
+        if hooks is None:
+            y = adapter_matmul(*leaves, index, scaling=scaling)
+        else:
+            with hooks:
+                y = adapter_matmul(*leaves, index, scaling=scaling)
+        assert ("AdapterNode" in y.grad_fn.name()) == native
+        return torch.autograd.grad(y, leaves, base)
+
+    want = gradients()
+    hooks = torch.autograd.graph.saved_tensors_hooks
+    for same in (torch.autograd.graph.save_on_cpu(), hooks(lambda t: t.clone(), _spread), hooks(lambda t: t.clone(), _shifted), hooks(lambda t: t.cpu(), lambda t: t.to(DEV))):
+        assert all(torch.equal(a, b) for a, b in zip(gradients(same), want))
+    for other in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t.flatten(), lambda t: t[:1], lambda t: t.bfloat16() if t.dtype == torch.float16 else t):
+        with pytest.raises(RuntimeError, match="come back from its hooks"):
+            gradients(hooks(lambda t: t.clone(), other))
