@@ -6,7 +6,7 @@ import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from .kernels import _lib
-from .modules import QuantizedLinear, QuantizedLinearFunction
+from .modules import QuantizedLinear
 
 _DTYPES = (torch.float16, torch.bfloat16)
 
@@ -143,7 +143,8 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
 
 
 class AdaptedLinear(nn.Module):
-    """A QuantizedLinear and a bank of low-rank adapters beside it: forward(x, index) is layer(x) plus each row's adapter.
+    """A QuantizedLinear and a bank of low-rank adapters beside it: forward(x, index) is layer(x) plus each row's adapter.  (The layer is called as a module, with
+    its hooks; one whose class has a forward of its own, too.)
 
     The packed layer stays as it is (frozen, shared); `down` [adapters, rank, in_features] and `up` [adapters, rank, out_features] are
     parameters of `dtype` (fp16 or bf16), in which x is taken and the result is returned.  `scaling` is a buffer, [adapters].  New adapters
@@ -166,8 +167,14 @@ class AdaptedLinear(nn.Module):
     def forward(self, x, index):
         layer, dtype = self.layer, self.down.dtype
         x = x.to(dtype)
-        base = QuantizedLinearFunction.apply(x, layer.qweight, layer.scale, layer.zero_point, layer.bias, layer.bits, layer.group_size, dtype)
-        in_place = not (torch.is_grad_enabled() and (base.requires_grad or self.down.requires_grad or self.up.requires_grad))
+        if type(layer).forward is QuantizedLinear.forward and "forward" not in layer.__dict__:
+            base = layer(x, out_dtype=dtype)
+            # (what a hook has seen, or given, is not written over)
+            in_place = not (layer._forward_hooks or nn.modules.module._global_forward_hooks)
+        else:                                      # a layer with a forward of its own
+            base, in_place = layer(x), False
+        base = base.to(dtype)
+        in_place = in_place and not (torch.is_grad_enabled() and (base.requires_grad or self.down.requires_grad or self.up.requires_grad))
         return adapter_matmul(x, self.down, self.up, index, scaling=self.scaling.float(), base=base, out=base if in_place else None)
 
     def extra_repr(self):

@@ -73,11 +73,13 @@ class QuantizedLinear(nn.Module):
         else:
             self.bias = None
 
-    def forward(self, x):
-        # extension: set layer.out_dtype = torch.bfloat16.  (Where only nn.Module's own look-up is left, whose answer
+    def forward(self, x, out_dtype=None):
+        # extension: set layer.out_dtype = torch.bfloat16, or say so for one call.  (Where only nn.Module's own look-up is left, whose answer
         # to a missing name is an exception, it is not asked.)
-        out_dtype, cls = None, type(self)
-        if "out_dtype" in self.__dict__ or hasattr(cls, "out_dtype") or cls.__getattr__ is not nn.Module.__getattr__ \
+        cls = type(self)
+        if out_dtype is not None:
+            out_dtype = None if out_dtype is torch.float16 else out_dtype
+        elif "out_dtype" in self.__dict__ or hasattr(cls, "out_dtype") or cls.__getattr__ is not nn.Module.__getattr__ \
                 or cls.__getattribute__ is not nn.Module.__getattribute__:
             out_dtype = getattr(self, "out_dtype", None)
         if out_dtype is None:

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from bitween_b200 import adapter_matmul
+from bitween_b200 import AdaptedLinear, QuantizedLinear, adapter_matmul
 from bitween_b200.kernels import _lib
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +87,60 @@ def test_saved_tensors_that_hooks_have_moved_or_packed(native, monkeypatch):
     for other in (lambda t: t.cpu(), lambda t: t.double(), lambda t: t.flatten(), lambda t: t[:1], lambda t: t.bfloat16() if t.dtype == torch.float16 else t):
         with pytest.raises(RuntimeError, match="come back from its hooks"):
             gradients(hooks(lambda t: t.clone(), other))
+
+
+def _adapted(dtype, layer_class=QuantizedLinear):
+    lin = torch.nn.Linear(128, 256, bias=True).to(DEV)
+    with torch.no_grad():
+        lin.weight.copy_(torch.randn(256, 128, generator=_gen(5), device=DEV) * 0.05)
+        lin.bias.copy_(torch.randn(256, generator=_gen(6), device=DEV) * 0.05)
+    adapted = AdaptedLinear(layer_class.from_float(lin, bits=4, group_size=64), 2, 8, dtype=dtype)
+    with torch.no_grad():
+        adapted.down.copy_(torch.randn(adapted.down.shape, generator=_gen(7), device=DEV) * 0.1)
+        adapted.up.copy_(torch.randn(adapted.up.shape, generator=_gen(8), device=DEV) * 0.1)
+    return adapted, torch.randn(5, 128, generator=_gen(9), device=DEV).to(dtype), torch.tensor([0, 1, -1, 0, 1], dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("recording", [True, False])
+def test_adapted_linear_calls_its_layer(dtype, recording):
+    """Hooks of the wrapped layer see its input and output, may change the output, and what they keep stays as it was."""
+    adapted, x, index = _adapted(dtype)
+    seen = []
+    with torch.set_grad_enabled(recording):
+        want = adapted(x, index).detach()
+        base = adapted.layer(x, out_dtype=dtype).detach()
+        pre = adapted.layer.register_forward_pre_hook(lambda m, args: seen.append(args[0]))
+        post = adapted.layer.register_forward_hook(lambda m, args, out: seen.append(out))
+        assert torch.equal(adapted(x, index).detach(), want)
+        assert len(seen) == 2 and torch.equal(seen[0], x) and torch.equal(seen[1].detach(), base)
+        pre.remove()
+        post.remove()
+        twice = adapted.layer.register_forward_hook(lambda m, args, out: out * 2)
+        doubled = adapted(x, index).detach()
+        twice.remove()
+        assert torch.equal(doubled, adapter_matmul(x, adapted.down.detach(), adapted.up.detach(), index, scaling=adapted.scaling, base=base * 2))
+        adapted.layer.out_dtype = torch.float32                       # (the layer's own setting is for its own callers)
+        assert torch.equal(adapted(x, index).detach(), want) and want.dtype == dtype
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_adapted_linear_with_a_layer_that_has_a_forward_of_its_own(dtype):
+    class Halved(QuantizedLinear):
+        def forward(self, x):
+            return super().forward(x) * 0.5
+
+    adapted, x, index = _adapted(dtype, Halved)
+    with torch.no_grad():
+        got = adapted(x, index)
+        assert torch.equal(got, adapter_matmul(x, adapted.down, adapted.up, index, scaling=adapted.scaling, base=adapted.layer(x).to(dtype)))
+        adapted.layer.forward = lambda x: torch.zeros(*x.shape[:-1], 256, dtype=dtype, device=DEV)
+        assert torch.equal(adapted(x, index), adapter_matmul(x, adapted.down, adapted.up, index, scaling=adapted.scaling))
+
+
+def test_adapted_linear_takes_the_native_way_where_nothing_is_recorded(monkeypatch):
+    adapted, x, index = _adapted(torch.float16)
+    with torch.no_grad():
+        want = adapted(x, index)
+        monkeypatch.setattr("bitween_b200.modules.QuantizedLinearFunction.apply", None)
+        assert torch.equal(adapted(x, index), want)
