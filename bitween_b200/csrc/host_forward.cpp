@@ -4,7 +4,7 @@
 // First QuantizedLinear's forward where no gradient is recorded: in Python the autograd function (7.5 us), the checks, torch.empty
 // and the foreign call took 21 us a layer.
 //
-// forward(x, qweight, scale, zero_point, bias, bits, group_size) returns the fp16 output, or None for every call that
+// forward(x, qweight, scale, zero_point, bias, bits, group_size[, dtype code]) returns the output (fp16, or bf16 where asked for), or None for every call that
 // is not plain: the caller then goes through QuantizedLinearFunction, which converts, records, or raises.  Plain means
 // exact torch tensors on the current CUDA device, contiguous and of their final types, no input that gradients are
 // recorded for, no forward-mode tangent, and no tracing, dispatch or function mode and no function transform in force.
@@ -68,15 +68,17 @@ bool modes_active() {
 
 PyObject *forward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
-    if (nargs != 7) {
-        PyErr_SetString(PyExc_TypeError, "forward(x, qweight, scale, zero_point, bias, bits, group_size)");
+    if (nargs != 7 && nargs != 8) {
+        PyErr_SetString(PyExc_TypeError, "forward(x, qweight, scale, zero_point, bias, bits, group_size[, dtype code])");
         return nullptr;
     }
     const at::Tensor *x = tensor_of(args[0]), *q = tensor_of(args[1]), *s = tensor_of(args[2]), *z = tensor_of(args[3]), *b = nullptr;
     if (!x || !q || !s || !z || !g_qmatmul || !PyLong_CheckExact(args[5]) || !PyLong_CheckExact(args[6])) Py_RETURN_NONE;
     if (args[4] != Py_None && !(b = tensor_of(args[4]))) Py_RETURN_NONE;
-    const long bits = PyLong_AsLong(args[5]), group = PyLong_AsLong(args[6]);
+    if (nargs == 8 && !PyLong_CheckExact(args[7])) Py_RETURN_NONE;
+    const long bits = PyLong_AsLong(args[5]), group = PyLong_AsLong(args[6]), out_code = nargs == 8 ? PyLong_AsLong(args[7]) : BW_F16;
     if (PyErr_Occurred()) { PyErr_Clear(); Py_RETURN_NONE; }
+    if (out_code != BW_F16 && out_code != BW_BF16) Py_RETURN_NONE;
     if ((bits != 2 && bits != 4 && bits != 8) || group < 1 || group > 1 << 30 || modes_active()) Py_RETURN_NONE;
 
     const c10::Device device = x->device();
@@ -106,9 +108,9 @@ PyObject *forward(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         pybind11::gil_scoped_release no_gil;
         c10::SmallVector<int64_t, 5> sizes(x->sizes().begin(), x->sizes().end());
         sizes.back() = N;
-        out = at::empty(sizes, at::TensorOptions().dtype(at::kHalf).device(device));
+        out = at::empty(sizes, at::TensorOptions().dtype(out_code == BW_F16 ? at::kHalf : at::kBFloat16).device(device));
         rc = g_qmatmul(x->const_data_ptr(), x_code, M, N, K, static_cast<const int32_t *>(q->const_data_ptr()),
-                       s->const_data_ptr(), z->const_data_ptr(), b ? b->const_data_ptr() : nullptr, out.mutable_data_ptr(), BW_F16,
+                       s->const_data_ptr(), z->const_data_ptr(), b ? b->const_data_ptr() : nullptr, out.mutable_data_ptr(), (int)out_code,
                        (int)bits, (int)group, scratch.defined() ? scratch.mutable_data_ptr() : nullptr,
                        scratch.defined() ? (size_t)scratch.numel() : 0, stream);
     }

@@ -78,6 +78,10 @@ class QuantizedLinear(nn.Module):
         # to a missing name is an exception, it is not asked.)
         cls = type(self)
         if out_dtype is not None:
+            if out_dtype is torch.bfloat16 and type(x) is torch.Tensor and x.is_cuda:
+                y = (_lib._host or _lib.host_forward())(x, self.qweight, self.scale, self.zero_point, self.bias, self.bits, self.group_size, _lib.BF16)
+                if y is not None:
+                    return y
             out_dtype = None if out_dtype is torch.float16 else out_dtype
         elif "out_dtype" in self.__dict__ or hasattr(cls, "out_dtype") or cls.__getattr__ is not nn.Module.__getattr__ \
                 or cls.__getattribute__ is not nn.Module.__getattribute__:

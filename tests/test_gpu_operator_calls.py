@@ -138,8 +138,9 @@ def test_adapted_linear_with_a_layer_that_has_a_forward_of_its_own(dtype):
         assert torch.equal(adapted(x, index), adapter_matmul(x, adapted.down, adapted.up, index, scaling=adapted.scaling))
 
 
-def test_adapted_linear_takes_the_native_way_where_nothing_is_recorded(monkeypatch):
-    adapted, x, index = _adapted(torch.float16)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_adapted_linear_takes_the_native_way_where_nothing_is_recorded(dtype, monkeypatch):
+    adapted, x, index = _adapted(dtype)
     with torch.no_grad():
         want = adapted(x, index)
         monkeypatch.setattr("bitween_b200.modules.QuantizedLinearFunction.apply", None)
