@@ -90,6 +90,11 @@ template <> struct Pair<__half> {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
+    // d = a * b
+    static __device__ __forceinline__ void mma_new(float (&d)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    }
 };
 template <> struct Pair<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t *>(&h); }
@@ -97,6 +102,11 @@ template <> struct Pair<__nv_bfloat16> {
     static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    // d = a * b
+    static __device__ __forceinline__ void mma_new(float (&d)[4], const uint32_t *a, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                     : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
     }
 };
 // (From L2, as all that a kernel before may have written: the SM's L1 may hold lines from before this kernel's start, at which they were still being written.)
@@ -399,16 +409,27 @@ __global__ void __launch_bounds__(128) adapter_shrink_kernel(const T *__restrict
             const uint32_t at = ring + stage * STAGE;
             stage = stage + 1 == STAGES ? 0 : stage + 1;
             if (busy) {
+                uint32_t xa[4][4];
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    uint32_t xa[4];
-                    load_matrices(at + (x_place ^ kk * 32), xa);
+                for (int kk = 0; kk < 4; ++kk) load_matrices(at + (x_place ^ kk * 32), xa[kk]);
+                // (sums of 64 columns, added up in fp32: an MMA truncates what it adds to, which is a bias of 2^-24 of the sum each time)
 #pragma unroll
-                    for (int nb = 0; nb < NBR; nb += 2) {
+                for (int nb = 0; nb < NBR; nb += 2) {
+                    float some[2][4];
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
                         uint32_t b[4];                                   // (rank 8: the second pair is the first again)
                         load_matrices(at + (w_place ^ kk * 32) + nb * 1024, b);
-                        Pair<T>::mma(acc[nb], xa, b[0], b[1]);
-                        if (nb + 1 < NBR) Pair<T>::mma(acc[nb + 1 < NBR ? nb + 1 : nb], xa, b[2], b[3]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (nb + i >= NBR) continue;
+                            else if (kk == 0) Pair<T>::mma_new(some[i], xa[kk], b[2 * i], b[2 * i + 1]);
+                            else Pair<T>::mma(some[i], xa[kk], b[2 * i], b[2 * i + 1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        acc[nb][e] += some[0][e];
+                        if (nb + 1 < NBR) acc[nb + 1 < NBR ? nb + 1 : nb][e] += some[1][e];
                     }
                 }
             }
@@ -887,11 +908,11 @@ __global__ void __launch_bounds__(EU_THREADS, 1) adapter_expand_umma_kernel(void
                 umma::tc_fence_after();
                 const uint32_t at = ring + slot * S::STAGE;
 #pragma unroll
-                for (int part = 0; part < PARTS<T>; ++part)
+                for (int part = PARTS<T> - 1; part >= 0; --part)          // (the smallest first: each MMA truncates what it adds to)
 #pragma unroll
                     for (int k = 0; k < KS; ++k)
                         umma::umma_f16_ts(tmem + acc * EU_COLS, tmem + 2 * EU_COLS + (part * KS + k) * 8, umma::umma_smem_desc_mn(at + k * 2048, S::W_BLOCK), idesc,
-                                          (part | k) != 0 ? 1u : 0u);
+                                          part != PARTS<T> - 1 || k != 0 ? 1u : 0u);
                 umma::umma_commit(&acc_full[acc]);
             }
         }
@@ -1166,21 +1187,35 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
                     }
                 }
 #pragma unroll
-                for (int rb = 0; rb < RB; ++rb)
+                for (int rb = 0; rb < RB; ++rb) {
+                    uint32_t ha[PARTS<T>][4];
 #pragma unroll
                     for (int part = 0; part < PARTS<T>; ++part) {
-                        uint32_t ha[4];
-                        load_matrices_transposed(h_at + h_place[rb] + (part * OUTER_STEP + step * 16) * S::ROW, ha);
+                        load_matrices_transposed(h_at + h_place[rb] + (part * OUTER_STEP + step * 16) * S::ROW, ha[part]);
                         if constexpr (F16) {
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
-                                const __half2 y = __hmul2(__hmul2(*reinterpret_cast<const __half2 *>(&ha[k]), scale[k / 2]), more[k / 2]);
-                                ha[k] = *reinterpret_cast<const uint32_t *>(&y);
+                                const __half2 y = __hmul2(__hmul2(*reinterpret_cast<const __half2 *>(&ha[part][k]), scale[k / 2]), more[k / 2]);
+                                ha[part][k] = *reinterpret_cast<const uint32_t *>(&y);
                             }
                         }
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) Pair<T>::mma(acc[rb][j], ha, b[j][0], b[j][1]);
                     }
+                    // (the parts' products of 16 tokens, from the smallest on, then added in fp32: an MMA truncates what it adds to, a bias of 2^-24 of the sum each time)
+#pragma unroll
+                    for (int j0 = 0; j0 < 8; j0 += 4) {
+                        float some[4][4];
+#pragma unroll
+                        for (int part = PARTS<T> - 1; part >= 0; --part)
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (part == PARTS<T> - 1) Pair<T>::mma_new(some[j], ha[part], b[j0 + j][0], b[j0 + j][1]);
+                                else Pair<T>::mma(some[j], ha[part], b[j0 + j][0], b[j0 + j][1]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[rb][j0 + j][e] += some[j][e];
+                    }
+                }
             }
             if (wr != 0) copy_stage(first + (S::STAGES - 1) * OUTER_STEP, refill);
         }
@@ -1207,6 +1242,8 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 // rests of 64 ranks are the two halves of the M dimension, so that one MMA multiplies both; their sums meet at the end.  Eight warps fill the ring with
 // 16-byte cp.async of rows that a list names, one warp issues the MMAs.  Between them stand pairs of warps, a stage each in turn: for fp16 one pair, which brings the rows' powers
 // of two into the rank values, for bf16 three, which split the fp32 rank values into parts behind the ring.  The third part takes MMAs of its own, with zeros as the other half.
+// Stages go to two sets of sums in turn: an MMA truncates what it adds up, a bias toward zero that grows with the number of MMAs into one sum.  (4096 tokens an adapter, 14336 columns:
+// bf16 gradients differ from the exact ones' roundings by 1.0e-4 of their 2-norm, with one set and the third part in the values' half by 2.2e-4, fp32 torch's by 0.7e-4.)
 // (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between the copies and themselves, waits for all that its own thread has in flight: 86 us
 // instead of 76.)  Bound by the rows of x and the rank values, which every 256 columns read again, and by shared memory: 8192 tokens of 1 adapter, 14336 columns, rank 64, on the
 // 112 SMs that there are CTAs for: bf16 93 us (in two parts that came as such 73; one pair of warps 113, two 105, four 93; parts in tensor memory, a rank a lane, 101).
@@ -1214,9 +1251,9 @@ constexpr int OU_LIST = 1024, OU_WINDOW = 512;
 template <typename T> struct OuterUmma {
     static constexpr int BLOCK = OUTER_STEP * 128, A = 2 * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 6;
     static constexpr int PAIRS = PARTS<T> == 2 ? 1 : 3, THREADS = 288 + 64 * PAIRS;                             // pairs of warps that work on rank values, a stage each in turn
-    static constexpr int SPLIT = STAGES * STAGE, ZEROS = SPLIT + (PARTS<T> == 3 ? PAIRS * 3 * BLOCK : 0);      // bf16: their parts, and zeros, behind the ring
-    static constexpr int SMEM = ZEROS + (PARTS<T> == 3 ? BLOCK : 0) + 1024;
-    static_assert(64 * SUM_ROW * 4 <= SPLIT, "the sums take the ring's place");
+    static constexpr int ZEROS = STAGES * STAGE, SPLIT = ZEROS + (PARTS<T> == 3 ? BLOCK : 0);                  // bf16: zeros, and the rank values' parts, behind the ring
+    static constexpr int SMEM = SPLIT + (PARTS<T> == 3 ? PAIRS * 3 * BLOCK : 0) + 1024;
+    static_assert(64 * SUM_ROW * 4 <= ZEROS, "the sums take the ring's place");
 };
 template <typename T>
 __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
@@ -1226,7 +1263,7 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
     const int rank_blocks = (p.rank + 63) / 64, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * 64;
     const int64_t col0 = (int64_t)blockIdx.x * 256;
     extern __shared__ uint8_t raw_smem[];
-    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [STAGES][rank values | 4 blocks of columns][tokens][128 B]; bf16: [PAIRS][parts][tokens][128 B]; zeros
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [STAGES][rank values | 4 blocks of columns][tokens][128 B]; bf16: zeros; [PAIRS][parts][tokens][128 B]
     float *sums = reinterpret_cast<float *>(smem);                                      // [64][SUM_ROW], at the end
     __shared__ int list[OU_LIST + OUTER_STEP], s_before[OU_WINDOW], s_count[8], s_end[S::STAGES], s_abort;
     __shared__ uint32_t s_bits[OU_WINDOW], s_tmem;
@@ -1251,7 +1288,7 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
         for (int i = threadIdx.x; i < S::BLOCK / 16; i += S::THREADS) reinterpret_cast<uint4 *>(smem + S::ZEROS)[i] = make_uint4(0, 0, 0, 0);
         umma::fence_proxy_async_smem();
     }
-    if (warp == 8) umma::tmem_alloc(&s_tmem, 256);
+    if (warp == 8) umma::tmem_alloc(&s_tmem, 512);
     umma::tc_fence_before();
     __syncthreads();
     umma::tc_fence_after();
@@ -1275,14 +1312,15 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
             }
             umma::fence_proxy_async_smem();
             umma::tc_fence_after();
+            const uint32_t sum = tmem + (stages & 1) * 256;
             const uint32_t at = ring + slot * S::STAGE, values = F16 ? at : ring + S::SPLIT + stages % S::PAIRS * 3 * S::BLOCK;
 #pragma unroll
             for (int k = 0; k < OUTER_STEP / 16; ++k) {
                 const uint64_t columns = umma::umma_smem_desc_mn(at + S::A + k * 2048, S::BLOCK);
-                umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(values + k * 2048, S::BLOCK), columns, idesc, (stages | k) != 0 ? 1u : 0u);
-                // (the third part above a block of zeros)
+                umma::umma_f16_ss(sum, umma::umma_smem_desc_mn(values + k * 2048, S::BLOCK), columns, idesc, (stages / 2 | k) != 0 ? 1u : 0u);
+                // (the third part to the rests' half, below a block of zeros)
                 if constexpr (!F16)
-                    umma::umma_f16_ss(tmem, umma::umma_smem_desc_mn(values + 2 * S::BLOCK + k * 2048, ring + S::ZEROS - (values + 2 * S::BLOCK)), columns, idesc, 1u);
+                    umma::umma_f16_ss(sum, umma::umma_smem_desc_mn(ring + S::ZEROS + k * 2048, values + 2 * S::BLOCK - (ring + S::ZEROS)), columns, idesc, 1u);
             }
             umma::umma_commit(&empty[slot]);
         }
@@ -1437,6 +1475,12 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
                 for (int cb = 0; cb < 256; cb += 32) {
                     uint32_t r[32] = {};
                     if (alive && stages) umma::tmem_ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + cb, r);
+                    if (alive && stages > 1) {
+                        uint32_t odd[32];
+                        umma::tmem_ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + 256 + cb, odd);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) + __uint_as_float(odd[k]));
+                    }
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
                         float4 v = make_float4(__uint_as_float(r[k]), __uint_as_float(r[k + 1]), __uint_as_float(r[k + 2]), __uint_as_float(r[k + 3]));
@@ -1459,7 +1503,7 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
     if (*abort_flag == 0) join_sums<T, S::THREADS, 64>(sums, p, a, rank0, col0, dw);
     cluster.sync();                                              // a CTA's sums stay until the others have read them
     umma::tc_fence_after();
-    if (warp == 8) umma::tmem_dealloc(tmem, 256);
+    if (warp == 8) umma::tmem_dealloc(tmem, 512);
 }
 
 // ---- host side -------------------------------------------------------------------------------------------------------

@@ -180,3 +180,39 @@ def test_gradients_of_many_tokens_and_a_rank_that_is_no_multiple_of_eight():
         xd, gd, dd, ud = x[t].double(), grad[t].double(), down[a].detach().double(), up[a].detach().double()
         _check(got[0][a], (gd @ ud.T).T @ xd, (gd.abs() @ ud.T.abs()).T @ xd.abs())
         _check(got[1][a], (xd @ dd.T).T @ gd, (xd.abs() @ dd.T.abs()).T @ gd.abs())
+
+
+# Long sums of positive products.  An MMA truncates the sum that it adds to, by up to 2^-23 of it: a bias that grows with the sum's length, where roundings to nearest mostly cancel
+# (n of them, independent and of at most 2^-24 of a sum that grows evenly: a standard deviation of 2^-24 / 3 * sqrt(n)).
+@pytest.mark.parametrize("M,n,r", [(40, 2, 16), (300, 2, 8), (300, 1, 64), (1100, 1, 128)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_rank_values_of_long_rows(M, n, r, dtype):
+    """14336 columns: 14 MMAs of a warp in a row (up to 64 tokens) or four and up to 224 fp32 additions (six deviations: 2^-19), and 15 additions of parts: 2^-18.5 in all."""
+    K, N = 14336, 1024
+    index = torch.randint(0, n, (M,), generator=_gen(51), device=DEV).sort().values.to(torch.int32)
+    x, down, up = (_rand(s, i + 52).to(dtype) for i, s in enumerate(((M, K), (n, r, K), (n, r, N))))
+    down *= 2.0 ** -10
+    up = torch.where((torch.arange(r, device=DEV) == 3)[:, None], up, 0)
+    want = torch.einsum("tk,tk->t", x.double(), down[:, 3].double()[index.long()])[:, None] * up[:, 3].double()[index.long()]
+    bad = _outside(adapter_matmul(x, down, up, index), want, 2.0 ** -18.5 * want)
+    assert bad == 0, f"{bad} of {want.numel()}"
+
+
+@pytest.mark.parametrize("M,r,N,bound", [
+    # tcgen05, a CTA for all tokens: 128 MMAs into each of two sums that grow evenly.  Each aligns 16 products and the sum to the largest of them and drops what lies below its
+    # 24 bits: up to 17 * 2^-23 of the sum, of one sign where the products have one; 17 * 64 * 2^-23 in all.
+    (4096, 64, 37888, 17 * 2.0 ** -17),
+    (8192, 16, 1024, 2.0 ** -18.5),        # mma.sync: 16 tokens' products (three truncations), then up to 512 fp32 additions (six deviations: 2^-18.6)
+    (8192, 8, 520, 2.0 ** -18.5),
+    (480, 64, 1024, 2.0 ** -18.5)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gradients_of_banks_summed_over_many_tokens(M, r, N, bound, dtype):
+    K = 64
+    index = torch.zeros(M, dtype=torch.int32, device=DEV)
+    x, down, up, grad = (_rand(s, i + 62).to(dtype) for i, s in enumerate(((M, K), (1, r, K), (1, r, N), (M, N))))
+    x *= 2.0 ** -9
+    up.requires_grad_()
+    (dup,) = torch.autograd.grad(adapter_matmul(x, down, up, index), (up,), grad)
+    want = (x.double() @ down[0].double().T).T @ grad.double()
+    bad = _outside(dup[0], want, (bound + 2.0 ** -20) * want)          # (2^-20: the rank values themselves, of 64 products)
+    assert bad == 0, f"{bad} of {want.numel()}"
