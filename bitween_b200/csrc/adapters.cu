@@ -153,11 +153,15 @@ struct AdapterArgs {
     bool behind;                // another launch of this call comes before: all that came before that is done when this one starts
 };
 
-// Rank values.  bf16: fp32 [M][rank].  fp16: [2][M][rank], values and their rests, and [M] powers of two by which both were divided.
+// Rank values.  bf16: fp32 [M][rank], and of many tokens their parts [3][M][rank] as well, for outer on tcgen05.  fp16: [2][M][rank], values and their rests, and [M] powers of
+// two by which both were divided.
+constexpr int64_t MANY = 512;
 template <typename T> constexpr int PARTS = __is_same(T, __half) ? 2 : 3;
 template <typename T> struct Hidden {
     float *sum;
-    __host__ __device__ Hidden(void *p, int64_t, int) : sum((float *)p) {}
+    T *parts;
+    int64_t size;             // of a part
+    __host__ __device__ Hidden(void *p, int64_t M, int r) : sum((float *)p), parts(reinterpret_cast<T *>(sum + M * r)), size(M * r) {}
 };
 template <> struct Hidden<__half> {
     __half *top, *rest;
@@ -276,7 +280,15 @@ __device__ __forceinline__ void finish_rows(float *sums, int rows, int row0, int
 #pragma unroll
             for (int i = 0; i < PAIRS; ++i) {
                 const int j = 2 * (lane + 32 * i);
-                if (j < p.rank) *reinterpret_cast<float2 *>(h.sum + t * p.rank + j) = v[i];
+                if (j < p.rank) {
+                    *reinterpret_cast<float2 *>(h.sum + t * p.rank + j) = v[i];
+                    if (p.M >= MANY) {
+                        uint32_t parts[3];
+                        split<T>(v[i], parts);
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) *reinterpret_cast<uint32_t *>(h.parts + k * h.size + t * p.rank + j) = parts[k];
+                    }
+                }
             }
         }
     }
@@ -1240,8 +1252,11 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 // The same on tcgen05, for adapters of many tokens: 64 ranks x 256 columns a CTA, reduced over tokens, 32 a stage.  Rows of x and of the rank values keep
 // the order in which memory holds them, which is the MN-major form of both operands (blocks of 64 elements by 32 tokens, 128-byte swizzle).  Values and
 // rests of 64 ranks are the two halves of the M dimension, so that one MMA multiplies both; their sums meet at the end.  Eight warps fill the ring with
-// 16-byte cp.async of rows that a list names, one warp issues the MMAs.  Between them stand pairs of warps, a stage each in turn: for fp16 one pair, which brings the rows' powers
-// of two into the rank values, for bf16 three, which split the fp32 rank values into parts behind the ring.  The third part takes MMAs of its own, with zeros as the other half.
+// 16-byte cp.async of rows that a list names, one warp issues the MMAs; for fp16 two warps between them bring the rows' powers of two into the rank
+// values.  The third part of bf16 takes MMAs of its own, with zeros as the other half.  (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between
+// the copies and themselves, waits for all that its own thread has in flight: 86 us instead of 76.)  Bound by the rows of x and the rank values, which every 256 columns read
+// again: 8192 tokens, 14336 columns, rank 64, on the 112 SMs that there are CTAs for: bf16 80 us (in two parts 73, mma.sync 129; fp32 rank values split on the way by one pair of warps
+// 113, by three 93, into tensor memory 101; sixteen copying warps: the same, and 2 us more to begin).
 // Stages go to two sets of sums in turn: an MMA truncates what it adds up, a bias toward zero that grows with the number of MMAs into one sum.  (4096 tokens an adapter, 14336 columns:
 // bf16 gradients differ from the exact ones' roundings by 1.0e-4 of their 2-norm, with one set and the third part in the values' half by 2.2e-4, fp32 torch's by 0.7e-4.)
 // (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between the copies and themselves, waits for all that its own thread has in flight: 86 us
@@ -1249,11 +1264,9 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 // 112 SMs that there are CTAs for: bf16 93 us (in two parts that came as such 73; one pair of warps 113, two 105, four 93; parts in tensor memory, a rank a lane, 101).
 constexpr int OU_LIST = 1024, OU_WINDOW = 512;
 template <typename T> struct OuterUmma {
-    static constexpr int BLOCK = OUTER_STEP * 128, A = 2 * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 6;
-    static constexpr int PAIRS = PARTS<T> == 2 ? 1 : 3, THREADS = 288 + 64 * PAIRS;                             // pairs of warps that work on rank values, a stage each in turn
-    static constexpr int ZEROS = STAGES * STAGE, SPLIT = ZEROS + (PARTS<T> == 3 ? BLOCK : 0);                  // bf16: zeros, and the rank values' parts, behind the ring
-    static constexpr int SMEM = SPLIT + (PARTS<T> == 3 ? PAIRS * 3 * BLOCK : 0) + 1024;
-    static_assert(64 * SUM_ROW * 4 <= ZEROS, "the sums take the ring's place");
+    static constexpr int BLOCK = OUTER_STEP * 128, A = PARTS<T> * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 7, THREADS = 352;
+    static constexpr int RING = PARTS<T> == 3 ? BLOCK : 0, SMEM = RING + STAGES * STAGE + 1024;                 // bf16: a block of zeros in front of the ring
+    static_assert(64 * SUM_ROW * 4 <= STAGES * STAGE, "the sums take the ring's place");
 };
 template <typename T>
 __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
@@ -1263,7 +1276,7 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
     const int rank_blocks = (p.rank + 63) / 64, a = blockIdx.y / rank_blocks, rank0 = blockIdx.y % rank_blocks * 64;
     const int64_t col0 = (int64_t)blockIdx.x * 256;
     extern __shared__ uint8_t raw_smem[];
-    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // [STAGES][rank values | 4 blocks of columns][tokens][128 B]; bf16: zeros; [PAIRS][parts][tokens][128 B]
+    uint8_t *smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);      // bf16: zeros; [STAGES][parts of the rank values | 4 blocks of columns][tokens][128 B]
     float *sums = reinterpret_cast<float *>(smem);                                      // [64][SUM_ROW], at the end
     __shared__ int list[OU_LIST + OUTER_STEP], s_before[OU_WINDOW], s_count[8], s_end[S::STAGES], s_abort;
     __shared__ uint32_t s_bits[OU_WINDOW], s_tmem;
@@ -1285,7 +1298,7 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
         umma::fence_proxy_async_smem();
     }
     if constexpr (PARTS<T> == 3) {
-        for (int i = threadIdx.x; i < S::BLOCK / 16; i += S::THREADS) reinterpret_cast<uint4 *>(smem + S::ZEROS)[i] = make_uint4(0, 0, 0, 0);
+        for (int i = threadIdx.x; i < S::BLOCK / 16; i += S::THREADS) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
         umma::fence_proxy_async_smem();
     }
     if (warp == 8) umma::tmem_alloc(&s_tmem, 512);
@@ -1302,10 +1315,10 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
         // ---- products ----
         if (p.behind) pdl_wait();
         const uint32_t idesc = umma::umma_idesc_f16(256, !F16, true) | 1u << 16;      // (B MN-major as well)
-        const uint32_t ring = smem_addr(smem);
+        const uint32_t zeros = smem_addr(smem), ring = zeros + S::RING;
         for (;; ++stages) {
             const int slot = stages % S::STAGES;
-            if (!__all_sync(0xffffffffu, umma::mbar_wait(&scaled[slot], stages / S::STAGES & 1, abort_flag, 1, &g_adapter_status))) break;
+            if (!__all_sync(0xffffffffu, umma::mbar_wait(F16 ? &scaled[slot] : &full[slot], stages / S::STAGES & 1, abort_flag, 1, &g_adapter_status))) break;
             if (*(volatile int *)&s_end[slot]) {
                 umma::umma_commit(&done);
                 break;
@@ -1313,61 +1326,43 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
             umma::fence_proxy_async_smem();
             umma::tc_fence_after();
             const uint32_t sum = tmem + (stages & 1) * 256;
-            const uint32_t at = ring + slot * S::STAGE, values = F16 ? at : ring + S::SPLIT + stages % S::PAIRS * 3 * S::BLOCK;
+            const uint32_t at = ring + slot * S::STAGE;
 #pragma unroll
             for (int k = 0; k < OUTER_STEP / 16; ++k) {
                 const uint64_t columns = umma::umma_smem_desc_mn(at + S::A + k * 2048, S::BLOCK);
-                umma::umma_f16_ss(sum, umma::umma_smem_desc_mn(values + k * 2048, S::BLOCK), columns, idesc, (stages / 2 | k) != 0 ? 1u : 0u);
+                umma::umma_f16_ss(sum, umma::umma_smem_desc_mn(at + k * 2048, S::BLOCK), columns, idesc, (stages / 2 | k) != 0 ? 1u : 0u);
                 // (the third part to the rests' half, below a block of zeros)
                 if constexpr (!F16)
-                    umma::umma_f16_ss(sum, umma::umma_smem_desc_mn(ring + S::ZEROS + k * 2048, values + 2 * S::BLOCK - (ring + S::ZEROS)), columns, idesc, 1u);
+                    umma::umma_f16_ss(sum, umma::umma_smem_desc_mn(zeros + k * 2048, at + 2 * S::BLOCK - zeros), columns, idesc, 1u);
             }
             umma::umma_commit(&empty[slot]);
         }
     } else if (warp > 8) {
-        // ---- fp16: rank values times their row's power of two; bf16: fp32 rank values in parts ----
+        // ---- fp16: rank values times their row's power of two ----
         if (p.behind) pdl_wait();
-        const int pair = (warp - 9) / 2, me = (warp - 9) % 2 * 32 + lane;
-        for (stages = pair;; stages += S::PAIRS) {
-            const int slot = stages % S::STAGES;
-            bool ok = umma::mbar_wait(&full[slot], stages / S::STAGES & 1, abort_flag, 5, &g_adapter_status);
-            // (the MMAs that took this pair's parts before are done)
-            if constexpr (!F16)
-                if (const int last = stages - S::PAIRS; last >= 0) ok = ok && umma::mbar_wait(&empty[last % S::STAGES], last / S::STAGES & 1, abort_flag, 6, &g_adapter_status);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            const bool end = *(volatile int *)&s_end[slot];
-            if (!end) {
-                uint8_t *stage = smem + slot * S::STAGE;
-                if constexpr (F16) {
+        if constexpr (F16)
+            for (;; ++stages) {
+                const int slot = stages % S::STAGES;
+                if (!__all_sync(0xffffffffu, umma::mbar_wait(&full[slot], stages / S::STAGES & 1, abort_flag, 5, &g_adapter_status))) break;
+                const bool end = *(volatile int *)&s_end[slot];
+                if (!end) {
 #pragma unroll
                     for (int i = 0; i < S::A / 16 / 64; ++i) {
-                        const int at = me + i * 64;      // of 16 bytes, eight a row
+                        const int at = (warp - 9) * 32 + lane + i * 64;      // of 16 bytes, eight a row
                         const float f = s_scale[slot][at / 8 % OUTER_STEP];
                         const __half2 scale = __float2half2_rn(fmaxf(f, 0x1p-24f)), more = __float2half2_rn(fminf(f * 0x1p24f, 1.0f));      // (powers below 2^-24 as well)
-                        uint4 *own = reinterpret_cast<uint4 *>(stage) + at, v = *own;
+                        uint4 *own = reinterpret_cast<uint4 *>(smem + S::RING + slot * S::STAGE) + at, v = *own;
                         __half2 *y = reinterpret_cast<__half2 *>(&v);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) y[k] = __hmul2(__hmul2(y[k], scale), more);
                         *own = v;
                     }
-                } else {
-                    uint8_t *to = smem + S::SPLIT + pair * 3 * S::BLOCK;
-#pragma unroll
-                    for (int i = 0; i < OUTER_STEP * 8 / 64; ++i) {
-                        const int at = me + i * 64, token = at / 8, piece = at % 8;      // of eight ranks
-                        const float4 *from = reinterpret_cast<const float4 *>(stage + token * 256);
-                        uint4 parts[3];
-                        split8<T>(from[(2 * piece) ^ (token & 7)], from[(2 * piece + 1) ^ (token & 7)], parts);
-#pragma unroll
-                        for (int part = 0; part < 3; ++part) *reinterpret_cast<uint4 *>(to + part * S::BLOCK + token * 128 + (piece ^ (token & 7)) * 16) = parts[part];
-                    }
+                    umma::fence_proxy_async_smem();
                 }
-                umma::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) umma::mbar_arrive(&scaled[slot]);
+                if (end) break;
             }
-            __syncwarp();
-            if (lane == 0) umma::mbar_arrive(&scaled[slot]);
-            if (end) break;
-        }
     } else {
         // ---- copies ----
         const auto meet = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
@@ -1395,25 +1390,16 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
         }
         f = big * (p.scaling ? __ldcg(p.scaling + a) : 1.0f);
 
-        // this thread's pieces: of rows warp, warp + 8, .. of x piece `lane`; of row threadIdx / 8 of the rank values pieces threadIdx % 8 of values and rests, or (fp32)
-        // that one and the one eight further on
-        const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0, token = threadIdx.x / 8, piece = threadIdx.x % 8;
-        const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0)), *h0[2];
-        const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * (F16 ? 2 : 4), ring = smem_addr(smem);
-        const uint32_t x_to = S::A + lane / 8 * S::BLOCK + warp * 128 + (lane % 8 ^ warp) * 16;
-        uint32_t h_to[2];
-        int h_bytes[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if constexpr (F16) {
-                h_bytes[i] = rank0 + piece * 8 < p.rank ? 16 : 0;
-                h0[i] = (const uint8_t *)((i ? h.rest : h.top) + (h_bytes[i] ? rank0 + piece * 8 : 0));
-                h_to[i] = i * S::BLOCK + token * 128 + (piece ^ (token & 7)) * 16;
-            } else {
-                h_bytes[i] = rank0 + (piece + 8 * i) * 4 < p.rank ? 16 : 0;
-                h0[i] = (const uint8_t *)(h.sum + (h_bytes[i] ? rank0 + (piece + 8 * i) * 4 : 0));
-                h_to[i] = token * 256 + ((piece + 8 * i) ^ (token & 7)) * 16;
-            }
+        // this thread's pieces: of rows warp, warp + 8, .. of x piece `lane`; of row threadIdx / 8 of the rank values' parts piece threadIdx % 8
+        const int x_bytes = col0 + lane * 8 < p.cols ? 16 : 0, token = threadIdx.x / 8, piece = threadIdx.x % 8, h_bytes = rank0 + piece * 8 < p.rank ? 16 : 0;
+        const uint8_t *xs0 = (const uint8_t *)(x + (x_bytes ? col0 + lane * 8 : 0));
+        const T *h0;
+        if constexpr (F16) h0 = h.top;
+        else h0 = h.parts;
+        h0 += h_bytes ? rank0 + piece * 8 : 0;
+        const int64_t part_size = p.M * p.rank;
+        const uint32_t x_row = (uint32_t)p.cols * 2, h_row = (uint32_t)p.rank * 2, ring = smem_addr(smem) + S::RING;
+        const uint32_t x_to = S::A + lane / 8 * S::BLOCK + warp * 128 + (lane % 8 ^ warp) * 16, h_to = token * 128 + (piece ^ (token & 7)) * 16;
         bool alive = true;                                       // (after a failed wait the loops go on without copies: the warps meet in them)
         int window = 0, passed = 0;
         for (int from = lo, n; from < hi; from += n) {
@@ -1446,7 +1432,8 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
                     const int at = first + token;
                     const uint64_t row = at < n ? (uint64_t)(uint32_t)list[at] * h_row : 0;
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) copy16(to + h_to[k], h0[k] + row, at < n ? h_bytes[k] : 0);
+                    for (int part = 0; part < PARTS<T>; ++part)
+                        copy16(to + h_to + part * S::BLOCK, (const uint8_t *)(h0 + part * part_size) + row, at < n ? h_bytes : 0);
                     if constexpr (F16)
                         if (piece == 0) s_scale[slot][token] = at < n ? s_back[at] : 0.0f;
                     copies_arrive(&full[slot]);
@@ -1455,15 +1442,13 @@ __global__ void __launch_bounds__(OuterUmma<T>::THREADS, 1) adapter_outer_umma_k
                 if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
             }
         }
-        // more stages, without tokens: the end, one for each pair
-        for (int i = 0; i < S::PAIRS; ++i) {
-            const int slot = (stages + i) % S::STAGES;
-            alive = alive && umma::mbar_wait(&empty[slot], ((stages + i) / S::STAGES & 1) ^ 1, abort_flag, 3, &g_adapter_status);
-            if (threadIdx.x == 0) *(volatile int *)&s_end[slot] = 1;
-            if (alive) copies_arrive(&full[slot]);
-            __syncwarp();
-            if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
-        }
+        // one more stage, without tokens: the end
+        const int slot = stages % S::STAGES;
+        alive = alive && umma::mbar_wait(&empty[slot], (stages / S::STAGES & 1) ^ 1, abort_flag, 3, &g_adapter_status);
+        if (threadIdx.x == 0) *(volatile int *)&s_end[slot] = 1;
+        if (alive) copies_arrive(&full[slot]);
+        __syncwarp();
+        if (lane == 0 && alive) umma::mbar_arrive(&full[slot]);
         asm volatile("cp.async.wait_all;" ::: "memory");
         // ---- sums of this CTA: tensor memory's lanes 0 to 63 are the values' ranks, 64 to 127 the rests' ----
         if (warp < 4) alive = __all_sync(0xffffffffu, umma::mbar_wait(&done, 0, abort_flag, 4, &g_adapter_status));
@@ -1685,6 +1670,7 @@ int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t s
     // 512 tokens 7.7 / 9.6; rank 16, 14336 columns, 8192 tokens 60 / 67.
     const int64_t rows = (int64_t)p.adapters * ((p.rank + 63) / 64);
     const bool at_once = (p.cols + 255) / 256 * rows <= SMS;
+    static_assert(MANY <= 512, "of fewer tokens the rank values have no parts");
     if (p.rank > 32 ? p.M >= 512 * rows || (at_once && p.M >= 512) : p.rank > 16 && at_once && p.M >= 2048) return outer_umma<T>(h, (const T *)x, p, (T *)dw, st);
     if (p.rank <= 16) return outer_fast<T, 1, 1>(h, (const T *)x, p, (T *)dw, st);
     if (p.rank <= 32) return outer_fast<T, 2, 1>(h, (const T *)x, p, (T *)dw, st);
@@ -1740,8 +1726,8 @@ int backward(const void *dy, const void *x, int64_t M, int64_t N, int64_t K, con
 
 }  // namespace
 
-// (two 16-bit parts and a power of two a row; fp32 values, of bf16 and of the general kernels, are less)
-size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * 4 + (size_t)M * 4; }
+// (two 16-bit parts and a power of two a row; fp32 values, of bf16 and of the general kernels, are less; three 16-bit parts more of many tokens of bf16)
+size_t adapter_hidden_bytes(int64_t M, int r) { return (size_t)M * r * (M >= MANY ? 10 : 4) + (size_t)M * 4; }
 
 int adapter_device_status() {
     int v = 0, zero = 0;
