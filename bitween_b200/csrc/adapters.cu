@@ -1259,9 +1259,6 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 // 113, by three 93, into tensor memory 101; sixteen copying warps: the same, and 2 us more to begin).
 // Stages go to two sets of sums in turn: an MMA truncates what it adds up, a bias toward zero that grows with the number of MMAs into one sum.  (4096 tokens an adapter, 14336 columns:
 // bf16 gradients differ from the exact ones' roundings by 1.0e-4 of their 2-norm, with one set and the third part in the values' half by 2.2e-4, fp32 torch's by 0.7e-4.)
-// (A warp with copies in flight does nothing else: a proxy fence, which the MMAs need between the copies and themselves, waits for all that its own thread has in flight: 86 us
-// instead of 76.)  Bound by the rows of x and the rank values, which every 256 columns read again, and by shared memory: 8192 tokens of 1 adapter, 14336 columns, rank 64, on the
-// 112 SMs that there are CTAs for: bf16 93 us (in two parts that came as such 73; one pair of warps 113, two 105, four 93; parts in tensor memory, a rank a lane, 101).
 constexpr int OU_LIST = 1024, OU_WINDOW = 512;
 template <typename T> struct OuterUmma {
     static constexpr int BLOCK = OUTER_STEP * 128, A = PARTS<T> * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 7, THREADS = 352;
