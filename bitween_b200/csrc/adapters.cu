@@ -1617,10 +1617,10 @@ int expand_umma(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaS
 template <typename T, int KS>
 int expand_fast(void *h, const T *w, AdapterArgs p, const T *base, T *out, cudaStream_t st) {
     // tcgen05 has one CTA an SM, whose start takes some microseconds.  Rank 64, bf16, shrink of 64 columns and expand, us, mma.sync / tcgen05: 8192 tokens of one
-    // adapter to 14336 columns 127 / 91, of 8 144 / 105; 8192 tokens to 4096 columns 49 / 36, 49 / 48; 2048 of one 19 / 17, of two 22 / 23; 1024 of one 14.7 / 13.6, to 1024 columns
-    // 9.3 / 11.9; rank 32, 8192 tokens of one to 14336 columns 99 / 91, of 8 in any order 370 / 488.
+    // adapter to 14336 columns 146 / 91, of 8 167 / 109; 8192 tokens to 4096 columns of one 57 / 37, of 8 57 / 50; 4096 of two to 4096 33.6 / 33.0, to 1024 16.8 / 18.5; 1024 of one to 4096
+    // 15.5 / 13.8, to 1024 10.1 / 12.3; 512 of one to 14336 20 / 15, of two 20 / 21.
     if constexpr (KS > 2)
-        if (p.M >= 1024 && p.M >= (int64_t)256 * p.adapters && p.M * p.cols >= (int64_t)(p.adapters == 1 ? 8 : 24) << 20) return expand_umma<T, KS>(h, w, p, base, out, st);
+        if (p.M >= 512 && p.M >= (int64_t)256 * p.adapters && p.M * p.cols >= (int64_t)(p.adapters == 1 ? 4 : 24) << 20) return expand_umma<T, KS>(h, w, p, base, out, st);
     constexpr int SMEM = (KS * 16 + TILE) * 128 * (KS <= 4 ? 4 : 3);
     p.slots = slots_of(p);
     if (p.M <= FEW)
@@ -1662,13 +1662,15 @@ int outer_umma(void *h, const T *x, const AdapterArgs &p, T *dw, cudaStream_t st
 }
 template <typename T>
 int outer(void *h, const void *x, const AdapterArgs &p, void *dw, cudaStream_t st) {
-    // tcgen05 has 64 ranks' work for any rank and one CTA an SM, mma.sync two or three of less.  bf16, us, mma.sync / tcgen05: rank 64, 14336 columns, 8192 tokens
-    // of one adapter 107 / 68, of 16 151 / 116; 512 tokens of 4096 columns of one 18 / 12, of 16 (256 CTAs) 10 / 15; rank 32, 1024 columns, 2048 tokens 13.3 / 12.9,
-    // 512 tokens 7.7 / 9.6; rank 16, 14336 columns, 8192 tokens 60 / 67.
+    // tcgen05 has 64 ranks' work for any rank and one CTA an SM, mma.sync two or three of less.  With shrink of 64 columns in front, us, mma.sync / tcgen05: bf16, rank 64, 14336 columns, 8192
+    // tokens of one adapter 174 / 74 (fp16 143 / 96), of 16 220 / 124; 512 tokens of 4096 columns of one 21 / 12, of 16 (256 CTAs) 11 / 17; 1024 of 16 14 / 18; rank 32, 1024 columns, 2048 tokens
+    // 17 / 14, 1024 tokens 11.7 / 11.8, 512 tokens 9.2 / 10.5; 1024 tokens of 4096 columns 16 / 13; 14336 columns, 8192 tokens of four 116 / 84, 512 tokens of four 13 / 19; rank 16, 14336
+    // columns, 8192 tokens 69 / 75 (fp16 70 / 94).
     const int64_t rows = (int64_t)p.adapters * ((p.rank + 63) / 64);
     const bool at_once = (p.cols + 255) / 256 * rows <= SMS;
     static_assert(MANY <= 512, "of fewer tokens the rank values have no parts");
-    if (p.rank > 32 ? p.M >= 512 * rows || (at_once && p.M >= 512) : p.rank > 16 && at_once && p.M >= 2048) return outer_umma<T>(h, (const T *)x, p, (T *)dw, st);
+    if (p.M >= 512 && (p.rank > 32 ? at_once || p.M > 64 * rows : p.rank > 16 && (at_once || p.M >= 512 * rows) && (p.M >= 2048 || p.M * p.cols >= (int64_t)4 << 20)))
+        return outer_umma<T>(h, (const T *)x, p, (T *)dw, st);
     if (p.rank <= 16) return outer_fast<T, 1, 1>(h, (const T *)x, p, (T *)dw, st);
     if (p.rank <= 32) return outer_fast<T, 2, 1>(h, (const T *)x, p, (T *)dw, st);
     return outer_fast<T, 2, 2>(h, (const T *)x, p, (T *)dw, st);

@@ -34,6 +34,10 @@ def _ran(M, K, N, n, r, dtype):
     (7, 100, 130, 3, 5, torch.float16, ["expand_general", "expand_general", "outer_general", "outer_general"]),
     (40, 4096, 96, 2, 1, torch.bfloat16, ["expand_general", "expand_general", "outer_general", "outer_general"]),
     (33, 8, 128, 2, 256, torch.bfloat16, ["expand_general", "expand_general", "outer_general", "outer_general"]),
+    (512, 4096, 4096, 16, 64, torch.bfloat16, ["expand", "expand", "outer", "outer"]),
+    (512, 4096, 14336, 1, 64, torch.bfloat16, ["expand_umma", "expand", "outer_umma", "outer_umma"]),
+    (1024, 1024, 4096, 1, 32, torch.float16, ["expand", "expand", "outer", "outer_umma"]),
+    (8192, 64, 1024, 1, 16, torch.bfloat16, ["expand", "expand", "outer", "outer"]),
     # sums over many tokens on tcgen05
     (512, 64, 264, 1, 64, torch.bfloat16, ["expand", "expand", "outer_umma", "outer_umma"]),
     (1023, 64, 2048, 2, 128, torch.bfloat16, ["expand", "expand", "outer_umma", "outer_umma"]),
@@ -42,7 +46,7 @@ def _ran(M, K, N, n, r, dtype):
     (17000, 64, 128, 2, 64, torch.float16, ["expand", "expand", "outer_umma", "outer_umma"]),
     # results of many tokens on tcgen05
     (1027, 64, 8200, 1, 64, torch.float16, ["expand_umma", "expand", "outer_umma", "outer_umma"]),
-    (2050, 128, 12296, 3, 128, torch.bfloat16, ["expand_umma", "expand", "outer_umma", "outer"]),
+    (2050, 128, 12296, 3, 128, torch.bfloat16, ["expand_umma", "expand", "outer_umma", "outer_umma"]),
     (6300, 64, 4000, 5, 40, torch.float16, ["expand_umma", "expand", "outer_umma", "outer_umma"]),
     (24600, 64, 1032, 2, 48, torch.bfloat16, ["expand_umma", "expand", "outer_umma", "outer_umma"]),
 ])
