@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
             }
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             if (lane == 0) {
-                s_factor[h] = a.alpha * 1.4426950408889634f * back;       // scores in powers of two
+                // scores in powers of two; of a sequence of one token (whose weight is 1) zero: its value comes out exactly as read gives it
+                s_factor[h] = n == 1 ? 0.0f : a.alpha * 1.4426950408889634f * back;
                 s_sum[h] = sum;
             }
         }
@@ -505,8 +506,11 @@ __global__ void __launch_bounds__(32 * WARPS, (Config<T, BITS, DIM, NB, PAIR>::C
             };
             weights();
             if (__any_sync(0xffffffffu, over)) {
-                // the maximum moves: the largest p * scale of this step becomes 2^12 (scales are 2^-24 at least; of rows that are zero p stays below 2^40)
-                const float lv[2] = {fmaxf(__log2f(fabsf(vs[0])), -27.0f) - 12.0f, fmaxf(__log2f(fabsf(vs[1])), -27.0f) - 12.0f};
+                // the maximum moves: the largest p * scale of this step becomes 2^12 or more, by the power of two under the scale (scales are 2^-24 at least; of rows that are zero
+                // p stays below 2^40)
+                float lv[2];
+#pragma unroll
+                for (int row = 0; row < 2; ++row) lv[row] = (float)(max((int)(__float_as_uint(vs[row]) >> 23 & 255) - 127, -27) - 12);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll

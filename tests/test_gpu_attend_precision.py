@@ -111,3 +111,27 @@ def test_many_tokens_far_below_one_that_dominates(dtype, below):
     ok = _between(got, want, slack + (2.0 ** -25 if dtype == torch.float16 else 0))
     bad = int((~ok).sum())
     assert bad == 0, (bad, got[0, 0, :3].tolist(), want[0, 0, :3].tolist())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,bits,batch,wide", [(8, 2, 128, 4, 40, 1), (4, 4, 64, 8, 40, 1), (6, 1, 128, 2, 40, 1), (32, 2, 64, 4, 20, 1), (4, 2, 256, 8, 20, 1), (8, 2, 128, 4, 60, 400),
+                                                                 (4, 2, 80, 4, 20, 1)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_sequence_of_one_token_gives_its_value(heads, kv_heads, dim, bits, batch, wide, dtype):
+    """The weight is 1: what comes out is the value, rounded once, also where it lies halfway between two results."""
+    cache = QuantizedKVCache(batch * wide, 16, kv_heads, dim, bits=bits, device=DEV)
+    table = torch.arange(batch * wide, dtype=torch.int32, device=DEV).view(batch, wide)
+    slots = table[:, 0].long() * 16
+    cache.append(torch.randn(batch, kv_heads, dim, generator=_gen(31), device=DEV), torch.randn(batch, kv_heads, dim, generator=_gen(32), device=DEV), slots)
+    lengths = torch.ones(batch, dtype=torch.int32, device=DEV)
+    if wide > 1:
+        lengths[0] = 16 * wide                          # (rows of zeros behind the first: shares of the line of work)
+    q = torch.randn(batch, heads, dim, generator=_gen(33), device=DEV).to(dtype)
+    want = cache.read(slots, dtype=dtype)[1].repeat_interleave(heads // kv_heads, 1)
+    got = cache.attend(q, table, lengths)
+    assert torch.equal(got[1:], want[1:]) and (wide > 1 or torch.equal(got[0], want[0]))
+    assert _lib.last_kernel() == ("kv_attend_general_kernel" if dim == 80 else "kv_attend_join_kernel" if wide > 1 else "kv_attend_kernel")
+    bad = torch.randn(1, kv_heads, dim, device=DEV)
+    bad[..., 3] = torch.nan
+    cache.append(bad, bad, slots[1:2])
+    got = cache.attend(q, table, lengths)
+    assert bool(got[1].isnan().all()) and torch.equal(got[2:], want[2:])
