@@ -69,7 +69,9 @@ __global__ void __launch_bounds__(256) adapter_outer_general_kernel(const float 
     float s = 0.0f, carry = 0.0f;
     for (int64_t t0 = 0; t0 < M; t0 += 64) {
         float block = 0.0f;
-        for (int64_t t = t0; t < M && t < t0 + 64; ++t)
+        const int64_t end = t0 + 64 < M ? t0 + 64 : M;
+#pragma unroll 8
+        for (int64_t t = t0; t < end; ++t)
             if (index[t] == a) block += h[t * r + j] * to_f32(x[t * N + c]);
         const float y = __fsub_rn(block, carry), next = __fadd_rn(s, y);
         carry = isfinite(next) ? __fsub_rn(__fsub_rn(next, s), y) : 0.0f;
