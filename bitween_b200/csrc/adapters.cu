@@ -5,8 +5,8 @@
 //
 // Both matrices of an adapter are stored rank-major, down [n][rank][K] and up [n][rank][N], so that forward and backward are the
 // same three passes: "shrink" (rows times a matrix of long rows -> rank values), "expand" (the reverse) and "outer" (sums of
-// products over an adapter's tokens).  All three are bound by the bytes of x, base, y and their gradients; the products run on
-// mma.sync.m16n8k16, whose fragments come from 16-byte loads:
+// products over an adapter's tokens).  What they cannot do without are the bytes of x, base, y and their gradients; what bounds each in fact is said at the kernels.  Products of few
+// tokens or ranks run on mma.sync.m16n8k16, whose fragments come from 16-byte loads:
 //   * the reduced index of a product may be permuted at will, if both operands are: where rows are long in it (shrink of a few tokens), a
 //     lane's 16 bytes of a row serve two MMAs, k pairs (0, 1), (2, 3) and (4, 5), (6, 7);
 //   * where it runs over rows (expand over ranks, outer over tokens), a lane takes 16 bytes of four rows, eight columns of its own, and
@@ -668,7 +668,8 @@ __global__ void __launch_bounds__(128, KS <= 4 ? 3 : 2) adapter_expand_kernel(vo
 // The same on tcgen05, for many tokens: 128 rows of one adapter (M) x blocks of 128 columns (N), reduced over the ranks of values and rests.  Rank values lie
 // in tensor memory, a row a lane, their parts one after the other, rows of w MN-major in shared memory.  Eight warps bring w and base into a ring, one issues the MMAs (accumulators in turn), eight
 // add the products to base in the ring, a row and half of its columns a lane, and write whole rows from there.
-// Bound by the bytes of base and out: 8192 tokens of 2 adapters, 14336 columns, rank 64, bf16: 88 us (mma.sync 133), 5.4 TB/s, on the 128 SMs that there are CTAs for.
+// Bound by the bytes of base and out: 8192 tokens, 14336 columns, rank 64, bf16: 85 us (mma.sync 133 with two parts; rank values in shared memory, a stage less, 104), 5.5 TB/s, on the 128
+// SMs that there are CTAs for.
 constexpr int EU_TILE = 128, EU_COLS = 128, EU_JOIN = 8, EU_COPY = 8, EU_THREADS = 32 * (EU_JOIN + EU_COPY + 1);
 __device__ int g_adapter_status = 0;
 
@@ -1038,8 +1039,8 @@ template <int RB, int RG, int PARTS> struct OuterShape {
 
 // dw[a][rank0 .. + RANKS][256 columns] = f_a * sum over the adapter's tokens of h[t] x[t]^T.  The CTAs of a cluster (blockIdx.z) take equal shares of
 // the tokens and add their sums through each other's shared memory.  Rows of x and of the rank values go through a ring, 32 tokens a stage.
-// (For few tokens and ranks up to 16; 64 ranks in the registers of one warp would leave eight warps an SM.  8192 tokens, 14336 columns, rank 64: 129 us, 43 % of
-// what mma.sync can do; the copies' issue, the barrier of a stage and the MMAs take turns.)
+// (For few tokens and ranks up to 16; 64 ranks in the registers of one warp would leave eight warps an SM.  The copies' issue, the barriers of a stage and the MMAs take turns: 8192 tokens,
+// 14336 columns, rank 16, with shrink of 64 columns in front, 69 us of bf16, whose fp32 rank values are split a stage at a time, 70 of fp16.)
 template <typename T, int RB, int RG>
 __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kernel(void *hidden, const T *__restrict__ x, const AdapterArgs p, T *dw) {
     using S = OuterShape<RB, RG, PARTS<T>>;

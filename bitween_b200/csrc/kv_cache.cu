@@ -107,8 +107,8 @@ __device__ __forceinline__ void load_values(const T *row, int at, int dim, bool 
     }
 }
 
-// One group of lanes a row, each with whole words of codes; a thread has its piece of the key and of the value.  Bound by the bytes: 16384 tokens
-// of 8 heads of 128, fp16 to 8 bits, 27 us (the division in four FMAs and the packed adds of rtn_quantize.cu; one element a
+// One group of lanes a row, each with whole words of codes; a thread has its piece of the key and of the value.  Bound by instruction issue: 16384 tokens
+// of 8 heads of 128, fp16 to 8 bits, 27 us, 3.8 TB/s, 66 % of the issue slots (the division in four FMAs and the packed adds of rtn_quantize.cu; one element a
 // load and a hardware division each: 174 us).
 template <typename T, int BITS, bool VEC>
 __global__ void __launch_bounds__(256) kv_append_kernel(const T *__restrict__ k, const T *__restrict__ v, const int64_t *__restrict__ slots,

@@ -32,7 +32,8 @@ class QuantizedKVCache:
 
     @classmethod
     def from_tensors(cls, k_codes, v_codes, params, bits):
-        """A cache around existing tensors of its format; they are adopted, not copied."""
+        """A cache around existing tensors of its format; they are adopted, not copied.  `params` may hold any scales and zero points, those of other quantizers too
+        (fractions, negative numbers)."""
         if bits not in (2, 4, 8):
             raise ValueError("Only 2, 4, or 8 bits are supported.")
         if k_codes.dim() != 4 or k_codes.dtype != torch.int32 or v_codes.dtype != torch.int32 or v_codes.shape != k_codes.shape:
