@@ -1265,7 +1265,11 @@ __global__ void __launch_bounds__(128 * RG, RG == 2 ? 2 : 3) adapter_outer_kerne
 constexpr int OU_LIST = 1024, OU_WINDOW = 512;
 template <typename T> struct OuterUmma {
     static constexpr int BLOCK = OUTER_STEP * 128, A = PARTS<T> * BLOCK, B = 4 * BLOCK, STAGE = A + B, STAGES = PARTS<T> == 2 ? 8 : 7, THREADS = 352;
-    static constexpr int RING = PARTS<T> == 3 ? BLOCK : 0, SMEM = RING + STAGES * STAGE + 1024;                 // bf16: a block of zeros in front of the ring
+    static constexpr int RING = PARTS<T> == 3 ? BLOCK : 0;                                                      // bf16: a block of zeros in front of the ring
+    // All of an SM's tensor memory is taken, so no other kernel that wants some may fit beside: of two clusters that each hold one SM's and want another's both would wait for good.  (The smallest
+    // such cluster kernel has 16 KB of shared memory; of 228 KB these and what is declared in the kernel leave less.)
+    static constexpr int SMEM = 210 * 1024;
+    static_assert(RING + STAGES * STAGE + 1024 <= SMEM, "zeros, the ring and its alignment");
     static_assert(64 * SUM_ROW * 4 <= STAGES * STAGE, "the sums take the ring's place");
 };
 template <typename T>

@@ -145,3 +145,48 @@ def test_adapted_linear_takes_the_native_way_where_nothing_is_recorded(dtype, mo
         want = adapted(x, index)
         monkeypatch.setattr("bitween_b200.modules.QuantizedLinearFunction.apply", None)
         assert torch.equal(adapted(x, index), want)
+
+
+def test_tensor_memory_is_shared_with_the_packed_linears_on_other_streams():
+    """Kernels that take an SM's whole tensor memory (many tokens beside adapters), in clusters and not, captured and replayed beside packed linears of all sizes."""
+    lin = torch.nn.Linear(1024, 2048).to(DEV).half()
+    layer = QuantizedLinear.from_float(lin, bits=4, group_size=128)
+    with torch.no_grad():
+        tokens = [torch.randn(m, 1024, generator=_gen(70 + m), device=DEV).half() for m in (33, 64, 200, 600, 2100)]
+        for t in tokens:
+            layer(t)
+    banks = [_bank(m, 1024, 2048, 2, 64, dtype, seed=80 + m) for m, dtype in ((2100, torch.float16), (2300, torch.bfloat16))]
+
+    def step(i):
+        if i == 2:
+            with torch.no_grad():
+                return [layer(t) for t in tokens]
+        x, down, up, index, base = banks[i]
+        leaves = [t.detach().requires_grad_() for t in (x, down, up)]
+        y = adapter_matmul(*leaves, index.sort().values, base=base)
+        return [y.detach(), *torch.autograd.grad(y, leaves, base)]
+
+    want = [step(i) for i in range(3)]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for i in range(3):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(i)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(i))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(got, ref))
+    assert _lib.lib().bw_device_status() == 0
