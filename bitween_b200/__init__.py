@@ -12,8 +12,10 @@ import sys
 from .adapters import AdaptedLinear, adapter_matmul  # noqa: F401
 from .functional import dequantize_rtn, quantize_rtn  # noqa: F401
 from .kv_cache import QuantizedKVCache  # noqa: F401
+from .log_probs import TokenLogProbs, token_log_probs  # noqa: F401
 from .modules import QuantizedLinear, QuantizedLinearFunction  # noqa: F401
 from .quantizer.quantizer import Bitween  # noqa: F401
+from .rotary import RotaryPositions  # noqa: F401
 
 __version__ = "0.1.0"
 

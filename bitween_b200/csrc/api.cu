@@ -81,7 +81,16 @@ int kv_read(const int32_t *kc, const int32_t *vc, const void *params, int heads,
 size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages);
 int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *kc, const int32_t *vc,
               const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *table, int64_t table_stride,
-              int max_pages, const int32_t *lengths, float alpha, void *out, void *workspace, cudaStream_t st);
+              int max_pages, const int32_t *lengths, int window, int sinks, float alpha, void *out, void *workspace, cudaStream_t st);
+int rotate(const bw_rotary &rotary, int64_t tokens, int dim, int dtype, bool inverse, const void *const *x, const int *heads, const int64_t *strides,
+           void *const *out, cudaStream_t st);
+int kv_append_rotated(const bw_rotary &rotary, const void *q, int q_heads, int64_t q_stride, int64_t q_head_stride, void *q_out, const void *k, const void *v,
+                      int dtype, int64_t tokens, const int64_t *strides, const int64_t *slots, int heads, int dim, int bits, int64_t pages, int page_size,
+                      int32_t *kc, int32_t *vc, void *params, cudaStream_t st);
+int token_log_probs(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, float *log_probs, float *entropy,
+                    int top, float *top_log_probs, int64_t *top_tokens, float *stats, cudaStream_t st);
+int token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, const float *stats,
+                         const float *g, const float *e, int top, const int64_t *top_tokens, const float *g_top, void *grad, cudaStream_t st);
 size_t adapter_hidden_bytes(int64_t M, int r);
 int adapter_forward(const void *x, int dtype, int64_t M, int64_t N, int64_t K, const void *down, const void *up, int n, int r, const int32_t *index,
                     const float *scaling, const void *base, void *out, void *h, cudaStream_t st);
@@ -614,10 +623,11 @@ size_t bw_kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int 
     return kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
 }
 
-int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *k_codes,
-                 const int32_t *v_codes, const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *page_table,
-                 int64_t table_stride, int64_t max_pages, const int32_t *lengths, float alpha, void *out, void *workspace, size_t workspace_bytes,
-                 void *stream) {
+// One checked call of the cache's attention; without a window INT32_MAX tokens are visible.
+static int kv_attend_checked(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *k_codes,
+                             const int32_t *v_codes, const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *page_table,
+                             int64_t table_stride, int64_t max_pages, const int32_t *lengths, int window, int sinks, float alpha, void *out, void *workspace,
+                             size_t workspace_bytes, size_t need, void *stream) {
     const int rc = kv_validate(k_codes, v_codes, params, pages, page_size, kv_heads, dim, bits);
     if (rc != BW_OK) return rc;
     if (dtype != BW_F16 && dtype != BW_BF16) return BW_ERR_DTYPE;
@@ -627,12 +637,120 @@ int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_s
     if (batch == 0) return BW_OK;
     if (!q || !out || !lengths || (max_pages > 0 && !page_table)) return BW_ERR_NULL;
     if (!aligned_to(q, 2) || !aligned_to(out, 2) || !aligned_to(page_table, 4) || !aligned_to(lengths, 4)) return BW_ERR_ALIGN;
-    const size_t need = kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
     if (need && (!workspace || workspace_bytes < need)) return BW_ERR_WORKSPACE;
     if (!aligned_to(workspace, 16)) return BW_ERR_ALIGN;
     std::lock_guard<std::mutex> lock(scratch_lock(workspace));
     return kv_attend(q, dtype, batch, heads, q_stride, q_head_stride, k_codes, v_codes, params, bits, pages, page_size, kv_heads, dim, page_table,
-                     table_stride, (int)max_pages, lengths, alpha, out, workspace, (cudaStream_t)stream);
+                     table_stride, (int)max_pages, lengths, window, sinks, alpha, out, workspace, (cudaStream_t)stream);
+}
+
+int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *k_codes,
+                 const int32_t *v_codes, const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *page_table,
+                 int64_t table_stride, int64_t max_pages, const int32_t *lengths, float alpha, void *out, void *workspace, size_t workspace_bytes,
+                 void *stream) {
+    return kv_attend_checked(q, dtype, batch, heads, q_stride, q_head_stride, k_codes, v_codes, params, bits, pages, page_size, kv_heads, dim, page_table,
+                             table_stride, max_pages, lengths, INT32_MAX, 0, alpha, out, workspace, workspace_bytes,
+                             bw_kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages), stream);
+}
+
+size_t bw_kv_attend_window_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages, int64_t window, int64_t sinks) {
+    if (window < 0 || sinks < 0) return 0;
+    return bw_kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
+}
+
+int bw_kv_attend_window(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *k_codes,
+                        const int32_t *v_codes, const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *page_table,
+                        int64_t table_stride, int64_t max_pages, const int32_t *lengths, int64_t window, int64_t sinks, float alpha, void *out,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+    if (window < 0 || sinks < 0) return BW_ERR_SHAPE;
+    // (lengths are int32: more than that is all of them)
+    const int w = (int)(window < INT32_MAX ? window : INT32_MAX), s = (int)(sinks < INT32_MAX ? sinks : INT32_MAX);
+    return kv_attend_checked(q, dtype, batch, heads, q_stride, q_head_stride, k_codes, v_codes, params, bits, pages, page_size, kv_heads, dim, page_table,
+                             table_stride, max_pages, lengths, s == INT32_MAX ? s : w, s == INT32_MAX || w == INT32_MAX ? 0 : s, alpha, out, workspace, workspace_bytes,
+                             bw_kv_attend_window_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages, window, sinks), stream);
+}
+
+// ---- rotary positions ----
+static int rotary_validate(const bw_rotary *r, int64_t tokens, int dim) {
+    if (!r) return BW_ERR_NULL;
+    if (r->rotary_dim < 2 || r->rotary_dim % 2 != 0 || r->rotary_dim > 256 || r->rotary_dim > dim || dim > 65536) return BW_ERR_SHAPE;
+    if (r->max_positions < 0 || r->max_positions > (int64_t)1 << 40 || r->num_axes < 1 || r->num_axes > 255) return BW_ERR_SHAPE;
+    if (r->axes)
+        for (int i = 0; i < r->rotary_dim / 2; ++i)
+            if (r->axes[i] >= r->num_axes) return BW_ERR_SHAPE;
+    if (tokens > 0 && (!r->positions || (r->max_positions > 0 && !r->table))) return BW_ERR_NULL;
+    if (!aligned_to(r->table, 16) || !aligned_to(r->positions, 8)) return BW_ERR_ALIGN;
+    return BW_OK;
+}
+
+int bw_rotate(const bw_rotary *rotary, int64_t tokens, int dim, int dtype, int inverse, const void *x0, int heads0, int64_t stride0, int64_t head_stride0,
+              void *out0, const void *x1, int heads1, int64_t stride1, int64_t head_stride1, void *out1, void *stream) {
+    const int rc = rotary_validate(rotary, tokens, dim);
+    if (rc != BW_OK) return rc;
+    if (!is_float_dtype(dtype)) return BW_ERR_DTYPE;
+    if (tokens < 0 || heads0 < 0 || heads1 < 0 || heads0 > 1 << 20 || heads1 > 1 << 20) return BW_ERR_SHAPE;
+    if (heads0 + heads1 > 0 && tokens > ((int64_t)1 << 31) / (heads0 + heads1) / 8) return BW_ERR_SHAPE;
+    if (tokens == 0 || heads0 + heads1 == 0) return BW_OK;
+    if ((heads0 && (!x0 || !out0)) || (heads1 && (!x1 || !out1))) return BW_ERR_NULL;
+    const size_t e = dtype_size(dtype);
+    if (!aligned_to(x0, e) || !aligned_to(out0, e) || !aligned_to(x1, e) || !aligned_to(out1, e)) return BW_ERR_ALIGN;
+    const void *const x[2] = {x0, x1};
+    void *const out[2] = {out0, out1};
+    const int heads[2] = {heads0, heads1};
+    const int64_t strides[4] = {stride0, head_stride0, stride1, head_stride1};
+    return rotate(*rotary, tokens, dim, dtype, inverse != 0, x, heads, strides, out, (cudaStream_t)stream);
+}
+
+int bw_kv_append_rotated(const bw_rotary *rotary, const void *q, int q_heads, int64_t q_stride, int64_t q_head_stride, void *q_out, const void *k, const void *v,
+                         int dtype, int64_t tokens, int64_t k_stride, int64_t k_head_stride, int64_t v_stride, int64_t v_head_stride, const int64_t *slots,
+                         int heads, int dim, int bits, int64_t pages, int page_size, int32_t *k_codes, int32_t *v_codes, void *params, void *stream) {
+    int rc = kv_validate(k_codes, v_codes, params, pages, page_size, heads, dim, bits);
+    if (rc == BW_OK) rc = rotary_validate(rotary, tokens, dim);
+    if (rc != BW_OK) return rc;
+    if (!is_float_dtype(dtype)) return BW_ERR_DTYPE;
+    if (q_heads < 0 || q_heads > 1 << 20 || heads > 1 << 20 || tokens < 0 || tokens > ((int64_t)1 << 31) / ((int64_t)2 * heads + q_heads) / 8) return BW_ERR_SHAPE;
+    if (tokens == 0) return BW_OK;
+    if (!k || !v || !slots || (q_heads && (!q || !q_out))) return BW_ERR_NULL;
+    const size_t e = dtype_size(dtype);
+    if (!aligned_to(k, e) || !aligned_to(v, e) || !aligned_to(q, e) || !aligned_to(q_out, e) || !aligned_to(slots, 8)) return BW_ERR_ALIGN;
+    const int64_t strides[4] = {k_stride, k_head_stride, v_stride, v_head_stride};
+    return kv_append_rotated(*rotary, q, q_heads, q_stride, q_head_stride, q_out, k, v, dtype, tokens, strides, slots, heads, dim, bits, pages, page_size,
+                             k_codes, v_codes, params, (cudaStream_t)stream);
+}
+
+// ---- log probabilities of tokens ----
+static int log_probs_validate(int dtype, const void *logits, int64_t rows, int64_t vocab, int64_t stride, int top) {
+    if (!is_float_dtype(dtype)) return BW_ERR_DTYPE;
+    if (rows < 0 || rows > ((int64_t)1 << 31) / 32 || vocab < 1 || vocab > (int64_t)1 << 28 || top < 0 || top > 32 || top > vocab) return BW_ERR_SHAPE;
+    if (rows > 0 && !logits) return BW_ERR_NULL;
+    if (!aligned_to(logits, dtype_size(dtype))) return BW_ERR_ALIGN;
+    return BW_OK;
+}
+
+int bw_token_log_probs(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, float *log_probs, float *entropy,
+                       int top, float *top_log_probs, int64_t *top_tokens, float *stats, void *stream) {
+    const int rc = log_probs_validate(dtype, logits, rows, vocab, stride, top);
+    if (rc != BW_OK) return rc;
+    if (rows == 0) return BW_OK;
+    if (!tokens != !log_probs || (top && (!top_log_probs || !top_tokens))) return BW_ERR_NULL;
+    if (!aligned_to(tokens, 8) || !aligned_to(log_probs, 4) || !aligned_to(entropy, 4) || !aligned_to(top_log_probs, 4) || !aligned_to(top_tokens, 8) ||
+        !aligned_to(stats, 16))
+        return BW_ERR_ALIGN;
+    return token_log_probs(logits, dtype, rows, vocab, stride, tokens, log_probs, entropy, top, top_log_probs, top_tokens, stats, (cudaStream_t)stream);
+}
+
+int bw_token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, const float *stats,
+                            const float *grad_log_probs, const float *grad_entropy, int top, const int64_t *top_tokens, const float *grad_top, void *grad,
+                            void *stream) {
+    const int rc = log_probs_validate(dtype, logits, rows, vocab, stride, top);
+    if (rc != BW_OK) return rc;
+    if (rows == 0) return BW_OK;
+    if (!stats || !grad || (grad_log_probs && !tokens) || (top && grad_top && !top_tokens)) return BW_ERR_NULL;
+    if (!aligned_to(tokens, 8) || !aligned_to(stats, 16) || !aligned_to(grad_log_probs, 4) || !aligned_to(grad_entropy, 4) || !aligned_to(top_tokens, 8) ||
+        !aligned_to(grad_top, 4) || !aligned_to(grad, dtype_size(dtype)))
+        return BW_ERR_ALIGN;
+    return token_log_probs_grad(logits, dtype, rows, vocab, stride, tokens, stats, grad_log_probs, grad_entropy, top, top_tokens, grad_top, grad,
+                                (cudaStream_t)stream);
 }
 
 // ---- low-rank adapters ----

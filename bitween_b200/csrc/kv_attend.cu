@@ -21,6 +21,7 @@ struct AttendArgs {
     int64_t q_stride, q_head_stride, table_stride, pages;
     int heads, kv_heads, dim, words, page_size, max_pages;
     float alpha;
+    int window, sinks;                         // tokens t < sinks or t >= length - window are visible
 };
 
 // Any head dimension up to 256, any page size: one CTA a head of a sequence, its warps on every fourth token.
@@ -37,8 +38,10 @@ __global__ void __launch_bounds__(128) kv_attend_general_kernel(AttendArgs p) {
     const int64_t most = (int64_t)p.max_pages * p.page_size, n = p.lengths[b];
     bool bad = n > most;
     const int64_t len = bad ? most : n;
-    for (int64_t t = warp; t < len; t += 4) {
-        const int64_t in = t / p.page_size, page = p.table[b * p.table_stride + in];
+    // the visible tokens: `first` of the beginning, then those from `from` on
+    const int64_t first = p.sinks < len ? p.sinks : len, from = n - p.window > first ? n - p.window : first, seen = first + (len > from ? len - from : 0);
+    for (int64_t i = warp; i < seen; i += 4) {
+        const int64_t t = i < first ? i : i - first + from, in = t / p.page_size, page = p.table[b * p.table_stride + in];
         if (page < 0 || page >= p.pages) {
             bad = true;
             continue;
@@ -88,7 +91,7 @@ __global__ void __launch_bounds__(128) kv_attend_general_kernel(AttendArgs p) {
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) v += f[w] * so[w][d];
-        ((T *)p.out)[(b * p.heads + h) * p.dim + d] = from_f32<T>(n <= 0 ? 0.0f : v / sum);
+        ((T *)p.out)[(b * p.heads + h) * p.dim + d] = from_f32<T>(seen <= 0 && !bad ? 0.0f : v / sum);
     }
 }
 
@@ -836,11 +839,11 @@ size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim
 
 int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *kc, const int32_t *vc,
               const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *table, int64_t table_stride,
-              int max_pages, const int32_t *lengths, float alpha, void *out, void *workspace, cudaStream_t st) {
+              int max_pages, const int32_t *lengths, int window, int sinks, float alpha, void *out, void *workspace, cudaStream_t st) {
     FastArgs f = {};
     AttendArgs p = {q, kc, vc, (const __half2 *)params, table, lengths, out, q_stride, q_head_stride, table_stride, pages,
-                    heads, kv_heads, dim, dim * bits / 32, page_size, max_pages, alpha};
-    if (fast_args(f, batch, heads, kv_heads, dim, pages, page_size, max_pages)) {
+                    heads, kv_heads, dim, dim * bits / 32, page_size, max_pages, alpha, window, sinks};
+    if (window == INT32_MAX && fast_args(f, batch, heads, kv_heads, dim, pages, page_size, max_pages)) {
         f.a = p;
         f.slots = (float *)workspace;
         return dtype == BW_F16 ? launch_bits<__half>(f, bits, st) : launch_bits<__nv_bfloat16>(f, bits, st);

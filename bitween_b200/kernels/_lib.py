@@ -51,6 +51,12 @@ class Epilogue(ctypes.Structure):
     _fields_ = [("activation", ctypes.c_int), ("residual", ctypes.c_void_p)]
 
 
+class Rotary(ctypes.Structure):
+    """bw_rotary of include/bitween_b200.h."""
+    _fields_ = [("table", ctypes.c_void_p), ("max_positions", ctypes.c_int64), ("rotary_dim", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("num_axes", ctypes.c_int), ("axes", ctypes.c_char_p), ("positions", ctypes.c_void_p), ("axis_stride", ctypes.c_int64)]
+
+
 class RtnJob(ctypes.Structure):
     """bw_rtn_job of include/bitween_b200.h."""
     _fields_ = [("w", ctypes.c_void_p), ("qweight", ctypes.c_void_p), ("scale", ctypes.c_void_p),
@@ -98,6 +104,19 @@ def _declare(L):
     L.bw_kv_attend_workspace_bytes.restype = sz
     L.bw_kv_attend.argtypes = [vp, i32, i64, i32, i64, i64, vp, vp, vp, i32, i64, i32, i32, i32, vp, i64, i64, vp, f32, vp, vp, sz, vp]
     L.bw_kv_attend.restype = i32
+    L.bw_kv_attend_window_workspace_bytes.argtypes = [i64, i32, i32, i32, i32, i64, i64, i64]
+    L.bw_kv_attend_window_workspace_bytes.restype = sz
+    L.bw_kv_attend_window.argtypes = [vp, i32, i64, i32, i64, i64, vp, vp, vp, i32, i64, i32, i32, i32, vp, i64, i64, vp, i64, i64, f32, vp, vp, sz, vp]
+    L.bw_kv_attend_window.restype = i32
+    rotary = ctypes.POINTER(Rotary)
+    L.bw_rotate.argtypes = [rotary, i64, i32, i32, i32, vp, i32, i64, i64, vp, vp, i32, i64, i64, vp, vp]
+    L.bw_rotate.restype = i32
+    L.bw_kv_append_rotated.argtypes = [rotary, vp, i32, i64, i64, vp, vp, vp, i32, i64, i64, i64, i64, i64, vp, i32, i32, i32, i64, i32, vp, vp, vp, vp]
+    L.bw_kv_append_rotated.restype = i32
+    L.bw_token_log_probs.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp, i32, vp, vp, vp, vp]
+    L.bw_token_log_probs.restype = i32
+    L.bw_token_log_probs_grad.argtypes = [vp, i32, i64, i64, i64, vp, vp, vp, vp, i32, vp, vp, vp, vp]
+    L.bw_token_log_probs_grad.restype = i32
     L.bw_adapter_hidden_bytes.argtypes = [i64, i32]
     L.bw_adapter_hidden_bytes.restype = sz
     L.bw_adapter_forward.argtypes = [vp, i32, i64, i64, i64, vp, vp, i32, i32, vp, vp, vp, vp, vp, sz, vp]

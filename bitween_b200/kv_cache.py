@@ -1,11 +1,13 @@
 """A paged key-value cache quantised as it is written: 2, 4 or 8 bits, one scale and zero point per token and head, by the
 rounding of quantize_rtn.  No counterpart in the reference; computed by the sm_100a kernels behind bw_kv_append, bw_kv_read and
 bw_kv_attend (include/bitween_b200.h has the format)."""
+import ctypes
 import math
 
 import torch
 
 from .kernels import _lib
+from .rotary import RotaryPositions
 
 _FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
@@ -104,6 +106,51 @@ class QuantizedKVCache:
                                 _lib.raw_stream(self.device))
         _lib.check(rc)
 
+    def append_rotated(self, q, k, v, slots, rotary, positions):
+        """`append` of keys that `rotary` (a RotaryPositions) turns by `positions` on the way, and the queries q [tokens, heads, head_dim] turned alike, in
+        one launch.  Returns the queries, rounded once to their dtype; q may be None.
+
+        Keys are rotated in fp32 and quantised from there: the cache holds what `append(rotary.rotate(positions, k.float()), v.float(), slots)` would
+        leave.  `positions`: int64 [tokens], or [axes, tokens].  A position outside the table gives NaN: that token's queries, and its key when it is read.  Queries
+        of skipped slots are rotated too.  Nothing is recorded: a q that requires a gradient is refused where gradients are recorded."""
+        _lib.require_cuda(self.k_codes, "cache")
+        slots = self._check_slots(slots)
+        tokens = slots.shape[0]
+        shape = (tokens, self.num_kv_heads, self.head_dim)
+        for name, t in (("k", k), ("v", v)):
+            _lib.require_cuda(t, name)
+            if tuple(t.shape) != shape:
+                raise ValueError(f"`{name}` must have shape {shape}")
+        for name, t in (("k", k), ("v", v), ("q", q)):
+            if t is None:
+                continue
+            if t.dtype not in _FLOAT_DTYPES or t.dtype != k.dtype:
+                raise TypeError("q, k and v must have one dtype: float32, float16 or bfloat16")
+            if t.device != self.device:
+                raise RuntimeError(f"`{name}` is on {t.device} but the cache is on {self.device}")
+        if q is not None:
+            if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != self.head_dim:
+                raise ValueError(f"q must be [{tokens}, heads, {self.head_dim}]")
+            if q.requires_grad and torch.is_grad_enabled():
+                raise ValueError("append_rotated has no gradient; detach q, or rotate it by itself")
+        if not isinstance(rotary, RotaryPositions):
+            raise TypeError("rotary must be a RotaryPositions")
+        if rotary.device != self.device:
+            raise RuntimeError(f"`rotary` is on {rotary.device} but the cache is on {self.device}")
+        if rotary.rotary_dim > self.head_dim:
+            raise ValueError(f"rotary turns {rotary.rotary_dim} values but head_dim is {self.head_dim}")
+        positions, axis_stride = rotary._positions(positions, (tokens,))
+        q, k, v = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (t if t is None else t.resolve_neg() for t in (q, k, v)))
+        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=self.device)
+        L = _lib.lib()
+        with _lib.on_device(self.device):
+            rc = L.bw_kv_append_rotated(ctypes.byref(rotary._struct(rotary.table, positions, axis_stride)), *((None, 0, 0, 0, None) if q is None else (
+                q.data_ptr(), q.shape[1], q.stride(0), q.stride(1), out.data_ptr())), k.data_ptr(), v.data_ptr(), _lib.dtype_code(k.dtype), tokens,
+                k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), self.num_kv_heads, self.head_dim, self.bits, self.num_pages, self.page_size,
+                *self._tensors(), _lib.raw_stream(self.device))
+        _lib.check(rc)
+        return out
+
     def read(self, slots, dtype=torch.float16):
         """(k, v) of `slots` as [tokens, num_kv_heads, head_dim] tensors of `dtype` (fp16, bf16 or fp32): the values that the cache
         stands for, rounded once.  Slots outside the cache give zeros."""
@@ -123,7 +170,7 @@ class QuantizedKVCache:
         _lib.check(rc)
         return k, v
 
-    def attend(self, q, page_table, lengths, softmax_scale=None):
+    def attend(self, q, page_table, lengths, softmax_scale=None, window=None, sinks=0):
         """Attention of one new token per sequence: q [batch, heads, head_dim] (fp16 or bf16; heads a multiple of num_kv_heads, head h
         reads cache head h // (heads / num_kv_heads)) over the first lengths[b] tokens of the sequence whose pages page_table[b]
         names (int32 [batch, pages of the longest]).  Returns [batch, heads, head_dim] in q's dtype.
@@ -131,12 +178,49 @@ class QuantizedKVCache:
         `softmax_scale` defaults to head_dim ** -0.5.  The new token's own row is attended to if it has been appended and counted.  Sequences
         of length 0 (or less) give zeros.  A length that is more than the table holds, and a page outside the cache within the
         length, give NaN for that sequence; nothing is read there.  There is no gradient: a q that requires one is refused where
-        gradients are recorded."""
+        gradients are recorded.
+
+        `window` (None: all): only the last `window` tokens of a sequence and its first `sinks` are attended to.  Pages that hold none of those are
+        not looked up: they may have been given to others, and their entries of the table may be anything."""
         if softmax_scale is None:
             softmax_scale = self._softmax_scale
+        if window is not None:
+            return self._attend_window(q, page_table, lengths, softmax_scale, window, sinks)
         out = (_lib._operators or _lib.host_operators()).kv_attend(*self._cache, q, page_table, lengths, softmax_scale)
         if out is not None:
             return out
+        q, page_table, lengths, out = self._attend_args(q, page_table, lengths)
+        batch, heads = q.shape[:2]
+        L = _lib.lib()
+        with _lib.on_device(self.device):
+            ws = _lib.workspace(self.device, L.bw_kv_attend_workspace_bytes(batch, heads, self.num_kv_heads, self.head_dim, self.page_size,
+                                                                            page_table.shape[1]))
+            rc = L.bw_kv_attend(q.data_ptr(), _lib.dtype_code(q.dtype), batch, heads, q.stride(0), q.stride(1), *self._tensors(), self.bits, self.num_pages,
+                                self.page_size, self.num_kv_heads, self.head_dim, page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+                                lengths.data_ptr(), float(softmax_scale), out.data_ptr(), None if ws is None else ws.data_ptr(),
+                                0 if ws is None else ws.numel(), _lib.raw_stream(self.device))
+        _lib.check(rc)
+        return out
+
+    def _attend_window(self, q, page_table, lengths, softmax_scale, window, sinks):
+        if not isinstance(window, int) or not isinstance(sinks, int) or window < 0 or sinks < 0:
+            raise ValueError("window and sinks must be numbers of tokens, 0 or more")
+        window, sinks = min(window, 2 ** 31), min(sinks, 2 ** 31)
+        q, page_table, lengths, out = self._attend_args(q, page_table, lengths)
+        batch, heads = q.shape[:2]
+        L = _lib.lib()
+        with _lib.on_device(self.device):
+            ws = _lib.workspace(self.device, L.bw_kv_attend_window_workspace_bytes(batch, heads, self.num_kv_heads, self.head_dim, self.page_size,
+                                                                                   page_table.shape[1], window, sinks))
+            rc = L.bw_kv_attend_window(q.data_ptr(), _lib.dtype_code(q.dtype), batch, heads, q.stride(0), q.stride(1), *self._tensors(), self.bits, self.num_pages,
+                                       self.page_size, self.num_kv_heads, self.head_dim, page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+                                       lengths.data_ptr(), window, sinks, float(softmax_scale), out.data_ptr(), None if ws is None else ws.data_ptr(),
+                                       0 if ws is None else ws.numel(), _lib.raw_stream(self.device))
+        _lib.check(rc)
+        return out
+
+    def _attend_args(self, q, page_table, lengths):
+        """Checked arguments of a call of attention as the kernels take them, and its output."""
         _lib.require_cuda(q, "q")
         if q.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"attend: unsupported dtype {q.dtype} (float16/bfloat16)")
@@ -158,17 +242,7 @@ class QuantizedKVCache:
             page_table = page_table.contiguous()
         if not lengths.is_contiguous():
             lengths = lengths.contiguous()
-        out = torch.empty((batch, heads, self.head_dim), dtype=q.dtype, device=self.device)
-        L = _lib.lib()
-        with _lib.on_device(self.device):
-            ws = _lib.workspace(self.device, L.bw_kv_attend_workspace_bytes(batch, heads, self.num_kv_heads, self.head_dim, self.page_size,
-                                                                            page_table.shape[1]))
-            rc = L.bw_kv_attend(q.data_ptr(), _lib.dtype_code(q.dtype), batch, heads, q.stride(0), q.stride(1), *self._tensors(), self.bits, self.num_pages,
-                                self.page_size, self.num_kv_heads, self.head_dim, page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                                lengths.data_ptr(), float(softmax_scale), out.data_ptr(), None if ws is None else ws.data_ptr(),
-                                0 if ws is None else ws.numel(), _lib.raw_stream(self.device))
-        _lib.check(rc)
-        return out
+        return q, page_table, lengths, torch.empty((batch, heads, self.head_dim), dtype=q.dtype, device=self.device)
 
     def __repr__(self):
         return (f"QuantizedKVCache(num_pages={self.num_pages}, page_size={self.page_size}, num_kv_heads={self.num_kv_heads}, "

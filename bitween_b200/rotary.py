@@ -1,0 +1,152 @@
+"""Rotary positions of one or several axes (time, height, width): queries and keys turned by the angles of their positions, with gradients.
+No counterpart in the reference; computed by the sm_100a kernels behind bw_rotate (include/bitween_b200.h has the formula).
+`QuantizedKVCache.append_rotated` rotates on the way into the cache."""
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .kernels import _lib
+
+_FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+class RotaryPositions:
+    """The cosines and sines of positions 0 to max_positions - 1.
+
+    Pair j of a head's first `rotary_dim` values, (j, j + rotary_dim/2) or where `interleaved` (2j, 2j+1), is turned by position * inv_freq[j].
+    `inv_freq` defaults to base ** (-2j / rotary_dim).  With several axes of positions each pair follows one of them: `sections`, how many
+    consecutive pairs each axis has, or `axes`, the axis of each pair.  `factor` multiplies cosines and sines.  Angles are computed in 64 bits; `table`, fp32
+    [max_positions, rotary_dim/2, 2], holds them (cosine, sine).
+    """
+
+    def __init__(self, rotary_dim, max_positions, base=10000.0, inv_freq=None, sections=None, axes=None, interleaved=False, factor=1.0, device="cuda"):
+        if rotary_dim < 2 or rotary_dim > 256 or rotary_dim % 2 != 0:
+            raise ValueError("rotary_dim must be even, 2 to 256")
+        if max_positions < 1:
+            raise ValueError("a table needs at least one position")
+        pairs = rotary_dim // 2
+        if inv_freq is None:
+            inv_freq = base ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim)
+        inv_freq = torch.as_tensor(inv_freq, dtype=torch.float64).detach().to(device)
+        if tuple(inv_freq.shape) != (pairs,):
+            raise ValueError(f"inv_freq must have {pairs} frequencies")
+        if sections is not None:
+            if axes is not None:
+                raise ValueError("give either sections or axes")
+            sections = [int(n) for n in sections]
+            if min(sections, default=-1) < 0 or sum(sections) != pairs:
+                raise ValueError(f"sections must add up to {pairs} pairs")
+            axes, self.num_axes = [a for a, n in enumerate(sections) for _ in range(n)], len(sections)
+        else:
+            axes = [0] * pairs if axes is None else [int(a) for a in axes]
+            if len(axes) != pairs or min(axes) < 0:
+                raise ValueError(f"axes must name an axis for each of {pairs} pairs")
+            self.num_axes = max(axes) + 1
+        if self.num_axes > 255:
+            raise ValueError("at most 255 axes")
+        angles = torch.arange(max_positions, dtype=torch.float64, device=inv_freq.device)[:, None] * inv_freq
+        self.table = torch.stack(((angles.cos() * factor).float(), (angles.sin() * factor).float()), -1)
+        self.rotary_dim, self.max_positions, self.interleaved = rotary_dim, max_positions, bool(interleaved)
+        self.axes = tuple(axes)
+        self.device = self.table.device
+        self._axes = bytes(axes)
+        self._shape = self.table.shape
+
+    def _checked(self, table):
+        """`table` (this one's, or what came back of it for a backward pass), if the kernels can take it."""
+        if table.shape != self._shape or table.dtype != torch.float32 or not table.is_contiguous() or table.device != self.device or table.data_ptr() % 16 != 0:
+            raise RuntimeError("the table has been changed in shape, type or place")
+        return table
+
+    def _positions(self, positions, lead):
+        """(positions with whole rows of tokens, elements between axes) for rows of the leading shape `lead`."""
+        _lib.require_cuda(positions, "positions")
+        if positions.dtype != torch.int64:
+            raise TypeError("positions must be int64")
+        if positions.device != self.device:
+            raise RuntimeError(f"`positions` is on {positions.device} but the table is on {self.device}")
+        if tuple(positions.shape) == tuple(lead):
+            return positions.contiguous(), 0
+        if tuple(positions.shape) != (self.num_axes, *lead):
+            raise ValueError(f"positions must have shape {tuple(lead)} or {(self.num_axes, *lead)}")
+        flat = positions.reshape(self.num_axes, math.prod(lead))
+        if flat.shape[1] > 1 and flat.stride(1) != 1:
+            flat = flat.contiguous()
+        return flat, flat.stride(0) if self.num_axes > 1 else 0
+
+    def _struct(self, table, positions, axis_stride):
+        return _lib.Rotary(self._checked(table).data_ptr(), self.max_positions, self.rotary_dim, int(self.interleaved), self.num_axes, self._axes,
+                           positions.data_ptr(), axis_stride)
+
+    def rotate(self, positions, *xs):
+        """One or two tensors [..., heads, dim] (queries, and keys with heads of their own; fp32, fp16 or bf16; dim at least rotary_dim) rotated, in
+        one launch.  Returns new tensors, rounded once: one for one, a tuple for two.  `positions`, int64: of the tensors' leading shape, or
+        with several axes [axes, *leading shape].  A position outside the table gives NaN.  Values behind the first rotary_dim are copied.  Differentiable."""
+        if not 1 <= len(xs) <= 2:
+            raise ValueError("rotate takes one or two tensors")
+        for x in xs:
+            _lib.require_cuda(x, "x")
+            if x.dtype not in _FLOAT_DTYPES or x.dtype != xs[0].dtype:
+                raise TypeError("the tensors to rotate must have one dtype: float32, float16 or bfloat16")
+            if x.device != self.device:
+                raise RuntimeError(f"`x` is on {x.device} but the table is on {self.device}")
+            if x.dim() < 2 or x.shape[:-2] != xs[0].shape[:-2] or x.shape[-1] != xs[0].shape[-1] or x.shape[-1] < self.rotary_dim:
+                raise ValueError(f"the tensors to rotate must be [..., heads, dim] of one leading shape and one dim of at least {self.rotary_dim}")
+        positions, axis_stride = self._positions(positions, xs[0].shape[:-2])
+        if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
+            out = RotateFunction.apply(self, positions, axis_stride, *xs)
+        else:
+            out = _rotate(self, self.table, positions, axis_stride, xs, False)
+        return out[0] if len(xs) == 1 else tuple(out)
+
+    def __repr__(self):
+        return f"RotaryPositions(rotary_dim={self.rotary_dim}, max_positions={self.max_positions}, num_axes={self.num_axes}, interleaved={self.interleaved})"
+
+
+def _rows(x):
+    """x [..., heads, dim] as [tokens, heads, dim] whose values lie side by side."""
+    x = x.resolve_neg()
+    x = x.reshape(math.prod(x.shape[:-2]), *x.shape[-2:]) if x.dim() != 3 else x
+    return x if x.stride(2) == 1 else x.contiguous()
+
+
+def _rotate(rotary, table, positions, axis_stride, xs, inverse):
+    """New tensors: those of `xs` that are there, turned (or turned back).  None where there is none."""
+    outs = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
+    given = [(_rows(x), out) for x, out in zip(xs, outs) if out is not None and out.numel()]
+    if given:
+        args = []
+        for x, out in given:
+            args += [x.data_ptr(), x.shape[1], x.stride(0), x.stride(1), out.data_ptr()]
+        args += [None, 0, 0, 0, None] * (2 - len(given))
+        x = given[0][0]
+        L = _lib.lib()
+        with _lib.on_device(rotary.device):
+            rc = L.bw_rotate(ctypes.byref(rotary._struct(table, positions, axis_stride)), x.shape[0], x.shape[2], _lib.dtype_code(x.dtype), int(inverse), *args,
+                             _lib.raw_stream(rotary.device))
+        _lib.check(rc)
+    return outs
+
+
+class RotateFunction(torch.autograd.Function):
+    """apply(rotary, positions, axis_stride, *xs) with what `rotate` has checked."""
+
+    @staticmethod
+    def forward(ctx, rotary, positions, axis_stride, *xs):
+        ctx.rotary, ctx.axis_stride = rotary, axis_stride
+        ctx.save_for_backward(rotary.table, positions)
+        ctx.like = (positions.shape, positions.stride(), positions.dtype, positions.device)
+        ctx.set_materialize_grads(False)
+        return tuple(_rotate(rotary, rotary.table, positions, axis_stride, xs, False))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        table, positions = ctx.saved_tensors
+        # (hooks may have made other tensors of them in the meantime: moved, packed)
+        if (positions.shape, positions.stride(), positions.dtype, positions.device) != ctx.like:
+            raise RuntimeError("rotate: a tensor saved for the backward pass has come back from its hooks in another shape, type or place")
+        wanted = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[3:])]
+        return (None, None, None, *_rotate(ctx.rotary, table, positions, ctx.axis_stride, wanted, True))

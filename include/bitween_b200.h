@@ -378,6 +378,74 @@ BW_API int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int6
                  const int32_t *lengths, float alpha, void *out, void *workspace, size_t workspace_bytes, void *stream);
 
 /*
+ * The same over the tokens of a sliding window and of the sequence's beginning: the softmax runs over the t < lengths[b] with t < sinks or
+ * t >= lengths[b] - window (both 0 or more; where neither leaves a token the output is zero).  Pages without such a token are not looked up: their entries
+ * of the table may be anything.  A page outside the cache gives NaN only where it holds a visible token.
+ */
+BW_API size_t bw_kv_attend_window_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages, int64_t window,
+                                           int64_t sinks);
+BW_API int bw_kv_attend_window(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride,
+                        const int32_t *k_codes, const int32_t *v_codes, const void *params, int bits, int64_t pages, int page_size,
+                        int kv_heads, int dim, const int32_t *page_table, int64_t table_stride, int64_t max_pages,
+                        const int32_t *lengths, int64_t window, int64_t sinks, float alpha, void *out, void *workspace,
+                        size_t workspace_bytes, void *stream);
+
+/*
+ * Rotary positions: of the first `rotary_dim` values of a head pair j, (j, j + rotary_dim/2) or where interleaved (2j, 2j+1), is turned:
+ *   (a, b) -> (a c - b s, b c + a s),  (c, s) = table[position][j],   position = positions[axes[j] * axis_stride + t] of token t
+ * every operation rounded once in fp32.  A position outside the table gives NaN.  Values behind the first rotary_dim stay as they are.
+ */
+typedef struct bw_rotary {
+    const float *table;         /* [max_positions][rotary_dim/2][2]: cosine, sine; 16-byte aligned */
+    int64_t max_positions;
+    int rotary_dim;             /* even, 2 to 256 */
+    int interleaved;
+    int num_axes;               /* 1 to 255 */
+    const uint8_t *axes;        /* HOST memory, [rotary_dim/2]: the axis of each pair; NULL: all 0 */
+    const int64_t *positions;   /* token t of axis a at a * axis_stride + t */
+    int64_t axis_stride;
+} bw_rotary;
+
+/*
+ * Rotates the rows of x0 [tokens][heads0] and, unless heads1 is 0, x1 [tokens][heads1] (BW_F32 | BW_F16 | BW_BF16; value d of head h of token t at
+ * t*stride + h*head_stride + d) into dense out0, out1 of the same type, rounded once.  `inverse`: turned back, (a c + b s, b c - a s), which is
+ * also the gradient.  The outputs may not overlap the inputs.
+ */
+BW_API int bw_rotate(const bw_rotary *rotary, int64_t tokens, int dim, int dtype, int inverse, const void *x0, int heads0, int64_t stride0,
+              int64_t head_stride0, void *out0, const void *x1, int heads1, int64_t stride1, int64_t head_stride1, void *out1,
+              void *stream);
+
+/*
+ * bw_kv_append of rotated keys: the rows of k are rotated in fp32 and quantised from there, those of v as they are; the rows of q [tokens][q_heads]
+ * (none where q_heads is 0) are rotated into dense q_out of the same type, those of skipped slots too.
+ */
+BW_API int bw_kv_append_rotated(const bw_rotary *rotary, const void *q, int q_heads, int64_t q_stride, int64_t q_head_stride, void *q_out,
+                         const void *k, const void *v, int dtype, int64_t tokens, int64_t k_stride, int64_t k_head_stride,
+                         int64_t v_stride, int64_t v_head_stride, const int64_t *slots, int heads, int dim, int bits, int64_t pages,
+                         int page_size, int32_t *k_codes, int32_t *v_codes, void *params, void *stream);
+
+/*
+ * Log probabilities of given tokens: of row r of logits (value j at r*stride + j) and t = tokens[r]
+ *   log_probs[r] = x[t] - log sum exp x;  0 where t < 0, NaN where t >= vocab
+ *   entropy[r]   = -sum p log p  (p log p = 0 where p is 0)
+ *   top          the `top` largest logits (0 to 32, at most vocab), in falling order, equal ones by rising index (NaN before all others):
+ *                their indexes in top_tokens [rows][top], their log probabilities in top_log_probs [rows][top]
+ * A row with a NaN or +infinity, and one of nothing but -infinity, has NaN in all of these but top_tokens.
+ * entropy may be NULL; tokens and log_probs may both be NULL.  stats, [rows][4] fp32 (16-byte aligned) or NULL, takes what the gradient needs.
+ * Sums are fp32 over the largest logit.  logits BW_F32 | BW_F16 | BW_BF16; all outputs fp32 and dense.
+ */
+BW_API int bw_token_log_probs(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, float *log_probs,
+                       float *entropy, int top, float *top_log_probs, int64_t *top_tokens, float *stats, void *stream);
+/*
+ * Its gradient, into dense grad [rows][vocab] of the logits' type, rounded once; with g, e, g_i the gradients of log_probs, entropy and
+ * top_log_probs (each may be NULL: zeros; g is 0 where t < 0)
+ *   grad[j] = p[j] * (-(g + sum g_i) - e * (log p[j] + H)) + (j == t) g + sum (j == top_tokens[i]) g_i
+ */
+BW_API int bw_token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens,
+                            const float *stats, const float *grad_log_probs, const float *grad_entropy, int top,
+                            const int64_t *top_tokens, const float *grad_top, void *grad, void *stream);
+
+/*
  * Low-rank adapters of many requests beside a shared projection:
  *   h[t] = down[i] x[t],  out[t] = base[t] + scaling[i] * up[i]^T h[t],  i = index[t]
  * Rows whose index is negative have no adapter: out[t] = base[t].  An index of `adapters` or more gives NaN.
