@@ -78,7 +78,7 @@ int kv_append(const void *k, const void *v, int dtype, int64_t tokens, const int
               int64_t pages, int page_size, int32_t *kc, int32_t *vc, void *params, cudaStream_t st);
 int kv_read(const int32_t *kc, const int32_t *vc, const void *params, int heads, int dim, int bits, int64_t pages, int page_size,
             const int64_t *slots, int64_t tokens, void *k, void *v, int dtype, cudaStream_t st);
-size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages);
+size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages, int64_t window, int64_t sinks);
 int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *kc, const int32_t *vc,
               const void *params, int bits, int64_t pages, int page_size, int kv_heads, int dim, const int32_t *table, int64_t table_stride,
               int max_pages, const int32_t *lengths, int window, int sinks, float alpha, void *out, void *workspace, cudaStream_t st);
@@ -620,7 +620,7 @@ int bw_kv_read(const int32_t *k_codes, const int32_t *v_codes, const void *param
 
 size_t bw_kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages) {
     if (batch <= 0 || kv_heads < 1 || heads < kv_heads || dim < 1 || page_size < 1 || max_pages < 0) return 0;
-    return kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
+    return kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages, INT32_MAX, 0);
 }
 
 // One checked call of the cache's attention; without a window INT32_MAX tokens are visible.
@@ -653,9 +653,18 @@ int bw_kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_s
                              bw_kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages), stream);
 }
 
+// (lengths are int32: a window or sinks of more are all of them, and then it is attention without a window)
+static void window_of(int64_t window, int64_t sinks, int *w, int *s) {
+    const bool all = window >= INT32_MAX || sinks >= INT32_MAX;
+    *w = all ? INT32_MAX : (int)window;
+    *s = all ? 0 : (int)sinks;
+}
+
 size_t bw_kv_attend_window_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages, int64_t window, int64_t sinks) {
-    if (window < 0 || sinks < 0) return 0;
-    return bw_kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages);
+    if (batch <= 0 || kv_heads < 1 || heads < kv_heads || dim < 1 || page_size < 1 || max_pages < 0 || window < 0 || sinks < 0) return 0;
+    int w, s;
+    window_of(window, sinks, &w, &s);
+    return kv_attend_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages, w, s);
 }
 
 int bw_kv_attend_window(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *k_codes,
@@ -663,10 +672,10 @@ int bw_kv_attend_window(const void *q, int dtype, int64_t batch, int heads, int6
                         int64_t table_stride, int64_t max_pages, const int32_t *lengths, int64_t window, int64_t sinks, float alpha, void *out,
                         void *workspace, size_t workspace_bytes, void *stream) {
     if (window < 0 || sinks < 0) return BW_ERR_SHAPE;
-    // (lengths are int32: more than that is all of them)
-    const int w = (int)(window < INT32_MAX ? window : INT32_MAX), s = (int)(sinks < INT32_MAX ? sinks : INT32_MAX);
+    int w, s;
+    window_of(window, sinks, &w, &s);
     return kv_attend_checked(q, dtype, batch, heads, q_stride, q_head_stride, k_codes, v_codes, params, bits, pages, page_size, kv_heads, dim, page_table,
-                             table_stride, max_pages, lengths, s == INT32_MAX ? s : w, s == INT32_MAX || w == INT32_MAX ? 0 : s, alpha, out, workspace, workspace_bytes,
+                             table_stride, max_pages, lengths, w, s, alpha, out, workspace, workspace_bytes,
                              bw_kv_attend_window_workspace_bytes(batch, heads, kv_heads, dim, page_size, max_pages, window, sinks), stream);
 }
 

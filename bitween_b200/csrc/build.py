@@ -19,7 +19,7 @@ OUT_DIR = os.path.join(PKG, "_C")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(OUT_DIR, "libbitween_b200.so")
 
-SOURCES = ["api.cu", "rtn_quantize.cu", "dequantize.cu", "qmatmul_smallm.cu", "qmatmul_rows.cu", "qmatmul_decode.cu", "qmatmul_tc.cu", "qmatmul_grad_input.cu", "fake_quant.cu", "kv_cache.cu", "kv_attend.cu", "rotary.cu", "log_probs.cu", "adapters.cu", "peer_allreduce.cu"]
+SOURCES = ["api.cu", "rtn_quantize.cu", "dequantize.cu", "qmatmul_smallm.cu", "qmatmul_rows.cu", "qmatmul_decode.cu", "qmatmul_tc.cu", "qmatmul_grad_input.cu", "fake_quant.cu", "kv_cache.cu", "kv_attend.cu", "kv_attend_window.cu", "rotary.cu", "log_probs.cu", "adapters.cu", "peer_allreduce.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,0 +1,15 @@
+// The tiled kernels of attention over the quantised cache, compiled for a window and sinks: only the tiles of 16 tokens that hold a visible
+// one are in the line of work, and tokens of those tiles that are not visible are masked like those behind the sequence.
+#include "kv_attend_tiles.cuh"
+
+namespace bw {
+
+int attend_window_tiles(const AttendArgs &a, int64_t batch, int dtype, int bits, void *workspace, cudaStream_t st) {
+    FastArgs f = {};
+    if (!fast_args(f, batch, a.heads, a.kv_heads, a.dim, a.pages, a.page_size, a.max_pages, a.window, a.sinks)) return BW_ERR_UNSUPPORTED;
+    f.a = a;
+    f.slots = (float *)workspace;
+    return dtype == BW_F16 ? launch_bits<true, __half>(f, bits, st) : launch_bits<true, __nv_bfloat16>(f, bits, st);
+}
+
+}  // namespace bw
