@@ -3,20 +3,122 @@
 // Of a row x with largest value m:  s = sum 2^u, w = sum 2^u u  with u = (x - m) / ln 2;
 //     log p[j] = (x[j] - m) - ln s,   H = ln s - ln2 * w / s
 // The gradient of g log p[t] + e H + sum g_i log p[t_i] in x[j] is  p[j] (-(g + sum g_i) - e (log p[j] + H)) + (j == t) g + sum (j == t_i) g_i.
-#include "bw_common.cuh"
+//
+// One pass over the row with the running maximum; x - m is formed before the product, so that masks of the type's lowest value stay finite or become
+// exact zeros.  Sums are fp32: 32 terms (16 of fp32 logits) by themselves, then those sums, then a tree: a chain of 500 equal terms rounds the same way each time and was
+// off by 7e-6.  Bound by the bytes of the logits where there are many rows (ex2: 16 of an SM's clock, 9 TB/s of 16-bit logits), by latency where there are few.
+//
+// A row is taken by a cluster of one to eight CTAs, which join through distributed shared memory.
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+#include "early_launch.cuh"
 
 namespace bw {
 namespace {
 
-constexpr int MOST_TOP = 32;
+namespace cg = cooperative_groups;
+
+constexpr int THREADS = 256, UNROLL = 4, BLOCKS = 16;     // of a CTA; 16-byte loads of a step; blocks of steps of a thread
+constexpr int STEP = THREADS * UNROLL;                     // 16-byte pieces of a CTA's step
+constexpr int CANDIDATES = 512;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
-// The order of the alternatives: falling value, rising index; NaN before all.  Larger is better.
+// The order of the alternatives: falling value, rising index; NaN before all.  Larger is better; nothing is 0.
 __device__ __forceinline__ uint32_t order_of(float x) {
     if (x != x) return 0xfffffffeu;                       // (below the mark of no value yet, whatever the index)
     const uint32_t b = __float_as_uint(x + 0.0f);         // (-0 counts as 0)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t order) {
+    return order == 0xfffffffeu ? NAN : __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float ld_l2(const float *p) { return __ldcg(p); }
+__device__ __forceinline__ float ld_l2(const __half *p) { return __half2float(__ldcg(p)); }
+__device__ __forceinline__ float ld_l2(const __nv_bfloat16 *p) { return __bfloat162float(__ldcg(p)); }
+
+// 16 bytes of a row.
+template <typename T> struct Piece {
+    static constexpr int V = 16 / sizeof(T);
+    uint4 raw;
+    __device__ __forceinline__ void load(const T *p) { raw = __ldcg(reinterpret_cast<const uint4 *>(p)); }
+    // (in the place of pieces that are not there: -infinity)
+    __device__ __forceinline__ void nothing() {
+        const uint32_t w = __is_same(T, float) ? 0xff800000u : __is_same(T, __half) ? 0xfc00fc00u : 0xff80ff80u;
+        raw = make_uint4(w, w, w, w);
+    }
+    __device__ __forceinline__ float2 pair(int i) const {
+        const uint32_t *w = reinterpret_cast<const uint32_t *>(&raw);
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else if constexpr (__is_same(T, __half)) return __half22float2(*reinterpret_cast<const __half2 *>(w + i));
+        else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+    __device__ __forceinline__ void put(int i, float2 v) {
+        uint32_t *w = reinterpret_cast<uint32_t *>(&raw);
+        if constexpr (sizeof(T) == 4) {
+            w[2 * i] = __float_as_uint(v.x);
+            w[2 * i + 1] = __float_as_uint(v.y);
+        } else if constexpr (__is_same(T, __half)) *reinterpret_cast<__half2 *>(w + i) = __float22half2_rn(v);
+        else *reinterpret_cast<__nv_bfloat162 *>(w + i) = __float22bfloat162_rn(v);
+    }
+};
+// The largest value of pieces; NaN where there is one.
+template <typename T>
+__device__ __forceinline__ float largest(const Piece<T> (&x)[UNROLL]) {
+    if constexpr (sizeof(T) == 4) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) m = max_nan(m, max_nan(x[u].pair(i).x, x[u].pair(i).y));
+        return m;
+    } else {
+        using T2 = typename std::conditional<__is_same(T, __half), __half2, __nv_bfloat162>::type;
+        T2 m = *reinterpret_cast<const T2 *>(&x[0].raw.x);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = __hmax2_nan(m, reinterpret_cast<const T2 *>(&x[u].raw)[i]);
+        return max_nan(to_f32(m.x), to_f32(m.y));
+    }
+}
+
+// The running maximum and sums of some values of a row.
+struct Sums {
+    float m, s, w;
+    // To a larger maximum.  (Without a value above -infinity there is nothing to keep, but for a NaN.)
+    __device__ __forceinline__ void raise(float to) {
+        if (m == -INFINITY) {
+            s *= 0.0f;
+            w = 0.0f;
+        } else {
+            // (products rounded by themselves: the same log probability whatever else is asked for)
+            const float d = __fmul_rn(m - to, LOG2E), f = ex2(d);
+            // (what fell by so much that nothing of it is left: infinite d)
+            w = f == 0.0f ? 0.0f : f * fmaf(s, d, w);
+            s = __fmul_rn(s, f);
+        }
+        m = to;
+    }
+    __device__ __forceinline__ void add(Sums o) {
+        if (o.m > m) raise(o.m);
+        else if (o.m < m) o.raise(m);
+        s += o.s;
+        w += o.w;
+    }
+};
 
 struct LogProbs {
     const void *logits;
@@ -25,86 +127,330 @@ struct LogProbs {
     int64_t *top_tokens;
     float4 *stats;                       // m, log2 s, H
     int64_t stride;
-    int vocab, top;
+    int vocab, top, cluster;
 };
 
-// Any size and stride: a CTA a row, and a pass over the row for each alternative.
-template <typename T>
-__global__ void __launch_bounds__(256) log_probs_general_kernel(const LogProbs p) {
-    const int64_t row = blockIdx.x;
-    const T *x = (const T *)p.logits + row * p.stride;
-    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    __shared__ float s_a[8], s_b[8];
-    __shared__ uint64_t s_best[8];
-    // the largest value; NaN if there is one
-    float m = -INFINITY;
-    bool nan = false;
-    for (int j = tid; j < p.vocab; j += 256) {
-        const float v = to_f32(x[j]);
-        nan |= v != v;
-        m = fmaxf(m, v);
+// A row as 16-byte pieces on their boundaries and the values before and behind them (`extra` of them), which rank 0 takes; and a rank's share of the pieces.
+template <typename T> struct Row {
+    const T *x;
+    int head, behind, extra, v0, v1;
+    __device__ __forceinline__ Row(const T *row, int vocab, int rank, int ranks) : x(row) {
+        constexpr int V = Piece<T>::V;
+        head = (int)((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16 / sizeof(T));
+        if (head > vocab) head = vocab;
+        const int pieces = (vocab - head) / V, each = (pieces + ranks - 1) / ranks;
+        behind = head + pieces * V;
+        extra = rank == 0 ? head + vocab - behind : 0;
+        v0 = rank * each < pieces ? rank * each : pieces;
+        v1 = v0 + each < pieces ? v0 + each : pieces;
     }
-    if (nan) m = INFINITY;
-    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    if (lane == 0) s_a[warp] = m;
+    __device__ __forceinline__ const T *piece(int v) const { return x + head + (int64_t)v * Piece<T>::V; }
+    __device__ __forceinline__ int extra_at(int i) const { return i < head ? i : behind + i - head; }
+};
+
+struct __align__(16) TopScratch {
+    float largest[BLOCKS + 1][THREADS];  // of a thread's blocks, and of its extra value
+    __align__(16) uint32_t key[THREADS];
+    __align__(16) uint64_t list[CANDIDATES + 2];      // (order << 32) | ~index
+    uint64_t best[32];
+    uint32_t histogram[256];
+    int count, blocks, need;
+    uint32_t least, prefix;
+    int scan[THREADS / 32];
+};
+
+__device__ __forceinline__ uint64_t candidate(float x, int at) { return (uint64_t)order_of(x) << 32 | (uint32_t)~at; }
+
+// The best `top` of n candidates, in order, into `best`; 0 where there are fewer.  All candidates differ.
+__device__ __forceinline__ void rank_candidates(TopScratch &s, int n, int top) {
+    const int tid = threadIdx.x;
+    if (tid < top) s.best[tid] = 0;
+    if (tid < 2) s.list[n + tid] = 0;
     __syncthreads();
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, s_a[i]);
-    __syncthreads();
-    // (a thread's sums in blocks of 32: equal values round the same way each time, and 500 of them in a row were off by 100 half steps)
-    float s = 0.0f, w = 0.0f;
-    for (int j0 = tid; j0 < p.vocab; j0 += 32 * 256) {
-        float sb = 0.0f, wb = 0.0f;
-        for (int j = j0; j < p.vocab && j < j0 + 32 * 256; j += 256) {
-            const float u = (to_f32(x[j]) - m) * LOG2E, e = exp2f(u);
-            sb += e;
-            wb += e == 0.0f ? 0.0f : e * u;
+    for (int i = tid; i < n; i += THREADS) {
+        const uint64_t mine = s.list[i];
+        int before = 0;
+        for (int k = 0; k < n; k += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(s.list + k);
+            before += (two.x > mine) + (two.y > mine);
         }
-        s += sb;
-        w += wb;
+        if (before < top) s.best[before] = mine;
+    }
+    __syncthreads();
+}
+
+// The best `top` values of a rank's share.  A thread's largest value is `key`; those of its blocks of `per` steps lie in s.largest.
+//
+// The top-th largest of the threads' largest values is a bound from below.  Only blocks that reach it are read again, some more than `top` of them, and the
+// values that reach it are ranked.  Where too many do (many equal values, as masks leave them; many large ones in few threads' places) the bound is
+// found digit by digit over the whole share instead.
+template <typename T>
+__device__ __forceinline__ void find_top(TopScratch &s, const Row<T> &row, int top, int blocks, int per, uint32_t key) {
+    constexpr int V = Piece<T>::V;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    s.key[tid] = key;
+    if (tid == 0) {
+        s.count = s.blocks = 0;
+        s.least = 0xffffffffu;
+    }
+    __syncthreads();
+    int larger = 0;
+    for (int i = 0; i < THREADS; i += 4) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(s.key + i);
+        larger += (k.x > key) + (k.y > key) + (k.z > key) + (k.w > key);
+    }
+    const uint32_t low = __reduce_min_sync(0xffffffffu, larger < top ? key : 0xffffffffu);
+    if (lane == 0) atomicMin(&s.least, low);
+    __syncthreads();
+    const uint32_t least = s.least;
+    if (key >= least) {
+        for (int b = 0; b <= BLOCKS; ++b) {
+            if (b < BLOCKS ? b >= blocks : tid >= row.extra) continue;
+            if (order_of(s.largest[b][tid]) >= least) {
+                const int i = atomicAdd(&s.blocks, 1);
+                if (i < THREADS) s.key[i] = b * THREADS + tid;          // (the threads' keys have been read)
+            }
+        }
+    }
+    __syncthreads();
+    const int listed = s.blocks;
+    auto offer = [&](float x, int at) {
+        if (order_of(x) < least) return;
+        const int i = atomicAdd(&s.count, 1);
+        if (i < CANDIDATES) s.list[i] = candidate(x, at);
+    };
+    if (listed <= THREADS) {
+        for (int i = warp; i < listed; i += THREADS / 32) {
+            const int b = (int)s.key[i] / THREADS, t = (int)s.key[i] % THREADS;
+            if (b == BLOCKS) {
+                if (lane == 0) offer(s.largest[b][t], row.extra_at(t));
+                continue;
+            }
+            for (int e = lane; e < per * UNROLL * V; e += 32) {
+                const int v = row.v0 + (b * per + e / (UNROLL * V)) * STEP + e / V % UNROLL * THREADS + t;
+                if (v < row.v1) {
+                    const int at = row.head + v * V + e % V;
+                    offer(ld_l2(row.x + at), at);
+                }
+            }
+        }
+        __syncthreads();
+        const int n = s.count;
+        if (n <= CANDIDATES) {
+            rank_candidates(s, n, top);
+            return;
+        }
+    }
+    // The top-th largest value of the share, eight bits at a time: `prefix`; `need` of those that equal it are taken, the first ones.
+    __syncthreads();
+    if (tid == 0) {
+        s.prefix = 0;
+        s.need = top;
+        s.count = 0;
+    }
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        s.histogram[tid] = 0;
+        __syncthreads();
+        const uint32_t prefix = s.prefix;
+        auto count = [&](float x) {
+            const uint32_t o = order_of(x);
+            if (shift == 24 || o >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s.histogram[o >> shift & 255], 1u);
+        };
+        for (int v = row.v0 + tid; v < row.v1; v += THREADS) {
+            Piece<T> x;
+            x.load(row.piece(v));
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                count(x.pair(i).x);
+                count(x.pair(i).y);
+            }
+        }
+        if (tid < row.extra) count(ld_l2(row.x + row.extra_at(tid)));
+        __syncthreads();
+        if (tid == 0) {
+            int need = s.need, digit = 255;
+            while (digit > 0 && (int)s.histogram[digit] < need) need -= (int)s.histogram[digit--];
+            s.need = need;
+            s.prefix = prefix | (uint32_t)digit << shift;
+        }
+        __syncthreads();
+    }
+    const uint32_t bound = s.prefix;
+    const int need = s.need;
+    // (fewer than `top` values are larger; of the equal ones the first `need` in rising order: before the pieces, in them, behind them)
+    int taken = 0;
+    auto round = [&](const float (&x)[V], int n, int at) {      // n values of this thread from index `at` on; threads' indexes rise
+        int equal = 0;
+        for (int i = 0; i < V; ++i)
+            if (i < n) {
+                const uint32_t o = order_of(x[i]);
+                if (o > bound) {
+                    const int k = atomicAdd(&s.count, 1);
+                    if (k < CANDIDATES) s.list[k] = candidate(x[i], at + i);
+                }
+                equal += o == bound;
+            }
+        if (!__syncthreads_or(equal)) return;
+        int sum = equal;
+        for (int d = 1; d < 32; d *= 2) {
+            const int o = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += o;
+        }
+        if (lane == 31) s.scan[warp] = sum;
+        __syncthreads();
+        int before = taken + sum - equal, all = 0;
+        for (int i = 0; i < THREADS / 32; ++i) {
+            before += i < warp ? s.scan[i] : 0;
+            all += s.scan[i];
+        }
+        for (int i = 0; i < V; ++i)
+            if (i < n && order_of(x[i]) == bound && before++ < need) {
+                const int k = atomicAdd(&s.count, 1);
+                if (k < CANDIDATES) s.list[k] = candidate(x[i], at + i);
+            }
+        taken += all;
+        __syncthreads();
+    };
+    float x[V];
+    const int head = row.extra ? row.head : 0;
+    x[0] = tid < head ? ld_l2(row.x + tid) : 0.0f;
+    round(x, tid < head, tid);
+    for (int v0 = row.v0; v0 < row.v1; v0 += THREADS) {
+        Piece<T> piece;
+        if (v0 + tid < row.v1) piece.load(row.piece(v0 + tid));
+        else piece.nothing();
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            x[2 * i] = piece.pair(i).x;
+            x[2 * i + 1] = piece.pair(i).y;
+        }
+        round(x, v0 + tid < row.v1 ? V : 0, row.head + (v0 + tid) * V);
+    }
+    const int rest = row.extra - head;
+    x[0] = tid < rest ? ld_l2(row.x + row.behind + tid) : 0.0f;
+    round(x, tid < rest, row.behind + tid);
+    __syncthreads();
+    rank_candidates(s, s.count < CANDIDATES ? s.count : CANDIDATES, top);
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const LogProbs p) {
+    constexpr int V = Piece<T>::V;
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+    const int rank = (int)(blockIdx.x % p.cluster);
+    const int64_t r = blockIdx.x / p.cluster;
+    __shared__ Sums s_warp[THREADS / 32], s_all;
+    __shared__ typename std::conditional<TOP, TopScratch, int>::type s_top;
+    pdl_wait();
+    pdl_launch_dependents();
+    const Row<T> row((const T *)p.logits + r * p.stride, p.vocab, rank, p.cluster);
+    const int64_t t = p.tokens ? __ldcg(p.tokens + r) : -1;
+    if (!ENTROPY && !TOP && t < 0) {         // padding: nothing of the row is asked for
+        if (rank == 0 && tid == 0) {
+            if (p.tokens) p.log_probs[r] = 0.0f;
+            if (p.stats) p.stats[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        return;
+    }
+    const float xt = t >= 0 && t < p.vocab ? ld_l2(row.x + t) : NAN;
+
+    const int steps = (row.v1 - row.v0 + STEP - 1) / STEP, per = (steps + BLOCKS - 1) / BLOCKS;
+    Sums a = {-INFINITY, 0.0f, 0.0f};
+    uint32_t key = 0;
+    float block = -INFINITY;
+    int in_block = 0, blocks = 0;
+    Piece<T> next[UNROLL];
+    auto load = [&](int step) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int v = row.v0 + step * STEP + u * THREADS + tid;
+            if (v < row.v1) next[u].load(row.piece(v));
+            else next[u].nothing();
+        }
+    };
+    if (steps) load(0);
+    for (int step = 0; step < steps; ++step) {
+        Piece<T> x[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) x[u] = next[u];
+        if (step + 1 < steps) load(step + 1);
+        const float m = largest(x);
+        if (m > a.m) a.raise(m);
+        if constexpr (TOP) {
+            block = max_nan(block, m);
+            if (++in_block == per || step + 1 == steps) {
+                s_top.largest[blocks++][tid] = block;
+                key = max(key, order_of(block));
+                block = -INFINITY;
+                in_block = 0;
+            }
+        }
+        const float by = a.m == -INFINITY ? 0.0f : -a.m;
+        float2 s = {0.0f, 0.0f}, w = {0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 d = fmul2(fadd2(x[u].pair(i), make_float2(by, by)), make_float2(LOG2E, LOG2E)), e = make_float2(ex2(d.x), ex2(d.y));
+                s = fadd2(s, e);
+                // (0 * -infinity is not wanted: below 2^-1000 a weight is 0.  NaN stands in s.)
+                if constexpr (ENTROPY) w = ffma2(e, make_float2(fmaxf(d.x, -1000.0f), fmaxf(d.y, -1000.0f)), w);
+            }
+        a.s += s.x + s.y;
+        if constexpr (ENTROPY) a.w += w.x + w.y;
+    }
+    if (tid < row.extra) {
+        const float x = ld_l2(row.x + row.extra_at(tid));
+        if constexpr (TOP) {
+            s_top.largest[BLOCKS][tid] = x;
+            key = max(key, order_of(x));
+        }
+        // (NaN is larger than no maximum: its difference goes into the sum)
+        if (x > a.m) a.raise(x);
+        const float d = __fmul_rn(x - (a.m == -INFINITY ? 0.0f : a.m), LOG2E), e = ex2(d);
+        a.s += e;
+        if constexpr (ENTROPY) a.w += e * fmaxf(d, -1000.0f);
     }
     for (int d = 16; d; d >>= 1) {
-        s += __shfl_xor_sync(0xffffffffu, s, d);
-        w += __shfl_xor_sync(0xffffffffu, w, d);
+        const Sums o = {__shfl_xor_sync(0xffffffffu, a.m, d), __shfl_xor_sync(0xffffffffu, a.s, d), ENTROPY ? __shfl_xor_sync(0xffffffffu, a.w, d) : 0.0f};
+        a.add(o);
     }
-    if (lane == 0) {
-        s_a[warp] = s;
-        s_b[warp] = w;
-    }
+    if (lane == 0) s_warp[warp] = a;
     __syncthreads();
-    s = w = 0.0f;
-    for (int i = 0; i < 8; ++i) {
-        s += s_a[i];
-        w += s_b[i];
+    a = s_warp[0];
+    for (int i = 1; i < THREADS / 32; ++i) a.add(s_warp[i]);
+    if constexpr (TOP) find_top(s_top, row, p.top, blocks, per, key);
+    if (p.cluster > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        if (tid == 0) s_all = a;
+        cluster.sync();
+        if (rank == 0) {
+            for (int i = 1; i < p.cluster; ++i) a.add(*cluster.map_shared_rank(&s_all, i));
+            if constexpr (TOP) {
+                // the ranks' best become one list
+                const int n = p.cluster * p.top;
+                if (tid < n) s_top.list[tid] = *cluster.map_shared_rank(&s_top.best[tid % p.top], tid / p.top);
+                __syncthreads();
+                // (a share of few values has less than `top`: zeros, of which none comes before a value)
+                rank_candidates(s_top, n, p.top);
+            }
+        }
+        cluster.sync();
+        if (rank != 0) return;
     }
     // (infinities of either sign as the largest value, and NaN: nothing is known of the row)
-    const float log2s = fabsf(m) == INFINITY ? NAN : log2f(s), ln_s = LN2 * log2s, h = ln_s - LN2 * (w / s);
+    const float log2s = fabsf(a.m) == INFINITY ? NAN : log2f(a.s), ln_s = __fmul_rn(LN2, log2s), h = ENTROPY ? ln_s - LN2 * (a.w / a.s) : 0.0f;
     if (tid == 0) {
-        if (p.tokens) {
-            const int64_t t = p.tokens[row];
-            p.log_probs[row] = t < 0 ? 0.0f : t >= p.vocab ? NAN : (to_f32(x[t]) - m) - ln_s;
-        }
-        if (p.entropy) p.entropy[row] = h;
-        if (p.stats) p.stats[row] = make_float4(m, log2s, h, 0.0f);
+        if (p.tokens) p.log_probs[r] = t < 0 ? 0.0f : (xt - a.m) - ln_s;
+        if (ENTROPY) p.entropy[r] = h;
+        if (p.stats) p.stats[r] = make_float4(a.m, log2s, h, 0.0f);
     }
-    uint64_t last = ~0ull;               // (order << 32) | ~index
-    for (int i = 0; i < p.top; ++i) {
-        uint64_t best = 0;
-        for (int j = tid; j < p.vocab; j += 256) {
-            const uint64_t key = (uint64_t)order_of(to_f32(x[j])) << 32 | (uint32_t)~j;
-            if (key < last && key > best) best = key;
+    if constexpr (TOP)
+        if (tid < p.top) {
+            const uint64_t best = s_top.best[tid];
+            p.top_tokens[r * p.top + tid] = (uint32_t)~best;
+            p.top_log_probs[r * p.top + tid] = (value_of((uint32_t)(best >> 32)) - a.m) - ln_s;
         }
-        for (int d = 16; d; d >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
-        __syncthreads();
-        if (lane == 0) s_best[warp] = best;
-        __syncthreads();
-        for (int k = 0; k < 8; ++k) best = max(best, s_best[k]);
-        last = best;
-        const uint32_t at = ~(uint32_t)best;
-        if (tid == 0 && at < (uint32_t)p.vocab) {
-            p.top_tokens[row * p.top + i] = at;
-            p.top_log_probs[row * p.top + i] = (to_f32(x[at]) - m) - ln_s;
-        }
-    }
 }
 
 struct LogProbsGrad {
@@ -114,48 +460,127 @@ struct LogProbsGrad {
     const float4 *stats;
     const float *g, *e, *g_top;
     int64_t stride;
-    int vocab, top;
+    int vocab, top, parts;               // parts: CTAs of a row
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) log_probs_grad_general_kernel(const LogProbsGrad p) {
-    const int64_t row = blockIdx.x;
-    const T *x = (const T *)p.logits + row * p.stride;
-    T *out = (T *)p.grad + row * p.vocab;
-    const float4 st = p.stats[row];
-    const int64_t t = p.tokens ? p.tokens[row] : -1;
-    const float g = p.g && t >= 0 ? (t < p.vocab ? p.g[row] : NAN) : 0.0f, e = p.e ? p.e[row] : 0.0f;
+// Bound by the bytes of the logits and of their gradient.  ALIGNED: pieces of a row start where those of its gradient do.  The entries of the tokens are written again
+// behind a barrier, by themselves: no comparison in the loop.
+template <typename T, bool ENTROPY, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogProbsGrad p) {
+    constexpr int V = Piece<T>::V;
+    const int tid = threadIdx.x, part = (int)(blockIdx.x % p.parts);
+    const int64_t r = blockIdx.x / p.parts;
+    pdl_wait();
+    pdl_launch_dependents();
+    const T *x = (const T *)p.logits + r * p.stride;
+    T *out = (T *)p.grad + r * p.vocab;
+    const float4 st = __ldcg(p.stats + r);
+    const int64_t t = p.g ? __ldcg(p.tokens + r) : -1;
+    const float g = t < 0 ? 0.0f : t < p.vocab ? __ldcg(p.g + r) : NAN, e = ENTROPY ? __ldcg(p.e + r) : 0.0f;
+    const int top = p.g_top ? p.top : 0;
     float all = g;
-    if (p.g_top)
-        for (int i = 0; i < p.top; ++i) all += p.g_top[row * p.top + i];
-    const float c = -fmaf(e, st.z, all);
-    for (int j = threadIdx.x; j < p.vocab; j += 256) {
-        const float u = (to_f32(x[j]) - st.x) * LOG2E - st.y, prob = exp2f(u);
-        float v = prob == 0.0f ? 0.0f : prob * fmaf(-e * LN2, u, c);
-        if (j == t) v += g;
-        if (p.g_top)
-            for (int i = 0; i < p.top; ++i)
-                if (p.top_tokens[row * p.top + i] == j) v += p.g_top[row * p.top + i];
-        out[j] = from_f32<T>(v);
+    bool any = g != 0.0f || e != 0.0f;
+    for (int i = 0; i < top; ++i) {
+        const float gi = __ldcg(p.g_top + r * top + i);
+        all += gi;
+        any |= gi != 0.0f;
+    }
+    const float c = -fmaf(e, st.z, all), slope = -e * LN2;
+    auto value = [&](float v) {
+        const float u = fmaf(v - st.x, LOG2E, -st.y);
+        // (0 * -infinity is not wanted: where a probability is 0, so is its gradient)
+        return ex2(u) * (ENTROPY ? fmaf(slope, fmaxf(u, -1000.0f), c) : c);
+    };
+    const Row<T> row(ALIGNED ? x : (const T *)out, p.vocab, part, p.parts);      // (of the gradient's boundaries where they differ)
+    if (!any) {                          // a row that nothing is asked of (padding): zeros, whatever stands in it
+        for (int v = row.v0 + tid; v < row.v1; v += THREADS) *reinterpret_cast<uint4 *>(out + row.head + (int64_t)v * V) = make_uint4(0, 0, 0, 0);
+        if (tid < row.extra) out[row.extra_at(tid)] = from_f32<T>(0.0f);
+        return;
+    }
+    const int steps = (row.v1 - row.v0 + STEP - 1) / STEP;
+    Piece<T> next[UNROLL];
+    auto load = [&](int step) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int v = row.v0 + step * STEP + u * THREADS + tid;
+            if (v >= row.v1) continue;
+            if constexpr (ALIGNED) next[u].load(row.piece(v));
+            else
+#pragma unroll
+                for (int i = 0; i < V / 2; ++i) next[u].put(i, make_float2(ld_l2(x + row.head + v * V + 2 * i), ld_l2(x + row.head + v * V + 2 * i + 1)));
+        }
+    };
+    if (steps) load(0);
+    for (int step = 0; step < steps; ++step) {
+        Piece<T> y[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) y[u] = next[u];
+        if (step + 1 < steps) load(step + 1);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int v = row.v0 + step * STEP + u * THREADS + tid;
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) {
+                const float2 d = ffma2(fadd2(y[u].pair(i), make_float2(-st.x, -st.x)), make_float2(LOG2E, LOG2E), make_float2(-st.y, -st.y));
+                const float2 prob = make_float2(ex2(d.x), ex2(d.y));
+                float2 f = make_float2(c, c);
+                if constexpr (ENTROPY) f = ffma2(make_float2(slope, slope), make_float2(fmaxf(d.x, -1000.0f), fmaxf(d.y, -1000.0f)), f);
+                y[u].put(i, fmul2(prob, f));
+            }
+            if (v < row.v1) __stcs(reinterpret_cast<uint4 *>(out + row.head + (int64_t)v * V), y[u].raw);
+        }
+    }
+    if (tid < row.extra) out[row.extra_at(tid)] = from_f32<T>(value(ld_l2(x + row.extra_at(tid))));
+    __syncthreads();
+    if (tid <= top) {
+        const int64_t at = tid < top ? __ldcg(p.top_tokens + r * top + tid) : t;
+        const int64_t from = row.head + (int64_t)row.v0 * V, to = row.head + (int64_t)row.v1 * V;
+        const bool mine = (at >= from && at < to) || (part == 0 && ((at >= 0 && at < row.head) || (at >= row.behind && at < p.vocab)));
+        if (mine) {
+            float v = value(ld_l2(x + at)), more = at == t ? g : 0.0f;
+            for (int i = 0; i < top; ++i)
+                if (__ldcg(p.top_tokens + r * top + i) == at) more += __ldcg(p.g_top + r * top + i);
+            out[at] = from_f32<T>(v + more);
+        }
     }
 }
 
-template <typename T>
-int log_probs_typed(const LogProbs &p, int64_t rows, cudaStream_t st) {
-    log_probs_general_kernel<T><<<(unsigned)rows, 256, 0, st>>>(p);
-    return check_launch("log_probs_general_kernel");
+// CTAs of a row: so many that all rows together fill the SMs eight times over with 256 threads, of at least a step (16 KB) each.
+int ctas_of(int64_t rows, int64_t vocab, size_t size) {
+    int n = 1;
+    while (n < 8 && rows * n < 148 * 8 && vocab * (int64_t)size > (int64_t)n * STEP * 16) n *= 2;
+    return n;
+}
+
+template <typename T, bool ENTROPY, bool TOP>
+int log_probs_launch(const LogProbs &p, int64_t rows, cudaStream_t st) {
+    return launch_early("log_probs_kernel", log_probs_kernel<T, ENTROPY, TOP>, dim3((unsigned)(rows * p.cluster)), THREADS, 0, st, dim3(p.cluster), p);
 }
 template <typename T>
-int log_probs_grad_typed(const LogProbsGrad &p, int64_t rows, cudaStream_t st) {
-    log_probs_grad_general_kernel<T><<<(unsigned)rows, 256, 0, st>>>(p);
-    return check_launch("log_probs_grad_general_kernel");
+int log_probs_typed(LogProbs &p, int64_t rows, cudaStream_t st) {
+    p.cluster = ctas_of(rows, p.vocab, sizeof(T));
+    if (p.top) return p.entropy ? log_probs_launch<T, true, true>(p, rows, st) : log_probs_launch<T, false, true>(p, rows, st);
+    return p.entropy ? log_probs_launch<T, true, false>(p, rows, st) : log_probs_launch<T, false, false>(p, rows, st);
+}
+
+template <typename T, bool ENTROPY, bool ALIGNED>
+int log_probs_grad_launch(const LogProbsGrad &p, int64_t rows, cudaStream_t st) {
+    return launch_early("log_probs_grad_kernel", log_probs_grad_kernel<T, ENTROPY, ALIGNED>, dim3((unsigned)(rows * p.parts)), THREADS, 0, st, dim3(1), p);
+}
+template <typename T>
+int log_probs_grad_typed(LogProbsGrad &p, int64_t rows, cudaStream_t st) {
+    p.parts = ctas_of(rows, p.vocab, sizeof(T));
+    const uintptr_t apart = (reinterpret_cast<uintptr_t>(p.logits) - reinterpret_cast<uintptr_t>(p.grad)) % 16;
+    const bool aligned = apart == 0 && (rows == 1 || (p.stride - p.vocab) * (int64_t)sizeof(T) % 16 == 0);
+    if (p.e) return aligned ? log_probs_grad_launch<T, true, true>(p, rows, st) : log_probs_grad_launch<T, true, false>(p, rows, st);
+    return aligned ? log_probs_grad_launch<T, false, true>(p, rows, st) : log_probs_grad_launch<T, false, false>(p, rows, st);
 }
 
 }  // namespace
 
 int token_log_probs(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, float *log_probs, float *entropy,
                     int top, float *top_log_probs, int64_t *top_tokens, float *stats, cudaStream_t st) {
-    const LogProbs p = {logits, tokens, log_probs, entropy, top_log_probs, top_tokens, (float4 *)stats, stride, (int)vocab, top};
+    LogProbs p = {logits, tokens, log_probs, entropy, top_log_probs, top_tokens, (float4 *)stats, stride, (int)vocab, top, 1};
     if (dtype == BW_F32) return log_probs_typed<float>(p, rows, st);
     if (dtype == BW_F16) return log_probs_typed<__half>(p, rows, st);
     return log_probs_typed<__nv_bfloat16>(p, rows, st);
@@ -163,7 +588,7 @@ int token_log_probs(const void *logits, int dtype, int64_t rows, int64_t vocab, 
 
 int token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, const float *stats,
                          const float *g, const float *e, int top, const int64_t *top_tokens, const float *g_top, void *grad, cudaStream_t st) {
-    const LogProbsGrad p = {logits, grad, tokens, top_tokens, (const float4 *)stats, g, e, g_top, stride, (int)vocab, top};
+    LogProbsGrad p = {logits, grad, tokens, top_tokens, (const float4 *)stats, g, e, g_top, stride, (int)vocab, top, 1};
     if (dtype == BW_F32) return log_probs_grad_typed<float>(p, rows, st);
     if (dtype == BW_F16) return log_probs_grad_typed<__half>(p, rows, st);
     return log_probs_grad_typed<__nv_bfloat16>(p, rows, st);

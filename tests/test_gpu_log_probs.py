@@ -120,6 +120,33 @@ def test_rows_at_the_edges(vocab, dtype):
     assert float(r.log_probs[2]) == 0.0 and float(r.entropy[2]) == 0.0
 
 
+@pytest.mark.parametrize("vocab", [40, 9001, 131072])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_a_nan_beside_masked_values_is_not_lost(vocab, dtype):
+    """NaN where nothing else of a thread's first values is finite, at every place in turn of some rows."""
+    places = sorted({0, 1, 7, 8, 9, vocab // 3, vocab - 9, vocab - 1})
+    x = torch.full((2 * len(places), vocab), -math.inf, device=DEV)
+    x[:, vocab // 2:] = torch.randn(len(x), vocab - vocab // 2, generator=_gen(18), device=DEV)
+    for i, at in enumerate(places):
+        x[2 * i, at] = math.nan
+        x[2 * i + 1, at] = math.inf
+    x = x.to(dtype)
+    r = token_log_probs(x, torch.full((len(x),), vocab - 2, device=DEV), entropy=True, top=3)
+    assert bool(r.log_probs.isnan().all()) and bool(r.entropy.isnan().all()) and bool(r.top_log_probs.isnan().all())
+    assert torch.equal(r.top_tokens, _order(x, 3))
+
+
+def test_padding_reads_nothing_of_its_row():
+    """Rows that no token, entropy or alternative is asked of: 0 and a gradient of 0, whatever stands in them."""
+    x = _logits(6, 50272, torch.bfloat16, 19)
+    x[1], x[4, 77] = math.nan, math.inf
+    tokens = torch.tensor([5, -100, 9, 50271, -1, 0], device=DEV)
+    x.requires_grad_()
+    r = token_log_probs(x, tokens)
+    (dx,) = torch.autograd.grad(r.log_probs, x, torch.ones(6, device=DEV))
+    assert not bool(r.log_probs[[1, 4]].any()) and not bool(dx[[1, 4]].any()) and bool(dx[[0, 2, 3, 5]].isfinite().all()) and bool(dx[[0, 2, 3, 5]].any(-1).all())
+
+
 def _grads(x, tokens, g, e, top_tokens=None, g_top=None):
     """The formula, and a bound of what fp32 leaves out: (gradient, size)."""
     lp, _, h = _want(x, tokens)
