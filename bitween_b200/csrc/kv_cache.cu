@@ -17,9 +17,6 @@
 namespace bw {
 namespace {
 
-constexpr float MAGIC = 12582912.0f;                         // 1.5 * 2^23: the sum of 0 <= t <= 255 and this has rint(t) in its low bits
-constexpr uint32_t MAGIC_BITS = 0x4B400000u;
-
 // (From L2, as all that a kernel before may have written: the SM's L1 may hold lines from before this kernel's start, at which they were still being written.)
 __device__ __forceinline__ float ld_l2(const float *p) { return __ldcg(p); }
 __device__ __forceinline__ __half ld_l2(const __half *p) { return __ldcg(p); }

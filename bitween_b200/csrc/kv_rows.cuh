@@ -37,6 +37,9 @@ __device__ __forceinline__ int64_t cache_row(const KvRows &p, int64_t slot, int 
 // fp16 not below s (finite, positive), at least 2^-24; infinity beyond fp16's range.
 __device__ __forceinline__ __half scale_up(float s) { return __float2half_ru(fmaxf(s, 0x1p-24f)); }
 
+constexpr float MAGIC = 12582912.0f;                         // 1.5 * 2^23: the sum of 0 <= t <= 255 and this has rint(t) in its low bits
+constexpr uint32_t MAGIC_BITS = 0x4B400000u;
+
 // min and max that keep NaN
 __device__ __forceinline__ float min_nan(float a, float b) {
     float y;
