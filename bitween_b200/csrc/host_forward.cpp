@@ -29,6 +29,9 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <array>
+#include <cstring>
+
 #include "bitween_b200.h"
 
 namespace {
@@ -134,7 +137,7 @@ PyObject *set_entry(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     Py_RETURN_NONE;
 }
 
-// ---- the quantised key-value cache and the adapters ------------------------------------------------------------------
+// ---- the quantised key-value cache, rotary positions, the adapters, log probabilities --------------------------------
 // None, again, for every call that is not plain (the Python path converts, copies or raises).  Scratch comes from the caching allocator, so
 // that calls of other streams, threads and graphs have their own.
 
@@ -145,7 +148,7 @@ using KvAttendBytes = decltype(&bw_kv_attend_workspace_bytes);
 using AdapterBytes = decltype(&bw_adapter_hidden_bytes);
 using AdapterForward = decltype(&bw_adapter_forward);
 using AdapterBackward = decltype(&bw_adapter_backward);
-struct Operators {
+struct Operators {                        // in the order of set_operators
     KvAppend kv_append;
     KvRead kv_read;
     KvAttend kv_attend;
@@ -153,7 +156,14 @@ struct Operators {
     AdapterBytes adapter_bytes;
     AdapterForward adapter_forward;
     AdapterBackward adapter_backward;
+    decltype(&bw_kv_attend_window) kv_attend_window;
+    decltype(&bw_kv_attend_window_workspace_bytes) kv_attend_window_bytes;
+    decltype(&bw_rotate) rotate;
+    decltype(&bw_kv_append_rotated) kv_append_rotated;
+    decltype(&bw_token_log_probs) token_log_probs;
+    decltype(&bw_token_log_probs_grad) token_log_probs_grad;
 } g_ops = {};
+constexpr int OPERATORS = sizeof(Operators) / sizeof(void *);
 
 int float_code(at::ScalarType t) { return t == at::kHalf ? BW_F16 : t == at::kBFloat16 ? BW_BF16 : t == at::kFloat ? BW_F32 : -1; }
 
@@ -255,11 +265,21 @@ PyObject *kv_read(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
-// kv_attend(k_codes, v_codes, params, bits, q, page_table, lengths, softmax_scale): the attended values
+// kv_attend(k_codes, v_codes, params, bits, q, page_table, lengths, softmax_scale[, window, sinks]): the attended values
 PyObject *kv_attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     HANDLE_TH_ERRORS
     Cache c;
-    if (nargs != 8 || !g_ops.kv_attend || !PyFloat_CheckExact(args[7]) || !c.of(args)) Py_RETURN_NONE;
+    if ((nargs != 8 && nargs != 10) || !g_ops.kv_attend || !PyFloat_CheckExact(args[7]) || !c.of(args)) Py_RETURN_NONE;
+    int64_t window = -1, sinks = 0;
+    if (nargs == 10) {
+        if (!PyLong_CheckExact(args[8]) || !PyLong_CheckExact(args[9])) Py_RETURN_NONE;
+        window = PyLong_AsLongLong(args[8]);
+        sinks = PyLong_AsLongLong(args[9]);
+        if (window < 0 || sinks < 0) {
+            PyErr_Clear();
+            Py_RETURN_NONE;
+        }
+    }
     const at::Tensor *q = tensor_of(args[4]), *table = tensor_of(args[5]), *lengths = tensor_of(args[6]);
     if (!usable(q, c.device) || !usable(table, c.device) || !dense(lengths, c.device) || (c10::GradMode::is_enabled() && q->requires_grad())) Py_RETURN_NONE;
     const int code = float_code(q->scalar_type());
@@ -274,15 +294,49 @@ PyObject *kv_attend(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         pybind11::gil_scoped_release no_gil;
         const int heads = (int)q->size(1);
         out = fresh({batch, heads, c.dim}, q->scalar_type(), c.device);
-        const at::Tensor ws = bytes_of(g_ops.kv_attend_bytes(batch, heads, c.heads, c.dim, c.page_size, table->size(1)), c.device);
-        rc = g_ops.kv_attend(q->const_data_ptr(), code, batch, heads, q->stride(0), q->stride(1), c.k_codes(), c.v_codes(), c.params->const_data_ptr(), c.bits,
-                             c.pages, c.page_size, c.heads, c.dim, static_cast<const int32_t *>(table->const_data_ptr()), table->stride(0), table->size(1),
-                             static_cast<const int32_t *>(lengths->const_data_ptr()), scale, out.mutable_data_ptr(), ws.defined() ? ws.mutable_data_ptr() : nullptr,
-                             ws.defined() ? (size_t)ws.numel() : 0, c10::cuda::getCurrentCUDAStream(c.device.index()).stream());
+        const at::Tensor ws = bytes_of(window < 0 ? g_ops.kv_attend_bytes(batch, heads, c.heads, c.dim, c.page_size, table->size(1))
+                                                  : g_ops.kv_attend_window_bytes(batch, heads, c.heads, c.dim, c.page_size, table->size(1), window, sinks), c.device);
+        void *scratch = ws.defined() ? ws.mutable_data_ptr() : nullptr;
+        const size_t bytes = ws.defined() ? (size_t)ws.numel() : 0;
+        const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(c.device.index()).stream();
+        const int32_t *pages = static_cast<const int32_t *>(table->const_data_ptr()), *n = static_cast<const int32_t *>(lengths->const_data_ptr());
+        if (window < 0)
+            rc = g_ops.kv_attend(q->const_data_ptr(), code, batch, heads, q->stride(0), q->stride(1), c.k_codes(), c.v_codes(), c.params->const_data_ptr(), c.bits,
+                                 c.pages, c.page_size, c.heads, c.dim, pages, table->stride(0), table->size(1), n, scale, out.mutable_data_ptr(), scratch, bytes, stream);
+        else
+            rc = g_ops.kv_attend_window(q->const_data_ptr(), code, batch, heads, q->stride(0), q->stride(1), c.k_codes(), c.v_codes(), c.params->const_data_ptr(), c.bits,
+                                        c.pages, c.page_size, c.heads, c.dim, pages, table->stride(0), table->size(1), n, window, sinks, scale, out.mutable_data_ptr(),
+                                        scratch, bytes, stream);
     }
     if (rc != BW_OK) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS
+}
+
+// The engine hands each gradient to the stream on which its consumer was recorded.  The default stream cannot take one from a capture, and torch
+// does not survive the attempt.
+void check_capture(torch::autograd::Node &node, const char *name) {
+    if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+    for (uint32_t i = 0; i < node.num_outputs(); ++i) {
+        if (!node.task_should_compute_output(i)) continue;
+        const auto stream = node.next_edge(i).function->stream();
+        TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()), name,
+                    ": this backward pass cannot be captured while a graph of the same tensors, recorded on the default stream, is alive; free it, or "
+                    "record it on another stream");
+    }
+}
+// Gradients as once_differentiable has them: an error for whoever differentiates these.
+void once_only(torch::autograd::variable_list &result) {
+    for (auto &t : result)
+        if (t.defined()) t = (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", 1))(
+                             {t.detach().requires_grad_()})[0];
+}
+// A saved tensor.  Hooks may have made another one of it in the meantime (moved, packed).
+at::Tensor saved(const torch::autograd::SavedVariable &v, const char *name, const c10::Device &device, at::IntArrayRef sizes, at::ScalarType type) {
+    at::Tensor t = v.unpack();
+    TORCH_CHECK(t.defined() && t.layout() == c10::kStrided && t.device() == device && t.scalar_type() == type && t.sizes() == sizes, name,
+                ": a tensor saved for the backward pass has come back from its hooks in another shape, type or place");
+    return t.resolve_neg();
 }
 
 // One call of bw_adapter_forward; `hidden` is what the backward pass needs again.  x [..., K] and the rest are checked.
@@ -313,12 +367,9 @@ struct AdapterNode : torch::autograd::Node {
     at::ScalarType type = at::kHalf;
     c10::Device device = c10::Device(c10::kCPU);
 
-    // A saved tensor, as the kernels take it.  Hooks may have made another tensor of it in the meantime (moved, packed).
-    at::Tensor back(const torch::autograd::SavedVariable &saved, at::IntArrayRef sizes, at::ScalarType as) const {
-        at::Tensor t = saved.unpack();
-        TORCH_CHECK(t.defined() && t.layout() == c10::kStrided && t.device() == device && t.scalar_type() == as && t.sizes() == sizes,
-                    "adapter_matmul: a tensor saved for the backward pass has come back from its hooks in another shape, type or place");
-        t = t.resolve_neg().contiguous();
+    // A saved tensor, as the kernels take it.
+    at::Tensor back(const torch::autograd::SavedVariable &v, at::IntArrayRef sizes, at::ScalarType as) const {
+        const at::Tensor t = saved(v, "adapter_matmul", device, sizes, as).contiguous();
         return on_16_bytes(t) ? t : t.clone();
     }
 
@@ -327,24 +378,12 @@ struct AdapterNode : torch::autograd::Node {
         const std::lock_guard<std::mutex> lock(mutex_);
         for (auto *v : {&x, &down, &up, &index, &scaling, &hidden}) v->reset_data();
     }
-    // The engine hands each gradient to the stream on which its consumer was recorded.  The default stream cannot take one from a capture, and torch
-    // does not survive the attempt.
-    void check_capture() const {
-        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
-        for (uint32_t i = 0; i < num_outputs(); ++i) {
-            if (!task_should_compute_output(i)) continue;
-            const auto stream = next_edge(i).function->stream();
-            TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()),
-                        "adapter_matmul: this backward pass cannot be captured while a graph of the same tensors, recorded on the default stream, is alive; free it, or "
-                        "record it on another stream");
-        }
-    }
     torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
         const std::lock_guard<std::mutex> lock(mutex_);
         torch::autograd::variable_list result(4);
         const at::Tensor g = grads[0];
         if (!g.defined()) return result;
-        check_capture();
+        check_capture(*this, "adapter_matmul");
         const bool again = c10::GradMode::is_enabled();
         if (task_should_compute_output(0) || task_should_compute_output(1) || task_should_compute_output(2)) {
             at::AutoGradMode off(false);
@@ -364,12 +403,7 @@ struct AdapterNode : torch::autograd::Node {
                                                   ws.mutable_data_ptr(), (size_t)ws.numel(), c10::cuda::getCurrentCUDAStream(xt.device().index()).stream());
             TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_adapter_backward returned status ", rc);
         }
-        if (again) {
-            // as once_differentiable has it: an error for whoever differentiates these
-            for (auto &t : result)
-                if (t.defined()) t = (*std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that was marked with @once_differentiable", 1))(
-                                     {t.detach().requires_grad_()})[0];
-        }
+        if (again) once_only(result);
         if (task_should_compute_output(3)) result[3] = g;
         return result;
     }
@@ -459,19 +493,357 @@ PyObject *adapter_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions ----
+// Tensors [..., heads, dim] as rows: whether the leading dimensions are one with a stride.
+struct HeadRows {
+    int64_t tokens = 1, stride = 0;
+    bool of(const at::Tensor &x) {
+        const int64_t n = x.dim();
+        if (n < 2 || x.stride(n - 1) != 1 || x.numel() < 1 || x.size(n - 2) > INT32_MAX || x.size(n - 1) > INT32_MAX) return false;
+        for (int64_t i = n - 3; i >= 0; --i) {
+            if (x.size(i) == 1) continue;
+            if (tokens == 1) stride = x.stride(i);
+            else if (x.stride(i) != tokens * stride) return false;
+            tokens *= x.size(i);
+        }
+        return true;
+    }
+};
+// The table and what belongs to it: (table, (rotary_dim, interleaved, number of axes, axes of the pairs as bytes, max_positions)).
+struct RotaryCall {
+    const at::Tensor *table = nullptr;
+    bw_rotary r = {};
+    std::array<uint8_t, 128> axes = {};
+    bool of(PyObject *t, PyObject *meta, const c10::Device &device) {
+        table = tensor_of(t);
+        if (!PyTuple_CheckExact(meta) || PyTuple_GET_SIZE(meta) != 5 || !dense(table, device) || table->scalar_type() != at::kFloat || !on_16_bytes(*table)) return false;
+        r.rotary_dim = (int)PyLong_AsLong(PyTuple_GET_ITEM(meta, 0));
+        r.interleaved = (int)PyLong_AsLong(PyTuple_GET_ITEM(meta, 1));
+        r.num_axes = (int)PyLong_AsLong(PyTuple_GET_ITEM(meta, 2));
+        r.max_positions = PyLong_AsLongLong(PyTuple_GET_ITEM(meta, 4));
+        char *bytes = nullptr;
+        Py_ssize_t n = 0;
+        if (PyErr_Occurred() || PyBytes_AsStringAndSize(PyTuple_GET_ITEM(meta, 3), &bytes, &n) != 0) {
+            PyErr_Clear();
+            return false;
+        }
+        if (r.rotary_dim < 2 || n != r.rotary_dim / 2 || n > 128) return false;
+        if (table->dim() != 3 || table->size(0) != r.max_positions || table->size(1) != n || table->size(2) != 2) return false;
+        std::memcpy(axes.data(), bytes, (size_t)n);
+        r.table = static_cast<const float *>(table->const_data_ptr());
+        return true;
+    }
+    // Positions of the leading shape, or of each axis.
+    bool at(const at::Tensor *positions, at::IntArrayRef lead, int64_t tokens, const c10::Device &device) {
+        if (!dense(positions, device) || positions->scalar_type() != at::kLong) return false;
+        const at::IntArrayRef sizes = positions->sizes();
+        if (sizes == lead) r.axis_stride = 0;
+        else if (sizes.size() == lead.size() + 1 && sizes[0] == r.num_axes && sizes.slice(1) == lead) r.axis_stride = tokens;
+        else return false;
+        r.positions = static_cast<const int64_t *>(positions->const_data_ptr());
+        return true;
+    }
+};
+
+// Rows of one or two tensors turned, or turned back, into new tensors; BW_OK or nothing has been launched.
+int rotate_call(bw_rotary r, const uint8_t *axes, bool inverse, const at::Tensor *const *x, at::Tensor *out) {
+    r.axes = axes;
+    const void *from[2] = {};
+    void *to[2] = {};
+    int heads[2] = {};
+    int64_t strides[4] = {}, tokens = 0, dim = 0;
+    int n = 0;
+    for (int i = 0; i < 2; ++i) {
+        if (!x[i]) continue;
+        HeadRows rows;
+        if (!rows.of(*x[i])) return BW_ERR_UNSUPPORTED;
+        out[i] = fresh(x[i]->sizes(), x[i]->scalar_type(), x[i]->device());
+        from[n] = x[i]->const_data_ptr();
+        to[n] = out[i].mutable_data_ptr();
+        heads[n] = (int)x[i]->size(-2);
+        strides[2 * n] = rows.stride;
+        strides[2 * n + 1] = x[i]->stride(-2);
+        tokens = rows.tokens;
+        dim = x[i]->size(-1);
+        ++n;
+    }
+    const at::Tensor &any = x[0] ? *x[0] : *x[1];
+    return g_ops.rotate(&r, tokens, (int)dim, float_code(any.scalar_type()), inverse, from[0], heads[0], strides[0], strides[1], to[0], from[1], heads[1], strides[2], strides[3],
+                        to[1], c10::cuda::getCurrentCUDAStream(any.device().index()).stream());
+}
+
+// RotateFunction of the Python package (rotary.py) as a node of the graph.  Edges, and inputs, are the tensors that were rotated.
+struct RotateNode : torch::autograd::Node {
+    torch::autograd::SavedVariable table, positions;
+    c10::SmallVector<int64_t, 5> table_sizes, position_sizes;
+    bw_rotary r = {};
+    std::array<uint8_t, 128> axes = {};
+    c10::Device device = c10::Device(c10::kCPU);
+
+    std::string name() const override { return "RotateNode"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        table.reset_data();
+        positions.reset_data();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        torch::autograd::variable_list result(num_outputs());
+        at::Tensor held[2], out[2];
+        const at::Tensor *x[2] = {};
+        for (uint32_t i = 0; i < num_outputs() && i < 2; ++i) {
+            if (!grads[i].defined() || !task_should_compute_output(i)) continue;
+            held[i] = grads[i].resolve_neg();
+            HeadRows rows;
+            if (!rows.of(held[i])) held[i] = held[i].contiguous();
+            x[i] = &held[i];
+        }
+        if (!x[0] && !x[1]) return result;
+        check_capture(*this, "rotate");
+        const bool again = c10::GradMode::is_enabled();
+        {
+            at::AutoGradMode off(false);
+            const at::Tensor t = saved(table, "rotate", device, table_sizes, at::kFloat).contiguous(), p = saved(positions, "rotate", device, position_sizes, at::kLong).contiguous();
+            TORCH_CHECK(on_16_bytes(t), "rotate: the table has come back from its hooks off a 16-byte boundary");
+            bw_rotary call = r;
+            call.table = static_cast<const float *>(t.const_data_ptr());
+            call.positions = static_cast<const int64_t *>(p.const_data_ptr());
+            const int rc = rotate_call(call, axes.data(), true, x, out);
+            TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_rotate returned status ", rc);
+        }
+        for (uint32_t i = 0; i < num_outputs() && i < 2; ++i) result[i] = out[i];
+        if (again) once_only(result);
+        return result;
+    }
+};
+
+// rotate(table, what belongs to it, positions, x[, y]): the rotated tensor, or both
+PyObject *rotate(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if ((nargs != 4 && nargs != 5) || !g_ops.rotate || modes_active()) Py_RETURN_NONE;
+    const at::Tensor *positions = tensor_of(args[2]), *x[2] = {tensor_of(args[3]), nargs == 5 ? tensor_of(args[4]) : nullptr};
+    if (!x[0] || (nargs == 5 && !x[1])) Py_RETURN_NONE;
+    const c10::Device device = x[0]->device();
+    if (!device.is_cuda() || device.index() != c10::cuda::current_device()) Py_RETURN_NONE;
+    RotaryCall c;
+    const int n = nargs == 5 ? 2 : 1;
+    bool recording = false;
+    for (int i = 0; i < n; ++i) {
+        HeadRows rows;
+        if (!usable(x[i], device) || float_code(x[i]->scalar_type()) < 0 || x[i]->scalar_type() != x[0]->scalar_type() || !rows.of(*x[i])) Py_RETURN_NONE;
+        if (x[i]->dim() != x[0]->dim() || x[i]->size(-1) != x[0]->size(-1) || x[i]->sizes().slice(0, x[i]->dim() - 2) != x[0]->sizes().slice(0, x[0]->dim() - 2)) Py_RETURN_NONE;
+        recording = recording || (c10::GradMode::is_enabled() && x[i]->requires_grad());
+        if (i == 0 && (!c.of(args[0], args[1], device) || !c.at(positions, x[0]->sizes().slice(0, x[0]->dim() - 2), rows.tokens, device))) Py_RETURN_NONE;
+    }
+    if (x[0]->size(-1) < c.r.rotary_dim) Py_RETURN_NONE;
+    at::Tensor out[2];
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        rc = rotate_call(c.r, c.axes.data(), false, x, out);
+        if (rc == BW_OK && recording) {
+            const std::shared_ptr<RotateNode> node(new RotateNode(), torch::autograd::deleteNode);
+            node->set_next_edges(n == 2 ? torch::autograd::collect_next_edges(*x[0], *x[1]) : torch::autograd::collect_next_edges(*x[0]));
+            node->table_sizes.assign(c.table->sizes().begin(), c.table->sizes().end());
+            node->position_sizes.assign(positions->sizes().begin(), positions->sizes().end());
+            node->r = c.r;
+            node->axes = c.axes;
+            node->device = device;
+            node->table = torch::autograd::SavedVariable(*c.table, false);
+            node->positions = torch::autograd::SavedVariable(*positions, false);
+            for (int i = 0; i < n; ++i) torch::autograd::set_history(out[i], node);
+        }
+    }
+    if (rc != BW_OK) Py_RETURN_NONE;
+    if (n == 1) return THPVariable_Wrap(std::move(out[0]));
+    PyObject *first = THPVariable_Wrap(std::move(out[0])), *second = THPVariable_Wrap(std::move(out[1]));
+    return Py_BuildValue("(NN)", first, second);
+    END_HANDLE_TH_ERRORS
+}
+
+// kv_append_rotated(k_codes, v_codes, params, bits, q or None, k, v, slots, table, what belongs to it, positions): the rotated queries, or True
+PyObject *kv_append_rotated(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    Cache c;
+    if (nargs != 11 || !g_ops.kv_append_rotated || !c.of(args)) Py_RETURN_NONE;
+    const bool queries = args[4] != Py_None;
+    const at::Tensor *q = queries ? tensor_of(args[4]) : nullptr, *k = tensor_of(args[5]), *v = tensor_of(args[6]), *slots = tensor_of(args[7]), *positions = tensor_of(args[10]);
+    if (!usable(k, c.device) || !usable(v, c.device) || !slots_ok(slots, c) || (queries && !usable(q, c.device))) Py_RETURN_NONE;
+    const int code = float_code(k->scalar_type());
+    if (code < 0 || v->scalar_type() != k->scalar_type() || k->dim() != 3 || v->sizes() != k->sizes()) Py_RETURN_NONE;
+    const int64_t tokens = slots->size(0);
+    if (tokens < 1 || k->size(0) != tokens || k->size(1) != c.heads || k->size(2) != c.dim || k->stride(2) != 1 || v->stride(2) != 1) Py_RETURN_NONE;
+    if (queries && (q->scalar_type() != k->scalar_type() || q->dim() != 3 || q->size(0) != tokens || q->size(2) != c.dim || q->stride(2) != 1 || q->size(1) < 1 ||
+                    q->size(1) > INT32_MAX || (c10::GradMode::is_enabled() && q->requires_grad())))
+        Py_RETURN_NONE;
+    RotaryCall r;
+    if (!r.of(args[8], args[9], c.device) || !r.at(positions, slots->sizes(), tokens, c.device) || r.r.rotary_dim > c.dim) Py_RETURN_NONE;
+    r.r.axes = r.axes.data();
+    at::Tensor out;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        if (queries) out = fresh(q->sizes(), q->scalar_type(), c.device);
+        rc = g_ops.kv_append_rotated(&r.r, queries ? q->const_data_ptr() : nullptr, queries ? (int)q->size(1) : 0, queries ? q->stride(0) : 0, queries ? q->stride(1) : 0,
+                                     queries ? out.mutable_data_ptr() : nullptr, k->const_data_ptr(), v->const_data_ptr(), code, tokens, k->stride(0), k->stride(1),
+                                     v->stride(0), v->stride(1), static_cast<const int64_t *>(slots->const_data_ptr()), c.heads, c.dim, c.bits, c.pages, c.page_size,
+                                     c.k_codes(), c.v_codes(), c.params->mutable_data_ptr(), c10::cuda::getCurrentCUDAStream(c.device.index()).stream());
+    }
+    if (rc != BW_OK) Py_RETURN_NONE;
+    if (!queries) Py_RETURN_TRUE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- log probabilities ----
+// Logits [..., vocab] as rows with a stride.
+struct LogitRows {
+    int64_t rows = 1, stride = 0;
+    bool of(const at::Tensor &x) {
+        const int64_t n = x.dim();
+        if (n < 1 || x.stride(n - 1) != 1 || x.numel() < 1) return false;
+        for (int64_t i = n - 2; i >= 0; --i) {
+            if (x.size(i) == 1) continue;
+            if (rows == 1) stride = x.stride(i);
+            else if (x.stride(i) != rows * stride) return false;
+            rows *= x.size(i);
+        }
+        return true;
+    }
+};
+
+// TokenLogProbsFunction of the Python package (log_probs.py) as a node of the graph.  Inputs: the gradients of what was asked for.
+struct LogProbsNode : torch::autograd::Node {
+    torch::autograd::SavedVariable logits, tokens, top_tokens, stats;
+    c10::SmallVector<int64_t, 5> sizes;
+    int at_log_probs = -1, at_entropy = -1, at_top = -1, top = 0;      // which input is which
+    bool given = false;                                              // there are tokens
+    int64_t rows = 0;
+    at::ScalarType type = at::kHalf;
+    c10::Device device = c10::Device(c10::kCPU);
+
+    std::string name() const override { return "LogProbsNode"; }
+    void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        for (auto *v : {&logits, &tokens, &top_tokens, &stats}) v->reset_data();
+    }
+    torch::autograd::variable_list apply(torch::autograd::variable_list &&grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
+        torch::autograd::variable_list result(1);
+        const auto of = [&](int i) { return i >= 0 && grads[i].defined() ? grads[i].resolve_neg().contiguous() : at::Tensor(); };
+        const at::Tensor g = of(at_log_probs), e = of(at_entropy), gt = of(at_top);
+        if (!(g.defined() || e.defined() || gt.defined()) || !task_should_compute_output(0)) return result;
+        check_capture(*this, "token_log_probs");
+        const bool again = c10::GradMode::is_enabled();
+        {
+            at::AutoGradMode off(false);
+            const char *me = "token_log_probs";
+            const at::IntArrayRef all(sizes), lead = all.slice(0, all.size() - 1);
+            c10::SmallVector<int64_t, 5> top_sizes(lead.begin(), lead.end());
+            top_sizes.push_back(top);
+            at::Tensor x = saved(logits, me, device, all, type);
+            LogitRows r;
+            if (!r.of(x)) {
+                x = x.contiguous();
+                r = LogitRows();
+                r.of(x);
+            }
+            const at::Tensor t = given ? saved(tokens, me, device, lead, at::kLong).contiguous() : at::Tensor(),
+                             tt = top ? saved(top_tokens, me, device, top_sizes, at::kLong).contiguous() : at::Tensor(), s = saved(stats, me, device, {rows, 4}, at::kFloat).contiguous();
+            TORCH_CHECK(on_16_bytes(s), "token_log_probs: a tensor saved for the backward pass has come back from its hooks off a 16-byte boundary");
+            result[0] = fresh(all, type, device);
+            const auto pointer = [](const at::Tensor &v) { return v.defined() ? v.const_data_ptr() : nullptr; };
+            const int rc = g_ops.token_log_probs_grad(x.const_data_ptr(), float_code(type), rows, all.back(), r.stride, static_cast<const int64_t *>(pointer(t)),
+                                                      static_cast<const float *>(s.const_data_ptr()), static_cast<const float *>(pointer(g)), static_cast<const float *>(pointer(e)),
+                                                      top, static_cast<const int64_t *>(pointer(tt)), static_cast<const float *>(pointer(gt)), result[0].mutable_data_ptr(),
+                                                      c10::cuda::getCurrentCUDAStream(device.index()).stream());
+            TORCH_CHECK(rc == BW_OK, "libbitween_b200: bw_token_log_probs_grad returned status ", rc);
+        }
+        if (again) once_only(result);
+        return result;
+    }
+};
+
+// token_log_probs(logits, tokens or None, entropy, top): (log_probs, entropy, top_log_probs, top_tokens), None for what is not asked
+PyObject *token_log_probs(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 4 || !g_ops.token_log_probs || modes_active() || !PyBool_Check(args[2]) || !PyLong_CheckExact(args[3])) Py_RETURN_NONE;
+    const at::Tensor *x = tensor_of(args[0]), *t = args[1] == Py_None ? nullptr : tensor_of(args[1]);
+    if (!x || (args[1] != Py_None && !t)) Py_RETURN_NONE;
+    const bool entropy = args[2] == Py_True;
+    const long top = PyLong_AsLong(args[3]);
+    if (top < 0 || top > 32) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    const c10::Device device = x->device();
+    LogitRows r;
+    if (!device.is_cuda() || device.index() != c10::cuda::current_device() || !usable(x, device) || float_code(x->scalar_type()) < 0 || !r.of(*x)) Py_RETURN_NONE;
+    const int64_t vocab = x->size(-1);
+    const at::IntArrayRef lead = x->sizes().slice(0, x->dim() - 1);
+    if (top > vocab || (t && (!dense(t, device) || t->scalar_type() != at::kLong || t->sizes() != lead))) Py_RETURN_NONE;
+    const bool recording = c10::GradMode::is_enabled() && x->requires_grad() && (t || entropy || top);
+    at::Tensor lp, h, top_lp, top_t, stats;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        c10::SmallVector<int64_t, 5> top_sizes(lead.begin(), lead.end());
+        top_sizes.push_back(top);
+        if (t) lp = fresh(lead, at::kFloat, device);
+        if (entropy) h = fresh(lead, at::kFloat, device);
+        if (top) {
+            top_lp = fresh(top_sizes, at::kFloat, device);
+            top_t = fresh(top_sizes, at::kLong, device);
+        }
+        if (recording) stats = fresh({r.rows, 4}, at::kFloat, device);
+        const auto into = [](at::Tensor &v) { return v.defined() ? v.mutable_data_ptr() : nullptr; };
+        rc = g_ops.token_log_probs(x->const_data_ptr(), float_code(x->scalar_type()), r.rows, vocab, r.stride, t ? static_cast<const int64_t *>(t->const_data_ptr()) : nullptr,
+                                   static_cast<float *>(into(lp)), static_cast<float *>(into(h)), (int)top, static_cast<float *>(into(top_lp)),
+                                   static_cast<int64_t *>(into(top_t)), static_cast<float *>(into(stats)), c10::cuda::getCurrentCUDAStream(device.index()).stream());
+        if (rc == BW_OK && recording) {
+            const std::shared_ptr<LogProbsNode> node(new LogProbsNode(), torch::autograd::deleteNode);
+            node->set_next_edges(torch::autograd::collect_next_edges(*x));
+            node->sizes.assign(x->sizes().begin(), x->sizes().end());
+            node->top = (int)top;
+            node->given = t != nullptr;
+            node->rows = r.rows;
+            node->type = x->scalar_type();
+            node->device = device;
+            node->logits = torch::autograd::SavedVariable(*x, false);
+            node->tokens = torch::autograd::SavedVariable(t ? *t : at::Tensor(), false);
+            node->top_tokens = torch::autograd::SavedVariable(top_t, false);
+            node->stats = torch::autograd::SavedVariable(stats, false);
+            int n = 0;
+            for (auto [tensor, place] : {std::make_pair(&lp, &node->at_log_probs), std::make_pair(&h, &node->at_entropy), std::make_pair(&top_lp, &node->at_top)})
+                if (tensor->defined()) {
+                    *place = n++;
+                    torch::autograd::set_history(*tensor, node);
+                }
+        }
+    }
+    if (rc != BW_OK) Py_RETURN_NONE;
+    const auto wrapped = [](at::Tensor &v) -> PyObject * {
+        if (v.defined()) return THPVariable_Wrap(std::move(v));
+        Py_RETURN_NONE;
+    };
+    PyObject *a = wrapped(lp), *b = wrapped(h), *c = wrapped(top_lp), *d = wrapped(top_t);
+    return Py_BuildValue("(NNNN)", a, b, c, d);
+    END_HANDLE_TH_ERRORS
+}
+
 // set_operators(addresses of the entry points, in the order of Operators)
 PyObject *set_operators(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
-    void *p[7];
-    if (nargs != 7) {
-        PyErr_SetString(PyExc_TypeError, "set_operators(seven addresses)");
+    if (nargs != OPERATORS) {
+        PyErr_Format(PyExc_TypeError, "set_operators(%d addresses)", OPERATORS);
         return nullptr;
     }
-    for (int i = 0; i < 7; ++i) {
+    void *p[OPERATORS];
+    for (int i = 0; i < OPERATORS; ++i) {
         p[i] = PyLong_AsVoidPtr(args[i]);
         if (!p[i] && PyErr_Occurred()) return nullptr;
     }
-    g_ops = {reinterpret_cast<KvAppend>(p[0]),     reinterpret_cast<KvRead>(p[1]),         reinterpret_cast<KvAttend>(p[2]),       reinterpret_cast<KvAttendBytes>(p[3]),
-             reinterpret_cast<AdapterBytes>(p[4]), reinterpret_cast<AdapterForward>(p[5]), reinterpret_cast<AdapterBackward>(p[6])};
+    static_assert(sizeof(p) == sizeof(g_ops), "the operators are pointers, one address each");
+    std::memcpy(&g_ops, p, sizeof(p));
     Py_RETURN_NONE;
 }
 
@@ -481,6 +853,9 @@ PyMethodDef methods[] = {
     BW_METHOD(kv_read),
     BW_METHOD(kv_attend),
     BW_METHOD(adapter_matmul),
+    BW_METHOD(rotate),
+    BW_METHOD(kv_append_rotated),
+    BW_METHOD(token_log_probs),
     BW_METHOD(set_operators),
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
     {"set_entry", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(set_entry)), METH_FASTCALL, nullptr},

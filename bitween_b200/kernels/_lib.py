@@ -185,7 +185,7 @@ def _takes_no_call(*args):
 
 class _NoOperators:
     """Stands for the native host side of the operators where there is none: it takes no call."""
-    kv_append = kv_read = kv_attend = adapter_matmul = staticmethod(_takes_no_call)
+    kv_append = kv_read = kv_attend = adapter_matmul = rotate = kv_append_rotated = token_log_probs = staticmethod(_takes_no_call)
 
 
 _host = None
@@ -213,7 +213,8 @@ def host_forward():
                     module.set_entry(ctypes.cast(L.bw_qmatmul, ctypes.c_void_p).value, _workspaces)
                     module.set_operators(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                         L.bw_kv_append, L.bw_kv_read, L.bw_kv_attend, L.bw_kv_attend_workspace_bytes, L.bw_adapter_hidden_bytes,
-                        L.bw_adapter_forward, L.bw_adapter_backward)))
+                        L.bw_adapter_forward, L.bw_adapter_backward, L.bw_kv_attend_window, L.bw_kv_attend_window_workspace_bytes, L.bw_rotate,
+                        L.bw_kv_append_rotated, L.bw_token_log_probs, L.bw_token_log_probs_grad)))
                     _operators = module
                     _host = module.forward
                 except Exception as e:  # noqa: BLE001
@@ -224,11 +225,18 @@ def host_forward():
 
 
 def host_operators():
-    """The native host side of the key-value cache's and the adapters' calls, from the same module: each takes plain calls and
-    answers None to the others."""
+    """The native host side of the operators beside the linears (cache, rotary positions, adapters, log probabilities), from the same
+    module: each takes plain calls and answers None to the others."""
     if _operators is None:
         host_forward()
     return _operators
+
+
+def refuse_capture(name):
+    """For backward passes of the Python path: which stream a gradient's consumer was recorded on is not known here, and where that is the default
+    stream (a graph of the same leaves that still lives) torch does not survive handing it a captured gradient."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{name}: this backward pass cannot be captured without the native host side of the operators, or of tensors that it does not take")
 
 
 def check(status):

@@ -113,6 +113,10 @@ class QuantizedKVCache:
         Keys are rotated in fp32 and quantised from there: the cache holds what `append(rotary.rotate(positions, k.float()), v.float(), slots)` would
         leave.  `positions`: int64 [tokens], or [axes, tokens].  A position outside the table gives NaN: that token's queries, and its key when it is read.  Queries
         of skipped slots are rotated too.  Nothing is recorded: a q that requires a gradient is refused where gradients are recorded."""
+        if type(rotary) is RotaryPositions:
+            out = (_lib._operators or _lib.host_operators()).kv_append_rotated(*self._cache, q, k, v, slots, rotary.table, rotary._meta, positions)
+            if out is not None:
+                return None if q is None else out
         _lib.require_cuda(self.k_codes, "cache")
         slots = self._check_slots(slots)
         tokens = slots.shape[0]
@@ -139,12 +143,12 @@ class QuantizedKVCache:
             raise RuntimeError(f"`rotary` is on {rotary.device} but the cache is on {self.device}")
         if rotary.rotary_dim > self.head_dim:
             raise ValueError(f"rotary turns {rotary.rotary_dim} values but head_dim is {self.head_dim}")
-        positions, axis_stride = rotary._positions(positions, (tokens,))
+        positions = rotary._positions(positions, (tokens,))
         q, k, v = (t if t is None or t.stride(2) == 1 else t.contiguous() for t in (t if t is None else t.resolve_neg() for t in (q, k, v)))
         out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=self.device)
         L = _lib.lib()
         with _lib.on_device(self.device):
-            rc = L.bw_kv_append_rotated(ctypes.byref(rotary._struct(rotary.table, positions, axis_stride)), *((None, 0, 0, 0, None) if q is None else (
+            rc = L.bw_kv_append_rotated(ctypes.byref(rotary._struct(rotary.table, positions)), *((None, 0, 0, 0, None) if q is None else (
                 q.data_ptr(), q.shape[1], q.stride(0), q.stride(1), out.data_ptr())), k.data_ptr(), v.data_ptr(), _lib.dtype_code(k.dtype), tokens,
                 k.stride(0), k.stride(1), v.stride(0), v.stride(1), slots.data_ptr(), self.num_kv_heads, self.head_dim, self.bits, self.num_pages, self.page_size,
                 *self._tensors(), _lib.raw_stream(self.device))
@@ -205,7 +209,10 @@ class QuantizedKVCache:
     def _attend_window(self, q, page_table, lengths, softmax_scale, window, sinks):
         if not isinstance(window, int) or not isinstance(sinks, int) or window < 0 or sinks < 0:
             raise ValueError("window and sinks must be numbers of tokens, 0 or more")
-        window, sinks = min(window, 2 ** 31), min(sinks, 2 ** 31)
+        window, sinks = min(int(window), 2 ** 31), min(int(sinks), 2 ** 31)
+        out = (_lib._operators or _lib.host_operators()).kv_attend(*self._cache, q, page_table, lengths, softmax_scale, window, sinks)
+        if out is not None:
+            return out
         q, page_table, lengths, out = self._attend_args(q, page_table, lengths)
         batch, heads = q.shape[:2]
         L = _lib.lib()

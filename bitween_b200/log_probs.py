@@ -52,6 +52,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, e, g_top, _):
+        _lib.refuse_capture("token_log_probs")
         saved = ctx.saved_tensors
         # (hooks may have made other tensors of them in the meantime: moved, packed)
         if any((t is None) != (like is None) or (t is not None and (t.shape, t.dtype, t.device) != like) for t, like in zip(saved, ctx.like)):
@@ -88,6 +89,10 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0):
 
     Where a probability is 0 (a logit of -infinity) it adds nothing to the entropy.  A row with NaN or +infinity, or of -infinity alone, gives NaN.
     Differentiable in the logits through log_probs, entropy and top_log_probs; the gradient is formed in fp32 and rounded once."""
+    ops = _lib._operators or _lib.host_operators()
+    out = ops.token_log_probs(logits, tokens, entropy, top)
+    if out is not None:
+        return TokenLogProbs._make(out)
     _lib.require_cuda(logits, "logits")
     if logits.dtype not in _FLOAT_DTYPES:
         raise TypeError(f"token_log_probs: unsupported dtype {logits.dtype} (float32/float16/bfloat16)")
@@ -105,8 +110,8 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0):
             raise RuntimeError(f"`tokens` is on {tokens.device} but logits is on {logits.device}")
         tokens = tokens.reshape(-1).contiguous()
     x = _rows(logits.reshape(-1, vocab))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        out = TokenLogProbsFunction.apply(x, tokens, bool(entropy), top)
-    else:
-        out = _forward(x, tokens, bool(entropy), top, False)[:4]
+    entropy = bool(entropy)
+    out = ops.token_log_probs(x, tokens, entropy, top)
+    if out is None:
+        out = TokenLogProbsFunction.apply(x, tokens, entropy, top) if torch.is_grad_enabled() and logits.requires_grad else _forward(x, tokens, entropy, top, False)[:4]
     return TokenLogProbs(*(t if t is None else t.view((*lead, *t.shape[1:])) for t in out))

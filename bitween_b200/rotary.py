@@ -51,8 +51,8 @@ class RotaryPositions:
         self.rotary_dim, self.max_positions, self.interleaved = rotary_dim, max_positions, bool(interleaved)
         self.axes = tuple(axes)
         self.device = self.table.device
-        self._axes = bytes(axes)
         self._shape = self.table.shape
+        self._meta = (int(rotary_dim), int(self.interleaved), self.num_axes, bytes(axes), int(max_positions))
 
     def _checked(self, table):
         """`table` (this one's, or what came back of it for a backward pass), if the kernels can take it."""
@@ -61,29 +61,30 @@ class RotaryPositions:
         return table
 
     def _positions(self, positions, lead):
-        """(positions with whole rows of tokens, elements between axes) for rows of the leading shape `lead`."""
+        """Positions for rows of the leading shape `lead`, as [tokens] or [axes, tokens]."""
         _lib.require_cuda(positions, "positions")
         if positions.dtype != torch.int64:
             raise TypeError("positions must be int64")
         if positions.device != self.device:
             raise RuntimeError(f"`positions` is on {positions.device} but the table is on {self.device}")
         if tuple(positions.shape) == tuple(lead):
-            return positions.contiguous(), 0
+            return positions.reshape(math.prod(lead)).contiguous()
         if tuple(positions.shape) != (self.num_axes, *lead):
             raise ValueError(f"positions must have shape {tuple(lead)} or {(self.num_axes, *lead)}")
-        flat = positions.reshape(self.num_axes, math.prod(lead))
-        if flat.shape[1] > 1 and flat.stride(1) != 1:
-            flat = flat.contiguous()
-        return flat, flat.stride(0) if self.num_axes > 1 else 0
+        return positions.reshape(self.num_axes, math.prod(lead)).contiguous()
 
-    def _struct(self, table, positions, axis_stride):
-        return _lib.Rotary(self._checked(table).data_ptr(), self.max_positions, self.rotary_dim, int(self.interleaved), self.num_axes, self._axes,
-                           positions.data_ptr(), axis_stride)
+    def _struct(self, table, positions):
+        return _lib.Rotary(self._checked(table).data_ptr(), self.max_positions, self.rotary_dim, int(self.interleaved), self.num_axes, self._meta[3],
+                           positions.data_ptr(), 0 if positions.dim() == 1 else positions.shape[1])
 
     def rotate(self, positions, *xs):
         """One or two tensors [..., heads, dim] (queries, and keys with heads of their own; fp32, fp16 or bf16; dim at least rotary_dim) rotated, in
         one launch.  Returns new tensors, rounded once: one for one, a tuple for two.  `positions`, int64: of the tensors' leading shape, or
         with several axes [axes, *leading shape].  A position outside the table gives NaN.  Values behind the first rotary_dim are copied.  Differentiable."""
+        ops = _lib._operators or _lib.host_operators()
+        out = ops.rotate(self.table, self._meta, positions, *xs)
+        if out is not None:
+            return out
         if not 1 <= len(xs) <= 2:
             raise ValueError("rotate takes one or two tensors")
         for x in xs:
@@ -94,12 +95,14 @@ class RotaryPositions:
                 raise RuntimeError(f"`x` is on {x.device} but the table is on {self.device}")
             if x.dim() < 2 or x.shape[:-2] != xs[0].shape[:-2] or x.shape[-1] != xs[0].shape[-1] or x.shape[-1] < self.rotary_dim:
                 raise ValueError(f"the tensors to rotate must be [..., heads, dim] of one leading shape and one dim of at least {self.rotary_dim}")
-        positions, axis_stride = self._positions(positions, xs[0].shape[:-2])
-        if torch.is_grad_enabled() and any(x.requires_grad for x in xs):
-            out = RotateFunction.apply(self, positions, axis_stride, *xs)
-        else:
-            out = _rotate(self, self.table, positions, axis_stride, xs, False)
-        return out[0] if len(xs) == 1 else tuple(out)
+        positions, rows = self._positions(positions, xs[0].shape[:-2]), [_rows(x) for x in xs]
+        out = ops.rotate(self._checked(self.table), self._meta, positions, *rows)
+        if out is None:
+            out = RotateFunction.apply(self, positions, *rows) if torch.is_grad_enabled() and any(x.requires_grad for x in xs) else _rotate(self, self.table, positions, rows, False)
+        elif len(xs) == 1:
+            out = (out,)
+        out = tuple(y.view(x.shape) for x, y in zip(xs, out))
+        return out[0] if len(xs) == 1 else out
 
     def __repr__(self):
         return f"RotaryPositions(rotary_dim={self.rotary_dim}, max_positions={self.max_positions}, num_axes={self.num_axes}, interleaved={self.interleaved})"
@@ -112,8 +115,8 @@ def _rows(x):
     return x if x.stride(2) == 1 else x.contiguous()
 
 
-def _rotate(rotary, table, positions, axis_stride, xs, inverse):
-    """New tensors: those of `xs` that are there, turned (or turned back).  None where there is none."""
+def _rotate(rotary, table, positions, xs, inverse):
+    """New tensors: those of `xs` ([tokens, heads, dim]) that are there, turned (or turned back).  None where there is none."""
     outs = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
     given = [(_rows(x), out) for x, out in zip(xs, outs) if out is not None and out.numel()]
     if given:
@@ -124,29 +127,30 @@ def _rotate(rotary, table, positions, axis_stride, xs, inverse):
         x = given[0][0]
         L = _lib.lib()
         with _lib.on_device(rotary.device):
-            rc = L.bw_rotate(ctypes.byref(rotary._struct(table, positions, axis_stride)), x.shape[0], x.shape[2], _lib.dtype_code(x.dtype), int(inverse), *args,
+            rc = L.bw_rotate(ctypes.byref(rotary._struct(table, positions)), x.shape[0], x.shape[2], _lib.dtype_code(x.dtype), int(inverse), *args,
                              _lib.raw_stream(rotary.device))
         _lib.check(rc)
     return outs
 
 
 class RotateFunction(torch.autograd.Function):
-    """apply(rotary, positions, axis_stride, *xs) with what `rotate` has checked."""
+    """apply(rotary, positions, *xs) with what `rotate` has checked."""
 
     @staticmethod
-    def forward(ctx, rotary, positions, axis_stride, *xs):
-        ctx.rotary, ctx.axis_stride = rotary, axis_stride
+    def forward(ctx, rotary, positions, *xs):
+        ctx.rotary = rotary
         ctx.save_for_backward(rotary.table, positions)
-        ctx.like = (positions.shape, positions.stride(), positions.dtype, positions.device)
+        ctx.like = (positions.shape, positions.dtype, positions.device)
         ctx.set_materialize_grads(False)
-        return tuple(_rotate(rotary, rotary.table, positions, axis_stride, xs, False))
+        return tuple(_rotate(rotary, rotary.table, positions, xs, False))
 
     @staticmethod
     @once_differentiable
     def backward(ctx, *grads):
+        _lib.refuse_capture("rotate")
         table, positions = ctx.saved_tensors
         # (hooks may have made other tensors of them in the meantime: moved, packed)
-        if (positions.shape, positions.stride(), positions.dtype, positions.device) != ctx.like:
+        if (positions.shape, positions.dtype, positions.device) != ctx.like:
             raise RuntimeError("rotate: a tensor saved for the backward pass has come back from its hooks in another shape, type or place")
-        wanted = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[3:])]
-        return (None, None, None, *_rotate(ctx.rotary, table, positions, ctx.axis_stride, wanted, True))
+        wanted = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[2:])]
+        return (None, None, *_rotate(ctx.rotary, table, positions.contiguous(), wanted, True))
