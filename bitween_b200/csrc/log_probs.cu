@@ -23,6 +23,7 @@ namespace cg = cooperative_groups;
 constexpr int THREADS = 256, UNROLL = 4, BLOCKS = 16;     // of a CTA; 16-byte loads of a step; blocks of steps of a thread
 constexpr int STEP = THREADS * UNROLL;                     // 16-byte pieces of a CTA's step
 constexpr int CANDIDATES = 512;
+constexpr int MOST_CTAS = 4 * 148;                         // at once, at least: four an SM
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // The order of the alternatives: falling value, rising index; NaN before all.  Larger is better; nothing is 0.
@@ -112,12 +113,6 @@ struct Sums {
         }
         m = to;
     }
-    __device__ __forceinline__ void add(Sums o) {
-        if (o.m > m) raise(o.m);
-        else if (o.m < m) o.raise(m);
-        s += o.s;
-        w += o.w;
-    }
 };
 
 struct LogProbs {
@@ -126,7 +121,7 @@ struct LogProbs {
     float *log_probs, *entropy, *top_log_probs;
     int64_t *top_tokens;
     float4 *stats;                       // m, log2 s, H
-    int64_t stride;
+    int64_t stride, rows;
     int vocab, top, cluster;
 };
 
@@ -148,100 +143,50 @@ template <typename T> struct Row {
     __device__ __forceinline__ int extra_at(int i) const { return i < head ? i : behind + i - head; }
 };
 
+// The values of a call's rows that are looked at for alternatives.
+//
+// The threads of a row's CTAs form 64 groups.  The top-th largest of the groups' largest values is a bound from below: `top` groups hold a value that
+// reaches it.  Only blocks that reach it are read again, some more than `top` of them in all CTAs together, and the values that reach it are ranked.  Where too many do (many equal
+// values, as masks leave them; many large ones in few threads' places) a CTA finds the `top` best of its share digit by digit instead.
+constexpr int GROUPS = 64;
 struct __align__(16) TopScratch {
-    float largest[BLOCKS + 1][THREADS];  // of a thread's blocks, and of its extra value
-    __align__(16) uint32_t key[THREADS];
-    __align__(16) uint64_t list[CANDIDATES + 2];      // (order << 32) | ~index
+    float largest[BLOCKS][THREADS];                    // of a thread's blocks
+    __align__(16) uint32_t group[GROUPS];              // the groups' largest values, of all CTAs
+    __align__(16) uint64_t list[CANDIDATES + 2];       // this CTA's candidates: (order << 32) | ~index
+    __align__(16) uint64_t all[CANDIDATES + 2];        // all CTAs' (rank 0)
     uint64_t best[32];
-    uint32_t histogram[256];
-    int count, blocks, need;
-    uint32_t least, prefix;
+    uint32_t histogram[THREADS], entry[THREADS];
+    int count, entries, need, counts[8];
+    uint32_t least[2], prefix;
     int scan[THREADS / 32];
 };
 
 __device__ __forceinline__ uint64_t candidate(float x, int at) { return (uint64_t)order_of(x) << 32 | (uint32_t)~at; }
 
 // The best `top` of n candidates, in order, into `best`; 0 where there are fewer.  All candidates differ.
-__device__ __forceinline__ void rank_candidates(TopScratch &s, int n, int top) {
+__device__ __forceinline__ void rank_candidates(uint64_t *list, int n, int top, uint64_t *best) {
     const int tid = threadIdx.x;
-    if (tid < top) s.best[tid] = 0;
-    if (tid < 2) s.list[n + tid] = 0;
+    if (tid < top) best[tid] = 0;
+    if (tid < 2) list[n + tid] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += THREADS) {
-        const uint64_t mine = s.list[i];
+        const uint64_t mine = list[i];
         int before = 0;
+#pragma unroll 4
         for (int k = 0; k < n; k += 2) {
-            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(s.list + k);
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(list + k);
             before += (two.x > mine) + (two.y > mine);
         }
-        if (before < top) s.best[before] = mine;
+        if (before < top) best[before] = mine;
     }
     __syncthreads();
 }
 
-// The best `top` values of a rank's share.  A thread's largest value is `key`; those of its blocks of `per` steps lie in s.largest.
-//
-// The top-th largest of the threads' largest values is a bound from below.  Only blocks that reach it are read again, some more than `top` of them, and the
-// values that reach it are ranked.  Where too many do (many equal values, as masks leave them; many large ones in few threads' places) the bound is
-// found digit by digit over the whole share instead.
+// The best `top` values of a rank's share, as candidates into s.list: the top-th largest value is found eight bits at a time.
 template <typename T>
-__device__ __forceinline__ void find_top(TopScratch &s, const Row<T> &row, int top, int blocks, int per, uint32_t key) {
+__device__ __noinline__ void search_share(TopScratch &s, const Row<T> &row, int top) {
     constexpr int V = Piece<T>::V;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-    s.key[tid] = key;
-    if (tid == 0) {
-        s.count = s.blocks = 0;
-        s.least = 0xffffffffu;
-    }
-    __syncthreads();
-    int larger = 0;
-    for (int i = 0; i < THREADS; i += 4) {
-        const uint4 k = *reinterpret_cast<const uint4 *>(s.key + i);
-        larger += (k.x > key) + (k.y > key) + (k.z > key) + (k.w > key);
-    }
-    const uint32_t low = __reduce_min_sync(0xffffffffu, larger < top ? key : 0xffffffffu);
-    if (lane == 0) atomicMin(&s.least, low);
-    __syncthreads();
-    const uint32_t least = s.least;
-    if (key >= least) {
-        for (int b = 0; b <= BLOCKS; ++b) {
-            if (b < BLOCKS ? b >= blocks : tid >= row.extra) continue;
-            if (order_of(s.largest[b][tid]) >= least) {
-                const int i = atomicAdd(&s.blocks, 1);
-                if (i < THREADS) s.key[i] = b * THREADS + tid;          // (the threads' keys have been read)
-            }
-        }
-    }
-    __syncthreads();
-    const int listed = s.blocks;
-    auto offer = [&](float x, int at) {
-        if (order_of(x) < least) return;
-        const int i = atomicAdd(&s.count, 1);
-        if (i < CANDIDATES) s.list[i] = candidate(x, at);
-    };
-    if (listed <= THREADS) {
-        for (int i = warp; i < listed; i += THREADS / 32) {
-            const int b = (int)s.key[i] / THREADS, t = (int)s.key[i] % THREADS;
-            if (b == BLOCKS) {
-                if (lane == 0) offer(s.largest[b][t], row.extra_at(t));
-                continue;
-            }
-            for (int e = lane; e < per * UNROLL * V; e += 32) {
-                const int v = row.v0 + (b * per + e / (UNROLL * V)) * STEP + e / V % UNROLL * THREADS + t;
-                if (v < row.v1) {
-                    const int at = row.head + v * V + e % V;
-                    offer(ld_l2(row.x + at), at);
-                }
-            }
-        }
-        __syncthreads();
-        const int n = s.count;
-        if (n <= CANDIDATES) {
-            rank_candidates(s, n, top);
-            return;
-        }
-    }
-    // The top-th largest value of the share, eight bits at a time: `prefix`; `need` of those that equal it are taken, the first ones.
     __syncthreads();
     if (tid == 0) {
         s.prefix = 0;
@@ -330,35 +275,99 @@ __device__ __forceinline__ void find_top(TopScratch &s, const Row<T> &row, int t
     x[0] = tid < rest ? ld_l2(row.x + row.behind + tid) : 0.0f;
     round(x, tid < rest, row.behind + tid);
     __syncthreads();
-    rank_candidates(s, s.count < CANDIDATES ? s.count : CANDIDATES, top);
 }
 
+// This CTA's candidates into s.list, s.count of them (at most `room`, which is `top` or more).  s.group holds the groups' largest values; `key` is this thread's largest
+// value; those of its blocks of `per` steps lie in s.largest; `extra` is its value before or behind the pieces.
+template <typename T>
+__device__ __forceinline__ void find_candidates(TopScratch &s, const Row<T> &row, int top, int room, int blocks, int per, uint32_t key, float extra) {
+    constexpr int V = Piece<T>::V, BLOCK = UNROLL * V;
+    const int tid = threadIdx.x;
+    if (tid < GROUPS) {
+        const uint32_t mine = s.group[tid];
+        int larger = 0;
+#pragma unroll
+        for (int i = 0; i < GROUPS; i += 4) {
+            const uint4 k = *reinterpret_cast<const uint4 *>(s.group + i);
+            larger += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
+        }
+        const uint32_t low = __reduce_min_sync(0xffffffffu, larger < top ? mine : 0xffffffffu);
+        if (tid % 32 == 0) s.least[tid / 32] = low;
+    }
+    if (tid == 0) s.count = s.entries = 0;
+    __syncthreads();
+    const uint32_t least = min(s.least[0], s.least[1]);
+    auto offer = [&](float x, int at) {
+        if (order_of(x) < least) return;
+        const int i = atomicAdd(&s.count, 1);
+        if (i < room) s.list[i] = candidate(x, at);
+    };
+    if (key >= least) {
+        for (int b = 0; b < blocks; ++b)
+            if (order_of(s.largest[b][tid]) >= least) {
+                const int i = atomicAdd(&s.entries, 1);
+                if (i < THREADS) s.entry[i] = b * THREADS + tid;
+            }
+        if (tid < row.extra) offer(extra, row.extra_at(tid));
+    }
+    __syncthreads();
+    const int entries = s.entries;
+    if (entries <= THREADS) {
+        const int n = entries * per * BLOCK;
+        for (int e0 = tid; e0 < n; e0 += 4 * THREADS) {
+            float x[4];
+            int at[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int e = e0 + k * THREADS;
+                at[k] = -1;
+                if (e >= n) continue;
+                const int step = e / BLOCK, entry = (int)s.entry[step / per], v = row.v0 + (entry / THREADS * per + step % per) * STEP + e / V % UNROLL * THREADS + entry % THREADS;
+                if (v >= row.v1) continue;
+                at[k] = row.head + v * V + e % V;
+                x[k] = ld_l2(row.x + at[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (at[k] >= 0) offer(x[k], at[k]);
+        }
+        __syncthreads();
+        if (s.count <= room) return;
+    }
+    search_share(s, row, top);
+}
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// The sums of `lanes` lanes (a power of two) as one.
+__device__ __forceinline__ Sums joined(Sums a, int lanes) {
+    float m = a.m;
+    for (int d = lanes / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if (m > a.m) a.raise(m);
+    for (int d = lanes / 2; d; d >>= 1) {
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, d);
+        a.w += __shfl_xor_sync(0xffffffffu, a.w, d);
+    }
+    return a;
+}
+
+// A row a cluster.
 template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const LogProbs p) {
-    constexpr int V = Piece<T>::V;
+__global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const LogProbs p) {
+    constexpr int V = Piece<T>::V, WARPS = THREADS / 32;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int rank = (int)(blockIdx.x % p.cluster);
     const int64_t r = blockIdx.x / p.cluster;
-    __shared__ Sums s_warp[THREADS / 32], s_all;
+    __shared__ Sums s_warp[WARPS], s_all[8];
     __shared__ typename std::conditional<TOP, TopScratch, int>::type s_top;
+    const cg::cluster_group cluster = cg::this_cluster();
+    if (p.cluster > 1) cluster_arrive();                   // (all CTAs have begun before one writes into another's memory)
     pdl_wait();
     pdl_launch_dependents();
+
     const Row<T> row((const T *)p.logits + r * p.stride, p.vocab, rank, p.cluster);
     const int64_t t = p.tokens ? __ldcg(p.tokens + r) : -1;
-    if (!ENTROPY && !TOP && t < 0) {         // padding: nothing of the row is asked for
-        if (rank == 0 && tid == 0) {
-            if (p.tokens) p.log_probs[r] = 0.0f;
-            if (p.stats) p.stats[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        }
-        return;
-    }
-    const float xt = t >= 0 && t < p.vocab ? ld_l2(row.x + t) : NAN;
-
-    const int steps = (row.v1 - row.v0 + STEP - 1) / STEP, per = (steps + BLOCKS - 1) / BLOCKS;
-    Sums a = {-INFINITY, 0.0f, 0.0f};
-    uint32_t key = 0;
-    float block = -INFINITY;
-    int in_block = 0, blocks = 0;
     Piece<T> next[UNROLL];
     auto load = [&](int step) {
 #pragma unroll
@@ -368,7 +377,15 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const LogProbs p)
             else next[u].nothing();
         }
     };
-    if (steps) load(0);
+    load(0);
+    const float extra = tid < row.extra ? ld_l2(row.x + row.extra_at(tid)) : -INFINITY;
+    const float xt = t >= 0 && t < p.vocab ? ld_l2(row.x + t) : NAN;
+    const bool skipped = !ENTROPY && !TOP && t < 0;      // padding: nothing of the row is asked for
+    const int steps = skipped ? 0 : (row.v1 - row.v0 + STEP - 1) / STEP, per = (steps + BLOCKS - 1) / BLOCKS;
+    Sums a = {-INFINITY, 0.0f, 0.0f};
+    uint32_t key = 0;
+    float block = -INFINITY;
+    int in_block = 0, blocks = 0;
     for (int step = 0; step < steps; ++step) {
         Piece<T> x[UNROLL];
 #pragma unroll
@@ -399,51 +416,71 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_kernel(const LogProbs p)
         a.s += s.x + s.y;
         if constexpr (ENTROPY) a.w += w.x + w.y;
     }
-    if (tid < row.extra) {
-        const float x = ld_l2(row.x + row.extra_at(tid));
-        if constexpr (TOP) {
-            s_top.largest[BLOCKS][tid] = x;
-            key = max(key, order_of(x));
-        }
+    if (tid < row.extra && !skipped) {
+        if constexpr (TOP) key = max(key, order_of(extra));
         // (NaN is larger than no maximum: its difference goes into the sum)
-        if (x > a.m) a.raise(x);
-        const float d = __fmul_rn(x - (a.m == -INFINITY ? 0.0f : a.m), LOG2E), e = ex2(d);
+        if (extra > a.m) a.raise(extra);
+        const float d = __fmul_rn(extra - (a.m == -INFINITY ? 0.0f : a.m), LOG2E), e = ex2(d);
         a.s += e;
         if constexpr (ENTROPY) a.w += e * fmaxf(d, -1000.0f);
     }
-    for (int d = 16; d; d >>= 1) {
-        const Sums o = {__shfl_xor_sync(0xffffffffu, a.m, d), __shfl_xor_sync(0xffffffffu, a.s, d), ENTROPY ? __shfl_xor_sync(0xffffffffu, a.w, d) : 0.0f};
-        a.add(o);
-    }
+    a = joined(a, 32);
     if (lane == 0) s_warp[warp] = a;
-    __syncthreads();
-    a = s_warp[0];
-    for (int i = 1; i < THREADS / 32; ++i) a.add(s_warp[i]);
-    if constexpr (TOP) find_top(s_top, row, p.top, blocks, per, key);
-    if (p.cluster > 1) {
-        cg::cluster_group cluster = cg::this_cluster();
-        if (tid == 0) s_all = a;
-        cluster.sync();
-        if (rank == 0) {
-            for (int i = 1; i < p.cluster; ++i) a.add(*cluster.map_shared_rank(&s_all, i));
-            if constexpr (TOP) {
-                // the ranks' best become one list
-                const int n = p.cluster * p.top;
-                if (tid < n) s_top.list[tid] = *cluster.map_shared_rank(&s_top.best[tid % p.top], tid / p.top);
-                __syncthreads();
-                // (a share of few values has less than `top`: zeros, of which none comes before a value)
-                rank_candidates(s_top, n, p.top);
+    const int room = CANDIDATES / p.cluster;
+    if constexpr (TOP) {
+        const int size = THREADS * p.cluster / GROUPS;       // threads of a group, 4 to 32
+        uint32_t k = key;
+        for (int d = 1; d < size; d *= 2) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
+        if (p.cluster > 1) cluster_wait();
+        if (tid % size == 0)
+            for (int i = 0; i < p.cluster; ++i) {
+                uint32_t *to = s_top.group + rank * (GROUPS / p.cluster) + tid / size;
+                *(p.cluster > 1 ? cluster.map_shared_rank(to, i) : to) = k;
             }
-        }
-        cluster.sync();
+    }
+    __syncthreads();
+    a = joined(s_warp[lane % WARPS], WARPS);                 // (in every warp)
+    if (p.cluster > 1) {
+        if constexpr (TOP) {
+            cluster_arrive();
+            cluster_wait();
+        } else cluster_wait();
+        if (tid == 0) *cluster.map_shared_rank(s_all + rank, 0) = a;
+    }
+    if constexpr (TOP) {
+        find_candidates(s_top, row, p.top, room, blocks, per, key, extra);
+        const int n = s_top.count;
+        if (p.cluster > 1) {
+            uint64_t *to = cluster.map_shared_rank(s_top.all, 0);
+            for (int i = tid; i < n; i += THREADS) to[rank * room + i] = s_top.list[i];
+            if (tid == 0) *cluster.map_shared_rank(s_top.counts + rank, 0) = n;
+        } else rank_candidates(s_top.list, n, p.top, s_top.best);
+    }
+    if (p.cluster > 1) {
+        cluster_arrive();
         if (rank != 0) return;
+        cluster_wait();
+        a = joined(s_all[lane % p.cluster], p.cluster);
+        if constexpr (TOP) {
+            // (s_top.list, whose candidates are rank 0's part of `all`, takes them all)
+            const int mine = lane < p.cluster ? s_top.counts[lane] : 0;      // (a warp a rank)
+            int sum = mine;
+            for (int d = 1; d < 8; d *= 2) {
+                const int o = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += o;
+            }
+            const int n = __shfl_sync(0xffffffffu, sum, 7), from = __shfl_sync(0xffffffffu, sum - mine, warp), here = __shfl_sync(0xffffffffu, mine, warp);
+            for (int k = lane; k < here; k += 32) s_top.list[from + k] = s_top.all[warp * room + k];
+            __syncthreads();
+            rank_candidates(s_top.list, n, p.top, s_top.best);
+        }
     }
     // (infinities of either sign as the largest value, and NaN: nothing is known of the row)
     const float log2s = fabsf(a.m) == INFINITY ? NAN : log2f(a.s), ln_s = __fmul_rn(LN2, log2s), h = ENTROPY ? ln_s - LN2 * (a.w / a.s) : 0.0f;
     if (tid == 0) {
         if (p.tokens) p.log_probs[r] = t < 0 ? 0.0f : (xt - a.m) - ln_s;
         if (ENTROPY) p.entropy[r] = h;
-        if (p.stats) p.stats[r] = make_float4(a.m, log2s, h, 0.0f);
+        if (p.stats) p.stats[r] = skipped ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(a.m, log2s, h, 0.0f);
     }
     if constexpr (TOP)
         if (tid < p.top) {
@@ -545,22 +582,31 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogPro
     }
 }
 
-// CTAs of a row: so many that all rows together fill the SMs eight times over with 256 threads, of at least a step (16 KB) each.
+// CTAs of a row: as many as all run at once, of at least a step (16 KB) each.  (61 x 131071 bf16: 12.8 us with one, 8.5 two, 6.6 four, 7.0 eight; 300 x 50272 13.4, 12.8, 14.3, 20.1;
+// 2000 x 32000 28.5, 40.6, 61, 120.)
 int ctas_of(int64_t rows, int64_t vocab, size_t size) {
     int n = 1;
-    while (n < 8 && rows * n < 148 * 8 && vocab * (int64_t)size > (int64_t)n * STEP * 16) n *= 2;
+    while (n < 8 && rows * n * 2 <= MOST_CTAS && vocab * (int64_t)size > (int64_t)n * STEP * 16) n *= 2;
     return n;
 }
 
 template <typename T, bool ENTROPY, bool TOP>
-int log_probs_launch(const LogProbs &p, int64_t rows, cudaStream_t st) {
-    return launch_early("log_probs_kernel", log_probs_kernel<T, ENTROPY, TOP>, dim3((unsigned)(rows * p.cluster)), THREADS, 0, st, dim3(p.cluster), p);
+int log_probs_launch(const LogProbs &p, cudaStream_t st) {
+    return launch_early("log_probs_kernel", log_probs_kernel<T, ENTROPY, TOP>, dim3((unsigned)(p.rows * p.cluster)), THREADS, 0, st, dim3(p.cluster), p);
 }
 template <typename T>
-int log_probs_typed(LogProbs &p, int64_t rows, cudaStream_t st) {
-    p.cluster = ctas_of(rows, p.vocab, sizeof(T));
-    if (p.top) return p.entropy ? log_probs_launch<T, true, true>(p, rows, st) : log_probs_launch<T, false, true>(p, rows, st);
-    return p.entropy ? log_probs_launch<T, true, false>(p, rows, st) : log_probs_launch<T, false, false>(p, rows, st);
+int log_probs_typed(LogProbs &p, cudaStream_t st) {
+    p.cluster = ctas_of(p.rows, p.vocab, sizeof(T));
+    if (p.top) return p.entropy ? log_probs_launch<T, true, true>(p, st) : log_probs_launch<T, false, true>(p, st);
+    return p.entropy ? log_probs_launch<T, true, false>(p, st) : log_probs_launch<T, false, false>(p, st);
+}
+
+// CTAs of a row of the gradient, which do not join: so many that all rows together fill the SMs twice over, of at least a step (16 KB) each; and of at most 64 KB.
+// (8192 x 131072 bf16: 657 us with one, 650 two, 640 four, 669 eight; 2048 x 32000 46, 48, 58, 91; 61 x 131071 15.6, 10.5, 8.5, 8.9.)
+int parts_of(int64_t rows, int64_t vocab, size_t size) {
+    int n = 1;
+    while (n < 8 && ((rows * n < 2 * MOST_CTAS && vocab * (int64_t)size > (int64_t)n * STEP * 16) || vocab * (int64_t)size > (int64_t)n << 16)) n *= 2;
+    return n;
 }
 
 template <typename T, bool ENTROPY, bool ALIGNED>
@@ -569,7 +615,7 @@ int log_probs_grad_launch(const LogProbsGrad &p, int64_t rows, cudaStream_t st) 
 }
 template <typename T>
 int log_probs_grad_typed(LogProbsGrad &p, int64_t rows, cudaStream_t st) {
-    p.parts = ctas_of(rows, p.vocab, sizeof(T));
+    p.parts = parts_of(rows, p.vocab, sizeof(T));
     const uintptr_t apart = (reinterpret_cast<uintptr_t>(p.logits) - reinterpret_cast<uintptr_t>(p.grad)) % 16;
     const bool aligned = apart == 0 && (rows == 1 || (p.stride - p.vocab) * (int64_t)sizeof(T) % 16 == 0);
     if (p.e) return aligned ? log_probs_grad_launch<T, true, true>(p, rows, st) : log_probs_grad_launch<T, true, false>(p, rows, st);
@@ -580,10 +626,10 @@ int log_probs_grad_typed(LogProbsGrad &p, int64_t rows, cudaStream_t st) {
 
 int token_log_probs(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, float *log_probs, float *entropy,
                     int top, float *top_log_probs, int64_t *top_tokens, float *stats, cudaStream_t st) {
-    LogProbs p = {logits, tokens, log_probs, entropy, top_log_probs, top_tokens, (float4 *)stats, stride, (int)vocab, top, 1};
-    if (dtype == BW_F32) return log_probs_typed<float>(p, rows, st);
-    if (dtype == BW_F16) return log_probs_typed<__half>(p, rows, st);
-    return log_probs_typed<__nv_bfloat16>(p, rows, st);
+    LogProbs p = {logits, tokens, log_probs, entropy, top_log_probs, top_tokens, (float4 *)stats, stride, rows, (int)vocab, top, 1};
+    if (dtype == BW_F32) return log_probs_typed<float>(p, st);
+    if (dtype == BW_F16) return log_probs_typed<__half>(p, st);
+    return log_probs_typed<__nv_bfloat16>(p, st);
 }
 
 int token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, const float *stats,
