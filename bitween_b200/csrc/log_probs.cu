@@ -150,7 +150,7 @@ template <typename T> struct Row {
 // values, as masks leave them; many large ones in few threads' places) a CTA finds the `top` best of its share digit by digit instead.
 constexpr int GROUPS = 64;
 struct __align__(16) TopScratch {
-    float largest[BLOCKS][THREADS];                    // of a thread's blocks
+    float largest[BLOCKS][THREADS + 1];                // of a thread's blocks
     __align__(16) uint32_t group[GROUPS];              // the groups' largest values, of all CTAs
     __align__(16) uint64_t list[CANDIDATES + 2];       // this CTA's candidates: (order << 32) | ~index
     __align__(16) uint64_t all[CANDIDATES + 2];        // all CTAs' (rank 0)
@@ -281,8 +281,9 @@ __device__ __noinline__ void search_share(TopScratch &s, const Row<T> &row, int 
 // value; those of its blocks of `per` steps lie in s.largest; `extra` is its value before or behind the pieces.
 template <typename T>
 __device__ __forceinline__ void find_candidates(TopScratch &s, const Row<T> &row, int top, int room, int blocks, int per, uint32_t key, float extra) {
-    constexpr int V = Piece<T>::V, BLOCK = UNROLL * V;
-    const int tid = threadIdx.x;
+    constexpr int V = Piece<T>::V, BLOCK = UNROLL * V;      // values of a thread's step: 16 or 32
+    static_assert(BLOCK <= 32, "a lane a value");
+    const int tid = threadIdx.x, lane = tid % 32;
     if (tid < GROUPS) {
         const uint32_t mine = s.group[tid];
         int larger = 0;
@@ -302,35 +303,36 @@ __device__ __forceinline__ void find_candidates(TopScratch &s, const Row<T> &row
         const int i = atomicAdd(&s.count, 1);
         if (i < room) s.list[i] = candidate(x, at);
     };
-    if (key >= least) {
-        for (int b = 0; b < blocks; ++b)
-            if (order_of(s.largest[b][tid]) >= least) {
-                const int i = atomicAdd(&s.entries, 1);
-                if (i < THREADS) s.entry[i] = b * THREADS + tid;
-            }
-        if (tid < row.extra) offer(extra, row.extra_at(tid));
+    if (key >= least && tid < row.extra) offer(extra, row.extra_at(tid));
+    // (a warp looks at all blocks of one of its threads at once)
+    for (unsigned left = __ballot_sync(0xffffffffu, key >= least); left; left &= left - 1) {
+        const int t = tid - lane + __ffs(left) - 1;
+        const bool hit = lane < blocks && order_of(s.largest[lane % BLOCKS][t]) >= least;
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        int at = 0;
+        if (lane == 0 && hits) at = atomicAdd(&s.entries, __popc(hits));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(hits & ((1u << lane) - 1));
+        if (hit && at < THREADS) s.entry[at] = lane * THREADS + t;
     }
     __syncthreads();
     const int entries = s.entries;
     if (entries <= THREADS) {
-        const int n = entries * per * BLOCK;
-        for (int e0 = tid; e0 < n; e0 += 4 * THREADS) {
-            float x[4];
-            int at[4];
+        // a warp a block, four of them in flight
+        for (int step = 0; step < per; ++step)
+            for (int i0 = tid / 32; i0 < entries; i0 += 4 * (THREADS / 32)) {
+                float x[4];
+                int at[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int e = e0 + k * THREADS;
-                at[k] = -1;
-                if (e >= n) continue;
-                const int step = e / BLOCK, entry = (int)s.entry[step / per], v = row.v0 + (entry / THREADS * per + step % per) * STEP + e / V % UNROLL * THREADS + entry % THREADS;
-                if (v >= row.v1) continue;
-                at[k] = row.head + v * V + e % V;
-                x[k] = ld_l2(row.x + at[k]);
+                for (int k = 0; k < 4; ++k) {
+                    const int i = i0 + k * (THREADS / 32), entry = i < entries ? (int)s.entry[i] : 0;
+                    const int v = row.v0 + (entry / THREADS * per + step) * STEP + lane / V * THREADS + entry % THREADS;
+                    at[k] = i < entries && lane < BLOCK && v < row.v1 ? row.head + v * V + lane % V : -1;
+                    if (at[k] >= 0) x[k] = ld_l2(row.x + at[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (at[k] >= 0) offer(x[k], at[k]);
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (at[k] >= 0) offer(x[k], at[k]);
-        }
         __syncthreads();
         if (s.count <= room) return;
     }
