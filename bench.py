@@ -499,15 +499,18 @@ def run_case(args, torch, device):
     plain (ungraphed) launches over 4 distinct layer copies, so that a profiler can capture a single
     launch without the rest of the benchmark.  kind: decode | prefill (both the qmatmul call),
     rtn, gradinput, fakequant; adapter | adaptertrain (`...:shape:tokens:rank`, one adapter beside that shape);
-    attend | append | read (`...:sequences x tokens:bits`, 32 query and 8 cache heads of 128).
+    attend | append | read | appendrotated | rotate (`...:sequences x tokens:bits[:window:sinks]`, 32 query and 8 cache heads of 128);
+    logprobs | logprobstrain (`...:rows x vocabulary:alternatives`).
     Prints one small JSON line with the CUDA-event time per launch."""
     from bitween_b200 import functional as fn
     from bitween_b200.kernels import _lib
     from bitween_b200.kernels.cuda_loader import quantized_matmul_cuda as qmm, quantized_matmul_grad_input as qgrad
     parts = args.case.split(":")
     kind, shape = parts[0], parts[1]
-    if kind in ("attend", "append", "read"):
-        return run_cache_case(args, torch, device, kind, *(int(v) for v in shape.split("x")), int(parts[2]) if len(parts) > 2 else 4)
+    if kind in ("attend", "append", "read", "appendrotated", "rotate"):
+        return run_cache_case(args, torch, device, kind, *(int(v) for v in shape.split("x")), *(int(v) for v in parts[2:]))
+    if kind in ("logprobs", "logprobstrain"):
+        return run_log_probs_case(args, torch, device, kind, *(int(v) for v in shape.split("x")), *(int(v) for v in parts[2:]))
     M = int(parts[2]) if len(parts) > 2 else 1
     bits = int(parts[3]) if len(parts) > 3 else 4
     g = int(parts[4]) if len(parts) > 4 else 128
@@ -557,9 +560,31 @@ def run_case(args, torch, device):
                       "note": "plain launches, back to back, no L2 flush: a profiling aid, not a benchmark value"}), flush=True)
 
 
-def run_cache_case(args, torch, device, kind, sequences, tokens, bits):
+def run_log_probs_case(args, torch, device, kind, rows, vocab, top=0):
+    """The log probabilities' part of run_case: bf16 rows, entropy and `top` alternatives; with their gradient."""
+    from bitween_b200 import token_log_probs
+    from bitween_b200.kernels import _lib
+    gen = torch.Generator(device=device).manual_seed(7)
+    copies = 4
+    logits = [torch.randn(rows, vocab, device=device, generator=gen, dtype=torch.bfloat16).mul_(2.5).requires_grad_(kind == "logprobstrain") for _ in range(copies)]
+    tokens = torch.randint(0, vocab, (rows,), device=device, generator=gen)
+    grad = torch.full((rows,), -1.0 / rows, device=device)
+
+    def some():
+        for x in logits:
+            r = token_log_probs(x, tokens, entropy=True, top=top)
+            if kind == "logprobstrain":
+                torch.autograd.grad((r.log_probs, r.entropy), x, (grad, grad))
+
+    some()
+    ms = time_region(torch, some) / copies
+    print(json.dumps({"case": args.case, "kernel": _lib.last_kernel(), "us_per_launch": round(ms * 1e3, 2), "copies": copies,
+                      "note": "plain calls, back to back, no L2 flush: a profiling aid, not a benchmark value"}), flush=True)
+
+
+def run_cache_case(args, torch, device, kind, sequences, tokens, bits=4, window=None, sinks=0):
     """The key-value cache's part of run_case: every sequence has `tokens` rows on scattered pages of 16."""
-    from bitween_b200 import QuantizedKVCache
+    from bitween_b200 import QuantizedKVCache, RotaryPositions
     from bitween_b200.kernels import _lib
     gen = torch.Generator(device=device).manual_seed(6)
     wide = -(-tokens // 16)
@@ -575,8 +600,13 @@ def run_cache_case(args, torch, device, kind, sequences, tokens, bits):
     table = table.to(torch.int32)
     last = slots[-(1 << 16):]
     rows = torch.randn(last.numel(), 16, 128, device=device, generator=gen).to(torch.bfloat16)
-    body = {"attend": lambda: cache.attend(q, table, lengths), "append": lambda: cache.append(rows[:, :8], rows[:, 8:], last),
-            "read": lambda: cache.read(last, dtype=torch.bfloat16)}[kind]
+    if kind in ("appendrotated", "rotate"):
+        rotary = RotaryPositions(128, 1 << 16, sections=(16, 24, 24), device=device)
+        positions = torch.arange(last.numel(), device=device).expand(3, -1).contiguous()
+        queries = torch.randn(last.numel(), 32, 128, device=device, generator=gen).to(torch.bfloat16)
+    body = {"attend": lambda: cache.attend(q, table, lengths, window=window, sinks=sinks), "append": lambda: cache.append(rows[:, :8], rows[:, 8:], last),
+            "read": lambda: cache.read(last, dtype=torch.bfloat16), "rotate": lambda: rotary.rotate(positions, queries, rows[:, :8]),
+            "appendrotated": lambda: cache.append_rotated(queries, rows[:, :8], rows[:, 8:], last, rotary, positions)}[kind]
     copies = 4
 
     def some():
