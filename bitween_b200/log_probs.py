@@ -111,6 +111,8 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0):
         tokens = tokens.reshape(-1).contiguous()
     x = _rows(logits.reshape(-1, vocab))
     entropy = bool(entropy)
+    if tokens is None and not entropy and not top:
+        return TokenLogProbs(None, None, None, None)
     out = ops.token_log_probs(x, tokens, entropy, top)
     if out is None:
         out = TokenLogProbsFunction.apply(x, tokens, entropy, top) if torch.is_grad_enabled() and logits.requires_grad else _forward(x, tokens, entropy, top, False)[:4]
