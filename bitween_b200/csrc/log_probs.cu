@@ -150,14 +150,14 @@ template <typename T> struct Row {
 // values, as masks leave them; many large ones in few threads' places) a CTA finds the `top` best of its share digit by digit instead.
 constexpr int GROUPS = 64;
 struct __align__(16) TopScratch {
-    float largest[BLOCKS][THREADS + 1];                // of a thread's blocks
+    float largest[BLOCKS][THREADS];                    // of a thread's blocks
     __align__(16) uint32_t group[GROUPS];              // the groups' largest values, of all CTAs
     __align__(16) uint64_t list[CANDIDATES + 2];       // this CTA's candidates: (order << 32) | ~index
     __align__(16) uint64_t all[CANDIDATES + 2];        // all CTAs' (rank 0)
     uint64_t best[32];
     uint32_t histogram[THREADS], entry[THREADS];
     int count, entries, need, counts[8];
-    uint32_t least[2], prefix;
+    uint32_t least[THREADS / 32], prefix;
     int scan[THREADS / 32];
 };
 
@@ -284,35 +284,39 @@ __device__ __forceinline__ void find_candidates(TopScratch &s, const Row<T> &row
     constexpr int V = Piece<T>::V, BLOCK = UNROLL * V;      // values of a thread's step: 16 or 32
     static_assert(BLOCK <= 32, "a lane a value");
     const int tid = threadIdx.x, lane = tid % 32;
-    if (tid < GROUPS) {
-        const uint32_t mine = s.group[tid];
-        int larger = 0;
+    static_assert(THREADS == 4 * GROUPS, "four threads a group");
+    const uint32_t mine = s.group[tid / 4];
+    int larger = 0;
 #pragma unroll
-        for (int i = 0; i < GROUPS; i += 4) {
-            const uint4 k = *reinterpret_cast<const uint4 *>(s.group + i);
-            larger += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
-        }
-        const uint32_t low = __reduce_min_sync(0xffffffffu, larger < top ? mine : 0xffffffffu);
-        if (tid % 32 == 0) s.least[tid / 32] = low;
+    for (int i = 0; i < GROUPS / 4; i += 4) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(s.group + tid % 4 * (GROUPS / 4) + i);
+        larger += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
     }
+    larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+    larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+    const uint32_t low = __reduce_min_sync(0xffffffffu, larger < top ? mine : 0xffffffffu);
+    if (lane == 0) s.least[tid / 32] = low;
     if (tid == 0) s.count = s.entries = 0;
     __syncthreads();
-    const uint32_t least = min(s.least[0], s.least[1]);
+    uint32_t least = s.least[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) least = min(least, s.least[i]);
     auto offer = [&](float x, int at) {
         if (order_of(x) < least) return;
         const int i = atomicAdd(&s.count, 1);
         if (i < room) s.list[i] = candidate(x, at);
     };
-    if (key >= least && tid < row.extra) offer(extra, row.extra_at(tid));
-    // (a warp looks at all blocks of one of its threads at once)
-    for (unsigned left = __ballot_sync(0xffffffffu, key >= least); left; left &= left - 1) {
-        const int t = tid - lane + __ffs(left) - 1;
-        const bool hit = lane < blocks && order_of(s.largest[lane % BLOCKS][t]) >= least;
-        const unsigned hits = __ballot_sync(0xffffffffu, hit);
-        int at = 0;
-        if (lane == 0 && hits) at = atomicAdd(&s.entries, __popc(hits));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(hits & ((1u << lane) - 1));
-        if (hit && at < THREADS) s.entry[at] = lane * THREADS + t;
+    if (key >= least) {
+        if (tid < row.extra) offer(extra, row.extra_at(tid));
+        uint32_t hits = 0;
+#pragma unroll
+        for (int b = 0; b < BLOCKS; ++b)
+            if (b < blocks) hits |= (uint32_t)(order_of(s.largest[b][tid]) >= least) << b;
+        if (hits) {
+            int at = atomicAdd(&s.entries, __popc(hits));
+            for (; hits; hits &= hits - 1, ++at)
+                if (at < THREADS) s.entry[at] = (__ffs(hits) - 1) * THREADS + tid;
+        }
     }
     __syncthreads();
     const int entries = s.entries;
@@ -342,10 +346,9 @@ __device__ __forceinline__ void find_candidates(TopScratch &s, const Row<T> &row
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
-// The sums of `lanes` lanes (a power of two) as one.
+// The sums of `lanes` neighbouring lanes (a power of two, and other lanes' the same again) as one.
 __device__ __forceinline__ Sums joined(Sums a, int lanes) {
-    float m = a.m;
-    for (int d = lanes / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    const float m = value_of(__reduce_max_sync(0xffffffffu, order_of(a.m)));
     if (m > a.m) a.raise(m);
     for (int d = lanes / 2; d; d >>= 1) {
         a.s += __shfl_xor_sync(0xffffffffu, a.s, d);
@@ -426,8 +429,6 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
         a.s += e;
         if constexpr (ENTROPY) a.w += e * fmaxf(d, -1000.0f);
     }
-    a = joined(a, 32);
-    if (lane == 0) s_warp[warp] = a;
     const int room = CANDIDATES / p.cluster;
     if constexpr (TOP) {
         const int size = THREADS * p.cluster / GROUPS;       // threads of a group, 4 to 32
@@ -439,22 +440,22 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
                 uint32_t *to = s_top.group + rank * (GROUPS / p.cluster) + tid / size;
                 *(p.cluster > 1 ? cluster.map_shared_rank(to, i) : to) = k;
             }
+        if (p.cluster > 1) cluster_arrive();                 // (on their way while the sums are joined)
     }
+    a = joined(a, 32);
+    if (lane == 0) s_warp[warp] = a;
     __syncthreads();
     a = joined(s_warp[lane % WARPS], WARPS);                 // (in every warp)
     if (p.cluster > 1) {
-        if constexpr (TOP) {
-            cluster_arrive();
-            cluster_wait();
-        } else cluster_wait();
+        cluster_wait();
         if (tid == 0) *cluster.map_shared_rank(s_all + rank, 0) = a;
     }
     if constexpr (TOP) {
         find_candidates(s_top, row, p.top, room, blocks, per, key, extra);
         const int n = s_top.count;
         if (p.cluster > 1) {
-            uint64_t *to = cluster.map_shared_rank(s_top.all, 0);
-            for (int i = tid; i < n; i += THREADS) to[rank * room + i] = s_top.list[i];
+            uint64_t *to = cluster.map_shared_rank(s_top.all, 0) + rank * room;
+            for (int i = tid; i < n; i += THREADS) to[i] = s_top.list[i];
             if (tid == 0) *cluster.map_shared_rank(s_top.counts + rank, 0) = n;
         } else rank_candidates(s_top.list, n, p.top, s_top.best);
     }
@@ -462,10 +463,10 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
         cluster_arrive();
         if (rank != 0) return;
         cluster_wait();
-        a = joined(s_all[lane % p.cluster], p.cluster);
         if constexpr (TOP) {
-            // (s_top.list, whose candidates are rank 0's part of `all`, takes them all)
-            const int mine = lane < p.cluster ? s_top.counts[lane] : 0;      // (a warp a rank)
+            // (s_top.list, whose candidates are rank 0's part of `all`, takes them all, a warp those of one rank)
+            static_assert(WARPS == 8, "a warp a rank");
+            const int mine = lane < p.cluster ? s_top.counts[lane] : 0;
             int sum = mine;
             for (int d = 1; d < 8; d *= 2) {
                 const int o = __shfl_up_sync(0xffffffffu, sum, d);
@@ -476,6 +477,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
             __syncthreads();
             rank_candidates(s_top.list, n, p.top, s_top.best);
         }
+        a = joined(s_all[lane % p.cluster], p.cluster);
     }
     // (infinities of either sign as the largest value, and NaN: nothing is known of the row)
     const float log2s = fabsf(a.m) == INFINITY ? NAN : log2f(a.s), ln_s = __fmul_rn(LN2, log2s), h = ENTROPY ? ln_s - LN2 * (a.w / a.s) : 0.0f;
