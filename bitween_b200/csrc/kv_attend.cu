@@ -94,10 +94,12 @@ int attend_general(const AttendArgs &p, int64_t batch, int bits, cudaStream_t st
 }  // namespace
 
 size_t kv_attend_workspace_bytes(int64_t batch, int heads, int kv_heads, int dim, int page_size, int64_t max_pages, int64_t window, int64_t sinks) {
-    FastArgs p;
-    // (a cache of more rows asks for scratch that it does not use)
-    if (!fast_args(p, batch, heads, kv_heads, dim, 0, page_size, max_pages, window, sinks) || p.cluster) return 0;
-    return (size_t)2 * MOST_CTAS * p.cols * (dim + 2) * sizeof(float);
+    // (what any number of bits needs; and a cache of more rows asks for scratch that it does not use)
+    for (int bits : {2, 4, 8}) {
+        FastArgs p;
+        if (fast_args(p, batch, heads, kv_heads, dim, bits, 0, page_size, max_pages, window, sinks) && !p.cluster) return (size_t)2 * MOST_CTAS * p.cols * (dim + 2) * sizeof(float);
+    }
+    return 0;
 }
 
 int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stride, int64_t q_head_stride, const int32_t *kc, const int32_t *vc,
@@ -106,7 +108,7 @@ int kv_attend(const void *q, int dtype, int64_t batch, int heads, int64_t q_stri
     FastArgs f = {};
     AttendArgs p = {q, kc, vc, (const __half2 *)params, table, lengths, out, q_stride, q_head_stride, table_stride, pages,
                     heads, kv_heads, dim, dim * bits / 32, page_size, max_pages, alpha, window, sinks};
-    if (fast_args(f, batch, heads, kv_heads, dim, pages, page_size, max_pages, window, sinks)) {
+    if (fast_args(f, batch, heads, kv_heads, dim, bits, pages, page_size, max_pages, window, sinks)) {
         if (window < INT32_MAX) return attend_window_tiles(p, batch, dtype, bits, workspace, st);
         f.a = p;
         f.slots = (float *)workspace;

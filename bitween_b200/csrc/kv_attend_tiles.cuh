@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "early_launch.cuh"
 
@@ -714,9 +715,30 @@ __global__ void __launch_bounds__(128) kv_attend_join_kernel(const FastArgs p) {
         out[d] = from_f32<T>((s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) / (s_part[0] + s_part[1] + s_part[2] + s_part[3]));
 }
 
+// CTAs of a cluster that takes a unit of a window of `steps`; 0: the line of work.  A window's sequences are alike, so that CTAs need no equal shares, and without a join one CTA a unit is
+// as fast as the chip goes from some hundred units on.  Times in steps of a warp (0.75 us of 32 tokens of 128 values): a part's own, two more for a cluster's join; or what
+// the chip needs for all, each CTA's start and end counting 13 steps, and a third of what its last wave leaves idle; the line's parts and join count 30.  Measured, 4 bits, line / 1 / 2 / 4 / 8 CTAs:
+// 64 units of 17 steps 10.7 / 8.2 / 8.9 / 8.1 / 8.6 us, 64 of 129 17.7 / 29.1 / 19.1 / 15.2 / 15.8, 512 of 17 25.7 / 15.2 / 23.0 / 34.6 / 58.3, 1536 of 129 205 / 172 / 181 / 216 / 290; 8 bits, 512 of 129 97 / 121 /
+// 113 / 110 / 150.
+int window_cluster(int64_t units, int64_t steps, int dim, int cols, int pair, int bits) {
+    const double slots = 148 * (dim == 256 ? 2 : cols == 16 ? (dim == 64 ? 3 : 2) : bits == 8 && dim == 128 ? 3 : 4);
+    const double rate = 600.0 * 128 / dim * (pair == 2 ? 1 : 2) * (bits == 8 ? 1.0 : 1.6);      // steps of all SMs in a warp's
+    double best = std::max(12.0, units * (steps + 30) / rate);
+    int found = 0;
+    for (int c = 1; c <= 8 && (c == 1 || steps > c / 2 * WARPS); c *= 2) {
+        const double waves = units * c / slots, idle = waves > 1 ? (std::ceil(waves) / waves - 1) / 3 : 0;
+        const double own = (double)((steps + WARPS * c - 1) / (WARPS * c)) + (c > 1 ? 2 : 0), all = units * (13 * c + steps) / rate * (1 + idle);
+        if (std::max(own, all) < best) {
+            best = std::max(own, all);
+            found = c;
+        }
+    }
+    return found;
+}
+
 // Whether the tiled kernel takes this cache, and how it divides a call.
-// `window`, `sinks`: INT32_MAX and 0 where everything is seen.
-bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int64_t pages, int page_size, int64_t max_pages, int64_t window, int64_t sinks) {
+// `window`, `sinks`: INT32_MAX and 0 where everything is seen.  (Without a window `bits` does not matter.)
+bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int bits, int64_t pages, int page_size, int64_t max_pages, int64_t window, int64_t sinks) {
     // (rows of the cache are numbered in 32 bits)
     if ((dim != 64 && dim != 128 && dim != 256) || page_size % TILE != 0 || pages * kv_heads * page_size >= 0xfffffffell) return false;
     const int group = heads / kv_heads;
@@ -737,6 +759,8 @@ bool fast_args(FastArgs &p, int64_t batch, int heads, int kv_heads, int dim, int
     if (size > wide) size = wide;
     size = size > 8 ? 8 : size < 1 ? 1 : size;
     p.cluster = steps <= size * WARPS * (size > 1 ? CLUSTER_ROUNDS : 2) ? (int)size : 0;
+    // (a long window of more than half of the longest sequence meets lengths as ragged as attention without one does)
+    if (window < INT32_MAX && (steps <= 64 || 2 * tiles <= p.most_tiles)) p.cluster = window_cluster(items, steps, dim, p.cols, p.pair, bits);
     return batch * p.units < (int64_t)1 << 28;
 }
 
