@@ -25,7 +25,7 @@ namespace cg = cooperative_groups;
 constexpr int THREADS = 256, UNROLL = 4, BLOCKS = 16;     // of a CTA; 16-byte loads of a step; blocks of steps of a thread
 constexpr int STEP = THREADS * UNROLL;                     // 16-byte pieces of a CTA's step
 constexpr int CANDIDATES = 512;
-constexpr int MOST_CTAS = 4 * 148;                         // at once, at least: four an SM
+constexpr int MOST_CTAS = 4 * 148;                         // four an SM
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // The order of the alternatives: falling value, rising index; NaN before all.  Larger is better; nothing is 0.
@@ -588,11 +588,13 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogPro
     }
 }
 
-// CTAs of a row: as many as all run at once, of at least a step (16 KB) each.  (61 x 131071 bf16: 12.8 us with one, 8.5 two, 6.6 four, 7.0 eight; 300 x 50272 13.4, 12.8, 14.3, 20.1;
-// 2000 x 32000 28.5, 40.6, 61, 120.)
+// CTAs of a row, of at least a step (16 KB) each, rows of more than two steps: so many that all rows together have two an SM; of rows of more than 384 KB four.  bf16 with entropy and five
+// alternatives, 1 / 2 / 4 / 8 CTAs: 32 x 50272 7.8 / 7.7 / 7.0 / 7.1 us, 64 x 50272 7.8 / 7.7 / 7.6 / 9.4, 128 x 50272 9.7 / 9.7 / 11.1 / 16.9, 256 x 50272 11.7 / 14.6 / 20.2 / 31.6, 64 x 16000 5.2 / 6.0 / 6.7 / 8.9, 64 x 131072 16.4 /
+// 12.0 / 10.1 / 11.2; fp32, 80 x 131072 27.7 / 18.8 / 16.3 / 20.7, without alternatives 23.8 / 14.6 / 11.0 / 10.1.
 int ctas_of(int64_t rows, int64_t vocab, size_t size) {
+    const int64_t bytes = vocab * (int64_t)size, most = bytes > 384 << 10 ? MOST_CTAS : MOST_CTAS / 2;
     int n = 1;
-    while (n < 8 && rows * n * 2 <= MOST_CTAS && vocab * (int64_t)size > (int64_t)n * STEP * 16) n *= 2;
+    while (n < 8 && rows * n * 2 <= most && bytes > (int64_t)n * STEP * 16 && bytes > 2 * STEP * 16) n *= 2;
     return n;
 }
 

@@ -173,3 +173,44 @@ def test_windows_on_threads_of_their_own_streams():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_long_and_overlapping_rows(dtype):
+    """Rows of 30 million values, whose blocks are hundreds of steps; rows that begin inside each other."""
+    x = (2 * torch.randn(2, 30000001, generator=_gen(14), device=DEV)).to(dtype)
+    x[1, 29999990:] = 7.5
+    t = torch.tensor([29999999, 0], device=DEV)
+    r = token_log_probs(x, t, entropy=True, top=32)
+    assert torch.equal(r.top_tokens, torch.sort(x.float(), descending=True, stable=True).indices[:, :32])
+    lp = torch.log_softmax(x.double(), -1)
+    h = torch.special.entr(lp.exp()).sum(-1)
+    # spans of 25: 2^-22 of them for a weight's exponent, sums of some hundred parts a thread (2^-17 of a sum of parts of one sign)
+    assert bool(((r.log_probs.double() - lp.gather(1, t[:, None])[:, 0]).abs() <= 2.0 ** -16).all())
+    assert bool(((r.entropy.double() - h).abs() <= 2.0 ** -15 * 20).all())
+    flat = x[0, :100000]
+    rows = flat.as_strided((50, 5000), (1201, 1))
+    a, b = token_log_probs(rows, top=3, entropy=True), token_log_probs(rows.contiguous(), top=3, entropy=True)
+    assert torch.equal(a.top_tokens, b.top_tokens)
+    # (pieces begin elsewhere in a row: the same sums in another order)
+    assert bool(((a.entropy - b.entropy).abs() <= 2.0 ** -18 * 10).all())
+
+
+def test_one_value_and_few():
+    """Vocabularies of 1 to 40, each as dense rows and as rows off their boundaries: fewer values than threads, pieces or alternatives' groups."""
+    for vocab in range(1, 41):
+        big = torch.randn(9, vocab + 3, generator=_gen(vocab), device=DEV)
+        for x in (big[:, :vocab].contiguous(), big[:, 1:1 + vocab], big[:, 2:2 + vocab].half(), big.bfloat16()[:, 3:3 + vocab]):
+            t = torch.arange(9, device=DEV) % vocab
+            top = min(vocab, 32)
+            x = x.detach().requires_grad_()
+            r = token_log_probs(x, t, entropy=True, top=top)
+            lp = torch.log_softmax(x.detach().double(), -1)
+            assert torch.equal(r.top_tokens, torch.sort(x.detach().float(), descending=True, stable=True).indices[:, :top])
+            assert bool(((r.log_probs.double() - lp.gather(1, t[:, None])[:, 0]).abs() <= 2.0 ** -18).all())
+            assert bool(((r.top_log_probs.double() - lp.gather(1, r.top_tokens)).abs() <= 2.0 ** -18).all())
+            (g,) = torch.autograd.grad(r.log_probs, x, torch.ones(9, device=DEV))
+            want = -lp.exp()
+            want[torch.arange(9, device=DEV), t] += 1
+            # (the token's entry is 1 - p from parts good to 2^-20)
+            assert bool(((g.double() - want).abs() <= 2.0 ** -18 + torch.finfo(x.dtype).eps / 2 * want.abs()).all())
