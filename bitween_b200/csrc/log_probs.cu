@@ -25,7 +25,7 @@ namespace cg = cooperative_groups;
 constexpr int THREADS = 256, UNROLL = 4, BLOCKS = 16;     // of a CTA; 16-byte loads of a step; blocks of steps of a thread
 constexpr int STEP = THREADS * UNROLL;                     // 16-byte pieces of a CTA's step
 constexpr int CANDIDATES = 512;
-constexpr int MOST_CTAS = 4 * 148;                         // four an SM
+constexpr int SMS = 148;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // The order of the alternatives: falling value, rising index; NaN before all.  Larger is better; nothing is 0.
@@ -588,13 +588,14 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogPro
     }
 }
 
-// CTAs of a row, of at least a step (16 KB) each, rows of more than two steps: so many that all rows together have two an SM; of rows of more than 384 KB four.  bf16 with entropy and five
-// alternatives, 1 / 2 / 4 / 8 CTAs: 32 x 50272 7.8 / 7.7 / 7.0 / 7.1 us, 64 x 50272 7.8 / 7.7 / 7.6 / 9.4, 128 x 50272 9.7 / 9.7 / 11.1 / 16.9, 256 x 50272 11.7 / 14.6 / 20.2 / 31.6, 64 x 16000 5.2 / 6.0 / 6.7 / 8.9, 64 x 131072 16.4 /
-// 12.0 / 10.1 / 11.2; fp32, 80 x 131072 27.7 / 18.8 / 16.3 / 20.7, without alternatives 23.8 / 14.6 / 11.0 / 10.1.
+// CTAs of a row, of at least a step (16 KB) each, rows of more than two steps: so many that all rows together have one an SM; the first division where two an SM have more than 64 KB each; rows of more
+// than 384 KB until there are four.  us a call among others / alone (with the wait for the GPU), entropy and twenty alternatives, 1, 2, 4, 8 CTAs: 16 x 50272 bf16 8.5/20.1, 8.2/19.7, 7.0/18.6, 6.9/18.5;
+// 61 x 50272 8.5/20.2, 8.2/19.8, 9.3/19.6, 9.1/20.7; 61 x 131071 13.3/24.7, 10.5/22.1, 12.0/21.4, 11.2/23.0; 128 x 131072 17.3/28.8, 14.5/26.0, 15.4/26.7, 21.3/32.4; 128 x 32000 6.9/18.8, 9.5/19.7, 9.4/21.2,
+// 16.9/28.3; 61 x 131071 fp32 28.0/39.6, 17.6/29.3, 12.8/24.2, 12.4/24.3.
 int ctas_of(int64_t rows, int64_t vocab, size_t size) {
-    const int64_t bytes = vocab * (int64_t)size, most = bytes > 384 << 10 ? MOST_CTAS : MOST_CTAS / 2;
+    const int64_t bytes = vocab * (int64_t)size;
     int n = 1;
-    while (n < 8 && rows * n * 2 <= most && bytes > (int64_t)n * STEP * 16 && bytes > 2 * STEP * 16) n *= 2;
+    while (n < 8 && rows * n * 2 <= (bytes > 384 << 10 ? 4 * SMS : n == 1 && bytes > 128 << 10 ? 2 * SMS : SMS) && bytes > (int64_t)n * STEP * 16 && bytes > 2 * STEP * 16) n *= 2;
     return n;
 }
 
@@ -613,7 +614,7 @@ int log_probs_typed(LogProbs &p, cudaStream_t st) {
 // (8192 x 131072 bf16: 657 us with one, 650 two, 640 four, 669 eight; 2048 x 32000 46, 48, 58, 91; 61 x 131071 15.6, 10.5, 8.5, 8.9.)
 int parts_of(int64_t rows, int64_t vocab, size_t size) {
     int n = 1;
-    while (n < 8 && ((rows * n < 2 * MOST_CTAS && vocab * (int64_t)size > (int64_t)n * STEP * 16) || vocab * (int64_t)size > (int64_t)n << 16)) n *= 2;
+    while (n < 8 && ((rows * n < 8 * SMS && vocab * (int64_t)size > (int64_t)n * STEP * 16) || vocab * (int64_t)size > (int64_t)n << 16)) n *= 2;
     return n;
 }
 
