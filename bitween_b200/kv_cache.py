@@ -3,6 +3,7 @@ rounding of quantize_rtn.  No counterpart in the reference; computed by the sm_1
 bw_kv_attend (include/bitween_b200.h has the format)."""
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -207,9 +208,12 @@ class QuantizedKVCache:
         return out
 
     def _attend_window(self, q, page_table, lengths, softmax_scale, window, sinks):
-        if not isinstance(window, int) or not isinstance(sinks, int) or window < 0 or sinks < 0:
+        try:
+            window, sinks = min(operator.index(window), 2 ** 31), min(operator.index(sinks), 2 ** 31)
+        except TypeError:
+            window = -1
+        if window < 0 or sinks < 0:
             raise ValueError("window and sinks must be numbers of tokens, 0 or more")
-        window, sinks = min(int(window), 2 ** 31), min(int(sinks), 2 ** 31)
         out = (_lib._operators or _lib.host_operators()).kv_attend(*self._cache, q, page_table, lengths, softmax_scale, window, sinks)
         if out is not None:
             return out

@@ -1,6 +1,7 @@
 """Log probabilities of given tokens, with the entropy and the likeliest alternatives, and their gradient: what evaluation of a quantised model,
 serving and fine-tuning of adapters ask of its logits.  Computed by the sm_100a kernels behind bw_token_log_probs and
 bw_token_log_probs_grad."""
+import operator
 from collections import namedtuple
 
 import torch
@@ -99,7 +100,8 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0):
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError("logits must be [..., vocab] of at least one token")
     lead, vocab = logits.shape[:-1], logits.shape[-1]
-    if not isinstance(top, int) or not 0 <= top <= min(32, vocab):
+    top = operator.index(top)
+    if not 0 <= top <= min(32, vocab):
         raise ValueError(f"top must be 0 to {min(32, vocab)}")
     if tokens is not None:
         if tokens.dtype != torch.int64:

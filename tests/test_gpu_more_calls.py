@@ -214,3 +214,19 @@ def test_one_value_and_few():
             want[torch.arange(9, device=DEV), t] += 1
             # (the token's entry is 1 - p from parts good to 2^-20)
             assert bool(((g.double() - want).abs() <= 2.0 ** -18 + torch.finfo(x.dtype).eps / 2 * want.abs()).all())
+
+
+def test_numbers_of_other_types():
+    np = pytest.importorskip("numpy")
+    cache = QuantizedKVCache(4, 16, 2, 64, bits=4, device=DEV)
+    x = torch.randn(3, 2, 64, generator=_gen(15), device=DEV).half()
+    cache.append(x, x, torch.arange(3, device=DEV))
+    table, n = torch.zeros(3, 1, dtype=torch.int32, device=DEV), torch.full((3,), 3, dtype=torch.int32, device=DEV)
+    want = cache.attend(x, table, n, window=2, sinks=1)
+    assert torch.equal(cache.attend(x, table, n, window=np.int64(2), sinks=np.int32(1)), want)
+    assert torch.equal(cache.attend(x, table, n, window=2, sinks=True), want)
+    logits = torch.randn(3, 50, generator=_gen(16), device=DEV)
+    a, b = token_log_probs(logits, entropy=np.bool_(True), top=np.int64(4)), token_log_probs(logits, entropy=True, top=4)
+    assert torch.equal(a.entropy, b.entropy) and torch.equal(a.top_tokens, b.top_tokens)
+    with pytest.raises(TypeError):
+        token_log_probs(logits, top=1.5)
