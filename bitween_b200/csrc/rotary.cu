@@ -70,19 +70,45 @@ __global__ void __launch_bounds__(THREADS) rotate_kernel(const RotateRows p, con
     rotate_rows<T>(p, r, blockIdx.x * THREADS + threadIdx.x);
 }
 
-// Any size and stride: a warp a row.  (16384 tokens of 40 heads of 128: 750 us.)
+// Any size and stride: a warp the heads of a token slots apart from `slot`, a lane every 32nd pair, whose cosine and sine it keeps for all of them.  (The 16384 tokens from
+// above off a 16-byte boundary 114 us, with 20 pairs of a head 156; a row a warp and each value by itself 750.)
+template <typename T>
+__device__ __forceinline__ void rotate_any(const RotateRows &p, const Rotary &r, int64_t token, int slot) {
+    const int lane = threadIdx.x % 32, heads = p.heads[0] + p.heads[1];
+    auto rows = [&](int h, const T *&x, T *&out) {
+        if (h < p.heads[0]) {
+            x = (const T *)p.x[0] + token * p.stride[0] + h * p.head_stride[0];
+            out = (T *)p.out[0] + (token * p.heads[0] + h) * p.dim;
+        } else {
+            x = (const T *)p.x[1] + token * p.stride[1] + (h - p.heads[0]) * p.head_stride[1];
+            out = (T *)p.out[1] + (token * p.heads[1] + h - p.heads[0]) * p.dim;
+        }
+    };
+    for (int pair = lane; pair < r.pairs; pair += 32) {
+        const int first = r.interleaved ? 2 * pair : pair, second = r.interleaved ? first + 1 : pair + r.pairs;
+        const float2 t = turn_of(r, token, pair);
+        for (int h = slot; h < heads; h += p.slots) {
+            const T *x;
+            T *out;
+            rows(h, x, out);
+            const float u = to_f32(x[first]), v = to_f32(x[second]);
+            out[first] = from_f32<T>(turned_first(u, v, t));
+            out[second] = from_f32<T>(turned_second(u, v, t));
+        }
+    }
+    for (int d = 2 * r.pairs + lane; d < p.dim; d += 32)
+        for (int h = slot; h < heads; h += p.slots) {
+            const T *x;
+            T *out;
+            rows(h, x, out);
+            out[d] = x[d];
+        }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) rotate_general_kernel(const RotateRows p, const Rotary r) {
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int all = p.heads[0] + p.heads[1];
-    const int64_t row = (int64_t)blockIdx.x * 8 + warp, token = row / all;
-    if (token >= p.tokens) return;
-    int h = (int)(row - token * all);
-    const int i = h >= p.heads[0];
-    if (i) h -= p.heads[0];
-    const T *x = (const T *)p.x[i] + token * p.stride[i] + h * p.head_stride[i];
-    T *out = (T *)p.out[i] + (token * p.heads[i] + h) * p.dim;
-    for (int d = lane; d < p.dim; d += 32) out[d] = from_f32<T>(turned_value(r, x, token, d));
+    const int64_t i = (int64_t)blockIdx.x * 8 + threadIdx.x / 32, token = i / p.slots;
+    if (token < p.tokens) rotate_any<T>(p, r, token, (int)(i - token * p.slots));
 }
 
 struct AppendRotated {
@@ -192,20 +218,17 @@ __global__ void __launch_bounds__(THREADS) kv_append_rotated_kernel(const Append
     }
 }
 
-// Any size and stride: a warp a row of q, k or v.
+// Any size and stride: a warp a row of k or v, or the heads of q that are slots apart (316 to 330 us).
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256) kv_append_rotated_general_kernel(const AppendRotated p, const Rotary r) {
     constexpr float Q = (1 << BITS) - 1, RQ = 1.0f / Q;
     __shared__ uint8_t s_codes[8][256];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, kv = p.rows.heads, all = p.q.heads[0] + 2 * kv;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, kv = p.rows.heads, all = p.q.slots + 2 * kv;
     const int64_t row = (int64_t)blockIdx.x * 8 + warp, token = row / all;
     if (token >= p.rows.tokens) return;
     int h = (int)(row - token * all);
     if (h >= 2 * kv) {
-        h -= 2 * kv;
-        const T *x = (const T *)p.q.x[0] + token * p.q.stride[0] + h * p.q.head_stride[0];
-        T *out = (T *)p.q.out[0] + (token * p.q.heads[0] + h) * p.q.dim;
-        for (int d = lane; d < p.q.dim; d += 32) out[d] = from_f32<T>(turned_value(r, x, token, d));
+        rotate_any<T>(p.q, r, token, h - 2 * kv);
         return;
     }
     const int j = h >= kv;
@@ -273,6 +296,12 @@ int slots_of(int64_t tokens, int dim, int heads) {
     while (each > 1 && tokens * (dim / 16) * ((heads + each - 1) / each) < 148 * 1024) each /= 2;
     return (heads + each - 1) / each;
 }
+// Warps of a token on the general kernel: eight heads a warp where that leaves 32 warps an SM, else four, two or one.
+int warps_of(int64_t tokens, int heads) {
+    int each = 8;
+    while (each > 1 && tokens * ((heads + each - 1) / each) < 148 * 32) each /= 2;
+    return (heads + each - 1) / each;
+}
 // The threads of a call's rows; 0 where the general kernel takes them.
 int64_t fast_rows(RotateRows &p, const Rotary &r, size_t size) {
     const int heads = p.heads[0] + p.heads[1];
@@ -290,8 +319,8 @@ template <typename T>
 int rotate_typed(RotateRows &p, const Rotary &r, cudaStream_t st) {
     if (const int64_t threads = fast_rows(p, r, sizeof(T)))
         return launch_early("rotate_kernel", rotate_kernel<T>, dim3((unsigned)((threads + THREADS - 1) / THREADS)), THREADS, 0, st, dim3(1), p, r);
-    const int64_t rows = p.tokens * (p.heads[0] + p.heads[1]);
-    rotate_general_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, r);
+    p.slots = warps_of(p.tokens, p.heads[0] + p.heads[1]);
+    rotate_general_kernel<T><<<(unsigned)((p.tokens * p.slots + 7) / 8), 256, 0, st>>>(p, r);
     return check_launch("rotate_general_kernel");
 }
 
@@ -308,7 +337,8 @@ int append_rotated_typed(AppendRotated &p, const Rotary &r, cudaStream_t st) {
         p.by_kv_slots = divisor((uint32_t)p.kv_slots);
         return launch_early("kv_append_rotated_kernel", kv_append_rotated_kernel<T, BITS>, dim3((unsigned)ctas), THREADS, 0, st, dim3(1), p, r);
     }
-    const int64_t rows = p.rows.tokens * (p.q.heads[0] + 2 * p.rows.heads);
+    p.q.slots = p.q.heads[0] ? warps_of(k.tokens, p.q.heads[0]) : 0;
+    const int64_t rows = k.tokens * (p.q.slots + 2 * k.heads);
     kv_append_rotated_general_kernel<T, BITS><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p, r);
     return check_launch("kv_append_rotated_general_kernel");
 }
