@@ -22,7 +22,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int THREADS = 256, UNROLL = 4, BLOCKS = 16;     // of a CTA; 16-byte loads of a step; blocks of steps of a thread
+constexpr int THREADS = 256, UNROLL = 4, BLOCKS = 16;     // of a CTA (of short rows fewer, N below); 16-byte loads of a step; blocks of steps of a thread
 constexpr int STEP = THREADS * UNROLL;                     // 16-byte pieces of a CTA's step
 constexpr int CANDIDATES = 512;
 constexpr int SMS = 148;
@@ -151,27 +151,28 @@ template <typename T> struct Row {
 // reaches it.  Only blocks that reach it are read again, some more than `top` of them in all CTAs together, and the values that reach it are ranked.  Where too many do (many equal
 // values, as masks leave them; many large ones in few threads' places) a CTA finds the `top` best of its share digit by digit instead.
 constexpr int GROUPS = 64;
-struct __align__(16) TopScratch {
-    float largest[BLOCKS][THREADS];                    // of a thread's blocks
+template <int N> struct __align__(16) TopScratch {
+    float largest[BLOCKS][N];                    // of a thread's blocks
     __align__(16) uint32_t group[GROUPS];              // the groups' largest values, of all CTAs
     __align__(16) uint64_t list[CANDIDATES + 2];       // this CTA's candidates: (order << 32) | ~index
-    __align__(16) uint64_t all[CANDIDATES + 2];        // all CTAs' (rank 0)
+    __align__(16) uint64_t all[N == THREADS ? CANDIDATES : 2];      // all CTAs' (rank 0)
     uint64_t best[32];
-    uint32_t histogram[THREADS], entry[THREADS];
+    uint32_t histogram[256], entry[N];
     int count, entries, need, counts[8];
-    uint32_t least[THREADS / 32], prefix;
-    int scan[THREADS / 32];
+    uint32_t least[N / 32], prefix;
+    int scan[N / 32];
 };
 
 __device__ __forceinline__ uint64_t candidate(float x, int at) { return (uint64_t)order_of(x) << 32 | (uint32_t)~at; }
 
 // The best `top` of n candidates, in order, into `best`; 0 where there are fewer.  All candidates differ.
+template <int N>
 __device__ __forceinline__ void rank_candidates(uint64_t *list, int n, int top, uint64_t *best) {
     const int tid = threadIdx.x;
     if (tid < top) best[tid] = 0;
     if (tid < 2) list[n + tid] = 0;
     __syncthreads();
-    for (int i = tid; i < n; i += THREADS) {
+    for (int i = tid; i < n; i += N) {
         const uint64_t mine = list[i];
         int before = 0;
 #pragma unroll 4
@@ -185,8 +186,8 @@ __device__ __forceinline__ void rank_candidates(uint64_t *list, int n, int top, 
 }
 
 // The best `top` values of a rank's share, as candidates into s.list: the top-th largest value is found eight bits at a time.
-template <typename T>
-__device__ __noinline__ void search_share(TopScratch &s, const Row<T> &row, int top) {
+template <typename T, int N>
+__device__ __noinline__ void search_share(TopScratch<N> &s, const Row<T> &row, int top) {
     constexpr int V = Piece<T>::V;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     __syncthreads();
@@ -196,14 +197,14 @@ __device__ __noinline__ void search_share(TopScratch &s, const Row<T> &row, int 
         s.count = 0;
     }
     for (int shift = 24; shift >= 0; shift -= 8) {
-        s.histogram[tid] = 0;
+        for (int i = tid; i < 256; i += N) s.histogram[i] = 0;
         __syncthreads();
         const uint32_t prefix = s.prefix;
         auto count = [&](float x) {
             const uint32_t o = order_of(x);
             if (shift == 24 || o >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&s.histogram[o >> shift & 255], 1u);
         };
-        for (int v = row.v0 + tid; v < row.v1; v += THREADS) {
+        for (int v = row.v0 + tid; v < row.v1; v += N) {
             Piece<T> x;
             x.load(row.piece(v));
 #pragma unroll
@@ -246,7 +247,7 @@ __device__ __noinline__ void search_share(TopScratch &s, const Row<T> &row, int 
         if (lane == 31) s.scan[warp] = sum;
         __syncthreads();
         int before = taken + sum - equal, all = 0;
-        for (int i = 0; i < THREADS / 32; ++i) {
+        for (int i = 0; i < N / 32; ++i) {
             before += i < warp ? s.scan[i] : 0;
             all += s.scan[i];
         }
@@ -262,7 +263,7 @@ __device__ __noinline__ void search_share(TopScratch &s, const Row<T> &row, int 
     const int head = row.extra ? row.head : 0;
     x[0] = tid < head ? ld_l2(row.x + tid) : 0.0f;
     round(x, tid < head, tid);
-    for (int v0 = row.v0; v0 < row.v1; v0 += THREADS) {
+    for (int v0 = row.v0; v0 < row.v1; v0 += N) {
         Piece<T> piece;
         if (v0 + tid < row.v1) piece.load(row.piece(v0 + tid));
         else piece.nothing();
@@ -281,28 +282,29 @@ __device__ __noinline__ void search_share(TopScratch &s, const Row<T> &row, int 
 
 // This CTA's candidates into s.list, s.count of them (at most `room`, which is `top` or more).  s.group holds the groups' largest values; `key` is this thread's largest
 // value; those of its blocks of `per` steps lie in s.largest; `extra` is its value before or behind the pieces.
-template <typename T>
-__device__ __forceinline__ void find_candidates(TopScratch &s, const Row<T> &row, int top, int room, int blocks, int per, uint32_t key, float extra) {
+template <typename T, int N>
+__device__ __forceinline__ void find_candidates(TopScratch<N> &s, const Row<T> &row, int top, int room, int blocks, int per, uint32_t key, float extra) {
     constexpr int V = Piece<T>::V, BLOCK = UNROLL * V;      // values of a thread's step: 16 or 32
     static_assert(BLOCK <= 32, "a lane a value");
     const int tid = threadIdx.x, lane = tid % 32;
-    static_assert(THREADS == 4 * GROUPS, "four threads a group");
-    const uint32_t mine = s.group[tid / 4];
+    constexpr int EACH = N / GROUPS;         // threads that compare one group's value with the others'
+    static_assert(EACH == 1 || EACH == 2 || EACH == 4, "one, two or four threads a group");
+    const uint32_t mine = s.group[tid / EACH];
     int larger = 0;
 #pragma unroll
-    for (int i = 0; i < GROUPS / 4; i += 4) {
-        const uint4 k = *reinterpret_cast<const uint4 *>(s.group + tid % 4 * (GROUPS / 4) + i);
+    for (int i = 0; i < GROUPS / EACH; i += 4) {
+        const uint4 k = *reinterpret_cast<const uint4 *>(s.group + tid % EACH * (GROUPS / EACH) + i);
         larger += (k.x > mine) + (k.y > mine) + (k.z > mine) + (k.w > mine);
     }
-    larger += __shfl_xor_sync(0xffffffffu, larger, 1);
-    larger += __shfl_xor_sync(0xffffffffu, larger, 2);
+#pragma unroll
+    for (int d = 1; d < EACH; d *= 2) larger += __shfl_xor_sync(0xffffffffu, larger, d);
     const uint32_t low = __reduce_min_sync(0xffffffffu, larger < top ? mine : 0xffffffffu);
     if (lane == 0) s.least[tid / 32] = low;
     if (tid == 0) s.count = s.entries = 0;
     __syncthreads();
     uint32_t least = s.least[0];
 #pragma unroll
-    for (int i = 1; i < THREADS / 32; ++i) least = min(least, s.least[i]);
+    for (int i = 1; i < N / 32; ++i) least = min(least, s.least[i]);
     auto offer = [&](float x, int at) {
         if (order_of(x) < least) return;
         const int i = atomicAdd(&s.count, 1);
@@ -317,21 +319,21 @@ __device__ __forceinline__ void find_candidates(TopScratch &s, const Row<T> &row
         if (hits) {
             int at = atomicAdd(&s.entries, __popc(hits));
             for (; hits; hits &= hits - 1, ++at)
-                if (at < THREADS) s.entry[at] = (__ffs(hits) - 1) * THREADS + tid;
+                if (at < N) s.entry[at] = (__ffs(hits) - 1) * N + tid;
         }
     }
     __syncthreads();
     const int entries = s.entries;
-    if (entries <= THREADS) {
+    if (entries <= N) {
         // a warp a block, four of them in flight
         for (int step = 0; step < per; ++step)
-            for (int i0 = tid / 32; i0 < entries; i0 += 4 * (THREADS / 32)) {
+            for (int i0 = tid / 32; i0 < entries; i0 += 4 * (N / 32)) {
                 float x[4];
                 int at[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int i = i0 + k * (THREADS / 32), entry = i < entries ? (int)s.entry[i] : 0;
-                    const int v = row.v0 + (entry / THREADS * per + step) * STEP + lane / V * THREADS + entry % THREADS;
+                    const int i = i0 + k * (N / 32), entry = i < entries ? (int)s.entry[i] : 0;
+                    const int v = row.v0 + (entry / N * per + step) * (N * UNROLL) + lane / V * N + entry % N;
                     at[k] = i < entries && lane < BLOCK && v < row.v1 ? row.head + v * V + lane % V : -1;
                     if (at[k] >= 0) x[k] = ld_l2(row.x + at[k]);
                 }
@@ -359,15 +361,15 @@ __device__ __forceinline__ Sums joined(Sums a, int lanes) {
     return a;
 }
 
-// A row a cluster.
-template <typename T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const LogProbs p) {
-    constexpr int V = Piece<T>::V, WARPS = THREADS / 32;
+// A row a cluster, of CTAs of N threads.
+template <typename T, int N, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(N, (TOP ? 4 : 5) * THREADS / N) log_probs_kernel(const LogProbs p) {
+    constexpr int V = Piece<T>::V, WARPS = N / 32, STEP = N * UNROLL;
     const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
     const int rank = (int)(blockIdx.x % p.cluster);
     const int64_t r = blockIdx.x / p.cluster;
     __shared__ Sums s_warp[WARPS], s_all[8];
-    __shared__ typename std::conditional<TOP, TopScratch, int>::type s_top;
+    __shared__ typename std::conditional<TOP, TopScratch<N>, int>::type s_top;
     const cg::cluster_group cluster = cg::this_cluster();
     if (p.cluster > 1) cluster_arrive();                   // (all CTAs have begun before one writes into another's memory)
     pdl_wait();
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
     auto load = [&](int step) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int v = row.v0 + step * STEP + u * THREADS + tid;
+            const int v = row.v0 + step * STEP + u * N + tid;
             if (v < row.v1) next[u].load(row.piece(v));
             else next[u].nothing();
         }
@@ -393,6 +395,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
     uint32_t key = 0;
     float block = -INFINITY;
     int in_block = 0, blocks = 0;
+    bool any = false;                                    // whether the block has a piece: a thread's last one may have none
     for (int step = 0; step < steps; ++step) {
         Piece<T> x[UNROLL];
 #pragma unroll
@@ -402,11 +405,15 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
         if (m > a.m) a.raise(m);
         if constexpr (TOP) {
             block = max_nan(block, m);
+            any |= row.v0 + step * STEP + tid < row.v1;
             if (++in_block == per || step + 1 == steps) {
-                s_top.largest[blocks++][tid] = block;
-                key = max(key, order_of(block));
+                if (any) {
+                    s_top.largest[blocks++][tid] = block;
+                    key = max(key, order_of(block));
+                }
                 block = -INFINITY;
                 in_block = 0;
+                any = false;
             }
         }
         const float by = a.m == -INFINITY ? 0.0f : -a.m;
@@ -433,7 +440,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
     }
     const int room = CANDIDATES / p.cluster;
     if constexpr (TOP) {
-        const int size = THREADS * p.cluster / GROUPS;       // threads of a group, 4 to 32
+        const int size = N * p.cluster / GROUPS;             // threads of a group, 2 to 32
         uint32_t k = key;
         for (int d = 1; d < size; d *= 2) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
         if (p.cluster > 1) cluster_wait();
@@ -457,9 +464,9 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
         const int n = s_top.count;
         if (p.cluster > 1) {
             uint64_t *to = cluster.map_shared_rank(s_top.all, 0) + rank * room;
-            for (int i = tid; i < n; i += THREADS) to[i] = s_top.list[i];
+            for (int i = tid; i < n; i += N) to[i] = s_top.list[i];
             if (tid == 0) *cluster.map_shared_rank(s_top.counts + rank, 0) = n;
-        } else rank_candidates(s_top.list, n, p.top, s_top.best);
+        } else rank_candidates<N>(s_top.list, n, p.top, s_top.best);
     }
     if (p.cluster > 1) {
         cluster_arrive();
@@ -467,7 +474,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
         cluster_wait();
         if constexpr (TOP) {
             // (s_top.list, whose candidates are rank 0's part of `all`, takes them all, a warp those of one rank)
-            static_assert(WARPS == 8, "a warp a rank");
+            // (clusters are of CTAs of eight warps)
             const int mine = lane < p.cluster ? s_top.counts[lane] : 0;
             int sum = mine;
             for (int d = 1; d < 8; d *= 2) {
@@ -477,7 +484,7 @@ __global__ void __launch_bounds__(THREADS, TOP ? 4 : 5) log_probs_kernel(const L
             const int n = __shfl_sync(0xffffffffu, sum, 7), from = __shfl_sync(0xffffffffu, sum - mine, warp), here = __shfl_sync(0xffffffffu, mine, warp);
             for (int k = lane; k < here; k += 32) s_top.list[from + k] = s_top.all[warp * room + k];
             __syncthreads();
-            rank_candidates(s_top.list, n, p.top, s_top.best);
+            rank_candidates<N>(s_top.list, n, p.top, s_top.best);
         }
         a = joined(s_all[lane % p.cluster], p.cluster);
     }
@@ -599,9 +606,23 @@ int ctas_of(int64_t rows, int64_t vocab, size_t size) {
     return n;
 }
 
+// Threads of a CTA.  A row's end (its sums, its alternatives) costs a CTA as much whatever its threads are: short rows, and long ones with alternatives where there are many, take fewer.  bf16 with entropy,
+// 64 / 128 / 256 threads, without alternatives: 8000 x 1000 10.7 / 18.9 / 35.8 us, 8000 x 8000 26.5 / 29.6 / 39.8, 8000 x 16000 46.4 / 48.4 / 56.9, 2000 x 32000 33.2 / 28.8 / 27.2; with five: 20 x 4000 5.1 / 4.6 / 4.8, 8000 x 1000
+// 27.6 / 46.1 / 75.8, 300 x 8000 6.4 / 5.7 / 7.6, 2000 x 8000 14.1 / 16.3 / 22.5, 600 x 32000 15.9 / 17.6 / 15.5, 2000 x 32000 36.9 / 34.7 / 39.5, 2000 x 131071 126 / 103 / 105.
+int threads_of(int64_t rows, int64_t vocab, size_t size, int cluster, bool top) {
+    const int64_t bytes = vocab * (int64_t)size;
+    if (cluster > 1) return THREADS;
+    // (of 1 KB: fewer pieces than groups of two threads)
+    if (bytes < 1 << 10 || (bytes <= 8 << 10 && rows >= SMS) || (bytes <= 16 << 10 && rows >= 2000)) return 64;
+    return bytes <= 32 << 10 || (top && bytes <= 256 << 10 && rows >= 8 * SMS) ? 128 : THREADS;
+}
+
 template <typename T, bool ENTROPY, bool TOP>
 int log_probs_launch(const LogProbs &p, cudaStream_t st) {
-    return launch_early("log_probs_kernel", log_probs_kernel<T, ENTROPY, TOP>, dim3((unsigned)(p.rows * p.cluster)), THREADS, 0, st, dim3(p.cluster), p);
+    const int n = threads_of(p.rows, p.vocab, sizeof(T), p.cluster, TOP);
+    if (n == 64) return launch_early("log_probs_kernel", log_probs_kernel<T, 64, ENTROPY, TOP>, dim3((unsigned)p.rows), 64, 0, st, dim3(1), p);
+    if (n == 128) return launch_early("log_probs_kernel", log_probs_kernel<T, 128, ENTROPY, TOP>, dim3((unsigned)p.rows), 128, 0, st, dim3(1), p);
+    return launch_early("log_probs_kernel", log_probs_kernel<T, THREADS, ENTROPY, TOP>, dim3((unsigned)(p.rows * p.cluster)), THREADS, 0, st, dim3(p.cluster), p);
 }
 template <typename T>
 int log_probs_typed(LogProbs &p, cudaStream_t st) {

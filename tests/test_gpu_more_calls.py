@@ -230,3 +230,35 @@ def test_numbers_of_other_types():
     assert torch.equal(a.entropy, b.entropy) and torch.equal(a.top_tokens, b.top_tokens)
     with pytest.raises(TypeError):
         token_log_probs(logits, top=1.5)
+
+
+@pytest.mark.parametrize("rows,vocab", [(160, 300), (160, 4000), (2100, 7000), (30, 500), (30, 8000), (200, 15000), (1300, 20000), (1300, 40), (2100, 2000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_many_short_rows_with_masks(rows, vocab, dtype):
+    """Rows that take CTAs of fewer threads, half of them masked (so that alternatives tie), some of one value, with gradients."""
+    x = (2.5 * torch.randn(rows, vocab, generator=_gen(20), device=DEV)).to(dtype)
+    x[::2, vocab // 7:] = -math.inf
+    x[1::7] = 0.5
+    x[2::9, vocab // 2:] = torch.finfo(dtype).min
+    x[5] = -math.inf
+    x[6, vocab // 3] = math.nan
+    t = torch.randint(-1, max(1, vocab // 7), (rows,), generator=_gen(21), device=DEV)
+    top = min(vocab, 32)
+    x.requires_grad_()
+    r = token_log_probs(x, t, entropy=True, top=top)
+    d = x.detach().double()
+    lp = torch.log_softmax(d, -1)
+    assert torch.equal(r.top_tokens, torch.sort(x.detach().float(), descending=True, stable=True).indices[:, :top])
+    want = torch.where(t < 0, 0.0, lp.gather(1, t.clamp(min=0)[:, None])[:, 0])
+    h = torch.special.entr(lp.exp()).sum(-1)
+    for got, ref, slack in ((r.log_probs, want, 2.0 ** -17), (r.entropy, h, 2.0 ** -16), (r.top_log_probs, lp.gather(1, r.top_tokens), 2.0 ** -17)):
+        # (spans of 25: exponents good to 2^-20, sums to 2^-19; values of the type's lowest have their own rounding)
+        ok = ref.isfinite()
+        skip = (t < 0) & ~ok if ref.dim() == 1 and got is r.log_probs else torch.zeros_like(ok)
+        assert torch.equal(got.double()[~ok & ~skip].nan_to_num(nan=7.0), ref[~ok & ~skip].nan_to_num(nan=7.0))
+        assert bool(((got.double() - ref)[ok].abs() <= slack + 2.0 ** -23 * ref[ok].abs()).all())
+    (g,) = torch.autograd.grad(r.log_probs, x, torch.ones(rows, device=DEV))
+    fine = lp.exp().isfinite().all(-1) & (t >= 0)
+    ref = -lp.exp()
+    ref[torch.arange(rows, device=DEV), t.clamp(min=0)] += 1
+    assert bool(((g.double() - ref)[fine].abs() <= 2.0 ** -17 + torch.finfo(dtype).eps / 2 * ref[fine].abs()).all()) and not bool(g[t < 0].any())
