@@ -7,8 +7,8 @@
 // One pass over the row with the running maximum; x - m is formed before the product, so that masks of the type's lowest value stay finite or become
 // exact zeros.  Sums are fp32: 32 terms (16 of fp32 logits) by themselves, then those sums, then a tree: a chain of 500 equal terms rounds the same way each time and was
 // off by 7e-6.  Bound by the bytes of the logits where there are many rows, by latency where there are few (bf16, with entropy): 8192 x 131072 333 us, 6.4 TB/s (the measured copy
-// rate is 6.5), their gradient 640 us, 6.7 TB/s; 61 x 131071 7.7 us; one row of 50272 2.9 us.  Twenty alternatives add 20 us to 2000 x 131071 (88.8), 15 to 2000 x 32000 (27.7), 4 to 61 x 131071
-// and 3 to one row: six barriers' worth of latency behind each row, of which four CTAs an SM hide a part.
+// rate is 6.5), their gradient 640 us, 6.7 TB/s; 61 x 131071 7.0 us; one row of 50272 2.9 us.  Twenty alternatives add 19 us to 2000 x 131071 (88.8), 10 to 2000 x 32000 (27.7), 3 to 61 x 131071
+// and to one row: six barriers' worth of latency behind each row, of which an SM's other CTAs hide a part.
 //
 // A row is taken by a cluster of one to eight CTAs, which join through distributed shared memory.
 #include <cooperative_groups.h>
@@ -515,9 +515,9 @@ struct LogProbsGrad {
 
 // Bound by the bytes of the logits and of their gradient.  ALIGNED: pieces of a row start where those of its gradient do.  The entries of the tokens are written again
 // behind a barrier, by themselves: no comparison in the loop.
-template <typename T, bool ENTROPY, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogProbsGrad p) {
-    constexpr int V = Piece<T>::V;
+template <typename T, int N, bool ENTROPY, bool ALIGNED>
+__global__ void __launch_bounds__(N, 4 * THREADS / N) log_probs_grad_kernel(const LogProbsGrad p) {
+    constexpr int V = Piece<T>::V, STEP = N * UNROLL;
     const int tid = threadIdx.x, part = (int)(blockIdx.x % p.parts);
     const int64_t r = blockIdx.x / p.parts;
     pdl_wait();
@@ -543,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogPro
     };
     const Row<T> row(ALIGNED ? x : (const T *)out, p.vocab, part, p.parts);      // (of the gradient's boundaries where they differ)
     if (!any) {                          // a row that nothing is asked of (padding): zeros, whatever stands in it
-        for (int v = row.v0 + tid; v < row.v1; v += THREADS) *reinterpret_cast<uint4 *>(out + row.head + (int64_t)v * V) = make_uint4(0, 0, 0, 0);
+        for (int v = row.v0 + tid; v < row.v1; v += N) *reinterpret_cast<uint4 *>(out + row.head + (int64_t)v * V) = make_uint4(0, 0, 0, 0);
         if (tid < row.extra) out[row.extra_at(tid)] = from_f32<T>(0.0f);
         return;
     }
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogPro
     auto load = [&](int step) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int v = row.v0 + step * STEP + u * THREADS + tid;
+            const int v = row.v0 + step * STEP + u * N + tid;
             if (v >= row.v1) continue;
             if constexpr (ALIGNED) next[u].load(row.piece(v));
             else
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(THREADS, 4) log_probs_grad_kernel(const LogPro
         if (step + 1 < steps) load(step + 1);
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int v = row.v0 + step * STEP + u * THREADS + tid;
+            const int v = row.v0 + step * STEP + u * N + tid;
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) {
                 const float2 d = ffma2(fadd2(y[u].pair(i), make_float2(-st.x, -st.x)), make_float2(LOG2E, LOG2E), make_float2(-st.y, -st.y));
@@ -639,9 +639,19 @@ int parts_of(int64_t rows, int64_t vocab, size_t size) {
     return n;
 }
 
+// Threads of a CTA of the gradient: fewer for many short rows.  (bf16 with an entropy's gradient, 64 / 128 / 256: 8000 x 1000 11.4 / 18.2 / 34.4 us, 8000 x 8000 45.0 / 46.7 / 60.4, 8000 x 16000 84.8 / 82.7 / 90.8, 2000 x 32000
+// 50.1 / 46.5 / 45.5.)
+int grad_threads_of(int64_t rows, int64_t vocab, size_t size) {
+    const int64_t bytes = vocab * (int64_t)size;
+    return rows < SMS || bytes > 32 << 10 ? THREADS : bytes <= 16 << 10 ? 64 : 128;
+}
+
 template <typename T, bool ENTROPY, bool ALIGNED>
 int log_probs_grad_launch(const LogProbsGrad &p, int64_t rows, cudaStream_t st) {
-    return launch_early("log_probs_grad_kernel", log_probs_grad_kernel<T, ENTROPY, ALIGNED>, dim3((unsigned)(rows * p.parts)), THREADS, 0, st, dim3(1), p);
+    const int n = grad_threads_of(rows, p.vocab, sizeof(T));
+    if (n == 64) return launch_early("log_probs_grad_kernel", log_probs_grad_kernel<T, 64, ENTROPY, ALIGNED>, dim3((unsigned)(rows * p.parts)), 64, 0, st, dim3(1), p);
+    if (n == 128) return launch_early("log_probs_grad_kernel", log_probs_grad_kernel<T, 128, ENTROPY, ALIGNED>, dim3((unsigned)(rows * p.parts)), 128, 0, st, dim3(1), p);
+    return launch_early("log_probs_grad_kernel", log_probs_grad_kernel<T, THREADS, ENTROPY, ALIGNED>, dim3((unsigned)(rows * p.parts)), THREADS, 0, st, dim3(1), p);
 }
 template <typename T>
 int log_probs_grad_typed(LogProbsGrad &p, int64_t rows, cudaStream_t st) {

@@ -262,3 +262,27 @@ def test_many_short_rows_with_masks(rows, vocab, dtype):
     ref = -lp.exp()
     ref[torch.arange(rows, device=DEV), t.clamp(min=0)] += 1
     assert bool(((g.double() - ref)[fine].abs() <= 2.0 ** -17 + torch.finfo(dtype).eps / 2 * ref[fine].abs()).all()) and not bool(g[t < 0].any())
+
+
+@pytest.mark.parametrize("rows,vocab", [(20, 700), (200, 700), (160, 8191), (300, 15001), (150, 20003), (3, 100003)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("apart", [0, 1])
+def test_gradients_of_rows_of_every_kind(rows, vocab, dtype, apart):
+    """The gradient's CTAs of each size and number, of rows that start where their gradient does and of rows that start elsewhere."""
+    big = (2.5 * torch.randn(rows, vocab + 5 * apart, generator=_gen(30), device=DEV)).to(dtype)
+    x = big[:, apart:vocab + apart].detach().requires_grad_()
+    t = torch.randint(0, vocab, (rows,), generator=_gen(31), device=DEV)
+    t[0], t[-1] = 0, vocab - 1
+    r = token_log_probs(x, t, entropy=True, top=2)
+    g, e, k = (torch.randn(*s, generator=_gen(32 + i), device=DEV) for i, s in enumerate(((rows,), (rows,), (rows, 2))))
+    (got,) = torch.autograd.grad((r.log_probs, r.entropy, r.top_log_probs), x, (g, e, k))
+    lp = torch.log_softmax(x.detach().double(), -1)
+    p, h = lp.exp(), torch.special.entr(lp.exp()).sum(-1)
+    all_g = (g.double() + k.double().sum(-1))[:, None]
+    want = p * (-all_g - e.double()[:, None] * (lp + h[:, None]))
+    want.scatter_add_(1, t[:, None], g.double()[:, None])
+    want.scatter_add_(1, r.top_tokens, k.double())
+    size = p * (all_g.abs() + g.double().abs()[:, None] + k.double().abs().sum(-1)[:, None] + e.double().abs()[:, None] * ((lp + h[:, None]).abs() + h[:, None]))
+    # exponents of spans of 25 good to 2^-20, relative; entries of tokens are sums of up to four parts
+    off = 2.0 ** -17 * size + 2.0 ** -21 * (g.abs() + k.abs().sum(-1)).double()[:, None]
+    assert bool(((got.double() - want).abs() <= off + torch.finfo(dtype).eps / 2 * (want.abs() + off) + 2.0 ** -130).all())
