@@ -13,6 +13,7 @@ import threading
 import warnings
 
 import torch
+from torch.utils._python_dispatch import _get_current_dispatch_mode_stack as _dispatch_modes
 
 F32, F16, BF16, I32 = 0, 1, 2, 3
 RTN_UPCAST_F32 = 1
@@ -237,6 +238,13 @@ def refuse_capture(name):
     stream (a graph of the same leaves that still lives) torch does not survive handing it a captured gradient."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name}: this backward pass cannot be captured without the native host side of the operators, or of tensors that it does not take")
+
+
+def refuse_recorders(name, traced=False):
+    """For the Python path of the operators, whose kernels are foreign calls: whoever writes torch operations down to run them again (make_fx, fake tensors) would keep the
+    allocation of an output and nothing that fills it.  `traced`: so would torch.jit.trace, which keeps an autograd function, where there is one, whole."""
+    if (traced and torch.jit.is_tracing()) or any(getattr(mode, "_mode_key", None) is not None for mode in _dispatch_modes()):
+        raise RuntimeError(f"{name}: calls of this library cannot be recorded as torch operations")
 
 
 def check(status):

@@ -85,6 +85,18 @@ class RotaryPositions:
         out = ops.rotate(self.table, self._meta, positions, *xs)
         if out is not None:
             return out
+        _lib.refuse_recorders("rotate")
+        if not torch.jit.is_tracing():
+            rows = self._rows(positions, xs)
+            out = ops.rotate(self._checked(self.table), self._meta, *rows)
+            if out is not None:
+                out = tuple(y.view(x.shape) for x, y in zip(xs, (out,) if len(xs) == 1 else out))
+        if out is None:
+            out = RotateFunction.apply(self, positions, *xs)
+        return out[0] if len(xs) == 1 else out
+
+    def _rows(self, positions, xs):
+        """(positions, tensors...) of a call, checked, as the kernels take them."""
         if not 1 <= len(xs) <= 2:
             raise ValueError("rotate takes one or two tensors")
         for x in xs:
@@ -95,14 +107,7 @@ class RotaryPositions:
                 raise RuntimeError(f"`x` is on {x.device} but the table is on {self.device}")
             if x.dim() < 2 or x.shape[:-2] != xs[0].shape[:-2] or x.shape[-1] != xs[0].shape[-1] or x.shape[-1] < self.rotary_dim:
                 raise ValueError(f"the tensors to rotate must be [..., heads, dim] of one leading shape and one dim of at least {self.rotary_dim}")
-        positions, rows = self._positions(positions, xs[0].shape[:-2]), [_rows(x) for x in xs]
-        out = ops.rotate(self._checked(self.table), self._meta, positions, *rows)
-        if out is None:
-            out = RotateFunction.apply(self, positions, *rows) if torch.is_grad_enabled() and any(x.requires_grad for x in xs) else _rotate(self, self.table, positions, rows, False)
-        elif len(xs) == 1:
-            out = (out,)
-        out = tuple(y.view(x.shape) for x, y in zip(xs, out))
-        return out[0] if len(xs) == 1 else out
+        return self._positions(positions, xs[0].shape[:-2]), *(_rows(x) for x in xs)
 
     def __repr__(self):
         return f"RotaryPositions(rotary_dim={self.rotary_dim}, max_positions={self.max_positions}, num_axes={self.num_axes}, interleaved={self.interleaved})"
@@ -115,10 +120,10 @@ def _rows(x):
     return x if x.stride(2) == 1 else x.contiguous()
 
 
-def _rotate(rotary, table, positions, xs, inverse):
-    """New tensors: those of `xs` ([tokens, heads, dim]) that are there, turned (or turned back).  None where there is none."""
-    outs = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in xs]
-    given = [(_rows(x), out) for x, out in zip(xs, outs) if out is not None and out.numel()]
+def _rotate(rotary, table, positions, rows, shapes, inverse):
+    """New tensors of `shapes`: those of `rows` ([tokens, heads, dim], as `_rows` gives them) that are there, turned (or turned back).  None where there is none."""
+    outs = [None if x is None else torch.empty(shape, dtype=x.dtype, device=x.device) for x, shape in zip(rows, shapes)]
+    given = [(x, out) for x, out in zip(rows, outs) if out is not None and out.numel()]
     if given:
         args = []
         for x, out in given:
@@ -134,15 +139,16 @@ def _rotate(rotary, table, positions, xs, inverse):
 
 
 class RotateFunction(torch.autograd.Function):
-    """apply(rotary, positions, *xs) with what `rotate` has checked."""
+    """apply(rotary, positions, *xs): what `rotate` says, of tensors that it may have checked or not (a traced call runs again with others)."""
 
     @staticmethod
     def forward(ctx, rotary, positions, *xs):
+        positions, *rows = rotary._rows(positions, xs)
         ctx.rotary = rotary
         ctx.save_for_backward(rotary.table, positions)
         ctx.like = (positions.shape, positions.dtype, positions.device)
         ctx.set_materialize_grads(False)
-        return tuple(_rotate(rotary, rotary.table, positions, xs, False))
+        return tuple(_rotate(rotary, rotary.table, positions, rows, [x.shape for x in xs], False))
 
     @staticmethod
     @once_differentiable
@@ -152,5 +158,5 @@ class RotateFunction(torch.autograd.Function):
         # (hooks may have made other tensors of them in the meantime: moved, packed)
         if (positions.shape, positions.dtype, positions.device) != ctx.like:
             raise RuntimeError("rotate: a tensor saved for the backward pass has come back from its hooks in another shape, type or place")
-        wanted = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[2:])]
-        return (None, None, *_rotate(ctx.rotary, table, positions.contiguous(), wanted, True))
+        wanted = [_rows(g) if g is not None and need else None for g, need in zip(grads, ctx.needs_input_grad[2:])]
+        return (None, None, *_rotate(ctx.rotary, table, positions.contiguous(), wanted, [None if g is None else g.shape for g in grads], True))
