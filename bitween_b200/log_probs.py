@@ -14,14 +14,14 @@ _FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 TokenLogProbs = namedtuple("TokenLogProbs", "log_probs entropy top_log_probs top_tokens")
 
 
-def _forward(logits, tokens, entropy, top, keep):
-    """(log_probs, entropy, top_log_probs, top_tokens, stats) of logits [rows, vocab]; None for what is not asked."""
+def _forward(logits, tokens, entropy, top, keep, lead):
+    """(log_probs, entropy, top_log_probs, top_tokens, stats) of logits [rows, vocab], the first four of the leading shape `lead`; None for what is not asked."""
     rows, vocab = logits.shape
     dev = logits.device
-    lp = None if tokens is None else torch.empty(rows, dtype=torch.float32, device=dev)
-    h = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
-    top_lp = torch.empty((rows, top), dtype=torch.float32, device=dev) if top else None
-    top_t = torch.empty((rows, top), dtype=torch.int64, device=dev) if top else None
+    lp = None if tokens is None else torch.empty(lead, dtype=torch.float32, device=dev)
+    h = torch.empty(lead, dtype=torch.float32, device=dev) if entropy else None
+    top_lp = torch.empty((*lead, top), dtype=torch.float32, device=dev) if top else None
+    top_t = torch.empty((*lead, top), dtype=torch.int64, device=dev) if top else None
     stats = torch.empty((rows, 4), dtype=torch.float32, device=dev) if keep else None
     L = _lib.lib()
     with _lib.on_device(dev):
@@ -37,14 +37,15 @@ def _dense(t):
 
 
 class TokenLogProbsFunction(torch.autograd.Function):
-    """apply(logits [rows, vocab], tokens, entropy, top) with what `token_log_probs` has checked."""
+    """apply(logits, tokens, entropy, top): what `token_log_probs` says, of arguments that it may have checked or not (a traced call runs again with other tensors)."""
 
     @staticmethod
     def forward(ctx, logits, tokens, entropy, top):
-        lp, h, top_lp, top_t, stats = _forward(logits, tokens, entropy, top, True)
-        ctx.save_for_backward(logits, tokens, top_t, stats)
-        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in (logits, tokens, top_t, stats)]
-        ctx.top = top
+        x, tokens = _arguments(logits, tokens, top)
+        lp, h, top_lp, top_t, stats = _forward(x, tokens, entropy, top, ctx.needs_input_grad[0], logits.shape[:-1])
+        ctx.save_for_backward(x, tokens, top_t, stats)
+        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in (x, tokens, top_t, stats)]
+        ctx.top, ctx.shape = top, logits.shape
         ctx.set_materialize_grads(False)
         if top_t is not None:
             ctx.mark_non_differentiable(top_t)
@@ -66,7 +67,7 @@ class TokenLogProbsFunction(torch.autograd.Function):
         g, e, g_top = _dense(g), _dense(e), _dense(g_top)
         rows, vocab = logits.shape
         dev = logits.device
-        grad = torch.empty((rows, vocab), dtype=logits.dtype, device=dev)
+        grad = torch.empty(ctx.shape, dtype=logits.dtype, device=dev)
         L = _lib.lib()
         with _lib.on_device(dev):
             rc = L.bw_token_log_probs_grad(logits.data_ptr(), _lib.dtype_code(logits.dtype), rows, vocab, logits.stride(0),
@@ -79,6 +80,27 @@ class TokenLogProbsFunction(torch.autograd.Function):
 def _rows(logits):
     logits = logits.resolve_neg()
     return logits if logits.stride(1) == 1 and logits.stride(0) >= 0 else logits.contiguous()
+
+
+def _arguments(logits, tokens, top):
+    """(logits [rows, vocab], tokens [rows]) of a call, checked, as the kernels take them."""
+    _lib.require_cuda(logits, "logits")
+    if logits.dtype not in _FLOAT_DTYPES:
+        raise TypeError(f"token_log_probs: unsupported dtype {logits.dtype} (float32/float16/bfloat16)")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError("logits must be [..., vocab] of at least one token")
+    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    if not 0 <= top <= min(32, vocab):
+        raise ValueError(f"top must be 0 to {min(32, vocab)}")
+    if tokens is not None:
+        if tokens.dtype != torch.int64:
+            raise TypeError("tokens must be int64")
+        if tokens.shape != lead:
+            raise ValueError(f"tokens must have shape {tuple(lead)}")
+        if tokens.device != logits.device:
+            raise RuntimeError(f"`tokens` is on {tokens.device} but logits is on {logits.device}")
+        tokens = tokens.reshape(-1).contiguous()
+    return _rows(logits.reshape(-1, vocab)), tokens
 
 
 def token_log_probs(logits, tokens=None, entropy=False, top=0):
@@ -94,28 +116,13 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0):
     out = ops.token_log_probs(logits, tokens, entropy, top)
     if out is not None:
         return TokenLogProbs._make(out)
-    _lib.require_cuda(logits, "logits")
-    if logits.dtype not in _FLOAT_DTYPES:
-        raise TypeError(f"token_log_probs: unsupported dtype {logits.dtype} (float32/float16/bfloat16)")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError("logits must be [..., vocab] of at least one token")
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
-    top = operator.index(top)
-    if not 0 <= top <= min(32, vocab):
-        raise ValueError(f"top must be 0 to {min(32, vocab)}")
-    if tokens is not None:
-        if tokens.dtype != torch.int64:
-            raise TypeError("tokens must be int64")
-        if tokens.shape != lead:
-            raise ValueError(f"tokens must have shape {tuple(lead)}")
-        if tokens.device != logits.device:
-            raise RuntimeError(f"`tokens` is on {tokens.device} but logits is on {logits.device}")
-        tokens = tokens.reshape(-1).contiguous()
-    x = _rows(logits.reshape(-1, vocab))
-    entropy = bool(entropy)
+    _lib.refuse_recorders("token_log_probs")
+    entropy, top = bool(entropy), operator.index(top)
+    x, t = (logits, tokens) if torch.jit.is_tracing() else _arguments(logits, tokens, top)
     if tokens is None and not entropy and not top:
         return TokenLogProbs(None, None, None, None)
-    out = ops.token_log_probs(x, tokens, entropy, top)
-    if out is None:
-        out = TokenLogProbsFunction.apply(x, tokens, entropy, top) if torch.is_grad_enabled() and logits.requires_grad else _forward(x, tokens, entropy, top, False)[:4]
-    return TokenLogProbs(*(t if t is None else t.view((*lead, *t.shape[1:])) for t in out))
+    out = ops.token_log_probs(x, t, entropy, top)
+    if out is not None:
+        return TokenLogProbs(*(y if y is None else y.view((*logits.shape[:-1], *y.shape[1:])) for y in out))
+    del x, t                                             # (a copy of strided rows is made again)
+    return TokenLogProbs._make(TokenLogProbsFunction.apply(logits, tokens, entropy, top))

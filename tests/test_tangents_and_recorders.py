@@ -7,7 +7,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from bitween_b200 import RotaryPositions
+from bitween_b200 import RotaryPositions, token_log_probs
 from bitween_b200.kernels import _lib
 
 
@@ -89,3 +89,69 @@ def test_a_traced_rotate_runs_again_on_other_tensors():
     with fwad.dual_level(), pytest.raises(NotImplementedError):
         r.rotate(p, fwad.make_dual(x, x))
     _not_recorded(lambda x: r.rotate(p, x), x)
+
+
+def test_token_log_probs(library):
+    t, x, column = torch.arange(3), torch.randn(3, 50), torch.arange(3)[:, None]
+    for call in (lambda x: token_log_probs(x, t).log_probs, lambda x: token_log_probs(x, entropy=True).entropy, lambda x: tuple(token_log_probs(x, t, entropy=True, top=3)),
+                 lambda x: token_log_probs(x[:, :40].unflatten(0, (3, 1)), column, top=2).top_log_probs):
+        _tangent_refused(call, x)
+        _not_recorded(call, x)
+        traced = _traced(call, x)
+        assert "^TokenLogProbsFunction" in str(traced.graph) and "aten::empty" not in str(traced.graph)
+        library.calls.clear()
+        traced(x)
+        assert library.calls == ["bw_token_log_probs"]
+    traced = _traced(lambda x, t: token_log_probs(x, t, top=3).log_probs, (x, t))
+    library.calls.clear()
+    for bad in ((x.double(), t), (x, t.int()), (x, t[:2]), (x[:, :2], t)):
+        with pytest.raises(Exception, match="must|unsupported"):
+            traced(*bad)
+    assert not library.calls
+    assert token_log_probs(x) == (None,) * 4
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_traced_log_probs_run_again_on_other_tensors():
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x, other = (torch.randn(4, 7, 1003, generator=g, device="cuda").bfloat16() for _ in range(2))
+    t = torch.randint(-1, 1003, (4, 7), generator=g, device="cuda")
+    traced = torch.jit.trace(lambda x, t: tuple(token_log_probs(x, t, entropy=True, top=4)), (x, t), check_trace=False)
+    columns = torch.randn(1003, 7, 4, generator=g, device="cuda").bfloat16().permute(2, 1, 0)
+    for a in (x, other, columns, torch.cat((x, other), 1)[:, 3:10]):
+        for at in (t, t.flip(0)):
+            assert all(torch.equal(got, want) for got, want in zip(traced(a, at), token_log_probs(a, at, entropy=True, top=4)))
+    leaf = other.clone().requires_grad_()
+    ones = torch.ones(4, 7, device="cuda")
+    (got,) = torch.autograd.grad(traced(leaf, t)[0], leaf, ones)
+    (want,) = torch.autograd.grad(token_log_probs(leaf, t).log_probs, leaf, ones)
+    assert torch.equal(got, want)
+    with fwad.dual_level(), pytest.raises(NotImplementedError):
+        token_log_probs(fwad.make_dual(x, x), t)
+    _not_recorded(lambda x: token_log_probs(x, t).log_probs, x)
+
+
+@pytest.mark.gpu
+def test_gradients_of_rows_with_two_strides_on_both_paths(monkeypatch):
+    """Rows whose leading dimensions are not one stride, and outputs that are written in place."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    big, t = torch.randn(4, 9, 1003, generator=g, device="cuda"), torch.randint(0, 1003, (4, 8), generator=g, device="cuda")
+    results = []
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(_lib, "_operators", _lib._NoOperators)
+        leaf = big.clone().requires_grad_()
+        r = token_log_probs(leaf[:, :-1], t, entropy=True, top=2)
+        r.log_probs.mul_(0.5)
+        (r.log_probs.sum() + r.entropy.sum() + r.top_log_probs[..., 1].sum()).backward()
+        results.append((*(y.detach() for y in r), leaf.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and not bool(results[0][-1][:, -1].any())
+    p = torch.softmax(big[:, :-1].double(), -1)
+    inner = p.log() + torch.special.entr(p).sum(-1, keepdim=True)
+    want = p * (-1.5 - inner)
+    want.scatter_add_(-1, t[..., None], torch.full((4, 8, 1), 0.5, dtype=torch.float64, device="cuda"))
+    want.scatter_add_(-1, results[0][3][..., 1:], torch.ones(4, 8, 1, dtype=torch.float64, device="cuda"))
+    # exponents of spans of less than 16 good to 2^-18, relative, of p (1.5 + |inner| + H); an entry of a token is a sum of up to three parts
+    size = p * (1.5 + inner.abs() + 7)
+    assert bool(((results[0][-1][:, :-1].double() - want).abs() <= 2.0 ** -18 * size + 2.0 ** -21 * (want.abs() + size)).all())
