@@ -6,11 +6,19 @@ import math
 import operator
 
 import torch
+import torch.autograd.forward_ad as fwad
 
 from .kernels import _lib
 from .rotary import RotaryPositions
 
 _FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _refuse_derivatives(name, q):
+    if q.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} has no gradient; detach q or call it under torch.no_grad()")
+    if fwad.unpack_dual(q).tangent is not None:
+        raise ValueError(f"{name} has no forward-mode derivative; detach q")
 
 
 class QuantizedKVCache:
@@ -85,6 +93,7 @@ class QuantizedKVCache:
         infinity, or whose scale leaves fp16's range, reads back as NaN.  Codes have no gradient: nothing is recorded."""
         if (_lib._operators or _lib.host_operators()).kv_append(*self._cache, k, v, slots):
             return
+        _lib.refuse_recorders("append", traced=True)
         _lib.require_cuda(self.k_codes, "cache")
         slots = self._check_slots(slots)
         shape = (slots.shape[0], self.num_kv_heads, self.head_dim)
@@ -113,11 +122,12 @@ class QuantizedKVCache:
 
         Keys are rotated in fp32 and quantised from there: the cache holds what `append(rotary.rotate(positions, k.float()), v.float(), slots)` would
         leave.  `positions`: int64 [tokens], or [axes, tokens].  A position outside the table gives NaN: that token's queries, and its key when it is read.  Queries
-        of skipped slots are rotated too.  Nothing is recorded: a q that requires a gradient is refused where gradients are recorded."""
+        of skipped slots are rotated too.  Nothing is recorded: a q that requires a gradient is refused where gradients are recorded, and one with a forward-mode tangent."""
         if type(rotary) is RotaryPositions:
             out = (_lib._operators or _lib.host_operators()).kv_append_rotated(*self._cache, q, k, v, slots, rotary.table, rotary._meta, positions)
             if out is not None:
                 return None if q is None else out
+        _lib.refuse_recorders("append_rotated", traced=True)
         _lib.require_cuda(self.k_codes, "cache")
         slots = self._check_slots(slots)
         tokens = slots.shape[0]
@@ -136,8 +146,7 @@ class QuantizedKVCache:
         if q is not None:
             if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != self.head_dim:
                 raise ValueError(f"q must be [{tokens}, heads, {self.head_dim}]")
-            if q.requires_grad and torch.is_grad_enabled():
-                raise ValueError("append_rotated has no gradient; detach q, or rotate it by itself")
+            _refuse_derivatives("append_rotated", q)
         if not isinstance(rotary, RotaryPositions):
             raise TypeError("rotary must be a RotaryPositions")
         if rotary.device != self.device:
@@ -164,6 +173,7 @@ class QuantizedKVCache:
         both = (_lib._operators or _lib.host_operators()).kv_read(*self._cache, slots, _lib.dtype_code(dtype))
         if both is not None:
             return both
+        _lib.refuse_recorders("read", traced=True)
         _lib.require_cuda(self.k_codes, "cache")
         slots = self._check_slots(slots)
         shape = (slots.shape[0], self.num_kv_heads, self.head_dim)
@@ -183,7 +193,7 @@ class QuantizedKVCache:
         `softmax_scale` defaults to head_dim ** -0.5.  The new token's own row is attended to if it has been appended and counted.  Sequences
         of length 0 (or less) give zeros.  A length that is more than the table holds, and a page outside the cache within the
         length, give NaN for that sequence; nothing is read there.  There is no gradient: a q that requires one is refused where
-        gradients are recorded.
+        gradients are recorded, and one with a forward-mode tangent.
 
         `window` (None: all): only the last `window` tokens of a sequence and its first `sinks` are attended to.  Pages that hold none of those are
         not looked up: they may have been given to others, and their entries of the table may be anything."""
@@ -232,11 +242,11 @@ class QuantizedKVCache:
 
     def _attend_args(self, q, page_table, lengths):
         """Checked arguments of a call of attention as the kernels take them, and its output."""
+        _lib.refuse_recorders("attend", traced=True)
         _lib.require_cuda(q, "q")
         if q.dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"attend: unsupported dtype {q.dtype} (float16/bfloat16)")
-        if q.requires_grad and torch.is_grad_enabled():
-            raise ValueError("attend has no gradient; detach q or call it under torch.no_grad()")
+        _refuse_derivatives("attend", q)
         if q.dim() != 3 or q.shape[2] != self.head_dim or q.shape[1] < 1 or q.shape[1] % self.num_kv_heads != 0:
             raise ValueError(f"q must be [batch, heads, {self.head_dim}] with a multiple of {self.num_kv_heads} heads")
         if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:

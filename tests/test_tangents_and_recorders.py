@@ -7,7 +7,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from bitween_b200 import RotaryPositions, token_log_probs
+from bitween_b200 import QuantizedKVCache, RotaryPositions, token_log_probs
 from bitween_b200.kernels import _lib
 
 
@@ -155,3 +155,38 @@ def test_gradients_of_rows_with_two_strides_on_both_paths(monkeypatch):
     # exponents of spans of less than 16 good to 2^-18, relative, of p (1.5 + |inner| + H); an entry of a token is a sum of up to three parts
     size = p * (1.5 + inner.abs() + 7)
     assert bool(((results[0][-1][:, :-1].double() - want).abs() <= 2.0 ** -18 * size + 2.0 ** -21 * (want.abs() + size)).all())
+
+
+def _cache_calls(dev):
+    """Calls of a cache whose codes have no derivative: (call, its float tensor or slots, whether a tangent of that is refused)."""
+    cache, r, p = QuantizedKVCache(4, 16, 2, 64, bits=4, device=dev), RotaryPositions(64, 50, device=dev), torch.arange(3, device=dev)
+    x, table, n = torch.randn(3, 2, 64, device=dev).half(), torch.zeros(3, 1, dtype=torch.int32, device=dev), torch.ones(3, dtype=torch.int32, device=dev)
+    return [(lambda q: cache.attend(q, table, n), x, True), (lambda q: cache.attend(q, table, n, window=3), x, True),
+            (lambda q: cache.append_rotated(q, x, x, p, r, p), x, True), (lambda k: cache.append_rotated(None, k, k, p, r, p), x, False),
+            (lambda k: cache.append(k, k, p), x, False), (lambda s: cache.read(s), p, False)]
+
+
+def _cache_refusals(dev):
+    for call, x, derived in _cache_calls(dev):
+        _not_recorded(call, x)
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            torch.jit.trace(call, x, check_trace=False)
+        if derived:
+            with pytest.raises(ValueError, match="no gradient"):
+                call(x.clone().requires_grad_())
+        for mode in (contextlib.nullcontext, torch.no_grad) if derived else ():
+            with fwad.dual_level(), mode():
+                dual = fwad.make_dual(x, torch.ones_like(x))
+                with pytest.raises(ValueError, match="no forward-mode derivative"):
+                    call(dual)
+                call(dual.detach())
+
+
+def test_the_cache(library):
+    _cache_refusals("cpu")
+    assert "bw_kv_attend" in library.calls and "bw_kv_attend_window" in library.calls and "bw_kv_append_rotated" in library.calls
+
+
+@pytest.mark.gpu
+def test_the_cache_on_the_gpu():
+    _cache_refusals("cuda")
