@@ -35,55 +35,8 @@ def _forward(x, down, up, index, scaling, base, out, keep):
     return out, hidden if keep else None
 
 
-class AdapterFunction(torch.autograd.Function):
-    """apply(x [M, K], down, up, index, scaling, base) with what `adapter_matmul` has checked."""
-
-    @staticmethod
-    def forward(ctx, x, down, up, index, scaling, base):
-        out, hidden = _forward(x, down, up, index, scaling, base, None, ctx.needs_input_grad[2])
-        ctx.save_for_backward(x, down, up, index, scaling, hidden)
-        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in (x, down, up, index, scaling, hidden)]
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_out):
-        saved = ctx.saved_tensors
-        # (hooks may have made other tensors of them in the meantime: moved, packed)
-        if any((t is None) != (like is None) or (t is not None and (t.shape, t.dtype, t.device) != like) for t, like in zip(saved, ctx.like)):
-            raise RuntimeError("adapter_matmul: a tensor saved for the backward pass has come back from its hooks in another shape, type or place")
-        x, down, up, index, scaling, hidden = (t if t is None else _aligned(t.resolve_neg()) for t in saved)
-        want_x, want_down, want_up = ctx.needs_input_grad[:3]
-        grads = [torch.empty_like(t) if want else None for t, want in ((x, want_x), (down, want_down), (up, want_up))]
-        if want_x or want_down or want_up:
-            M, K = x.shape
-            adapters, rank, N = up.shape
-            dev = x.device
-            g = _aligned(grad_out)
-            L = _lib.lib()
-            with _lib.on_device(dev):
-                ws = _lib.workspace(dev, L.bw_adapter_hidden_bytes(M, rank))
-                rc = L.bw_adapter_backward(g.data_ptr(), _lib.dtype_code(x.dtype), x.data_ptr(), M, N, K, down.data_ptr(), up.data_ptr(), adapters, rank,
-                                           index.data_ptr(), None if scaling is None else scaling.data_ptr(),
-                                           None if hidden is None else hidden.data_ptr(), 0 if hidden is None else hidden.numel(),
-                                           *(None if t is None else t.data_ptr() for t in grads),
-                                           None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _lib.raw_stream(dev))
-            _lib.check(rc)
-        return (*grads, None, None, grad_out if ctx.needs_input_grad[5] else None)
-
-
-def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
-    """base[t] + scaling[i] * up[i]^T (down[i] x[t]) with i = index[t], for x [..., K] and the bank `down` [adapters, rank, K], `up`
-    [adapters, rank, N] (both rank-major: `up` is the transpose of a PEFT checkpoint's lora_B).  Returns [..., N].
-
-    `index`, int32 of x's leading shape (or flat): the adapter of each row; rows below 0 have none and get `base` (zeros without
-    one); an index beyond the bank gives NaN.  `scaling`: fp32 [adapters] or None (ones); it has no gradient.  x, down, up and base share one
-    dtype, fp16 or bf16; sums are fp32 and the result is rounded once.  Ranks up to 256.  Differentiable in x, down, up and base.
-    `out`, a contiguous tensor of the result's shape, takes the result where no gradient is recorded (one that requires a gradient is refused, too); it may be `base`
-    itself."""
-    y = (_lib._operators or _lib.host_operators()).adapter_matmul(x, down, up, index, scaling, base, out)
-    if y is not None:
-        return y
+def _arguments(x, down, up, index, scaling, base, out=None):
+    """(x [M, K], down, up, index [M], scaling, base [M, N]) of a call, checked, as the kernels take them."""
     _lib.require_cuda(x, "x")
     if x.dtype not in _DTYPES:
         raise TypeError(f"adapter_matmul: unsupported dtype {x.dtype} (float16/bfloat16)")
@@ -120,26 +73,85 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
     if scaling is not None:
         scaling = scaling.contiguous()
     base2 = None if base is None else _aligned(base.reshape(M, N))
-    args = (_aligned(x2), _aligned(down), _aligned(up), index, scaling, base2)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, base))
-    if out is not None:
-        if grad or (torch.is_grad_enabled() and out.requires_grad):
-            raise ValueError("`out` is for calls that record no gradient")
-        if out.shape != (*lead, N) or not out.is_contiguous():
-            raise ValueError(f"`out` must be contiguous {(*lead, N)}")
-        if out.data_ptr() % 16 != 0:
-            return out.copy_(_forward(*args, None, False)[0].view(*lead, N))
-        for i in range(6):          # kernels store outputs while others still read
-            t = args[i]
-            if t is not None and t.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < t.data_ptr() + t.nbytes and \
-                    not (i == 5 and t.data_ptr() == out.data_ptr()):
-                args = (*args[:i], t.clone(), *args[i + 1:])
-        _forward(*args, out.view(M, N), False)
-        if not out.is_inference():
-            torch.autograd.graph.increment_version(out)      # (written in place, as autograd has to know)
+    return _aligned(x2), _aligned(down), _aligned(up), index, scaling, base2
+
+
+class AdapterFunction(torch.autograd.Function):
+    """apply(x, down, up, index, scaling, base): what `adapter_matmul` says, of arguments that it may have checked or not (a traced call runs again with other tensors)."""
+
+    @staticmethod
+    def forward(ctx, x, down, up, index, scaling, base):
+        ctx.shape = x.shape
+        x, down, up, index, scaling, base = _arguments(x, down, up, index, scaling, base)
+        out = torch.empty((*ctx.shape[:-1], up.shape[2]), dtype=x.dtype, device=x.device)
+        _, hidden = _forward(x, down, up, index, scaling, base, out, ctx.needs_input_grad[2])
+        ctx.save_for_backward(x, down, up, index, scaling, hidden)
+        ctx.like = [None if t is None else (t.shape, t.dtype, t.device) for t in (x, down, up, index, scaling, hidden)]
         return out
-    y = AdapterFunction.apply(*args) if grad else _forward(*args, None, False)[0]
-    return y.view(*lead, N)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        saved = ctx.saved_tensors
+        # (hooks may have made other tensors of them in the meantime: moved, packed)
+        if any((t is None) != (like is None) or (t is not None and (t.shape, t.dtype, t.device) != like) for t, like in zip(saved, ctx.like)):
+            raise RuntimeError("adapter_matmul: a tensor saved for the backward pass has come back from its hooks in another shape, type or place")
+        x, down, up, index, scaling, hidden = (t if t is None else _aligned(t.resolve_neg()) for t in saved)
+        want_x, want_down, want_up = ctx.needs_input_grad[:3]
+        grads = [torch.empty_like(t) if want else None for t, want in ((x, want_x), (down, want_down), (up, want_up))]
+        if want_x or want_down or want_up:
+            M, K = x.shape
+            adapters, rank, N = up.shape
+            dev = x.device
+            g = _aligned(grad_out)
+            L = _lib.lib()
+            with _lib.on_device(dev):
+                ws = _lib.workspace(dev, L.bw_adapter_hidden_bytes(M, rank))
+                rc = L.bw_adapter_backward(g.data_ptr(), _lib.dtype_code(x.dtype), x.data_ptr(), M, N, K, down.data_ptr(), up.data_ptr(), adapters, rank,
+                                           index.data_ptr(), None if scaling is None else scaling.data_ptr(),
+                                           None if hidden is None else hidden.data_ptr(), 0 if hidden is None else hidden.numel(),
+                                           *(None if t is None else t.data_ptr() for t in grads),
+                                           None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _lib.raw_stream(dev))
+            _lib.check(rc)
+        if want_x:
+            grads[0] = grads[0].view(ctx.shape)
+        return (*grads, None, None, grad_out if ctx.needs_input_grad[5] else None)
+
+
+def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
+    """base[t] + scaling[i] * up[i]^T (down[i] x[t]) with i = index[t], for x [..., K] and the bank `down` [adapters, rank, K], `up`
+    [adapters, rank, N] (both rank-major: `up` is the transpose of a PEFT checkpoint's lora_B).  Returns [..., N].
+
+    `index`, int32 of x's leading shape (or flat): the adapter of each row; rows below 0 have none and get `base` (zeros without
+    one); an index beyond the bank gives NaN.  `scaling`: fp32 [adapters] or None (ones); it has no gradient.  x, down, up and base share one
+    dtype, fp16 or bf16; sums are fp32 and the result is rounded once.  Ranks up to 256.  Differentiable in x, down, up and base.
+    `out`, a contiguous tensor of the result's shape, takes the result where no gradient is recorded (one that requires a gradient is refused, too, and so is any tensor with a
+    forward-mode tangent); it may be `base` itself."""
+    y = (_lib._operators or _lib.host_operators()).adapter_matmul(x, down, up, index, scaling, base, out)
+    if y is not None:
+        return y
+    _lib.refuse_recorders("adapter_matmul", traced=out is not None)
+    if out is None:
+        return AdapterFunction.apply(x, down, up, index, scaling, base)
+    args = _arguments(x, down, up, index, scaling, base, out)
+    lead, (M, N) = x.shape[:-1], (args[0].shape[0], up.shape[2])
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, base, out)):
+        raise ValueError("`out` is for calls that record no gradient")
+    if _lib.any_tangent(x, down, up, scaling, base, out):
+        raise ValueError("`out` is for calls without a forward-mode tangent")
+    if out.shape != (*lead, N) or not out.is_contiguous():
+        raise ValueError(f"`out` must be contiguous {(*lead, N)}")
+    if out.data_ptr() % 16 != 0:
+        return out.copy_(_forward(*args, None, False)[0].view(*lead, N))
+    for i in range(6):          # kernels store outputs while others still read
+        t = args[i]
+        if t is not None and t.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < t.data_ptr() + t.nbytes and \
+                not (i == 5 and t.data_ptr() == out.data_ptr()):
+            args = (*args[:i], t.clone(), *args[i + 1:])
+    _forward(*args, out.view(M, N), False)
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)      # (written in place, as autograd has to know)
+    return out
 
 
 class AdaptedLinear(nn.Module):
@@ -174,7 +186,9 @@ class AdaptedLinear(nn.Module):
         else:                                      # a layer with a forward of its own
             base, in_place = layer(x), False
         base = base.to(dtype)
-        in_place = in_place and not (torch.is_grad_enabled() and (base.requires_grad or self.down.requires_grad or self.up.requires_grad))
+        # (nor is it where the call is traced or asked for a tangent, which is for the autograd function)
+        in_place = in_place and not (torch.is_grad_enabled() and (base.requires_grad or self.down.requires_grad or self.up.requires_grad)) and \
+            not torch.jit.is_tracing() and not _lib.any_tangent(x, self.down, self.up)
         return adapter_matmul(x, self.down, self.up, index, scaling=self.scaling.float(), base=base, out=base if in_place else None)
 
     def extra_repr(self):

@@ -13,6 +13,7 @@ import threading
 import warnings
 
 import torch
+import torch.autograd.forward_ad as fwad
 from torch.utils._python_dispatch import _get_current_dispatch_mode_stack as _dispatch_modes
 
 F32, F16, BF16, I32 = 0, 1, 2, 3
@@ -238,6 +239,11 @@ def refuse_capture(name):
     stream (a graph of the same leaves that still lives) torch does not survive handing it a captured gradient."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name}: this backward pass cannot be captured without the native host side of the operators, or of tensors that it does not take")
+
+
+def any_tangent(*tensors):
+    """Whether one of them has a forward-mode tangent.  (Only asked where a level of such is open.)"""
+    return getattr(fwad, "_current_level", 0) >= 0 and any(t is not None and fwad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def refuse_recorders(name, traced=False):

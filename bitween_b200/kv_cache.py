@@ -6,7 +6,6 @@ import math
 import operator
 
 import torch
-import torch.autograd.forward_ad as fwad
 
 from .kernels import _lib
 from .rotary import RotaryPositions
@@ -17,7 +16,7 @@ _FLOAT_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 def _refuse_derivatives(name, q):
     if q.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} has no gradient; detach q or call it under torch.no_grad()")
-    if fwad.unpack_dual(q).tangent is not None:
+    if _lib.any_tangent(q):
         raise ValueError(f"{name} has no forward-mode derivative; detach q")
 
 

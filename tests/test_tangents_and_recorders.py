@@ -7,7 +7,7 @@ import torch
 import torch.autograd.forward_ad as fwad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from bitween_b200 import QuantizedKVCache, RotaryPositions, token_log_probs
+from bitween_b200 import AdaptedLinear, QuantizedKVCache, QuantizedLinear, RotaryPositions, adapter_matmul, token_log_probs
 from bitween_b200.kernels import _lib
 
 
@@ -190,3 +190,56 @@ def test_the_cache(library):
 @pytest.mark.gpu
 def test_the_cache_on_the_gpu():
     _cache_refusals("cuda")
+
+
+def test_adapter_matmul(library):
+    x, down, up, index = torch.randn(3, 64).half(), torch.randn(2, 8, 64).half(), torch.randn(2, 8, 32).half(), torch.zeros(3, dtype=torch.int32)
+    base = torch.zeros(3, 32).half()
+    lead, lead_base = index[:, None], base[:, None]
+    for call, arg in ((lambda x: adapter_matmul(x, down, up, index), x), (lambda u: adapter_matmul(x, down, u, index, base=base), up),
+                      (lambda x: adapter_matmul(x[:, None], down, up, lead, base=lead_base), x)):
+        _tangent_refused(call, arg)
+        _not_recorded(call, arg)
+        traced = _traced(call, arg)
+        assert "^AdapterFunction" in str(traced.graph) and "aten::empty" not in str(traced.graph)
+        library.calls.clear()
+        traced(arg)
+        assert library.calls == ["bw_adapter_hidden_bytes", "bw_adapter_forward"]
+    out = torch.empty(3, 32).half()
+    with torch.no_grad():
+        _not_recorded(lambda x: adapter_matmul(x, down, up, index, out=out), x)
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            torch.jit.trace(lambda x: adapter_matmul(x, down, up, index, out=out), x, check_trace=False)
+        with fwad.dual_level():
+            for kw in ({"x": fwad.make_dual(x, x)}, {"up": fwad.make_dual(up, up)}, {"base": fwad.make_dual(base, base)}):
+                with pytest.raises(ValueError, match="forward-mode"):
+                    adapter_matmul(**({"x": x, "down": down, "up": up, "index": index, "out": out} | kw))
+
+
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_traced_adapters_run_again_on_other_tensors(monkeypatch):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    layer = AdaptedLinear(QuantizedLinear.from_float(torch.nn.Linear(128, 96).cuda().half(), bits=4, group_size=64), 2, 8)
+    with torch.no_grad():
+        layer.up.copy_(torch.randn(layer.up.shape, generator=g, device="cuda"))
+    x, other = (torch.randn(2, 3, 128, generator=g, device="cuda").half() for _ in range(2))
+    index, turned = torch.tensor([[0, 1, -1], [1, 1, 0]], dtype=torch.int32, device="cuda"), torch.randn(128, 3, 2, generator=g, device="cuda").half().permute(2, 1, 0)
+    for mode in (torch.no_grad, torch.enable_grad):
+        with mode():
+            traced = torch.jit.trace(layer, (x, index), check_trace=False)
+            for a in (x, other, turned):
+                for i in (index, index.flip(0)):
+                    assert torch.equal(traced(a, i), layer(a, i))
+            with fwad.dual_level(), pytest.raises(NotImplementedError):
+                layer(fwad.make_dual(x, x), index)
+    down, up = (t.detach() for t in (layer.down, layer.up))
+    results = []
+    for native in (True, False):
+        if not native:
+            monkeypatch.setattr(_lib, "_operators", _lib._NoOperators)
+        leaf, bank = turned.clone().requires_grad_(), up.clone().requires_grad_()
+        y = adapter_matmul(leaf, down, bank, index)
+        y.mul_(0.5)
+        results.append((y.detach(), *torch.autograd.grad(y, (leaf, bank), torch.ones_like(y))))
+    assert all(torch.equal(a, b) for a, b in zip(*results)) and results[0][1].shape == (2, 3, 128)
