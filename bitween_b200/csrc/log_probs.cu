@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(N, 4 * THREADS / N) log_probs_grad_kernel(cons
     T *out = (T *)p.grad + r * p.vocab;
     const float4 st = __ldcg(p.stats + r);
     const int64_t t = p.g ? __ldcg(p.tokens + r) : -1;
-    const float g = t < 0 ? 0.0f : t < p.vocab ? __ldcg(p.g + r) : NAN, e = ENTROPY ? __ldcg(p.e + r) : 0.0f;
+    const float given = t < 0 ? 0.0f : __ldcg(p.g + r), g = t >= p.vocab && given != 0.0f ? NAN : given, e = ENTROPY ? __ldcg(p.e + r) : 0.0f;
     const int top = p.g_top ? p.top : 0;
     float all = g;
     bool any = g != 0.0f || e != 0.0f;

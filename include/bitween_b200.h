@@ -440,7 +440,7 @@ BW_API int bw_token_log_probs(const void *logits, int dtype, int64_t rows, int64
  * Its gradient, into dense grad [rows][vocab] of the logits' type, rounded once; with g, e, g_i the gradients of log_probs, entropy and
  * top_log_probs (each may be NULL: zeros; g is 0 where t < 0)
  *   grad[j] = p[j] * (-(g + sum g_i) - e * (log p[j] + H)) + (j == t) g + sum (j == top_tokens[i]) g_i
- * A row whose g, e and g_i are all 0 gets zeros, whatever stands in its logits.
+ * A row whose g, e and g_i are all 0 gets zeros, whatever stands in its logits and whatever its token is; one with t >= vocab and a g that is not 0 gets NaN.
  */
 BW_API int bw_token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens,
                             const float *stats, const float *grad_log_probs, const float *grad_entropy, int top,
