@@ -736,6 +736,19 @@ static int log_probs_validate(int dtype, const void *logits, int64_t rows, int64
     return BW_OK;
 }
 
+// Whether one of `rows` rows of `width` bytes, `stride` bytes apart, meets the `bytes` at y.
+static bool rows_overlap(const void *x, int64_t rows, int64_t width, int64_t stride, const void *y, int64_t bytes) {
+    int64_t first = (int64_t)reinterpret_cast<uintptr_t>(x);
+    const int64_t lo = (int64_t)reinterpret_cast<uintptr_t>(y);
+    if (stride < 0) {
+        first += (rows - 1) * stride;
+        stride = -stride;
+    }
+    // the first row that ends behind lo
+    const int64_t r = first + width > lo ? 0 : stride ? (lo - first - width) / stride + 1 : rows;
+    return r < rows && first + r * stride < lo + bytes;
+}
+
 int bw_token_log_probs(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens, float *log_probs, float *entropy,
                        int top, float *top_log_probs, int64_t *top_tokens, float *stats, void *stream) {
     const int rc = log_probs_validate(dtype, logits, rows, vocab, stride, top);
@@ -758,6 +771,9 @@ int bw_token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t
     if (!aligned_to(tokens, 8) || !aligned_to(stats, 16) || !aligned_to(grad_log_probs, 4) || !aligned_to(grad_entropy, 4) || !aligned_to(top_tokens, 8) ||
         !aligned_to(grad_top, 4) || !aligned_to(grad, dtype_size(dtype)))
         return BW_ERR_ALIGN;
+    // (a token's entry is formed from its logit once more when the rest of the row has been written)
+    const int64_t e = (int64_t)dtype_size(dtype);
+    if (rows_overlap(logits, rows, vocab * e, stride * e, grad, rows * vocab * e)) return BW_ERR_UNSUPPORTED;
     return token_log_probs_grad(logits, dtype, rows, vocab, stride, tokens, stats, grad_log_probs, grad_entropy, top, top_tokens, grad_top, grad,
                                 (cudaStream_t)stream);
 }

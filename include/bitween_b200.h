@@ -417,7 +417,7 @@ BW_API int bw_rotate(const bw_rotary *rotary, int64_t tokens, int dim, int dtype
 
 /*
  * bw_kv_append of rotated keys: the rows of k are rotated in fp32 and quantised from there, those of v as they are; the rows of q [tokens][q_heads]
- * (none where q_heads is 0) are rotated into dense q_out of the same type, those of skipped slots too.
+ * (none where q_heads is 0) are rotated into dense q_out of the same type, those of skipped slots too.  q_out may not overlap q, k or v.
  */
 BW_API int bw_kv_append_rotated(const bw_rotary *rotary, const void *q, int q_heads, int64_t q_stride, int64_t q_head_stride, void *q_out,
                          const void *k, const void *v, int dtype, int64_t tokens, int64_t k_stride, int64_t k_head_stride,
@@ -441,6 +441,8 @@ BW_API int bw_token_log_probs(const void *logits, int dtype, int64_t rows, int64
  * top_log_probs (each may be NULL: zeros; g is 0 where t < 0)
  *   grad[j] = p[j] * (-(g + sum g_i) - e * (log p[j] + H)) + (j == t) g + sum (j == top_tokens[i]) g_i
  * A row whose g, e and g_i are all 0 gets zeros, whatever stands in its logits and whatever its token is; one with t >= vocab and a g that is not 0 gets NaN.
+ * `stats` and `top_tokens` are those of bw_token_log_probs on the same logits and tokens; with grad_entropy, of a call that was asked for the entropy.  grad may not overlap the logits
+ * (BW_ERR_UNSUPPORTED).
  */
 BW_API int bw_token_log_probs_grad(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t stride, const int64_t *tokens,
                             const float *stats, const float *grad_log_probs, const float *grad_entropy, int top,
