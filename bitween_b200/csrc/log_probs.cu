@@ -107,7 +107,8 @@ struct Sums {
             s *= 0.0f;
             w = 0.0f;
         } else {
-            // (products rounded by themselves: the same log probability whatever else is asked for)
+            // (products rounded by themselves: the same log probability with the entropy and without; with alternatives too, where they do not change how many threads
+            // take the row, which threads_of says: the last bits are those of the order of the sums)
             const float d = __fmul_rn(m - to, LOG2E), f = ex2(d);
             // (what fell by so much that nothing of it is left: infinite d)
             w = f == 0.0f ? 0.0f : f * fmaf(s, d, w);
@@ -389,7 +390,8 @@ __global__ void __launch_bounds__(N, (TOP ? 4 : 5) * THREADS / N) log_probs_kern
     load(0);
     const float extra = tid < row.extra ? ld_l2(row.x + row.extra_at(tid)) : -INFINITY;
     const float xt = t >= 0 && t < p.vocab ? ld_l2(row.x + t) : NAN;
-    const bool skipped = !ENTROPY && !TOP && t < 0;      // padding: nothing of the row is asked for
+    // padding: nothing of the row is asked for.  (Its first step, at most 16 KB a CTA, is read all the same: loads that waited for the token would come later in every row.)
+    const bool skipped = !ENTROPY && !TOP && t < 0;
     const int steps = skipped ? 0 : (row.v1 - row.v0 + STEP - 1) / STEP, per = (steps + BLOCKS - 1) / BLOCKS;
     Sums a = {-INFINITY, 0.0f, 0.0f};
     uint32_t key = 0;
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(N, (TOP ? 4 : 5) * THREADS / N) log_probs_kern
     }
     const int room = CANDIDATES / p.cluster;
     if constexpr (TOP) {
-        const int size = N * p.cluster / GROUPS;             // threads of a group, 2 to 32
+        const int size = N * p.cluster / GROUPS;             // threads of a group, 1 to 32
         uint32_t k = key;
         for (int d = 1; d < size; d *= 2) k = max(k, __shfl_xor_sync(0xffffffffu, k, d));
         if (p.cluster > 1) cluster_wait();
