@@ -186,10 +186,14 @@ class AdaptedLinear(nn.Module):
         else:                                      # a layer with a forward of its own
             base, in_place = layer(x), False
         base = base.to(dtype)
-        # (nor is it where the call is traced or asked for a tangent, which is for the autograd function)
-        in_place = in_place and not (torch.is_grad_enabled() and (base.requires_grad or self.down.requires_grad or self.up.requires_grad)) and \
-            not torch.jit.is_tracing() and not _lib.any_tangent(x, self.down, self.up)
-        return adapter_matmul(x, self.down, self.up, index, scaling=self.scaling.float(), base=base, out=base if in_place else None)
+        in_place = in_place and not (torch.is_grad_enabled() and (base.requires_grad or self.down.requires_grad or self.up.requires_grad))
+        scaling = self.scaling.float()
+        y = (_lib._operators or _lib.host_operators()).adapter_matmul(x, self.down, self.up, index, scaling, base, base if in_place else None)
+        if y is not None:
+            return y
+        # (a traced call, and one with a tangent, is the autograd function's)
+        in_place = in_place and not torch.jit.is_tracing() and not _lib.any_tangent(x, self.down, self.up)
+        return adapter_matmul(x, self.down, self.up, index, scaling=scaling, base=base, out=base if in_place else None)
 
     def extra_repr(self):
         return f"num_adapters={self.down.shape[0]}, rank={self.down.shape[1]}"
