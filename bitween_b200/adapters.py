@@ -131,11 +131,14 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
     if y is not None:
         return y
     _lib.refuse_recorders("adapter_matmul", traced=out is not None)
-    if out is None:
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, base, out))
+    if out is None and (grad or torch.jit.is_tracing() or _lib.any_tangent(x, down, up, scaling, base)):
         return AdapterFunction.apply(x, down, up, index, scaling, base)
     args = _arguments(x, down, up, index, scaling, base, out)
     lead, (M, N) = x.shape[:-1], (args[0].shape[0], up.shape[2])
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, base, out)):
+    if out is None:
+        return _forward(*args, None, False)[0].view(*lead, N)
+    if grad:
         raise ValueError("`out` is for calls that record no gradient")
     if _lib.any_tangent(x, down, up, scaling, base, out):
         raise ValueError("`out` is for calls without a forward-mode tangent")
