@@ -131,17 +131,14 @@ def adapter_matmul(x, down, up, index, scaling=None, base=None, out=None):
     if y is not None:
         return y
     _lib.refuse_recorders("adapter_matmul", traced=out is not None)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, down, up, base, out))
-    if out is None and (grad or torch.jit.is_tracing() or _lib.any_tangent(x, down, up, scaling, base)):
+    if out is None and _lib.for_autograd(x, down, up, scaling, base):
         return AdapterFunction.apply(x, down, up, index, scaling, base)
     args = _arguments(x, down, up, index, scaling, base, out)
     lead, (M, N) = x.shape[:-1], (args[0].shape[0], up.shape[2])
     if out is None:
         return _forward(*args, None, False)[0].view(*lead, N)
-    if grad:
-        raise ValueError("`out` is for calls that record no gradient")
-    if _lib.any_tangent(x, down, up, scaling, base, out):
-        raise ValueError("`out` is for calls without a forward-mode tangent")
+    if _lib.for_autograd(x, down, up, scaling, base, out):
+        raise ValueError("`out` is for calls that record no gradient and have no forward-mode tangent")
     if out.shape != (*lead, N) or not out.is_contiguous():
         raise ValueError(f"`out` must be contiguous {(*lead, N)}")
     if out.data_ptr() % 16 != 0:

@@ -246,6 +246,11 @@ def any_tangent(*tensors):
     return getattr(fwad, "_current_level", 0) >= 0 and any(t is not None and fwad.unpack_dual(t).tangent is not None for t in tensors)
 
 
+def for_autograd(*tensors):
+    """Whether a call that the native side has left is one for the operator's autograd function: recorded, traced, or with a tangent.  (Others are spared it.)"""
+    return torch.jit.is_tracing() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or any_tangent(*tensors)
+
+
 def refuse_recorders(name, traced=False):
     """For the Python path of the operators, whose kernels are foreign calls: whoever writes torch operations down to run them again (make_fx, fake tensors) would keep the
     allocation of an output and nothing that fills it.  `traced`: so would torch.jit.trace, which keeps an autograd function, where there is one, whole."""

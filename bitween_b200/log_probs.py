@@ -124,5 +124,7 @@ def token_log_probs(logits, tokens=None, entropy=False, top=0):
     out = ops.token_log_probs(x, t, entropy, top)
     if out is not None:
         return TokenLogProbs(*(y if y is None else y.view((*logits.shape[:-1], *y.shape[1:])) for y in out))
+    if not _lib.for_autograd(logits):
+        return TokenLogProbs._make(_forward(x, t, entropy, top, False, logits.shape[:-1])[:4])
     del x, t                                             # (a copy of strided rows is made again)
     return TokenLogProbs._make(TokenLogProbsFunction.apply(logits, tokens, entropy, top))

@@ -87,13 +87,15 @@ class RotaryPositions:
             return out
         _lib.refuse_recorders("rotate")
         if not torch.jit.is_tracing():
-            rows = self._rows(positions, xs)
-            out = ops.rotate(self._checked(self.table), self._meta, *rows)
-            if out is not None:
-                out = tuple(y.view(x.shape) for x, y in zip(xs, (out,) if len(xs) == 1 else out))
-        if out is None:
+            at, *rows = self._rows(positions, xs)
+            out = ops.rotate(self._checked(self.table), self._meta, at, *rows)
+        if out is not None:
+            out = tuple(y.view(x.shape) for x, y in zip(xs, (out,) if len(xs) == 1 else out))
+        elif _lib.for_autograd(*xs):
             out = RotateFunction.apply(self, positions, *xs)
-        return out[0] if len(xs) == 1 else out
+        else:
+            out = _rotate(self, self.table, at, rows, [x.shape for x in xs], False)
+        return out[0] if len(xs) == 1 else tuple(out)
 
     def _rows(self, positions, xs):
         """(positions, tensors...) of a call, checked, as the kernels take them."""
