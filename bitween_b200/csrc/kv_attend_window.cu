@@ -2,7 +2,8 @@
 // one are in the line of work, and tokens of those tiles that are not visible are masked like those behind the sequence.
 //
 // 64 sequences of up to 131071 tokens, window 4096 and 64 sinks, 32 and 8 heads of 128, 8 bits, bf16: 99.5 us with the join, 5.7 TB/s of the visible rows, 0.87 of the measured
-// copy rate (on the general kernel 5.5 ms); 16 of up to 8192, window 1000, 4 bits: 11.3 us, the latency of nine steps of a warp.
+// copy rate (on the general kernel 5.5 ms); 16 of up to 8192, window 1000, 4 bits: 11.2 to 12.0 us. Those are 128 units of 33 steps, which take two CTAs a unit: five steps of a warp and the
+// join of a cluster. One CTA (nine steps) takes 11.3, two 12.0, four (three steps) 12.1: a cluster's start and join cost what its fewer steps save.
 #include "kv_attend_tiles.cuh"
 
 namespace bw {

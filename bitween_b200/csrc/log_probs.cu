@@ -7,8 +7,9 @@
 // One pass over the row with the running maximum; x - m is formed before the product, so that masks of the type's lowest value stay finite or become
 // exact zeros.  Sums are fp32: 32 terms (16 of fp32 logits) by themselves, then those sums, then a tree: a chain of 500 equal terms rounds the same way each time and was
 // off by 7e-6.  Bound by the bytes of the logits where there are many rows, by latency where there are few (bf16, with entropy): 8192 x 131072 333 us, 6.4 TB/s (the measured copy
-// rate is 6.5), their gradient 640 us, 6.7 TB/s; 61 x 131071 7.0 us; one row of 50272 2.9 us.  Twenty alternatives add 19 us to 2000 x 131071 (88.8), 10 to 2000 x 32000 (27.7), 3 to 61 x 131071
-// and to one row: six barriers' worth of latency behind each row, of which an SM's other CTAs hide a part.
+// rate is 6.5), their gradient 640 us, 6.7 TB/s (1120 of rows that start elsewhere than their gradient); 61 x 131071 7.0 to 8.0 us; one row of 50272 2.9 to 3.6 us.  Twenty alternatives add 20 us to
+// 2000 x 131071 (92 to 98), 10 to 2000 x 32000 (28), 4 to 61 x 131071, five add 3 to one row: six barriers' worth of latency behind each row, of which an SM's other CTAs hide a part.  Rows whose masks leave
+// fewer values than alternatives are searched digit by digit (search_share): 61 x 131071 with all but three masked and five alternatives 120 us, 2000 x 32000 313, one row of 50272 35.
 //
 // A row is taken by a cluster of one to eight CTAs, which join through distributed shared memory.
 #include <cooperative_groups.h>
