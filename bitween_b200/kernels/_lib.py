@@ -14,7 +14,7 @@ import warnings
 
 import torch
 import torch.autograd.forward_ad as fwad
-from torch.utils._python_dispatch import _get_current_dispatch_mode_stack as _dispatch_modes
+from torch.utils import _python_dispatch
 
 F32, F16, BF16, I32 = 0, 1, 2, 3
 RTN_UPCAST_F32 = 1
@@ -239,6 +239,10 @@ def refuse_capture(name):
     stream (a graph of the same leaves that still lives) torch does not survive handing it a captured gradient."""
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError(f"{name}: this backward pass cannot be captured without the native host side of the operators, or of tensors that it does not take")
+
+
+# (not public: where a torch build has no such function, recorders are not told from other modes)
+_dispatch_modes = getattr(_python_dispatch, "_get_current_dispatch_mode_stack", tuple)
 
 
 def any_tangent(*tensors):

@@ -87,7 +87,7 @@ class RotaryPositions:
             return out
         _lib.refuse_recorders("rotate")
         if not torch.jit.is_tracing():
-            at, *rows = self._rows(positions, xs)
+            at, *rows = self._arguments(positions, xs)
             out = ops.rotate(self._checked(self.table), self._meta, at, *rows)
         if out is not None:
             out = tuple(y.view(x.shape) for x, y in zip(xs, (out,) if len(xs) == 1 else out))
@@ -97,7 +97,7 @@ class RotaryPositions:
             out = _rotate(self, self.table, at, rows, [x.shape for x in xs], False)
         return out[0] if len(xs) == 1 else tuple(out)
 
-    def _rows(self, positions, xs):
+    def _arguments(self, positions, xs):
         """(positions, tensors...) of a call, checked, as the kernels take them."""
         if not 1 <= len(xs) <= 2:
             raise ValueError("rotate takes one or two tensors")
@@ -145,7 +145,7 @@ class RotateFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, rotary, positions, *xs):
-        positions, *rows = rotary._rows(positions, xs)
+        positions, *rows = rotary._arguments(positions, xs)
         ctx.rotary = rotary
         ctx.save_for_backward(rotary.table, positions)
         ctx.like = (positions.shape, positions.dtype, positions.device)

@@ -243,3 +243,34 @@ def test_traced_adapters_run_again_on_other_tensors(monkeypatch):
         y.mul_(0.5)
         results.append((y.detach(), *torch.autograd.grad(y, (leaf, bank), torch.ones_like(y))))
     assert all(torch.equal(a, b) for a, b in zip(*results)) and results[0][1].shape == (2, 3, 128)
+
+
+@pytest.mark.gpu
+def test_modes_that_only_look_on_change_nothing():
+    """Dispatch modes of a program's own (counters, loggers) see the outputs' allocations and are no recorders."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from torch.utils.flop_counter import FlopCounterMode
+
+    class Mode(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    r, p = RotaryPositions(64, 50), torch.arange(3, device="cuda")
+    x, logits = torch.randn(3, 2, 64, generator=g, device="cuda").half(), torch.randn(3, 50, generator=g, device="cuda")
+    down, up, index = torch.randn(2, 8, 64, generator=g, device="cuda").half(), torch.randn(2, 8, 32, generator=g, device="cuda").half(), torch.tensor([0, -1, 1], dtype=torch.int32, device="cuda")
+    cache, table, n = QuantizedKVCache(4, 16, 2, 64, bits=4), torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.full((3,), 3, dtype=torch.int32, device="cuda")
+
+    def step():
+        cache.append(x, x, p)
+        q = cache.append_rotated(x, x, x, p, r, p)
+        leaf = x.clone().requires_grad_()
+        y = r.rotate(p, leaf)
+        return [q, *cache.read(p), cache.attend(q, table, n, window=2), cache.attend(q, table, n), r.rotate(p, x), *token_log_probs(logits, p, entropy=True, top=2),
+                adapter_matmul(x[:, 0], down, up, index), adapter_matmul(x[:, 0], down, up, index, out=torch.empty(3, 32, device="cuda").half()), *torch.autograd.grad(y, leaf, x)]
+
+    want = step()
+    for mode in (Mode, lambda: FlopCounterMode(display=False), lambda: torch.device("cuda")):
+        with mode():
+            got = step()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
